@@ -599,6 +599,132 @@ int llmp_hip_decode_matrix_staged(int decoder, const llmp_decode_operand* weight
                                   const float* x, uint64_t rows, uint64_t x_stride, float* y, uint64_t y_stride, int path,
                                   void* scratch, size_t scratch_bytes, void* stream);
 
+/* ------------------------------------------------------------ the paged 8-bit KV cache
+ * No counterpart in the reference (its caches are one sequence's, in GGML blocks): the cache of a program that serves many
+ * requests at once. A page holds `page` tokens (a multiple of 16, 16 to 256) of every KV head:
+ *   k        int8 [pages][kv_heads][page][head_dim]   codes -127 to 127
+ *   v        int8 [pages][kv_heads][head_dim][page]   the tokens innermost: they are the attention's inner index
+ *   k_scale  F32 [pages][kv_heads], v_scale the same: a value is its code times its page's and head's scale
+ *   low/high int8 [pages][kv_heads][head_dim]         every dimension's smallest and largest K code, for the selection;
+ *                                                     both null: not kept
+ * head_dim is 64, 128 or 256. The cache's arrays lie at 16-byte boundaries. A request's table row names its pages in order
+ * (page numbers; one outside [0, pages) is never read or written: its tokens count as not there). Tokens of a step lie request
+ * after request: request r's rows are starts[r] to starts[r + 1] - 1, at the last positions of its lengths[r] tokens. */
+typedef struct llmp_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  void* low;
+  void* high;
+  int32_t pages, kv_heads, page, head_dim;
+} llmp_paged_cache;
+
+/* llmp.paged.plan: a step's bookkeeping from the requests' lengths before and after it (device I32 [requests]; negative
+ * ones count as zero). A request that shrinks (after < before; 0: it has ended) gives its last pages back, one that grows
+ * takes pages for what its last page has no room for. Free pages lie in a ring (I32 [ring_size]; counters_in: {index of the
+ * first, how many}): taken from its head in the order of the requests, given back at its tail (those serve the next step).
+ * When they run out, later pages are not given: lengths[r] = min(after, what the pages hold). Written:
+ *   table     the new pages' entries, nothing else of it
+ *   ring      the pages given back
+ *   counters  I32 [3]: the ring's first and count after the step, tokens that found no page (may be counters_in)
+ *   starts    I32 [requests + 1]: the exclusive sums of max(after - before, 0)
+ *   lengths   I32 [requests]: tokens held after the step
+ *   slots, positions, owners  I32 [tokens]: page * `page` + offset (-1: no page), the position and the request of every new
+ *             token; -1 past starts[requests]
+ *   work      I32 [work_items][4], 16-byte aligned: {page, first row, tokens held before, new tokens} of every page that new
+ *             tokens touch, request after request; {-1, 0, 0, 0} past them. llmp_hip_paged_work_items(requests, tokens, page) are
+ *             always enough.
+ * scratch: llmp_hip_paged_plan_scratch(requests) bytes. One launch for a decode step's sizes, two for larger ones. */
+typedef struct llmp_paged_plan {
+  const int32_t* before;
+  const int32_t* after;
+  int32_t* table;
+  int32_t* ring;
+  const int32_t* counters_in;
+  int32_t* counters;
+  int32_t* starts;
+  int32_t* lengths;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* owners;
+  int32_t* work;
+  void* scratch;
+  int64_t table_stride;
+  int32_t requests, table_width, ring_size, page, tokens, work_items;
+} llmp_paged_plan;
+int64_t llmp_hip_paged_work_items(int requests, int tokens, int page);
+size_t llmp_hip_paged_plan_scratch(int requests);
+int llmp_hip_paged_plan(const llmp_paged_plan* op, void* stream);
+
+/* llmp.paged.store: the new tokens' K and V rows (LLMP_X_* `type`; element strides; rows of head_dim consecutive values at
+ * 16-byte boundaries) into the pages that a plan's work items name. The scale of a page and head is the largest of the one
+ * it has (where it held tokens before) and the new rows' largest finite magnitude times F32(1 / 127); where it rises the held
+ * codes are rounded to it again (code * F32(old / new)). A code is value / scale rounded to nearest even, at most 127 in magnitude (so an infinity is 127, a
+ * NaN 0). low and high widen by the new codes (a page that held nothing begins anew). Items that do not fit
+ * (page out of range, rows outside `tokens`, more than `page` tokens, none) are skipped. One launch. */
+typedef struct llmp_paged_store {
+  llmp_paged_cache cache;
+  const void* k;
+  const void* v;
+  const int32_t* work;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int32_t type, tokens, work_items;
+} llmp_paged_store;
+int llmp_hip_paged_store(const llmp_paged_store* op, void* stream);
+
+/* llmp.paged.read: whole pages back as values: k_out and v_out [count][kv_heads][page][head_dim] of LLMP_X_* `type`, 16-byte
+ * aligned; pages[i * page_stride] (device I32) names them, one outside the cache gives zeros. One launch. */
+int llmp_hip_paged_read(const llmp_paged_cache* cache, const int32_t* pages, int64_t page_stride, int count, int type, void* k_out,
+                        void* v_out, void* stream);
+
+/* llmp.paged.attend: causal attention of a step's queries over their requests' pages: token t of a request with n new
+ * tokens is at position p = length - n + t and sees positions max(0, p - window + 1) (window 0: from 0) to p; with `lists`
+ * (llmp.paged.select's: I32 [tokens][kv_heads][list_pages], a request's pages by their place in its table row, -1: none, each at most
+ * once) only those pages' tokens among them. Logits are scale * q . k, capped to softcap * tanh(logit / softcap) where softcap
+ * is not 0; sinks (F32 [heads] or null) adds exp(sink) to a head's sum. A row that sees nothing is zero. q and out are
+ * LLMP_X_* `type`, element strides, rows of head_dim consecutive values at 16-byte boundaries; heads a multiple of kv_heads.
+ * most_tokens: at least every request's new tokens (a bound from the host; the launches' choice goes by it). K codes multiply the
+ * queries as whole numbers: a query row is two 8-bit digits of 1/32639 of its largest magnitude (three, 1/8355584,
+ * for F32). Probabilities times the V scale are rounded to F16 (for F32 to a sum of two) against V codes as F16 (exact).
+ * scratch: llmp_hip_paged_attend_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal, the reason in last_error).
+ * Launch arguments depend on the descriptor alone, never on the lengths: a captured launch replays at other lengths. */
+typedef struct llmp_paged_attend {
+  llmp_paged_cache cache;
+  const void* q;
+  void* out;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const int32_t* table;
+  const int32_t* lists;
+  const float* sinks;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride, table_stride;
+  int32_t type, heads, requests, tokens, most_tokens, table_width, list_pages, window;
+  float scale, softcap;
+} llmp_paged_attend;
+size_t llmp_hip_paged_attend_scratch(const llmp_paged_attend* op, int cus);
+int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream);
+
+/* llmp.paged.select: for every new token and KV head the `keep` pages of its request whose keys could have the largest logit: a
+ * head's query as 8-bit codes c of unit u = max|q| * F32(1 / 127) (q / u to nearest even), a page's score the largest of the group's heads' of
+ * F32(F32(sum over d of c_d * (c_d > 0 ? high_d : low_d)) * u) * k_scale, which bounds every key's c . k in the page. The token's
+ * first `first` and last `recent` pages are always among them (those up to its own count; at most `keep` together); ties go to
+ * the lower page; a score that is not a number counts as the smallest. lists: I32 [tokens][kv_heads][keep], ascending,
+ * -1 past a token's pages; tokens past starts[requests] get -1 throughout. scratch: llmp_hip_paged_select_scratch(op) bytes at
+ * a 16-byte boundary. The cache has low and high. keep at most 4096. */
+typedef struct llmp_paged_select {
+  llmp_paged_cache cache;
+  const void* q;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const int32_t* table;
+  int32_t* lists;
+  int64_t q_token_stride, q_head_stride, table_stride;
+  int32_t type, heads, requests, tokens, most_tokens, table_width, keep, first, recent;
+} llmp_paged_select;
+size_t llmp_hip_paged_select_scratch(const llmp_paged_select* op);
+int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ------------------------------------------------------------ a yardstick
  * No counterpart in the reference: a launch that only reads `bytes` (whole 16-byte chunks at a 16-byte boundary),
  * eight loads in flight a lane, folded into `sink` (llmp_hip_stream_read_sink(cus) bytes, the caller's). What it

@@ -113,6 +113,48 @@ class RopeStore(C.Structure):
                 ("attn_factor", C.c_float), ("theta_scale", C.c_float), ("corr_dims", C.c_float * 2)]
 
 
+class PagedCache(C.Structure):
+    """llmp_paged_cache: a paged 8-bit KV cache's arrays and sizes."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("low", C.c_void_p),
+                ("high", C.c_void_p), ("pages", C.c_int32), ("kv_heads", C.c_int32), ("page", C.c_int32),
+                ("head_dim", C.c_int32)]
+
+
+class PagedPlan(C.Structure):
+    """llmp_paged_plan: a step's bookkeeping from the requests' lengths."""
+    _fields_ = [("before", C.c_void_p), ("after", C.c_void_p), ("table", C.c_void_p), ("ring", C.c_void_p),
+                ("counters_in", C.c_void_p), ("counters", C.c_void_p), ("starts", C.c_void_p), ("lengths", C.c_void_p),
+                ("slots", C.c_void_p), ("positions", C.c_void_p), ("owners", C.c_void_p), ("work", C.c_void_p),
+                ("scratch", C.c_void_p), ("table_stride", C.c_int64), ("requests", C.c_int32), ("table_width", C.c_int32),
+                ("ring_size", C.c_int32), ("page", C.c_int32), ("tokens", C.c_int32), ("work_items", C.c_int32)]
+
+
+class PagedStore(C.Structure):
+    """llmp_paged_store: new K and V rows into the pages a plan's work items name."""
+    _fields_ = [("cache", PagedCache), ("k", C.c_void_p), ("v", C.c_void_p), ("work", C.c_void_p),
+                ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64),
+                ("v_head_stride", C.c_int64), ("type", C.c_int32), ("tokens", C.c_int32), ("work_items", C.c_int32)]
+
+
+class PagedAttend(C.Structure):
+    """llmp_paged_attend: a step's queries over their requests' pages."""
+    _fields_ = [("cache", PagedCache), ("q", C.c_void_p), ("out", C.c_void_p), ("lengths", C.c_void_p), ("starts", C.c_void_p),
+                ("table", C.c_void_p), ("lists", C.c_void_p), ("sinks", C.c_void_p), ("q_token_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("type", C.c_int32), ("heads", C.c_int32), ("requests", C.c_int32),
+                ("tokens", C.c_int32), ("most_tokens", C.c_int32), ("table_width", C.c_int32), ("list_pages", C.c_int32),
+                ("window", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float)]
+
+
+class PagedSelect(C.Structure):
+    """llmp_paged_select: the pages that could hold the largest logits."""
+    _fields_ = [("cache", PagedCache), ("q", C.c_void_p), ("lengths", C.c_void_p), ("starts", C.c_void_p), ("table", C.c_void_p),
+                ("lists", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("table_stride", C.c_int64),
+                ("type", C.c_int32), ("heads", C.c_int32), ("requests", C.c_int32), ("tokens", C.c_int32),
+                ("most_tokens", C.c_int32), ("table_width", C.c_int32), ("keep", C.c_int32), ("first", C.c_int32),
+                ("recent", C.c_int32)]
+
+
 class VecQSource(C.Structure):
     _fields_ = [("x", C.c_void_p), ("x_type", C.c_int), ("x_token", C.c_int64),
                 ("x_slot", C.c_int64)]
@@ -150,6 +192,15 @@ SYMBOLS = {
     "llmp_hip_moe_token": (_int, [C.POINTER(MoeToken), _int, _int, _vp]),
     "llmp_hip_attn_vec_quant_scratch": (C.c_size_t, [C.POINTER(AttnVecQuant), _int]),
     "llmp_hip_attn_vec_quant": (_int, [C.POINTER(AttnVecQuant), _vp, C.c_size_t, _int, _vp]),
+    "llmp_hip_paged_work_items": (_i64, [_int, _int, _int]),
+    "llmp_hip_paged_plan_scratch": (C.c_size_t, [_int]),
+    "llmp_hip_paged_plan": (_int, [C.POINTER(PagedPlan), _vp]),
+    "llmp_hip_paged_store": (_int, [C.POINTER(PagedStore), _vp]),
+    "llmp_hip_paged_read": (_int, [C.POINTER(PagedCache), _vp, _i64, _int, _int, _vp, _vp, _vp]),
+    "llmp_hip_paged_attend_scratch": (C.c_size_t, [C.POINTER(PagedAttend), _int]),
+    "llmp_hip_paged_attend": (_int, [C.POINTER(PagedAttend), _vp, C.c_size_t, _int, _vp]),
+    "llmp_hip_paged_select_scratch": (C.c_size_t, [C.POINTER(PagedSelect)]),
+    "llmp_hip_paged_select": (_int, [C.POINTER(PagedSelect), _vp, C.c_size_t, _vp]),
     "llmp_hip_mxfp8_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
     "llmp_hip_mxfp8_swizzle": (_int, [_vp, _i64, _i64, _vp, _vp]),
     "llmp_hip_mxfp8_gemv": (_int, [_vp, _vp, _i64, _i64, _vp, _int, _vp, _vp]),

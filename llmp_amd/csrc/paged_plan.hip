@@ -1,0 +1,295 @@
+// llmp.paged.plan: the requests' lengths before and after a step, in; the pages that change hands, the new tokens' slots
+// and the pages they touch, out. Four exclusive sums over the requests (new tokens, pages wanted, pages given back, pages
+// touched) say where everything goes; every output is then an index of its own, found by a binary search in those sums, so
+// nothing is ordered by atomics and the same lengths give the same answer.
+//
+// The kernel is latency: a decode step of 64 requests moves some kilobytes. Sizes whose outputs one workgroup writes in a few
+// sweeps are one launch, the sums in LDS; larger ones sum in a first launch of one workgroup (a pass of the requests, 1024
+// at a time, the sums to scratch) and write in a second of many.
+#include "paged.h"
+
+namespace llmp_hip {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kOneLaunchRequests = 1024;  // four sums of them in LDS
+constexpr int kOneLaunchOutputs = 8192;   // tokens and work items together: sweeps of 1024
+
+// A request's numbers before the sums.
+struct PlanRequest {
+  int before, after, have, want;
+};
+__device__ __forceinline__ int CeilPages(int tokens, int page) { return (tokens + page - 1) / page; }
+__device__ __forceinline__ PlanRequest ReadPlanRequest(const llmp_paged_plan& op, int r) {
+  PlanRequest q;
+  const int most = static_cast<int>(kMostPagedLength);
+  q.before = min(max(op.before[r], 0), most);
+  q.after = min(max(op.after[r], 0), most);
+  q.have = min(CeilPages(q.before, op.page), op.table_width);
+  q.want = min(CeilPages(q.after, op.page), op.table_width);
+  return q;
+}
+// Pages a request gets, and its length after the step, once the wants before it are known.
+__device__ __forceinline__ int PagesGot(const PlanRequest& q, int wants_before, int free) {
+  return min(max(q.want - q.have, 0), max(free - wants_before, 0));
+}
+__device__ __forceinline__ int LengthAfter(const PlanRequest& q, int got, int page) {
+  if (q.after <= q.before) return q.after;
+  // (64 bits: a table's width times a page may pass an int.)
+  return static_cast<int>(min(static_cast<int64_t>(q.after), max(static_cast<int64_t>(q.before), static_cast<int64_t>(q.have + got) * page)));
+}
+__device__ __forceinline__ int PagesTouched(const PlanRequest& q, int length, int page) {
+  return length > q.before ? (length - 1) / page - q.before / page + 1 : 0;
+}
+
+// What the sums leave: the ring as it was, and the totals.
+struct PlanTotals {
+  int head, free, wants, gives, touched, tokens, missing;
+};
+constexpr int kTotalInts = 8;
+
+// Inclusive sums over a workgroup of 1024 of three values at once; `carry` the running totals, known to every thread.
+template <int N>
+__device__ void BlockSums(int (&v)[N], int (&carry)[N], int* wave_sums) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  constexpr int kWaves = kPlanThreads / kWave;
+#pragma unroll
+  for (int step = 1; step < kWave; step <<= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int up = __shfl_up(v[i], step);
+      if (lane >= step) v[i] += up;
+    }
+  }
+  if (lane == kWave - 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) wave_sums[i * kWaves + wave] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    int before = 0, all = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      const int s = wave_sums[i * kWaves + w];
+      before += w < wave ? s : 0;
+      all += s;
+    }
+    v[i] += before + carry[i];
+    carry[i] += all;
+  }
+  __syncthreads();
+}
+
+// The sums' pass by one workgroup: starts and lengths written, exclusive sums of wants, gives and touched pages to `sums`
+// ([3][requests + 1]), the starts also to `starts_too` where that is not null.
+__device__ PlanTotals SumRequests(const llmp_paged_plan& op, int* sums, int* starts_too, int* wave_sums) {
+  PlanTotals t;
+  t.head = op.counters_in[0] % op.ring_size;
+  if (t.head < 0) t.head += op.ring_size;
+  t.free = min(max(op.counters_in[1], 0), op.ring_size);
+  const int n1 = op.requests + 1;
+  int carry[3] = {0, 0, 0}, carry_touched[2] = {0, 0};
+  for (int base = 0; base < op.requests; base += kPlanThreads) {
+    const int r = base + threadIdx.x;
+    const bool real = r < op.requests;
+    PlanRequest q = {0, 0, 0, 0};
+    if (real) q = ReadPlanRequest(op, r);
+    const int fresh = max(q.after - q.before, 0), wants = max(q.want - q.have, 0), gives = max(q.have - q.want, 0);
+    int v[3] = {fresh, wants, gives};
+    BlockSums(v, carry, wave_sums);
+    const int got = PagesGot(q, v[1] - wants, t.free);
+    const int length = LengthAfter(q, got, op.page);
+    const int touched = PagesTouched(q, length, op.page);
+    int u[2] = {touched, max(q.after - length, 0)};
+    BlockSums(u, carry_touched, wave_sums);
+    if (real) {
+      op.starts[r] = v[0] - fresh;
+      op.lengths[r] = length;
+      sums[r] = v[1] - wants;
+      sums[n1 + r] = v[2] - gives;
+      sums[2 * n1 + r] = u[0] - touched;
+      if (starts_too != nullptr) starts_too[r] = v[0] - fresh;
+    }
+  }
+  t.tokens = carry[0];
+  t.wants = carry[1];
+  t.gives = carry[2];
+  t.touched = carry_touched[0];
+  t.missing = carry_touched[1];
+  if (threadIdx.x == 0) {
+    op.starts[op.requests] = t.tokens;
+    if (starts_too != nullptr) starts_too[op.requests] = t.tokens;
+    sums[op.requests] = t.wants;
+    sums[n1 + op.requests] = t.gives;
+    sums[2 * n1 + op.requests] = t.touched;
+    const int taken = min(t.wants, t.free);
+    op.counters[0] = static_cast<int>((static_cast<int64_t>(t.head) + taken) % op.ring_size);
+    op.counters[1] = min(t.free - taken + t.gives, op.ring_size);
+    op.counters[2] = t.missing;
+  }
+  return t;
+}
+
+// The request whose share of the sums holds `index`: the last r with sums[r] <= index (requests with nothing are passed over).
+__device__ __forceinline__ int OwnerOf(const int* sums, int requests, int index) {
+  int low = 0, high = requests;  // sums[low] <= index < sums[high]
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (sums[mid] <= index) {
+      low = mid;
+    } else {
+      high = mid;
+    }
+  }
+  return low;
+}
+__device__ __forceinline__ int RingAt(const llmp_paged_plan& op, int64_t index) { return op.ring[index % op.ring_size]; }
+
+// Page j of request r: an old entry of the table, or the ring's (the new entry itself is another thread's to write).
+__device__ __forceinline__ int PageOf(const llmp_paged_plan& op, const PlanTotals& t, const PlanRequest& q, int r, int wants_before, int j) {
+  return j < q.have ? op.table[r * op.table_stride + j] : RingAt(op, static_cast<int64_t>(t.head) + wants_before + j - q.have);
+}
+
+// Every output by its index, spread over `threads` threads. What the ring takes back lies past all that it gives out, and new
+// entries of the table past all that are read, so the order does not matter. (The ranges are checked where they index
+// memory: lengths whose sums pass an int give wrong numbers, not accesses outside the arrays.)
+__device__ void WriteOutputs(const llmp_paged_plan& op, const PlanTotals& t, const int* starts, const int* sums, int thread, int threads) {
+  const int n1 = op.requests + 1;
+  const int *wants = sums, *gives = sums + n1, *touched = sums + 2 * n1;
+  for (int i = thread; i < op.tokens; i += threads) {
+    int slot = -1, position = -1, owner = -1;
+    if (i < t.tokens) {
+      owner = OwnerOf(starts, op.requests, i);
+      const PlanRequest q = ReadPlanRequest(op, owner);
+      position = q.before + i - starts[owner];
+      const int length = LengthAfter(q, PagesGot(q, wants[owner], t.free), op.page);
+      if (position >= 0 && position < length) slot = PageOf(op, t, q, owner, wants[owner], position / op.page) * op.page + position % op.page;
+    }
+    op.slots[i] = slot;
+    op.positions[i] = position;
+    op.owners[i] = owner;
+  }
+  for (int i = thread; i < op.work_items; i += threads) {
+    I32x4 item = {-1, 0, 0, 0};
+    if (i < t.touched) {
+      const int r = OwnerOf(touched, op.requests, i);
+      const PlanRequest q = ReadPlanRequest(op, r);
+      const int length = LengthAfter(q, PagesGot(q, wants[r], t.free), op.page);
+      const int j = q.before / op.page + i - touched[r];
+      if (j < 0 || j >= CeilPages(length, op.page)) continue;
+      const int low = max(j * op.page, q.before), high = static_cast<int>(min(static_cast<int64_t>(length), static_cast<int64_t>(j + 1) * op.page));
+      item = I32x4{PageOf(op, t, q, r, wants[r], j), starts[r] + low - q.before, low - j * op.page, high - low};
+    }
+    *reinterpret_cast<I32x4*>(op.work + 4 * static_cast<int64_t>(i)) = item;
+  }
+  const int taken = min(t.wants, t.free);
+  for (int i = thread; i < taken; i += threads) {
+    const int r = OwnerOf(wants, op.requests, i);
+    const PlanRequest q = ReadPlanRequest(op, r);
+    const int j = q.have + i - wants[r];
+    if (j >= q.have && j < q.want) op.table[r * op.table_stride + j] = RingAt(op, static_cast<int64_t>(t.head) + i);
+  }
+  const int back = min(t.gives, op.ring_size - t.free);  // (all of them, unless the ring's count was wrong)
+  for (int i = thread; i < back; i += threads) {
+    const int r = OwnerOf(gives, op.requests, i);
+    const PlanRequest q = ReadPlanRequest(op, r);
+    const int j = q.want + i - gives[r];
+    if (j >= q.want && j < q.have) op.ring[(static_cast<int64_t>(t.head) + t.free + i) % op.ring_size] = op.table[r * op.table_stride + j];
+  }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void PlanOneKernel(const llmp_paged_plan op) {
+  __shared__ int sums[3 * (kOneLaunchRequests + 1)], starts[kOneLaunchRequests + 1], wave_sums[3 * kPlanThreads / kWave];
+  const PlanTotals t = SumRequests(op, sums, starts, wave_sums);
+  __syncthreads();
+  WriteOutputs(op, t, starts, sums, threadIdx.x, kPlanThreads);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void PlanSumKernel(const llmp_paged_plan op) {
+  __shared__ int wave_sums[3 * kPlanThreads / kWave];
+  int* totals = static_cast<int*>(op.scratch);
+  const PlanTotals t = SumRequests(op, totals + kTotalInts, nullptr, wave_sums);
+  // (The counters may be overwritten in place: the second launch takes what they were from here.)
+  if (threadIdx.x == 0) {
+    totals[0] = t.head, totals[1] = t.free, totals[2] = t.wants, totals[3] = t.gives, totals[4] = t.touched, totals[5] = t.tokens;
+  }
+}
+
+constexpr int kWriteThreads = 256;
+__global__ __launch_bounds__(kWriteThreads) void PlanWriteKernel(const llmp_paged_plan op) {
+  const int* totals = static_cast<const int*>(op.scratch);
+  PlanTotals t;
+  t.head = totals[0], t.free = totals[1], t.wants = totals[2], t.gives = totals[3], t.touched = totals[4], t.tokens = totals[5];
+  t.missing = 0;
+  WriteOutputs(op, t, op.starts, totals + kTotalInts, blockIdx.x * kWriteThreads + threadIdx.x, gridDim.x * kWriteThreads);
+}
+
+}  // namespace
+
+int CheckPagedCache(const char* who, const llmp_paged_cache& c, bool needs_edges) {
+  if (c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr) return Refuse(1, "%s: null array of the cache", who);
+  if ((c.low == nullptr) != (c.high == nullptr) || (needs_edges && c.low == nullptr))
+    return Refuse(1, "%s: the cache's low and high codes come together%s", who, needs_edges ? ", and are needed here" : "");
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return Refuse(1, "%s: head sizes 64, 128 and 256, not %d", who, c.head_dim);
+  if (c.page < 16 || c.page > 256 || c.page % 16 != 0) return Refuse(1, "%s: pages of 16 to 256 tokens, a multiple of 16, not %d", who, c.page);
+  if (c.pages < 1 || c.kv_heads < 1 || c.kv_heads > 65535) return Refuse(1, "%s: at least one page and 1 to 65535 KV heads (%d, %d)", who, c.pages, c.kv_heads);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | reinterpret_cast<uintptr_t>(c.k_scale) |
+                        reinterpret_cast<uintptr_t>(c.v_scale) | reinterpret_cast<uintptr_t>(c.low) | reinterpret_cast<uintptr_t>(c.high);
+  if (all % 16 != 0) return Refuse(1, "%s: the cache's arrays lie at 16-byte boundaries", who);
+  return 0;
+}
+
+int CheckPagedRows(const char* who, const char* name, const void* rows, int64_t token_stride, int64_t head_stride, int type) {
+  if (rows == nullptr) return Refuse(1, "%s: null %s", who, name);
+  if (type != LLMP_X_F32 && type != LLMP_X_BF16 && type != LLMP_X_F16) return Refuse(1, "%s: F32, BF16 or F16 rows, not type %d", who, type);
+  const int per = 16 / PagedElementBytes(type);
+  if (reinterpret_cast<uintptr_t>(rows) % 16 != 0 || token_stride < 0 || head_stride < 0 || token_stride % per != 0 || head_stride % per != 0)
+    return Refuse(1, "%s: %s's rows lie at 16-byte boundaries (strides %lld, %lld)", who, name, (long long)token_stride, (long long)head_stride);
+  return 0;
+}
+
+}  // namespace llmp_hip
+
+using namespace llmp_hip;
+
+extern "C" int64_t llmp_hip_paged_work_items(int requests, int tokens, int page) {
+  if (requests < 1 || tokens < 0 || page < 1) return 0;
+  // n new tokens touch at most (n - 2) / page + 2 pages, and never more than n.
+  const int64_t most = 2 * static_cast<int64_t>(requests) + tokens / page;
+  return most < tokens ? most : tokens;
+}
+
+extern "C" size_t llmp_hip_paged_plan_scratch(int requests) {
+  return requests < 1 ? 0 : (kTotalInts + 3 * (static_cast<size_t>(requests) + 1)) * sizeof(int);
+}
+
+extern "C" int llmp_hip_paged_plan(const llmp_paged_plan* op, void* stream) {
+  if (op == nullptr) return Refuse(1, "paged_plan: null operands");
+  if (op->requests < 1 || op->requests > 1 << 24 || op->table_width < 1 || op->ring_size < 1 || op->tokens < 0 || op->work_items < 0)
+    return Refuse(1, "paged_plan: 1 to 2^24 requests, a table and a ring of at least one page (%d, %d, %d), tokens %d, work items %d", op->requests,
+                  op->table_width, op->ring_size, op->tokens, op->work_items);
+  if (op->page < 1 || op->page > 65536) return Refuse(1, "paged_plan: pages of 1 to 65536 tokens, not %d", op->page);
+  if (op->before == nullptr || op->after == nullptr || op->table == nullptr || op->ring == nullptr || op->counters_in == nullptr ||
+      op->counters == nullptr || op->starts == nullptr || op->lengths == nullptr || op->scratch == nullptr ||
+      (op->tokens > 0 && (op->slots == nullptr || op->positions == nullptr || op->owners == nullptr)) || (op->work_items > 0 && op->work == nullptr))
+    return Refuse(1, "paged_plan: null operand");
+  if (op->table_stride < op->table_width) return Refuse(1, "paged_plan: a table row of %d entries every %lld", op->table_width, (long long)op->table_stride);
+  const uintptr_t words = reinterpret_cast<uintptr_t>(op->before) | reinterpret_cast<uintptr_t>(op->after) | reinterpret_cast<uintptr_t>(op->table) |
+                          reinterpret_cast<uintptr_t>(op->ring) | reinterpret_cast<uintptr_t>(op->counters_in) | reinterpret_cast<uintptr_t>(op->counters) |
+                          reinterpret_cast<uintptr_t>(op->starts) | reinterpret_cast<uintptr_t>(op->lengths) | reinterpret_cast<uintptr_t>(op->slots) |
+                          reinterpret_cast<uintptr_t>(op->positions) | reinterpret_cast<uintptr_t>(op->owners) | reinterpret_cast<uintptr_t>(op->scratch);
+  if (words % 4 != 0 || reinterpret_cast<uintptr_t>(op->work) % 16 != 0) return Refuse(1, "paged_plan: I32 arrays at 4-byte boundaries, the work items at 16");
+  if (op->work_items < llmp_hip_paged_work_items(op->requests, op->tokens, op->page))
+    return Refuse(1, "paged_plan: %d work items, %lld may be needed", op->work_items, (long long)llmp_hip_paged_work_items(op->requests, op->tokens, op->page));
+  BeginLaunches();
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  const int64_t outputs = static_cast<int64_t>(op->tokens) + op->work_items;
+  if (op->requests <= kOneLaunchRequests && outputs <= kOneLaunchOutputs) {
+    hipLaunchKernelGGL(PlanOneKernel, dim3(1), dim3(kPlanThreads), 0, on, *op);
+  } else {
+    hipLaunchKernelGGL(PlanSumKernel, dim3(1), dim3(kPlanThreads), 0, on, *op);
+    const int64_t blocks = (outputs + kWriteThreads - 1) / kWriteThreads;
+    hipLaunchKernelGGL(PlanWriteKernel, dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), dim3(kWriteThreads), 0, on, *op);
+  }
+  return LaunchStatus("paged_plan");
+}

@@ -649,3 +649,151 @@ def decode_matrix(decoder, weight, x, first=0, outputs=None, path=0, out=None):
     _lib.check(lib.llmp_hip_decode_matrix_staged(decoder, C.byref(op), first, outputs, _ptr(x), rows, x.stride(0), _ptr(y),
                                                  y.stride(0), path, _ptr(scratch) if size else None, size, _stream()))
     return y
+
+
+def paged_cache(pages, kv_heads, page, head_dim, device="cuda", edges=True):
+    """An empty paged 8-bit KV cache (include/llmp_hip.h, llmp_paged_cache) as a dict of tensors: k int8 [pages, kv_heads,
+    page, head_dim], v int8 [pages, kv_heads, head_dim, page], k_scale and v_scale float32 [pages, kv_heads] and, with
+    `edges` (for paged_select), low and high int8 [pages, kv_heads, head_dim]."""
+    cache = {"k": torch.zeros((pages, kv_heads, page, head_dim), dtype=torch.int8, device=device),
+             "v": torch.zeros((pages, kv_heads, head_dim, page), dtype=torch.int8, device=device)}
+    for name in ("k_scale", "v_scale"):
+        cache[name] = torch.zeros((pages, kv_heads), dtype=torch.float32, device=device)
+    if edges:
+        for name in ("low", "high"):
+            cache[name] = torch.zeros((pages, kv_heads, head_dim), dtype=torch.int8, device=device)
+    return cache
+
+
+def _paged_cache(cache):
+    k, v = cache["k"], cache["v"]
+    pages, kv_heads, page, head_dim = k.shape
+    low, high = cache.get("low"), cache.get("high")
+    shapes = [(k, (pages, kv_heads, page, head_dim), torch.int8), (v, (pages, kv_heads, head_dim, page), torch.int8),
+              (cache["k_scale"], (pages, kv_heads), torch.float32), (cache["v_scale"], (pages, kv_heads), torch.float32)]
+    shapes += [(t, (pages, kv_heads, head_dim), torch.int8) for t in (low, high) if t is not None]
+    for t, shape, dtype in shapes:
+        assert t.shape == shape and t.dtype == dtype and t.is_contiguous(), "the cache's arrays are whole, of one set of sizes"
+    return _lib.PagedCache(k.data_ptr(), v.data_ptr(), cache["k_scale"].data_ptr(), cache["v_scale"].data_ptr(), _ptr(low), _ptr(high),
+                           pages, kv_heads, page, head_dim)
+
+
+def _int32(*tensors):
+    for t in tensors:
+        assert t.dtype == torch.int32 and t.stride(-1) == 1, "int32 arrays in one piece"
+
+
+def _table_stride(table):
+    """(A single row's stride can be anything.)"""
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
+    """llmp.paged.plan: what a step does to a paged cache, from the requests' lengths before and after it (int32
+    [requests]). `table` (int32 [requests, width]) and `ring` (int32, the free pages) are updated in place; `counters` is
+    {first free page's index in the ring, how many}; `tokens` at least the new tokens. Returns a dict of int32 tensors: starts
+    [requests + 1], lengths [requests], slots, positions and requests [tokens], work [items, 4] (page, first row, tokens held,
+    new tokens) and the counters after the step {first, how many, tokens without a page}. `out`, such a dict, is filled
+    instead of a new one (its counters may be the ones passed in)."""
+    lib = _lib.load()
+    _int32(before, after, table, ring, counters)
+    n = before.shape[0]
+    assert before.dim() == after.dim() == ring.dim() == 1 and after.shape[0] == n and table.dim() == 2 and table.shape[0] == n and counters.numel() >= 2
+    items = lib.llmp_hip_paged_work_items(n, tokens, page)
+    if out is None:
+        # One allocation: the work items first, for their 16-byte boundary.
+        sizes = {"work": 4 * items, "slots": tokens, "positions": tokens, "requests": tokens, "starts": n + 1, "lengths": n, "counters": 3}
+        parts = torch.empty(sum(sizes.values()), dtype=torch.int32, device=before.device).split(list(sizes.values()))
+        out = dict(zip(sizes, parts))
+        out["work"] = out["work"].view(items, 4)
+    _int32(*out.values())
+    assert out["work"].shape[0] >= items and out["starts"].numel() > n and out["lengths"].numel() >= n and out["counters"].numel() >= 3
+    assert min(out[k].numel() for k in ("slots", "positions", "requests")) >= tokens and out["work"].is_contiguous()
+    scratch = torch.empty(lib.llmp_hip_paged_plan_scratch(n), dtype=torch.uint8, device=before.device)
+    op = _lib.PagedPlan(before.data_ptr(), after.data_ptr(), table.data_ptr(), ring.data_ptr(), counters.data_ptr(), out["counters"].data_ptr(),
+                        out["starts"].data_ptr(), out["lengths"].data_ptr(), out["slots"].data_ptr(), out["positions"].data_ptr(),
+                        out["requests"].data_ptr(), out["work"].data_ptr(), scratch.data_ptr(), _table_stride(table), n, table.shape[1],
+                        ring.shape[0], page, tokens, out["work"].shape[0])
+    _lib.check(lib.llmp_hip_paged_plan(C.byref(op), _stream()))
+    return out
+
+
+def paged_store(cache, k, v, work):
+    """llmp.paged.store: k and v (float32, bfloat16 or float16 [tokens, kv_heads, head_dim]) into the pages that `work` (paged_plan's)
+    names, quantized with a scale for each page and head; the cache is updated in place."""
+    lib = _lib.load()
+    c = _paged_cache(cache)
+    assert k.shape == v.shape == (k.shape[0], c.kv_heads, c.head_dim) and k.dtype == v.dtype and k.stride(-1) == v.stride(-1) == 1
+    _int32(work)
+    assert work.dim() == 2 and work.shape[1] == 4 and work.is_contiguous()
+    op = _lib.PagedStore(c, k.data_ptr(), v.data_ptr(), work.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _x_type(k), k.shape[0],
+                         work.shape[0])
+    _lib.check(lib.llmp_hip_paged_store(C.byref(op), _stream()))
+
+
+def paged_read(cache, pages, dtype=torch.float32):
+    """llmp.paged.read: the cache's pages named by `pages` (int32 [n], any stride) as values, k and v [n, kv_heads, page, head_dim]; a
+    number outside the cache gives zeros."""
+    lib = _lib.load()
+    c = _paged_cache(cache)
+    assert pages.dim() == 1 and pages.dtype == torch.int32
+    k, v = (torch.empty((pages.shape[0], c.kv_heads, c.page, c.head_dim), dtype=dtype, device=pages.device) for _ in range(2))
+    _lib.check(lib.llmp_hip_paged_read(C.byref(c), pages.data_ptr(), pages.stride(0), pages.shape[0], _X_TYPES[dtype], k.data_ptr(), v.data_ptr(),
+                                       _stream()))
+    return k, v
+
+
+def _paged_queries(q, c, table, lengths, starts):
+    _int32(table, lengths, starts)
+    assert q.dim() == 3 and q.shape[2] == c.head_dim and q.stride(2) == 1
+    assert table.dim() == 2 and lengths.shape == (table.shape[0],) and starts.shape == (table.shape[0] + 1,)
+
+
+def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0.0, sinks=None, lists=None, most=None, out=None, scratch=None):
+    """llmp.paged.attend: causal attention of q (float32, bfloat16 or float16 [tokens, heads, head_dim]: request r's rows are starts[r] to
+    starts[r + 1] - 1, at the last of its lengths[r] positions) over the requests' pages (table int32 [requests, width]). `lists`
+    (paged_select's) leaves a (token, KV head) those pages only. `most`: the largest number of new tokens of a request, if it is
+    known. Returns q's shape and type; rows past starts[requests] are not written."""
+    lib = _lib.load()
+    c = _paged_cache(cache)
+    _paged_queries(q, c, table, lengths, starts)
+    tokens, heads, _ = q.shape
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+    if lists is not None:
+        _int32(lists)
+        assert lists.is_contiguous() and lists.shape[:2] == (tokens, c.kv_heads)
+    assert sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (heads,) and sinks.is_contiguous())
+    if tokens == 0:
+        return out
+    op = _lib.PagedAttend(c, q.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(lists), _ptr(sinks),
+                          q.stride(0), q.stride(1), out.stride(0), out.stride(1), _table_stride(table), _x_type(q), heads, table.shape[0], tokens,
+                          tokens if most is None else most, table.shape[1], lists.shape[2] if lists is not None else 0, window, scale, softcap)
+    cus = lib.llmp_hip_compute_units()
+    if scratch is None:
+        scratch = torch.empty(max(lib.llmp_hip_paged_attend_scratch(C.byref(op), cus), 16), dtype=torch.uint8, device=q.device)
+    _lib.check(lib.llmp_hip_paged_attend(C.byref(op), scratch.data_ptr(), scratch.numel(), cus, _stream()))
+    return out
+
+
+def paged_select(cache, q, table, lengths, starts, keep, *, first=1, recent=1, most=None, out=None, scratch=None):
+    """llmp.paged.select: for every row of q and KV head the `keep` pages (places in the request's table row, ascending, -1 past them) whose
+    keys have the largest bound on a logit of the head's group; the first `first` and the last `recent` pages up to the token's own
+    are always among them. int32 [tokens, kv_heads, keep]."""
+    lib = _lib.load()
+    c = _paged_cache(cache)
+    _paged_queries(q, c, table, lengths, starts)
+    tokens, heads, _ = q.shape
+    if out is None:
+        out = torch.empty((tokens, c.kv_heads, keep), dtype=torch.int32, device=q.device)
+    assert out.shape == (tokens, c.kv_heads, keep) and out.dtype == torch.int32 and out.is_contiguous()
+    if tokens == 0:
+        return out
+    op = _lib.PagedSelect(c, q.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1),
+                          _table_stride(table), _x_type(q), heads, table.shape[0], tokens, tokens if most is None else most, table.shape[1], keep, first,
+                          recent)
+    if scratch is None:
+        scratch = torch.empty(max(lib.llmp_hip_paged_select_scratch(C.byref(op)), 16), dtype=torch.uint8, device=q.device)
+    _lib.check(lib.llmp_hip_paged_select(C.byref(op), scratch.data_ptr(), scratch.numel(), _stream()))
+    return out
