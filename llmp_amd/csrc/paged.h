@@ -74,6 +74,13 @@ __device__ __forceinline__ void StoreValues(void* base, int64_t element, const f
   }
 }
 
+template <int TYPE>
+__device__ __forceinline__ void StoreOne(void* base, int64_t element, float x) {
+  if constexpr (TYPE == LLMP_X_F32) static_cast<float*>(base)[element] = x;
+  if constexpr (TYPE == LLMP_X_BF16) static_cast<uint16_t*>(base)[element] = static_cast<uint16_t>(FloatToBf16Bits(x));
+  if constexpr (TYPE == LLMP_X_F16) static_cast<uint16_t*>(base)[element] = static_cast<uint16_t>(FloatToHalfBits(x));
+}
+
 // A request's new tokens and length, whatever the device arrays hold: `n` 0 where its rows are not rows of the call.
 struct PagedRequest {
   int start, n, length;

@@ -102,8 +102,9 @@ __device__ __forceinline__ float Capped(float s, float softcap, float inverse) {
 // log2 of a page's V scale, as the running maximum takes it.
 __device__ __forceinline__ float ScaleLog(float vs) { return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-100f)); }
 
-// The many rows' form (its own file): launched for requests of more than few_rows rows.
-bool PagedManyRows(const PagedAttendArgs& args, int cus, hipStream_t stream);
+// The many rows' form (its own file), for requests of more than few_rows rows.
+size_t PagedManyScratch(const llmp_paged_attend& op, int cus);
+void PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStream_t stream);
 
 }  // namespace llmp_hip
 

@@ -457,12 +457,7 @@ __global__ __launch_bounds__(kFewThreads) void FewJoinKernel(const PagedAttendAr
   const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
   const int64_t to = (q.start + token) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const float x = value[e] * inverse;
-    if constexpr (TYPE == LLMP_X_F32) static_cast<float*>(op.out)[to + e] = x;
-    if constexpr (TYPE == LLMP_X_BF16) static_cast<uint16_t*>(op.out)[to + e] = static_cast<uint16_t>(FloatToBf16Bits(x));
-    if constexpr (TYPE == LLMP_X_F16) static_cast<uint16_t*>(op.out)[to + e] = static_cast<uint16_t>(FloatToHalfBits(x));
-  }
+  for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e] * inverse);
 }
 
 // Workgroups of the few rows' launch: two a compute unit (their registers' limit), a wave of each a SIMD.
@@ -472,6 +467,15 @@ size_t PartBytes(int groups) { return static_cast<size_t>(groups) * 4 * sizeof(i
 size_t FewScratch(int head_dim, int cus) {
   const int groups = FewGroups(cus);
   return PartBytes(groups) + 2 * static_cast<size_t>(groups) * kRows * (head_dim + 2) * sizeof(float);
+}
+
+// Requests of more rows than this are the many rows' form's, where the call has any.
+constexpr int kFewRows = 64;
+bool HasMany(const llmp_paged_attend& op) {
+  return op.lists == nullptr && static_cast<int64_t>(op.most_tokens < op.tokens ? op.most_tokens : op.tokens) * (op.heads / op.cache.kv_heads) > kFewRows;
+}
+size_t AttendScratch(const llmp_paged_attend& op, int cus) {
+  return FewScratch(op.cache.head_dim, cus) + (HasMany(op) ? PagedManyScratch(op, cus) : 0);
 }
 
 template <int TYPE, int D, bool LISTS>
@@ -529,12 +533,12 @@ using namespace llmp_hip;
 
 extern "C" size_t llmp_hip_paged_attend_scratch(const llmp_paged_attend* op, int cus) {
   if (CheckAttend(op) != 0) return 0;
-  return FewScratch(op->cache.head_dim, cus);
+  return AttendScratch(*op, cus);
 }
 
 extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream) {
   if (const int bad = CheckAttend(op); bad != 0) return bad;
-  const size_t needs = FewScratch(op->cache.head_dim, cus);
+  const size_t needs = AttendScratch(*op, cus);
   if (scratch == nullptr || scratch_bytes < needs || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
     return Refuse(1, "paged_attend: %zu bytes of scratch at a 16-byte boundary, %zu given", needs, scratch_bytes);
   BeginLaunches();
@@ -547,8 +551,11 @@ extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch,
   args.page_magic = p16 == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / p16 + 1);
   args.group = op->heads / op->cache.kv_heads;
   args.most_length = op->table_width * op->cache.page;
-  args.few_rows = INT_MAX;
+  const bool many = HasMany(*op);
+  args.few_rows = many ? kFewRows : INT_MAX;
   const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (many) PagedManyRows(args, static_cast<uint8_t*>(scratch) + FewScratch(op->cache.head_dim, cus), cus, on);
+  if (many && op->requests == 1 && op->most_tokens == op->tokens) return LaunchStatus("paged_attend");  // the one request has been answered
   if (op->type == LLMP_X_F32) LaunchFewOf<LLMP_X_F32>(args, groups, on);
   if (op->type == LLMP_X_BF16) LaunchFewOf<LLMP_X_BF16>(args, groups, on);
   if (op->type == LLMP_X_F16) LaunchFewOf<LLMP_X_F16>(args, groups, on);

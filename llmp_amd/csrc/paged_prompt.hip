@@ -1,0 +1,592 @@
+// llmp.paged.attend, the form for many rows: prompts, whole or in chunks.
+//
+// What bounds it is the vector units: per logit about seven operations and an exponential, against the matrix instructions' 4 D
+// operations; the cache's bytes come from L2 (a head's pages are read by every workgroup of its rows). A workgroup of four
+// waves takes 128 rows of one KV head, (token, head) pairs in order, so that a group's query heads share the tile; a
+// wave has 32 rows. A tile of 64 tokens goes through LDS, double-buffered, its loads in flight under the previous tile's
+// work: K as its codes, V turned into F16 once for all the waves. Products as in the few rows' form, 32 x 32:
+//   S^T = K Q^T by v_mfma_i32_32x32x32_i8. Row 8a + 4h + b of a product is token 16h + 4a + b of its 32, so that a lane (half h) ends
+//   with 16 consecutive tokens of one query row, all of one page;
+//   O^T += V^T P^T by v_mfma_f32_32x32x16_f16, P from the same lane's registers.
+// LDS rows are 16-byte pieces in an order turned by the row (Turn), so that the 32 rows a matrix operand reads lie in
+// different banks.
+//
+// A first small launch lists the (request, 128 rows) pairs and their tiles. With at least as many (pair, head) segments as workgroups
+// each is one workgroup's, longest first, dealt to the compute units there and back so that a unit's two workgroups
+// together have about the same; with fewer, all segments' tiles lie on one line that the workgroups share evenly, and a third
+// launch joins the parts.
+#include "paged_attend.h"
+
+namespace llmp_hip {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kWaveRows = 32;
+constexpr int kManyRows = kWaves * kWaveRows;
+constexpr int kListThreads = 1024;
+constexpr int kBuckets = 1024;  // of the segments' lengths, for their order
+
+// The list: a header, the pairs, the tiles before each pair (times KV heads), the pairs' order by length.
+struct ListHeader {
+  int64_t total;   // tiles of all segments
+  int pairs, whole;  // whole: every segment is one workgroup's
+};
+struct Pair {
+  int request, chunk, first_tile, tiles;
+};
+struct List {
+  ListHeader* header;
+  Pair* pairs;
+  int64_t* before;  // [pairs + 1]
+  int32_t* order;
+};
+
+struct ManyArgs {
+  PagedAttendArgs a;
+  List list;
+  float* partial;  // [2 * workgroups][kManyRows][D + 2]
+  int32_t* parts;  // [workgroups][4]
+  int most_pairs;
+  int a_unit;  // workgroups a compute unit holds
+};
+
+__device__ __forceinline__ int ChunksOf(const PagedAttendArgs& a, const PagedRequest& q) {
+  const int64_t rows = static_cast<int64_t>(q.n) * a.group;
+  return rows > a.few_rows ? static_cast<int>((rows + kManyRows - 1) / kManyRows) : 0;
+}
+
+// One workgroup: the pairs in the order of the requests, their sums, and their order by length.
+__global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int groups) {
+  __shared__ int64_t wave_sums[kListThreads / kWave];
+  __shared__ int buckets[kBuckets];
+  const PagedAttendArgs& a = m.a;
+  const llmp_paged_attend& op = a.op;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const auto block_sum = [&](int64_t v, int64_t* all) {  // inclusive
+#pragma unroll
+    for (int step = 1; step < kWave; step <<= 1) {
+      const int64_t up = __shfl_up(v, step);
+      if (lane >= step) v += up;
+    }
+    if (lane == kWave - 1) wave_sums[wave] = v;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w < kListThreads / kWave; ++w) {
+      const int64_t s = wave_sums[w];
+      v += w < wave ? s : 0;
+      total += s;
+    }
+    __syncthreads();
+    *all = total;
+    return v;
+  };
+  // The pairs: a request's by all threads where it has many.
+  int64_t pairs = 0;
+  for (int base = 0; base < op.requests; base += kListThreads) {
+    const int r = base + tid;
+    const int mine = r < op.requests ? ChunksOf(a, RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length)) : 0;
+    int64_t all;
+    const int64_t upto = block_sum(mine, &all);
+    for (int j = 0; j < mine; ++j) {
+      const int64_t at = pairs + upto - mine + j;
+      if (at < m.most_pairs) m.list.pairs[at].request = r, m.list.pairs[at].chunk = j;
+    }
+    pairs += all;
+  }
+  const int count = static_cast<int>(pairs < m.most_pairs ? pairs : m.most_pairs);
+  buckets[tid] = 0;
+  __syncthreads();
+  int64_t before = 0;
+  for (int base = 0; base < count; base += kListThreads) {
+    const int p = base + tid;
+    int tiles = 0;
+    if (p < count) {
+      Pair pair = m.list.pairs[p];
+      const PagedRequest q = RequestOf(op.starts, op.lengths, pair.request, op.tokens, a.most_length);
+      const int first_token = pair.chunk * kManyRows / a.group, last_token = min((pair.chunk * kManyRows + kManyRows - 1) / a.group, q.n - 1);
+      const int to = max(q.length - q.n + last_token + 1, 0), window = op.window > 0 ? op.window : INT_MAX / 2;
+      pair.first_tile = max(q.length - q.n + first_token - window + 1, 0) / kTileTokens;
+      pair.tiles = tiles = max((to + kTileTokens - 1) / kTileTokens - pair.first_tile, 1);  // (rows that see nothing are written too)
+      m.list.pairs[p] = pair;
+    }
+    int64_t all;
+    const int64_t upto = block_sum(static_cast<int64_t>(tiles) * op.cache.kv_heads, &all);
+    if (p < count) {
+      m.list.before[p] = before + upto - static_cast<int64_t>(tiles) * op.cache.kv_heads;
+      atomicAdd(&buckets[kBuckets - 1 - min(tiles / 4, kBuckets - 1)], 1);
+    }
+    before += all;
+  }
+  __syncthreads();
+  int64_t all;
+  const int mine = buckets[tid];
+  const int upto = static_cast<int>(block_sum(mine, &all));
+  buckets[tid] = upto - mine;
+  __syncthreads();
+  // (The order within a bucket is any: a segment's result does not depend on its turn.)
+  for (int p = tid; p < count; p += kListThreads) m.list.order[atomicAdd(&buckets[kBuckets - 1 - min(m.list.pairs[p].tiles / 4, kBuckets - 1)], 1)] = p;
+  if (tid == 0) {
+    m.list.before[count] = before;
+    m.list.header->total = before;
+    m.list.header->pairs = count;
+    m.list.header->whole = static_cast<int64_t>(count) * op.cache.kv_heads >= groups;
+  }
+}
+
+// Where a 16-byte piece of a row of `PIECES` lies: 256 bytes of rows side by side hold a piece number once.
+template <int PIECES>
+__device__ __forceinline__ int Turn(int row, int piece) { return piece ^ ((row / (16 / PIECES)) & (PIECES - 1)); }
+
+template <int D>
+struct ManyGeo {
+  static constexpr int kKBytes = kTileTokens * D;
+  static constexpr int kVBytes = D * kTileTokens * 2;
+  static constexpr int kBuffer = kKBytes + kVBytes;
+  static constexpr int kLds = 2 * kBuffer + 2 * 4 * 16;  // and the four 16-token groups' scales
+  static constexpr int kAUnit = D == 256 ? 1 : 2;        // workgroups a compute unit: 512 or 256 registers a lane
+};
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const ManyArgs m) {
+  using G = ManyGeo<D>;
+  constexpr int kDig = kDigits<TYPE>;
+  constexpr int kSteps = D / 32, kBlocks = D / 32, kPieces = D / 16, kLoads = D / 64;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const PagedAttendArgs& a = m.a;
+  const llmp_paged_attend& op = a.op;
+  const llmp_paged_cache& c = op.cache;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int half = lane >> 5, column = lane & 31;
+  const int groups = gridDim.x, w = blockIdx.x;
+  const ListHeader header = *m.list.header;
+  F32x4* const group_scales = reinterpret_cast<F32x4*>(lds + 2 * G::kBuffer);  // [buffer][group]: K's and V's scale, 1 if there is a page
+
+  int64_t u = 0, u_end = 0, per = 1;
+  int turn = 0, pair_index = 0;
+  const int units = groups / m.a_unit, unit_of = w % units;
+  const int64_t segments = static_cast<int64_t>(header.pairs) * c.kv_heads;
+  if (header.whole) {
+    turn = w / units;
+  } else {
+    per = (header.total + groups - 1) / groups;
+    u = w * per;
+    u_end = min(u + per, header.total);
+    if (u < u_end) {  // the pair that holds unit u
+      int low = 0, high = header.pairs;
+      while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (m.list.before[mid] <= u) {
+          low = mid;
+        } else {
+          high = mid;
+        }
+      }
+      pair_index = low;
+    }
+  }
+  I32x4 part = {-1, 0, 0, 0};
+
+  for (;;) {
+    // ---- the next segment, or part of one.
+    int head, t_first, t_count;
+    if (header.whole) {
+      const int64_t index = turn % 2 == 0 ? static_cast<int64_t>(turn) * units + unit_of : static_cast<int64_t>(turn + 1) * units - 1 - unit_of;
+      if (static_cast<int64_t>(turn) * units >= segments) break;
+      turn += m.a_unit;
+      if (index >= segments) continue;
+      pair_index = m.list.order[index / c.kv_heads];
+      head = static_cast<int>(index % c.kv_heads);
+      t_first = 0;
+      t_count = m.list.pairs[pair_index].tiles;
+    } else {
+      if (u >= u_end) break;
+      if (u >= m.list.before[pair_index + 1]) {
+        ++pair_index;
+        continue;
+      }
+      const int64_t in = u - m.list.before[pair_index];
+      const int tiles = m.list.pairs[pair_index].tiles;
+      head = static_cast<int>(in / tiles);
+      t_first = static_cast<int>(in % tiles);
+      t_count = static_cast<int>(min(static_cast<int64_t>(tiles - t_first), u_end - u));
+      u += t_count;
+    }
+    pair_index = __builtin_amdgcn_readfirstlane(pair_index);
+    head = __builtin_amdgcn_readfirstlane(head);
+    t_first = __builtin_amdgcn_readfirstlane(t_first);
+    t_count = __builtin_amdgcn_readfirstlane(t_count);
+    const Pair pair = m.list.pairs[pair_index];
+    const int r = __builtin_amdgcn_readfirstlane(pair.request);
+    const PagedRequest q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
+    const int32_t* const table = op.table + r * op.table_stride;
+
+    // ---- this lane's query row, and what the wave's rows see.
+    const int row0 = pair.chunk * kManyRows + wave * kWaveRows;
+    const int row = row0 + column, rows = q.n * a.group;
+    const bool real = row < rows;
+    const int token = row / a.group, query_head = row % a.group;
+    const int base_position = q.length - q.n;
+    const int position = base_position + token;
+    const int window = op.window > 0 ? op.window : INT_MAX / 2;
+    const int see_from = max(position - window + 1, 0), see_to = real ? position + 1 : 0;
+    const int first_position = base_position + row0 / a.group, last_position = base_position + min((row0 + kWaveRows - 1) / a.group, q.n - 1);
+    const int all_from = max(last_position - window + 1, 0), all_to = first_position + 1;
+    const int any_from = max(first_position - window + 1, 0), any_to = row0 < rows ? last_position + 1 : 0;
+
+    I32x4 digits[kDig][kSteps];
+    float unit;
+    {
+      const int64_t from = (q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride;
+      float most = 0.0f;
+      bool finite = true;
+#pragma unroll
+      for (int s = 0; s < 2 * kSteps; ++s) {
+        float v[8];
+        LoadEight<TYPE>(op.q, from + 32 * (s / 2) + 16 * half + 8 * (s % 2), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          finite = finite && fabsf(v[e]) <= 3.402823466e38f;
+          most = fmaxf(most, fabsf(v[e]));
+        }
+      }
+      most = AcrossHalvesMax(most);
+      const float bad = AcrossHalvesMax(finite ? 0.0f : 1.0f);
+      const bool small = !(most > 0x1p-100f);
+      const float inverse = small ? 0.0f : kDigitMax<TYPE> / most;
+      unit = bad > 0.0f ? __builtin_nanf("") : small ? 0.0f : most / kDigitMax<TYPE>;
+      // (A negative scale goes into the digits: the units stay positive, so the largest product is the largest logit.)
+      const float turned = op.scale < 0.0f ? -inverse : inverse;
+#pragma unroll
+      for (int s = 0; s < 2 * kSteps; ++s) {
+        float v[8];
+        LoadEight<TYPE>(op.q, from + 32 * (s / 2) + 16 * half + 8 * (s % 2), v);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t packed[kDig];
+#pragma unroll
+          for (int d = 0; d < kDig; ++d) packed[d] = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            int digit[kDig];
+            SplitDigits<kDig>(bad > 0.0f || !real ? 0 : static_cast<int>(rintf(v[4 * k + e] * turned)), digit);
+#pragma unroll
+            for (int d = 0; d < kDig; ++d) packed[d] |= static_cast<uint32_t>(digit[d] & 0xFF) << (8 * e);
+          }
+#pragma unroll
+          for (int d = 0; d < kDig; ++d) digits[d][s / 2][2 * (s % 2) + k] = static_cast<int>(packed[d]);
+        }
+      }
+      unit *= fabsf(op.scale) * (op.softcap != 0.0f ? 1.0f : kLog2E);
+    }
+    const float cap_inverse = op.softcap != 0.0f ? 1.0f / op.softcap : 0.0f;
+
+    // ---- the tiles' loads. The page of the tile's 16-token group `lane & 3`, from every lane.
+    const int p16 = c.page / 16;
+    struct Group {
+      int page, offset;
+    };
+    const auto group_of = [&](int tile) {
+      Group g;
+      const int n16 = 4 * tile + (lane & 3);
+      const int entry = static_cast<int>(PagedDivide(n16, a.page_magic));
+      g.offset = 16 * (n16 - entry * p16);
+      g.page = -1;
+      if (entry < op.table_width && 16 * n16 < q.length) g.page = table[entry];
+      if (g.page >= c.pages) g.page = -1;
+      return g;
+    };
+    const int64_t page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
+    const uint8_t* const k_base = static_cast<const uint8_t*>(c.k) + static_cast<int64_t>(head) * c.page * D;
+    const uint8_t* const v_base = static_cast<const uint8_t*>(c.v) + static_cast<int64_t>(head) * c.page * D;
+    U32x4 k_in[kLoads], v_in[kLoads];
+    F32x4 scales_in;
+    const auto fetch = [&](const Group& g) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int i = tid + kThreads * j;
+        const int t = i / kPieces, k_group = t >> 4;
+        const uint8_t* from = k_base + max(__shfl(g.page, k_group), 0) * page_bytes + (__shfl(g.offset, k_group) + (t & 15)) * D + 16 * (i % kPieces);
+        k_in[j] = *reinterpret_cast<const U32x4*>(from);
+        from = v_base + max(__shfl(g.page, i & 3), 0) * page_bytes + (i >> 2) * c.page + __shfl(g.offset, i & 3);
+        v_in[j] = *reinterpret_cast<const U32x4*>(from);
+      }
+      if (tid < 4) {
+        const int64_t at = static_cast<int64_t>(max(g.page, 0)) * c.kv_heads + head;
+        scales_in = F32x4{c.k_scale[at], c.v_scale[at], g.page >= 0 ? 1.0f : 0.0f, 0.0f};
+      }
+    };
+    const auto place = [&](int buffer) {
+      uint8_t* const k_at = lds + buffer * G::kBuffer;
+      uint8_t* const v_at = k_at + G::kKBytes;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int i = tid + kThreads * j;
+        const int t = i / kPieces, x = t & 31;
+        const int k_row = (t & 32) + 8 * ((x >> 2) & 3) + 4 * (x >> 4) + (x & 3);
+        *reinterpret_cast<U32x4*>(k_at + k_row * D + 16 * Turn<kPieces>(k_row, i % kPieces)) = k_in[j];
+        const int d = i >> 2, piece = 2 * (i & 3);
+        *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece)) = EightCodes(v_in[j][0], v_in[j][1]);
+        *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece + 1)) = EightCodes(v_in[j][2], v_in[j][3]);
+      }
+      if (tid < 4) group_scales[buffer * 4 + tid] = scales_in;
+    };
+
+    float top = -INFINITY, sum = 0.0f;
+    F32x16 out[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) out[b][i] = 0.0f;
+    }
+    const int tile_from = pair.first_tile + t_first, tile_to = tile_from + t_count;
+    Group next = group_of(tile_from);
+    fetch(next);
+    next = group_of(tile_from + 1);
+    place(0);
+    __syncthreads();
+    for (int tile = tile_from; tile < tile_to; ++tile) {
+      const int buffer = (tile - tile_from) & 1;
+      const bool more = tile + 1 < tile_to;
+      if (more) {
+        fetch(next);
+        next = group_of(tile + 2);
+      }
+      if (tile * kTileTokens < any_to && (tile + 1) * kTileTokens > any_from) {
+        const uint8_t* const k_at = lds + buffer * G::kBuffer;
+        const uint8_t* const v_at = k_at + G::kKBytes;
+        // ---- S^T = K Q^T: 32 tokens at a time
+        float s[2][16], ks[2], vs[2];
+        bool there[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          I32x16 dots[kDig];
+#pragma unroll
+          for (int d = 0; d < kDig; ++d) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dots[d][i] = 0;
+          }
+          const int k_row = 32 * h + column;
+#pragma unroll
+          for (int x = 0; x < kSteps; ++x) {
+            const I32x4 k = *reinterpret_cast<const I32x4*>(k_at + k_row * D + 16 * Turn<kPieces>(k_row, 2 * x + half));
+#pragma unroll
+            for (int d = 0; d < kDig; ++d) dots[d] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, digits[d][x], dots[d], 0, 0, 0);
+          }
+          const F32x4 scales = group_scales[buffer * 4 + 2 * h + half];
+          ks[h] = scales[0], vs[h] = scales[1], there[h] = scales[2] != 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[h][i] = JoinDigits<kDig>(dots[0][i], kDig == 3 ? dots[1][i] : 0, dots[kDig - 1][i]);
+        }
+        // ---- softmax
+        const bool whole = (tile + 1) * kTileTokens <= all_to && tile * kTileTokens >= all_from && __all(there[0] && there[1]);
+        float worth[2] = {unit * ks[0], unit * ks[1]};
+        uint32_t seen[2] = {0xFFFFu, 0xFFFFu};
+        if (op.softcap != 0.0f || !whole) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (op.softcap != 0.0f) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[h][i] = Capped<TYPE>(s[h][i] * worth[h], op.softcap, cap_inverse) * kLog2E;
+              worth[h] = 1.0f;
+            }
+            if (!whole) {
+              if (!there[h]) vs[h] = 0.0f, worth[h] = 1.0f;
+              seen[h] = 0;
+              const int p0 = tile * kTileTokens + 32 * h + 16 * half;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const bool sees = there[h] && p0 + i >= see_from && p0 + i < see_to;
+                seen[h] |= sees ? 1u << i : 0u;
+                s[h][i] = sees ? s[h][i] : -INFINITY;
+              }
+            }
+          }
+        }
+        float peak = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float high = s[h][0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) high = fmaxf(high, s[h][i]);
+          // (-inf times a unit of zero is no number: nothing seen stays nothing.)
+          peak = fmaxf(peak, high == -INFINITY ? high : fmaf(high, worth[h], ScaleLog(vs[h])));
+        }
+        peak = AcrossHalvesMax(peak);
+        if (__any(peak > top)) {
+          const float higher = fmaxf(top, peak);
+          const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+          top = higher;
+          sum *= keep;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
+        }
+        const float from = top == -INFINITY ? 0.0f : top;
+        F16x8 p[2][2], p_low[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[i] = __builtin_amdgcn_exp2f(fmaf(s[h][i], worth[h], -from));
+            if (!whole) v[i] = (seen[h] >> i) & 1u ? v[i] : 0.0f;  // (a hidden token's weight is zero whatever its page's scales are)
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sum += v[i];
+            v[i] *= vs[h];
+            if (!whole) v[i] = (seen[h] >> i) & 1u ? v[i] : 0.0f;
+            p[h][i / 8][i % 8] = static_cast<_Float16>(v[i]);
+            if constexpr (kDig == 3) p_low[h][i / 8][i % 8] = static_cast<_Float16>(v[i] - static_cast<float>(p[h][i / 8][i % 8]));
+          }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+              const int d = 32 * b + column;
+              const F16x8 v = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 4 * h + 2 * half + x));
+              out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[h][x], out[b], 0, 0, 0);
+              if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[h][x], out[b], 0, 0, 0);
+            }
+          }
+        }
+      }
+      if (more) place(buffer ^ 1);
+      __syncthreads();
+    }
+    sum = AcrossHalvesSum(sum);
+
+    // ---- the rows' values, or this part's.
+    const bool begins = t_first == 0, ends = t_first + t_count == pair.tiles;
+    if (begins && ends) {
+      if (real) {
+        const int h = head * a.group + query_head;
+        if (op.sinks != nullptr) sum += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(top == -INFINITY ? 0.0f : top)));
+        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t to = (q.start + token) * op.out_token_stride + h * op.out_head_stride;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x[4] = {out[b][4 * i] * inverse, out[b][4 * i + 1] * inverse, out[b][4 * i + 2] * inverse, out[b][4 * i + 3] * inverse};
+            StoreValues<TYPE, 4>(op.out, to + 32 * b + 8 * i + 4 * half, x);
+          }
+        }
+      }
+    } else {
+      float* const to = m.partial + ((2 * static_cast<int64_t>(w) + (begins ? 1 : 0)) * kManyRows + wave * kWaveRows + column) * (D + 2);
+      if (half == 0) to[0] = top, to[1] = sum;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[2 + 32 * b + 8 * (i / 4) + 4 * half + i % 4] = out[b][i];
+      }
+      if (begins) {
+        const int64_t segment_end = m.list.before[pair_index] + static_cast<int64_t>(head + 1) * pair.tiles;
+        part = I32x4{static_cast<int>((segment_end - 1) / per), pair_index, head, 0};
+      }
+    }
+  }
+  if (tid == 0) *reinterpret_cast<I32x4*>(m.parts + 4 * w) = part;
+}
+
+// grid (workgroups of the launch before, kManyRows / 4): the parts of the segment that begins in workgroup x and ends in
+// another, a wave a row.
+template <int TYPE, int D>
+__global__ __launch_bounds__(kThreads) void ManyJoinKernel(const ManyArgs m) {
+  constexpr int kPer = D / kWave;
+  const PagedAttendArgs& a = m.a;
+  const llmp_paged_attend& op = a.op;
+  const I32x4 part = *reinterpret_cast<const I32x4*>(m.parts + 4 * blockIdx.x);
+  if (part.x < 0) return;
+  const int lane = threadIdx.x & (kWave - 1), in_slot = 4 * blockIdx.y + threadIdx.x / kWave;
+  const Pair pair = m.list.pairs[part.y];
+  const PagedRequest q = RequestOf(op.starts, op.lengths, pair.request, op.tokens, a.most_length);
+  const int row = pair.chunk * kManyRows + in_slot;
+  if (row >= q.n * a.group) return;
+  const int first = blockIdx.x, last = part.x;
+  const auto slot_of = [&](int w) { return m.partial + ((2 * static_cast<int64_t>(w) + (w == first ? 1 : 0)) * kManyRows + in_slot) * (D + 2); };
+  float high = -INFINITY;
+  for (int w = first + lane; w <= last; w += kWave) high = fmaxf(high, slot_of(w)[0]);
+#pragma unroll
+  for (int step = 1; step < kWave; step <<= 1) high = fmaxf(high, __shfl_xor(high, step));
+  float all = 0.0f, value[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
+#pragma unroll 4
+  for (int w = first; w <= last; ++w) {
+    const float* from = slot_of(w);
+    const float top = from[0];
+    const float keep = top == -INFINITY ? (high == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top - high);
+    all += from[1] * keep;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) value[e] += from[2 + kPer * lane + e] * keep;
+  }
+  const int h = part.z * a.group + row % a.group;
+  if (op.sinks != nullptr) all += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(high == -INFINITY ? 0.0f : high)));
+  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
+  const int64_t to = (q.start + row / a.group) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e] * inverse);
+}
+
+int ManyGroups(int head_dim, int cus) { return (head_dim == 256 ? 1 : 2) * (cus > 0 ? cus : 256); }
+int64_t MostPairs(const llmp_paged_attend& op, int group) {
+  // (Requests of more than few_rows rows only, and few_rows is at least half of kManyRows: two pairs of every kManyRows rows at most.)
+  return 2 * (static_cast<int64_t>(op.tokens) * group / kManyRows + 1);
+}
+size_t Up(size_t bytes) { return (bytes + 15) & ~static_cast<size_t>(15); }
+
+template <int TYPE, int D>
+void LaunchMany(const ManyArgs& m, int groups, hipStream_t stream) {
+  using G = ManyGeo<D>;
+  static bool sized = false;
+  if (G::kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&ManyKernel<TYPE, D>), G::kLds, &sized)) return;
+  hipLaunchKernelGGL(ListKernel, dim3(1), dim3(kListThreads), 0, stream, m, groups);
+  hipLaunchKernelGGL((ManyKernel<TYPE, D>), dim3(groups), dim3(kThreads), G::kLds, stream, m);
+  hipLaunchKernelGGL((ManyJoinKernel<TYPE, D>), dim3(groups, kManyRows / 4), dim3(kThreads), 0, stream, m);
+}
+template <int TYPE>
+void LaunchManyOf(const ManyArgs& m, int groups, hipStream_t stream) {
+  if (m.a.op.cache.head_dim == 64) LaunchMany<TYPE, 64>(m, groups, stream);
+  if (m.a.op.cache.head_dim == 128) LaunchMany<TYPE, 128>(m, groups, stream);
+  if (m.a.op.cache.head_dim == 256) LaunchMany<TYPE, 256>(m, groups, stream);
+}
+
+}  // namespace
+
+size_t PagedManyScratch(const llmp_paged_attend& op, int cus) {
+  const int groups = ManyGroups(op.cache.head_dim, cus);
+  const size_t pairs = static_cast<size_t>(MostPairs(op, op.heads / op.cache.kv_heads));
+  return Up(sizeof(ListHeader)) + Up(pairs * sizeof(Pair)) + Up((pairs + 1) * sizeof(int64_t)) + Up(pairs * sizeof(int32_t)) + 16 * static_cast<size_t>(groups) +
+         2 * static_cast<size_t>(groups) * kManyRows * (op.cache.head_dim + 2) * sizeof(float);
+}
+
+void PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStream_t stream) {
+  const int groups = ManyGroups(args.op.cache.head_dim, cus);
+  ManyArgs m;
+  m.a = args;
+  m.most_pairs = static_cast<int>(MostPairs(args.op, args.group));
+  m.a_unit = args.op.cache.head_dim == 256 ? 1 : 2;
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  const auto take = [&](size_t bytes) {
+    void* p = at;
+    at += Up(bytes);
+    return p;
+  };
+  m.list.header = static_cast<ListHeader*>(take(sizeof(ListHeader)));
+  m.list.pairs = static_cast<Pair*>(take(m.most_pairs * sizeof(Pair)));
+  m.list.before = static_cast<int64_t*>(take((m.most_pairs + 1) * sizeof(int64_t)));
+  m.list.order = static_cast<int32_t*>(take(m.most_pairs * sizeof(int32_t)));
+  m.parts = static_cast<int32_t*>(take(16 * static_cast<size_t>(groups)));
+  m.partial = reinterpret_cast<float*>(at);
+  if (args.op.type == LLMP_X_F32) LaunchManyOf<LLMP_X_F32>(m, groups, stream);
+  if (args.op.type == LLMP_X_BF16) LaunchManyOf<LLMP_X_BF16>(m, groups, stream);
+  if (args.op.type == LLMP_X_F16) LaunchManyOf<LLMP_X_F16>(m, groups, stream);
+}
+
+}  // namespace llmp_hip
