@@ -25,6 +25,7 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kWaveRows = 32;
 constexpr int kManyRows = kWaves * kWaveRows;
 constexpr int kListThreads = 1024;
+constexpr float kSlack = 8.0f;   // how far the running maximum may lag, in log2
 constexpr int kBuckets = 1024;  // of the segments' lengths, for their order
 
 // The list: a header, the pairs, the tiles before each pair (times KV heads), the pairs' order by length.
@@ -147,7 +148,7 @@ struct ManyGeo {
   static constexpr int kAUnit = D == 256 ? 1 : 2;        // workgroups a compute unit: 512 or 256 registers a lane
 };
 
-template <int TYPE, int D>
+template <int TYPE, int D, bool CAPPED>
 __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const ManyArgs m) {
   using G = ManyGeo<D>;
   constexpr int kDig = kDigits<TYPE>;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
   const int half = lane >> 5, column = lane & 31;
   const int groups = gridDim.x, w = blockIdx.x;
   const ListHeader header = *m.list.header;
-  F32x4* const group_scales = reinterpret_cast<F32x4*>(lds + 2 * G::kBuffer);  // [buffer][group]: K's and V's scale, 1 if there is a page
+  F32x4* const group_scales = reinterpret_cast<F32x4*>(lds + 2 * G::kBuffer);  // [buffer][group]: K's and V's scale, V's log2 and reciprocal
 
   int64_t u = 0, u_end = 0, per = 1;
   int turn = 0, pair_index = 0;
@@ -313,7 +314,9 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
       }
       if (tid < 4) {
         const int64_t at = static_cast<int64_t>(max(g.page, 0)) * c.kv_heads + head;
-        scales_in = F32x4{c.k_scale[at], c.v_scale[at], g.page >= 0 ? 1.0f : 0.0f, 0.0f};
+        const float vs = c.v_scale[at];
+        // (A logarithm of -infinity: no page.)
+        scales_in = F32x4{c.k_scale[at], vs, g.page >= 0 ? ScaleLog(vs) : -INFINITY, g.page >= 0 ? 1.0f / vs : 0.0f};
       }
     };
     const auto place = [&](int buffer) {
@@ -355,9 +358,8 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
       if (tile * kTileTokens < any_to && (tile + 1) * kTileTokens > any_from) {
         const uint8_t* const k_at = lds + buffer * G::kBuffer;
         const uint8_t* const v_at = k_at + G::kKBytes;
-        // ---- S^T = K Q^T: 32 tokens at a time
-        float s[2][16], ks[2], vs[2];
-        bool there[2];
+        const bool inside = (tile + 1) * kTileTokens <= all_to && tile * kTileTokens >= all_from;
+        // ---- 32 tokens at a time: S^T = K Q^T, their softmax, O^T += V^T P^T
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           I32x16 dots[kDig];
@@ -373,84 +375,73 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
 #pragma unroll
             for (int d = 0; d < kDig; ++d) dots[d] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, digits[d][x], dots[d], 0, 0, 0);
           }
-          const F32x4 scales = group_scales[buffer * 4 + 2 * h + half];
-          ks[h] = scales[0], vs[h] = scales[1], there[h] = scales[2] != 0.0f;
+          __builtin_amdgcn_sched_barrier(0);
+          const F32x4 scales = group_scales[buffer * 4 + 2 * h + half];  // K's, V's, log2 of V's, 1 / V's
+          float s[16], worth = unit * scales[0], value_log = scales[2];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[h][i] = JoinDigits<kDig>(dots[0][i], kDig == 3 ? dots[1][i] : 0, dots[kDig - 1][i]);
-        }
-        // ---- softmax
-        const bool whole = (tile + 1) * kTileTokens <= all_to && tile * kTileTokens >= all_from && __all(there[0] && there[1]);
-        float worth[2] = {unit * ks[0], unit * ks[1]};
-        uint32_t seen[2] = {0xFFFFu, 0xFFFFu};
-        if (op.softcap != 0.0f || !whole) {
+          for (int i = 0; i < 16; ++i) s[i] = JoinDigits<kDig>(dots[0][i], kDig == 3 ? dots[1][i] : 0, dots[kDig - 1][i]);
+          if constexpr (CAPPED) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (op.softcap != 0.0f) {
+            for (int i = 0; i < 16; ++i) s[i] = Capped<TYPE>(s[i] * worth, op.softcap, cap_inverse) * kLog2E;
+            worth = 1.0f;
+          }
+          // The short way: every row sees all 32 tokens, and V's scales have logarithms and reciprocals that no exponent runs out of.
+          const bool whole = inside && __all(scales[3] > 0x1p-60f && scales[3] < 0x1p60f);
+          if (!whole) {
+            asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
+            const int p0 = tile * kTileTokens + 32 * h + 16 * half;
+            const int from = value_log == -INFINITY ? 16 : max(see_from - p0, 0), to = see_to - p0;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) s[h][i] = Capped<TYPE>(s[h][i] * worth[h], op.softcap, cap_inverse) * kLog2E;
-              worth[h] = 1.0f;
+            for (int i = 0; i < 16; ++i) s[i] = i >= from && i < to ? s[i] * worth : -INFINITY;
+            worth = 1.0f;
+          }
+          float peak = s[0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) peak = fmaxf(peak, s[i]);
+          peak = AcrossHalvesMax(fmaf(peak, worth, value_log));
+          // The maximum follows once it is kSlack behind: weights up to 2^kSlack keep their F16's precision, and the sums rarely turn.
+          if (__any(peak > top + kSlack)) {
+            const float higher = fmaxf(top, peak);
+            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+            top = higher;
+            sum *= keep;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
+          }
+          F16x8 p[2], p_low[2];
+          const auto pack = [&](int i, float weight) {
+            p[i / 8][i % 8] = static_cast<_Float16>(weight);
+            if constexpr (kDig == 3) p_low[i / 8][i % 8] = static_cast<_Float16>(weight - static_cast<float>(p[i / 8][i % 8]));
+          };
+          if (whole) {  // V's scale in the exponent: the weights at once, and the probabilities' sum from theirs
+            const float less = value_log - top;
+            float weights = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float v = __builtin_amdgcn_exp2f(fmaf(s[i], worth, less));
+              weights += v;
+              pack(i, v);
             }
-            if (!whole) {
-              if (!there[h]) vs[h] = 0.0f, worth[h] = 1.0f;
-              seen[h] = 0;
-              const int p0 = tile * kTileTokens + 32 * h + 16 * half;
+            sum = fmaf(weights, scales[3], sum);
+          } else {
+            asm volatile("" ::: "memory");
+            const float less = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const bool sees = there[h] && p0 + i >= see_from && p0 + i < see_to;
-                seen[h] |= sees ? 1u << i : 0u;
-                s[h][i] = sees ? s[h][i] : -INFINITY;
-              }
+            for (int i = 0; i < 16; ++i) {
+              const float v = __builtin_amdgcn_exp2f(s[i] - less);
+              sum += v;
+              pack(i, s[i] == -INFINITY ? 0.0f : v * scales[1]);  // (a hidden token's weight is zero whatever its page's scales are)
             }
           }
-        }
-        float peak = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float high = s[h][0];
-#pragma unroll
-          for (int i = 1; i < 16; ++i) high = fmaxf(high, s[h][i]);
-          // (-inf times a unit of zero is no number: nothing seen stays nothing.)
-          peak = fmaxf(peak, high == -INFINITY ? high : fmaf(high, worth[h], ScaleLog(vs[h])));
-        }
-        peak = AcrossHalvesMax(peak);
-        if (__any(peak > top)) {
-          const float higher = fmaxf(top, peak);
-          const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
-          top = higher;
-          sum *= keep;
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
-        }
-        const float from = top == -INFINITY ? 0.0f : top;
-        F16x8 p[2][2], p_low[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float v[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            v[i] = __builtin_amdgcn_exp2f(fmaf(s[h][i], worth[h], -from));
-            if (!whole) v[i] = (seen[h] >> i) & 1u ? v[i] : 0.0f;  // (a hidden token's weight is zero whatever its page's scales are)
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            sum += v[i];
-            v[i] *= vs[h];
-            if (!whole) v[i] = (seen[h] >> i) & 1u ? v[i] : 0.0f;
-            p[h][i / 8][i % 8] = static_cast<_Float16>(v[i]);
-            if constexpr (kDig == 3) p_low[h][i / 8][i % 8] = static_cast<_Float16>(v[i] - static_cast<float>(p[h][i / 8][i % 8]));
-          }
-        }
-        // ---- O^T += V^T P^T
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
               const int d = 32 * b + column;
               const F16x8 v = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 4 * h + 2 * half + x));
-              out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[h][x], out[b], 0, 0, 0);
-              if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[h][x], out[b], 0, 0, 0);
+              out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], out[b], 0, 0, 0);
+              if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[x], out[b], 0, 0, 0);
             }
           }
         }
@@ -544,10 +535,16 @@ size_t Up(size_t bytes) { return (bytes + 15) & ~static_cast<size_t>(15); }
 template <int TYPE, int D>
 void LaunchMany(const ManyArgs& m, int groups, hipStream_t stream) {
   using G = ManyGeo<D>;
-  static bool sized = false;
-  if (G::kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&ManyKernel<TYPE, D>), G::kLds, &sized)) return;
+  static bool sized = false, sized_capped = false;
+  const bool capped = m.a.op.softcap != 0.0f;
+  if (G::kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&ManyKernel<TYPE, D, false>), G::kLds, &sized)) return;
+  if (G::kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&ManyKernel<TYPE, D, true>), G::kLds, &sized_capped)) return;
   hipLaunchKernelGGL(ListKernel, dim3(1), dim3(kListThreads), 0, stream, m, groups);
-  hipLaunchKernelGGL((ManyKernel<TYPE, D>), dim3(groups), dim3(kThreads), G::kLds, stream, m);
+  if (capped) {
+    hipLaunchKernelGGL((ManyKernel<TYPE, D, true>), dim3(groups), dim3(kThreads), G::kLds, stream, m);
+  } else {
+    hipLaunchKernelGGL((ManyKernel<TYPE, D, false>), dim3(groups), dim3(kThreads), G::kLds, stream, m);
+  }
   hipLaunchKernelGGL((ManyJoinKernel<TYPE, D>), dim3(groups, kManyRows / 4), dim3(kThreads), 0, stream, m);
 }
 template <int TYPE>
