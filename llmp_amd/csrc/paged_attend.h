@@ -16,18 +16,21 @@ namespace llmp_hip {
 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kTileTokens = 64;
+constexpr float kSlack = 8.0f;  // how far the running maximum may lag, in log2
 
 struct PagedAttendArgs {
   llmp_paged_attend op;
   float* partial;       // the few rows' form: [2 * workgroups][16][D + 2]: E, sum, values
   int32_t* parts;       // [workgroups][4]
-  uint32_t page_magic;  // n / (page / 16) by a multiplication: PagedDivide
+  uint32_t page_magic;   // n / (page / 16) by a multiplication: PagedDivide
+  uint32_t group_magic;  // n / group
   int group;            // query heads a KV head
   int most_length;      // tokens a table row can name
+  int shift;            // the few rows' form: a unit of the line is 2^shift tiles
   int few_rows;         // requests of more (token, head) rows than these are the many rows' form's
 };
 
-// n / d for n < 2^26 and d from 1 to 16, magic = 2^32 / d + 1 (0 for d = 1): n times the magic's excess stays below 2^32 / d.
+// n / d for n * d < 2^32, magic = 2^32 / d + 1 (0 for d = 1): n times the magic's excess stays below 2^32 / d.
 __device__ __forceinline__ uint32_t PagedDivide(uint32_t n, uint32_t magic) { return magic == 0 ? n : __umulhi(n, magic); }
 
 // Over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (the same column of a 16-column matrix tile): x in two registers, the odd rows of
@@ -35,6 +38,16 @@ __device__ __forceinline__ uint32_t PagedDivide(uint32_t n, uint32_t magic) { re
 // compiler's builtin gives one of the two results for both. The wait states are those between a vector write and the swap.)
 __device__ __forceinline__ void SwapRows16(float& a, float& b) { asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
 __device__ __forceinline__ void SwapHalves(float& a, float& b) { asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ uint32_t AcrossHalvesMost(uint32_t v) {
+  float a = __builtin_bit_cast(float, v), b = a;
+  SwapHalves(a, b);
+  return max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
+__device__ __forceinline__ uint32_t AcrossGroupsMost(uint32_t v) {
+  float a = __builtin_bit_cast(float, v), b = a;
+  SwapRows16(a, b);
+  return AcrossHalvesMost(max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)));
+}
 __device__ __forceinline__ float AcrossHalvesMax(float v) {
   float w = v;
   SwapHalves(v, w);
@@ -56,20 +69,116 @@ __device__ __forceinline__ float AcrossGroupsSum(float v) {
   return AcrossHalvesSum(v + w);
 }
 
+// Over the lanes of a column of a ROWS-column tile.
+template <int ROWS>
+__device__ __forceinline__ float Across(float v) { return ROWS == 32 ? AcrossHalvesMax(v) : AcrossGroupsMax(v); }
+template <int ROWS>
+__device__ __forceinline__ uint32_t Across(uint32_t v) { return ROWS == 32 ? AcrossHalvesMost(v) : AcrossGroupsMost(v); }
+template <int ROWS>
+__device__ __forceinline__ float AcrossSum(float v) { return ROWS == 32 ? AcrossHalvesSum(v) : AcrossGroupsSum(v); }
+// Inclusive sums over the wave's lanes: within rows of 16 by shifts, then each row's last to the next row, the lower half's to the
+// upper one.
+__device__ __forceinline__ uint32_t WaveSums(uint32_t v) {
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x111, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x112, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x114, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x118, 0xF, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xA, 0xF, false));
+  v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xC, 0xF, false));
+  return v;
+}
+
 template <int TYPE>
 constexpr int kDigits = TYPE == LLMP_X_F32 ? 3 : 2;
 template <int TYPE>
 constexpr float kDigitMax = TYPE == LLMP_X_F32 ? 8355584.0f : 32639.0f;  // 0x7F7F00: a rounding up still fits three digits; 0x7F7F
 
-// Whole numbers' balanced digits, the highest first: each in -128 to 127.
-template <int DIGITS>
-__device__ __forceinline__ void SplitDigits(int x, int (&digit)[DIGITS]) {
+// Part of a query row: N eights of values as they lie in memory.
+template <int TYPE, int N>
+struct QueryPart {
+  static constexpr int kWords = TYPE == LLMP_X_F32 ? 2 : 1;  // 16-byte words an eight
+  U32x4 raw[N * kWords];
+  __device__ __forceinline__ void Load(const void* base, int i, int64_t element) {
+    const U32x4* from = TYPE == LLMP_X_F32 ? reinterpret_cast<const U32x4*>(static_cast<const float*>(base) + element)
+                                           : reinterpret_cast<const U32x4*>(static_cast<const uint16_t*>(base) + element);
 #pragma unroll
-  for (int i = DIGITS - 1; i > 0; --i) {
-    digit[i] = static_cast<int8_t>(x);
-    x = (x - digit[i]) >> 8;
+    for (int w = 0; w < kWords; ++w) raw[i * kWords + w] = from[w];
   }
-  digit[0] = x;
+  // The largest magnitude as bits: their order is the magnitudes', infinities and NaN the largest.
+  __device__ __forceinline__ uint32_t MostBits() const {
+    typedef unsigned short U16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (TYPE == LLMP_X_F32) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < N * kWords; ++i) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = max(most, raw[i][w] & 0x7FFFFFFFu);
+      }
+      return most;
+    } else {
+      U16x2 most = {0, 0};
+#pragma unroll
+      for (int i = 0; i < N * kWords; ++i) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(U16x2, raw[i][w] & 0x7FFF7FFFu));
+      }
+      return max(most.x, most.y);
+    }
+  }
+  __device__ __forceinline__ void Four(int i, int half, float (&v)[4]) const {
+    if constexpr (TYPE == LLMP_X_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t word = raw[2 * i + half][e];  // (a copy: the cast of the element itself reads the vector's first)
+        v[e] = __builtin_bit_cast(float, word);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t word = raw[i][2 * half + e / 2], bits = e % 2 ? word >> 16 : word & 0xFFFFu;
+        v[e] = TYPE == LLMP_X_BF16 ? (e % 2 ? __builtin_bit_cast(float, word & 0xFFFF0000u) : Bf16BitsToFloat(bits)) : HalfBitsToFloat(bits);
+      }
+    }
+  }
+};
+// A row's unit from its largest magnitude's bits, and what takes values to whole numbers of it.
+struct QueryUnit {
+  float unit, inverse;
+};
+template <int TYPE>
+__device__ __forceinline__ QueryUnit UnitOf(uint32_t most_bits) {
+  constexpr uint32_t kInfinity = TYPE == LLMP_X_F32 ? 0x7F800000u : TYPE == LLMP_X_BF16 ? 0x7F80u : 0x7C00u;
+  const float most = TYPE == LLMP_X_F32 ? __builtin_bit_cast(float, most_bits) : TYPE == LLMP_X_BF16 ? Bf16BitsToFloat(most_bits) : HalfBitsToFloat(most_bits);
+  // (A row of zeros, or of magnitudes whose reciprocal is none, is zeros; one with an infinity or a NaN has no logits.)
+  const bool bad = most_bits >= kInfinity, small = !(most > 0x1p-100f);
+  return {bad ? __builtin_nanf("") : small ? 0.0f : most / kDigitMax<TYPE>, bad || small ? 0.0f : kDigitMax<TYPE> / most};
+}
+// Four values' digits, the highest first, each balanced (-128 to 127): the bytes of the whole number once what the lower digits
+// borrow is added.
+template <int DIGITS>
+__device__ __forceinline__ void PackDigits(const float (&v)[4], float inverse, uint32_t (&packed)[DIGITS]) {
+  uint32_t q[4], up[4];
+  const auto bytes = [](const uint32_t (&x)[4], uint32_t low_pair, uint32_t high_pair) {
+    return __builtin_amdgcn_perm(x[1], x[0], low_pair) | __builtin_amdgcn_perm(x[3], x[2], high_pair);
+  };
+  if constexpr (DIGITS == 2) {
+    // (Added to 1.5 * 2^23 a value is rounded to a whole number, and that is what the float's low bits are.)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = __builtin_bit_cast(uint32_t, fmaf(v[e], inverse, 12582912.0f)), up[e] = q[e] + 0x80u;
+    packed[0] = bytes(up, 0x0C0C0501u, 0x05010C0Cu);
+    packed[1] = bytes(q, 0x0C0C0400u, 0x04000C0Cu);
+  } else {
+    uint32_t top[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float whole = rintf(v[e] * inverse);
+      q[e] = static_cast<uint32_t>(static_cast<int>(whole == whole ? whole : 0.0f));
+      up[e] = q[e] + 0x80u, top[e] = q[e] + 0x8080u;
+    }
+    packed[0] = bytes(top, 0x0C0C0602u, 0x06020C0Cu);
+    packed[1] = bytes(up, 0x0C0C0501u, 0x05010C0Cu);
+    packed[2] = bytes(q, 0x0C0C0400u, 0x04000C0Cu);
+  }
 }
 
 // The sums of the digits' products as one float: three digits' pass 2^31.
@@ -89,6 +198,16 @@ __device__ __forceinline__ F16x8 EightCodes(uint32_t a, uint32_t b) {
   const F16x2 v0 = TwoCodes(a, 0x00050004u), v1 = TwoCodes(a, 0x00070006u), v2 = TwoCodes(b, 0x00050004u), v3 = TwoCodes(b, 0x00070006u);
   return F16x8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
 }
+
+// Where in a row of LDS a piece of 16 bytes lies (and which piece lies there): the 16 lanes that read a piece of 16 rows at once,
+// tokens 16a + 4t + b for K and dimensions in order for V, find it at 16 places of the 256 bytes that the banks hold.
+template <int D>
+__device__ __forceinline__ int KPiece(int token, int piece) {
+  if constexpr (D == 64) return piece ^ ((token >> 4) & 3);
+  if constexpr (D == 128) return piece ^ (((token >> 1) & 1) | ((token >> 4) & 3) << 1);
+  return piece ^ ((token & 3) | ((token >> 4) & 3) << 2);
+}
+__device__ __forceinline__ int VPiece(int d, int piece) { return piece ^ ((d >> 2) & 3); }
 
 // softcap * tanh(s / softcap). F32 results take the library's tanh; 16-bit ones 1 - 2 / (e^2x + 1), whose error (2^-23 of the
 // softcap) is far below their rounding.

@@ -25,13 +25,14 @@ constexpr int kFewWaves = 4;
 constexpr int kFewThreads = kFewWaves * kWave;
 constexpr int kRows = 16;  // rows of a segment: (token, head) pairs
 
-// A request's segments and tiles in this form; units = segments * tiles.
+// A request's segments and tiles in this form. A unit of the line is 2^shift tiles of a segment (shift 0 but where the line would
+// pass 2^31).
 struct FewRequest {
   PagedRequest q;
   int segments;    // row chunks times KV heads
   int first_tile;  // tiles before it lie before every row's window
   int tiles;
-  int64_t units;
+  uint32_t units;
 };
 template <bool LISTS>
 __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r) {
@@ -50,82 +51,118 @@ __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r) {
     f.tiles = max((f.q.length + kTileTokens - 1) / kTileTokens - f.first_tile, 1);  // (a row that sees nothing is written too)
   }
   f.segments = chunks * op.cache.kv_heads;
-  f.units = static_cast<int64_t>(f.segments) * f.tiles;
+  f.units = static_cast<uint32_t>(f.segments) * static_cast<uint32_t>(((f.tiles - 1) >> a.shift) + 1);
   return f;
 }
+// Lane `lane`'s in every lane.
+__device__ __forceinline__ FewRequest FewFrom(const FewRequest& f, int lane) {
+  const auto from = [&](int v) { return __builtin_amdgcn_readlane(v, lane); };
+  return {{from(f.q.start), from(f.q.n), from(f.q.length)}, from(f.segments), from(f.first_tile), from(f.tiles), static_cast<uint32_t>(from(static_cast<int>(f.units)))};
+}
 
-// Where a lane's 16 tokens lie.
+// A tile of K and V of a head.
+constexpr int TileBytes(int head_dim) { return 2 * kTileTokens * head_dim; }
+constexpr int FewLds(int head_dim) {
+  const int land = kFewWaves * TileBytes(head_dim), meet = kFewWaves * kRows * (head_dim + 4) * 4;
+  return land > meet ? land : meet;
+}
+// Workgroups a compute unit: by registers and LDS, 128 KB of tiles on their way either way (96 KB at 64).
+constexpr int FewAUnit(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
+// A lane's 16 bytes from memory to LDS at `to` (the same in every lane) + 16 lane.
+__device__ __forceinline__ void ToLds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(reinterpret_cast<uintptr_t>(from)),
+                                   reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(reinterpret_cast<uintptr_t>(to)), 16, 0, 0);
+}
+
+// Where a lane's 16 tokens of a tile lie.
 struct Place {
   int page;  // in the cache, -1: none
   int position;
   int offset;  // in the page
+  bool there;
 };
-
-__device__ __forceinline__ int64_t WaveSum64(int64_t v) {
-#pragma unroll
-  for (int step = 1; step < kWave; step <<= 1) v += __shfl_xor(v, step);
-  return v;
-}
+struct Entry {
+  int entry;  // of the table row
+  int offset;
+  bool there;
+};
 
 // grid (workgroups).
 template <int TYPE, int D, bool LISTS>
-__global__ __launch_bounds__(kFewThreads, 2) void FewKernel(const PagedAttendArgs a) {
+__global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const PagedAttendArgs a) {
   constexpr int kDig = kDigits<TYPE>;
   constexpr int kSteps = D / 64, kBlocks = D / 16;  // inner steps of K's product, row blocks of V's
+  constexpr int kMine = kTileTokens / 4, kProducts = kTileTokens / 16;  // a lane's tokens of a tile, products of 16 tokens
   constexpr int kPitch = D + 4;
-  extern __shared__ __attribute__((aligned(16))) float meet[];  // [wave][row][kPitch]
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  float* const meet = reinterpret_cast<float*>(lds);  // [wave][row][kPitch]
   __shared__ float tops[kFewWaves][kRows], sums[kFewWaves][kRows];
   const llmp_paged_attend& op = a.op;
   const llmp_paged_cache& c = op.cache;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int group_of = lane >> 4, column = lane & 15;
+  uint8_t* const landing = lds + wave * TileBytes(D);
 
-  // ---- this workgroup's run of the line of units.
-  int64_t total = 0;
-  for (int base = 0; base < op.requests; base += kWave) total += WaveSum64(base + lane < op.requests ? FewOf<LISTS>(a, base + lane).units : 0);
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  per = (per + kFewWaves - 1) / kFewWaves * kFewWaves;  // whole rounds of the waves
-  int64_t u = blockIdx.x * per;
-  const int64_t u_end = min(u + per, total);
+  // ---- this workgroup's run of the line of units: the requests 64 at a time, a lane each.
+  const auto block = [&](int base) {
+    FewRequest f = {};
+    if (base + lane < op.requests) f = FewOf<LISTS>(a, base + lane);
+    return f;
+  };
+  FewRequest mine = block(0);
+  uint32_t upto = WaveSums(mine.units);
+  uint32_t total = __builtin_amdgcn_readlane(upto, kWave - 1), segments = __builtin_amdgcn_readlane(WaveSums(mine.segments), kWave - 1);
+  for (int base = kWave; base < op.requests; base += kWave) {
+    const FewRequest f = block(base);
+    total += __builtin_amdgcn_readlane(WaveSums(f.units), kWave - 1);
+    segments += __builtin_amdgcn_readlane(WaveSums(f.segments), kWave - 1);
+  }
+  // Whole rounds of the waves; where a round is more than there is, no more than an average segment (short ones are not strung
+  // together while there are workgroups for each).
+  const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
+  uint32_t per = (even + kFewWaves - 1) / kFewWaves * kFewWaves;
+  if (even < kFewWaves) per = min(per, max(even, (total + segments - 1) / max(segments, 1u)));
+  uint32_t u = blockIdx.x * per;
+  const uint32_t u_end = min(u + per, total);
   I32x4 part = {-1, 0, 0, 0};
-  if (u >= u_end) {
+  if (u >= u_end || total >= 1u << 31) {
     if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * blockIdx.x) = part;
     return;
   }
   // The request that holds unit u, and the units before it.
-  int r = 0;
-  int64_t before = 0;
-  for (int base = 0, found = 0; base < op.requests && !found; base += kWave) {
-    const int64_t mine = base + lane < op.requests ? FewOf<LISTS>(a, base + lane).units : 0;
-    int64_t upto = mine;
-#pragma unroll
-    for (int step = 1; step < kWave; step <<= 1) {
-      const int64_t other = __shfl_up(upto, step);
-      if (lane >= step) upto += other;
-    }
+  int base = 0, r = 0;
+  uint32_t before = 0;
+  for (;;) {
     const uint64_t past = __ballot(before + upto > u);
     if (past != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
       r = base + at;
-      before += __shfl(upto - mine, at);
-      found = 1;
-    } else {
-      before += __shfl(upto, kWave - 1);
+      before += __builtin_amdgcn_readlane(upto - mine.units, at);
+      break;
     }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    base += kWave;
+    if (base >= op.requests) break;  // (not reached: u is below the sum)
+    mine = block(base);
+    upto = WaveSums(mine.units);
   }
-  r = __builtin_amdgcn_readfirstlane(r);
 
   while (u < u_end && r < op.requests) {
-    const FewRequest f = FewOf<LISTS>(a, r);
-    if (u >= before + f.units) {
+    if (r - base >= kWave) {
+      base += kWave;
+      mine = block(base);
+    }
+    const FewRequest f = FewFrom(mine, r - base);
+    if (u - before >= f.units) {
       before += f.units;
       ++r;
       continue;
     }
-    const int segment = __builtin_amdgcn_readfirstlane(static_cast<int>((u - before) / f.tiles));
-    const int t_first = __builtin_amdgcn_readfirstlane(static_cast<int>((u - before) % f.tiles));
-    const int t_count = static_cast<int>(min(static_cast<int64_t>(f.tiles - t_first), u_end - u));
-    const int head = segment % c.kv_heads, chunk = segment / c.kv_heads;
+    const uint32_t a_segment = static_cast<uint32_t>(((f.tiles - 1) >> a.shift) + 1);  // units
+    const int segment = __builtin_amdgcn_readfirstlane(static_cast<int>((u - before) / a_segment));
+    const uint32_t in_segment = u - before - segment * a_segment, u_count = min(a_segment - in_segment, u_end - u);
+    const int t_first = static_cast<int>(in_segment << a.shift), t_count = min(f.tiles - t_first, static_cast<int>(u_count << a.shift));
+    const int chunk = segment / c.kv_heads, head = segment - chunk * c.kv_heads;
 
     // ---- this lane's query row, and what the segment's rows see.
     int token, query_head, first_token, last_token;
@@ -133,15 +170,15 @@ __global__ __launch_bounds__(kFewThreads, 2) void FewKernel(const PagedAttendArg
     if constexpr (LISTS) {
       const int a_token = (a.group + kRows - 1) / kRows;
       first_token = last_token = token = chunk / a_token;
-      query_head = kRows * (chunk % a_token) + column;
+      query_head = kRows * (chunk - token * a_token) + column;
       real = query_head < a.group;
     } else {
       const int row = kRows * chunk + column;
-      token = row / a.group;
-      query_head = row % a.group;
+      token = static_cast<int>(PagedDivide(row, a.group_magic));
+      query_head = row - token * a.group;
       real = row < f.q.n * a.group;
-      first_token = kRows * chunk / a.group;
-      last_token = min((kRows * chunk + kRows - 1) / a.group, f.q.n - 1);
+      first_token = static_cast<int>(PagedDivide(kRows * chunk, a.group_magic));
+      last_token = min(static_cast<int>(PagedDivide(kRows * chunk + kRows - 1, a.group_magic)), f.q.n - 1);
     }
     const int base_position = f.q.length - f.q.n;  // of the request's first new token
     const int position = base_position + token;
@@ -150,177 +187,168 @@ __global__ __launch_bounds__(kFewThreads, 2) void FewKernel(const PagedAttendArg
     const int all_from = max(base_position + last_token - window + 1, 0), all_to = base_position + first_token + 1;  // seen by every row
     const int any_from = max(base_position + first_token - window + 1, 0), any_to = base_position + last_token + 1;  // seen by any
 
+    // The row's loads before all others: its digits are made while the first tile is on its way.
+    QueryPart<TYPE, 2 * kSteps> row;
+    {
+      const int64_t from = (f.q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * group_of;
+#pragma unroll
+      for (int i = 0; i < 2 * kSteps; ++i) row.Load(op.q, i, from + 64 * (i / 2) + 8 * (i % 2));
+    }
     I32x4 digits[kDig][kSteps];
     float unit;  // a digit product's worth in log2 units, but for K's scale
-    {
-      float x[kSteps][16];
-      const int64_t from = (f.q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride;
-      float most = 0.0f;
-      bool finite = true;
+    const auto query = [&]() {
+      const QueryUnit made = UnitOf<TYPE>(AcrossGroupsMost(row.MostBits()));
+      const float inverse = real ? made.inverse : 0.0f;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int i = 0; i < 2 * kSteps; ++i) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float v[8];
-          LoadEight<TYPE>(op.q, from + 64 * s + 16 * group_of + 8 * half, v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[s][8 * half + e] = v[e];
-            finite = finite && fabsf(v[e]) <= 3.402823466e38f;
-            most = fmaxf(most, fabsf(v[e]));
-          }
-        }
-      }
-      most = AcrossGroupsMax(most);
-      const float bad = AcrossGroupsMax(finite ? 0.0f : 1.0f);
-      // (A row of zeros, or of magnitudes whose reciprocal is none, is zeros; one with an infinity or a NaN has no logits.)
-      const bool small = !(most > 0x1p-100f);
-      const float inverse = small ? 0.0f : kDigitMax<TYPE> / most;
-      unit = bad > 0.0f ? __builtin_nanf("") : small ? 0.0f : most / kDigitMax<TYPE>;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
+          float v[4];
+          row.Four(i, half, v);
           uint32_t packed[kDig];
+          PackDigits<kDig>(v, inverse, packed);
 #pragma unroll
-          for (int k = 0; k < kDig; ++k) packed[k] = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            int digit[kDig];
-            SplitDigits<kDig>(bad > 0.0f || !real ? 0 : static_cast<int>(rintf(x[s][4 * w + e] * inverse)), digit);
-#pragma unroll
-            for (int k = 0; k < kDig; ++k) packed[k] |= static_cast<uint32_t>(digit[k] & 0xFF) << (8 * e);
-          }
-#pragma unroll
-          for (int k = 0; k < kDig; ++k) digits[k][s][w] = static_cast<int>(packed[k]);
+          for (int k = 0; k < kDig; ++k) digits[k][i / 2][2 * (i % 2) + half] = static_cast<int>(packed[k]);
         }
       }
-      unit *= op.softcap != 0.0f ? op.scale : op.scale * kLog2E;
-    }
+      unit = made.unit * (op.softcap != 0.0f ? op.scale : op.scale * kLog2E);
+    };
     const float cap_inverse = op.softcap != 0.0f ? 1.0f / op.softcap : 0.0f;
 
-    // ---- the places of a tile's tokens.
     const int32_t* const table = op.table + r * op.table_stride;
     const int32_t* const list =
         LISTS ? op.lists + (static_cast<int64_t>(f.q.start + token) * c.kv_heads + head) * op.list_pages : nullptr;
+    // ---- this wave's tiles, four apart.
+    int tile_from = t_first + f.first_tile + wave, tile_to = t_first + t_count + f.first_tile;
+    if constexpr (!LISTS) {  // (not those that no row of this chunk sees)
+      while (tile_from < tile_to && (tile_from + 1) * kTileTokens <= any_from) tile_from += kFewWaves;
+      tile_to = min(tile_to, max(any_to + kTileTokens - 1, 0) / kTileTokens);
+    }
+    const int tiles = tile_from < tile_to ? (tile_to - tile_from + kFewWaves - 1) / kFewWaves : 0;
+    // ---- the places of a tile's tokens.
     const int p16 = c.page / 16;
-    const auto place_of = [&](int tile) {
-      Place at;
-      const int n16 = 4 * tile + group_of;
-      int entry = static_cast<int>(PagedDivide(n16, a.page_magic));
-      at.offset = 16 * (n16 - entry * p16);
-      if constexpr (LISTS) entry = entry < op.list_pages ? list[entry] : -1;
-      at.page = -1;
-      at.position = 0;
-      if (entry >= 0 && entry < op.table_width) {
-        at.position = entry * c.page + at.offset;
-        if (at.position < f.q.length) at.page = table[entry];
+    // What a place is read from is asked for a tile or two before it is looked at (a look waits for all loads before it, the
+    // tiles' among them): the list's entry, then the table's, then the place.
+    const auto entry_of = [&](int i) {
+      const int n16 = 4 * (tile_from + i * kFewWaves) + group_of;
+      Entry e;
+      e.entry = static_cast<int>(PagedDivide(n16, a.page_magic));
+      e.offset = 16 * (n16 - e.entry * p16);
+      if constexpr (LISTS) {
+        e.there = e.entry < op.list_pages;
+        e.entry = list[min(e.entry, op.list_pages - 1)];
+      } else {
+        e.there = true;
       }
-      if (at.page >= c.pages) at.page = -1;
+      return e;
+    };
+    const auto page_of = [&](const Entry& e) {
+      Place at;
+      at.position = e.entry * c.page + e.offset;
+      at.there = e.there && e.entry >= 0 && e.entry < op.table_width && at.position < f.q.length;
+      at.offset = e.offset;
+      at.page = table[at.there ? e.entry : 0];
       return at;
     };
-    const int tile_end = t_first + t_count + f.first_tile;
-    int tile = t_first + f.first_tile + wave;
-    int stop = tile_end;
-    if constexpr (!LISTS) {  // tiles that no row of this chunk sees
-      while (tile < stop && (tile + 1) * kTileTokens <= any_from) tile += kFewWaves;
-      stop = min(stop, max(any_to + kTileTokens - 1, 0) / kTileTokens);
-    }
-
+    const auto check = [&](Place& at) {
+      if (!at.there || at.page < 0 || at.page >= c.pages) at.page = -1;
+    };
+    // ---- the loads of a tile, to the wave's part of LDS: no registers wait for memory, so a whole tile is on its way under
+    // another's work. A load takes 1024 bytes, in memory's order but for the pieces of 16 bytes of a row, which KPiece and VPiece turn.
+    const int64_t page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
+    const uint8_t* const k_base = static_cast<const uint8_t*>(c.k) + static_cast<int64_t>(head) * c.page * D;
+    const uint8_t* const v_base = static_cast<const uint8_t*>(c.v) + static_cast<int64_t>(head) * c.page * D;
+    constexpr int kPieces = D / 16, kLoadTokens = kWave / kPieces;  // 16-byte pieces of a K row, rows a load
+    const int v_piece = VPiece(lane >> 2, lane & 3);
+    const auto load = [&](const Place& at, float* ks, float* vs) {
+#pragma unroll
+      for (int j = 0; j < kTileTokens / kLoadTokens; ++j) {
+        // (A load's tokens are of one group of 16, so of one page: the same for every lane.)
+        constexpr int kLoads = 16 / kLoadTokens;
+        const int group = j / kLoads, in_group = j % kLoads * kLoadTokens;
+        const int page = max(__builtin_amdgcn_readlane(at.page, 16 * group), 0), offset = __builtin_amdgcn_readlane(at.offset, 16 * group);
+        const int token = kLoadTokens * j + lane / kPieces;
+        ToLds(k_base + page * page_bytes + (offset + in_group) * D + static_cast<uint32_t>(lane / kPieces * D + 16 * KPiece<D>(token, lane % kPieces)),
+              landing + 1024 * j);
+      }
+      const int page = max(__shfl(at.page, 16 * v_piece), 0), offset = __shfl(at.offset, 16 * v_piece);
+      const uint8_t* from = v_base + page * page_bytes + (lane >> 2) * c.page + offset;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) ToLds(from + 16 * b * c.page, landing + kTileTokens * D + 1024 * b);
+      const int64_t i = static_cast<int64_t>(max(at.page, 0)) * c.kv_heads + head;
+      *ks = c.k_scale[i], *vs = c.v_scale[i];
+    };
+    // What has landed, into registers.
+    struct Landed {
+      I32x4 k[kProducts][kSteps];
+      U32x4 v[kBlocks];
+    };
+    const auto take = [&](Landed& in) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int t = 0; t < kProducts; ++t) {
+        const int token = 16 * (column >> 2) + 4 * t + (column & 3);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) in.k[t][s] = *reinterpret_cast<const I32x4*>(landing + token * D + 16 * KPiece<D>(token, 4 * s + group_of));
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const int d = 16 * b + column;
+        in.v[b] = *reinterpret_cast<const U32x4*>(landing + kTileTokens * D + d * kTileTokens + 16 * VPiece(d, group_of));
+      }
+      // (The place is filled again at once: everything has to have left it.)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
     float top = -INFINITY, sum = 0.0f;
     F32x4 out[kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) out[b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // ---- the loads of a tile: K by (token row, inner step), V by block of dimensions, the scales of the lane's page.
-    I32x4 k[4][kSteps];
-    U32x4 v[kBlocks];
-    float ks = 0.0f, vs = 0.0f;
-    const int64_t page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
-    const uint8_t* const k_base = static_cast<const uint8_t*>(c.k) + static_cast<int64_t>(head) * c.page * D + 16 * group_of + (column & 3) * D;
-    const uint8_t* const v_base = static_cast<const uint8_t*>(c.v) + static_cast<int64_t>(head) * c.page * D + column * c.page;
-    const auto load_k = [&](const Place& at) {
-      // K's row `column` of product t is token 16 (column / 4) + 4 t + column % 4: of another group's page.
-      const int page = max(__shfl(at.page, (column >> 2) * 16), 0), offset = __shfl(at.offset, (column >> 2) * 16);
-      const uint8_t* from = k_base + page * page_bytes + offset * D;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) k[t][s] = *reinterpret_cast<const I32x4*>(from + 4 * t * D + 64 * s);
-      }
-    };
-    const auto load_v = [&](const Place& at) {
-      const uint8_t* from = v_base + max(at.page, 0) * page_bytes + at.offset;
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) v[b] = *reinterpret_cast<const U32x4*>(from + 16 * b * c.page);
-    };
-    const auto load_scales = [&](const Place& at, float* to_k, float* to_v) {
-      const int64_t i = static_cast<int64_t>(max(at.page, 0)) * c.kv_heads + head;
-      *to_k = c.k_scale[i], *to_v = c.v_scale[i];
-    };
-    Place here = {-1, 0, 0}, next = {-1, 0, 0};
-    if (tile < stop) {
-      here = place_of(tile);
-      load_k(here);
-      load_scales(here, &ks, &vs);
-      load_v(here);
-      if (tile + kFewWaves < stop) next = place_of(tile + kFewWaves);
-    }
-    for (; tile < stop; tile += kFewWaves) {
-      const bool more = tile + kFewWaves < stop;
-      float next_ks = 0.0f, next_vs = 0.0f;
+    const auto attend = [&](const Landed& in, const Place& at, float ks, float vs) {
       // ---- S^T = K Q^T
-      I32x4 dots[kDig][4];
+      float s[kMine];
+      {
+        I32x4 dots[kDig][kProducts];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < kProducts; ++t) {
 #pragma unroll
-        for (int d = 0; d < kDig; ++d) {
-          I32x4 acc = {0, 0, 0, 0};
+          for (int d = 0; d < kDig; ++d) {
+            I32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][s], digits[d][s], acc, 0, 0, 0);
-          dots[d][t] = acc;
+            for (int x = 0; x < kSteps; ++x) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(in.k[t][x], digits[d][x], acc, 0, 0, 0);
+            dots[d][t] = acc;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) s[i] = JoinDigits<kDig>(dots[0][i / 4][i % 4], kDig == 3 ? dots[1][i / 4][i % 4] : 0, dots[kDig - 1][i / 4][i % 4]);
       }
-      if (more) load_k(next), load_scales(next, &next_ks, &next_vs);
-      Place after = {-1, 0, 0};
-      if (tile + 2 * kFewWaves < stop) after = place_of(tile + 2 * kFewWaves);
       // ---- the tile's softmax
-      float s[16];
       const float worth = unit * ks;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = JoinDigits<kDig>(dots[0][i / 4][i % 4], kDig == 3 ? dots[1][i / 4][i % 4] : 0, dots[kDig - 1][i / 4][i % 4]);
-      }
+      for (int i = 0; i < kMine; ++i) s[i] *= worth;
       if (op.softcap != 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = Capped<TYPE>(s[i] * worth, op.softcap, cap_inverse) * kLog2E;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] *= worth;
+        for (int i = 0; i < kMine; ++i) s[i] = Capped<TYPE>(s[i], op.softcap, cap_inverse) * kLog2E;
       }
-      bool whole = __all(here.page >= 0);
-      if constexpr (LISTS) {
-        whole = whole && __all(here.position + 16 <= all_to && here.position >= all_from);
-      } else {
-        whole = whole && (tile + 1) * kTileTokens <= all_to && tile * kTileTokens >= all_from;
-      }
+      const bool whole = __all(at.page >= 0 && at.position + kMine <= all_to && at.position >= all_from);
       uint32_t seen = 0xFFFFu;
       if (!whole) {
         seen = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int p = here.position + i;
-          const bool sees = here.page >= 0 && p >= see_from && p < see_to;
+        for (int i = 0; i < kMine; ++i) {
+          const int p = at.position + i;
+          const bool sees = at.page >= 0 && p >= see_from && p < see_to;
           seen |= sees ? 1u << i : 0u;
           s[i] = sees ? s[i] : -INFINITY;
         }
-        if (here.page < 0) vs = 0.0f;
+        if (at.page < 0) vs = 0.0f;
       }
       float peak = s[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) peak = fmaxf(peak, s[i]);
+      for (int i = 1; i < kMine; ++i) peak = fmaxf(peak, s[i]);
       peak = AcrossGroupsMax(peak + ScaleLog(vs));
-      if (__any(peak > top)) {
+      if (__any(peak > top + kSlack)) {
         const float higher = fmaxf(top, peak);
         const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
         top = higher;
@@ -329,40 +357,65 @@ __global__ __launch_bounds__(kFewThreads, 2) void FewKernel(const PagedAttendArg
         for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
       }
       const float from = top == -INFINITY ? 0.0f : top;
-      float p[16];
+      float p[kMine];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < kMine; ++i) {
         p[i] = __builtin_amdgcn_exp2f(s[i] - from);
         sum += p[i];
         p[i] *= vs;
       }
       if (!whole) {  // (a hidden token's weight is zero whatever its page's scale is)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = (seen >> i) & 1u ? p[i] : 0.0f;
+        for (int i = 0; i < kMine; ++i) p[i] = (seen >> i) & 1u ? p[i] : 0.0f;
       }
       F16x8 w[2], w_low[2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < kMine; ++i) {
         w[i / 8][i % 8] = static_cast<_Float16>(p[i]);
         if constexpr (kDig == 3) w_low[i / 8][i % 8] = static_cast<_Float16>(p[i] - static_cast<float>(w[i / 8][i % 8]));
       }
       // ---- O^T += V^T P^T
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        const F16x8 v0 = EightCodes(v[b][0], v[b][1]), v1 = EightCodes(v[b][2], v[b][3]);
-        out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[0], out[b], 0, 0, 0);
-        out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[1], out[b], 0, 0, 0);
-        if constexpr (kDig == 3) {
-          out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w_low[0], out[b], 0, 0, 0);
-          out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w_low[1], out[b], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const F16x8 v = EightCodes(in.v[b][2 * x], in.v[b][2 * x + 1]);
+          out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[x], out[b], 0, 0, 0);
+          if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w_low[x], out[b], 0, 0, 0);
         }
       }
-      if (more) load_v(next);
-      here = next, next = after, ks = next_ks, vs = next_vs;
+    };
+
+    // ---- the tiles, the next one's loads in flight under each.
+    Place here = {}, next = {};
+    Entry after = {};
+    float ks = 0.0f, vs = 0.0f;
+    if (tiles > 0) {
+      here = page_of(entry_of(0));
+      check(here);
+      load(here, &ks, &vs);
+      if (tiles > 1) next = page_of(entry_of(1));
+      if (tiles > 2) after = entry_of(2);
+    }
+    query();
+    for (int i = 0; i < tiles; ++i) {
+      Landed in;
+      take(in);
+      const Place now = here;
+      const float now_ks = ks, now_vs = vs;
+      if (i + 1 < tiles) {
+        here = next;
+        check(here);
+        load(here, &ks, &vs);
+        if (i + 2 < tiles) next = page_of(after);
+        if (i + 3 < tiles) after = entry_of(i + 3);
+      }
+      attend(in, now, now_ks, now_vs);
     }
     sum = AcrossGroupsSum(sum);
 
-    // ---- the waves' results meet.
+    // ---- the waves' results meet, where the tiles landed.
+    __syncthreads();
     if (group_of == 0) tops[wave][column] = top, sums[wave][column] = sum;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
@@ -389,7 +442,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void FewKernel(const PagedAttendArg
           to_token = token, to_head = kRows * (chunk % ((a.group + kRows - 1) / kRows)) + row, is_real = to_head < a.group;
         } else {
           const int at = kRows * chunk + row;
-          to_token = at / a.group, to_head = at % a.group, is_real = at < f.q.n * a.group;
+          to_token = static_cast<int>(PagedDivide(at, a.group_magic)), to_head = at - to_token * a.group, is_real = at < f.q.n * a.group;
         }
         if (is_real) {
           const int h = head * a.group + to_head;
@@ -405,24 +458,85 @@ __global__ __launch_bounds__(kFewThreads, 2) void FewKernel(const PagedAttendArg
         for (int e = 0; e < 4; ++e) to[2 + d + e] = value[e];
       }
     }
-    if (begins && !ends) part = I32x4{static_cast<int>((before + static_cast<int64_t>(segment + 1) * f.tiles - 1) / per), r, segment, 0};
+    if (begins && !ends) part = I32x4{static_cast<int>((before + (segment + 1) * a_segment - 1) / per), f.q.start, segment, f.q.n};
     __syncthreads();
-    u += t_count;
+    u += u_count;
   }
   if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * blockIdx.x) = part;
 }
 
-// grid (workgroups of the first launch, 4): the parts of the segment that begins in workgroup x and ends in another, a
-// wave a row.
+// Parts p from 0 to `count` - 1 of a row (top, sum, D values at part_of(p)) as one, the waves taking
+// every fourth; all of a wave's next eight are asked for at once, since such a launch is a chain of round trips. Every thread
+// of the first wave gets D / 64 of the row's values, times one over its sum.
+template <int D, class F>
+__device__ __forceinline__ bool JoinParts(int count, const float* sink, F&& part_of, float (&value)[D / kWave]) {
+  constexpr int kPer = D / kWave, kBatch = 8;
+  __shared__ float tops[kFewWaves], totals[kFewWaves], values[kFewWaves][D];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  float high = -INFINITY, all = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
+  for (int p0 = wave; p0 < count; p0 += kFewWaves * kBatch) {
+    float top[kBatch], total[kBatch], v[kBatch][kPer];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float* from = part_of(min(p0 + kFewWaves * i, count - 1));
+      top[i] = from[0], total[i] = from[1];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[i][e] = from[2 + kPer * lane + e];
+    }
+    float higher = high;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) higher = fmaxf(higher, top[i]);  // (a part asked for twice changes no maximum)
+    const float keep = high == -INFINITY ? (higher == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(high - higher);
+    all *= keep;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) value[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      // (A row without a logit has a top of -infinity and sums of zero, or no numbers, which stay.)
+      float weight = top[i] == -INFINITY ? (higher == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top[i] - higher);
+      if (p0 + kFewWaves * i < count) {
+        all += total[i] * weight;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) value[e] += v[i][e] * weight;
+      }
+    }
+    high = higher;
+  }
+  if (lane == 0) tops[wave] = high, totals[wave] = all;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) values[wave][kPer * lane + e] = value[e];
+  __syncthreads();
+  if (wave != 0) return false;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) top = fmaxf(top, tops[w]);
+  all = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) {
+    const float weight = tops[w] == -INFINITY ? (top == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(tops[w] - top);
+    all += totals[w] * weight;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) value[e] += values[w][kPer * lane + e] * weight;
+  }
+  if (sink != nullptr) all += __builtin_amdgcn_exp2f(fmaf(*sink, kLog2E, -(top == -INFINITY ? 0.0f : top)));
+  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) value[e] *= inverse;
+  return true;
+}
+
+// grid (workgroups of the first launch, rows of a segment): the parts of the segment that begins in workgroup x and ends in another.
 template <int TYPE, int D, bool LISTS>
 __global__ __launch_bounds__(kFewThreads) void FewJoinKernel(const PagedAttendArgs a) {
   constexpr int kPer = D / kWave;
   const llmp_paged_attend& op = a.op;
   const I32x4 part = *reinterpret_cast<const I32x4*>(a.parts + 4 * blockIdx.x);
   if (part.x < 0) return;
-  const int lane = threadIdx.x & (kWave - 1), row = 4 * blockIdx.y + threadIdx.x / kWave;
-  const int r = part.y, head = part.z % op.cache.kv_heads, chunk = part.z / op.cache.kv_heads;
-  const PagedRequest q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
+  const int row = blockIdx.y, first = blockIdx.x, chunk = part.z / op.cache.kv_heads, head = part.z - chunk * op.cache.kv_heads;
   int token, query_head;
   bool real;
   if constexpr (LISTS) {
@@ -430,61 +544,35 @@ __global__ __launch_bounds__(kFewThreads) void FewJoinKernel(const PagedAttendAr
     token = chunk / a_token, query_head = kRows * (chunk % a_token) + row, real = query_head < a.group;
   } else {
     const int at = kRows * chunk + row;
-    token = at / a.group, query_head = at % a.group, real = at < q.n * a.group;
+    token = static_cast<int>(PagedDivide(at, a.group_magic)), query_head = at - token * a.group, real = at < part.w * a.group;
   }
   if (!real) return;
-  constexpr int64_t kSlot = kRows * (D + 2);
-  const int first = blockIdx.x, last = part.x;
-  const auto slot_of = [&](int w) { return a.partial + (2 * static_cast<int64_t>(w) + (w == first ? 1 : 0)) * kSlot + row * (D + 2); };
-  float high = -INFINITY;
-  for (int w = first + lane; w <= last; w += kWave) high = fmaxf(high, slot_of(w)[0]);
-#pragma unroll
-  for (int step = 1; step < kWave; step <<= 1) high = fmaxf(high, __shfl_xor(high, step));
-  float all = 0.0f, value[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
-#pragma unroll 8
-  for (int w = first; w <= last; ++w) {
-    const float* from = slot_of(w);
-    const float top = from[0];
-    const float keep = top == -INFINITY ? (high == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top - high);
-    all += from[1] * keep;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) value[e] += from[2 + kPer * lane + e] * keep;
-  }
   const int h = head * a.group + query_head;
-  if (op.sinks != nullptr) all += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(high == -INFINITY ? 0.0f : high)));
-  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
-  const int64_t to = (q.start + token) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
+  float value[kPer];
+  const bool mine = JoinParts<D>(part.x - first + 1, op.sinks != nullptr ? op.sinks + h : nullptr,
+                                 [&](int p) { return a.partial + ((2 * static_cast<int64_t>(first + p) + (p == 0 ? 1 : 0)) * kRows + row) * (D + 2); }, value);
+  if (!mine) return;
+  const int64_t to = (part.y + token) * op.out_token_stride + h * op.out_head_stride + kPer * (threadIdx.x & (kWave - 1));
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e] * inverse);
+  for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e]);
 }
 
-// Workgroups of the few rows' launch: two a compute unit (their registers' limit), a wave of each a SIMD.
-int FewGroups(int cus) { return 2 * (cus > 0 ? cus : 256); }
+int FewGroups(int head_dim, int cus) { return FewAUnit(head_dim) * (cus > 0 ? cus : 256); }
 
 size_t PartBytes(int groups) { return static_cast<size_t>(groups) * 4 * sizeof(int32_t); }
 size_t FewScratch(int head_dim, int cus) {
-  const int groups = FewGroups(cus);
+  const int groups = FewGroups(head_dim, cus);
   return PartBytes(groups) + 2 * static_cast<size_t>(groups) * kRows * (head_dim + 2) * sizeof(float);
-}
-
-// Requests of more rows than this are the many rows' form's, where the call has any.
-constexpr int kFewRows = 64;
-bool HasMany(const llmp_paged_attend& op) {
-  return op.lists == nullptr && static_cast<int64_t>(op.most_tokens < op.tokens ? op.most_tokens : op.tokens) * (op.heads / op.cache.kv_heads) > kFewRows;
-}
-size_t AttendScratch(const llmp_paged_attend& op, int cus) {
-  return FewScratch(op.cache.head_dim, cus) + (HasMany(op) ? PagedManyScratch(op, cus) : 0);
 }
 
 template <int TYPE, int D, bool LISTS>
 void LaunchFew(const PagedAttendArgs& args, int groups, hipStream_t stream) {
-  constexpr int kLds = kFewWaves * kRows * (D + 4) * static_cast<int>(sizeof(float));
+  constexpr int kLds = FewLds(D);
   static bool sized = false;
   if (kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&FewKernel<TYPE, D, LISTS>), kLds, &sized)) return;
   hipLaunchKernelGGL((FewKernel<TYPE, D, LISTS>), dim3(groups), dim3(kFewThreads), kLds, stream, args);
-  hipLaunchKernelGGL((FewJoinKernel<TYPE, D, LISTS>), dim3(groups, kRows / 4), dim3(kFewThreads), 0, stream, args);
+  const int64_t rows = static_cast<int64_t>(LISTS ? 1 : args.op.most_tokens) * args.group;  // at most, of a segment
+  hipLaunchKernelGGL((FewJoinKernel<TYPE, D, LISTS>), dim3(groups, rows < kRows ? static_cast<unsigned>(rows) : kRows), dim3(kFewThreads), 0, stream, args);
 }
 
 template <int TYPE, int D>
@@ -502,6 +590,26 @@ void LaunchFewOf(const PagedAttendArgs& args, int groups, hipStream_t stream) {
   if (args.op.cache.head_dim == 256) LaunchFewFor<TYPE, 256>(args, groups, stream);
 }
 
+// Requests of more rows than this are the many rows' form's, where the call has any.
+constexpr int kFewRows = 64;
+constexpr int kMostGroup = 1024, kMostFewRows = 1 << 20;  // (PagedDivide's range together)
+// Tiles a unit of the line, as a power of two: a call's units stay below 2^31.
+int FewShift(const llmp_paged_attend& op) {
+  const int64_t group = op.heads / op.cache.kv_heads, chunks_a_token = (group + kRows - 1) / kRows;
+  const int64_t segments = op.tokens * chunks_a_token * op.cache.kv_heads;
+  const int64_t tokens = op.lists != nullptr ? static_cast<int64_t>(op.list_pages) * op.cache.page : static_cast<int64_t>(op.table_width) * op.cache.page;
+  const int64_t tiles = tokens / kTileTokens + 1;
+  int shift = 0;
+  while (segments * ((tiles >> shift) + 1) >= 1ll << 31 && shift < 24) ++shift;
+  return shift;
+}
+bool HasMany(const llmp_paged_attend& op) {
+  return op.lists == nullptr && static_cast<int64_t>(op.most_tokens < op.tokens ? op.most_tokens : op.tokens) * (op.heads / op.cache.kv_heads) > kFewRows;
+}
+size_t AttendScratch(const llmp_paged_attend& op, int cus) {
+  return FewScratch(op.cache.head_dim, cus) + (HasMany(op) ? PagedManyScratch(op, cus) : 0);
+}
+
 int CheckAttend(const llmp_paged_attend* op) {
   if (op == nullptr) return Refuse(1, "paged_attend: null operands");
   if (const int bad = CheckPagedCache("paged_attend", op->cache, false); bad != 0) return bad;
@@ -510,8 +618,9 @@ int CheckAttend(const llmp_paged_attend* op) {
   if (op->requests < 1 || op->requests > 1 << 24 || op->tokens < 1 || op->most_tokens < 1 || op->table_width < 1)
     return Refuse(1, "paged_attend: 1 to 2^24 requests, at least one token and one page a table row (%d, %d, %d, %d)", op->requests, op->tokens,
                   op->most_tokens, op->table_width);
-  if (op->heads < 1 || op->heads % op->cache.kv_heads != 0 || static_cast<int64_t>(op->heads) * op->tokens > INT_MAX)
-    return Refuse(1, "paged_attend: a whole number of query heads a KV head (%d, %d), at most 2^31 of them in all tokens", op->heads, op->cache.kv_heads);
+  if (op->heads < 1 || op->heads % op->cache.kv_heads != 0 || static_cast<int64_t>(op->heads) * op->tokens > INT_MAX / 2)
+    return Refuse(1, "paged_attend: a whole number of query heads a KV head (%d, %d), at most 2^30 of them in all tokens", op->heads, op->cache.kv_heads);
+  if (op->heads / op->cache.kv_heads > kMostGroup) return Refuse(1, "paged_attend: at most %d query heads a KV head, not %d", kMostGroup, op->heads / op->cache.kv_heads);
   if (op->lengths == nullptr || op->starts == nullptr || op->table == nullptr) return Refuse(1, "paged_attend: null operand");
   if ((reinterpret_cast<uintptr_t>(op->lengths) | reinterpret_cast<uintptr_t>(op->starts) | reinterpret_cast<uintptr_t>(op->table) |
        reinterpret_cast<uintptr_t>(op->lists) | reinterpret_cast<uintptr_t>(op->sinks)) % 4 != 0)
@@ -544,15 +653,17 @@ extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch,
   BeginLaunches();
   PagedAttendArgs args;
   args.op = *op;
-  const int groups = FewGroups(cus);
+  const int groups = FewGroups(op->cache.head_dim, cus);
   args.parts = static_cast<int32_t*>(scratch);
   args.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + PartBytes(groups));
   const uint32_t p16 = static_cast<uint32_t>(op->cache.page / 16);
   args.page_magic = p16 == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / p16 + 1);
   args.group = op->heads / op->cache.kv_heads;
+  args.group_magic = args.group == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / args.group + 1);
   args.most_length = op->table_width * op->cache.page;
   const bool many = HasMany(*op);
-  args.few_rows = many ? kFewRows : INT_MAX;
+  args.few_rows = many ? kFewRows : kMostFewRows;
+  args.shift = FewShift(*op);
   const hipStream_t on = static_cast<hipStream_t>(stream);
   if (many) PagedManyRows(args, static_cast<uint8_t*>(scratch) + FewScratch(op->cache.head_dim, cus), cus, on);
   if (many && op->requests == 1 && op->most_tokens == op->tokens) return LaunchStatus("paged_attend");  // the one request has been answered

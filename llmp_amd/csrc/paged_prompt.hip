@@ -3,7 +3,7 @@
 // What bounds it is the vector units: per logit about seven operations and an exponential, against the matrix instructions' 4 D
 // operations; the cache's bytes come from L2 (a head's pages are read by every workgroup of its rows). A workgroup of four
 // waves takes 128 rows of one KV head, (token, head) pairs in order, so that a group's query heads share the tile; a
-// wave has 32 rows. A tile of 64 tokens goes through LDS, double-buffered, its loads in flight under the previous tile's
+// wave has 32 rows (16 at head size 256). A tile of 64 tokens goes through LDS, double-buffered, its loads in flight under the previous tile's
 // work: K as its codes, V turned into F16 once for all the waves. Products as in the few rows' form, 32 x 32:
 //   S^T = K Q^T by v_mfma_i32_32x32x32_i8. Row 8a + 4h + b of a product is token 16h + 4a + b of its 32, so that a lane (half h) ends
 //   with 16 consecutive tokens of one query row, all of one page;
@@ -15,17 +15,16 @@
 // each is one workgroup's, longest first, dealt to the compute units there and back so that a unit's two workgroups
 // together have about the same; with fewer, all segments' tiles lie on one line that the workgroups share evenly, and a third
 // launch joins the parts.
+#include <type_traits>
+
 #include "paged_attend.h"
 
 namespace llmp_hip {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
-constexpr int kWaveRows = 32;
-constexpr int kManyRows = kWaves * kWaveRows;
+constexpr int kManyRows = 128;  // of a workgroup
+constexpr int kJoinThreads = 256;
 constexpr int kListThreads = 1024;
-constexpr float kSlack = 8.0f;   // how far the running maximum may lag, in log2
 constexpr int kBuckets = 1024;  // of the segments' lengths, for their order
 
 // The list: a header, the pairs, the tiles before each pair (times KV heads), the pairs' order by length.
@@ -139,26 +138,46 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
 template <int PIECES>
 __device__ __forceinline__ int Turn(int row, int piece) { return piece ^ ((row / (16 / PIECES)) & (PIECES - 1)); }
 
+// By head size: four waves of 32 rows, or at 256, where 32 rows' values alone would be half a lane's registers and the
+// compiler then carries them to and fro, eight of 16 with 16 x 16 products (twice the reads of LDS).
 template <int D>
 struct ManyGeo {
+  static constexpr int kWaveRows = D == 256 ? 16 : 32;
+  static constexpr int kWaves = kManyRows / kWaveRows, kThreads = kWaves * kWave;
+  static constexpr int kInner = 1024 / kWaveRows;              // K's dimensions a product: 32, 64
+  static constexpr int kTurns = kWaveRows == 32 ? 2 : 1;       // a tile's tokens by 32 or all at once: 16 of them a lane either way
   static constexpr int kKBytes = kTileTokens * D;
   static constexpr int kVBytes = D * kTileTokens * 2;
   static constexpr int kBuffer = kKBytes + kVBytes;
   static constexpr int kLds = 2 * kBuffer + 2 * 4 * 16;  // and the four 16-token groups' scales
-  static constexpr int kAUnit = D == 256 ? 1 : 2;        // workgroups a compute unit: 512 or 256 registers a lane
+  static constexpr int kAUnit = D == 256 ? 1 : 2;        // workgroups a compute unit
+  // K's row of a token in LDS, and where a piece of it lies: rows in the products' order, or as KPiece has them.
+  static __device__ __forceinline__ int KRow(int t) {
+    if constexpr (kWaveRows == 16) return t;
+    const int x = t & 31;
+    return (t & 32) + 8 * ((x >> 2) & 3) + 4 * (x >> 4) + (x & 3);
+  }
+  static __device__ __forceinline__ int KSlot(int row, int piece) {
+    if constexpr (kWaveRows == 16) return KPiece<D>(row, piece);
+    return Turn<D / 16>(row, piece);
+  }
 };
 
 template <int TYPE, int D, bool CAPPED>
-__global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const ManyArgs m) {
+__global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const ManyArgs m) {
   using G = ManyGeo<D>;
   constexpr int kDig = kDigits<TYPE>;
-  constexpr int kSteps = D / 32, kBlocks = D / 32, kPieces = D / 16, kLoads = D / 64;
+  constexpr int kWaveRows = G::kWaveRows, kThreads = G::kThreads, kInner = G::kInner;
+  constexpr int kSteps = D / kInner, kBlocks = D / kWaveRows, kPieces = D / 16, kLoads = 4 * D / kThreads;
+  typedef std::conditional_t<kWaveRows == 32, F32x16, F32x4> Values;  // a lane's of a block of dimensions
+  typedef std::conditional_t<kWaveRows == 32, I32x16, I32x4> Dots;
+  constexpr int kValues = kWaveRows * kWaveRows / kWave;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const PagedAttendArgs& a = m.a;
   const llmp_paged_attend& op = a.op;
   const llmp_paged_cache& c = op.cache;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int half = lane >> 5, column = lane & 31;
+  const int half = lane / kWaveRows, column = lane % kWaveRows;  // (`half` a quarter where rows are 16)
   const int groups = gridDim.x, w = blockIdx.x;
   const ListHeader header = *m.list.header;
   F32x4* const group_scales = reinterpret_cast<F32x4*>(lds + 2 * G::kBuffer);  // [buffer][group]: K's and V's scale, V's log2 and reciprocal
@@ -238,47 +257,26 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
     I32x4 digits[kDig][kSteps];
     float unit;
     {
-      const int64_t from = (q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride;
-      float most = 0.0f;
-      bool finite = true;
+      QueryPart<TYPE, 2 * kSteps> part_of_row;
+      const int64_t from = (q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * half;
 #pragma unroll
-      for (int s = 0; s < 2 * kSteps; ++s) {
-        float v[8];
-        LoadEight<TYPE>(op.q, from + 32 * (s / 2) + 16 * half + 8 * (s % 2), v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          finite = finite && fabsf(v[e]) <= 3.402823466e38f;
-          most = fmaxf(most, fabsf(v[e]));
-        }
-      }
-      most = AcrossHalvesMax(most);
-      const float bad = AcrossHalvesMax(finite ? 0.0f : 1.0f);
-      const bool small = !(most > 0x1p-100f);
-      const float inverse = small ? 0.0f : kDigitMax<TYPE> / most;
-      unit = bad > 0.0f ? __builtin_nanf("") : small ? 0.0f : most / kDigitMax<TYPE>;
+      for (int i = 0; i < 2 * kSteps; ++i) part_of_row.Load(op.q, i, from + kInner * (i / 2) + 8 * (i % 2));
+      const QueryUnit made = UnitOf<TYPE>(Across<kWaveRows>(part_of_row.MostBits()));
       // (A negative scale goes into the digits: the units stay positive, so the largest product is the largest logit.)
-      const float turned = op.scale < 0.0f ? -inverse : inverse;
+      const float inverse = !real ? 0.0f : op.scale < 0.0f ? -made.inverse : made.inverse;
 #pragma unroll
-      for (int s = 0; s < 2 * kSteps; ++s) {
-        float v[8];
-        LoadEight<TYPE>(op.q, from + 32 * (s / 2) + 16 * half + 8 * (s % 2), v);
+      for (int i = 0; i < 2 * kSteps; ++i) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+          float v[4];
+          part_of_row.Four(i, k, v);
           uint32_t packed[kDig];
+          PackDigits<kDig>(v, inverse, packed);
 #pragma unroll
-          for (int d = 0; d < kDig; ++d) packed[d] = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            int digit[kDig];
-            SplitDigits<kDig>(bad > 0.0f || !real ? 0 : static_cast<int>(rintf(v[4 * k + e] * turned)), digit);
-#pragma unroll
-            for (int d = 0; d < kDig; ++d) packed[d] |= static_cast<uint32_t>(digit[d] & 0xFF) << (8 * e);
-          }
-#pragma unroll
-          for (int d = 0; d < kDig; ++d) digits[d][s / 2][2 * (s % 2) + k] = static_cast<int>(packed[d]);
+          for (int d = 0; d < kDig; ++d) digits[d][i / 2][2 * (i % 2) + k] = static_cast<int>(packed[d]);
         }
       }
-      unit *= fabsf(op.scale) * (op.softcap != 0.0f ? 1.0f : kLog2E);
+      unit = made.unit * fabsf(op.scale) * (op.softcap != 0.0f ? 1.0f : kLog2E);
     }
     const float cap_inverse = op.softcap != 0.0f ? 1.0f / op.softcap : 0.0f;
 
@@ -325,9 +323,8 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int i = tid + kThreads * j;
-        const int t = i / kPieces, x = t & 31;
-        const int k_row = (t & 32) + 8 * ((x >> 2) & 3) + 4 * (x >> 4) + (x & 3);
-        *reinterpret_cast<U32x4*>(k_at + k_row * D + 16 * Turn<kPieces>(k_row, i % kPieces)) = k_in[j];
+        const int k_row = G::KRow(i / kPieces);
+        *reinterpret_cast<U32x4*>(k_at + k_row * D + 16 * G::KSlot(k_row, i % kPieces)) = k_in[j];
         const int d = i >> 2, piece = 2 * (i & 3);
         *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece)) = EightCodes(v_in[j][0], v_in[j][1]);
         *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece + 1)) = EightCodes(v_in[j][2], v_in[j][3]);
@@ -336,11 +333,11 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
     };
 
     float top = -INFINITY, sum = 0.0f;
-    F32x16 out[kBlocks];
+    Values out[kBlocks];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) out[b][i] = 0.0f;
+      for (int i = 0; i < kValues; ++i) out[b][i] = 0.0f;
     }
     const int tile_from = pair.first_tile + t_first, tile_to = tile_from + t_count;
     Group next = group_of(tile_from);
@@ -359,27 +356,48 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
         const uint8_t* const k_at = lds + buffer * G::kBuffer;
         const uint8_t* const v_at = k_at + G::kKBytes;
         const bool inside = (tile + 1) * kTileTokens <= all_to && tile * kTileTokens >= all_from;
-        // ---- 32 tokens at a time: S^T = K Q^T, their softmax, O^T += V^T P^T
+        // ---- 32 tokens at a time (all 64 where rows are 16): S^T = K Q^T, their softmax, O^T += V^T P^T
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          I32x16 dots[kDig];
+        for (int h = 0; h < G::kTurns; ++h) {
+          float s[16];
+          if constexpr (kWaveRows == 32) {
+            I32x16 dots[kDig];
 #pragma unroll
-          for (int d = 0; d < kDig; ++d) {
+            for (int d = 0; d < kDig; ++d) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dots[d][i] = 0;
+              for (int i = 0; i < 16; ++i) dots[d][i] = 0;
+            }
+            const int k_row = 32 * h + column;
+#pragma unroll
+            for (int x = 0; x < kSteps; ++x) {
+              const I32x4 k = *reinterpret_cast<const I32x4*>(k_at + k_row * D + 16 * G::KSlot(k_row, 2 * x + half));
+#pragma unroll
+              for (int d = 0; d < kDig; ++d) dots[d] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, digits[d][x], dots[d], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = JoinDigits<kDig>(dots[0][i], kDig == 3 ? dots[1][i] : 0, dots[kDig - 1][i]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              I32x4 dots[kDig];
+#pragma unroll
+              for (int d = 0; d < kDig; ++d) dots[d] = I32x4{0, 0, 0, 0};
+              const int k_row = 16 * (column >> 2) + 4 * t + (column & 3);
+#pragma unroll
+              for (int x = 0; x < kSteps; ++x) {
+                const I32x4 k = *reinterpret_cast<const I32x4*>(k_at + k_row * D + 16 * G::KSlot(k_row, 4 * x + half));
+#pragma unroll
+                for (int d = 0; d < kDig; ++d) dots[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, digits[d][x], dots[d], 0, 0, 0);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[4 * t + i] = JoinDigits<kDig>(dots[0][i], kDig == 3 ? dots[1][i] : 0, dots[kDig - 1][i]);
+            }
           }
-          const int k_row = 32 * h + column;
-#pragma unroll
-          for (int x = 0; x < kSteps; ++x) {
-            const I32x4 k = *reinterpret_cast<const I32x4*>(k_at + k_row * D + 16 * Turn<kPieces>(k_row, 2 * x + half));
-#pragma unroll
-            for (int d = 0; d < kDig; ++d) dots[d] = __builtin_amdgcn_mfma_i32_32x32x32_i8(k, digits[d][x], dots[d], 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          const F32x4 scales = group_scales[buffer * 4 + 2 * h + half];  // K's, V's, log2 of V's, 1 / V's
-          float s[16], worth = unit * scales[0], value_log = scales[2];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = JoinDigits<kDig>(dots[0][i], kDig == 3 ? dots[1][i] : 0, dots[kDig - 1][i]);
+          const int token_group = kWaveRows == 32 ? 2 * h + half : half;  // of the tile's four: the lane's tokens
+          const F32x4 scales = group_scales[buffer * 4 + token_group];  // K's, V's, log2 of V's, 1 / V's
+          float worth = unit * scales[0];
+          const float value_log = scales[2];
           if constexpr (CAPPED) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = Capped<TYPE>(s[i] * worth, op.softcap, cap_inverse) * kLog2E;
@@ -389,7 +407,7 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
           const bool whole = inside && __all(scales[3] > 0x1p-60f && scales[3] < 0x1p60f);
           if (!whole) {
             asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
-            const int p0 = tile * kTileTokens + 32 * h + 16 * half;
+            const int p0 = tile * kTileTokens + 16 * token_group;
             const int from = value_log == -INFINITY ? 16 : max(see_from - p0, 0), to = see_to - p0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = i >= from && i < to ? s[i] * worth : -INFINITY;
@@ -398,7 +416,7 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
           float peak = s[0];
 #pragma unroll
           for (int i = 1; i < 16; ++i) peak = fmaxf(peak, s[i]);
-          peak = AcrossHalvesMax(fmaf(peak, worth, value_log));
+          peak = Across<kWaveRows>(fmaf(peak, worth, value_log));
           // The maximum follows once it is kSlack behind: weights up to 2^kSlack keep their F16's precision, and the sums rarely turn.
           if (__any(peak > top + kSlack)) {
             const float higher = fmaxf(top, peak);
@@ -438,10 +456,15 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
           for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-              const int d = 32 * b + column;
-              const F16x8 v = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 4 * h + 2 * half + x));
-              out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], out[b], 0, 0, 0);
-              if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[x], out[b], 0, 0, 0);
+              const int d = kWaveRows * b + column;
+              const F16x8 v = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 2 * token_group + x));
+              if constexpr (kWaveRows == 32) {
+                out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], out[b], 0, 0, 0);
+                if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[x], out[b], 0, 0, 0);
+              } else {
+                out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[x], out[b], 0, 0, 0);
+                if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p_low[x], out[b], 0, 0, 0);
+              }
             }
           }
         }
@@ -449,7 +472,7 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
       if (more) place(buffer ^ 1);
       __syncthreads();
     }
-    sum = AcrossHalvesSum(sum);
+    sum = AcrossSum<kWaveRows>(sum);
 
     // ---- the rows' values, or this part's.
     const bool begins = t_first == 0, ends = t_first + t_count == pair.tiles;
@@ -462,9 +485,9 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kValues / 4; ++i) {
             const float x[4] = {out[b][4 * i] * inverse, out[b][4 * i + 1] * inverse, out[b][4 * i + 2] * inverse, out[b][4 * i + 3] * inverse};
-            StoreValues<TYPE, 4>(op.out, to + 32 * b + 8 * i + 4 * half, x);
+            StoreValues<TYPE, 4>(op.out, to + kWaveRows * b + 8 * i + 4 * half, x);
           }
         }
       }
@@ -474,7 +497,7 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) to[2 + 32 * b + 8 * (i / 4) + 4 * half + i % 4] = out[b][i];
+        for (int i = 0; i < kValues; ++i) to[2 + kWaveRows * b + 8 * (i / 4) + 4 * half + i % 4] = out[b][i];
       }
       if (begins) {
         const int64_t segment_end = m.list.before[pair_index] + static_cast<int64_t>(head + 1) * pair.tiles;
@@ -485,44 +508,46 @@ __global__ __launch_bounds__(kThreads, ManyGeo<D>::kAUnit) void ManyKernel(const
   if (tid == 0) *reinterpret_cast<I32x4*>(m.parts + 4 * w) = part;
 }
 
-// grid (workgroups of the launch before, kManyRows / 4): the parts of the segment that begins in workgroup x and ends in
-// another, a wave a row.
+// grid (workgroups of the launch before, kManyRows / 16): the parts of the segment that begins in workgroup x and ends in
+// another, a wave a row, four rows a wave. (Parts are few here and rows many.)
 template <int TYPE, int D>
-__global__ __launch_bounds__(kThreads) void ManyJoinKernel(const ManyArgs m) {
+__global__ __launch_bounds__(kJoinThreads) void ManyJoinKernel(const ManyArgs m) {
   constexpr int kPer = D / kWave;
   const PagedAttendArgs& a = m.a;
   const llmp_paged_attend& op = a.op;
   const I32x4 part = *reinterpret_cast<const I32x4*>(m.parts + 4 * blockIdx.x);
   if (part.x < 0) return;
-  const int lane = threadIdx.x & (kWave - 1), in_slot = 4 * blockIdx.y + threadIdx.x / kWave;
   const Pair pair = m.list.pairs[part.y];
   const PagedRequest q = RequestOf(op.starts, op.lengths, pair.request, op.tokens, a.most_length);
-  const int row = pair.chunk * kManyRows + in_slot;
-  if (row >= q.n * a.group) return;
-  const int first = blockIdx.x, last = part.x;
-  const auto slot_of = [&](int w) { return m.partial + ((2 * static_cast<int64_t>(w) + (w == first ? 1 : 0)) * kManyRows + in_slot) * (D + 2); };
-  float high = -INFINITY;
-  for (int w = first + lane; w <= last; w += kWave) high = fmaxf(high, slot_of(w)[0]);
+  const int lane = threadIdx.x & (kWave - 1), first = blockIdx.x, last = part.x;
 #pragma unroll
-  for (int step = 1; step < kWave; step <<= 1) high = fmaxf(high, __shfl_xor(high, step));
-  float all = 0.0f, value[kPer];
+  for (int i = 0; i < 4; ++i) {
+    const int in_slot = 16 * blockIdx.y + 4 * i + threadIdx.x / kWave, row = pair.chunk * kManyRows + in_slot;
+    if (row >= q.n * a.group) return;
+    const auto slot_of = [&](int w) { return m.partial + ((2 * static_cast<int64_t>(w) + (w == first ? 1 : 0)) * kManyRows + in_slot) * (D + 2); };
+    float high = -INFINITY;
+    for (int w = first + lane; w <= last; w += kWave) high = fmaxf(high, slot_of(w)[0]);
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
+    for (int step = 1; step < kWave; step <<= 1) high = fmaxf(high, __shfl_xor(high, step));
+    float all = 0.0f, value[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
 #pragma unroll 4
-  for (int w = first; w <= last; ++w) {
-    const float* from = slot_of(w);
-    const float top = from[0];
-    const float keep = top == -INFINITY ? (high == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top - high);
-    all += from[1] * keep;
+    for (int w = first; w <= last; ++w) {
+      const float* from = slot_of(w);
+      const float top = from[0];
+      const float keep = top == -INFINITY ? (high == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top - high);
+      all += from[1] * keep;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) value[e] += from[2 + kPer * lane + e] * keep;
+      for (int e = 0; e < kPer; ++e) value[e] += from[2 + kPer * lane + e] * keep;
+    }
+    const int h = part.z * a.group + row % a.group;
+    if (op.sinks != nullptr) all += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(high == -INFINITY ? 0.0f : high)));
+    const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
+    const int64_t to = (q.start + row / a.group) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e] * inverse);
   }
-  const int h = part.z * a.group + row % a.group;
-  if (op.sinks != nullptr) all += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(high == -INFINITY ? 0.0f : high)));
-  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
-  const int64_t to = (q.start + row / a.group) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e] * inverse);
 }
 
 int ManyGroups(int head_dim, int cus) { return (head_dim == 256 ? 1 : 2) * (cus > 0 ? cus : 256); }
@@ -541,11 +566,11 @@ void LaunchMany(const ManyArgs& m, int groups, hipStream_t stream) {
   if (G::kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&ManyKernel<TYPE, D, true>), G::kLds, &sized_capped)) return;
   hipLaunchKernelGGL(ListKernel, dim3(1), dim3(kListThreads), 0, stream, m, groups);
   if (capped) {
-    hipLaunchKernelGGL((ManyKernel<TYPE, D, true>), dim3(groups), dim3(kThreads), G::kLds, stream, m);
+    hipLaunchKernelGGL((ManyKernel<TYPE, D, true>), dim3(groups), dim3(G::kThreads), G::kLds, stream, m);
   } else {
-    hipLaunchKernelGGL((ManyKernel<TYPE, D, false>), dim3(groups), dim3(kThreads), G::kLds, stream, m);
+    hipLaunchKernelGGL((ManyKernel<TYPE, D, false>), dim3(groups), dim3(G::kThreads), G::kLds, stream, m);
   }
-  hipLaunchKernelGGL((ManyJoinKernel<TYPE, D>), dim3(groups, kManyRows / 4), dim3(kThreads), 0, stream, m);
+  hipLaunchKernelGGL((ManyJoinKernel<TYPE, D>), dim3(groups, kManyRows / 16), dim3(kJoinThreads), 0, stream, m);
 }
 template <int TYPE>
 void LaunchManyOf(const ManyArgs& m, int groups, hipStream_t stream) {
