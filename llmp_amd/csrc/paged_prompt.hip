@@ -280,19 +280,20 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
     }
     const float cap_inverse = op.softcap != 0.0f ? 1.0f / op.softcap : 0.0f;
 
-    // ---- the tiles' loads. The page of the tile's 16-token group `lane & 3`, from every lane.
+    // ---- the tiles' loads. A lane knows the page of the tile's 16-token group `lane & 3`; it is looked at a tile after it was
+    // asked for (a look waits for all loads before it).
     const int p16 = c.page / 16;
     struct Group {
       int page, offset;
+      bool there;
     };
     const auto group_of = [&](int tile) {
       Group g;
       const int n16 = 4 * tile + (lane & 3);
       const int entry = static_cast<int>(PagedDivide(n16, a.page_magic));
       g.offset = 16 * (n16 - entry * p16);
-      g.page = -1;
-      if (entry < op.table_width && 16 * n16 < q.length) g.page = table[entry];
-      if (g.page >= c.pages) g.page = -1;
+      g.there = entry < op.table_width && 16 * n16 < q.length;
+      g.page = table[g.there ? entry : 0];
       return g;
     };
     const int64_t page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
@@ -300,21 +301,22 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
     const uint8_t* const v_base = static_cast<const uint8_t*>(c.v) + static_cast<int64_t>(head) * c.page * D;
     U32x4 k_in[kLoads], v_in[kLoads];
     F32x4 scales_in;
+    bool page_in;
     const auto fetch = [&](const Group& g) {
+      page_in = g.there && g.page >= 0 && g.page < c.pages;
+      const int page = page_in ? g.page : 0;
+      const uint8_t* const v_from = v_base + page * page_bytes + g.offset + (tid >> 2) * c.page;  // (a lane's piece of V is of its group)
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int i = tid + kThreads * j;
-        const int t = i / kPieces, k_group = t >> 4;
-        const uint8_t* from = k_base + max(__shfl(g.page, k_group), 0) * page_bytes + (__shfl(g.offset, k_group) + (t & 15)) * D + 16 * (i % kPieces);
-        k_in[j] = *reinterpret_cast<const U32x4*>(from);
-        from = v_base + max(__shfl(g.page, i & 3), 0) * page_bytes + (i >> 2) * c.page + __shfl(g.offset, i & 3);
-        v_in[j] = *reinterpret_cast<const U32x4*>(from);
+        // (A wave's rows of K are of one group.)
+        const int t = (wave * kWave + kThreads * j) / kPieces, k_group = t >> 4;
+        const uint8_t* const k_from = k_base + __builtin_amdgcn_readlane(page, k_group) * page_bytes + (__builtin_amdgcn_readlane(g.offset, k_group) + (t & 15)) * D;
+        k_in[j] = *reinterpret_cast<const U32x4*>(k_from + static_cast<uint32_t>(16 * lane));
+        v_in[j] = *reinterpret_cast<const U32x4*>(v_from + kThreads / 4 * j * c.page);
       }
       if (tid < 4) {
-        const int64_t at = static_cast<int64_t>(max(g.page, 0)) * c.kv_heads + head;
-        const float vs = c.v_scale[at];
-        // (A logarithm of -infinity: no page.)
-        scales_in = F32x4{c.k_scale[at], vs, g.page >= 0 ? ScaleLog(vs) : -INFINITY, g.page >= 0 ? 1.0f / vs : 0.0f};
+        const int64_t at = static_cast<int64_t>(page) * c.kv_heads + head;
+        scales_in = F32x4{c.k_scale[at], c.v_scale[at], 0.0f, 0.0f};
       }
     };
     const auto place = [&](int buffer) {
@@ -329,7 +331,10 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
         *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece)) = EightCodes(v_in[j][0], v_in[j][1]);
         *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece + 1)) = EightCodes(v_in[j][2], v_in[j][3]);
       }
-      if (tid < 4) group_scales[buffer * 4 + tid] = scales_in;
+      if (tid < 4) {  // (a logarithm of -infinity: no page)
+        const float vs = scales_in[1];
+        group_scales[buffer * 4 + tid] = F32x4{scales_in[0], vs, page_in ? ScaleLog(vs) : -INFINITY, page_in ? 1.0f / vs : 0.0f};
+      }
     };
 
     float top = -INFINITY, sum = 0.0f;
