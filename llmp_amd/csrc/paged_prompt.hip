@@ -400,6 +400,19 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
             }
           }
           const int token_group = kWaveRows == 32 ? 2 * h + half : half;  // of the tile's four: the lane's tokens
+          // (V's operands are asked for here, before the softmax that makes them useful: a read's latency is the softmax's.)
+          F16x8 v_half[2][kBlocks];
+          const auto read_v = [&](int x) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+              const int d = kWaveRows * b + column;
+              v_half[x][b] = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 2 * token_group + x));
+            }
+          };
+          if constexpr (kWaveRows == 32) {
+            read_v(0);
+            read_v(1);
+          }
           const F32x4 scales = group_scales[buffer * 4 + token_group];  // K's, V's, log2 of V's, 1 / V's
           float worth = unit * scales[0];
           const float value_log = scales[2];
@@ -459,10 +472,10 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
+            if constexpr (kWaveRows == 16) read_v(x);
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-              const int d = kWaveRows * b + column;
-              const F16x8 v = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 2 * token_group + x));
+              const F16x8 v = v_half[x][b];
               if constexpr (kWaveRows == 32) {
                 out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], out[b], 0, 0, 0);
                 if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[x], out[b], 0, 0, 0);
