@@ -209,6 +209,12 @@ __device__ __forceinline__ int KPiece(int token, int piece) {
 }
 __device__ __forceinline__ int VPiece(int d, int piece) { return piece ^ ((d >> 2) & 3); }
 
+// A lane's 16 bytes from memory to LDS at `to` (the same in every lane) + 16 lane.
+__device__ __forceinline__ void ToLds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(reinterpret_cast<uintptr_t>(from)),
+                                   reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(reinterpret_cast<uintptr_t>(to)), 16, 0, 0);
+}
+
 // softcap * tanh(s / softcap). F32 results take the library's tanh; 16-bit ones 1 - 2 / (e^2x + 1), whose error (2^-23 of the
 // softcap) is far below their rounding.
 template <int TYPE>

@@ -68,12 +68,6 @@ constexpr int FewLds(int head_dim) {
 }
 // Workgroups a compute unit: by registers and LDS, 128 KB of tiles on their way either way (96 KB at 64).
 constexpr int FewAUnit(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
-// A lane's 16 bytes from memory to LDS at `to` (the same in every lane) + 16 lane.
-__device__ __forceinline__ void ToLds(const uint8_t* from, uint8_t* to) {
-  __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(reinterpret_cast<uintptr_t>(from)),
-                                   reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(reinterpret_cast<uintptr_t>(to)), 16, 0, 0);
-}
-
 // Where a lane's 16 tokens of a tile lie.
 struct Place {
   int page;  // in the cache, -1: none

@@ -151,11 +151,10 @@ struct ManyGeo {
   static constexpr int kBuffer = kKBytes + kVBytes;
   static constexpr int kLds = 2 * kBuffer + 2 * 4 * 16;  // and the four 16-token groups' scales
   static constexpr int kAUnit = D == 256 ? 1 : 2;        // workgroups a compute unit
-  // K's row of a token in LDS, and where a piece of it lies: rows in the products' order, or as KPiece has them.
-  static __device__ __forceinline__ int KRow(int t) {
-    if constexpr (kWaveRows == 16) return t;
-    const int x = t & 31;
-    return (t & 32) + 8 * ((x >> 2) & 3) + 4 * (x >> 4) + (x & 3);
+  // The token of a row of K in LDS, and where a piece of it lies: rows in the products' order, or as KPiece has them.
+  static __device__ __forceinline__ int KToken(int row) {
+    if constexpr (kWaveRows == 16) return row;
+    return (row & 32) + 16 * ((row >> 2) & 1) + 4 * ((row >> 3) & 3) + (row & 3);
   }
   static __device__ __forceinline__ int KSlot(int row, int piece) {
     if constexpr (kWaveRows == 16) return KPiece<D>(row, piece);
@@ -299,34 +298,55 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
     const int64_t page_bytes = static_cast<int64_t>(c.kv_heads) * c.page * D;
     const uint8_t* const k_base = static_cast<const uint8_t*>(c.k) + static_cast<int64_t>(head) * c.page * D;
     const uint8_t* const v_base = static_cast<const uint8_t*>(c.v) + static_cast<int64_t>(head) * c.page * D;
-    U32x4 k_in[kLoads], v_in[kLoads];
+    // K goes from memory to LDS by itself (a lane's 16 bytes of a load to 16 lane: the row and piece that belong there), V through
+    // registers, where it becomes F16. Where a tile is of one page, places are the same for every lane but for constants.
+    U32x4 v_in[kLoads];
     F32x4 scales_in;
     bool page_in;
-    const auto fetch = [&](const Group& g) {
+    constexpr int kLoadRows = kWave / kPieces, kWaveKRows = kTileTokens / G::kWaves;  // K's rows a load, a wave
+    uint32_t k_from[kLoads];  // from the token group's first row
+    int k_group[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int k_row = wave * kWaveKRows + kLoadRows * j + lane / kPieces, t = G::KToken(k_row);
+      k_group[j] = t >> 4;
+      k_from[j] = (t & 15) * D + 16 * G::KSlot(k_row, lane % kPieces);
+    }
+    const uint32_t v_from = (tid >> 2) * c.page;
+    const bool one_page = p16 % 4 == 0;
+    const auto fetch = [&](const Group& g, int buffer) {
       page_in = g.there && g.page >= 0 && g.page < c.pages;
       const int page = page_in ? g.page : 0;
-      const uint8_t* const v_from = v_base + page * page_bytes + g.offset + (tid >> 2) * c.page;  // (a lane's piece of V is of its group)
+      uint8_t* const k_to = lds + buffer * G::kBuffer + wave * kWaveKRows * D;
+      if (one_page) {
+        const int64_t at = __builtin_amdgcn_readfirstlane(page) * page_bytes;
+        const int offset = __builtin_amdgcn_readfirstlane(g.offset);
+        const uint8_t* const k_tile = k_base + at + offset * D;
+        const uint8_t* const v_tile = v_base + at + offset;
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        // (A wave's rows of K are of one group.)
-        const int t = (wave * kWave + kThreads * j) / kPieces, k_group = t >> 4;
-        const uint8_t* const k_from = k_base + __builtin_amdgcn_readlane(page, k_group) * page_bytes + (__builtin_amdgcn_readlane(g.offset, k_group) + (t & 15)) * D;
-        k_in[j] = *reinterpret_cast<const U32x4*>(k_from + static_cast<uint32_t>(16 * lane));
-        v_in[j] = *reinterpret_cast<const U32x4*>(v_from + kThreads / 4 * j * c.page);
+        for (int j = 0; j < kLoads; ++j) {
+          ToLds(k_tile + static_cast<uint32_t>(k_from[j] + 16 * k_group[j] * D), k_to + 1024 * j);
+          v_in[j] = *reinterpret_cast<const U32x4*>(v_tile + kThreads / 4 * j * c.page + static_cast<uint32_t>(v_from + 16 * (lane & 3)));
+        }
+      } else {
+        const int64_t at = page * page_bytes;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const int k_page = __shfl(page, k_group[j]), k_offset = __shfl(g.offset, k_group[j]);
+          ToLds(k_base + k_page * page_bytes + k_offset * D + k_from[j], k_to + 1024 * j);
+          v_in[j] = *reinterpret_cast<const U32x4*>(v_base + at + g.offset + kThreads / 4 * j * c.page + v_from);  // (a lane's piece of V is of its group)
+        }
       }
       if (tid < 4) {
-        const int64_t at = static_cast<int64_t>(page) * c.kv_heads + head;
-        scales_in = F32x4{c.k_scale[at], c.v_scale[at], 0.0f, 0.0f};
+        const int64_t i = static_cast<int64_t>(page) * c.kv_heads + head;
+        scales_in = F32x4{c.k_scale[i], c.v_scale[i], 0.0f, 0.0f};
       }
     };
     const auto place = [&](int buffer) {
-      uint8_t* const k_at = lds + buffer * G::kBuffer;
-      uint8_t* const v_at = k_at + G::kKBytes;
+      uint8_t* const v_at = lds + buffer * G::kBuffer + G::kKBytes;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int i = tid + kThreads * j;
-        const int k_row = G::KRow(i / kPieces);
-        *reinterpret_cast<U32x4*>(k_at + k_row * D + 16 * G::KSlot(k_row, i % kPieces)) = k_in[j];
         const int d = i >> 2, piece = 2 * (i & 3);
         *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece)) = EightCodes(v_in[j][0], v_in[j][1]);
         *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece + 1)) = EightCodes(v_in[j][2], v_in[j][3]);
@@ -345,16 +365,21 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
       for (int i = 0; i < kValues; ++i) out[b][i] = 0.0f;
     }
     const int tile_from = pair.first_tile + t_first, tile_to = tile_from + t_count;
+    // A tile is whole in LDS once every wave's loads have landed.
+    const auto meet = [&]() {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      __syncthreads();
+    };
     Group next = group_of(tile_from);
-    fetch(next);
+    fetch(next, 0);
     next = group_of(tile_from + 1);
     place(0);
-    __syncthreads();
+    meet();
     for (int tile = tile_from; tile < tile_to; ++tile) {
       const int buffer = (tile - tile_from) & 1;
       const bool more = tile + 1 < tile_to;
       if (more) {
-        fetch(next);
+        fetch(next, buffer ^ 1);
         next = group_of(tile + 2);
       }
       if (tile * kTileTokens < any_to && (tile + 1) * kTileTokens > any_from) {
@@ -488,7 +513,7 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
         }
       }
       if (more) place(buffer ^ 1);
-      __syncthreads();
+      meet();
     }
     sum = AcrossSum<kWaveRows>(sum);
 
