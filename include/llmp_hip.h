@@ -635,7 +635,7 @@ typedef struct llmp_paged_cache {
  *   work      I32 [work_items][4], 16-byte aligned: {page, first row, tokens held before, new tokens} of every page that new
  *             tokens touch, request after request; {-1, 0, 0, 0} past them. llmp_hip_paged_work_items(requests, tokens, page) are
  *             always enough.
- * scratch: llmp_hip_paged_plan_scratch(requests) bytes. One launch for a decode step's sizes, two for larger ones. */
+ * scratch: llmp_hip_paged_plan_scratch(requests) bytes at a 16-byte boundary. One launch for a decode step's sizes, two for larger ones. */
 typedef struct llmp_paged_plan {
   const int32_t* before;
   const int32_t* after;

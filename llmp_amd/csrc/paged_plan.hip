@@ -4,16 +4,18 @@
 // nothing is ordered by atomics and the same lengths give the same answer.
 //
 // The kernel is latency: a decode step of 64 requests moves some kilobytes. Sizes whose outputs one workgroup writes in a few
-// sweeps are one launch, the sums in LDS; larger ones sum in a first launch of one workgroup (a pass of the requests, 1024
-// at a time, the sums to scratch) and write in a second of many.
-#include "paged.h"
+// sweeps are one launch, the sums and what is known of each request in LDS; the kinds of outputs lie on one line, so that
+// they are written beside each other and not one after another. Larger sizes sum in a first launch of one workgroup (a pass of
+// the requests, 1024 at a time, to scratch) and write in a second of many, a workgroup one kind's, its sums in LDS.
+#include "paged_attend.h"
 
 namespace llmp_hip {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kOneLaunchRequests = 1024;  // four sums of them in LDS
-constexpr int kOneLaunchOutputs = 8192;   // tokens and work items together: sweeps of 1024
+constexpr int kOneLaunchRequests = 1024;  // their sums in LDS
+constexpr int kOneLaunchOutputs = 4096;   // tokens and work items together: a few sweeps
+constexpr int kSearchRequests = 4096;     // the second launch's sums in LDS
 
 // A request's numbers before the sums.
 struct PlanRequest {
@@ -44,23 +46,26 @@ __device__ __forceinline__ int PagesTouched(const PlanRequest& q, int length, in
 
 // What the sums leave: the ring as it was, and the totals.
 struct PlanTotals {
-  int head, free, wants, gives, touched, tokens, missing;
+  int head, free, wants, gives, touched, tokens;
 };
 constexpr int kTotalInts = 8;
+// What the outputs need of a request.
+struct PlanRecord {
+  int before, length, have, want;
+};
+// The sums' and the records' places, in LDS or in scratch.
+struct PlanSums {
+  int *starts, *wants, *gives, *touched;  // [requests + 1], exclusive
+  I32x4* records;
+};
 
-// Inclusive sums over a workgroup of 1024 of three values at once; `carry` the running totals, known to every thread.
-template <int N>
+// Inclusive sums over a workgroup of N values at once; `carry` the running totals, known to every thread.
+template <int THREADS, int N>
 __device__ void BlockSums(int (&v)[N], int (&carry)[N], int* wave_sums) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  constexpr int kWaves = kPlanThreads / kWave;
+  constexpr int kWaves = THREADS / kWave;
 #pragma unroll
-  for (int step = 1; step < kWave; step <<= 1) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int up = __shfl_up(v[i], step);
-      if (lane >= step) v[i] += up;
-    }
-  }
+  for (int i = 0; i < N; ++i) v[i] = static_cast<int>(WaveSums(static_cast<uint32_t>(v[i])));
   if (lane == kWave - 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) wave_sums[i * kWaves + wave] = v[i];
@@ -69,6 +74,7 @@ __device__ void BlockSums(int (&v)[N], int (&carry)[N], int* wave_sums) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     int before = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const int s = wave_sums[i * kWaves + w];
       before += w < wave ? s : 0;
@@ -80,52 +86,54 @@ __device__ void BlockSums(int (&v)[N], int (&carry)[N], int* wave_sums) {
   __syncthreads();
 }
 
-// The sums' pass by one workgroup: starts and lengths written, exclusive sums of wants, gives and touched pages to `sums`
-// ([3][requests + 1]), the starts also to `starts_too` where that is not null.
-__device__ PlanTotals SumRequests(const llmp_paged_plan& op, int* sums, int* starts_too, int* wave_sums) {
+// The sums' pass by one workgroup: starts, lengths and counters written, the sums and records left in `to`.
+template <int THREADS>
+__device__ PlanTotals SumRequests(const llmp_paged_plan& op, const PlanSums& to, int* wave_sums) {
   PlanTotals t;
-  t.head = op.counters_in[0] % op.ring_size;
-  if (t.head < 0) t.head += op.ring_size;
+  t.head = op.counters_in[0];
   t.free = min(max(op.counters_in[1], 0), op.ring_size);
-  const int n1 = op.requests + 1;
+  if (t.head < 0 || t.head >= op.ring_size) {
+    t.head %= op.ring_size;
+    if (t.head < 0) t.head += op.ring_size;
+  }
   int carry[3] = {0, 0, 0}, carry_touched[2] = {0, 0};
-  for (int base = 0; base < op.requests; base += kPlanThreads) {
+  for (int base = 0; base < op.requests; base += THREADS) {
     const int r = base + threadIdx.x;
     const bool real = r < op.requests;
     PlanRequest q = {0, 0, 0, 0};
     if (real) q = ReadPlanRequest(op, r);
     const int fresh = max(q.after - q.before, 0), wants = max(q.want - q.have, 0), gives = max(q.have - q.want, 0);
     int v[3] = {fresh, wants, gives};
-    BlockSums(v, carry, wave_sums);
+    BlockSums<THREADS>(v, carry, wave_sums);
     const int got = PagesGot(q, v[1] - wants, t.free);
     const int length = LengthAfter(q, got, op.page);
     const int touched = PagesTouched(q, length, op.page);
     int u[2] = {touched, max(q.after - length, 0)};
-    BlockSums(u, carry_touched, wave_sums);
+    BlockSums<THREADS>(u, carry_touched, wave_sums);
     if (real) {
       op.starts[r] = v[0] - fresh;
       op.lengths[r] = length;
-      sums[r] = v[1] - wants;
-      sums[n1 + r] = v[2] - gives;
-      sums[2 * n1 + r] = u[0] - touched;
-      if (starts_too != nullptr) starts_too[r] = v[0] - fresh;
+      if (to.starts != op.starts) to.starts[r] = v[0] - fresh;
+      to.wants[r] = v[1] - wants;
+      to.gives[r] = v[2] - gives;
+      to.touched[r] = u[0] - touched;
+      to.records[r] = I32x4{q.before, length, q.have, q.want};
     }
   }
   t.tokens = carry[0];
   t.wants = carry[1];
   t.gives = carry[2];
   t.touched = carry_touched[0];
-  t.missing = carry_touched[1];
   if (threadIdx.x == 0) {
     op.starts[op.requests] = t.tokens;
-    if (starts_too != nullptr) starts_too[op.requests] = t.tokens;
-    sums[op.requests] = t.wants;
-    sums[n1 + op.requests] = t.gives;
-    sums[2 * n1 + op.requests] = t.touched;
+    to.starts[op.requests] = t.tokens;
+    to.wants[op.requests] = t.wants;
+    to.gives[op.requests] = t.gives;
+    to.touched[op.requests] = t.touched;
     const int taken = min(t.wants, t.free);
     op.counters[0] = static_cast<int>((static_cast<int64_t>(t.head) + taken) % op.ring_size);
     op.counters[1] = min(t.free - taken + t.gives, op.ring_size);
-    op.counters[2] = t.missing;
+    op.counters[2] = carry_touched[1];
   }
   return t;
 }
@@ -143,72 +151,102 @@ __device__ __forceinline__ int OwnerOf(const int* sums, int requests, int index)
   }
   return low;
 }
-__device__ __forceinline__ int RingAt(const llmp_paged_plan& op, int64_t index) { return op.ring[index % op.ring_size]; }
-
+// The ring's entry `index` past its head (head and index both below its size).
+__device__ __forceinline__ uint32_t RingPlace(const llmp_paged_plan& op, int head, int index) {
+  const uint32_t at = static_cast<uint32_t>(head) + static_cast<uint32_t>(index), size = static_cast<uint32_t>(op.ring_size);
+  return at >= size ? (at - size >= size ? 0 : at - size) : at;
+}
+__device__ __forceinline__ PlanRecord RecordOf(const PlanSums& s, int r) {
+  const I32x4 w = s.records[r];
+  return {w.x, w.y, w.z, w.w};
+}
 // Page j of request r: an old entry of the table, or the ring's (the new entry itself is another thread's to write).
-__device__ __forceinline__ int PageOf(const llmp_paged_plan& op, const PlanTotals& t, const PlanRequest& q, int r, int wants_before, int j) {
-  return j < q.have ? op.table[r * op.table_stride + j] : RingAt(op, static_cast<int64_t>(t.head) + wants_before + j - q.have);
+__device__ __forceinline__ int PageOf(const llmp_paged_plan& op, const PlanTotals& t, const PlanRecord& q, int r, int wants_before, int j) {
+  return j < q.have ? op.table[r * op.table_stride + j] : op.ring[RingPlace(op, t.head, wants_before + j - q.have)];
 }
 
-// Every output by its index, spread over `threads` threads. What the ring takes back lies past all that it gives out, and new
-// entries of the table past all that are read, so the order does not matter. (The ranges are checked where they index
-// memory: lengths whose sums pass an int give wrong numbers, not accesses outside the arrays.)
-__device__ void WriteOutputs(const llmp_paged_plan& op, const PlanTotals& t, const int* starts, const int* sums, int thread, int threads) {
-  const int n1 = op.requests + 1;
-  const int *wants = sums, *gives = sums + n1, *touched = sums + 2 * n1;
-  for (int i = thread; i < op.tokens; i += threads) {
-    int slot = -1, position = -1, owner = -1;
-    if (i < t.tokens) {
-      owner = OwnerOf(starts, op.requests, i);
-      const PlanRequest q = ReadPlanRequest(op, owner);
-      position = q.before + i - starts[owner];
-      const int length = LengthAfter(q, PagesGot(q, wants[owner], t.free), op.page);
-      if (position >= 0 && position < length) slot = PageOf(op, t, q, owner, wants[owner], position / op.page) * op.page + position % op.page;
+// The outputs, each by its index. What the ring takes back lies past all that it gives out, and new entries of the table past all
+// that are read, so the order does not matter. (The ranges are checked where they index memory: lengths whose sums
+// pass an int give wrong numbers, not accesses outside the arrays.)
+__device__ __forceinline__ void WriteToken(const llmp_paged_plan& op, const PlanTotals& t, const PlanSums& s, int i) {
+  int slot = -1, position = -1, owner = -1;
+  if (i < t.tokens) {
+    owner = OwnerOf(s.starts, op.requests, i);
+    const PlanRecord q = RecordOf(s, owner);
+    position = q.before + i - s.starts[owner];
+    if (position >= 0 && position < q.length) {
+      const int j = position / op.page;
+      slot = PageOf(op, t, q, owner, s.wants[owner], j) * op.page + position - j * op.page;
     }
-    op.slots[i] = slot;
-    op.positions[i] = position;
-    op.owners[i] = owner;
   }
-  for (int i = thread; i < op.work_items; i += threads) {
-    I32x4 item = {-1, 0, 0, 0};
-    if (i < t.touched) {
-      const int r = OwnerOf(touched, op.requests, i);
-      const PlanRequest q = ReadPlanRequest(op, r);
-      const int length = LengthAfter(q, PagesGot(q, wants[r], t.free), op.page);
-      const int j = q.before / op.page + i - touched[r];
-      if (j < 0 || j >= CeilPages(length, op.page)) continue;
-      const int low = max(j * op.page, q.before), high = static_cast<int>(min(static_cast<int64_t>(length), static_cast<int64_t>(j + 1) * op.page));
-      item = I32x4{PageOf(op, t, q, r, wants[r], j), starts[r] + low - q.before, low - j * op.page, high - low};
-    }
-    *reinterpret_cast<I32x4*>(op.work + 4 * static_cast<int64_t>(i)) = item;
-  }
-  const int taken = min(t.wants, t.free);
-  for (int i = thread; i < taken; i += threads) {
-    const int r = OwnerOf(wants, op.requests, i);
-    const PlanRequest q = ReadPlanRequest(op, r);
-    const int j = q.have + i - wants[r];
-    if (j >= q.have && j < q.want) op.table[r * op.table_stride + j] = RingAt(op, static_cast<int64_t>(t.head) + i);
-  }
-  const int back = min(t.gives, op.ring_size - t.free);  // (all of them, unless the ring's count was wrong)
-  for (int i = thread; i < back; i += threads) {
-    const int r = OwnerOf(gives, op.requests, i);
-    const PlanRequest q = ReadPlanRequest(op, r);
-    const int j = q.want + i - gives[r];
-    if (j >= q.want && j < q.have) op.ring[(static_cast<int64_t>(t.head) + t.free + i) % op.ring_size] = op.table[r * op.table_stride + j];
-  }
+  op.slots[i] = slot;
+  op.positions[i] = position;
+  op.owners[i] = owner;
 }
+__device__ __forceinline__ void WriteItem(const llmp_paged_plan& op, const PlanTotals& t, const PlanSums& s, int i) {
+  I32x4 item = {-1, 0, 0, 0};
+  if (i < t.touched) {
+    const int r = OwnerOf(s.touched, op.requests, i);
+    const PlanRecord q = RecordOf(s, r);
+    const int j = q.before / op.page + i - s.touched[r];
+    if (j >= 0 && j < CeilPages(q.length, op.page)) {
+      const int low = max(j * op.page, q.before), high = static_cast<int>(min(static_cast<int64_t>(q.length), static_cast<int64_t>(j + 1) * op.page));
+      item = I32x4{PageOf(op, t, q, r, s.wants[r], j), s.starts[r] + low - q.before, low - j * op.page, high - low};
+    }
+  }
+  *reinterpret_cast<I32x4*>(op.work + 4 * static_cast<int64_t>(i)) = item;
+}
+__device__ __forceinline__ void WriteTaken(const llmp_paged_plan& op, const PlanTotals& t, const PlanSums& s, int i) {
+  const int r = OwnerOf(s.wants, op.requests, i);
+  const PlanRecord q = RecordOf(s, r);
+  const int j = q.have + i - s.wants[r];
+  if (j >= q.have && j < q.want) op.table[r * op.table_stride + j] = op.ring[RingPlace(op, t.head, i)];
+}
+__device__ __forceinline__ void WriteBack(const llmp_paged_plan& op, const PlanTotals& t, const PlanSums& s, int i) {
+  const int r = OwnerOf(s.gives, op.requests, i);
+  const PlanRecord q = RecordOf(s, r);
+  const int j = q.want + i - s.gives[r];
+  if (j >= q.want && j < q.have) op.ring[RingPlace(op, t.head, t.free + i)] = op.table[r * op.table_stride + j];
+}
+__device__ __forceinline__ int TakenOf(const PlanTotals& t) { return min(t.wants, t.free); }
+// (All of them, unless the ring's count was wrong.)
+__device__ __forceinline__ int BackOf(const llmp_paged_plan& op, const PlanTotals& t) { return min(t.gives, op.ring_size - t.free); }
 
-__global__ __launch_bounds__(kPlanThreads) void PlanOneKernel(const llmp_paged_plan op) {
-  __shared__ int sums[3 * (kOneLaunchRequests + 1)], starts[kOneLaunchRequests + 1], wave_sums[3 * kPlanThreads / kWave];
-  const PlanTotals t = SumRequests(op, sums, starts, wave_sums);
+// THREADS: 256 for up to 256 requests, whose barriers four waves then meet at, or 1024.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void PlanOneKernel(const llmp_paged_plan op) {
+  constexpr int kMost = THREADS;  // requests
+  __shared__ int starts[kMost + 1], wants[kMost + 1], gives[kMost + 1], touched[kMost + 1], wave_sums[3 * THREADS / kWave];
+  __shared__ I32x4 records[kMost];
+  const PlanSums s = {starts, wants, gives, touched, records};
+  const PlanTotals t = SumRequests<THREADS>(op, s, wave_sums);
   __syncthreads();
-  WriteOutputs(op, t, starts, sums, threadIdx.x, kPlanThreads);
+  const int items = op.tokens, taken = items + op.work_items, back = taken + TakenOf(t), end = back + BackOf(op, t);
+  for (int i = threadIdx.x; i < end; i += THREADS) {
+    if (i < items) {
+      WriteToken(op, t, s, i);
+    } else if (i < taken) {
+      WriteItem(op, t, s, i - items);
+    } else if (i < back) {
+      WriteTaken(op, t, s, i - taken);
+    } else {
+      WriteBack(op, t, s, i - back);
+    }
+  }
+}
+
+__device__ __forceinline__ PlanSums ScratchSums(const llmp_paged_plan& op) {
+  int* const at = static_cast<int*>(op.scratch) + kTotalInts;
+  const int n1 = op.requests + 1;
+  I32x4* const records = reinterpret_cast<I32x4*>(at);
+  int* const sums = at + 4 * static_cast<int64_t>(op.requests);
+  return {op.starts, sums, sums + n1, sums + 2 * static_cast<int64_t>(n1), records};
 }
 
 __global__ __launch_bounds__(kPlanThreads) void PlanSumKernel(const llmp_paged_plan op) {
   __shared__ int wave_sums[3 * kPlanThreads / kWave];
   int* totals = static_cast<int*>(op.scratch);
-  const PlanTotals t = SumRequests(op, totals + kTotalInts, nullptr, wave_sums);
+  const PlanTotals t = SumRequests<kPlanThreads>(op, ScratchSums(op), wave_sums);
   // (The counters may be overwritten in place: the second launch takes what they were from here.)
   if (threadIdx.x == 0) {
     totals[0] = t.head, totals[1] = t.free, totals[2] = t.wants, totals[3] = t.gives, totals[4] = t.touched, totals[5] = t.tokens;
@@ -216,12 +254,36 @@ __global__ __launch_bounds__(kPlanThreads) void PlanSumKernel(const llmp_paged_p
 }
 
 constexpr int kWriteThreads = 256;
-__global__ __launch_bounds__(kWriteThreads) void PlanWriteKernel(const llmp_paged_plan op) {
+// grid (blocks for tokens, then for items, then `moves` for the pages that move).
+__global__ __launch_bounds__(kWriteThreads) void PlanWriteKernel(const llmp_paged_plan op, int token_blocks, int item_blocks) {
+  __shared__ int search[kSearchRequests + 1];
   const int* totals = static_cast<const int*>(op.scratch);
-  PlanTotals t;
-  t.head = totals[0], t.free = totals[1], t.wants = totals[2], t.gives = totals[3], t.touched = totals[4], t.tokens = totals[5];
-  t.missing = 0;
-  WriteOutputs(op, t, op.starts, totals + kTotalInts, blockIdx.x * kWriteThreads + threadIdx.x, gridDim.x * kWriteThreads);
+  const PlanTotals t = {totals[0], totals[1], totals[2], totals[3], totals[4], totals[5]};
+  PlanSums s = ScratchSums(op);
+  const int block = blockIdx.x, kind = block < token_blocks ? 0 : block < token_blocks + item_blocks ? 1 : 2;
+  // The sums that this kind's outputs are searched in.
+  const auto stage = [&](int*& sums) {
+    if (op.requests > kSearchRequests) return;
+    __syncthreads();
+    for (int r = threadIdx.x; r <= op.requests; r += kWriteThreads) search[r] = sums[r];
+    sums = search;
+    __syncthreads();
+  };
+  if (kind == 0) {
+    stage(s.starts);
+    for (int i = block * kWriteThreads + threadIdx.x; i < op.tokens; i += token_blocks * kWriteThreads) WriteToken(op, t, s, i);
+  } else if (kind == 1) {
+    stage(s.touched);
+    for (int i = (block - token_blocks) * kWriteThreads + threadIdx.x; i < op.work_items; i += item_blocks * kWriteThreads) WriteItem(op, t, s, i);
+  } else {
+    const int first = (block - token_blocks - item_blocks) * kWriteThreads + threadIdx.x, step = (gridDim.x - token_blocks - item_blocks) * kWriteThreads;
+    const PlanSums from = s;
+    stage(s.wants);
+    for (int i = first; i < TakenOf(t); i += step) WriteTaken(op, t, s, i);
+    s = from;
+    stage(s.gives);
+    for (int i = first; i < BackOf(op, t); i += step) WriteBack(op, t, s, i);
+  }
 }
 
 }  // namespace
@@ -260,7 +322,7 @@ extern "C" int64_t llmp_hip_paged_work_items(int requests, int tokens, int page)
 }
 
 extern "C" size_t llmp_hip_paged_plan_scratch(int requests) {
-  return requests < 1 ? 0 : (kTotalInts + 3 * (static_cast<size_t>(requests) + 1)) * sizeof(int);
+  return requests < 1 ? 0 : (kTotalInts + 4 * static_cast<size_t>(requests) + 3 * (static_cast<size_t>(requests) + 1)) * sizeof(int);
 }
 
 extern "C" int llmp_hip_paged_plan(const llmp_paged_plan* op, void* stream) {
@@ -277,19 +339,25 @@ extern "C" int llmp_hip_paged_plan(const llmp_paged_plan* op, void* stream) {
   const uintptr_t words = reinterpret_cast<uintptr_t>(op->before) | reinterpret_cast<uintptr_t>(op->after) | reinterpret_cast<uintptr_t>(op->table) |
                           reinterpret_cast<uintptr_t>(op->ring) | reinterpret_cast<uintptr_t>(op->counters_in) | reinterpret_cast<uintptr_t>(op->counters) |
                           reinterpret_cast<uintptr_t>(op->starts) | reinterpret_cast<uintptr_t>(op->lengths) | reinterpret_cast<uintptr_t>(op->slots) |
-                          reinterpret_cast<uintptr_t>(op->positions) | reinterpret_cast<uintptr_t>(op->owners) | reinterpret_cast<uintptr_t>(op->scratch);
-  if (words % 4 != 0 || reinterpret_cast<uintptr_t>(op->work) % 16 != 0) return Refuse(1, "paged_plan: I32 arrays at 4-byte boundaries, the work items at 16");
+                          reinterpret_cast<uintptr_t>(op->positions) | reinterpret_cast<uintptr_t>(op->owners);
+  if (words % 4 != 0 || (reinterpret_cast<uintptr_t>(op->work) | reinterpret_cast<uintptr_t>(op->scratch)) % 16 != 0)
+    return Refuse(1, "paged_plan: I32 arrays at 4-byte boundaries, the work items and the scratch at 16");
   if (op->work_items < llmp_hip_paged_work_items(op->requests, op->tokens, op->page))
     return Refuse(1, "paged_plan: %d work items, %lld may be needed", op->work_items, (long long)llmp_hip_paged_work_items(op->requests, op->tokens, op->page));
   BeginLaunches();
   const hipStream_t on = static_cast<hipStream_t>(stream);
   const int64_t outputs = static_cast<int64_t>(op->tokens) + op->work_items;
   if (op->requests <= kOneLaunchRequests && outputs <= kOneLaunchOutputs) {
-    hipLaunchKernelGGL(PlanOneKernel, dim3(1), dim3(kPlanThreads), 0, on, *op);
+    if (op->requests <= 256 && outputs <= 1024) {
+      hipLaunchKernelGGL(PlanOneKernel<256>, dim3(1), dim3(256), 0, on, *op);
+    } else {
+      hipLaunchKernelGGL(PlanOneKernel<kPlanThreads>, dim3(1), dim3(kPlanThreads), 0, on, *op);
+    }
   } else {
+    const auto blocks = [](int64_t n) { return static_cast<int>(n < 1 ? 1 : (n + kWriteThreads - 1) / kWriteThreads < 512 ? (n + kWriteThreads - 1) / kWriteThreads : 512); };
+    const int tokens = blocks(op->tokens), items = blocks(op->work_items), moves = blocks(op->ring_size);  // (no more pages can move)
     hipLaunchKernelGGL(PlanSumKernel, dim3(1), dim3(kPlanThreads), 0, on, *op);
-    const int64_t blocks = (outputs + kWriteThreads - 1) / kWriteThreads;
-    hipLaunchKernelGGL(PlanWriteKernel, dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024)), dim3(kWriteThreads), 0, on, *op);
+    hipLaunchKernelGGL(PlanWriteKernel, dim3(tokens + items + moves), dim3(kWriteThreads), 0, on, *op, tokens, items);
   }
   return LaunchStatus("paged_plan");
 }

@@ -666,21 +666,35 @@ def paged_cache(pages, kv_heads, page, head_dim, device="cuda", edges=True):
 
 
 def _paged_cache(cache):
-    k, v = cache["k"], cache["v"]
-    pages, kv_heads, page, head_dim = k.shape
+    k, v, k_scale, v_scale = cache["k"], cache["v"], cache["k_scale"], cache["v_scale"]
     low, high = cache.get("low"), cache.get("high")
-    shapes = [(k, (pages, kv_heads, page, head_dim), torch.int8), (v, (pages, kv_heads, head_dim, page), torch.int8),
-              (cache["k_scale"], (pages, kv_heads), torch.float32), (cache["v_scale"], (pages, kv_heads), torch.float32)]
-    shapes += [(t, (pages, kv_heads, head_dim), torch.int8) for t in (low, high) if t is not None]
-    for t, shape, dtype in shapes:
-        assert t.shape == shape and t.dtype == dtype and t.is_contiguous(), "the cache's arrays are whole, of one set of sizes"
-    return _lib.PagedCache(k.data_ptr(), v.data_ptr(), cache["k_scale"].data_ptr(), cache["v_scale"].data_ptr(), _ptr(low), _ptr(high),
-                           pages, kv_heads, page, head_dim)
+    pages, kv_heads, page, head_dim = k.shape
+    heads = pages * kv_heads
+    whole = (k.dtype is torch.int8 and k.is_contiguous() and v.dtype is torch.int8 and v.is_contiguous() and v.shape == (pages, kv_heads, head_dim, page)
+             and k_scale.dtype is torch.float32 and k_scale.is_contiguous() and k_scale.numel() == heads
+             and v_scale.dtype is torch.float32 and v_scale.is_contiguous() and v_scale.numel() == heads)
+    for edge in (low, high):
+        whole = whole and (edge is None or (edge.dtype is torch.int8 and edge.is_contiguous() and edge.numel() == heads * head_dim))
+    assert whole, "the cache's arrays are whole, of one set of sizes"
+    return _lib.PagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), low.data_ptr() if low is not None else None,
+                           high.data_ptr() if high is not None else None, pages, kv_heads, page, head_dim)
 
 
 def _int32(*tensors):
     for t in tensors:
-        assert t.dtype == torch.int32 and t.stride(-1) == 1, "int32 arrays in one piece"
+        assert t.dtype is torch.int32 and t.stride(-1) == 1, "int32 arrays in one piece"
+
+
+_UNITS = {}
+
+
+def _compute_units():
+    """The current device's compute units, asked for once a device."""
+    device = torch._C._cuda_getDevice()
+    units = _UNITS.get(device)
+    if units is None:
+        units = _UNITS[device] = _lib.load().llmp_hip_compute_units()
+    return units
 
 
 def _table_stride(table):
@@ -697,23 +711,29 @@ def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
     instead of a new one (its counters may be the ones passed in)."""
     lib = _lib.load()
     _int32(before, after, table, ring, counters)
-    n = before.shape[0]
-    assert before.dim() == after.dim() == ring.dim() == 1 and after.shape[0] == n and table.dim() == 2 and table.shape[0] == n and counters.numel() >= 2
+    n, width = table.shape
+    assert before.shape == after.shape == (n,) and ring.dim() == 1 and counters.numel() >= 2
     items = lib.llmp_hip_paged_work_items(n, tokens, page)
+    scratch_ints = lib.llmp_hip_paged_plan_scratch(n) // 4
     if out is None:
-        # One allocation: the work items first, for their 16-byte boundary.
-        sizes = {"work": 4 * items, "slots": tokens, "positions": tokens, "requests": tokens, "starts": n + 1, "lengths": n, "counters": 3}
-        parts = torch.empty(sum(sizes.values()), dtype=torch.int32, device=before.device).split(list(sizes.values()))
-        out = dict(zip(sizes, parts))
-        out["work"] = out["work"].view(items, 4)
-    _int32(*out.values())
-    assert out["work"].shape[0] >= items and out["starts"].numel() > n and out["lengths"].numel() >= n and out["counters"].numel() >= 3
-    assert min(out[k].numel() for k in ("slots", "positions", "requests")) >= tokens and out["work"].is_contiguous()
-    scratch = torch.empty(lib.llmp_hip_paged_plan_scratch(n), dtype=torch.uint8, device=before.device)
-    op = _lib.PagedPlan(before.data_ptr(), after.data_ptr(), table.data_ptr(), ring.data_ptr(), counters.data_ptr(), out["counters"].data_ptr(),
-                        out["starts"].data_ptr(), out["lengths"].data_ptr(), out["slots"].data_ptr(), out["positions"].data_ptr(),
-                        out["requests"].data_ptr(), out["work"].data_ptr(), scratch.data_ptr(), _table_stride(table), n, table.shape[1],
-                        ring.shape[0], page, tokens, out["work"].shape[0])
+        # One allocation: the work items and the scratch first, at 16-byte boundaries.
+        padded = (scratch_ints + 3) // 4 * 4
+        work, scratch, slots, positions, requests, starts, lengths, counted = torch.empty(
+            4 * items + padded + 3 * tokens + 2 * n + 4, dtype=torch.int32, device=before.device).split_with_sizes(
+            (4 * items, padded, tokens, tokens, tokens, n + 1, n, 3))
+        out = {"work": work.view(items, 4), "slots": slots, "positions": positions, "requests": requests, "starts": starts, "lengths": lengths,
+               "counters": counted}
+    else:
+        work, slots, positions, requests, starts, lengths, counted = (
+            out[name] for name in ("work", "slots", "positions", "requests", "starts", "lengths", "counters"))
+        _int32(work, slots, positions, requests, starts, lengths, counted)
+        assert work.shape[0] >= items and work.is_contiguous() and starts.numel() > n and lengths.numel() >= n and counted.numel() >= 3
+        assert slots.numel() >= tokens and positions.numel() >= tokens and requests.numel() >= tokens
+        items = work.shape[0]
+        scratch = torch.empty(scratch_ints, dtype=torch.int32, device=before.device)
+    op = _lib.PagedPlan(before.data_ptr(), after.data_ptr(), table.data_ptr(), ring.data_ptr(), counters.data_ptr(), counted.data_ptr(),
+                        starts.data_ptr(), lengths.data_ptr(), slots.data_ptr(), positions.data_ptr(), requests.data_ptr(), work.data_ptr(),
+                        scratch.data_ptr(), _table_stride(table), n, width, ring.shape[0], page, tokens, items)
     _lib.check(lib.llmp_hip_paged_plan(C.byref(op), _stream()))
     return out
 
@@ -723,11 +743,11 @@ def paged_store(cache, k, v, work):
     names, quantized with a scale for each page and head; the cache is updated in place."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    assert k.shape == v.shape == (k.shape[0], c.kv_heads, c.head_dim) and k.dtype == v.dtype and k.stride(-1) == v.stride(-1) == 1
-    _int32(work)
-    assert work.dim() == 2 and work.shape[1] == 4 and work.is_contiguous()
-    op = _lib.PagedStore(c, k.data_ptr(), v.data_ptr(), work.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), _x_type(k), k.shape[0],
-                         work.shape[0])
+    tokens, kv_heads, head_dim = k.shape
+    (kt, kh, kd), (vt, vh, vd) = k.stride(), v.stride()
+    assert kv_heads == c.kv_heads and head_dim == c.head_dim and v.shape == k.shape and k.dtype is v.dtype and kd == vd == 1
+    assert work.dtype is torch.int32 and work.is_contiguous() and work.shape[1] == 4
+    op = _lib.PagedStore(c, k.data_ptr(), v.data_ptr(), work.data_ptr(), kt, kh, vt, vh, _X_TYPES[k.dtype], tokens, work.shape[0])
     _lib.check(lib.llmp_hip_paged_store(C.byref(op), _stream()))
 
 
@@ -736,17 +756,20 @@ def paged_read(cache, pages, dtype=torch.float32):
     number outside the cache gives zeros."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    assert pages.dim() == 1 and pages.dtype == torch.int32
-    k, v = (torch.empty((pages.shape[0], c.kv_heads, c.page, c.head_dim), dtype=dtype, device=pages.device) for _ in range(2))
-    _lib.check(lib.llmp_hip_paged_read(C.byref(c), pages.data_ptr(), pages.stride(0), pages.shape[0], _X_TYPES[dtype], k.data_ptr(), v.data_ptr(),
-                                       _stream()))
+    assert pages.dim() == 1 and pages.dtype is torch.int32
+    n = pages.shape[0]
+    k, v = torch.empty((2, n, c.kv_heads, c.page, c.head_dim), dtype=dtype, device=pages.device).unbind()
+    _lib.check(lib.llmp_hip_paged_read(C.byref(c), pages.data_ptr(), pages.stride(0), n, _X_TYPES[dtype], k.data_ptr(), v.data_ptr(), _stream()))
     return k, v
 
 
 def _paged_queries(q, c, table, lengths, starts):
     _int32(table, lengths, starts)
-    assert q.dim() == 3 and q.shape[2] == c.head_dim and q.stride(2) == 1
-    assert table.dim() == 2 and lengths.shape == (table.shape[0],) and starts.shape == (table.shape[0] + 1,)
+    tokens, heads, head_dim = q.shape
+    n, width = table.shape
+    token_stride, head_stride, one = q.stride()
+    assert head_dim == c.head_dim and one == 1 and lengths.shape == (n,) and starts.shape == (n + 1,)
+    return tokens, heads, n, width, token_stride, head_stride
 
 
 def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0.0, sinks=None, lists=None, most=None, out=None, scratch=None):
@@ -756,11 +779,13 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0
     known. Returns q's shape and type; rows past starts[requests] are not written."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    _paged_queries(q, c, table, lengths, starts)
-    tokens, heads, _ = q.shape
+    tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        out = torch.empty((tokens, heads, c.head_dim), dtype=q.dtype, device=q.device)
+        out_token, out_head = heads * c.head_dim, c.head_dim
+    else:
+        out_token, out_head, one = out.stride()
+        assert out.shape == q.shape and out.dtype is q.dtype and one == 1
     if lists is not None:
         _int32(lists)
         assert lists.is_contiguous() and lists.shape[:2] == (tokens, c.kv_heads)
@@ -768,12 +793,12 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0
     if tokens == 0:
         return out
     op = _lib.PagedAttend(c, q.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(lists), _ptr(sinks),
-                          q.stride(0), q.stride(1), out.stride(0), out.stride(1), _table_stride(table), _x_type(q), heads, table.shape[0], tokens,
-                          tokens if most is None else most, table.shape[1], lists.shape[2] if lists is not None else 0, window, scale, softcap)
-    cus = lib.llmp_hip_compute_units()
+                          q_token, q_head, out_token, out_head, _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens,
+                          tokens if most is None else most, width, lists.shape[2] if lists is not None else 0, window, scale, softcap)
+    cus, at = _compute_units(), C.byref(op)
     if scratch is None:
-        scratch = torch.empty(max(lib.llmp_hip_paged_attend_scratch(C.byref(op), cus), 16), dtype=torch.uint8, device=q.device)
-    _lib.check(lib.llmp_hip_paged_attend(C.byref(op), scratch.data_ptr(), scratch.numel(), cus, _stream()))
+        scratch = torch.empty(max(lib.llmp_hip_paged_attend_scratch(at, cus), 16), dtype=torch.uint8, device=q.device)
+    _lib.check(lib.llmp_hip_paged_attend(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
     return out
 
 
@@ -783,17 +808,17 @@ def paged_select(cache, q, table, lengths, starts, keep, *, first=1, recent=1, m
     are always among them. int32 [tokens, kv_heads, keep]."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    _paged_queries(q, c, table, lengths, starts)
-    tokens, heads, _ = q.shape
+    tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts)
     if out is None:
         out = torch.empty((tokens, c.kv_heads, keep), dtype=torch.int32, device=q.device)
-    assert out.shape == (tokens, c.kv_heads, keep) and out.dtype == torch.int32 and out.is_contiguous()
+    else:
+        assert out.shape == (tokens, c.kv_heads, keep) and out.dtype is torch.int32 and out.is_contiguous()
     if tokens == 0:
         return out
-    op = _lib.PagedSelect(c, q.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1),
-                          _table_stride(table), _x_type(q), heads, table.shape[0], tokens, tokens if most is None else most, table.shape[1], keep, first,
-                          recent)
+    op = _lib.PagedSelect(c, q.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), out.data_ptr(), q_token, q_head,
+                          _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens, tokens if most is None else most, width, keep, first, recent)
+    at = C.byref(op)
     if scratch is None:
-        scratch = torch.empty(max(lib.llmp_hip_paged_select_scratch(C.byref(op)), 16), dtype=torch.uint8, device=q.device)
-    _lib.check(lib.llmp_hip_paged_select(C.byref(op), scratch.data_ptr(), scratch.numel(), _stream()))
+        scratch = torch.empty(max(lib.llmp_hip_paged_select_scratch(at), 16), dtype=torch.uint8, device=q.device)
+    _lib.check(lib.llmp_hip_paged_select(at, scratch.data_ptr(), scratch.numel(), _stream()))
     return out
