@@ -81,6 +81,27 @@ __device__ __forceinline__ void StoreOne(void* base, int64_t element, float x) {
   if constexpr (TYPE == LLMP_X_F16) static_cast<uint16_t*>(base)[element] = static_cast<uint16_t>(FloatToHalfBits(x));
 }
 
+// Eight values' codes at a scale: the IEEE quotients rounded to nearest even, at most 127 in magnitude, 0 for NaN. By products with
+// the reciprocal, whose errors (below 2^-15 at 127) matter only near the middle between two codes: there, and at scales without a
+// reciprocal, by divisions.
+__device__ __forceinline__ void CodesOf(const float (&x)[8], float scale, float inverse, int (&code)[8]) {
+  bool near = !(scale > 0x1p-120f);
+  float r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float y = x[e] * inverse;
+    r[e] = rintf(y);
+    near = near || fabsf(y - r[e]) > 0.5f - 0x1p-14f;
+  }
+  if (__any(near)) {
+    asm volatile("" ::: "memory");  // (a branch: it is rarely taken)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = scale > 0.0f ? rintf(x[e] / scale) : 0.0f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) code[e] = __builtin_isnan(r[e]) ? 0 : static_cast<int>(fminf(fmaxf(r[e], -127.0f), 127.0f));
+}
+
 // A request's new tokens and length, whatever the device arrays hold: `n` 0 where its rows are not rows of the call.
 struct PagedRequest {
   int start, n, length;

@@ -39,23 +39,19 @@ __global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a)
   const int group_of = lane >> 4, column = lane & 15, head = blockIdx.y;
   // The request and the tile of its tokens.
   int r = -1, first = 0;
-  for (int base = 0, before = 0; base < op.requests; base += kWave) {
-    int tiles = 0;
+  uint32_t before = 0;
+  for (int base = 0; base < op.requests; base += kWave) {
+    uint32_t tiles = 0;
     if (base + lane < op.requests) tiles = (RequestOf(op.starts, op.lengths, base + lane, op.tokens, a.most_length).n + a.tokens_a_tile - 1) / a.tokens_a_tile;
-    int upto = tiles;
-#pragma unroll
-    for (int step = 1; step < kWave; step <<= 1) {
-      const int other = __shfl_up(upto, step);
-      if (lane >= step) upto += other;
-    }
-    const uint64_t past = __ballot(before + upto > static_cast<int>(blockIdx.x));
+    const uint32_t upto = WaveSums(tiles);
+    const uint64_t past = __ballot(before + upto > blockIdx.x);
     if (past != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
       r = base + at;
-      first = (static_cast<int>(blockIdx.x) - before - __shfl(upto - tiles, at)) * a.tokens_a_tile;
+      first = static_cast<int>(blockIdx.x - before - __builtin_amdgcn_readlane(upto - tiles, at)) * a.tokens_a_tile;
       break;
     }
-    before += __shfl(upto, kWave - 1);
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   if (r < 0) return;
   const PagedRequest q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
@@ -64,6 +60,48 @@ __global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a)
   if (q.length - q.n + last < 0 || static_cast<int>(blockIdx.z) * kScoreWaves * 16 >= pages) return;
   const int32_t* const table = op.table + r * op.table_stride;
 
+  // The columns' queries as codes, those above zero and those below apart.
+  I32x4 up[kSteps], down[kSteps];
+  float unit;
+  bool real;
+  const auto query = [&](int h0) {
+    const int token = first + (a.tokens_a_tile > 1 ? column / a.group : 0);
+    const int query_head = a.tokens_a_tile > 1 ? column % a.group : h0 + column;
+    real = token <= last && query_head < a.group;
+    QueryPart<TYPE, 2 * kSteps> part;
+    const int64_t start = (q.start + (real ? token : first)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * group_of;
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) part.Load(op.q, i, start + 64 * (i / 2) + 8 * (i % 2));
+    const uint32_t bits = AcrossGroupsMost(part.MostBits());
+    constexpr uint32_t kInfinity = TYPE == LLMP_X_F32 ? 0x7F800000u : TYPE == LLMP_X_BF16 ? 0x7F80u : 0x7C00u;
+    const float most = TYPE == LLMP_X_F32 ? __builtin_bit_cast(float, bits) : TYPE == LLMP_X_BF16 ? Bf16BitsToFloat(bits) : HalfBitsToFloat(bits);
+    const float scale = bits >= kInfinity ? 0.0f : most * (1.0f / 127.0f), inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
+    unit = bits >= kInfinity ? __builtin_nanf("") : scale;
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) {
+      float v[8];
+      int code[8];
+      float four[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        part.Four(i, k, four);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * k + e] = four[e];
+      }
+      CodesOf(v, scale, inverse, code);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t positive = 0, negative = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          positive |= static_cast<uint32_t>(max(code[4 * k + e], 0)) << (8 * e);
+          negative |= static_cast<uint32_t>(min(code[4 * k + e], 0) & 0xFF) << (8 * e);
+        }
+        up[i / 2][2 * (i % 2) + k] = static_cast<int>(positive), down[i / 2][2 * (i % 2) + k] = static_cast<int>(negative);
+      }
+    }
+  };
+  bool made = false;
   for (int from = (blockIdx.z * kScoreWaves + wave) * 16; from < pages; from += gridDim.z * kScoreWaves * 16) {
     // The lane's page row: its low and high codes.
     const int row = min(from + column, pages - 1);
@@ -79,47 +117,13 @@ __global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a)
     const float page_scale = c.k_scale[static_cast<int64_t>(page) * c.kv_heads + head];
     float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of column groups, more than one where a KV head has over 16 heads
     for (int h0 = 0; h0 < a.group; h0 += 16) {
-      const int token = first + (a.tokens_a_tile > 1 ? column / a.group : 0);
-      const int query_head = a.tokens_a_tile > 1 ? column % a.group : h0 + column;
-      const bool real = token <= last && query_head < a.group;
-      float x[kSteps][16];
-      float most = 0.0f;
-      bool finite = true;
-      const int64_t start = (q.start + (real ? token : first)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float v[8];
-          LoadEight<TYPE>(op.q, start + 64 * s + 16 * group_of + 8 * half, v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[s][8 * half + e] = v[e];
-            finite = finite && fabsf(v[e]) <= 3.402823466e38f;
-            most = fmaxf(most, fabsf(v[e]));
-          }
-        }
-      }
-      most = AcrossGroupsMax(most);
-      const bool bad = AcrossGroupsMax(finite ? 0.0f : 1.0f) > 0.0f;
-      const float unit = bad ? __builtin_nanf("") : most * (1.0f / 127.0f);
+      if (!made || a.group > 16) query(h0);
+      made = true;
       I32x4 sum = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        I32x4 up, down;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t positive = 0, negative = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int code = unit > 0.0f ? static_cast<int>(fminf(fmaxf(rintf(x[s][4 * w + e] / unit), -127.0f), 127.0f)) : 0;
-            positive |= static_cast<uint32_t>(max(code, 0)) << (8 * e);
-            negative |= static_cast<uint32_t>(min(code, 0) & 0xFF) << (8 * e);
-          }
-          up[w] = static_cast<int>(positive), down[w] = static_cast<int>(negative);
-        }
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[s], up, sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[s], down, sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[s], up[s], sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[s], down[s], sum, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -151,19 +155,18 @@ __device__ __forceinline__ uint32_t KeyOf(float score) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// Flags' exclusive count over the workgroup in thread order, and their number.
-__device__ __forceinline__ int BlockCount(bool flag, int* shared, int* all) {
+// A count's exclusive sum over the workgroup in thread order, and the whole; `shared` another four words each time.
+__device__ __forceinline__ int BlockSum(int count, int* shared, int* all) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const uint64_t set = __ballot(flag);
-  if (lane == 0) shared[wave] = __popcll(set);
+  const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(count)));
+  if (lane == kWave - 1) shared[wave] = upto;
   __syncthreads();
-  int before = __popcll(set & ((1ull << lane) - 1));
-  int total = 0;
+  int before = upto - count, total = 0;
+#pragma unroll
   for (int w = 0; w < kPickThreads / kWave; ++w) {
     before += w < wave ? shared[w] : 0;
     total += shared[w];
   }
-  __syncthreads();
   *all = total;
   return before;
 }
@@ -171,7 +174,7 @@ __device__ __forceinline__ int BlockCount(bool flag, int* shared, int* all) {
 // grid (tokens, KV heads).
 __global__ __launch_bounds__(kPickThreads) void PickKernel(const SelectArgs a) {
   __shared__ uint32_t kept[kPickKeys];
-  __shared__ int bins[256], shared[kPickThreads / kWave], found[2];
+  __shared__ int bins[4][256], shared[2][kPickThreads / kWave], found[4][3];
   const llmp_paged_select& op = a.op;
   const int token = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1);
   int32_t* const list = op.lists + (static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.keep;
@@ -193,63 +196,62 @@ __global__ __launch_bounds__(kPickThreads) void PickKernel(const SelectArgs a) {
     return;
   }
   const float* const scores = a.scores + (static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.table_width;
-  const auto key_at = [&](int j) { return j < op.first || j >= pages - op.recent ? ~0u : KeyOf(scores[j]); };
+  const auto key_of = [&](int j) { return j < op.first || j >= pages - op.recent ? ~0u : KeyOf(scores[j]); };
   const bool in_lds = pages <= kPickKeys;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bins[i][tid] = 0;
   if (in_lds) {
-    for (int j = tid; j < pages; j += kPickThreads) kept[j] = key_at(j);
+#pragma unroll 4
+    for (int j = tid; j < pages; j += kPickThreads) kept[j] = key_of(j);
   }
-  // The keep-th largest key, its highest bits first: `want` of the keys that share the bits found so far are still to choose.
-  uint32_t prefix = 0;
+  __syncthreads();
+  const auto key_at = [&](int j) { return in_lds ? kept[j] : key_of(j); };
+  // The keep-th largest key, its highest bits first, until all of the keys that share the bits found so far are to be chosen:
+  // `want` of them are.
+  uint32_t prefix = 0, mask = 0;
   int want = op.keep;
 #pragma unroll
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    bins[tid] = 0;
-    __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
+  for (int i = 0; i < 4; ++i) {
+    const int shift = 24 - 8 * i;
     for (int j = tid; j < pages; j += kPickThreads) {
-      const uint32_t key = in_lds ? kept[j] : key_at(j);
-      if ((key & mask) == prefix) atomicAdd(&bins[(key >> shift) & 0xFF], 1);
+      const uint32_t key = key_at(j);
+      if ((key & mask) == prefix) atomicAdd(&bins[i][(key >> shift) & 0xFF], 1);
     }
     __syncthreads();
     if (tid < kWave) {  // from the top bin down: the one in which the count passes `want`
       int four[4], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) four[i] = bins[255 - 4 * lane - i], sum += four[i];
-      int upto = sum;
-#pragma unroll
-      for (int step = 1; step < kWave; step <<= 1) {
-        const int other = __shfl_up(upto, step);
-        if (lane >= step) upto += other;
-      }
+      for (int e = 0; e < 4; ++e) four[e] = bins[i][255 - 4 * lane - e], sum += four[e];
+      const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(sum)));
       int above = upto - sum;
       if (above < want && upto >= want) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (above < want && above + four[i] >= want) {
-            found[0] = 255 - 4 * lane - i;
-            found[1] = want - above;
-          }
-          above += four[i];
+        for (int e = 0; e < 4; ++e) {
+          if (above < want && above + four[e] >= want) found[i][0] = 255 - 4 * lane - e, found[i][1] = want - above, found[i][2] = four[e];
+          above += four[e];
         }
       }
     }
     __syncthreads();
-    prefix |= static_cast<uint32_t>(found[0]) << shift;
-    want = found[1];
+    prefix |= static_cast<uint32_t>(found[i][0]) << shift;
+    mask |= 0xFFu << shift;
+    want = found[i][1];
+    if (found[i][2] == want) break;
   }
-  // In order: all above the key found, and the first `want` that equal it.
-  int written = 0, equal_before = 0;
-  for (int base = 0; base < pages; base += kPickThreads) {
-    const int j = base + tid;
-    const uint32_t key = j < pages ? (in_lds ? kept[j] : key_at(j)) : 0u;
-    const bool equal = j < pages && key == prefix;
-    int all;
-    const int rank = equal_before + BlockCount(equal, shared, &all);
-    equal_before += all;
-    const bool chosen = j < pages && (key > prefix || (equal && rank < want));
-    const int to = written + BlockCount(chosen, shared, &all);
-    written += all;
-    if (chosen && to < op.keep) list[to] = j;
+  // In order, a run of pages a thread: all above the bits found, and the first `want` of those that have them.
+  const int run = (pages + kPickThreads - 1) / kPickThreads, from = min(tid * run, pages), to = min(from + run, pages);
+  int equal = 0, larger = 0, all;
+  for (int j = from; j < to; ++j) {
+    const uint32_t key = key_at(j) & mask;
+    equal += key == prefix, larger += key > prefix;
+  }
+  int rank = BlockSum(equal, shared[0], &all);
+  const int chosen = larger + min(max(want - rank, 0), equal);
+  int at = BlockSum(chosen, shared[1], &all);
+  for (int j = from; j < to; ++j) {
+    const uint32_t key = key_at(j) & mask;
+    if ((key > prefix || (key == prefix && rank < want)) && at < op.keep) list[at++] = j;
+    rank += key == prefix;
   }
 }
 

@@ -37,11 +37,7 @@ __device__ __forceinline__ float BlockMax(float v, float* shared) {
   return all;
 }
 
-// A value's code at a scale; a held code's at a higher one (`factor`, the old scale over the new).
-__device__ __forceinline__ int CodeOf(float x, float scale) {
-  const float q = scale > 0.0f ? rintf(x / scale) : 0.0f;
-  return __builtin_isnan(q) ? 0 : static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
-}
+// A held code's at a higher scale (`factor`, the old scale over the new).
 __device__ __forceinline__ int CodeAgain(int code, float factor) { return static_cast<int>(rintf(static_cast<float>(code) * factor)); }
 __device__ __forceinline__ int ByteOf(uint32_t word, int i) { return static_cast<int8_t>(word >> (8 * i)); }
 
@@ -93,7 +89,7 @@ __global__ __launch_bounds__(kStoreThreads) void StoreKernel(const llmp_paged_st
   const float most = BlockMax(RowsMax<TYPE, D>(x, first, token_stride, it.count), shared);  // (its barrier: every thread has read *scale_at)
   const float scale = fmaxf(before, most * (1.0f / 127.0f));
   const bool rises = it.held > 0 && scale > before;
-  const float factor = rises ? before / scale : 1.0f;
+  const float factor = rises ? before / scale : 1.0f, inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
   if (tid == 0) *scale_at = scale;
 
   const int d0 = 8 * (tid % kLanes);
@@ -112,12 +108,13 @@ __global__ __launch_bounds__(kStoreThreads) void StoreKernel(const llmp_paged_st
     for (int i = tid / kLanes; i < it.count; i += kRows) {
       float v[8];
       LoadEight<TYPE>(x, first + i * token_stride + d0, v);
+      int code[8];
+      CodesOf(v, scale, inverse, code);
       uint32_t w[2] = {0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int code = CodeOf(v[e], scale);
-        low[e] = min(low[e], code), high[e] = max(high[e], code);
-        w[e / 4] |= static_cast<uint32_t>(code & 0xFF) << (8 * (e % 4));
+        low[e] = min(low[e], code[e]), high[e] = max(high[e], code[e]);
+        w[e / 4] |= static_cast<uint32_t>(code[e] & 0xFF) << (8 * (e % 4));
       }
       *reinterpret_cast<uint2*>(codes + (it.held + i) * D + d0) = make_uint2(w[0], w[1]);
     }
@@ -146,8 +143,10 @@ __global__ __launch_bounds__(kStoreThreads) void StoreKernel(const llmp_paged_st
   for (int i = tid / kLanes; i < it.count; i += kRows) {
     float v[8];
     LoadEight<TYPE>(x, first + i * token_stride + d0, v);
+    int code[8];
+    CodesOf(v, scale, inverse, code);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) turned[(d0 + e) * pitch + it.held + i] = static_cast<uint8_t>(CodeOf(v[e], scale));
+    for (int e = 0; e < 8; ++e) turned[(d0 + e) * pitch + it.held + i] = static_cast<uint8_t>(code[e]);
   }
   __syncthreads();
   uint8_t* const codes = static_cast<uint8_t*>(c.v) + page_head * c.page * D;
