@@ -47,6 +47,12 @@ __device__ __forceinline__ void LoadEight(const void* base, int64_t element, flo
     }
   }
 }
+template <int TYPE>
+__device__ __forceinline__ float LoadOne(const void* base, int64_t element) {
+  if constexpr (TYPE == LLMP_X_F32) return static_cast<const float*>(base)[element];
+  const uint32_t bits = static_cast<const uint16_t*>(base)[element];
+  return TYPE == LLMP_X_BF16 ? Bf16BitsToFloat(bits) : HalfBitsToFloat(bits);
+}
 // N consecutive floats rounded once to the type (N a multiple of 4, at a boundary of N elements or 16 bytes).
 template <int TYPE, int N>
 __device__ __forceinline__ void StoreValues(void* base, int64_t element, const float (&x)[N]) {

@@ -9,7 +9,8 @@
 // products of whole numbers, pages as rows and (token, head) pairs of one KV head as columns
 // (v_mfma_i32_16x16x64_i8); a wave takes 16 pages at a time. What bounds it is the codes' bytes, 2 * head_dim a page and head.
 // Second launch, the choice: a workgroup a (token, KV head) finds the keep-th largest score by its bits, eight at a time
-// (a histogram a pass), and writes the pages at or above it in order; ties go to the lower page.
+// (a histogram a pass), and writes the pages at or above it in order; ties go to the lower page. Where there are workgroups enough
+// for the card, both are one launch and the scores stay in LDS.
 #include "paged_attend.h"
 
 namespace llmp_hip {
@@ -17,6 +18,8 @@ namespace {
 
 constexpr int kScoreWaves = 4;
 constexpr int kScoreThreads = kScoreWaves * kWave;
+constexpr int kWholeWaves = 16;
+constexpr int kWholeThreads = kWholeWaves * kWave;
 constexpr int kPickThreads = 256;
 constexpr int kPickKeys = 8192;  // scores a workgroup keeps in LDS; more are read from scratch again
 constexpr int kMostKeep = 4096;
@@ -28,50 +31,86 @@ struct SelectArgs {
   int tokens_a_tile;  // tokens whose heads fill the 16 columns
 };
 
-// grid (tiles of tokens, KV heads, blocks of pages).
-template <int TYPE, int D>
-__global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a) {
-  constexpr int kSteps = D / 64;
-  __shared__ float tile[kScoreWaves][16][17];  // [column][page]
+// A tile of a request's tokens: which, and how many pages its last one has.
+struct TokenTile {
+  PagedRequest q;
+  int request, first, last, pages;
+};
+// Tile `index` of all requests' (request -1: none).
+__device__ __forceinline__ TokenTile TileOf(const SelectArgs& a, uint32_t index) {
   const llmp_paged_select& op = a.op;
-  const llmp_paged_cache& c = op.cache;
-  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int group_of = lane >> 4, column = lane & 15, head = blockIdx.y;
-  // The request and the tile of its tokens.
-  int r = -1, first = 0;
+  const int lane = threadIdx.x & (kWave - 1);
+  TokenTile t = {};
+  t.request = -1;
   uint32_t before = 0;
   for (int base = 0; base < op.requests; base += kWave) {
     uint32_t tiles = 0;
-    if (base + lane < op.requests) tiles = (RequestOf(op.starts, op.lengths, base + lane, op.tokens, a.most_length).n + a.tokens_a_tile - 1) / a.tokens_a_tile;
+    PagedRequest q = {};
+    if (base + lane < op.requests) {
+      q = RequestOf(op.starts, op.lengths, base + lane, op.tokens, a.most_length);
+      tiles = (q.n + a.tokens_a_tile - 1) / a.tokens_a_tile;
+    }
     const uint32_t upto = WaveSums(tiles);
-    const uint64_t past = __ballot(before + upto > blockIdx.x);
+    const uint64_t past = __ballot(before + upto > index);
     if (past != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      r = base + at;
-      first = static_cast<int>(blockIdx.x - before - __builtin_amdgcn_readlane(upto - tiles, at)) * a.tokens_a_tile;
+      t.request = base + at;
+      t.first = static_cast<int>(index - before - __builtin_amdgcn_readlane(upto - tiles, at)) * a.tokens_a_tile;
+      t.q = {__builtin_amdgcn_readlane(q.start, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.length, at)};
+      t.last = min(t.first + a.tokens_a_tile, t.q.n) - 1;
+      const int position = t.q.length - t.q.n + t.last;
+      t.pages = position < 0 ? 0 : min(position / op.cache.page + 1, op.table_width);
       break;
     }
     before += __builtin_amdgcn_readlane(upto, kWave - 1);
   }
-  if (r < 0) return;
-  const PagedRequest q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
-  const int last = min(first + a.tokens_a_tile, q.n) - 1;
-  const int pages = min((q.length - q.n + last) / c.page + 1, op.table_width);  // the last token's
-  if (q.length - q.n + last < 0 || static_cast<int>(blockIdx.z) * kScoreWaves * 16 >= pages) return;
-  const int32_t* const table = op.table + r * op.table_stride;
+  return t;
+}
 
-  // The columns' queries as codes, those above zero and those below apart.
-  I32x4 up[kSteps], down[kSteps];
+// A wave's scores of 16 pages at a time; TAKEN: with queries that the workgroup's waves made once, a group of at most 16 heads.
+template <int TYPE, int D, bool TAKEN>
+struct Scorer {
+  static constexpr int kSteps = D / 64;
+  const SelectArgs& a;
+  const TokenTile& t;
+  const int head, lane, group_of, column;
+  const int32_t* const table;
+  I32x4 up[kSteps], down[kSteps];  // the columns' queries as codes, those above zero and those below apart
   float unit;
-  bool real;
-  const auto query = [&](int h0) {
-    const int token = first + (a.tokens_a_tile > 1 ? column / a.group : 0);
-    const int query_head = a.tokens_a_tile > 1 ? column % a.group : h0 + column;
-    real = token <= last && query_head < a.group;
-    QueryPart<TYPE, 2 * kSteps> part;
-    const int64_t start = (q.start + (real ? token : first)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * group_of;
+  bool real, again = false;  // again: the first heads' codes have made way for others'
+  struct Pages {
+    I32x4 low[kSteps], high[kSteps];
+    float scale;
+  };
+
+  __device__ __forceinline__ Scorer(const SelectArgs& args, const TokenTile& tile, int kv_head)
+      : a(args), t(tile), head(kv_head), lane(threadIdx.x & (kWave - 1)), group_of(lane >> 4), column(lane & 15),
+        table(args.op.table + tile.request * args.op.table_stride) {}
+
+  __device__ __forceinline__ int Entry(int from) const { return table[min(from + column, t.pages - 1)]; }
+  // The lane's page row: its low and high codes.
+  __device__ __forceinline__ void Load(int page, Pages* to) const {
+    const llmp_paged_cache& c = a.op.cache;
+    if (page < 0 || page >= c.pages) page = 0;
+    const int64_t page_head = static_cast<int64_t>(page) * c.kv_heads + head, at = page_head * D + 16 * group_of;
 #pragma unroll
-    for (int i = 0; i < 2 * kSteps; ++i) part.Load(op.q, i, start + 64 * (i / 2) + 8 * (i % 2));
+    for (int s = 0; s < kSteps; ++s) {
+      to->low[s] = *reinterpret_cast<const I32x4*>(static_cast<const uint8_t*>(c.low) + at + 64 * s);
+      to->high[s] = *reinterpret_cast<const I32x4*>(static_cast<const uint8_t*>(c.high) + at + 64 * s);
+    }
+    to->scale = c.k_scale[page_head];
+  }
+  // The columns' queries, heads h0 on of the group: asked for, and as codes.
+  __device__ __forceinline__ void Ask(int h0, QueryPart<TYPE, 2 * kSteps>* part) {
+    const llmp_paged_select& op = a.op;
+    const int token = t.first + (a.tokens_a_tile > 1 ? column / a.group : 0);
+    const int query_head = a.tokens_a_tile > 1 ? column % a.group : h0 + column;
+    real = token <= t.last && query_head < a.group;
+    const int64_t start = (t.q.start + (real ? token : t.first)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * group_of;
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) part->Load(op.q, i, start + 64 * (i / 2) + 8 * (i % 2));
+  }
+  __device__ __forceinline__ void Codes(const QueryPart<TYPE, 2 * kSteps>& part) {
     const uint32_t bits = AcrossGroupsMost(part.MostBits());
     constexpr uint32_t kInfinity = TYPE == LLMP_X_F32 ? 0x7F800000u : TYPE == LLMP_X_BF16 ? 0x7F80u : 0x7C00u;
     const float most = TYPE == LLMP_X_F32 ? __builtin_bit_cast(float, bits) : TYPE == LLMP_X_BF16 ? Bf16BitsToFloat(bits) : HalfBitsToFloat(bits);
@@ -81,9 +120,9 @@ __global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a)
     for (int i = 0; i < 2 * kSteps; ++i) {
       float v[8];
       int code[8];
-      float four[4];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        float four[4];
         part.Four(i, k, four);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * k + e] = four[e];
@@ -100,52 +139,83 @@ __global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a)
         up[i / 2][2 * (i % 2) + k] = static_cast<int>(positive), down[i / 2][2 * (i % 2) + k] = static_cast<int>(negative);
       }
     }
-  };
-  bool made = false;
-  for (int from = (blockIdx.z * kScoreWaves + wave) * 16; from < pages; from += gridDim.z * kScoreWaves * 16) {
-    // The lane's page row: its low and high codes.
-    const int row = min(from + column, pages - 1);
-    int page = table[row];
-    if (page < 0 || page >= c.pages) page = 0;
-    const int64_t at = (static_cast<int64_t>(page) * c.kv_heads + head) * D + 16 * group_of;
-    I32x4 low[kSteps], high[kSteps];
+  }
+  // The queries from LDS: [column][D] codes above zero, then those below, and the columns' units.
+  __device__ __forceinline__ void Take(const uint8_t* codes, const float* units) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      low[s] = *reinterpret_cast<const I32x4*>(static_cast<const uint8_t*>(c.low) + at + 64 * s);
-      high[s] = *reinterpret_cast<const I32x4*>(static_cast<const uint8_t*>(c.high) + at + 64 * s);
+      up[s] = *reinterpret_cast<const I32x4*>(codes + column * D + 64 * s + 16 * group_of);
+      down[s] = *reinterpret_cast<const I32x4*>(codes + 16 * D + column * D + 64 * s + 16 * group_of);
     }
-    const float page_scale = c.k_scale[static_cast<int64_t>(page) * c.kv_heads + head];
+    unit = units[column];
+    real = column < a.tokens_a_tile * a.group && t.first + (a.tokens_a_tile > 1 ? column / a.group : 0) <= t.last;
+  }
+  // The scores of pages `from` to from + 15 through `tile` ([column][page], the wave's own): give(token of the tile, page, score).
+  template <class F>
+  __device__ __forceinline__ void Score(int from, const Pages& pages, float (*tile)[17], F&& give) {
     float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of column groups, more than one where a KV head has over 16 heads
-    for (int h0 = 0; h0 < a.group; h0 += 16) {
-      if (!made || a.group > 16) query(h0);
-      made = true;
+    for (int h0 = 0; h0 < (TAKEN ? 1 : a.group); h0 += 16) {
+      if constexpr (!TAKEN) {
+        if (h0 > 0 || again) {
+          QueryPart<TYPE, 2 * kSteps> part;
+          Ask(h0, &part);
+          Codes(part);
+          again = true;
+        }
+      }
       I32x4 sum = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(high[s], up[s], sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(low[s], down[s], sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(pages.high[s], up[s], sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(pages.low[s], down[s], sum, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // (The scale is the page's of the sum's row: row 4 group_of + i's, that lane holds it.)
-        float score = (static_cast<float>(sum[i]) * unit) * __shfl(page_scale, 4 * group_of + i);
+        float score = (static_cast<float>(sum[i]) * unit) * __shfl(pages.scale, 4 * group_of + i);
         if (!real || score != score) score = -INFINITY;
         best[i] = fmaxf(best[i], score);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tile[wave][column][4 * group_of + i] = best[i];
+    for (int i = 0; i < 4; ++i) tile[column][4 * group_of + i] = best[i];
     __builtin_amdgcn_wave_barrier();
     // A lane a (token, page): the largest of the token's columns.
     const int columns = a.tokens_a_tile > 1 ? a.group : 16;
     for (int i = lane; i < a.tokens_a_tile * 16; i += kWave) {
-      const int t = i / 16, p = i % 16;
-      if (first + t > last || from + p >= pages) continue;
+      const int token = i / 16, p = i % 16;
+      if (t.first + token > t.last || from + p >= t.pages) continue;
       float top = -INFINITY;
-      for (int k = 0; k < columns; ++k) top = fmaxf(top, tile[wave][t * columns + k][p]);
-      a.scores[(static_cast<int64_t>(q.start + first + t) * c.kv_heads + head) * op.table_width + from + p] = top;
+      for (int k = 0; k < columns; ++k) top = fmaxf(top, tile[token * columns + k][p]);
+      give(token, from + p, top);
     }
     __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// grid (tiles of tokens, KV heads, blocks of pages).
+template <int TYPE, int D>
+__global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a) {
+  __shared__ float tile[kScoreWaves][16][17];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), head = blockIdx.y;
+  const TokenTile t = TileOf(a, blockIdx.x);
+  if (t.request < 0 || static_cast<int>(blockIdx.z) * kScoreWaves * 16 >= t.pages) return;
+  int from = (blockIdx.z * kScoreWaves + wave) * 16;
+  if (from >= t.pages) return;
+  Scorer<TYPE, D, false> scorer(a, t, head);
+  typename Scorer<TYPE, D, false>::Pages pages;
+  QueryPart<TYPE, D / 32> part;
+  int entry = scorer.Entry(from);
+  scorer.Ask(0, &part);
+  scorer.Load(entry, &pages);
+  scorer.Codes(part);
+  while (true) {
+    scorer.Score(from, pages, tile[wave], [&](int token, int page, float score) {
+      a.scores[(static_cast<int64_t>(t.q.start + t.first + token) * a.op.cache.kv_heads + head) * a.op.table_width + page] = score;
+    });
+    from += gridDim.z * kScoreWaves * 16;
+    if (from >= t.pages) break;
+    scorer.Load(scorer.Entry(from), &pages);
   }
 }
 
@@ -155,28 +225,110 @@ __device__ __forceinline__ uint32_t KeyOf(float score) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// A count's exclusive sum over the workgroup in thread order, and the whole; `shared` another four words each time.
-__device__ __forceinline__ int BlockSum(int count, int* shared, int* all) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(count)));
-  if (lane == kWave - 1) shared[wave] = upto;
-  __syncthreads();
-  int before = upto - count, total = 0;
-#pragma unroll
-  for (int w = 0; w < kPickThreads / kWave; ++w) {
-    before += w < wave ? shared[w] : 0;
-    total += shared[w];
+// What the threads of a share of a workgroup know together in a choice.
+struct Choice {
+  int bins[2][256], found[3];
+  uint32_t least[kWholeWaves], most[kWholeWaves];
+  int sums[2][kWholeWaves];
+};
+// The choice of op.keep of `count` pages (more than that, or 0: no choice) by a share of a workgroup, `threads` threads (whole
+// waves) of which the caller is number `me`: the first and the recent pages, and of the others those with the largest keys, written
+// in order. The workgroup's shares call it together, they meet at its barriers.
+template <class F>
+__device__ __forceinline__ void Choose(const llmp_paged_select& op, int count, int me, int threads, Choice* all, int share, int shares, F&& key_at, int32_t* list) {
+  const int lane = me & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(me / kWave), waves = threads / kWave;
+  Choice& my = all[share];
+  const int begin = count > 0 ? op.first : 0, end = count > 0 ? count - op.recent : 0;
+  for (int i = me; i < 512; i += threads) my.bins[0][i] = 0;
+  uint32_t least = ~0u, most = 0;
+  for (int j = begin + me; j < end; j += threads) {
+    const uint32_t key = key_at(j);
+    least = min(least, key), most = max(most, key);
   }
-  *all = total;
-  return before;
+  least = WaveMinU32(least), most = WaveMaxU32(most);
+  if (lane == 0) my.least[wave] = least, my.most[wave] = most;
+  int want = op.keep - op.first - op.recent;
+  if (me == 0) my.found[2] = count == 0 || want == 0;
+  __syncthreads();
+  for (int w = 0; w < waves; ++w) least = min(least, my.least[w]), most = max(most, my.most[w]);
+  // The want-th largest distance from the least key, its highest bits first (the bounds are mostly of one sign and near each other:
+  // eight bits of the distances tell them apart, where eight bits of the keys are the same few), until all that share the bits
+  // found so far are chosen.
+  uint32_t prefix = ~0u;  // (none wanted: no distance lies above)
+  int low = most > least ? 32 - __clz(most - least) : 0;
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    bool over = true;
+    for (int i = 0; i < shares; ++i) over = over && all[i].found[2] != 0;
+    if (over) break;
+    const bool mine = my.found[2] == 0;
+    const int upper = low, next = max(upper - 8, 0);
+    if (mine) {
+      const uint32_t digits = (1u << (upper - next)) - 1;
+      for (int j = begin + me; j < end; j += threads) {
+        const uint32_t d = key_at(j) - least;
+        if (pass == 0 || (d >> upper) == prefix) atomicAdd(&my.bins[pass & 1][(d >> next) & digits], 1);
+      }
+    }
+    if (pass > 0) {
+      for (int i = me; i < 256; i += threads) my.bins[(pass + 1) & 1][i] = 0;
+    }
+    __syncthreads();
+    if (mine && wave == 0) {  // from the top bin down: the one in which the count passes `want`
+      int four[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) four[e] = my.bins[pass & 1][255 - 4 * lane - e], sum += four[e];
+      const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(sum)));
+      int above = upto - sum;
+      if (above < want && upto >= want) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (above < want && above + four[e] >= want) {
+            my.found[0] = 255 - 4 * lane - e, my.found[1] = want - above;
+            my.found[2] = above + four[e] == want || next == 0;
+          }
+          above += four[e];
+        }
+      }
+    }
+    __syncthreads();
+    if (mine) {
+      prefix = (pass == 0 ? 0u : prefix << (upper - next)) | static_cast<uint32_t>(my.found[0]);
+      want = my.found[1];
+      low = next;
+    }
+  }
+  // In order, a run of pages a thread: all above the bits found, and the first `want` of those that have them.
+  const auto forced = [&](int j) { return j < begin || j >= end; };
+  const int run = (count + threads - 1) / threads, from = min(me * run, count), to = min(from + run, count);
+  int equal = 0, larger = 0;
+  for (int j = from; j < to; ++j) {
+    const uint32_t d = forced(j) ? 0u : (key_at(j) - least) >> low;
+    larger += forced(j) || d > prefix, equal += !forced(j) && d == prefix;
+  }
+  const auto before = [&](int value, int* sums) {  // the share's sum up to this thread
+    const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(value)));
+    if (lane == kWave - 1) sums[wave] = upto;
+    __syncthreads();
+    int sum = upto - value;
+    for (int w = 0; w < wave; ++w) sum += sums[w];
+    return sum;
+  };
+  int rank = before(equal, my.sums[0]);
+  int at = before(larger + min(max(want - rank, 0), equal), my.sums[1]);
+  for (int j = from; j < to; ++j) {
+    const uint32_t d = forced(j) ? 0u : (key_at(j) - least) >> low;
+    if ((forced(j) || d > prefix || (d == prefix && rank < want)) && at < op.keep) list[at++] = j;
+    rank += !forced(j) && d == prefix;
+  }
 }
 
 // grid (tokens, KV heads).
 __global__ __launch_bounds__(kPickThreads) void PickKernel(const SelectArgs a) {
   __shared__ uint32_t kept[kPickKeys];
-  __shared__ int bins[4][256], shared[2][kPickThreads / kWave], found[4][3];
+  __shared__ Choice choice;
   const llmp_paged_select& op = a.op;
-  const int token = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int token = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   int32_t* const list = op.lists + (static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.keep;
   // The token's request: the last that starts at or before it.
   int low = 0, high = op.requests;
@@ -196,74 +348,119 @@ __global__ __launch_bounds__(kPickThreads) void PickKernel(const SelectArgs a) {
     return;
   }
   const float* const scores = a.scores + (static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.table_width;
-  const auto key_of = [&](int j) { return j < op.first || j >= pages - op.recent ? ~0u : KeyOf(scores[j]); };
-  const bool in_lds = pages <= kPickKeys;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bins[i][tid] = 0;
-  if (in_lds) {
+  if (pages <= kPickKeys) {
+    // (A thread reads its own keys only until the choice's first barrier.)
 #pragma unroll 4
-    for (int j = tid; j < pages; j += kPickThreads) kept[j] = key_of(j);
-  }
-  __syncthreads();
-  const auto key_at = [&](int j) { return in_lds ? kept[j] : key_of(j); };
-  // The keep-th largest key, its highest bits first, until all of the keys that share the bits found so far are to be chosen:
-  // `want` of them are.
-  uint32_t prefix = 0, mask = 0;
-  int want = op.keep;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int shift = 24 - 8 * i;
-    for (int j = tid; j < pages; j += kPickThreads) {
-      const uint32_t key = key_at(j);
-      if ((key & mask) == prefix) atomicAdd(&bins[i][(key >> shift) & 0xFF], 1);
-    }
+    for (int j = tid; j < pages; j += kPickThreads) kept[j] = KeyOf(scores[j]);
     __syncthreads();
-    if (tid < kWave) {  // from the top bin down: the one in which the count passes `want`
-      int four[4], sum = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) four[e] = bins[i][255 - 4 * lane - e], sum += four[e];
-      const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(sum)));
-      int above = upto - sum;
-      if (above < want && upto >= want) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (above < want && above + four[e] >= want) found[i][0] = 255 - 4 * lane - e, found[i][1] = want - above, found[i][2] = four[e];
-          above += four[e];
-        }
-      }
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(found[i][0]) << shift;
-    mask |= 0xFFu << shift;
-    want = found[i][1];
-    if (found[i][2] == want) break;
-  }
-  // In order, a run of pages a thread: all above the bits found, and the first `want` of those that have them.
-  const int run = (pages + kPickThreads - 1) / kPickThreads, from = min(tid * run, pages), to = min(from + run, pages);
-  int equal = 0, larger = 0, all;
-  for (int j = from; j < to; ++j) {
-    const uint32_t key = key_at(j) & mask;
-    equal += key == prefix, larger += key > prefix;
-  }
-  int rank = BlockSum(equal, shared[0], &all);
-  const int chosen = larger + min(max(want - rank, 0), equal);
-  int at = BlockSum(chosen, shared[1], &all);
-  for (int j = from; j < to; ++j) {
-    const uint32_t key = key_at(j) & mask;
-    if ((key > prefix || (key == prefix && rank < want)) && at < op.keep) list[at++] = j;
-    rank += key == prefix;
+    Choose(op, pages, tid, kPickThreads, &choice, 0, 1, [&](int j) { return kept[j]; }, list);
+  } else {
+    Choose(op, pages, tid, kPickThreads, &choice, 0, 1, [&](int j) { return KeyOf(scores[j]); }, list);
   }
 }
 
+// One launch: a workgroup scores a tile of tokens in one KV head, its keys in LDS ([token][table_width]), and picks from them, a
+// token of the tile a share of the waves. grid (tiles of tokens, KV heads).
 template <int TYPE, int D>
-void LaunchScore(const SelectArgs& args, dim3 grid, hipStream_t stream) {
-  hipLaunchKernelGGL((ScoreKernel<TYPE, D>), grid, dim3(kScoreThreads), 0, stream, args);
+__global__ __launch_bounds__(kWholeThreads) void WholeKernel(const SelectArgs a, int shares) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t keys[];
+  __shared__ float tile[kWholeWaves][16][17];
+  __shared__ Choice choices[16];
+  __shared__ __attribute__((aligned(16))) uint8_t codes[2 * 16 * D];
+  __shared__ float units[kWholeWaves];
+  const llmp_paged_select& op = a.op;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), head = blockIdx.y;
+  if (blockIdx.x == 0) {  // rows of no request
+    const int begin = op.starts[0], end = max(op.starts[op.requests], 0);
+    for (int token = 0; token < op.tokens; ++token) {
+      if (token >= begin && token < end) token = end;
+      if (token >= op.tokens) break;
+      for (int i = tid; i < op.keep; i += kWholeThreads) op.lists[(static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.keep + i] = -1;
+    }
+  }
+  const TokenTile t = TileOf(a, blockIdx.x);
+  if (t.request < 0) return;
+  if (t.pages > op.keep) {
+    Scorer<TYPE, D, true> scorer(a, t, head);
+    // A wave a column: its query's codes, for all the waves (one launch: no group of more than 16).
+    constexpr int kPer = D / kWave;
+    const int token = t.first + wave / a.group;
+    const bool real = wave < a.tokens_a_tile * a.group && token <= t.last;
+    const int64_t at = (t.q.start + (real ? token : t.first)) * op.q_token_stride + (head * a.group + (real ? wave % a.group : 0)) * op.q_head_stride + kPer * lane;
+    float v[kPer];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      v[e] = LoadOne<TYPE>(op.q, at + e);
+      bits = max(bits, __builtin_bit_cast(uint32_t, v[e]) & 0x7FFFFFFFu);
+    }
+    bits = WaveMaxU32(bits);
+    const bool bad = bits >= 0x7F800000u;
+    const float unit = bad ? 0.0f : __builtin_bit_cast(float, bits) * (1.0f / 127.0f);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int code = unit > 0.0f ? static_cast<int>(fminf(fmaxf(rintf(v[e] / unit), -127.0f), 127.0f)) : 0;
+      codes[wave * D + kPer * lane + e] = static_cast<uint8_t>(max(code, 0));
+      codes[16 * D + wave * D + kPer * lane + e] = static_cast<uint8_t>(min(code, 0));
+    }
+    if (lane == 0) units[wave] = bad ? __builtin_nanf("") : unit;
+    __syncthreads();
+    if (16 * wave < t.pages) {
+      typename Scorer<TYPE, D, true>::Pages pages;
+      scorer.Take(codes, units);
+      int entry = scorer.Entry(16 * wave);
+      for (int from = 16 * wave; from < t.pages; from += 16 * kWholeWaves) {
+        scorer.Load(entry, &pages);
+        entry = scorer.Entry(from + 16 * kWholeWaves);
+        scorer.Score(from, pages, tile[wave], [&](int token, int page, float score) { keys[token * op.table_width + page] = KeyOf(score); });
+      }
+    }
+  }
+  __syncthreads();
+  const int threads = kWholeThreads / shares, share = tid / threads, me = tid - share * threads;
+  const bool mine = t.first + share <= t.last;
+  const int position = t.q.length - t.q.n + t.first + share;
+  const int pages = !mine || position < 0 ? 0 : min(position / op.cache.page + 1, op.table_width);
+  int32_t* const list = op.lists + (static_cast<int64_t>(t.q.start + t.first + (mine ? share : 0)) * op.cache.kv_heads + head) * op.keep;
+  if (mine && pages <= op.keep) {
+    for (int i = me; i < op.keep; i += threads) list[i] = i < pages ? i : -1;
+  }
+  if (t.pages <= op.keep) return;  // (every token's: the tile's last has the most)
+  const uint32_t* const key = keys + share * op.table_width;
+  Choose(op, pages > op.keep ? pages : 0, me, threads, choices, share, shares, [&](int j) { return key[j]; }, list);
+}
+
+// One launch where its workgroups, one a (tile of tokens, KV head), are at least half as many as the card's 256 compute units and hold
+// their keys in LDS: fewer leave the card idle while one reads a whole row's codes, and more spare the scores' way through memory
+// and each (token, page)'s part of a wave. In us, two launches against one, 8 KV heads of 128, pages of 16, 1024 a row: groups of 8, one
+// token of 1, 8, 32, 64 requests 12.6/18.0, 18.3/18.3, 38.6/25.6, 63.7/37.6 (8 requests of unlike lengths 17/24); groups of 4,
+// 4 tokens of 8 and 32 requests 25.3/22.4, 46.2/34.6, 100 of 8 215/97; groups of 1, 16 tokens of 8 and 64 28.5/37.0, 122/79.
+constexpr int kWholeWorkgroups = 128, kWholeKeys = 16384;
+bool IsWhole(const SelectArgs& a, int64_t tiles) {
+  return a.group <= 16 && tiles * a.op.cache.kv_heads >= kWholeWorkgroups && static_cast<int64_t>(a.tokens_a_tile) * a.op.table_width <= kWholeKeys;
+}
+
+template <int TYPE, int D>
+void LaunchSelect(const SelectArgs& args, int64_t tiles, hipStream_t stream) {
+  const llmp_paged_select& op = args.op;
+  if (IsWhole(args, tiles)) {
+    const int lds = args.tokens_a_tile * op.table_width * 4;
+    static bool sized = false;
+    if (!AllowLds(reinterpret_cast<const void*>(&WholeKernel<TYPE, D>), kWholeKeys * 4, &sized)) return;
+    int shares = 1;
+    while (shares < args.tokens_a_tile) shares *= 2;
+    hipLaunchKernelGGL((WholeKernel<TYPE, D>), dim3(static_cast<unsigned>(tiles), op.cache.kv_heads), dim3(kWholeThreads), lds, stream, args, shares);
+    return;
+  }
+  const int blocks = (op.table_width + 16 * kScoreWaves - 1) / (16 * kScoreWaves);
+  hipLaunchKernelGGL((ScoreKernel<TYPE, D>), dim3(static_cast<unsigned>(tiles), op.cache.kv_heads, blocks < 1024 ? blocks : 1024), dim3(kScoreThreads), 0, stream,
+                     args);
 }
 template <int TYPE>
-void LaunchScoreOf(const SelectArgs& args, dim3 grid, hipStream_t stream) {
-  if (args.op.cache.head_dim == 64) LaunchScore<TYPE, 64>(args, grid, stream);
-  if (args.op.cache.head_dim == 128) LaunchScore<TYPE, 128>(args, grid, stream);
-  if (args.op.cache.head_dim == 256) LaunchScore<TYPE, 256>(args, grid, stream);
+void LaunchSelectOf(const SelectArgs& args, int64_t tiles, hipStream_t stream) {
+  if (args.op.cache.head_dim == 64) LaunchSelect<TYPE, 64>(args, tiles, stream);
+  if (args.op.cache.head_dim == 128) LaunchSelect<TYPE, 128>(args, tiles, stream);
+  if (args.op.cache.head_dim == 256) LaunchSelect<TYPE, 256>(args, tiles, stream);
 }
 
 int CheckSelect(const llmp_paged_select* op) {
@@ -311,14 +508,14 @@ extern "C" int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch,
   args.tokens_a_tile = args.group >= 16 ? 1 : 16 / args.group;
   if (args.tokens_a_tile > op->most_tokens) args.tokens_a_tile = op->most_tokens;
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (op->table_width > op->keep) {  // otherwise every page is chosen
-    const int64_t tiles = static_cast<int64_t>(op->requests) + op->tokens / args.tokens_a_tile;
-    const int blocks = (op->table_width + 16 * kScoreWaves - 1) / (16 * kScoreWaves);
-    const dim3 grid(static_cast<unsigned>(tiles < op->tokens ? tiles : op->tokens), op->cache.kv_heads, blocks < 1024 ? blocks : 1024);
-    if (op->type == LLMP_X_F32) LaunchScoreOf<LLMP_X_F32>(args, grid, on);
-    if (op->type == LLMP_X_BF16) LaunchScoreOf<LLMP_X_BF16>(args, grid, on);
-    if (op->type == LLMP_X_F16) LaunchScoreOf<LLMP_X_F16>(args, grid, on);
+  const int64_t most_tiles = static_cast<int64_t>(op->requests) + op->tokens / args.tokens_a_tile;
+  const int64_t tiles = most_tiles < op->tokens ? most_tiles : op->tokens;
+  const bool scored = op->table_width > op->keep;  // otherwise every page is chosen
+  if (scored) {
+    if (op->type == LLMP_X_F32) LaunchSelectOf<LLMP_X_F32>(args, tiles, on);
+    if (op->type == LLMP_X_BF16) LaunchSelectOf<LLMP_X_BF16>(args, tiles, on);
+    if (op->type == LLMP_X_F16) LaunchSelectOf<LLMP_X_F16>(args, tiles, on);
   }
-  hipLaunchKernelGGL(PickKernel, dim3(op->tokens, op->cache.kv_heads), dim3(kPickThreads), 0, on, args);
+  if (!scored || !IsWhole(args, tiles)) hipLaunchKernelGGL(PickKernel, dim3(op->tokens, op->cache.kv_heads), dim3(kPickThreads), 0, on, args);
   return LaunchStatus("paged_select");
 }

@@ -386,6 +386,29 @@ def test_selection_ties_zeros_and_queries_that_are_no_numbers(device):
         same(got, plain.lists(cache, q, table, lengths, starts, keep), f"keep {keep}")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d,page", [(8, 1, 64, 16), (16, 4, 128, 16), (2, 2, 256, 48), (32, 2, 128, 32)])
+def test_selection_of_many_tokens(device, dtype, heads, kv_heads, d, page):
+    """As many rows as one launch takes (above), with requests of no fresh tokens, of one page, and rows of no request."""
+    g = np.random.default_rng(heads + d + page + 1)
+    fresh = ([1, 0, 7, 1, 16, 2, 3, 1] * 24)[:190]
+    fresh[40] = 33
+    held = [max(n, int(g.integers(0, 60 * page))) for n in fresh]
+    held[1], held[9] = 0, 0
+    held[40], held[41] = page * 80, page * 300 - 1
+    cache, table, lengths, starts = serving(g, held, fresh, kv_heads, page, d)
+    tokens = int(starts[-1])
+    qt, q = rounded(g.standard_normal((tokens + 3, heads, d)), dtype)
+    cache["k_scale"][table[41, 100:130]] = 0.5
+    cache["low"][table[41, 100:130]], cache["high"][table[41, 100:130]] = -3, 5
+    q[4, 0, 3] = qt[4, 0, 3] = np.nan
+    q[6], qt[6] = 0.0, 0.0
+    for keep, first, recent in [(1, 0, 1), (9, 0, 0), (20, 3, 4), (6, 2, 4), (70, 1, 1)]:
+        got = ops.paged_select(to_device(cache, device), qt.to(device), dev(table, device), dev(lengths, device), dev(starts, device), keep,
+                               first=first, recent=recent)
+        same(got, plain.lists(cache, q, table, lengths, starts, keep, first, recent), f"keep {keep}")
+
+
 def test_selection_of_more_pages_than_a_workgroup_keeps(device):
     g = np.random.default_rng(72)
     pages = 20011
