@@ -81,6 +81,16 @@ struct Entry {
   bool there;
 };
 
+// Workgroup `block` of `blocks`, of which `used` have work, on the line: the device deals the workgroups to its eight chiplets in
+// turn, each with an L2 of its own, and a chiplet's take a run of the line, since the rows of a (request, KV head), which share its
+// pages, lie side by side there.
+constexpr uint32_t kChiplets = 8;
+__device__ __forceinline__ uint32_t OnChiplet(uint32_t block, uint32_t blocks, uint32_t used) {
+  if (blocks % kChiplets != 0) return block;
+  const uint32_t chiplet = block % kChiplets, slot = block / kChiplets, run = (used + kChiplets - 1) / kChiplets;
+  return slot < run ? chiplet * run + slot : block;  // (run slots of every chiplet come first: the others keep their places)
+}
+
 // grid (workgroups).
 template <int TYPE, int D, bool LISTS>
 __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const PagedAttendArgs a) {
@@ -116,11 +126,12 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
   const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
   uint32_t per = (even + kFewWaves - 1) / kFewWaves * kFewWaves;
   if (even < kFewWaves) per = min(per, max(even, (total + segments - 1) / max(segments, 1u)));
-  uint32_t u = blockIdx.x * per;
+  const uint32_t group = OnChiplet(blockIdx.x, gridDim.x, (total + per - 1) / max(per, 1u));
+  uint32_t u = group * per;
   const uint32_t u_end = min(u + per, total);
   I32x4 part = {-1, 0, 0, 0};
   if (u >= u_end || total >= 1u << 31) {
-    if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * blockIdx.x) = part;
+    if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * group) = part;
     return;
   }
   // The request that holds unit u, and the units before it.
@@ -156,7 +167,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
     const int segment = __builtin_amdgcn_readfirstlane(static_cast<int>((u - before) / a_segment));
     const uint32_t in_segment = u - before - segment * a_segment, u_count = min(a_segment - in_segment, u_end - u);
     const int t_first = static_cast<int>(in_segment << a.shift), t_count = min(f.tiles - t_first, static_cast<int>(u_count << a.shift));
-    const int chunk = segment / c.kv_heads, head = segment - chunk * c.kv_heads;
+    const int chunks = f.segments / c.kv_heads, head = segment / chunks, chunk = segment - head * chunks;
 
     // ---- this lane's query row, and what the segment's rows see.
     int token, query_head, first_token, last_token;
@@ -416,7 +427,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
       *reinterpret_cast<F32x4*>(meet + (wave * kRows + column) * kPitch + 16 * b + 4 * group_of) = out[b];
     __syncthreads();
     const bool begins = t_first == 0, ends = t_first + t_count == f.tiles;
-    float* const slot = a.partial + (2 * static_cast<int64_t>(blockIdx.x) + (begins ? 1 : 0)) * kRows * (D + 2);
+    float* const slot = a.partial + (2 * static_cast<int64_t>(group) + (begins ? 1 : 0)) * kRows * (D + 2);
     for (int i = tid; i < kRows * D / 4; i += kFewThreads) {
       const int row = i / (D / 4), d = 4 * (i % (D / 4));
       float high = -INFINITY, all = 0.0f;
@@ -452,11 +463,11 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
         for (int e = 0; e < 4; ++e) to[2 + d + e] = value[e];
       }
     }
-    if (begins && !ends) part = I32x4{static_cast<int>((before + (segment + 1) * a_segment - 1) / per), f.q.start, segment, f.q.n};
+    if (begins && !ends) part = I32x4{static_cast<int>((before + (segment + 1) * a_segment - 1) / per), f.q.start, chunk * c.kv_heads + head, f.q.n};
     __syncthreads();
     u += u_count;
   }
-  if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * blockIdx.x) = part;
+  if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * group) = part;
 }
 
 // Parts p from 0 to `count` - 1 of a row (top, sum, D values at part_of(p)) as one, the waves taking
@@ -656,11 +667,12 @@ extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch,
   args.group_magic = args.group == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / args.group + 1);
   args.most_length = op->table_width * op->cache.page;
   const bool many = HasMany(*op);
-  args.few_rows = many ? kFewRows : kMostFewRows;
+  const bool alone = many && op->requests == 1 && op->most_tokens >= op->tokens;  // one request: of whatever rows, the many rows' form's
+  args.few_rows = alone ? 0 : many ? kFewRows : kMostFewRows;
   args.shift = FewShift(*op);
   const hipStream_t on = static_cast<hipStream_t>(stream);
   if (many) PagedManyRows(args, static_cast<uint8_t*>(scratch) + FewScratch(op->cache.head_dim, cus), cus, on);
-  if (many && op->requests == 1 && op->most_tokens == op->tokens) return LaunchStatus("paged_attend");  // the one request has been answered
+  if (alone) return LaunchStatus("paged_attend");
   if (op->type == LLMP_X_F32) LaunchFewOf<LLMP_X_F32>(args, groups, on);
   if (op->type == LLMP_X_BF16) LaunchFewOf<LLMP_X_BF16>(args, groups, on);
   if (op->type == LLMP_X_F16) LaunchFewOf<LLMP_X_F16>(args, groups, on);

@@ -239,6 +239,14 @@ def test_prompts_of_odd_lengths(device, dtype, heads, kv_heads, d, page):
         run_attend(device, cache, q, table, lengths, starts, d ** -0.5, dtype, window=window)
 
 
+@pytest.mark.parametrize("fresh", [0, 1, 5, 33, 100])
+def test_one_request_of_fewer_tokens_than_rows(device, fresh):
+    """The rows' count says what may come, the starts what does: a captured step answers both."""
+    g = np.random.default_rng(fresh + 17)
+    cache, table, lengths, starts = serving(g, [300], [fresh], 2, 16, 64)
+    run_attend(device, cache, g.standard_normal((100, 8, 64)), table, lengths, starts, 0.125, "bf16", most=100)
+
+
 def test_rows_that_see_nothing_are_zero(device):
     """More queries than a request has tokens (the first ones are before position 0), pages that are not in the cache."""
     g = np.random.default_rng(11)
