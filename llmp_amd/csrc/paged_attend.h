@@ -27,6 +27,7 @@ struct PagedAttendArgs {
   int group;            // query heads a KV head
   int most_length;      // tokens a table row can name
   int shift;            // the few rows' form: a unit of the line is 2^shift tiles
+  int whole_units;  // the few rows' form: units a workgroup takes where it takes whole segments, 0 where the line is cut evenly
   int few_rows;         // requests of more (token, head) rows than these are the many rows' form's
 };
 

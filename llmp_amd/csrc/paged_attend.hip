@@ -6,7 +6,8 @@
 // device alike. A workgroup's part of a (rows, head) segment that others share goes to scratch and a second launch joins the
 // parts; a segment that one workgroup has whole is finished there.
 //
-// A wave takes a tile alone, its operands straight from memory into the matrix instructions' registers, no LDS:
+// A wave takes a tile alone. Its K and V come to the wave's own part of LDS without a register waiting for them (a whole tile is on its
+// way under another's work), and from there into the matrix instructions' registers:
 //   S^T = K Q^T by v_mfma_i32_16x16x64_i8: a lane brings 16 bytes of a token's K row. Row 4a + b of the t-th product is token
 //   16a + 4t + b of the tile, so that a lane ends with 16 consecutive tokens (16 g to 16 g + 15, g its group of lanes) of one
 //   query row. That is the order in which
@@ -126,6 +127,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
   const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
   uint32_t per = (even + kFewWaves - 1) / kFewWaves * kFewWaves;
   if (even < kFewWaves) per = min(per, max(even, (total + segments - 1) / max(segments, 1u)));
+  if (LISTS && a.whole_units > 0) per = a.whole_units;
   const uint32_t group = OnChiplet(blockIdx.x, gridDim.x, (total + per - 1) / max(per, 1u));
   uint32_t u = group * per;
   const uint32_t u_end = min(u + per, total);
@@ -576,6 +578,7 @@ void LaunchFew(const PagedAttendArgs& args, int groups, hipStream_t stream) {
   static bool sized = false;
   if (kLds > 32768 && !AllowLds(reinterpret_cast<const void*>(&FewKernel<TYPE, D, LISTS>), kLds, &sized)) return;
   hipLaunchKernelGGL((FewKernel<TYPE, D, LISTS>), dim3(groups), dim3(kFewThreads), kLds, stream, args);
+  if (args.whole_units > 0) return;  // no segment is shared
   const int64_t rows = static_cast<int64_t>(LISTS ? 1 : args.op.most_tokens) * args.group;  // at most, of a segment
   hipLaunchKernelGGL((FewJoinKernel<TYPE, D, LISTS>), dim3(groups, rows < kRows ? static_cast<unsigned>(rows) : kRows), dim3(kFewThreads), 0, stream, args);
 }
@@ -607,6 +610,19 @@ int FewShift(const llmp_paged_attend& op) {
   int shift = 0;
   while (segments * ((tiles >> shift) + 1) >= 1ll << 31 && shift < 24) ++shift;
   return shift;
+}
+// With page lists all segments are of one size. Workgroups take whole ones (this many units) where an even cut would save less than
+// what it costs: a second segment's beginning and end, and the joining launch. In us, cut evenly against whole, 4 KV heads of 128, groups
+// of 4, 512 workgroups: 16 segments of 2, 12, 16 tiles 8.5/6.8, 10.7/10.3, 10.9/12.0; 64 of 8, 16, 64 10.4/8.8, 11.5/12.2, 19/30;
+// 256 of 8, 24 14.3/9.4, 20.6/16.6; 400 of 12, 24, 64 17.4/15.1, 29.2/22.1, 49/44; 800 of 24, 64 44.2/39.4, 80/83.
+constexpr int kVisit = 12;
+int WholeUnits(const PagedAttendArgs& args, int groups) {
+  const llmp_paged_attend& op = args.op;
+  if (op.lists == nullptr || args.shift > 0) return 0;
+  const int64_t segments = static_cast<int64_t>(op.tokens) * ((args.group + kRows - 1) / kRows) * op.cache.kv_heads;
+  const int64_t a_segment = (static_cast<int64_t>(op.list_pages) * op.cache.page + kTileTokens - 1) / kTileTokens;
+  const int64_t even = (segments * a_segment + groups - 1) / groups, whole = a_segment * ((segments + groups - 1) / groups);
+  return whole <= even + even / 8 + kVisit ? static_cast<int>(whole) : 0;
 }
 bool HasMany(const llmp_paged_attend& op) {
   return op.lists == nullptr && static_cast<int64_t>(op.most_tokens < op.tokens ? op.most_tokens : op.tokens) * (op.heads / op.cache.kv_heads) > kFewRows;
@@ -670,6 +686,7 @@ extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch,
   const bool alone = many && op->requests == 1 && op->most_tokens >= op->tokens;  // one request: of whatever rows, the many rows' form's
   args.few_rows = alone ? 0 : many ? kFewRows : kMostFewRows;
   args.shift = FewShift(*op);
+  args.whole_units = WholeUnits(args, groups);
   const hipStream_t on = static_cast<hipStream_t>(stream);
   if (many) PagedManyRows(args, static_cast<uint8_t*>(scratch) + FewScratch(op->cache.head_dim, cus), cus, on);
   if (alone) return LaunchStatus("paged_attend");
