@@ -27,14 +27,21 @@ constexpr int kJoinThreads = 256;
 constexpr int kListThreads = 1024;
 constexpr int kBuckets = 1024;  // of the segments' lengths, for their order
 
-// The list: a header, the pairs, the tiles before each pair (times KV heads), the pairs' order by length.
+// What a segment's beginning and end cost a workgroup, in tiles: where the line is cut evenly, a segment has that many places on it
+// before its tiles (a workgroup with eleven short segments otherwise ends last by far).
+constexpr int kVisit = 4;
+
+// The list: a header, the pairs, the line's length before each pair (all KV heads'), the pairs' order by length.
 struct ListHeader {
-  int64_t total;   // tiles of all segments
+  int64_t total;   // tiles of all segments, and kVisit for each
   int pairs, whole;  // whole: every segment is one workgroup's
 };
 struct Pair {
   int request, chunk, first_tile, tiles;
+  PagedRequest q;
+  int unused;
 };
+static_assert(sizeof(Pair) == 32);
 struct List {
   ListHeader* header;
   Pair* pairs;
@@ -59,7 +66,8 @@ __device__ __forceinline__ int ChunksOf(const PagedAttendArgs& a, const PagedReq
 // One workgroup: the pairs in the order of the requests, their sums, and their order by length.
 __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int groups) {
   __shared__ int64_t wave_sums[kListThreads / kWave];
-  __shared__ int buckets[kBuckets];
+  __shared__ int buckets[kBuckets], first_pair[kListThreads];
+  __shared__ PagedRequest requests[kListThreads];
   const PagedAttendArgs& a = m.a;
   const llmp_paged_attend& op = a.op;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
@@ -82,41 +90,48 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
     return v;
   };
   // The pairs: a request's by all threads where it has many.
-  int64_t pairs = 0;
-  for (int base = 0; base < op.requests; base += kListThreads) {
-    const int r = base + tid;
-    const int mine = r < op.requests ? ChunksOf(a, RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length)) : 0;
-    int64_t all;
-    const int64_t upto = block_sum(mine, &all);
-    for (int j = 0; j < mine; ++j) {
-      const int64_t at = pairs + upto - mine + j;
-      if (at < m.most_pairs) m.list.pairs[at].request = r, m.list.pairs[at].chunk = j;
-    }
-    pairs += all;
-  }
-  const int count = static_cast<int>(pairs < m.most_pairs ? pairs : m.most_pairs);
   buckets[tid] = 0;
-  __syncthreads();
-  int64_t before = 0;
-  for (int base = 0; base < count; base += kListThreads) {
-    const int p = base + tid;
-    int tiles = 0;
-    if (p < count) {
-      Pair pair = m.list.pairs[p];
-      const PagedRequest q = RequestOf(op.starts, op.lengths, pair.request, op.tokens, a.most_length);
-      const int first_token = pair.chunk * kManyRows / a.group, last_token = min((pair.chunk * kManyRows + kManyRows - 1) / a.group, q.n - 1);
-      const int to = max(q.length - q.n + last_token + 1, 0), window = op.window > 0 ? op.window : INT_MAX / 2;
-      pair.first_tile = max(q.length - q.n + first_token - window + 1, 0) / kTileTokens;
-      pair.tiles = tiles = max((to + kTileTokens - 1) / kTileTokens - pair.first_tile, 1);  // (rows that see nothing are written too)
-      m.list.pairs[p] = pair;
+  int64_t count = 0, before = 0;
+  for (int base = 0; base < op.requests; base += kListThreads) {
+    const int here = min(op.requests - base, kListThreads);
+    requests[tid] = tid < here ? RequestOf(op.starts, op.lengths, base + tid, op.tokens, a.most_length) : PagedRequest{};
+    const int mine = tid < here ? ChunksOf(a, requests[tid]) : 0;
+    int64_t pairs;
+    first_pair[tid] = static_cast<int>(block_sum(mine, &pairs)) - mine;
+    pairs = min(pairs, m.most_pairs - count);
+    __syncthreads();
+    // A thread a pair: its request is the last whose pairs begin at or before it (one without pairs begins where the next does).
+    for (int64_t p0 = 0; p0 < pairs; p0 += kListThreads) {
+      const int p = static_cast<int>(p0) + tid;
+      Pair pair = {};
+      int64_t length = 0;
+      if (p < pairs) {
+        int low = 0, high = here;
+        while (high - low > 1) {
+          const int mid = (low + high) >> 1;
+          if (first_pair[mid] <= p) {
+            low = mid;
+          } else {
+            high = mid;
+          }
+        }
+        const PagedRequest q = requests[low];
+        pair.request = base + low, pair.chunk = p - first_pair[low], pair.q = q;
+        const int first_token = pair.chunk * kManyRows / a.group, last_token = min((pair.chunk * kManyRows + kManyRows - 1) / a.group, q.n - 1);
+        const int to = max(q.length - q.n + last_token + 1, 0), window = op.window > 0 ? op.window : INT_MAX / 2;
+        pair.first_tile = max(q.length - q.n + first_token - window + 1, 0) / kTileTokens;
+        pair.tiles = max((to + kTileTokens - 1) / kTileTokens - pair.first_tile, 1);  // (rows that see nothing are written too)
+        length = static_cast<int64_t>(pair.tiles + kVisit) * op.cache.kv_heads;
+        m.list.pairs[count + p] = pair;
+        atomicAdd(&buckets[kBuckets - 1 - min(pair.tiles / 4, kBuckets - 1)], 1);
+      }
+      int64_t all;
+      const int64_t upto = block_sum(length, &all);
+      if (p < pairs) m.list.before[count + p] = before + upto - length;
+      before += all;
     }
-    int64_t all;
-    const int64_t upto = block_sum(static_cast<int64_t>(tiles) * op.cache.kv_heads, &all);
-    if (p < count) {
-      m.list.before[p] = before + upto - static_cast<int64_t>(tiles) * op.cache.kv_heads;
-      atomicAdd(&buckets[kBuckets - 1 - min(tiles / 4, kBuckets - 1)], 1);
-    }
-    before += all;
+    count += pairs;
+    __syncthreads();
   }
   __syncthreads();
   int64_t all;
@@ -129,8 +144,8 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
   if (tid == 0) {
     m.list.before[count] = before;
     m.list.header->total = before;
-    m.list.header->pairs = count;
-    m.list.header->whole = static_cast<int64_t>(count) * op.cache.kv_heads >= groups;
+    m.list.header->pairs = static_cast<int>(count);
+    m.list.header->whole = count * op.cache.kv_heads >= groups;
   }
 }
 
@@ -181,8 +196,15 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
   const ListHeader header = *m.list.header;
   F32x4* const group_scales = reinterpret_cast<F32x4*>(lds + 2 * G::kBuffer);  // [buffer][group]: K's and V's scale, V's log2 and reciprocal
 
-  int64_t u = 0, u_end = 0, per = 1;
-  int turn = 0, pair_index = 0;
+  int64_t u = 0, u_end = 0, per = 1, pair_from = 0;  // (where on the line the pair begins)
+  int turn = 0, pair_index = -1;
+  Pair pair = {};
+  const auto load_pair = [&]() {
+    const I32x4* const from = reinterpret_cast<const I32x4*>(m.list.pairs + pair_index);
+    const I32x4 x = from[0], y = from[1];
+    const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    pair = {one(x[0]), one(x[1]), one(x[2]), one(x[3]), {one(y[0]), one(y[1]), one(y[2])}, 0};
+  };
   const int units = groups / m.a_unit, unit_of = w % units;
   const int64_t segments = static_cast<int64_t>(header.pairs) * c.kv_heads;
   if (header.whole) {
@@ -191,17 +213,18 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
     per = (header.total + groups - 1) / groups;
     u = w * per;
     u_end = min(u + per, header.total);
-    if (u < u_end) {  // the pair that holds unit u
-      int low = 0, high = header.pairs;
-      while (high - low > 1) {
-        const int mid = (low + high) >> 1;
-        if (m.list.before[mid] <= u) {
-          low = mid;
-        } else {
-          high = mid;
+    if (u < u_end) {  // the pair that holds unit u: the last that begins at or before it
+      for (int base = 0; base < header.pairs; base += kWave) {
+        const int64_t before = base + lane < header.pairs ? m.list.before[base + lane] : INT64_MAX;
+        const int at = __popcll(__ballot(before <= u));
+        if (at > 0) {
+          const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(before), at - 1);
+          pair_index = base + at - 1;
+          pair_from = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(before >> 32), at - 1)) << 32 | low;
         }
+        if (at < kWave) break;
       }
-      pair_index = low;
+      load_pair();
     }
   }
   I32x4 part = {-1, 0, 0, 0};
@@ -214,69 +237,50 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
       if (static_cast<int64_t>(turn) * units >= segments) break;
       turn += m.a_unit;
       if (index >= segments) continue;
-      pair_index = m.list.order[index / c.kv_heads];
+      pair_index = __builtin_amdgcn_readfirstlane(m.list.order[index / c.kv_heads]);
       head = static_cast<int>(index % c.kv_heads);
+      load_pair();
       t_first = 0;
-      t_count = m.list.pairs[pair_index].tiles;
+      t_count = pair.tiles;
     } else {
       if (u >= u_end) break;
-      if (u >= m.list.before[pair_index + 1]) {
+      const int length = pair.tiles + kVisit;
+      if (u >= pair_from + static_cast<int64_t>(length) * c.kv_heads) {
+        pair_from += static_cast<int64_t>(length) * c.kv_heads;
         ++pair_index;
+        load_pair();
         continue;
       }
-      const int64_t in = u - m.list.before[pair_index];
-      const int tiles = m.list.pairs[pair_index].tiles;
-      head = static_cast<int>(in / tiles);
-      t_first = static_cast<int>(in % tiles);
-      t_count = static_cast<int>(min(static_cast<int64_t>(tiles - t_first), u_end - u));
-      u += t_count;
+      const int in = static_cast<int>(u - pair_from);
+      head = in / length;
+      const int from = in - head * length, to = static_cast<int>(min(static_cast<int64_t>(length), from + u_end - u));
+      u += to - from;
+      t_first = max(from - kVisit, 0);
+      t_count = max(to - kVisit, 0) - t_first;
+      if (t_count == 0) continue;  // the next workgroup begins it
     }
-    pair_index = __builtin_amdgcn_readfirstlane(pair_index);
     head = __builtin_amdgcn_readfirstlane(head);
     t_first = __builtin_amdgcn_readfirstlane(t_first);
     t_count = __builtin_amdgcn_readfirstlane(t_count);
-    const Pair pair = m.list.pairs[pair_index];
-    const int r = __builtin_amdgcn_readfirstlane(pair.request);
-    const PagedRequest q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
-    const int32_t* const table = op.table + r * op.table_stride;
+    const PagedRequest q = pair.q;
+    const int32_t* const table = op.table + pair.request * op.table_stride;
 
     // ---- this lane's query row, and what the wave's rows see.
     const int row0 = pair.chunk * kManyRows + wave * kWaveRows;
     const int row = row0 + column, rows = q.n * a.group;
     const bool real = row < rows;
-    const int token = row / a.group, query_head = row % a.group;
+    const int token0 = row0 / a.group, in_token0 = row0 - token0 * a.group;  // the wave's first row's
+    const int in_tokens = PagedDivide(in_token0 + column, a.group_magic);
+    const int token = token0 + in_tokens, query_head = in_token0 + column - in_tokens * a.group;
     const int base_position = q.length - q.n;
     const int position = base_position + token;
     const int window = op.window > 0 ? op.window : INT_MAX / 2;
     const int see_from = max(position - window + 1, 0), see_to = real ? position + 1 : 0;
-    const int first_position = base_position + row0 / a.group, last_position = base_position + min((row0 + kWaveRows - 1) / a.group, q.n - 1);
+    const int first_position = base_position + token0;
+    const int last_position = base_position + min(token0 + static_cast<int>(PagedDivide(in_token0 + kWaveRows - 1, a.group_magic)), q.n - 1);
     const int all_from = max(last_position - window + 1, 0), all_to = first_position + 1;
     const int any_from = max(first_position - window + 1, 0), any_to = row0 < rows ? last_position + 1 : 0;
 
-    I32x4 digits[kDig][kSteps];
-    float unit;
-    {
-      QueryPart<TYPE, 2 * kSteps> part_of_row;
-      const int64_t from = (q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * half;
-#pragma unroll
-      for (int i = 0; i < 2 * kSteps; ++i) part_of_row.Load(op.q, i, from + kInner * (i / 2) + 8 * (i % 2));
-      const QueryUnit made = UnitOf<TYPE>(Across<kWaveRows>(part_of_row.MostBits()));
-      // (A negative scale goes into the digits: the units stay positive, so the largest product is the largest logit.)
-      const float inverse = !real ? 0.0f : op.scale < 0.0f ? -made.inverse : made.inverse;
-#pragma unroll
-      for (int i = 0; i < 2 * kSteps; ++i) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float v[4];
-          part_of_row.Four(i, k, v);
-          uint32_t packed[kDig];
-          PackDigits<kDig>(v, inverse, packed);
-#pragma unroll
-          for (int d = 0; d < kDig; ++d) digits[d][i / 2][2 * (i % 2) + k] = static_cast<int>(packed[d]);
-        }
-      }
-      unit = made.unit * fabsf(op.scale) * (op.softcap != 0.0f ? 1.0f : kLog2E);
-    }
     const float cap_inverse = op.softcap != 0.0f ? 1.0f / op.softcap : 0.0f;
 
     // ---- the tiles' loads. A lane knows the page of the tile's 16-token group `lane & 3`; it is looked at a tile after it was
@@ -371,8 +375,35 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
       __syncthreads();
     };
     Group next = group_of(tile_from);
+    // The row's loads before the first tile's: its digits are made while that is on its way.
+    QueryPart<TYPE, 2 * kSteps> part_of_row;
+    {
+      const int64_t from = (q.start + (real ? token : 0)) * op.q_token_stride + (head * a.group + (real ? query_head : 0)) * op.q_head_stride + 16 * half;
+#pragma unroll
+      for (int i = 0; i < 2 * kSteps; ++i) part_of_row.Load(op.q, i, from + kInner * (i / 2) + 8 * (i % 2));
+    }
     fetch(next, 0);
     next = group_of(tile_from + 1);
+    I32x4 digits[kDig][kSteps];
+    float unit;
+    {
+      const QueryUnit made = UnitOf<TYPE>(Across<kWaveRows>(part_of_row.MostBits()));
+      // (A negative scale goes into the digits: the units stay positive, so the largest product is the largest logit.)
+      const float inverse = !real ? 0.0f : op.scale < 0.0f ? -made.inverse : made.inverse;
+#pragma unroll
+      for (int i = 0; i < 2 * kSteps; ++i) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float v[4];
+          part_of_row.Four(i, k, v);
+          uint32_t packed[kDig];
+          PackDigits<kDig>(v, inverse, packed);
+#pragma unroll
+          for (int d = 0; d < kDig; ++d) digits[d][i / 2][2 * (i % 2) + k] = static_cast<int>(packed[d]);
+        }
+      }
+      unit = made.unit * fabsf(op.scale) * (op.softcap != 0.0f ? 1.0f : kLog2E);
+    }
     place(0);
     meet();
     for (int tile = tile_from; tile < tile_to; ++tile) {
@@ -543,7 +574,7 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
         for (int i = 0; i < kValues; ++i) to[2 + kWaveRows * b + 8 * (i / 4) + 4 * half + i % 4] = out[b][i];
       }
       if (begins) {
-        const int64_t segment_end = m.list.before[pair_index] + static_cast<int64_t>(head + 1) * pair.tiles;
+        const int64_t segment_end = m.list.before[pair_index] + static_cast<int64_t>(head + 1) * (pair.tiles + kVisit);
         part = I32x4{static_cast<int>((segment_end - 1) / per), pair_index, head, 0};
       }
     }
@@ -561,41 +592,63 @@ __global__ __launch_bounds__(kJoinThreads) void ManyJoinKernel(const ManyArgs m)
   const I32x4 part = *reinterpret_cast<const I32x4*>(m.parts + 4 * blockIdx.x);
   if (part.x < 0) return;
   const Pair pair = m.list.pairs[part.y];
-  const PagedRequest q = RequestOf(op.starts, op.lengths, pair.request, op.tokens, a.most_length);
   const int lane = threadIdx.x & (kWave - 1), first = blockIdx.x, last = part.x;
+  constexpr int kJoinRows = 4, kBatch = 2;  // rows a wave, parts asked for at once
+  const int slot0 = 16 * blockIdx.y + kJoinRows * (threadIdx.x / kWave), row0 = pair.chunk * kManyRows + slot0, rows = pair.q.n * a.group;
+  if (row0 >= rows) return;
+  float high[kJoinRows], all[kJoinRows], value[kJoinRows][kPer];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int in_slot = 16 * blockIdx.y + 4 * i + threadIdx.x / kWave, row = pair.chunk * kManyRows + in_slot;
-    if (row >= q.n * a.group) return;
-    const auto slot_of = [&](int w) { return m.partial + ((2 * static_cast<int64_t>(w) + (w == first ? 1 : 0)) * kManyRows + in_slot) * (D + 2); };
-    float high = -INFINITY;
-    for (int w = first + lane; w <= last; w += kWave) high = fmaxf(high, slot_of(w)[0]);
+  for (int i = 0; i < kJoinRows; ++i) {
+    high[i] = -INFINITY, all[i] = 0.0f;
 #pragma unroll
-    for (int step = 1; step < kWave; step <<= 1) high = fmaxf(high, __shfl_xor(high, step));
-    float all = 0.0f, value[kPer];
+    for (int e = 0; e < kPer; ++e) value[i][e] = 0.0f;
+  }
+  for (int w0 = first; w0 <= last; w0 += kBatch) {
+    float top[kBatch][kJoinRows], total[kBatch][kJoinRows], v[kBatch][kJoinRows][kPer];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) value[e] = 0.0f;
-#pragma unroll 4
-    for (int w = first; w <= last; ++w) {
-      const float* from = slot_of(w);
-      const float top = from[0];
-      const float keep = top == -INFINITY ? (high == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(top - high);
-      all += from[1] * keep;
+    for (int k = 0; k < kBatch; ++k) {
+      const int w = min(w0 + k, last);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) value[e] += from[2 + kPer * lane + e] * keep;
+      for (int i = 0; i < kJoinRows; ++i) {  // (rows past the request's last have slots too, whose values go nowhere)
+        const float* from = m.partial + ((2 * static_cast<int64_t>(w) + (w == first ? 1 : 0)) * kManyRows + slot0 + i) * (D + 2);
+        top[k][i] = from[0], total[k][i] = from[1];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[k][i][e] = from[2 + kPer * lane + e];
+      }
     }
-    const int h = part.z * a.group + row % a.group;
-    if (op.sinks != nullptr) all += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(high == -INFINITY ? 0.0f : high)));
-    const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
-    const int64_t to = (q.start + row / a.group) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[e] * inverse);
+    for (int k = 0; k < kBatch; ++k) {
+      if (w0 + k > last) break;
+#pragma unroll
+      for (int i = 0; i < kJoinRows; ++i) {
+        const float higher = fmaxf(high[i], top[k][i]);
+        const auto weight = [&](float of) { return of == -INFINITY ? (higher == -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(of - higher); };
+        const float keep = weight(high[i]), add = weight(top[k][i]);
+        all[i] = all[i] * keep + total[k][i] * add;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) value[i][e] = value[i][e] * keep + v[k][i][e] * add;
+        high[i] = higher;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kJoinRows; ++i) {
+    const int row = row0 + i;
+    if (row >= rows) return;
+    const int token = row / a.group, h = part.z * a.group + row - token * a.group;
+    float sum = all[i];
+    if (op.sinks != nullptr) sum += __builtin_amdgcn_exp2f(fmaf(op.sinks[h], kLog2E, -(high[i] == -INFINITY ? 0.0f : high[i])));
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t to = (pair.q.start + token) * op.out_token_stride + h * op.out_head_stride + kPer * lane;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) StoreOne<TYPE>(op.out, to + e, value[i][e] * inverse);
   }
 }
 
 int ManyGroups(int head_dim, int cus) { return (head_dim == 256 ? 1 : 2) * (cus > 0 ? cus : 256); }
 int64_t MostPairs(const llmp_paged_attend& op, int group) {
-  // (Requests of more than few_rows rows only, and few_rows is at least half of kManyRows: two pairs of every kManyRows rows at most.)
+  // (Requests of more than few_rows rows only, and few_rows is at least half of kManyRows: two pairs of every kManyRows rows at most.
+  // A request alone, of any rows, has one for every kManyRows and one more.)
   return 2 * (static_cast<int64_t>(op.tokens) * group / kManyRows + 1);
 }
 size_t Up(size_t bytes) { return (bytes + 15) & ~static_cast<size_t>(15); }
