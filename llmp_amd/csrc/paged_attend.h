@@ -29,6 +29,7 @@ struct PagedAttendArgs {
   int shift;            // the few rows' form: a unit of the line is 2^shift tiles
   int whole_units;  // the few rows' form: units a workgroup takes where it takes whole segments, 0 where the line is cut evenly
   int few_rows;         // requests of more (token, head) rows than these are the many rows' form's
+  const int32_t* all_taken;  // in memory, not zero: by the many rows' form; null: none is
 };
 
 // n / d for n * d < 2^32, magic = 2^32 / d + 1 (0 for d = 1): n times the magic's excess stays below 2^32 / d.
@@ -228,9 +229,10 @@ __device__ __forceinline__ float Capped(float s, float softcap, float inverse) {
 // log2 of a page's V scale, as the running maximum takes it.
 __device__ __forceinline__ float ScaleLog(float vs) { return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-100f)); }
 
-// The many rows' form (its own file), for requests of more than few_rows rows.
+// The many rows' form (its own file), for requests of more than few_rows rows, and those of fewer where they are little work beside
+// them: the number that it gives the place of is then not zero.
 size_t PagedManyScratch(const llmp_paged_attend& op, int cus);
-void PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStream_t stream);
+const int32_t* PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStream_t stream);
 
 }  // namespace llmp_hip
 

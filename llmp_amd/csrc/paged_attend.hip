@@ -108,6 +108,10 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
   const int group_of = lane >> 4, column = lane & 15;
   uint8_t* const landing = lds + wave * TileBytes(D);
 
+  if (!LISTS && a.all_taken != nullptr && *a.all_taken != 0) {
+    if (tid == 0) *reinterpret_cast<I32x4*>(a.parts + 4 * blockIdx.x) = I32x4{-1, 0, 0, 0};
+    return;
+  }
   // ---- this workgroup's run of the line of units: the requests 64 at a time, a lane each.
   const auto block = [&](int base) {
     FewRequest f = {};
@@ -688,7 +692,8 @@ extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch,
   args.shift = FewShift(*op);
   args.whole_units = WholeUnits(args, groups);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (many) PagedManyRows(args, static_cast<uint8_t*>(scratch) + FewScratch(op->cache.head_dim, cus), cus, on);
+  args.all_taken = nullptr;
+  if (many) args.all_taken = PagedManyRows(args, static_cast<uint8_t*>(scratch) + FewScratch(op->cache.head_dim, cus), cus, on);
   if (alone) return LaunchStatus("paged_attend");
   if (op->type == LLMP_X_F32) LaunchFewOf<LLMP_X_F32>(args, groups, on);
   if (op->type == LLMP_X_BF16) LaunchFewOf<LLMP_X_BF16>(args, groups, on);

@@ -35,6 +35,7 @@ constexpr int kVisit = 4;
 struct ListHeader {
   int64_t total;   // tiles of all segments, and kVisit for each
   int pairs, whole;  // whole: every segment is one workgroup's
+  int all;           // the few rows' form has nothing left to do
 };
 struct Pair {
   int request, chunk, first_tile, tiles;
@@ -58,9 +59,22 @@ struct ManyArgs {
   int a_unit;  // workgroups a compute unit holds
 };
 
-__device__ __forceinline__ int ChunksOf(const PagedAttendArgs& a, const PagedRequest& q) {
+// A few-row request (a prompt's neighbours that decode) is taken along where all of them make the line no longer than this many
+// tiles a compute unit, about what the few rows' two launches cost (6 requests at head size 256, one of them decoding, 123 us without
+// and 109 with; 8 at 128 105 and 100).
+constexpr int kTakeAlong = 8, kTakeAlongRequests = kListThreads;
+
+__device__ __forceinline__ int ChunksOf(const PagedAttendArgs& a, const PagedRequest& q, int few_rows) {
   const int64_t rows = static_cast<int64_t>(q.n) * a.group;
-  return rows > a.few_rows ? static_cast<int>((rows + kManyRows - 1) / kManyRows) : 0;
+  return rows > few_rows ? static_cast<int>((rows + kManyRows - 1) / kManyRows) : 0;
+}
+// The tiles that a chunk of a request's rows sees.
+__device__ __forceinline__ void TilesOf(const PagedAttendArgs& a, Pair* pair) {
+  const PagedRequest& q = pair->q;
+  const int first_token = pair->chunk * kManyRows / a.group, last_token = min((pair->chunk * kManyRows + kManyRows - 1) / a.group, q.n - 1);
+  const int to = max(q.length - q.n + last_token + 1, 0), window = a.op.window > 0 ? a.op.window : INT_MAX / 2;
+  pair->first_tile = max(q.length - q.n + first_token - window + 1, 0) / kTileTokens;
+  pair->tiles = max((to + kTileTokens - 1) / kTileTokens - pair->first_tile, 1);  // (rows that see nothing are written too)
 }
 
 // One workgroup: the pairs in the order of the requests, their sums, and their order by length.
@@ -92,11 +106,23 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
   // The pairs: a request's by all threads where it has many.
   buckets[tid] = 0;
   int64_t count = 0, before = 0;
+  bool all_taken = false;
   for (int base = 0; base < op.requests; base += kListThreads) {
     const int here = min(op.requests - base, kListThreads);
     requests[tid] = tid < here ? RequestOf(op.starts, op.lengths, base + tid, op.tokens, a.most_length) : PagedRequest{};
-    const int mine = tid < here ? ChunksOf(a, requests[tid]) : 0;
     int64_t pairs;
+    int few_rows = a.few_rows;
+    if (op.requests <= kTakeAlongRequests) {
+      Pair pair = {};
+      pair.q = requests[tid];
+      TilesOf(a, &pair);
+      const bool few = pair.q.n > 0 && ChunksOf(a, pair.q, few_rows) == 0;
+      int64_t along;
+      block_sum(few ? static_cast<int64_t>(pair.tiles + kVisit) * op.cache.kv_heads : 0, &along);
+      if (along <= static_cast<int64_t>(kTakeAlong) * (groups / m.a_unit)) few_rows = 0;
+    }
+    all_taken = few_rows == 0;
+    const int mine = tid < here ? ChunksOf(a, requests[tid], few_rows) : 0;
     first_pair[tid] = static_cast<int>(block_sum(mine, &pairs)) - mine;
     pairs = min(pairs, m.most_pairs - count);
     __syncthreads();
@@ -115,12 +141,8 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
             high = mid;
           }
         }
-        const PagedRequest q = requests[low];
-        pair.request = base + low, pair.chunk = p - first_pair[low], pair.q = q;
-        const int first_token = pair.chunk * kManyRows / a.group, last_token = min((pair.chunk * kManyRows + kManyRows - 1) / a.group, q.n - 1);
-        const int to = max(q.length - q.n + last_token + 1, 0), window = op.window > 0 ? op.window : INT_MAX / 2;
-        pair.first_tile = max(q.length - q.n + first_token - window + 1, 0) / kTileTokens;
-        pair.tiles = max((to + kTileTokens - 1) / kTileTokens - pair.first_tile, 1);  // (rows that see nothing are written too)
+        pair.request = base + low, pair.chunk = p - first_pair[low], pair.q = requests[low];
+        TilesOf(a, &pair);
         length = static_cast<int64_t>(pair.tiles + kVisit) * op.cache.kv_heads;
         m.list.pairs[count + p] = pair;
         atomicAdd(&buckets[kBuckets - 1 - min(pair.tiles / 4, kBuckets - 1)], 1);
@@ -145,6 +167,7 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
     m.list.before[count] = before;
     m.list.header->total = before;
     m.list.header->pairs = static_cast<int>(count);
+    m.list.header->all = all_taken;
     m.list.header->whole = count * op.cache.kv_heads >= groups;
   }
 }
@@ -648,8 +671,8 @@ __global__ __launch_bounds__(kJoinThreads) void ManyJoinKernel(const ManyArgs m)
 int ManyGroups(int head_dim, int cus) { return (head_dim == 256 ? 1 : 2) * (cus > 0 ? cus : 256); }
 int64_t MostPairs(const llmp_paged_attend& op, int group) {
   // (Requests of more than few_rows rows only, and few_rows is at least half of kManyRows: two pairs of every kManyRows rows at most.
-  // A request alone, of any rows, has one for every kManyRows and one more.)
-  return 2 * (static_cast<int64_t>(op.tokens) * group / kManyRows + 1);
+  // A request alone, of any rows, has one for every kManyRows and one more; one taken along has one.)
+  return 2 * (static_cast<int64_t>(op.tokens) * group / kManyRows + 1) + (op.requests <= kTakeAlongRequests ? op.requests : 0);
 }
 size_t Up(size_t bytes) { return (bytes + 15) & ~static_cast<size_t>(15); }
 
@@ -684,7 +707,7 @@ size_t PagedManyScratch(const llmp_paged_attend& op, int cus) {
          2 * static_cast<size_t>(groups) * kManyRows * (op.cache.head_dim + 2) * sizeof(float);
 }
 
-void PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStream_t stream) {
+const int32_t* PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStream_t stream) {
   const int groups = ManyGroups(args.op.cache.head_dim, cus);
   ManyArgs m;
   m.a = args;
@@ -705,6 +728,7 @@ void PagedManyRows(const PagedAttendArgs& args, void* scratch, int cus, hipStrea
   if (args.op.type == LLMP_X_F32) LaunchManyOf<LLMP_X_F32>(m, groups, stream);
   if (args.op.type == LLMP_X_BF16) LaunchManyOf<LLMP_X_BF16>(m, groups, stream);
   if (args.op.type == LLMP_X_F16) LaunchManyOf<LLMP_X_F16>(m, groups, stream);
+  return &m.list.header->all;
 }
 
 }  // namespace llmp_hip
