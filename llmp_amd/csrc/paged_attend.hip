@@ -602,8 +602,12 @@ void LaunchFewOf(const PagedAttendArgs& args, int groups, hipStream_t stream) {
   if (args.op.cache.head_dim == 256) LaunchFewFor<TYPE, 256>(args, groups, stream);
 }
 
-// Requests of more rows than this are the many rows' form's, where the call has any.
+// Requests of more rows than this are the many rows' form's, where the call has any and is work enough: rows times their most tokens
+// times head size. In us, this form against that one, bf16, 8 KV heads of 128, groups of 4: of 1000 tokens, 128 and 512 and 1000 new
+// 24/41, 36/49, 58/50; of 2000, 32, 256, 512, 1000 24/42, 32/53, 52/57, 93/73; of 8000, 32, 128, 256, 512 31/60, 60/77, 98/90, 168/117;
+// groups of 2 at 256, of 2000 128, 256, 512 31/54, 40/55, 70/61; groups of 7 at 64, 64, 512, 1000 21/34, 38/38, 42/43.
 constexpr int kFewRows = 64;
+constexpr int64_t kFewWork = 4000000ll * 128;
 constexpr int kMostGroup = 1024, kMostFewRows = 1 << 20;  // (PagedDivide's range together)
 // Tiles a unit of the line, as a power of two: a call's units stay below 2^31.
 int FewShift(const llmp_paged_attend& op) {
@@ -629,7 +633,9 @@ int WholeUnits(const PagedAttendArgs& args, int groups) {
   return whole <= even + even / 8 + kVisit ? static_cast<int>(whole) : 0;
 }
 bool HasMany(const llmp_paged_attend& op) {
-  return op.lists == nullptr && static_cast<int64_t>(op.most_tokens < op.tokens ? op.most_tokens : op.tokens) * (op.heads / op.cache.kv_heads) > kFewRows;
+  const int64_t group = op.heads / op.cache.kv_heads, rows = op.tokens * group;  // (the heads of all tokens: at most 2^30)
+  return op.lists == nullptr && (op.most_tokens < op.tokens ? op.most_tokens : op.tokens) * group > kFewRows &&
+         rows * op.table_width > kFewWork / op.cache.head_dim / op.cache.page;
 }
 size_t AttendScratch(const llmp_paged_attend& op, int cus) {
   return FewScratch(op.cache.head_dim, cus) + (HasMany(op) ? PagedManyScratch(op, cus) : 0);

@@ -233,7 +233,8 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
   if (header.whole) {
     turn = w / units;
   } else {
-    per = (header.total + groups - 1) / groups;
+    // (No fewer than a visit and as many tiles: finer parts cost more to write and to join.)
+    per = max((header.total + groups - 1) / groups, static_cast<int64_t>(2 * kVisit));
     u = w * per;
     u_end = min(u + per, header.total);
     if (u < u_end) {  // the pair that holds unit u: the last that begins at or before it

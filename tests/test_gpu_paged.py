@@ -178,6 +178,17 @@ def serving(g, lengths, fresh, kv_heads, page, d, spare=3):
     return cache, table, np.asarray(lengths, dtype=np.int32), starts
 
 
+def widened(table, cache, tokens, most, heads):
+    """The table with as many more columns, of any entries, as make a call of rows for it one of the prompts' form (rows times the
+    tokens a table row can name times head size: llmp_amd/csrc/paged_attend.hip, kFewWork)."""
+    pages, kv_heads, page, d = cache["k"].shape
+    if most * heads // kv_heads <= 64:
+        return table
+    more = 4000000 * 128 // (tokens * heads // kv_heads * d * page) + 2
+    spoiled = np.random.default_rng(5).choice(np.array([-1, -7, pages, 1 << 30, 0], dtype=np.int32), (len(table), more))
+    return np.concatenate([table, spoiled], axis=1)
+
+
 def run_attend(device, cache, q, table, lengths, starts, scale, dtype, lists=None, sinks=None, most=None, **kw):
     """Through strided queries and a strided output, checked against the definition."""
     qt, qf = rounded(q, dtype)
@@ -186,18 +197,21 @@ def run_attend(device, cache, q, table, lengths, starts, scale, dtype, lists=Non
     wide[:tokens, :heads] = qt
     out = torch.full((tokens + 2, heads, d), 7.0, dtype=TYPES[dtype], device=device)
     wide = wide.to(device)
-    got = ops.paged_attend(to_device(cache, device), wide[:tokens, :heads], dev(table, device), dev(lengths, device), dev(starts, device), scale,
-                           lists=None if lists is None else dev(lists, device), sinks=None if sinks is None else dev(sinks, device),
-                           most=most or max(1, int(np.diff(starts).max())), out=out[:tokens], **kw)
+    most = most or max(1, int(np.diff(starts).max()))
     want, far = plain.attend(cache, qf, table, lengths.tolist(), starts.tolist(), scale, dtype, picked=lists, sinks=sinks, **kw)
-    x = got[:starts[-1]].double().cpu().numpy()
     want, far = want[:starts[-1]], far[:starts[-1]]
-    near = np.abs(x - want) <= far
-    if not near.all():
-        at = np.argwhere(~near)
-        worst = np.nanmax(np.abs(x - want) / np.maximum(far, 1e-30))
-        pytest.fail(f"{len(at)} of {near.size} values too far off, up to {worst} of the distance; the first at {at[:4].tolist()}: {x[tuple(at[0])]}, not {want[tuple(at[0])]}")
-    assert bool((out[starts[-1]:] == 7.0).all())  # rows of no request stay as they are
+    for form in (table, widened(table, cache, tokens, most, heads)) if lists is None else (table,):
+        out[:tokens] = 7.0
+        got = ops.paged_attend(to_device(cache, device), wide[:tokens, :heads], dev(form, device), dev(lengths, device), dev(starts, device), scale,
+                               lists=None if lists is None else dev(lists, device), sinks=None if sinks is None else dev(sinks, device),
+                               most=most, out=out[:tokens], **kw)
+        x = got[:starts[-1]].double().cpu().numpy()
+        near = np.abs(x - want) <= far
+        if not near.all():
+            at = np.argwhere(~near)
+            worst = np.nanmax(np.abs(x - want) / np.maximum(far, 1e-30))
+            pytest.fail(f"{len(at)} of {near.size} values too far off, up to {worst} of the distance; the first at {at[:4].tolist()}: {x[tuple(at[0])]}, not {want[tuple(at[0])]}")
+        assert bool((out[starts[-1]:] == 7.0).all())  # rows of no request stay as they are
     return x, want
 
 
@@ -239,6 +253,16 @@ def test_prompts_of_odd_lengths(device, dtype, heads, kv_heads, d, page):
         run_attend(device, cache, q, table, lengths, starts, d ** -0.5, dtype, window=window)
 
 
+@pytest.mark.parametrize("longest", [200, 1600])
+def test_prompts_beside_decoding_requests(device, longest):
+    """Decoding requests that the prompts' form takes along, and more of them than it does."""
+    g = np.random.default_rng(longest)
+    fresh = [100, 0, 17] + [1] * 40 + [33]
+    lengths = [400, 9, 100] + [longest - 7 * i % 160 for i in range(40)] + [33]
+    cache, table, lengths, starts = serving(g, lengths, fresh, 2, 16, 64)
+    run_attend(device, cache, g.standard_normal((starts[-1], 8, 64)), table, lengths, starts, 0.125, "f16")
+
+
 @pytest.mark.parametrize("fresh", [0, 1, 5, 33, 100])
 def test_one_request_of_fewer_tokens_than_rows(device, fresh):
     """The rows' count says what may come, the starts what does: a captured step answers both."""
@@ -273,31 +297,35 @@ def test_scales_of_any_size_and_spoiled_tokens(device, dtype, fresh):
     x, _ = run_attend(device, cache, q, table, lengths, starts, 128 ** -0.5, dtype)
     assert np.all(x[starts[1]:] == 0)
     if fresh > 16:  # the last page's scales are not numbers: rows before it do not notice
-        clean = ops.paged_attend(to_device(cache, device), rounded(q, dtype)[0].to(device), dev(table, device), dev(lengths, device), dev(starts, device), 0.1)
+        spoiled = {name: np.array(x) for name, x in cache.items()}
         for name in ("k_scale", "v_scale"):
-            cache[name][table[0, 39]] = np.nan
-        got = ops.paged_attend(to_device(cache, device), rounded(q, dtype)[0].to(device), dev(table, device), dev(lengths, device), dev(starts, device), 0.1)
-        assert torch.equal(got[:44], clean[:44]) and bool(torch.isnan(got[44:60]).all()) and torch.equal(got[60:], clean[60:])
+            spoiled[name][table[0, 39]] = np.nan
+        for form in (table, widened(table, cache, len(q), fresh, 4)):
+            clean, got = [ops.paged_attend(to_device(c, device), rounded(q, dtype)[0].to(device), dev(form, device), dev(lengths, device),
+                                           dev(starts, device), 0.1) for c in (cache, spoiled)]
+            assert torch.equal(got[:44], clean[:44]) and bool(torch.isnan(got[44:60]).all()) and torch.equal(got[60:], clean[60:])
 
 
 @pytest.mark.parametrize("fresh", [1, 40])
 def test_a_query_that_is_no_number_spoils_its_own_row_only(device, fresh):
     g = np.random.default_rng(31)
     cache, table, lengths, starts = serving(g, [300, 90], [fresh, fresh], 2, 32, 64)
-    c, t, n, s = to_device(cache, device), dev(table, device), dev(lengths, device), dev(starts, device)
-    q = torch.from_numpy(g.standard_normal((starts[-1], 8, 64)).astype(np.float32)).to(device)
-    clean = ops.paged_attend(c, q, t, n, s, 0.125)
-    q[0, 3, 9], q[-1, 5, 0] = float("nan"), float("inf")
-    got = ops.paged_attend(c, q, t, n, s, 0.125)
-    spoiled = torch.zeros_like(got, dtype=torch.bool)
-    spoiled[0, 3], spoiled[-1, 5] = True, True
-    assert bool(torch.isnan(got[spoiled]).all()) and torch.equal(got[~spoiled], clean[~spoiled])
-    q[0, 3], q[-1, 5] = 0.0, 0.0  # zeros: the plain mean of what is seen
-    got = ops.paged_attend(c, q, t, n, s, 0.125)
-    k, v = plain.values(cache, table[0, :10])
-    p = 300 - fresh + 1
-    mean = np.swapaxes(v, 0, 1).reshape(2, -1, 64)[:, :p].mean(1)
-    assert np.allclose(got[0, 3].cpu().numpy(), mean[0], rtol=1e-5, atol=1e-6)
+    c, n, s = to_device(cache, device), dev(lengths, device), dev(starts, device)
+    values = torch.from_numpy(g.standard_normal((starts[-1], 8, 64)).astype(np.float32)).to(device)
+    for form in (table, widened(table, cache, starts[-1], fresh, 8)):
+        t, q = dev(form, device), values.clone()
+        clean = ops.paged_attend(c, q, t, n, s, 0.125)
+        q[0, 3, 9], q[-1, 5, 0] = float("nan"), float("inf")
+        got = ops.paged_attend(c, q, t, n, s, 0.125)
+        spoiled = torch.zeros_like(got, dtype=torch.bool)
+        spoiled[0, 3], spoiled[-1, 5] = True, True
+        assert bool(torch.isnan(got[spoiled]).all()) and torch.equal(got[~spoiled], clean[~spoiled])
+        q[0, 3], q[-1, 5] = 0.0, 0.0  # zeros: the plain mean of what is seen
+        got = ops.paged_attend(c, q, t, n, s, 0.125)
+        k, v = plain.values(cache, table[0, :10])
+        p = 300 - fresh + 1
+        mean = np.swapaxes(v, 0, 1).reshape(2, -1, 64)[:, :p].mean(1)
+        assert np.allclose(got[0, 3].cpu().numpy(), mean[0], rtol=1e-5, atol=1e-6)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -353,10 +381,11 @@ def test_pages_past_four_gigabytes(device):
     for fresh in (1, 70):
         lengths, starts = np.array([1000], dtype=np.int32), np.array([0, fresh], dtype=np.int32)
         q = g.standard_normal((fresh, 8, d)).astype(np.float32)
-        got = ops.paged_attend(big, dev(q, device), dev(table, device), dev(lengths, device), dev(starts, device), 0.1).double().cpu().numpy()
         here = np.arange(8, dtype=np.int32)[None]
         want, far = plain.attend(small, q, here, [1000], [0, fresh], 0.1, "f32")
-        assert np.all(np.abs(got - want) <= far)
+        for form in (table, widened(table, small, fresh, fresh, 8)):
+            got = ops.paged_attend(big, dev(q, device), dev(form, device), dev(lengths, device), dev(starts, device), 0.1).double().cpu().numpy()
+            assert np.all(np.abs(got - want) <= far)
         got = ops.paged_select(big, dev(q, device), dev(table, device), dev(lengths, device), dev(starts, device), 4)
         same(got, plain.lists(small, q, here, [1000], [0, fresh], 4), "lists")
 
