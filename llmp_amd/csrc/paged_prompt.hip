@@ -198,6 +198,11 @@ struct ManyGeo {
     if constexpr (kWaveRows == 16) return KPiece<D>(row, piece);
     return Turn<D / 16>(row, piece);
   }
+  // Of V's rows of eight pieces: 32 rows are read at once, or 16 and, by other lanes, their pieces' neighbours but one.
+  static __device__ __forceinline__ int VSlot(int d, int piece) {
+    if constexpr (kWaveRows == 16) return piece ^ ((d >> 1) & 5);
+    return Turn<8>(d, piece);
+  }
 };
 
 template <int TYPE, int D, bool CAPPED>
@@ -376,8 +381,8 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
       for (int j = 0; j < kLoads; ++j) {
         const int i = tid + kThreads * j;
         const int d = i >> 2, piece = 2 * (i & 3);
-        *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece)) = EightCodes(v_in[j][0], v_in[j][1]);
-        *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, piece + 1)) = EightCodes(v_in[j][2], v_in[j][3]);
+        *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * G::VSlot(d, piece)) = EightCodes(v_in[j][0], v_in[j][1]);
+        *reinterpret_cast<F16x8*>(v_at + d * 128 + 16 * G::VSlot(d, piece + 1)) = EightCodes(v_in[j][2], v_in[j][3]);
       }
       if (tid < 4) {  // (a logarithm of -infinity: no page)
         const float vs = scales_in[1];
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
               const int d = kWaveRows * b + column;
-              v_half[x][b] = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * Turn<8>(d, 2 * token_group + x));
+              v_half[x][b] = *reinterpret_cast<const F16x8*>(v_at + d * 128 + 16 * G::VSlot(d, 2 * token_group + x));
             }
           };
           if constexpr (kWaveRows == 32) {
