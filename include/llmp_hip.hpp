@@ -569,6 +569,17 @@ inline std::vector<Implementation> Implementations() {
     add(std::string("ggml.flash_attn_ext.vec_") + kind, "flash_attn_ext", {kind}, {1, any, 64, 1}, Rung::kNative, 0,
         {"llmp_hip_attn_vec_quant"}, "a lane a cell for K, a lane D / 64 values for V, the cells split over workgroups");
   }
+  // The paged 8-bit KV cache (no counterpart in the reference). The attention's sums are cut by the step's whole work, so a
+  // row's last bits follow what else the step holds; the selection's and the store's do not.
+  add("llmp.paged.plan", "paged.plan", {"i32"}, {1, any, 1, 1}, Rung::kNative, 0, {"llmp_hip_paged_plan"},
+      "one workgroup, or two launches for more requests, tokens or work items than it takes");
+  add("llmp.paged.store", "paged.store", {"paged_q8"}, {1, any, 64, 1}, Rung::kNative, 0, {"llmp_hip_paged_store"}, "a workgroup a page and head");
+  add("llmp.paged.read", "paged.read", {"paged_q8"}, {1, any, 64, 1}, Rung::kNative, 0, {"llmp_hip_paged_read"}, "a workgroup a page and head");
+  add("llmp.paged.attend", "paged.attend", {"paged_q8"}, {1, any, 64, 1}, Rung::kNative, kInt8Mma, {"llmp_hip_paged_attend"},
+      "16 rows a wave on an even cut of the step's tiles and a join; 128 rows a workgroup for prompts");
+  follows_rows();
+  add("llmp.paged.select", "paged.select", {"paged_q8"}, {1, any, 64, 1}, Rung::kNative, kInt8Mma, {"llmp_hip_paged_select"},
+      "page bounds on the matrix cores, the choice by their bits; one launch or two");
   // One token through a routed-expert layer: the router, the experts' products, their GLU and the ordered sum fused
   // (no single counterpart in the reference: ir/decompose.cc:1080-1109 holds the five operations).
   add("llmp.moe.token", "fused.moe_ffn_token", {"q4_k"}, {1, 1, 256, 256}, Rung::kNative, 0, {"llmp_hip_moe_token"},

@@ -1,5 +1,8 @@
 """The paged 8-bit KV cache on the device (llmp_hip_paged_*) against its operators' definitions in tests/paged_plain.py: the
 plan, the store and the selection bit for bit, the attention within the distance that its stated roundings give."""
+import importlib.util
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -505,6 +508,28 @@ def test_a_server_of_the_operators(device):
             held = after
     stream.synchronize()
     assert counters.cpu().tolist()[2] == 0
+
+
+@pytest.mark.parametrize("keep", [0, 3])
+def test_the_example_server(device, keep):
+    """examples/paged_server.py: two layers on one plan, requests that come, answer and end, against the definition over each cache."""
+    spec = importlib.util.spec_from_file_location("paged_server", os.path.join(os.path.dirname(__file__), "..", "examples", "paged_server.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    g = np.random.default_rng(97)
+    server = module.PagedServer(3, 24, 8, layers=2, heads=8, kv_heads=2, head_dim=64, page=16, keep=keep, device=device)
+    for after in ([100, 0, 33], [101, 1, 34], [102, 40, 0], [103, 41, 1], [0, 42, 2]):
+        before = server.lengths.cpu().numpy()
+        fresh = np.maximum(np.array(after) - before, 0)
+        rows = [[g.standard_normal((fresh.sum(), h, 64)).astype(np.float32) for h in (8, 2, 2)] for _ in range(2)]
+        x, plan = server.step(dev(np.array(after, dtype=np.int32), device), int(fresh.sum()), int(fresh.max()),
+                              lambda layer, x: [dev(v, device) for v in rows[layer]])
+        assert plan["counters"][2].item() == 0 and plan["lengths"].tolist() == after
+        cache = {name: v.cpu().numpy() for name, v in server.caches[1].items()}
+        table, starts = server.table.cpu().numpy(), plan["starts"].tolist()
+        lists = plain.lists(cache, rows[1][0], table, after, starts, keep) if keep and fresh.max() == 1 else None
+        want, far = plain.attend(cache, rows[1][0], table, after, starts, 0.125, "f32", picked=lists)
+        assert np.all(np.abs(x.double().cpu().numpy() - want) <= far)
 
 
 def test_captured_launches_replay_at_other_lengths(device):
