@@ -14,6 +14,10 @@
 //   O^T += V^T P^T by v_mfma_f32_16x16x32_f16 takes P from the same lane's registers, and in which V, stored with the tokens
 //   innermost, is 16 bytes of one dimension a lane.
 // A lane's 16 tokens are of one page (pages are multiples of 16): one scale each for K and V.
+//
+// Measured (both launches, 8 KV heads): 131072 tokens of one request at head size 128, 268 MB, 61 us, 4.4 TB/s (a large copy reaches
+// 4.9, a read alone 7.0); 32 requests of up to 16384 tokens, 460 MB, 99 us, 4.6 TB/s; 8192 tokens at 256 in F32, 34 MB, a tile a
+// wave, 19.6 us: that is the chain of a launch, the lengths, the table, one tile and the waves' meeting, and the join's.
 #include <cmath>
 #include <type_traits>
 
@@ -541,6 +545,7 @@ __device__ __forceinline__ bool JoinParts(int count, const float* sink, F&& part
 }
 
 // grid (workgroups of the first launch, rows of a segment): the parts of the segment that begins in workgroup x and ends in another.
+// 4 to 5 us, what a launch with two reads after each other takes; 7.6 us for rows of 64 parts.
 template <int TYPE, int D, bool LISTS>
 __global__ __launch_bounds__(kFewThreads) void FewJoinKernel(const PagedAttendArgs a) {
   constexpr int kPer = D / kWave;

@@ -14,7 +14,9 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kOneLaunchRequests = 1024;  // their sums in LDS
-constexpr int kOneLaunchOutputs = 4096;   // tokens and work items together: a few sweeps
+// Tokens and work items together: a few sweeps. (One launch and two, us: 1000 requests of a token 8.9 and 8.6, 300 of 4 6.5 and 7.2, 8
+// of 250 5.6 and 6.5, of 500, past this, 13 in one workgroup of 256 and 6.5 in two launches.)
+constexpr int kOneLaunchOutputs = 4096;
 constexpr int kSearchRequests = 4096;     // the second launch's sums in LDS
 
 // A request's numbers before the sums.
@@ -212,7 +214,8 @@ __device__ __forceinline__ int TakenOf(const PlanTotals& t) { return min(t.wants
 // (All of them, unless the ring's count was wrong.)
 __device__ __forceinline__ int BackOf(const llmp_paged_plan& op, const PlanTotals& t) { return min(t.gives, op.ring_size - t.free); }
 
-// THREADS: 256 for up to 256 requests, whose barriers four waves then meet at, or 1024.
+// THREADS: 256 for a decode step's few outputs, whose barriers four waves then meet at, or 1024 (64 requests of a token 3.3 us and
+// 4.4, 200 5.2 and 5.4, 256 5.3 and 4.6). What a launch costs at all is 2 to 3 us of that.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void PlanOneKernel(const llmp_paged_plan op) {
   constexpr int kMost = THREADS;  // requests
@@ -348,7 +351,7 @@ extern "C" int llmp_hip_paged_plan(const llmp_paged_plan* op, void* stream) {
   const hipStream_t on = static_cast<hipStream_t>(stream);
   const int64_t outputs = static_cast<int64_t>(op->tokens) + op->work_items;
   if (op->requests <= kOneLaunchRequests && outputs <= kOneLaunchOutputs) {
-    if (op->requests <= 256 && outputs <= 1024) {
+    if (op->requests <= 256 && outputs < 512) {
       hipLaunchKernelGGL(PlanOneKernel<256>, dim3(1), dim3(256), 0, on, *op);
     } else {
       hipLaunchKernelGGL(PlanOneKernel<kPlanThreads>, dim3(1), dim3(kPlanThreads), 0, on, *op);

@@ -11,10 +11,15 @@
 // LDS rows are 16-byte pieces in an order turned by the row (Turn), so that the 32 rows a matrix operand reads lie in
 // different banks.
 //
-// A first small launch lists the (request, 128 rows) pairs and their tiles. With at least as many (pair, head) segments as workgroups
-// each is one workgroup's, longest first, dealt to the compute units there and back so that a unit's two workgroups
-// together have about the same; with fewer, all segments' tiles lie on one line that the workgroups share evenly, and a third
-// launch joins the parts.
+// A first small launch lists the (request, 128 rows) pairs and their tiles. With at least as many (pair, head) segments as workgroups,
+// none of them longer than a compute unit's share, each is one workgroup's, longest first, dealt to the compute units there and
+// back so that a unit's two workgroups together have about the same; otherwise all segments' tiles lie on one line that the workgroups
+// share evenly, and a third launch joins the parts. In us, whole against shared, 8 KV heads: a chunk of 2048 behind 2048 tokens
+// (groups of 4 at 128) 154/172, behind 6000 319/346, a prompt of 4000 (groups of 2 at 256) 196/216; of 2000 there, whose last 128
+// rows are nearly twice the share, 102/90, 6 ragged prompts 147/109.
+//
+// Measured at the chunk of 2048 behind 2048, 103 GFLOP: 150 us, 0.69 PFLOP/s (a large F16 product by the library reaches 1.15): 388
+// vector operations a wave's 32 x 64 logits, about 1800 cycles beside the products' 1024, at two waves a SIMD.
 #include <type_traits>
 
 #include "paged_attend.h"
@@ -60,8 +65,9 @@ struct ManyArgs {
 };
 
 // A few-row request (a prompt's neighbours that decode) is taken along where all of them make the line no longer than this many
-// tiles a compute unit, about what the few rows' two launches cost (6 requests at head size 256, one of them decoding, 123 us without
-// and 109 with; 8 at 128 105 and 100).
+// tiles a compute unit, about what the few rows' two launches cost: there a row's tile is 128 rows' work. In us, taken along and by
+// the few rows' form: 8 of 500 tokens beside a prompt of 1000 52/57, 4 of 60000 beside 256 180/141, 10 of 20000 beside 2000
+// 623/188 (8 KV heads of 128); 6 ragged requests at 256 109/123.
 constexpr int kTakeAlong = 8, kTakeAlongRequests = kListThreads;
 
 __device__ __forceinline__ int ChunksOf(const PagedAttendArgs& a, const PagedRequest& q, int few_rows) {
@@ -77,11 +83,14 @@ __device__ __forceinline__ void TilesOf(const PagedAttendArgs& a, Pair* pair) {
   pair->tiles = max((to + kTileTokens - 1) / kTileTokens - pair->first_tile, 1);  // (rows that see nothing are written too)
 }
 
-// One workgroup: the pairs in the order of the requests, their sums, and their order by length.
+// One workgroup: the pairs in the order of the requests, their sums, and their order by length, a thread a pair. 6 to 7 us, a chain of
+// reads and barriers.
 __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int groups) {
   __shared__ int64_t wave_sums[kListThreads / kWave];
   __shared__ int buckets[kBuckets], first_pair[kListThreads];
   __shared__ PagedRequest requests[kListThreads];
+  __shared__ int longest;
+  if (threadIdx.x == 0) longest = 0;
   const PagedAttendArgs& a = m.a;
   const llmp_paged_attend& op = a.op;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
@@ -146,6 +155,7 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
         length = static_cast<int64_t>(pair.tiles + kVisit) * op.cache.kv_heads;
         m.list.pairs[count + p] = pair;
         atomicAdd(&buckets[kBuckets - 1 - min(pair.tiles / 4, kBuckets - 1)], 1);
+        atomicMax(&longest, pair.tiles + kVisit);
       }
       int64_t all;
       const int64_t upto = block_sum(length, &all);
@@ -168,7 +178,7 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
     m.list.header->total = before;
     m.list.header->pairs = static_cast<int>(count);
     m.list.header->all = all_taken;
-    m.list.header->whole = count * op.cache.kv_heads >= groups;
+    m.list.header->whole = count * op.cache.kv_heads >= groups && longest * static_cast<int64_t>(groups / m.a_unit) <= before;
   }
 }
 
@@ -612,7 +622,8 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
 }
 
 // grid (workgroups of the launch before, kManyRows / 16): the parts of the segment that begins in workgroup x and ends in
-// another, a wave a row, four rows a wave. (Parts are few here and rows many.)
+// another, a wave four rows, asked for together, two parts at a time. (Parts are few here and rows many: 208 segments in 213
+// workgroups at head size 256, 28 MB of parts, 12.8 us.)
 template <int TYPE, int D>
 __global__ __launch_bounds__(kJoinThreads) void ManyJoinKernel(const ManyArgs m) {
   constexpr int kPer = D / kWave;

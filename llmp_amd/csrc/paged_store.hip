@@ -8,6 +8,11 @@
 //
 // A scale is F32(largest magnitude * F32(1 / 127)), a code the nearest to the IEEE quotient value / scale: single roundings, so
 // that the definition is the same in any program, bit for bit.
+//
+// Measured: a decode step of 63 tokens, 8 KV heads of 128, 5.8 us, the chain of item, rows, barrier and codes; prompts of 3139 tokens,
+// 8 heads of 256 in F16, 18.8 us for 39 MB, 2.1 TB/s (the chain again, with every workgroup on the device at once: rows kept in
+// registers, four a thread, took 20.0 us and the decode step 8.6, with code for four rows' divisions where one row is). Reading 14 MB of
+// codes back as 27 MB of F16 values 8.2 us, 4.9 TB/s.
 #include "paged.h"
 
 namespace llmp_hip {
