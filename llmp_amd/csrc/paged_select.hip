@@ -373,11 +373,10 @@ __global__ __launch_bounds__(kWholeThreads) void WholeKernel(const SelectArgs a,
   __shared__ float units[kWholeWaves];
   const llmp_paged_select& op = a.op;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), head = blockIdx.y;
-  if (blockIdx.x == 0) {  // rows of no request
-    const int begin = op.starts[0], end = max(op.starts[op.requests], 0);
-    for (int token = 0; token < op.tokens; ++token) {
-      if (token >= begin && token < end) token = end;
-      if (token >= op.tokens) break;
+  {  // rows of no request, a share of them each workgroup's
+    const int begin = op.starts[0], end = op.starts[op.requests];
+    for (int token = blockIdx.x; token < op.tokens; token += gridDim.x) {
+      if (token >= begin && token < end) continue;
       for (int i = tid; i < op.keep; i += kWholeThreads) op.lists[(static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.keep + i] = -1;
     }
   }

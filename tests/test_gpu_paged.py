@@ -266,6 +266,15 @@ def test_prompts_beside_decoding_requests(device, longest):
     run_attend(device, cache, g.standard_normal((starts[-1], 8, 64)), table, lengths, starts, 0.125, "f16")
 
 
+def test_a_prompt_among_more_requests_than_the_list_takes_at_once(device):
+    g = np.random.default_rng(1101)
+    fresh = [1, 0, 2, 1, 1] * 230
+    fresh[7], fresh[1100] = 90, 40
+    lengths = [max(n, int(g.integers(0, 120))) for n in fresh]
+    cache, table, lengths, starts = serving(g, lengths, fresh, 1, 16, 64)
+    run_attend(device, cache, g.standard_normal((starts[-1], 4, 64)), table, lengths, starts, 0.125, "bf16")
+
+
 @pytest.mark.parametrize("fresh", [0, 1, 5, 33, 100])
 def test_one_request_of_fewer_tokens_than_rows(device, fresh):
     """The rows' count says what may come, the starts what does: a captured step answers both."""
