@@ -682,7 +682,7 @@ def _paged_cache(cache):
 
 def _int32(*tensors):
     for t in tensors:
-        assert t.dtype is torch.int32 and t.stride(-1) == 1, "int32 arrays in one piece"
+        assert t.dtype is torch.int32 and (t.is_contiguous() or t.stride(-1) == 1), "int32 arrays in one piece"
 
 
 _UNITS = {}
@@ -716,13 +716,22 @@ def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
     items = lib.llmp_hip_paged_work_items(n, tokens, page)
     scratch_ints = lib.llmp_hip_paged_plan_scratch(n) // 4
     if out is None:
-        # One allocation: the work items and the scratch first, at 16-byte boundaries.
+        # One allocation, its pieces' places counted and not asked for one by one (the host's part of a call is as long as the
+        # launch): the work items and the scratch first, at 16-byte boundaries.
         padded = (scratch_ints + 3) // 4 * 4
-        work, scratch, slots, positions, requests, starts, lengths, counted = torch.empty(
-            4 * items + padded + 3 * tokens + 2 * n + 4, dtype=torch.int32, device=before.device).split_with_sizes(
+        whole = torch.empty(4 * items + padded + 3 * tokens + 2 * n + 4, dtype=torch.int32, device=before.device)
+        work, _, slots, positions, requests, starts, lengths, counted = whole.unsafe_split_with_sizes(
             (4 * items, padded, tokens, tokens, tokens, n + 1, n, 3))
         out = {"work": work.view(items, 4), "slots": slots, "positions": positions, "requests": requests, "starts": starts, "lengths": lengths,
                "counters": counted}
+        at_work = whole.data_ptr()
+        at_scratch = at_work + 16 * items
+        at_slots = at_scratch + 4 * padded
+        at_positions = at_slots + 4 * tokens
+        at_requests = at_positions + 4 * tokens
+        at_starts = at_requests + 4 * tokens
+        at_lengths = at_starts + 4 * (n + 1)
+        at_counted = at_lengths + 4 * n
     else:
         work, slots, positions, requests, starts, lengths, counted = (
             out[name] for name in ("work", "slots", "positions", "requests", "starts", "lengths", "counters"))
@@ -731,9 +740,11 @@ def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
         assert slots.numel() >= tokens and positions.numel() >= tokens and requests.numel() >= tokens
         items = work.shape[0]
         scratch = torch.empty(scratch_ints, dtype=torch.int32, device=before.device)
-    op = _lib.PagedPlan(before.data_ptr(), after.data_ptr(), table.data_ptr(), ring.data_ptr(), counters.data_ptr(), counted.data_ptr(),
-                        starts.data_ptr(), lengths.data_ptr(), slots.data_ptr(), positions.data_ptr(), requests.data_ptr(), work.data_ptr(),
-                        scratch.data_ptr(), _table_stride(table), n, width, ring.shape[0], page, tokens, items)
+        at_work, at_scratch, at_slots, at_positions, at_requests, at_starts, at_lengths, at_counted = (
+            x.data_ptr() for x in (work, scratch, slots, positions, requests, starts, lengths, counted))
+    op = _lib.PagedPlan(before.data_ptr(), after.data_ptr(), table.data_ptr(), ring.data_ptr(), counters.data_ptr(), at_counted, at_starts,
+                        at_lengths, at_slots, at_positions, at_requests, at_work, at_scratch, _table_stride(table), n, width, ring.shape[0], page,
+                        tokens, items)
     _lib.check(lib.llmp_hip_paged_plan(C.byref(op), _stream()))
     return out
 
