@@ -39,6 +39,11 @@ struct FewRequest {
   int tiles;
   uint32_t units;
 };
+// A segment's units: whole rounds of the workgroup's waves, so that a run of rounds ends where a segment does (a workgroup with the
+// end of one and the beginning of another takes both their visits: 217 tokens of a request and two shorter ones, 25 us and 13).
+__device__ __forceinline__ uint32_t SegmentUnits(int tiles, int shift) {
+  return static_cast<uint32_t>(shift > 0 ? ((tiles - 1) >> shift) + 1 : (tiles + kFewWaves - 1) / kFewWaves * kFewWaves);
+}
 template <bool LISTS>
 __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r) {
   const llmp_paged_attend& op = a.op;
@@ -56,7 +61,7 @@ __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r) {
     f.tiles = max((f.q.length + kTileTokens - 1) / kTileTokens - f.first_tile, 1);  // (a row that sees nothing is written too)
   }
   f.segments = chunks * op.cache.kv_heads;
-  f.units = static_cast<uint32_t>(f.segments) * static_cast<uint32_t>(((f.tiles - 1) >> a.shift) + 1);
+  f.units = static_cast<uint32_t>(f.segments) * SegmentUnits(f.tiles, a.shift);
   return f;
 }
 // Lane `lane`'s in every lane.
@@ -124,17 +129,13 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
   };
   FewRequest mine = block(0);
   uint32_t upto = WaveSums(mine.units);
-  uint32_t total = __builtin_amdgcn_readlane(upto, kWave - 1), segments = __builtin_amdgcn_readlane(WaveSums(mine.segments), kWave - 1);
+  uint32_t total = __builtin_amdgcn_readlane(upto, kWave - 1);
   for (int base = kWave; base < op.requests; base += kWave) {
     const FewRequest f = block(base);
     total += __builtin_amdgcn_readlane(WaveSums(f.units), kWave - 1);
-    segments += __builtin_amdgcn_readlane(WaveSums(f.segments), kWave - 1);
   }
-  // Whole rounds of the waves; where a round is more than there is, no more than an average segment (short ones are not strung
-  // together while there are workgroups for each).
   const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
   uint32_t per = (even + kFewWaves - 1) / kFewWaves * kFewWaves;
-  if (even < kFewWaves) per = min(per, max(even, (total + segments - 1) / max(segments, 1u)));
   if (LISTS && a.whole_units > 0) per = a.whole_units;
   const uint32_t group = OnChiplet(blockIdx.x, gridDim.x, (total + per - 1) / max(per, 1u));
   uint32_t u = group * per;
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
       ++r;
       continue;
     }
-    const uint32_t a_segment = static_cast<uint32_t>(((f.tiles - 1) >> a.shift) + 1);  // units
+    const uint32_t a_segment = SegmentUnits(f.tiles, a.shift);
     const int segment = __builtin_amdgcn_readfirstlane(static_cast<int>((u - before) / a_segment));
     const uint32_t in_segment = u - before - segment * a_segment, u_count = min(a_segment - in_segment, u_end - u);
     const int t_first = static_cast<int>(in_segment << a.shift), t_count = min(f.tiles - t_first, static_cast<int>(u_count << a.shift));
@@ -621,7 +622,7 @@ int FewShift(const llmp_paged_attend& op) {
   const int64_t tokens = op.lists != nullptr ? static_cast<int64_t>(op.list_pages) * op.cache.page : static_cast<int64_t>(op.table_width) * op.cache.page;
   const int64_t tiles = tokens / kTileTokens + 1;
   int shift = 0;
-  while (segments * ((tiles >> shift) + 1) >= 1ll << 31 && shift < 24) ++shift;
+  while (segments * ((tiles >> shift) + kFewWaves) >= 1ll << 31 && shift < 24) ++shift;
   return shift;
 }
 // With page lists all segments are of one size. Workgroups take whole ones (this many units) where an even cut would save less than
@@ -633,7 +634,8 @@ int WholeUnits(const PagedAttendArgs& args, int groups) {
   const llmp_paged_attend& op = args.op;
   if (op.lists == nullptr || args.shift > 0) return 0;
   const int64_t segments = static_cast<int64_t>(op.tokens) * ((args.group + kRows - 1) / kRows) * op.cache.kv_heads;
-  const int64_t a_segment = (static_cast<int64_t>(op.list_pages) * op.cache.page + kTileTokens - 1) / kTileTokens;
+  const int64_t tiles = (static_cast<int64_t>(op.list_pages) * op.cache.page + kTileTokens - 1) / kTileTokens;
+  const int64_t a_segment = (tiles + kFewWaves - 1) / kFewWaves * kFewWaves;
   const int64_t even = (segments * a_segment + groups - 1) / groups, whole = a_segment * ((segments + groups - 1) / groups);
   return whole <= even + even / 8 + kVisit ? static_cast<int>(whole) : 0;
 }
