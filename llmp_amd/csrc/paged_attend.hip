@@ -29,6 +29,7 @@ namespace {
 constexpr int kFewWaves = 4;
 constexpr int kFewThreads = kFewWaves * kWave;
 constexpr int kRows = 16;  // rows of a segment: (token, head) pairs
+constexpr uint32_t kVisit = 8;  // what a segment's beginning and end cost a workgroup, in tiles
 
 // A request's segments and tiles in this form. A unit of the line is 2^shift tiles of a segment (shift 0 but where the line would
 // pass 2^31).
@@ -41,11 +42,12 @@ struct FewRequest {
 };
 // A segment's units: whole rounds of the workgroup's waves, so that a run of rounds ends where a segment does (a workgroup with the
 // end of one and the beginning of another takes both their visits: 217 tokens of a request and two shorter ones, 25 us and 13).
-__device__ __forceinline__ uint32_t SegmentUnits(int tiles, int shift) {
-  return static_cast<uint32_t>(shift > 0 ? ((tiles - 1) >> shift) + 1 : (tiles + kFewWaves - 1) / kFewWaves * kFewWaves);
+__device__ __forceinline__ uint32_t SegmentUnits(int tiles, int shift, uint32_t round) {
+  if (shift > 0) return static_cast<uint32_t>(((tiles - 1) >> shift) + 1);
+  return round == kFewWaves ? (static_cast<uint32_t>(tiles) + kFewWaves - 1) / kFewWaves * kFewWaves : (static_cast<uint32_t>(tiles) + round - 1) / round * round;
 }
 template <bool LISTS>
-__device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r) {
+__device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r, uint32_t round) {
   const llmp_paged_attend& op = a.op;
   FewRequest f;
   f.q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
@@ -61,7 +63,7 @@ __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r) {
     f.tiles = max((f.q.length + kTileTokens - 1) / kTileTokens - f.first_tile, 1);  // (a row that sees nothing is written too)
   }
   f.segments = chunks * op.cache.kv_heads;
-  f.units = static_cast<uint32_t>(f.segments) * SegmentUnits(f.tiles, a.shift);
+  f.units = static_cast<uint32_t>(f.segments) * SegmentUnits(f.tiles, a.shift, round);
   return f;
 }
 // Lane `lane`'s in every lane.
@@ -122,20 +124,38 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
     return;
   }
   // ---- this workgroup's run of the line of units: the requests 64 at a time, a lane each.
+  uint32_t round = kFewWaves;
   const auto block = [&](int base) {
     FewRequest f = {};
-    if (base + lane < op.requests) f = FewOf<LISTS>(a, base + lane);
+    if (base + lane < op.requests) f = FewOf<LISTS>(a, base + lane, round);
     return f;
   };
   FewRequest mine = block(0);
   uint32_t upto = WaveSums(mine.units);
-  uint32_t total = __builtin_amdgcn_readlane(upto, kWave - 1);
-  for (int base = kWave; base < op.requests; base += kWave) {
-    const FewRequest f = block(base);
-    total += __builtin_amdgcn_readlane(WaveSums(f.units), kWave - 1);
-  }
+  // f(request) summed over all requests; the first 64 are at hand.
+  const auto over_all = [&](auto&& f) {
+    uint32_t sum = __builtin_amdgcn_readlane(WaveSums(f(mine)), kWave - 1);
+    for (int base = kWave; base < op.requests; base += kWave) sum += __builtin_amdgcn_readlane(WaveSums(f(block(base))), kWave - 1);
+    return sum;
+  };
+  const auto units_of = [](const FewRequest& f) { return f.units; };
+  uint32_t total = over_all(units_of);
   const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
   uint32_t per = (even + kFewWaves - 1) / kFewWaves * kFewWaves;
+  // A run a little longer may let every workgroup stay in one segment: a second's visit costs about kVisit tiles. (12 requests of up to
+  // 2000 tokens at head size 256 26.4 us without, 23.1 with; 30 of up to 3000 at 128 28.8 and 27.0.)
+  if (!LISTS && a.shift == 0 && per > kFewWaves) {
+    const auto fits = [&](uint32_t run) {
+      return over_all([&](const FewRequest& f) { return f.segments * ((static_cast<uint32_t>(f.tiles) + run - 1) / run); }) <= gridDim.x;
+    };
+    if (fits(per + kVisit)) {
+      while (!fits(per)) per += kFewWaves;  // (at the latest there)
+      round = per;
+      mine = block(0);
+      upto = WaveSums(mine.units);
+      total = over_all(units_of);
+    }
+  }
   if (LISTS && a.whole_units > 0) per = a.whole_units;
   const uint32_t group = OnChiplet(blockIdx.x, gridDim.x, (total + per - 1) / max(per, 1u));
   uint32_t u = group * per;
@@ -174,7 +194,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
       ++r;
       continue;
     }
-    const uint32_t a_segment = SegmentUnits(f.tiles, a.shift);
+    const uint32_t a_segment = SegmentUnits(f.tiles, a.shift, round);
     const int segment = __builtin_amdgcn_readfirstlane(static_cast<int>((u - before) / a_segment));
     const uint32_t in_segment = u - before - segment * a_segment, u_count = min(a_segment - in_segment, u_end - u);
     const int t_first = static_cast<int>(in_segment << a.shift), t_count = min(f.tiles - t_first, static_cast<int>(u_count << a.shift));
@@ -629,7 +649,7 @@ int FewShift(const llmp_paged_attend& op) {
 // what it costs: a second segment's beginning and end, and the joining launch. In us, cut evenly against whole, 4 KV heads of 128, groups
 // of 4, 512 workgroups: 16 segments of 2, 12, 16 tiles 8.5/6.8, 10.7/10.3, 10.9/12.0; 64 of 8, 16, 64 10.4/8.8, 11.5/12.2, 19/30;
 // 256 of 8, 24 14.3/9.4, 20.6/16.6; 400 of 12, 24, 64 17.4/15.1, 29.2/22.1, 49/44; 800 of 24, 64 44.2/39.4, 80/83.
-constexpr int kVisit = 12;
+constexpr int kSaving = 12;
 int WholeUnits(const PagedAttendArgs& args, int groups) {
   const llmp_paged_attend& op = args.op;
   if (op.lists == nullptr || args.shift > 0) return 0;
@@ -637,7 +657,7 @@ int WholeUnits(const PagedAttendArgs& args, int groups) {
   const int64_t tiles = (static_cast<int64_t>(op.list_pages) * op.cache.page + kTileTokens - 1) / kTileTokens;
   const int64_t a_segment = (tiles + kFewWaves - 1) / kFewWaves * kFewWaves;
   const int64_t even = (segments * a_segment + groups - 1) / groups, whole = a_segment * ((segments + groups - 1) / groups);
-  return whole <= even + even / 8 + kVisit ? static_cast<int>(whole) : 0;
+  return whole <= even + even / 8 + kSaving ? static_cast<int>(whole) : 0;
 }
 bool HasMany(const llmp_paged_attend& op) {
   const int64_t group = op.heads / op.cache.kv_heads, rows = op.tokens * group;  // (the heads of all tokens: at most 2^30)

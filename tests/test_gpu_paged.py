@@ -266,6 +266,16 @@ def test_prompts_beside_decoding_requests(device, longest):
     run_attend(device, cache, g.standard_normal((starts[-1], 8, 64)), table, lengths, starts, 0.125, "f16")
 
 
+@pytest.mark.parametrize("requests,kv_heads,d", [(70, 4, 128), (40, 2, 256), (130, 4, 64)])
+def test_runs_of_a_workgroup_longer_than_a_round(device, requests, kv_heads, d):
+    """Segments of unlike lengths, as many tiles as make a workgroup's run several rounds of its waves: whole segments and cut ones."""
+    g = np.random.default_rng(requests)
+    lengths = [int(n) for n in g.integers(700, 1100, requests)]
+    lengths[3], lengths[-1] = 1, 2900
+    cache, table, lengths, starts = serving(g, lengths, [1] * requests, kv_heads, 32, d)
+    run_attend(device, cache, g.standard_normal((requests, 2 * kv_heads, d)), table, lengths, starts, d ** -0.5, "bf16")
+
+
 def test_a_prompt_among_more_requests_than_the_list_takes_at_once(device):
     g = np.random.default_rng(1101)
     fresh = [1, 0, 2, 1, 1] * 230
