@@ -3,6 +3,7 @@
 lib/libllmp_hip.so and only queues work, as the reference's Run* operators do
 (src/kernels/ggml/vecq.cu:1095-1175)."""
 import ctypes as C
+import functools
 
 import torch
 
@@ -702,6 +703,13 @@ def _table_stride(table):
     return table.stride(0) if table.shape[0] > 1 else table.shape[1]
 
 
+@functools.lru_cache(maxsize=1024)
+def _plan_sizes(requests, tokens, page):
+    """(Work items, I32 of scratch) of a plan of these sizes."""
+    lib = _lib.load()
+    return lib.llmp_hip_paged_work_items(requests, tokens, page), lib.llmp_hip_paged_plan_scratch(requests) // 4
+
+
 def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
     """llmp.paged.plan: what a step does to a paged cache, from the requests' lengths before and after it (int32
     [requests]). `table` (int32 [requests, width]) and `ring` (int32, the free pages) are updated in place; `counters` is
@@ -713,8 +721,7 @@ def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
     _int32(before, after, table, ring, counters)
     n, width = table.shape
     assert before.shape == after.shape == (n,) and ring.dim() == 1 and counters.numel() >= 2
-    items = lib.llmp_hip_paged_work_items(n, tokens, page)
-    scratch_ints = lib.llmp_hip_paged_plan_scratch(n) // 4
+    items, scratch_ints = _plan_sizes(n, tokens, page)
     if out is None:
         # One allocation, its pieces' places counted and not asked for one by one (the host's part of a call is as long as the
         # launch): the work items and the scratch first, at 16-byte boundaries.
