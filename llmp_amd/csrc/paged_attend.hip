@@ -16,7 +16,7 @@
 // A lane's 16 tokens are of one page (pages are multiples of 16): one scale each for K and V.
 //
 // Measured (both launches, 8 KV heads): 131072 tokens of one request at head size 128, 268 MB, 61 us, 4.4 TB/s (a large copy reaches
-// 4.9, a read alone 7.0); 32 requests of up to 16384 tokens, 460 MB, 99 us, 4.6 TB/s; 8192 tokens at 256 in F32, 34 MB, a tile a
+// 4.9, a read alone 7.0); 32 requests of up to 16384 tokens, 453 MB, 98 us, 4.6 TB/s; 8192 tokens at 256 in F32, 34 MB, a tile a
 // wave, 19.6 us: that is the chain of a launch, the lengths, the table, one tile and the waves' meeting, and the join's.
 #include <cmath>
 #include <type_traits>
