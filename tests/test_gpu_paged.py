@@ -590,6 +590,45 @@ def test_captured_launches_replay_at_other_lengths(device):
         assert np.all(np.abs(out.double().cpu().numpy() - want) <= far)
 
 
+def test_captured_prompts_and_selections_replay_at_other_lengths(device):
+    """The launches of a step of at most 300 tokens, the prompts' form and a selection in one launch among them, with other tokens a request."""
+    g = np.random.default_rng(93)
+    cache, table, lengths, starts = serving(g, [900, 500, 400], [200, 60, 40], 4, 16, 64)
+    table = widened(table, cache, 300, 300, 16)
+    c, t = to_device(cache, device), dev(table[:, :80], device)
+    wide, n, s = dev(table, device), dev(lengths, device), dev(starts, device)
+    q = dev(g.standard_normal((300, 16, 64)).astype(np.float32), device)
+    out, lists = torch.zeros_like(q), torch.zeros((300, 4, 6), dtype=torch.int32, device=device)
+    scratch, scores = torch.empty(256 << 20, dtype=torch.uint8, device=device), torch.empty(16 << 20, dtype=torch.uint8, device=device)
+
+    def work():
+        ops.paged_attend(c, q, wide, n, s, 0.125, most=300, out=out, scratch=scratch)
+        ops.paged_select(c, q, t, n, s, 6, most=300, out=lists, scratch=scores)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        work()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        work()
+    for step, (now, fresh) in enumerate([([900, 500, 400], [200, 60, 40]), ([17, 299, 1], [17, 250, 1]), ([650, 64, 400], [0, 1, 299]), ([900, 500, 400], [1, 1, 1])]):
+        n.copy_(torch.tensor(now, dtype=torch.int32))
+        begins = [0, fresh[0], fresh[0] + fresh[1], sum(fresh)]
+        s.copy_(torch.tensor(begins, dtype=torch.int32))
+        q.copy_(dev(g.standard_normal((300, 16, 64)).astype(np.float32), device))
+        scratch.random_(0, 256)  # what a call before left there is no matter
+        out.zero_(), lists.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        end = begins[3]
+        want, far = plain.attend(cache, q.cpu().numpy(), table, now, begins, 0.125, "f32")
+        assert np.all(np.abs(out[:end].double().cpu().numpy() - want[:end]) <= far[:end]), f"replay {step}"
+        assert bool((out[end:] == 0).all())
+        same(lists, plain.lists(cache, q.cpu().numpy(), table, now, begins, 6), f"replay {step}")
+
+
 def test_seeded_inputs_are_what_synth_gives(device):
     """The benchmark's own activations through the cache: BF16 values that many codes hold."""
     x = synth.bf16_to_f32(synth.bf16_bits(synth.activations(64, 256, 3))).reshape(64, 2, 128)
