@@ -37,16 +37,18 @@ class PagedServer:
     def step(self, after, tokens, most, project):
         """Lengths `after` (int32 [slots], on the device: more than before for new tokens, 0 for a request that has ended), `tokens` new ones
         in all and at most `most` of a request. project(layer, x) gives the layer's q, k, v of the step's rows from the layer before's output
-        (None for the first). Returns the last layer's output and the plan."""
-        plan = ops.paged_plan(self.lengths, after, self.table, self.ring, self.counters, self.page, tokens)
+        (None for the first). Returns the last layer's output and the plan. When the pages run out the tokens without one (the plan's
+        third counter) are not in the cache: their rows are answered from what is, and a server stores them again in a later step."""
+        before = self.lengths
+        plan = ops.paged_plan(before, after, self.table, self.ring, self.counters, self.page, tokens)
         self.lengths, self.counters = plan["lengths"], plan["counters"]
         where = (self.table, plan["lengths"], plan["starts"])
         x = None
         for layer, cache in enumerate(self.caches):
             q, k, v = project(layer, x)
             ops.paged_store(cache, k, v, plan["work"])
-            lists = ops.paged_select(cache, q, *where, self.keep, most=most) if self.keep and most == 1 else None
-            x = ops.paged_attend(cache, q, *where, self.scale, lists=lists, most=most)
+            lists = ops.paged_select(cache, q, *where, self.keep, before=before, most=most) if self.keep and most == 1 else None
+            x = ops.paged_attend(cache, q, *where, self.scale, before=before, lists=lists, most=most)
         return x, plan
 
 

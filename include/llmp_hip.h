@@ -609,7 +609,9 @@ int llmp_hip_decode_matrix_staged(int decoder, const llmp_decode_operand* weight
  *                                                     both null: not kept
  * head_dim is 64, 128 or 256. The cache's arrays lie at 16-byte boundaries. A request's table row names its pages in order
  * (page numbers; one outside [0, pages) is never read or written: its tokens count as not there). Tokens of a step lie request
- * after request: request r's rows are starts[r] to starts[r + 1] - 1, at the last positions of its lengths[r] tokens. */
+ * after request: request r's rows are starts[r] to starts[r + 1] - 1, at positions before[r] on. It holds lengths[r] tokens, which a step
+ * that finds no page for some of them leaves below before[r] plus the new ones: those past it see all that is held. Without
+ * `before` (null) the rows are at the last positions of the lengths[r] tokens, which is the same where every token found a page. */
 typedef struct llmp_paged_cache {
   void* k;
   void* v;
@@ -624,7 +626,8 @@ typedef struct llmp_paged_cache {
  * ones count as zero). A request that shrinks (after < before; 0: it has ended) gives its last pages back, one that grows
  * takes pages for what its last page has no room for. Free pages lie in a ring (I32 [ring_size]; counters_in: {index of the
  * first, how many}): taken from its head in the order of the requests, given back at its tail (those serve the next step).
- * When they run out, later pages are not given: lengths[r] = min(after, what the pages hold). Written:
+ * When they run out, later pages are not given: lengths[r] = min(after, what the pages hold), while the tokens that found none keep
+ * their rows, and their positions with slots of -1. Attention and selection of such a step take `before` too (above). Written:
  *   table     the new pages' entries, nothing else of it
  *   ring      the pages given back
  *   counters  I32 [3]: the ring's first and count after the step, tokens that found no page (may be counters_in)
@@ -679,7 +682,8 @@ int llmp_hip_paged_read(const llmp_paged_cache* cache, const int32_t* pages, int
                         void* v_out, void* stream);
 
 /* llmp.paged.attend: causal attention of a step's queries over their requests' pages: token t of a request with n new
- * tokens is at position p = length - n + t and sees positions max(0, p - window + 1) (window 0: from 0) to p; with `lists`
+ * tokens is at position p = before + t (before null: length - n + t) and sees positions max(0, p - window + 1) (window 0: from 0)
+ * to min(p, length - 1); with `lists`
  * (llmp.paged.select's: I32 [tokens][kv_heads][list_pages], a request's pages by their place in its table row, -1: none, each at most
  * once) only those pages' tokens among them. Logits are scale * q . k, capped to softcap * tanh(logit / softcap) where softcap
  * is not 0; sinks (F32 [heads] or null) adds exp(sink) to a head's sum. A row that sees nothing is zero. q and out are
@@ -701,6 +705,7 @@ typedef struct llmp_paged_attend {
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride, table_stride;
   int32_t type, heads, requests, tokens, most_tokens, table_width, list_pages, window;
   float scale, softcap;
+  const int32_t* before; /* I32 [requests], the plan's; null: every new token found a page */
 } llmp_paged_attend;
 size_t llmp_hip_paged_attend_scratch(const llmp_paged_attend* op, int cus);
 int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream);
@@ -708,7 +713,7 @@ int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch, size_t scr
 /* llmp.paged.select: for every new token and KV head the `keep` pages of its request whose keys could have the largest logit: a
  * head's query as 8-bit codes c of unit u = max|q| * F32(1 / 127) (q / u to nearest even), a page's score the largest of the group's heads' of
  * F32(F32(sum over d of c_d * (c_d > 0 ? high_d : low_d)) * u) * k_scale, which bounds every key's c . k in the page. The token's
- * first `first` and last `recent` pages are always among them (those up to its own count; at most `keep` together); ties go to
+ * first `first` and last `recent` pages are always among them (of the pages with tokens that it sees, as llmp.paged.attend says; at most `keep` together); ties go to
  * the lower page; a score that is not a number counts as the smallest. lists: I32 [tokens][kv_heads][keep], ascending,
  * -1 past a token's pages; tokens past starts[requests] get -1 throughout. scratch: llmp_hip_paged_select_scratch(op) bytes at
  * a 16-byte boundary. The cache has low and high. keep at most 4096. */
@@ -721,6 +726,7 @@ typedef struct llmp_paged_select {
   int32_t* lists;
   int64_t q_token_stride, q_head_stride, table_stride;
   int32_t type, heads, requests, tokens, most_tokens, table_width, keep, first, recent;
+  const int32_t* before; /* I32 [requests], the plan's; null: every new token found a page */
 } llmp_paged_select;
 size_t llmp_hip_paged_select_scratch(const llmp_paged_select* op);
 int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch, size_t scratch_bytes, void* stream);

@@ -143,7 +143,7 @@ class PagedAttend(C.Structure):
                 ("q_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
                 ("table_stride", C.c_int64), ("type", C.c_int32), ("heads", C.c_int32), ("requests", C.c_int32),
                 ("tokens", C.c_int32), ("most_tokens", C.c_int32), ("table_width", C.c_int32), ("list_pages", C.c_int32),
-                ("window", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float)]
+                ("window", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float), ("before", C.c_void_p)]
 
 
 class PagedSelect(C.Structure):
@@ -152,7 +152,7 @@ class PagedSelect(C.Structure):
                 ("lists", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("table_stride", C.c_int64),
                 ("type", C.c_int32), ("heads", C.c_int32), ("requests", C.c_int32), ("tokens", C.c_int32),
                 ("most_tokens", C.c_int32), ("table_width", C.c_int32), ("keep", C.c_int32), ("first", C.c_int32),
-                ("recent", C.c_int32)]
+                ("recent", C.c_int32), ("before", C.c_void_p)]
 
 
 class VecQSource(C.Structure):

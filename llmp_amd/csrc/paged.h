@@ -108,18 +108,23 @@ __device__ __forceinline__ void CodesOf(const float (&x)[8], float scale, float 
   for (int e = 0; e < 8; ++e) code[e] = __builtin_isnan(r[e]) ? 0 : static_cast<int>(fminf(fmaxf(r[e], -127.0f), 127.0f));
 }
 
-// A request's new tokens and length, whatever the device arrays hold: `n` 0 where its rows are not rows of the call.
+// A request's new tokens, the tokens that it holds and the position of the first new one, whatever the device arrays hold: `n` 0 where its
+// rows are not rows of the call. Where `before` is given a token may be past all that is held (it found no page): its position stays,
+// what it sees ends at `length`. Positions stay below 2^31: fewer than 2^30 tokens from at most 2^30 on.
 struct PagedRequest {
-  int start, n, length;
+  int start, n, length, base;
 };
-__device__ __forceinline__ PagedRequest RequestOf(const int32_t* starts, const int32_t* lengths, int r, int tokens, int most_length) {
+__device__ __forceinline__ PagedRequest RequestOf(const int32_t* starts, const int32_t* lengths, const int32_t* before, int r, int tokens, int most_length) {
   const int a = starts[r], b = starts[r + 1];
   PagedRequest q;
   q.start = a;
   q.n = (a >= 0 && b <= tokens && b > a) ? b - a : 0;
   q.length = min(max(lengths[r], 0), most_length);
+  q.base = before != nullptr ? min(max(before[r], 0), static_cast<int>(kMostPagedLength)) : q.length - q.n;
   return q;
 }
+// The end of what the request's token at `position` sees.
+__device__ __forceinline__ int SeenTo(const PagedRequest& q, int position) { return min(position + 1, q.length); }
 
 }  // namespace llmp_hip
 

@@ -50,7 +50,7 @@ template <bool LISTS>
 __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r, uint32_t round) {
   const llmp_paged_attend& op = a.op;
   FewRequest f;
-  f.q = RequestOf(op.starts, op.lengths, r, op.tokens, a.most_length);
+  f.q = RequestOf(op.starts, op.lengths, op.before, r, op.tokens, a.most_length);
   f.first_tile = 0;
   int chunks;
   if constexpr (LISTS) {
@@ -59,7 +59,7 @@ __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r, uin
   } else {
     const int64_t rows = static_cast<int64_t>(f.q.n) * a.group;
     chunks = rows > a.few_rows ? 0 : static_cast<int>((rows + kRows - 1) / kRows);
-    if (op.window > 0) f.first_tile = max(f.q.length - f.q.n - op.window + 1, 0) / kTileTokens;
+    if (op.window > 0) f.first_tile = max(f.q.base - op.window + 1, 0) / kTileTokens;
     f.tiles = max((f.q.length + kTileTokens - 1) / kTileTokens - f.first_tile, 1);  // (a row that sees nothing is written too)
   }
   f.segments = chunks * op.cache.kv_heads;
@@ -69,7 +69,7 @@ __device__ __forceinline__ FewRequest FewOf(const PagedAttendArgs& a, int r, uin
 // Lane `lane`'s in every lane.
 __device__ __forceinline__ FewRequest FewFrom(const FewRequest& f, int lane) {
   const auto from = [&](int v) { return __builtin_amdgcn_readlane(v, lane); };
-  return {{from(f.q.start), from(f.q.n), from(f.q.length)}, from(f.segments), from(f.first_tile), from(f.tiles), static_cast<uint32_t>(from(static_cast<int>(f.units)))};
+  return {{from(f.q.start), from(f.q.n), from(f.q.length), from(f.q.base)}, from(f.segments), from(f.first_tile), from(f.tiles), static_cast<uint32_t>(from(static_cast<int>(f.units)))};
 }
 
 // A tile of K and V of a head.
@@ -216,12 +216,12 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
       first_token = static_cast<int>(PagedDivide(kRows * chunk, a.group_magic));
       last_token = min(static_cast<int>(PagedDivide(kRows * chunk + kRows - 1, a.group_magic)), f.q.n - 1);
     }
-    const int base_position = f.q.length - f.q.n;  // of the request's first new token
+    const int base_position = f.q.base;  // of the request's first new token
     const int position = base_position + token;
     const int window = op.window > 0 ? op.window : INT_MAX / 2;
-    const int see_from = max(position - window + 1, 0), see_to = real ? position + 1 : 0;
-    const int all_from = max(base_position + last_token - window + 1, 0), all_to = base_position + first_token + 1;  // seen by every row
-    const int any_from = max(base_position + first_token - window + 1, 0), any_to = base_position + last_token + 1;  // seen by any
+    const int see_from = max(position - window + 1, 0), see_to = real ? SeenTo(f.q, position) : 0;
+    const int all_from = max(base_position + last_token - window + 1, 0), all_to = SeenTo(f.q, base_position + first_token);  // seen by every row
+    const int any_from = max(base_position + first_token - window + 1, 0), any_to = SeenTo(f.q, base_position + last_token);  // seen by any
 
     // The row's loads before all others: its digits are made while the first tile is on its way.
     QueryPart<TYPE, 2 * kSteps> row;
@@ -681,7 +681,7 @@ int CheckAttend(const llmp_paged_attend* op) {
   if (op->heads / op->cache.kv_heads > kMostGroup) return Refuse(1, "paged_attend: at most %d query heads a KV head, not %d", kMostGroup, op->heads / op->cache.kv_heads);
   if (op->lengths == nullptr || op->starts == nullptr || op->table == nullptr) return Refuse(1, "paged_attend: null operand");
   if ((reinterpret_cast<uintptr_t>(op->lengths) | reinterpret_cast<uintptr_t>(op->starts) | reinterpret_cast<uintptr_t>(op->table) |
-       reinterpret_cast<uintptr_t>(op->lists) | reinterpret_cast<uintptr_t>(op->sinks)) % 4 != 0)
+       reinterpret_cast<uintptr_t>(op->lists) | reinterpret_cast<uintptr_t>(op->sinks) | reinterpret_cast<uintptr_t>(op->before)) % 4 != 0)
     return Refuse(1, "paged_attend: I32 and F32 arrays at 4-byte boundaries");
   if (op->table_stride < op->table_width) return Refuse(1, "paged_attend: a table row of %d entries every %lld", op->table_width, (long long)op->table_stride);
   if (static_cast<int64_t>(op->table_width) * op->cache.page > kMostPagedLength) return Refuse(1, "paged_attend: a table row of at most 2^30 tokens");

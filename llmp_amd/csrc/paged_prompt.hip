@@ -45,7 +45,6 @@ struct ListHeader {
 struct Pair {
   int request, chunk, first_tile, tiles;
   PagedRequest q;
-  int unused;
 };
 static_assert(sizeof(Pair) == 32);
 struct List {
@@ -78,8 +77,8 @@ __device__ __forceinline__ int ChunksOf(const PagedAttendArgs& a, const PagedReq
 __device__ __forceinline__ void TilesOf(const PagedAttendArgs& a, Pair* pair) {
   const PagedRequest& q = pair->q;
   const int first_token = pair->chunk * kManyRows / a.group, last_token = min((pair->chunk * kManyRows + kManyRows - 1) / a.group, q.n - 1);
-  const int to = max(q.length - q.n + last_token + 1, 0), window = a.op.window > 0 ? a.op.window : INT_MAX / 2;
-  pair->first_tile = max(q.length - q.n + first_token - window + 1, 0) / kTileTokens;
+  const int to = max(SeenTo(q, q.base + last_token), 0), window = a.op.window > 0 ? a.op.window : INT_MAX / 2;
+  pair->first_tile = max(q.base + first_token - window + 1, 0) / kTileTokens;
   pair->tiles = max((to + kTileTokens - 1) / kTileTokens - pair->first_tile, 1);  // (rows that see nothing are written too)
 }
 
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(kListThreads) void ListKernel(const ManyArgs m, int
   bool all_taken = false;
   for (int base = 0; base < op.requests; base += kListThreads) {
     const int here = min(op.requests - base, kListThreads);
-    requests[tid] = tid < here ? RequestOf(op.starts, op.lengths, base + tid, op.tokens, a.most_length) : PagedRequest{};
+    requests[tid] = tid < here ? RequestOf(op.starts, op.lengths, op.before, base + tid, op.tokens, a.most_length) : PagedRequest{};
     int64_t pairs;
     int few_rows = a.few_rows;
     if (op.requests <= kTakeAlongRequests) {
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
     const I32x4* const from = reinterpret_cast<const I32x4*>(m.list.pairs + pair_index);
     const I32x4 x = from[0], y = from[1];
     const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    pair = {one(x[0]), one(x[1]), one(x[2]), one(x[3]), {one(y[0]), one(y[1]), one(y[2])}, 0};
+    pair = {one(x[0]), one(x[1]), one(x[2]), one(x[3]), {one(y[0]), one(y[1]), one(y[2]), one(y[3])}};
   };
   const int units = groups / m.a_unit, unit_of = w % units;
   const int64_t segments = static_cast<int64_t>(header.pairs) * c.kv_heads;
@@ -311,14 +310,14 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
     const int token0 = row0 / a.group, in_token0 = row0 - token0 * a.group;  // the wave's first row's
     const int in_tokens = PagedDivide(in_token0 + column, a.group_magic);
     const int token = token0 + in_tokens, query_head = in_token0 + column - in_tokens * a.group;
-    const int base_position = q.length - q.n;
+    const int base_position = q.base;
     const int position = base_position + token;
     const int window = op.window > 0 ? op.window : INT_MAX / 2;
-    const int see_from = max(position - window + 1, 0), see_to = real ? position + 1 : 0;
+    const int see_from = max(position - window + 1, 0), see_to = real ? SeenTo(q, position) : 0;
     const int first_position = base_position + token0;
     const int last_position = base_position + min(token0 + static_cast<int>(PagedDivide(in_token0 + kWaveRows - 1, a.group_magic)), q.n - 1);
-    const int all_from = max(last_position - window + 1, 0), all_to = first_position + 1;
-    const int any_from = max(first_position - window + 1, 0), any_to = row0 < rows ? last_position + 1 : 0;
+    const int all_from = max(last_position - window + 1, 0), all_to = SeenTo(q, first_position);
+    const int any_from = max(first_position - window + 1, 0), any_to = row0 < rows ? SeenTo(q, last_position) : 0;
 
     const float cap_inverse = op.softcap != 0.0f ? 1.0f / op.softcap : 0.0f;
 

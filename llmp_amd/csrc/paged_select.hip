@@ -34,6 +34,11 @@ struct SelectArgs {
   int tokens_a_tile;  // tokens whose heads fill the 16 columns
 };
 
+// How many of its request's pages the token at `position` sees tokens of.
+__device__ __forceinline__ int PagesSeen(const llmp_paged_select& op, const PagedRequest& q, int position) {
+  const int seen = SeenTo(q, position);
+  return seen <= 0 ? 0 : min((seen - 1) / op.cache.page + 1, op.table_width);
+}
 // A tile of a request's tokens: which, and how many pages its last one has.
 struct TokenTile {
   PagedRequest q;
@@ -50,7 +55,7 @@ __device__ __forceinline__ TokenTile TileOf(const SelectArgs& a, uint32_t index)
     uint32_t tiles = 0;
     PagedRequest q = {};
     if (base + lane < op.requests) {
-      q = RequestOf(op.starts, op.lengths, base + lane, op.tokens, a.most_length);
+      q = RequestOf(op.starts, op.lengths, op.before, base + lane, op.tokens, a.most_length);
       tiles = (q.n + a.tokens_a_tile - 1) / a.tokens_a_tile;
     }
     const uint32_t upto = WaveSums(tiles);
@@ -59,10 +64,10 @@ __device__ __forceinline__ TokenTile TileOf(const SelectArgs& a, uint32_t index)
       const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
       t.request = base + at;
       t.first = static_cast<int>(index - before - __builtin_amdgcn_readlane(upto - tiles, at)) * a.tokens_a_tile;
-      t.q = {__builtin_amdgcn_readlane(q.start, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.length, at)};
+      t.q = {__builtin_amdgcn_readlane(q.start, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.length, at),
+             __builtin_amdgcn_readlane(q.base, at)};
       t.last = min(t.first + a.tokens_a_tile, t.q.n) - 1;
-      const int position = t.q.length - t.q.n + t.last;
-      t.pages = position < 0 ? 0 : min(position / op.cache.page + 1, op.table_width);
+      t.pages = PagesSeen(op, t.q, t.q.base + t.last);
       break;
     }
     before += __builtin_amdgcn_readlane(upto, kWave - 1);
@@ -343,9 +348,8 @@ __global__ __launch_bounds__(kPickThreads) void PickKernel(const SelectArgs a) {
       high = mid;
     }
   }
-  const PagedRequest q = RequestOf(op.starts, op.lengths, low, op.tokens, a.most_length);
-  const int position = token >= q.start && token < q.start + q.n ? q.length - q.n + token - q.start : -1;
-  const int pages = position < 0 ? 0 : min(position / op.cache.page + 1, op.table_width);
+  const PagedRequest q = RequestOf(op.starts, op.lengths, op.before, low, op.tokens, a.most_length);
+  const int pages = token >= q.start && token < q.start + q.n ? PagesSeen(op, q, q.base + token - q.start) : 0;
   if (pages <= op.keep) {
     for (int i = tid; i < op.keep; i += kPickThreads) list[i] = i < pages ? i : -1;
     return;
@@ -421,8 +425,7 @@ __global__ __launch_bounds__(kWholeThreads) void WholeKernel(const SelectArgs a,
   __syncthreads();
   const int threads = kWholeThreads / shares, share = tid / threads, me = tid - share * threads;
   const bool mine = t.first + share <= t.last;
-  const int position = t.q.length - t.q.n + t.first + share;
-  const int pages = !mine || position < 0 ? 0 : min(position / op.cache.page + 1, op.table_width);
+  const int pages = mine ? PagesSeen(op, t.q, t.q.base + t.first + share) : 0;
   int32_t* const list = op.lists + (static_cast<int64_t>(t.q.start + t.first + (mine ? share : 0)) * op.cache.kv_heads + head) * op.keep;
   if (mine && pages <= op.keep) {
     for (int i = me; i < op.keep; i += threads) list[i] = i < pages ? i : -1;
@@ -476,7 +479,7 @@ int CheckSelect(const llmp_paged_select* op) {
     return Refuse(1, "paged_select: a whole number of query heads a KV head (%d, %d)", op->heads, op->cache.kv_heads);
   if (op->lengths == nullptr || op->starts == nullptr || op->table == nullptr || op->lists == nullptr) return Refuse(1, "paged_select: null operand");
   if ((reinterpret_cast<uintptr_t>(op->lengths) | reinterpret_cast<uintptr_t>(op->starts) | reinterpret_cast<uintptr_t>(op->table) |
-       reinterpret_cast<uintptr_t>(op->lists)) % 4 != 0)
+       reinterpret_cast<uintptr_t>(op->lists) | reinterpret_cast<uintptr_t>(op->before)) % 4 != 0)
     return Refuse(1, "paged_select: I32 arrays at 4-byte boundaries");
   if (op->table_stride < op->table_width) return Refuse(1, "paged_select: a table row of %d entries every %lld", op->table_width, (long long)op->table_stride);
   if (static_cast<int64_t>(op->table_width) * op->cache.page > kMostPagedLength) return Refuse(1, "paged_select: a table row of at most 2^30 tokens");

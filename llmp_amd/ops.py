@@ -715,7 +715,8 @@ def paged_plan(before, after, table, ring, counters, page, tokens, out=None):
     [requests]). `table` (int32 [requests, width]) and `ring` (int32, the free pages) are updated in place; `counters` is
     {first free page's index in the ring, how many}; `tokens` at least the new tokens. Returns a dict of int32 tensors: starts
     [requests + 1], lengths [requests], slots, positions and requests [tokens], work [items, 4] (page, first row, tokens held,
-    new tokens) and the counters after the step {first, how many, tokens without a page}. `out`, such a dict, is filled
+    new tokens) and the counters after the step {first, how many, tokens without a page}. Where tokens found no page, lengths end before
+    them while starts count them: paged_attend and paged_select of the step then need `before` too. `out`, such a dict, is filled
     instead of a new one (its counters may be the ones passed in)."""
     lib = _lib.load()
     _int32(before, after, table, ring, counters)
@@ -781,8 +782,11 @@ def paged_read(cache, pages, dtype=torch.float32):
     return k, v
 
 
-def _paged_queries(q, c, table, lengths, starts):
+def _paged_queries(q, c, table, lengths, starts, before):
     _int32(table, lengths, starts)
+    if before is not None:
+        _int32(before)
+        assert before.shape == lengths.shape
     tokens, heads, head_dim = q.shape
     n, width = table.shape
     token_stride, head_stride, one = q.stride()
@@ -790,14 +794,16 @@ def _paged_queries(q, c, table, lengths, starts):
     return tokens, heads, n, width, token_stride, head_stride
 
 
-def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0.0, sinks=None, lists=None, most=None, out=None, scratch=None):
+def paged_attend(cache, q, table, lengths, starts, scale, *, before=None, window=0, softcap=0.0, sinks=None, lists=None, most=None, out=None, scratch=None):
     """llmp.paged.attend: causal attention of q (float32, bfloat16 or float16 [tokens, heads, head_dim]: request r's rows are starts[r] to
-    starts[r + 1] - 1, at the last of its lengths[r] positions) over the requests' pages (table int32 [requests, width]). `lists`
+    starts[r + 1] - 1, at the last of its lengths[r] positions) over the requests' pages (table int32 [requests, width]). `before`, the
+    lengths that the step's paged_plan took, places the rows at positions before[r] on: with it a step whose pages ran out is
+    answered too, its rows past lengths[r] from all that is held. `lists`
     (paged_select's) leaves a (token, KV head) those pages only. `most`: the largest number of new tokens of a request, if it is
     known. Returns q's shape and type; rows past starts[requests] are not written."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts)
+    tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts, before)
     if out is None:
         out = torch.empty((tokens, heads, c.head_dim), dtype=q.dtype, device=q.device)
         out_token, out_head = heads * c.head_dim, c.head_dim
@@ -812,7 +818,7 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0
         return out
     op = _lib.PagedAttend(c, q.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(lists), _ptr(sinks),
                           q_token, q_head, out_token, out_head, _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens,
-                          tokens if most is None else most, width, lists.shape[2] if lists is not None else 0, window, scale, softcap)
+                          tokens if most is None else most, width, lists.shape[2] if lists is not None else 0, window, scale, softcap, _ptr(before))
     cus, at = _compute_units(), C.byref(op)
     if scratch is None:
         scratch = torch.empty(max(lib.llmp_hip_paged_attend_scratch(at, cus), 16), dtype=torch.uint8, device=q.device)
@@ -820,13 +826,13 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, window=0, softcap=0
     return out
 
 
-def paged_select(cache, q, table, lengths, starts, keep, *, first=1, recent=1, most=None, out=None, scratch=None):
+def paged_select(cache, q, table, lengths, starts, keep, *, before=None, first=1, recent=1, most=None, out=None, scratch=None):
     """llmp.paged.select: for every row of q and KV head the `keep` pages (places in the request's table row, ascending, -1 past them) whose
-    keys have the largest bound on a logit of the head's group; the first `first` and the last `recent` pages up to the token's own
-    are always among them. int32 [tokens, kv_heads, keep]."""
+    keys have the largest bound on a logit of the head's group; the first `first` and the last `recent` pages that the token sees
+    are always among them (`before` as for paged_attend). int32 [tokens, kv_heads, keep]."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts)
+    tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts, before)
     if out is None:
         out = torch.empty((tokens, c.kv_heads, keep), dtype=torch.int32, device=q.device)
     else:
@@ -834,7 +840,7 @@ def paged_select(cache, q, table, lengths, starts, keep, *, first=1, recent=1, m
     if tokens == 0:
         return out
     op = _lib.PagedSelect(c, q.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), out.data_ptr(), q_token, q_head,
-                          _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens, tokens if most is None else most, width, keep, first, recent)
+                          _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens, tokens if most is None else most, width, keep, first, recent, _ptr(before))
     at = C.byref(op)
     if scratch is None:
         scratch = torch.empty(max(lib.llmp_hip_paged_select_scratch(at), 16), dtype=torch.uint8, device=q.device)
