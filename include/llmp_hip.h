@@ -712,11 +712,12 @@ int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch, size_t scr
 
 /* llmp.paged.select: for every new token and KV head the `keep` pages of its request whose keys could have the largest logit: a
  * head's query as 8-bit codes c of unit u = max|q| * F32(1 / 127) (q / u to nearest even), a page's score the largest of the group's heads' of
- * F32(F32(sum over d of c_d * (c_d > 0 ? high_d : low_d)) * u) * k_scale, which bounds every key's c . k in the page. The token's
- * first `first` and last `recent` pages are always among them (of the pages with tokens that it sees, as llmp.paged.attend says; at most `keep` together); ties go to
- * the lower page; a score that is not a number counts as the smallest. lists: I32 [tokens][kv_heads][keep], ascending,
- * -1 past a token's pages; tokens past starts[requests] get -1 throughout. scratch: llmp_hip_paged_select_scratch(op) bytes at
- * a 16-byte boundary. The cache has low and high. keep at most 4096. */
+ * F32(F32(sum over d of c_d * (c_d > 0 ? high_d : low_d)) * u) * k_scale, which bounds every key's c . k in the page. The first `first`
+ * and last `recent` of the pages with tokens that it sees (llmp.paged.attend) are always among them (at most `keep` together); ties go
+ * to the lower page; a score that is not a number counts as the smallest; a table entry that is no page of the cache is never among
+ * them, as first or recent neither. lists: I32 [tokens][kv_heads][keep], ascending, -1 past a token's chosen pages; tokens past
+ * starts[requests] get -1 throughout. scratch: llmp_hip_paged_select_scratch(op) bytes at a 16-byte boundary. The cache has low and
+ * high. keep at most 4096. */
 typedef struct llmp_paged_select {
   llmp_paged_cache cache;
   const void* q;

@@ -7,7 +7,7 @@
 //
 // First launch, the scores: as products of max(c, 0) with the high codes and of min(c, 0) with the low ones they are matrix
 // products of whole numbers, pages as rows and (token, head) pairs of one KV head as columns
-// (v_mfma_i32_16x16x64_i8); a wave takes 16 pages at a time. What bounds it is the codes' bytes, 2 * head_dim a page and head.
+// (v_mfma_i32_16x16x64_i8); a wave takes 16 pages at a time. A page that is not in the cache has no score and is never chosen. What bounds it is the codes' bytes, 2 * head_dim a page and head.
 // Second launch, the choice: a workgroup a (token, KV head) finds the keep-th largest score by its bits, eight at a time
 // (a histogram a pass), and writes the pages at or above it in order; ties go to the lower page. Where there are workgroups enough
 // for the card, both are one launch and the scores stay in LDS.
@@ -34,6 +34,7 @@ struct SelectArgs {
   int tokens_a_tile;  // tokens whose heads fill the 16 columns
 };
 
+__device__ __forceinline__ bool IsPage(const llmp_paged_cache& c, int page) { return page >= 0 && page < c.pages; }
 // How many of its request's pages the token at `position` sees tokens of.
 __device__ __forceinline__ int PagesSeen(const llmp_paged_select& op, const PagedRequest& q, int position) {
   const int seen = SeenTo(q, position);
@@ -89,6 +90,7 @@ struct Scorer {
   struct Pages {
     I32x4 low[kSteps], high[kSteps];
     float scale;
+    bool there;
   };
 
   __device__ __forceinline__ Scorer(const SelectArgs& args, const TokenTile& tile, int kv_head)
@@ -99,7 +101,8 @@ struct Scorer {
   // The lane's page row: its low and high codes.
   __device__ __forceinline__ void Load(int page, Pages* to) const {
     const llmp_paged_cache& c = a.op.cache;
-    if (page < 0 || page >= c.pages) page = 0;
+    to->there = IsPage(c, page);
+    if (!to->there) page = 0;  // (any that can be read)
     const int64_t page_head = static_cast<int64_t>(page) * c.kv_heads + head, at = page_head * D + 16 * group_of;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -158,7 +161,8 @@ struct Scorer {
     unit = units[column];
     real = column < a.tokens_a_tile * a.group && t.first + (a.tokens_a_tile > 1 ? column / a.group : 0) <= t.last;
   }
-  // The scores of pages `from` to from + 15 through `tile` ([column][page], the wave's own): give(token of the tile, page, score).
+  // The scores of pages `from` to from + 15 through `tile` ([column][page], the wave's own): give(token of the tile, page, score), NaN
+  // for a page that is not there.
   template <class F>
   __device__ __forceinline__ void Score(int from, const Pages& pages, float (*tile)[17], F&& give) {
     float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of column groups, more than one where a KV head has over 16 heads
@@ -195,7 +199,7 @@ struct Scorer {
       if (t.first + token > t.last || from + p >= t.pages) continue;
       float top = -INFINITY;
       for (int k = 0; k < columns; ++k) top = fmaxf(top, tile[token * columns + k][p]);
-      give(token, from + p, top);
+      give(token, from + p, pages.there ? top : __builtin_nanf(""));  // (p is the lane's column: the page whose row it loaded)
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -227,8 +231,9 @@ __global__ __launch_bounds__(kScoreThreads) void ScoreKernel(const SelectArgs a)
   }
 }
 
-// A score's bits in an order that whole numbers have: larger scores larger keys, 0 kept for none.
+// A score's bits in an order that whole numbers have: larger scores larger keys, 0 for a page that is not there.
 __device__ __forceinline__ uint32_t KeyOf(float score) {
+  if (score != score) return 0;
   const uint32_t bits = __builtin_bit_cast(uint32_t, score == 0.0f ? 0.0f : score);
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
@@ -236,46 +241,101 @@ __device__ __forceinline__ uint32_t KeyOf(float score) {
 // What the threads of a share of a workgroup know together in a choice.
 struct Choice {
   int bins[2][256], found[3];
-  uint32_t least[kWholeWaves], most[kWholeWaves];
-  int sums[2][kWholeWaves];
+  uint32_t least[kWholeWaves], most[kWholeWaves], least_there[kWholeWaves];
+  int others[kWholeWaves], forced[kWholeWaves], sums[2][kWholeWaves];
 };
-// The choice of op.keep of `count` pages (more than that, or 0: no choice) by a share of a workgroup, `threads` threads (whole
-// waves) of which the caller is number `me`: the first and the recent pages, and of the others those with the largest keys, written
-// in order. The workgroup's shares call it together, they meet at its barriers.
+// The sum of `value` over a share's threads before the caller, and all of it; `sums` [waves], written here.
+__device__ __forceinline__ int SumBefore(int value, int* sums, int lane, int wave, int waves, int* all) {
+  const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(value)));
+  if (lane == kWave - 1) sums[wave] = upto;
+  __syncthreads();
+  const int of_waves = static_cast<int>(WaveSums(lane < waves ? static_cast<uint32_t>(sums[lane]) : 0u));
+  *all = __builtin_amdgcn_readlane(of_waves, kWave - 1);
+  return upto - value + (wave > 0 ? __builtin_amdgcn_readlane(of_waves, max(wave - 1, 0)) : 0);
+}
+// All of a token's `count` pages, at most op.keep, that are there: what is chosen where none has to be left out. By a share of a workgroup, as
+// the choice below; `most` pages in any share: where that is a wave's, the share's first wave needs no barrier.
+__device__ __forceinline__ void TakeAll(const llmp_paged_select& op, int count, int most, int me, int threads, int* sums, const int32_t* table, int32_t* list) {
+  const int lane = me & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(me / kWave), waves = threads / kWave;
+  const int run = ((count + kWave - 1) / kWave + waves - 1) / waves * kWave, from = min(wave * run, count), to = min(from + run, count);
+  const auto there = [&](int j) { return j < to && IsPage(op.cache, table[j]); };
+  if (most <= kWave) {
+    if (list == nullptr || wave > 0) return;
+    const uint64_t mask = __ballot(there(lane));
+    if ((mask >> lane) & 1) list[__popcll(mask & ((1ull << lane) - 1))] = lane;
+    for (int i = __popcll(mask) + lane; i < op.keep; i += kWave) list[i] = -1;
+    return;
+  }
+  int mine = 0, all;
+  for (int j = from; j < to; j += kWave) mine += __popcll(__ballot(there(j + lane)));
+  int at = SumBefore(lane == 0 ? mine : 0, sums, lane, wave, waves, &all);
+  if (list == nullptr) return;
+  at = __builtin_amdgcn_readfirstlane(at);  // (lane 0's: what lies before the wave)
+  for (int j = from; j < to; j += kWave) {
+    const uint64_t mask = __ballot(there(j + lane));
+    if (there(j + lane)) list[at + __popcll(mask & ((1ull << lane) - 1))] = j + lane;
+    at += __popcll(mask);
+  }
+  for (int i = all + me; i < op.keep; i += threads) list[i] = -1;
+}
+// The choice of op.keep of `count` pages by a share of a workgroup, `threads` threads (whole waves) of which the caller is number `me`:
+// the first and the recent pages, and of the others those with the largest keys, of each those that are there (a key other than
+// 0), written in order with -1 past them (list null: nothing is). The workgroup's shares call it together, they meet at its barriers.
 template <class F>
 __device__ __forceinline__ void Choose(const llmp_paged_select& op, int count, int me, int threads, Choice* all, int share, int shares, F&& key_at, int32_t* list) {
   const int lane = me & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(me / kWave), waves = threads / kWave;
   Choice& my = all[share];
-  const int begin = count > 0 ? op.first : 0, end = count > 0 ? count - op.recent : 0;
+  const int begin = min(op.first, count), end = max(count - op.recent, begin);
   for (int i = me; i < 512; i += threads) my.bins[0][i] = 0;
   uint32_t least = ~0u, most = 0;
-  for (int j = begin + me; j < end; j += threads) {
+  for (int j = me; j < count; j += threads) {  // (the first and the recent ones for whether they are there: then the least is not 0)
     const uint32_t key = key_at(j);
-    least = min(least, key), most = max(most, key);
+    const bool other = (j >= begin) & (j < end);
+    least = min(least, (other | (key == 0)) ? key : ~0u), most = max(most, other ? key : 0u);
   }
   least = WaveMinU32(least), most = WaveMaxU32(most);
   if (lane == 0) my.least[wave] = least, my.most[wave] = most;
   int want = op.keep - op.first - op.recent;
-  if (me == 0) my.found[2] = count == 0 || want == 0;
+  bool every = count <= op.keep;
+  if (me == 0) my.found[2] = every || want == 0;
   __syncthreads();
   for (int w = 0; w < waves; ++w) least = min(least, my.least[w]), most = max(most, my.most[w]);
+  if (__any(lane < shares * waves && all[lane / waves].least[lane % waves] == 0)) {  // pages of some share are not there: those that are, counted
+    uint32_t low_key = ~0u;
+    int others = 0, forced = 0;
+    for (int j = me; j < count; j += threads) {
+      const uint32_t key = key_at(j);
+      const bool other = j >= begin && j < end;
+      if (key != 0 && other) low_key = min(low_key, key);
+      others += key != 0 && other, forced += key != 0 && !other;
+    }
+    low_key = WaveMinU32(low_key);
+    if (lane == 0) my.least_there[wave] = low_key;
+    others = static_cast<int>(WaveSums(static_cast<uint32_t>(others))), forced = static_cast<int>(WaveSums(static_cast<uint32_t>(forced)));
+    if (lane == kWave - 1) my.others[wave] = others, my.forced[wave] = forced;
+    __syncthreads();
+    least = ~0u, others = forced = 0;
+    for (int w = 0; w < waves; ++w) least = min(least, my.least_there[w]), others += my.others[w], forced += my.forced[w];
+    want = op.keep - forced;
+    every = others <= want;
+    if (me == 0) my.found[2] = every || want == 0;
+    __syncthreads();
+  }
   // The want-th largest distance from the least key, its highest bits first (the bounds are mostly of one sign and near each other:
   // eight bits of the distances tell them apart, where eight bits of the keys are the same few), until all that share the bits
   // found so far are chosen.
   uint32_t prefix = ~0u;  // (none wanted: no distance lies above)
-  int low = most > least ? 32 - __clz(most - least) : 0;
+  int low = every || want == 0 || most <= least ? 0 : 32 - __clz(most - least);
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
-    bool over = true;
-    for (int i = 0; i < shares; ++i) over = over && all[i].found[2] != 0;
-    if (over) break;
+    if (__all(lane >= shares || all[lane].found[2] != 0)) break;
     const bool mine = my.found[2] == 0;
     const int upper = low, next = max(upper - 8, 0);
     if (mine) {
       const uint32_t digits = (1u << (upper - next)) - 1;
       for (int j = begin + me; j < end; j += threads) {
-        const uint32_t d = key_at(j) - least;
-        if (pass == 0 || (d >> upper) == prefix) atomicAdd(&my.bins[pass & 1][(d >> next) & digits], 1);
+        const uint32_t key = key_at(j), d = key - least;
+        if ((key != 0) & ((pass == 0) | ((d >> min(upper, 31)) == prefix))) atomicAdd(&my.bins[pass & 1][(d >> next) & digits], 1);
       }
     }
     if (pass > 0) {
@@ -307,28 +367,29 @@ __device__ __forceinline__ void Choose(const llmp_paged_select& op, int count, i
     }
   }
   // In order, a run of pages a thread: all above the bits found, and the first `want` of those that have them.
-  const auto forced = [&](int j) { return j < begin || j >= end; };
+  const auto look = [&](int j, bool* is_equal) {
+    const uint32_t key = key_at(j), d = (key - least) >> low;
+    const bool there = key != 0, always = every | (j < begin) | (j >= end);
+    *is_equal = there & !always & (d == prefix);
+    return there & (always | (d > prefix));
+  };
   const int run = (count + threads - 1) / threads, from = min(me * run, count), to = min(from + run, count);
   int equal = 0, larger = 0;
   for (int j = from; j < to; ++j) {
-    const uint32_t d = forced(j) ? 0u : (key_at(j) - least) >> low;
-    larger += forced(j) || d > prefix, equal += !forced(j) && d == prefix;
+    bool is_equal;
+    larger += look(j, &is_equal), equal += is_equal;
   }
-  const auto before = [&](int value, int* sums) {  // the share's sum up to this thread
-    const int upto = static_cast<int>(WaveSums(static_cast<uint32_t>(value)));
-    if (lane == kWave - 1) sums[wave] = upto;
-    __syncthreads();
-    int sum = upto - value;
-    for (int w = 0; w < wave; ++w) sum += sums[w];
-    return sum;
-  };
-  int rank = before(equal, my.sums[0]);
-  int at = before(larger + min(max(want - rank, 0), equal), my.sums[1]);
+  int all_equal, all_chosen;
+  int rank = SumBefore(equal, my.sums[0], lane, wave, waves, &all_equal);
+  int at = SumBefore(larger + min(max(want - rank, 0), equal), my.sums[1], lane, wave, waves, &all_chosen);
+  if (list == nullptr) return;
   for (int j = from; j < to; ++j) {
-    const uint32_t d = forced(j) ? 0u : (key_at(j) - least) >> low;
-    if ((forced(j) || d > prefix || (d == prefix && rank < want)) && at < op.keep) list[at++] = j;
-    rank += !forced(j) && d == prefix;
+    bool is_equal;
+    const bool is_larger = look(j, &is_equal);
+    if ((is_larger || (is_equal && rank < want)) && at < op.keep) list[at++] = j;
+    rank += is_equal;
   }
+  for (int i = all_chosen + me; i < op.keep; i += threads) list[i] = -1;
 }
 
 // grid (tokens, KV heads).
@@ -350,8 +411,9 @@ __global__ __launch_bounds__(kPickThreads) void PickKernel(const SelectArgs a) {
   }
   const PagedRequest q = RequestOf(op.starts, op.lengths, op.before, low, op.tokens, a.most_length);
   const int pages = token >= q.start && token < q.start + q.n ? PagesSeen(op, q, q.base + token - q.start) : 0;
-  if (pages <= op.keep) {
-    for (int i = tid; i < op.keep; i += kPickThreads) list[i] = i < pages ? i : -1;
+  if (pages <= op.keep) {  // (no scores: all that are there)
+    const int32_t* const table = op.table + low * op.table_stride;
+    TakeAll(op, pages, pages, tid, kPickThreads, choice.sums[0], table, list);
     return;
   }
   const float* const scores = a.scores + (static_cast<int64_t>(token) * op.cache.kv_heads + head) * op.table_width;
@@ -426,13 +488,14 @@ __global__ __launch_bounds__(kWholeThreads) void WholeKernel(const SelectArgs a,
   const int threads = kWholeThreads / shares, share = tid / threads, me = tid - share * threads;
   const bool mine = t.first + share <= t.last;
   const int pages = mine ? PagesSeen(op, t.q, t.q.base + t.first + share) : 0;
-  int32_t* const list = op.lists + (static_cast<int64_t>(t.q.start + t.first + (mine ? share : 0)) * op.cache.kv_heads + head) * op.keep;
-  if (mine && pages <= op.keep) {
-    for (int i = me; i < op.keep; i += threads) list[i] = i < pages ? i : -1;
-  }
-  if (t.pages <= op.keep) return;  // (every token's: the tile's last has the most)
+  int32_t* const list = mine ? op.lists + (static_cast<int64_t>(t.q.start + t.first + share) * op.cache.kv_heads + head) * op.keep : nullptr;
   const uint32_t* const key = keys + share * op.table_width;
-  Choose(op, pages > op.keep ? pages : 0, me, threads, choices, share, shares, [&](int j) { return key[j]; }, list);
+  const int32_t* const table = op.table + t.request * op.table_stride;
+  if (t.pages <= op.keep) {  // (every token's: the tile's last has the most)
+    TakeAll(op, pages, t.pages, me, threads, choices[share].sums[0], table, list);
+    return;
+  }
+  Choose(op, pages, me, threads, choices, share, shares, [&](int j) { return key[j]; }, list);
 }
 
 // One launch where its workgroups, one a (tile of tokens, KV head), are at least half as many as the card's 256 compute units and hold

@@ -829,7 +829,7 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, before=None, window
 def paged_select(cache, q, table, lengths, starts, keep, *, before=None, first=1, recent=1, most=None, out=None, scratch=None):
     """llmp.paged.select: for every row of q and KV head the `keep` pages (places in the request's table row, ascending, -1 past them) whose
     keys have the largest bound on a logit of the head's group; the first `first` and the last `recent` pages that the token sees
-    are always among them (`before` as for paged_attend). int32 [tokens, kv_heads, keep]."""
+    are always among them (`before` as for paged_attend), and no table entry that is no page of the cache. int32 [tokens, kv_heads, keep]."""
     lib = _lib.load()
     c = _paged_cache(cache)
     tokens, heads, n, width, q_token, q_head = _paged_queries(q, c, table, lengths, starts, before)
