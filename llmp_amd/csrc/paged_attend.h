@@ -5,8 +5,11 @@
 // digits and 8355584 for F32), so hi . c and lo . c are integer products and s = (256 (hi . c) + lo . c) * (f * ks * scale) is exact up
 // to x's own rounding: 2^-16 of the row's largest magnitude, 2^-24 for F32.
 // V's scale vs differs from page to page, so the sum's weights are w = exp(s) * vs. The running maximum is of t = log2(e) s + log2(vs)
-// (vs at least 2^-100 there): p = exp2(log2(e) s - E) goes to the sum of probabilities, p * vs <= 1 is rounded to F16 for the
-// product with V's codes, and the F16's exponent range is used whatever the scales are. The common factor 2^E leaves at the end.
+// (vs at least 2^-80 there: p below then stays below 2^95, and its sums below 2^127 over all the tokens that a row can have):
+// p = exp2(log2(e) s - E) goes to the sum of probabilities, p * vs is rounded to F16 for the product with V's codes. E is set kLift below
+// the maximum and follows it once that is kSlack further, so a weight is at most 2^15 and the row's largest at least 2^kLift: the
+// whole of F16's range (largest 2^16, smallest step 2^-24) lies under the largest. A weight is off by 2^-11 of itself, or by
+// 2^-(25 + kLift) of the row's largest where that is more. The common factor 2^E leaves at the end.
 #ifndef LLMP_AMD_CSRC_PAGED_ATTEND_H_
 #define LLMP_AMD_CSRC_PAGED_ATTEND_H_
 
@@ -16,7 +19,9 @@ namespace llmp_hip {
 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kTileTokens = 64;
-constexpr float kSlack = 8.0f;  // how far the running maximum may lag, in log2
+// In log2, 15 together. (By a slack of 8, 5, 3, 2: a chunk of 2048 tokens behind 2048 156.0, 156.2, 157.5, 158.9 us, 6 ragged prompts at head
+// size 256 108.9, 109.6, 110.9, 111.8.)
+constexpr float kLift = 10.0f, kSlack = 5.0f;
 
 struct PagedAttendArgs {
   llmp_paged_attend op;
@@ -230,7 +235,7 @@ __device__ __forceinline__ float Capped(float s, float softcap, float inverse) {
 }
 
 // log2 of a page's V scale, as the running maximum takes it.
-__device__ __forceinline__ float ScaleLog(float vs) { return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-100f)); }
+__device__ __forceinline__ float ScaleLog(float vs) { return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-80f)); }
 
 // The many rows' form (its own file), for requests of more than few_rows rows, and those of fewer where they are little work beside
 // them: the number that it gives the place of is then not zero.

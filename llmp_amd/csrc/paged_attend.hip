@@ -384,8 +384,8 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
 #pragma unroll
       for (int i = 1; i < kMine; ++i) peak = fmaxf(peak, s[i]);
       peak = AcrossGroupsMax(peak + ScaleLog(vs));
-      if (__any(peak > top + kSlack)) {
-        const float higher = fmaxf(top, peak);
+      if (__any(peak > top + (kLift + kSlack))) {
+        const float higher = fmaxf(top, peak - kLift);
         const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
         top = higher;
         sum *= keep;

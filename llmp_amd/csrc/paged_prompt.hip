@@ -529,9 +529,9 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
 #pragma unroll
           for (int i = 1; i < 16; ++i) peak = fmaxf(peak, s[i]);
           peak = Across<kWaveRows>(fmaf(peak, worth, value_log));
-          // The maximum follows once it is kSlack behind: weights up to 2^kSlack keep their F16's precision, and the sums rarely turn.
-          if (__any(peak > top + kSlack)) {
-            const float higher = fmaxf(top, peak);
+          // (The maximum follows once it is kSlack behind: the sums rarely turn.)
+          if (__any(peak > top + (kLift + kSlack))) {
+            const float higher = fmaxf(top, peak - kLift);
             const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
             top = higher;
             sum *= keep;
