@@ -691,7 +691,7 @@ int llmp_hip_paged_read(const llmp_paged_cache* cache, const int32_t* pages, int
  * most_tokens: at least every request's new tokens (a bound from the host; the launches' choice goes by it). K codes multiply the
  * queries as whole numbers: a query row is two 8-bit digits of 1/32639 of its largest magnitude (three, 1/8355584,
  * for F32). Probabilities times the V scale are rounded to F16 (for F32 to a sum of two) against V codes as F16 (exact): one is off by 2^-11
- * (F32: 2^-22) of itself, or by 2^-35 of the row's largest where that is more.
+ * (F32: 2^-22) of itself, or by 2^-35 (F32: 2^-46) of the row's largest where that is more.
  * scratch: llmp_hip_paged_attend_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal, the reason in last_error).
  * Launch arguments depend on the descriptor alone, never on the lengths: a captured launch replays at other lengths. */
 typedef struct llmp_paged_attend {

@@ -9,7 +9,8 @@
 // p = exp2(log2(e) s - E) goes to the sum of probabilities, p * vs is rounded to F16 for the product with V's codes. E is set kLift below
 // the maximum and follows it once that is kSlack further, so a weight is at most 2^15 and the row's largest at least 2^kLift: the
 // whole of F16's range (largest 2^16, smallest step 2^-24) lies under the largest. A weight is off by 2^-11 of itself, or by
-// 2^-(25 + kLift) of the row's largest where that is more. The common factor 2^E leaves at the end.
+// 2^-(25 + kLift) of the row's largest where that is more. For F32 what the F16 leaves of a weight goes into a second product, 2^11 times
+// as large (a code times 2^-11 is exact in F16): off by 2^-22 of itself or 2^-(36 + kLift) of the largest. The common factor 2^E leaves at the end.
 #ifndef LLMP_AMD_CSRC_PAGED_ATTEND_H_
 #define LLMP_AMD_CSRC_PAGED_ATTEND_H_
 
@@ -205,6 +206,12 @@ __device__ __forceinline__ F16x8 EightCodes(uint32_t a, uint32_t b) {
   const F16x2 v0 = TwoCodes(a, 0x00050004u), v1 = TwoCodes(a, 0x00070006u), v2 = TwoCodes(b, 0x00050004u), v3 = TwoCodes(b, 0x00070006u);
   return F16x8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
 }
+
+// What a weight's F16 leaves of it, and the codes that it multiplies. (Without the factor an F32 prompt of 2000 tokens behind 2000 takes 207
+// us at head size 256, 158 at 128, 102 at 64, with it 229, 167, 107; a product of its own, added once a tile, 226 at 256.)
+constexpr float kRestUp = 0x1p11f;
+__device__ __forceinline__ _Float16 RestOf(float weight, _Float16 held) { return static_cast<_Float16>((weight - static_cast<float>(held)) * kRestUp); }
+__device__ __forceinline__ F16x8 RestCodes(F16x8 codes) { return codes * static_cast<_Float16>(1.0f / kRestUp); }
 
 // Where in a row of LDS a piece of 16 bytes lies (and which piece lies there). A wave's read of 16 bytes a lane takes lanes 0 to 3, 12 to
 // 15 and 20 to 27 at once, then the others of the first half, and the second half likewise; each 16 lanes are to find their pieces at 16 places

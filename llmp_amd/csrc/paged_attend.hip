@@ -408,7 +408,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         w[i / 8][i % 8] = static_cast<_Float16>(p[i]);
-        if constexpr (kDig == 3) w_low[i / 8][i % 8] = static_cast<_Float16>(p[i] - static_cast<float>(w[i / 8][i % 8]));
+        if constexpr (kDig == 3) w_low[i / 8][i % 8] = RestOf(p[i], w[i / 8][i % 8]);
       }
       // ---- O^T += V^T P^T
 #pragma unroll
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kFewThreads, FewAUnit(D)) void FewKernel(const Page
         for (int x = 0; x < 2; ++x) {
           const F16x8 v = EightCodes(in.v[b][2 * x], in.v[b][2 * x + 1]);
           out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[x], out[b], 0, 0, 0);
-          if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w_low[x], out[b], 0, 0, 0);
+          if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(RestCodes(v), w_low[x], out[b], 0, 0, 0);
         }
       }
     };

@@ -541,7 +541,7 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
           F16x8 p[2], p_low[2];
           const auto pack = [&](int i, float weight) {
             p[i / 8][i % 8] = static_cast<_Float16>(weight);
-            if constexpr (kDig == 3) p_low[i / 8][i % 8] = static_cast<_Float16>(weight - static_cast<float>(p[i / 8][i % 8]));
+            if constexpr (kDig == 3) p_low[i / 8][i % 8] = RestOf(weight, p[i / 8][i % 8]);
           };
           if (whole) {  // V's scale in the exponent: the weights at once, and the probabilities' sum from theirs
             const float less = value_log - top;
@@ -572,10 +572,10 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
               const F16x8 v = v_half[x][b];
               if constexpr (kWaveRows == 32) {
                 out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], out[b], 0, 0, 0);
-                if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p_low[x], out[b], 0, 0, 0);
+                if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(RestCodes(v), p_low[x], out[b], 0, 0, 0);
               } else {
                 out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[x], out[b], 0, 0, 0);
-                if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p_low[x], out[b], 0, 0, 0);
+                if constexpr (kDig == 3) out[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(RestCodes(v), p_low[x], out[b], 0, 0, 0);
               }
             }
           }

@@ -41,7 +41,7 @@ def attend(cache, q, table, length, dtype, scale):
     return out, far
 
 
-FLOOR = {"bf16": 2.0 ** -35, "f16": 2.0 ** -35}
+FLOOR = {"f32": 2.0 ** -46, "bf16": 2.0 ** -35, "f16": 2.0 ** -35}
 
 
 def dominated(g, length, fresh, kv_heads, page, d, nats, alike):
@@ -85,3 +85,10 @@ SHAPES = [(4000, 1, 2, 64, 128), (3001, 40, 1, 16, 64), (2500, 70, 1, 32, 256), 
 def test_a_dominating_token_leaves_the_others_their_weights(device, dtype, length, fresh, kv_heads, page, d, alike):
     for nats in (12, 18):
         check(device, dtype, length, fresh, kv_heads, page, d, nats, alike)
+
+
+@pytest.mark.parametrize("alike", [True, False])
+@pytest.mark.parametrize("length,fresh,kv_heads,page,d", SHAPES)
+def test_f32_keeps_what_an_f16_leaves_of_a_weight(device, length, fresh, kv_heads, page, d, alike):
+    for nats in (12, 16, 20):
+        check(device, "f32", length, fresh, kv_heads, page, d, nats, alike)
