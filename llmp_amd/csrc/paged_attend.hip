@@ -711,6 +711,8 @@ extern "C" int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch,
   BeginLaunches();
   PagedAttendArgs args;
   args.op = *op;
+  // (A window that no position passes is none: with one, a position before 0 less the window would pass an int.)
+  if (args.op.window >= kMostPagedLength) args.op.window = 0;
   const int groups = FewGroups(op->cache.head_dim, cus);
   args.parts = static_cast<int32_t*>(scratch);
   args.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + PartBytes(groups));

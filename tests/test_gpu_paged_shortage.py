@@ -168,3 +168,19 @@ def test_before_replays_with_the_launch(device):
         work()
         torch.cuda.synchronize()
         assert torch.equal(out, replayed)
+
+
+@pytest.mark.parametrize("window", [2147483647, 2147483646, 1 << 30, (1 << 30) - 1])
+def test_a_window_past_every_position_hides_nothing(device, window):
+    """Requests of fewer tokens than rows: their first positions lie before 0."""
+    g = np.random.default_rng(5)
+    cache = random_cache(g, 20, 2, 16, 64)
+    table = g.permutation(20)[:12].astype(np.int32).reshape(2, 6)
+    lengths, starts = np.array([40, 70], np.int32), np.array([0, 60, 135], np.int32)
+    q = g.standard_normal((135, 8, 64)).astype(np.float32)
+    c, x, n, s = to_device(cache, device), dev(q, device), dev(lengths, device), dev(starts, device)
+    want, far = plain.attend(cache, q, table, lengths.tolist(), starts.tolist(), 0.125, "f32")
+    for form in (table, widened(table, cache, 135, 75, 8)):
+        got = ops.paged_attend(c, x, dev(form, device), n, s, 0.125, window=window)
+        near(got, want, far, f"{form.shape[1]} pages a row")
+        assert torch.equal(got, ops.paged_attend(c, x, dev(form, device), n, s, 0.125))
