@@ -717,8 +717,8 @@ int llmp_hip_paged_attend(const llmp_paged_attend* op, void* scratch, size_t scr
  * and last `recent` of the pages with tokens that it sees (llmp.paged.attend) are always among them (at most `keep` together); ties go
  * to the lower page; a score that is not a number counts as the smallest; a table entry that is no page of the cache is never among
  * them, as first or recent neither. lists: I32 [tokens][kv_heads][keep], ascending, -1 past a token's chosen pages; tokens past
- * starts[requests] get -1 throughout. scratch: llmp_hip_paged_select_scratch(op) bytes at a 16-byte boundary. The cache has low and
- * high. keep at most 4096. */
+ * starts[requests] get -1 throughout. scratch: llmp_hip_paged_select_scratch(op) bytes at a 16-byte boundary (0: a refusal; the scores
+ * where they go through memory, else 16). The cache has low and high. keep at most 4096. */
 typedef struct llmp_paged_select {
   llmp_paged_cache cache;
   const void* q;

@@ -508,27 +508,51 @@ bool IsWhole(const SelectArgs& a, int64_t tiles) {
   return a.group <= 16 && tiles * a.op.cache.kv_heads >= kWholeWorkgroups && static_cast<int64_t>(a.tokens_a_tile) * a.op.table_width <= kWholeKeys;
 }
 
+// How a call is answered, from its sizes alone.
+struct SelectForm {
+  int64_t tiles;
+  bool scored, whole;  // scored: not every page is chosen; whole: in one launch, the scores in LDS
+  bool ScoresInMemory() const { return scored && !whole; }
+};
+SelectForm FormOf(const llmp_paged_select& op, SelectArgs* args) {
+  args->op = op;
+  args->group = op.heads / op.cache.kv_heads;
+  args->most_length = op.table_width * op.cache.page;
+  // (A request of one token fills no more columns than its heads.)
+  args->tokens_a_tile = args->group >= 16 ? 1 : 16 / args->group;
+  if (args->tokens_a_tile > op.most_tokens) args->tokens_a_tile = op.most_tokens;
+  const int64_t most_tiles = static_cast<int64_t>(op.requests) + op.tokens / args->tokens_a_tile;
+  SelectForm form;
+  form.tiles = most_tiles < op.tokens ? most_tiles : op.tokens;
+  form.scored = op.table_width > op.keep;
+  form.whole = form.scored && IsWhole(*args, form.tiles);
+  return form;
+}
+size_t SelectScratch(const llmp_paged_select& op, const SelectForm& form) {
+  return form.ScoresInMemory() ? static_cast<size_t>(op.tokens) * op.cache.kv_heads * op.table_width * sizeof(float) : 16;
+}
+
 template <int TYPE, int D>
-void LaunchSelect(const SelectArgs& args, int64_t tiles, hipStream_t stream) {
+void LaunchSelect(const SelectArgs& args, const SelectForm& form, hipStream_t stream) {
   const llmp_paged_select& op = args.op;
-  if (IsWhole(args, tiles)) {
+  if (form.whole) {
     const int lds = args.tokens_a_tile * op.table_width * 4;
     static bool sized = false;
     if (!AllowLds(reinterpret_cast<const void*>(&WholeKernel<TYPE, D>), kWholeKeys * 4, &sized)) return;
     int shares = 1;
     while (shares < args.tokens_a_tile) shares *= 2;
-    hipLaunchKernelGGL((WholeKernel<TYPE, D>), dim3(static_cast<unsigned>(tiles), op.cache.kv_heads), dim3(kWholeThreads), lds, stream, args, shares);
+    hipLaunchKernelGGL((WholeKernel<TYPE, D>), dim3(static_cast<unsigned>(form.tiles), op.cache.kv_heads), dim3(kWholeThreads), lds, stream, args, shares);
     return;
   }
   const int blocks = (op.table_width + 16 * kScoreWaves - 1) / (16 * kScoreWaves);
-  hipLaunchKernelGGL((ScoreKernel<TYPE, D>), dim3(static_cast<unsigned>(tiles), op.cache.kv_heads, blocks < 1024 ? blocks : 1024), dim3(kScoreThreads), 0, stream,
+  hipLaunchKernelGGL((ScoreKernel<TYPE, D>), dim3(static_cast<unsigned>(form.tiles), op.cache.kv_heads, blocks < 1024 ? blocks : 1024), dim3(kScoreThreads), 0, stream,
                      args);
 }
 template <int TYPE>
-void LaunchSelectOf(const SelectArgs& args, int64_t tiles, hipStream_t stream) {
-  if (args.op.cache.head_dim == 64) LaunchSelect<TYPE, 64>(args, tiles, stream);
-  if (args.op.cache.head_dim == 128) LaunchSelect<TYPE, 128>(args, tiles, stream);
-  if (args.op.cache.head_dim == 256) LaunchSelect<TYPE, 256>(args, tiles, stream);
+void LaunchSelectOf(const SelectArgs& args, const SelectForm& form, hipStream_t stream) {
+  if (args.op.cache.head_dim == 64) LaunchSelect<TYPE, 64>(args, form, stream);
+  if (args.op.cache.head_dim == 128) LaunchSelect<TYPE, 128>(args, form, stream);
+  if (args.op.cache.head_dim == 256) LaunchSelect<TYPE, 256>(args, form, stream);
 }
 
 int CheckSelect(const llmp_paged_select* op) {
@@ -558,32 +582,25 @@ using namespace llmp_hip;
 
 extern "C" size_t llmp_hip_paged_select_scratch(const llmp_paged_select* op) {
   if (CheckSelect(op) != 0) return 0;
-  return static_cast<size_t>(op->tokens) * op->cache.kv_heads * op->table_width * sizeof(float);
+  SelectArgs args;
+  return SelectScratch(*op, FormOf(*op, &args));
 }
 
 extern "C" int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch, size_t scratch_bytes, void* stream) {
   if (const int bad = CheckSelect(op); bad != 0) return bad;
-  const size_t needs = llmp_hip_paged_select_scratch(op);
+  SelectArgs args;
+  const SelectForm form = FormOf(*op, &args);
+  const size_t needs = SelectScratch(*op, form);
   if (scratch == nullptr || scratch_bytes < needs || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
     return Refuse(1, "paged_select: %zu bytes of scratch at a 16-byte boundary, %zu given", needs, scratch_bytes);
   BeginLaunches();
-  SelectArgs args;
-  args.op = *op;
   args.scores = static_cast<float*>(scratch);
-  args.group = op->heads / op->cache.kv_heads;
-  args.most_length = op->table_width * op->cache.page;
-  // (A request of one token fills no more columns than its heads.)
-  args.tokens_a_tile = args.group >= 16 ? 1 : 16 / args.group;
-  if (args.tokens_a_tile > op->most_tokens) args.tokens_a_tile = op->most_tokens;
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  const int64_t most_tiles = static_cast<int64_t>(op->requests) + op->tokens / args.tokens_a_tile;
-  const int64_t tiles = most_tiles < op->tokens ? most_tiles : op->tokens;
-  const bool scored = op->table_width > op->keep;  // otherwise every page is chosen
-  if (scored) {
-    if (op->type == LLMP_X_F32) LaunchSelectOf<LLMP_X_F32>(args, tiles, on);
-    if (op->type == LLMP_X_BF16) LaunchSelectOf<LLMP_X_BF16>(args, tiles, on);
-    if (op->type == LLMP_X_F16) LaunchSelectOf<LLMP_X_F16>(args, tiles, on);
+  if (form.scored) {
+    if (op->type == LLMP_X_F32) LaunchSelectOf<LLMP_X_F32>(args, form, on);
+    if (op->type == LLMP_X_BF16) LaunchSelectOf<LLMP_X_BF16>(args, form, on);
+    if (op->type == LLMP_X_F16) LaunchSelectOf<LLMP_X_F16>(args, form, on);
   }
-  if (!scored || !IsWhole(args, tiles)) hipLaunchKernelGGL(PickKernel, dim3(op->tokens, op->cache.kv_heads), dim3(kPickThreads), 0, on, args);
+  if (!form.whole) hipLaunchKernelGGL(PickKernel, dim3(op->tokens, op->cache.kv_heads), dim3(kPickThreads), 0, on, args);
   return LaunchStatus("paged_select");
 }

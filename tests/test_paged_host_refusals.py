@@ -11,3 +11,16 @@ def test_before_lies_at_a_4_byte_boundary():
     refused(lib.llmp_hip_paged_select(C.byref(select(before=0x7002)), 0x100000, 1 << 40, None), "4-byte")
     assert lib.llmp_hip_paged_attend_scratch(C.byref(attend(before=0x7000)), 256) == lib.llmp_hip_paged_attend_scratch(C.byref(attend()), 256) > 0
     assert lib.llmp_hip_paged_select_scratch(C.byref(select(before=0x7000))) == lib.llmp_hip_paged_select_scratch(C.byref(select())) > 0
+
+
+def test_scratch_of_a_selection_is_its_scores_where_they_go_through_memory():
+    lib = _lib.load()
+    wide = dict(table_width=4096, table_stride=4096, keep=4096, tokens=2048, most_tokens=2048, requests=8)
+    for kw, needs in [(dict(wide), 16),  # every page is chosen: no scores
+                      (dict(wide, keep=64, requests=1, table_width=200, table_stride=200), 16),  # one launch, the scores in LDS
+                      (dict(wide, keep=64), 2048 * 2 * 4096 * 4),  # a row of keys is more than LDS takes
+                      (dict(wide, keep=64, tokens=2, most_tokens=1, requests=2), 2 * 2 * 4096 * 4)]:  # few workgroups: two launches
+        op = select(heads=4, **kw)
+        assert lib.llmp_hip_paged_select_scratch(C.byref(op)) == needs, kw
+        for scratch, size in ((None, needs), (0x100000, needs - 1), (0x100008, needs)):
+            refused(lib.llmp_hip_paged_select(C.byref(op), scratch, size, None), "scratch")
