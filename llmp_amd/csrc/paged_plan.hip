@@ -333,6 +333,9 @@ extern "C" int llmp_hip_paged_plan(const llmp_paged_plan* op, void* stream) {
   if (op->requests < 1 || op->requests > 1 << 24 || op->table_width < 1 || op->ring_size < 1 || op->tokens < 0 || op->work_items < 0)
     return Refuse(1, "paged_plan: 1 to 2^24 requests, a table and a ring of at least one page (%d, %d, %d), tokens %d, work items %d", op->requests,
                   op->table_width, op->ring_size, op->tokens, op->work_items);
+  // (An index of an output and the step to its thread's next one stay an int together.)
+  if (op->tokens > kMostPagedLength || op->work_items > kMostPagedLength || op->ring_size > kMostPagedLength)
+    return Refuse(1, "paged_plan: at most 2^30 tokens, work items and pages of the ring (%d, %d, %d)", op->tokens, op->work_items, op->ring_size);
   if (op->page < 1 || op->page > 65536) return Refuse(1, "paged_plan: pages of 1 to 65536 tokens, not %d", op->page);
   if (op->before == nullptr || op->after == nullptr || op->table == nullptr || op->ring == nullptr || op->counters_in == nullptr ||
       op->counters == nullptr || op->starts == nullptr || op->lengths == nullptr || op->scratch == nullptr ||

@@ -2,7 +2,7 @@
 import ctypes as C
 
 from llmp_amd import _lib
-from test_paged_host import attend, refused, select
+from test_paged_host import attend, plan, refused, select
 
 
 def test_before_lies_at_a_4_byte_boundary():
@@ -24,3 +24,9 @@ def test_scratch_of_a_selection_is_its_scores_where_they_go_through_memory():
         assert lib.llmp_hip_paged_select_scratch(C.byref(op)) == needs, kw
         for scratch, size in ((None, needs), (0x100000, needs - 1), (0x100008, needs)):
             refused(lib.llmp_hip_paged_select(C.byref(op), scratch, size, None), "scratch")
+
+
+def test_plans_of_more_outputs_than_an_int_steps_through():
+    lib = _lib.load()
+    for kw in (dict(tokens=(1 << 30) + 1, work_items=1 << 30), dict(work_items=(1 << 30) + 1), dict(ring_size=(1 << 31) - 1)):
+        refused(lib.llmp_hip_paged_plan(C.byref(plan(**kw)), None), "2^30")
