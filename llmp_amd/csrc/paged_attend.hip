@@ -685,6 +685,10 @@ int CheckAttend(const llmp_paged_attend* op) {
     return Refuse(1, "paged_attend: I32 and F32 arrays at 4-byte boundaries");
   if (op->table_stride < op->table_width) return Refuse(1, "paged_attend: a table row of %d entries every %lld", op->table_width, (long long)op->table_stride);
   if (static_cast<int64_t>(op->table_width) * op->cache.page > kMostPagedLength) return Refuse(1, "paged_attend: a table row of at most 2^30 tokens");
+  // (A prompt's tiles of all KV heads are counted in an int.)
+  if (static_cast<int64_t>(op->table_width) * op->cache.page * op->cache.kv_heads > 1ll << 36)
+    return Refuse(1, "paged_attend: a table row of at most 2^36 tokens of all KV heads together (%d pages of %d, %d heads)", op->table_width, op->cache.page,
+                  op->cache.kv_heads);
   if (op->lists != nullptr && (op->list_pages < 1 || static_cast<int64_t>(op->list_pages) * op->cache.page > kMostPagedLength))
     return Refuse(1, "paged_attend: lists of one to 2^30 tokens' pages, not %d pages", op->list_pages);
   if (op->window < 0) return Refuse(1, "paged_attend: a window of no or some tokens, not %d", op->window);

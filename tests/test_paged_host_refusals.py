@@ -2,7 +2,7 @@
 import ctypes as C
 
 from llmp_amd import _lib
-from test_paged_host import attend, plan, refused, select
+from test_paged_host import attend, cache, plan, refused, select
 
 
 def test_before_lies_at_a_4_byte_boundary():
@@ -30,3 +30,12 @@ def test_plans_of_more_outputs_than_an_int_steps_through():
     lib = _lib.load()
     for kw in (dict(tokens=(1 << 30) + 1, work_items=1 << 30), dict(work_items=(1 << 30) + 1), dict(ring_size=(1 << 31) - 1)):
         refused(lib.llmp_hip_paged_plan(C.byref(plan(**kw)), None), "2^30")
+
+
+def test_tables_of_more_tokens_and_heads_than_an_int_counts_tiles_of():
+    lib = _lib.load()
+    wide = dict(table_width=1 << 26, table_stride=1 << 26)
+    for kv_heads, good in ((64, True), (65, False), (128, False)):
+        op = attend(cache(kv_heads=kv_heads), heads=kv_heads, **wide)
+        assert (lib.llmp_hip_paged_attend_scratch(C.byref(op), 256) > 0) == good
+    refused(lib.llmp_hip_paged_attend(C.byref(op), 0x100000, 1 << 40, 256, None), "2^36")
