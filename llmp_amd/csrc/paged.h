@@ -14,8 +14,9 @@ namespace llmp_hip {
 
 // 0, or the refusal: what every operator asks of a cache.
 int CheckPagedCache(const char* who, const llmp_paged_cache& cache, bool needs_edges);
-// ... of rows of head_dim values at element strides, 16-byte boundaries.
-int CheckPagedRows(const char* who, const char* name, const void* rows, int64_t token_stride, int64_t head_stride, int type);
+// ... of `tokens` times `heads` rows of head_dim values at element strides, 16-byte boundaries. (What one token or one head has for a stride
+// is not used.)
+int CheckPagedRows(const char* who, const char* name, const void* rows, int tokens, int heads, int64_t token_stride, int64_t head_stride, int type);
 
 inline int PagedElementBytes(int type) { return type == LLMP_X_F32 ? 4 : 2; }
 // (At most half of what an int counts: sums of a position and a tile's size stay in range.)

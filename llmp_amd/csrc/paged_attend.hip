@@ -671,8 +671,8 @@ size_t AttendScratch(const llmp_paged_attend& op, int cus) {
 int CheckAttend(const llmp_paged_attend* op) {
   if (op == nullptr) return Refuse(1, "paged_attend: null operands");
   if (const int bad = CheckPagedCache("paged_attend", op->cache, false); bad != 0) return bad;
-  if (const int bad = CheckPagedRows("paged_attend", "q", op->q, op->q_token_stride, op->q_head_stride, op->type); bad != 0) return bad;
-  if (const int bad = CheckPagedRows("paged_attend", "out", op->out, op->out_token_stride, op->out_head_stride, op->type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_attend", "q", op->q, op->tokens, op->heads, op->q_token_stride, op->q_head_stride, op->type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_attend", "out", op->out, op->tokens, op->heads, op->out_token_stride, op->out_head_stride, op->type); bad != 0) return bad;
   if (op->requests < 1 || op->requests > 1 << 24 || op->tokens < 1 || op->most_tokens < 1 || op->table_width < 1)
     return Refuse(1, "paged_attend: 1 to 2^24 requests, at least one token and one page a table row (%d, %d, %d, %d)", op->requests, op->tokens,
                   op->most_tokens, op->table_width);

@@ -304,11 +304,12 @@ int CheckPagedCache(const char* who, const llmp_paged_cache& c, bool needs_edges
   return 0;
 }
 
-int CheckPagedRows(const char* who, const char* name, const void* rows, int64_t token_stride, int64_t head_stride, int type) {
+int CheckPagedRows(const char* who, const char* name, const void* rows, int tokens, int heads, int64_t token_stride, int64_t head_stride, int type) {
   if (rows == nullptr) return Refuse(1, "%s: null %s", who, name);
   if (type != LLMP_X_F32 && type != LLMP_X_BF16 && type != LLMP_X_F16) return Refuse(1, "%s: F32, BF16 or F16 rows, not type %d", who, type);
   const int per = 16 / PagedElementBytes(type);
-  if (reinterpret_cast<uintptr_t>(rows) % 16 != 0 || token_stride < 0 || head_stride < 0 || token_stride % per != 0 || head_stride % per != 0)
+  const auto bad = [&](int count, int64_t stride) { return count > 1 && (stride < 0 || stride % per != 0); };
+  if (reinterpret_cast<uintptr_t>(rows) % 16 != 0 || bad(tokens, token_stride) || bad(heads, head_stride))
     return Refuse(1, "%s: %s's rows lie at 16-byte boundaries (strides %lld, %lld)", who, name, (long long)token_stride, (long long)head_stride);
   return 0;
 }

@@ -558,7 +558,7 @@ void LaunchSelectOf(const SelectArgs& args, const SelectForm& form, hipStream_t 
 int CheckSelect(const llmp_paged_select* op) {
   if (op == nullptr) return Refuse(1, "paged_select: null operands");
   if (const int bad = CheckPagedCache("paged_select", op->cache, true); bad != 0) return bad;
-  if (const int bad = CheckPagedRows("paged_select", "q", op->q, op->q_token_stride, op->q_head_stride, op->type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_select", "q", op->q, op->tokens, op->heads, op->q_token_stride, op->q_head_stride, op->type); bad != 0) return bad;
   if (op->requests < 1 || op->requests > 1 << 24 || op->tokens < 1 ||  op->most_tokens < 1 || op->table_width < 1)
     return Refuse(1, "paged_select: 1 to 2^24 requests, at least one token and one page a table row (%d, %d, %d, %d)", op->requests, op->tokens,
                   op->most_tokens, op->table_width);

@@ -257,8 +257,8 @@ extern "C" int llmp_hip_paged_store(const llmp_paged_store* op, void* stream) {
   if (const int bad = CheckPagedCache("paged_store", op->cache, false); bad != 0) return bad;
   if (op->tokens < 0 || op->work_items < 0) return Refuse(1, "paged_store: tokens %d, work items %d", op->tokens, op->work_items);
   if (op->tokens == 0 || op->work_items == 0) return 0;
-  if (const int bad = CheckPagedRows("paged_store", "k", op->k, op->k_token_stride, op->k_head_stride, op->type); bad != 0) return bad;
-  if (const int bad = CheckPagedRows("paged_store", "v", op->v, op->v_token_stride, op->v_head_stride, op->type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_store", "k", op->k, op->tokens, op->cache.kv_heads, op->k_token_stride, op->k_head_stride, op->type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_store", "v", op->v, op->tokens, op->cache.kv_heads, op->v_token_stride, op->v_head_stride, op->type); bad != 0) return bad;
   if (op->work == nullptr || reinterpret_cast<uintptr_t>(op->work) % 16 != 0) return Refuse(1, "paged_store: work items at a 16-byte boundary");
   BeginLaunches();
   WithTypeAndHead(op->type, op->cache.head_dim, [&](auto type, auto head) { LaunchStore<decltype(type)::value, decltype(head)::value>(*op, static_cast<hipStream_t>(stream)); });
@@ -272,8 +272,8 @@ extern "C" int llmp_hip_paged_read(const llmp_paged_cache* cache, const int32_t*
   if (count < 0 || page_stride < 0) return Refuse(1, "paged_read: %d pages every %lld", count, (long long)page_stride);
   if (count == 0) return 0;
   if (pages == nullptr || reinterpret_cast<uintptr_t>(pages) % 4 != 0) return Refuse(1, "paged_read: page numbers at a 4-byte boundary");
-  if (const int bad = CheckPagedRows("paged_read", "k_out", k_out, 0, 0, type); bad != 0) return bad;
-  if (const int bad = CheckPagedRows("paged_read", "v_out", v_out, 0, 0, type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_read", "k_out", k_out, 1, 1, 0, 0, type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("paged_read", "v_out", v_out, 1, 1, 0, 0, type); bad != 0) return bad;
   BeginLaunches();
   WithTypeAndHead(type, cache->head_dim, [&](auto t, auto head) {
     LaunchRead<decltype(t)::value, decltype(head)::value>(*cache, pages, page_stride, count, k_out, v_out, static_cast<hipStream_t>(stream));

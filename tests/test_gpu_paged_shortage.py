@@ -184,3 +184,21 @@ def test_a_window_past_every_position_hides_nothing(device, window):
         got = ops.paged_attend(c, x, dev(form, device), n, s, 0.125, window=window)
         near(got, want, far, f"{form.shape[1]} pages a row")
         assert torch.equal(got, ops.paged_attend(c, x, dev(form, device), n, s, 0.125))
+
+
+def test_one_token_of_a_row_of_odd_length(device):
+    """A step of one token whose q, k and v are pieces of a row that no 16 bytes divide: its stride is not used."""
+    g = np.random.default_rng(17)
+    cache = random_cache(g, 4, 2, 16, 64)
+    host, c = {name: x.copy() for name, x in cache.items()}, to_device(cache, device)
+    rows = torch.from_numpy(g.standard_normal((3, 12 * 64 + 3)).astype(np.float32)).to(device)
+    q, k, v = (rows[:, a * 64:b * 64].view(3, b - a, 64)[:1] for a, b in ((0, 8), (8, 10), (10, 12)))
+    assert q.stride(0) % 4 != 0
+    table, work = np.array([[2, 1]], np.int32), np.array([[1, 0, 3, 1]], np.int32)
+    ops.paged_store(c, k, v, dev(work, device))
+    plain.store(host, k.cpu().numpy(), v.cpu().numpy(), work.tolist())
+    for name in host:
+        same(c[name], host[name], name)
+    where = dev(table, device), dev(np.array([20], np.int32), device), dev(np.array([0, 1], np.int32), device)
+    near(ops.paged_attend(c, q, *where, 0.125), *plain.attend(host, q.cpu().numpy(), table, [20], [0, 1], 0.125, "f32"), "out")
+    same(ops.paged_select(c, q, *where, 1), plain.lists(host, q.cpu().numpy(), table, [20], [0, 1], 1), "lists")

@@ -2,7 +2,7 @@
 import ctypes as C
 
 from llmp_amd import _lib
-from test_paged_host import attend, cache, plan, refused, select
+from test_paged_host import attend, cache, plan, refused, select, store
 
 
 def test_before_lies_at_a_4_byte_boundary():
@@ -39,3 +39,13 @@ def test_tables_of_more_tokens_and_heads_than_an_int_counts_tiles_of():
         op = attend(cache(kv_heads=kv_heads), heads=kv_heads, **wide)
         assert (lib.llmp_hip_paged_attend_scratch(C.byref(op), 256) > 0) == good
     refused(lib.llmp_hip_paged_attend(C.byref(op), 0x100000, 1 << 40, 256, None), "2^36")
+
+
+def test_strides_of_one_token_or_one_head_are_not_looked_at():
+    lib = _lib.load()
+    one = dict(tokens=1, most_tokens=1, requests=1)
+    assert lib.llmp_hip_paged_attend_scratch(C.byref(attend(q_token_stride=257, out_token_stride=1, **one)), 256) > 0
+    assert lib.llmp_hip_paged_select_scratch(C.byref(select(q_token_stride=257, **one))) > 0
+    assert lib.llmp_hip_paged_attend_scratch(C.byref(attend(cache(kv_heads=1), heads=1, q_head_stride=1, out_head_stride=-1)), 256) > 0
+    refused(lib.llmp_hip_paged_attend(C.byref(attend(q_head_stride=65, **one)), 0x100000, 1 << 40, 256, None), "16-byte")
+    refused(lib.llmp_hip_paged_store(C.byref(store(cache(kv_heads=1), tokens=2, k_token_stride=65, k_head_stride=1)), None), "16-byte")
