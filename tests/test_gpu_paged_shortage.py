@@ -201,4 +201,4 @@ def test_one_token_of_a_row_of_odd_length(device):
         same(c[name], host[name], name)
     where = dev(table, device), dev(np.array([20], np.int32), device), dev(np.array([0, 1], np.int32), device)
     near(ops.paged_attend(c, q, *where, 0.125), *plain.attend(host, q.cpu().numpy(), table, [20], [0, 1], 0.125, "f32"), "out")
-    same(ops.paged_select(c, q, *where, 1), plain.lists(host, q.cpu().numpy(), table, [20], [0, 1], 1), "lists")
+    same(ops.paged_select(c, q, *where, 1, first=0), plain.lists(host, q.cpu().numpy(), table, [20], [0, 1], 1, first=0), "lists")
