@@ -671,19 +671,19 @@ def _paged_cache(cache):
     low, high = cache.get("low"), cache.get("high")
     pages, kv_heads, page, head_dim = k.shape
     heads = pages * kv_heads
-    whole = (k.dtype is torch.int8 and k.is_contiguous() and v.dtype is torch.int8 and v.is_contiguous() and v.shape == (pages, kv_heads, head_dim, page)
+    whole = (k.is_cuda and k.dtype is torch.int8 and k.is_contiguous() and v.dtype is torch.int8 and v.is_contiguous() and v.shape == (pages, kv_heads, head_dim, page)
              and k_scale.dtype is torch.float32 and k_scale.is_contiguous() and k_scale.numel() == heads
              and v_scale.dtype is torch.float32 and v_scale.is_contiguous() and v_scale.numel() == heads)
     for edge in (low, high):
         whole = whole and (edge is None or (edge.dtype is torch.int8 and edge.is_contiguous() and edge.numel() == heads * head_dim))
-    assert whole, "the cache's arrays are whole, of one set of sizes"
+    assert whole, "the cache's arrays are whole, of one set of sizes, on the GPU"
     return _lib.PagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), low.data_ptr() if low is not None else None,
                            high.data_ptr() if high is not None else None, pages, kv_heads, page, head_dim)
 
 
 def _int32(*tensors):
     for t in tensors:
-        assert t.dtype is torch.int32 and (t.is_contiguous() or t.stride(-1) == 1), "int32 arrays in one piece"
+        assert t.dtype is torch.int32 and t.is_cuda and (t.is_contiguous() or t.stride(-1) == 1), "int32 arrays in one piece on the GPU"
 
 
 _UNITS = {}
@@ -764,8 +764,8 @@ def paged_store(cache, k, v, work):
     c = _paged_cache(cache)
     tokens, kv_heads, head_dim = k.shape
     (kt, kh, kd), (vt, vh, vd) = k.stride(), v.stride()
-    assert kv_heads == c.kv_heads and head_dim == c.head_dim and v.shape == k.shape and k.dtype is v.dtype and kd == vd == 1
-    assert work.dtype is torch.int32 and work.is_contiguous() and work.shape[1] == 4
+    assert k.is_cuda and v.is_cuda and kv_heads == c.kv_heads and head_dim == c.head_dim and v.shape == k.shape and k.dtype is v.dtype and kd == vd == 1
+    assert work.is_cuda and work.dtype is torch.int32 and work.is_contiguous() and work.shape[1] == 4
     op = _lib.PagedStore(c, k.data_ptr(), v.data_ptr(), work.data_ptr(), kt, kh, vt, vh, _X_TYPES[k.dtype], tokens, work.shape[0])
     _lib.check(lib.llmp_hip_paged_store(C.byref(op), _stream()))
 
@@ -775,7 +775,7 @@ def paged_read(cache, pages, dtype=torch.float32):
     number outside the cache gives zeros."""
     lib = _lib.load()
     c = _paged_cache(cache)
-    assert pages.dim() == 1 and pages.dtype is torch.int32
+    assert pages.is_cuda and pages.dim() == 1 and pages.dtype is torch.int32
     n = pages.shape[0]
     k, v = torch.empty((2, n, c.kv_heads, c.page, c.head_dim), dtype=dtype, device=pages.device).unbind()
     _lib.check(lib.llmp_hip_paged_read(C.byref(c), pages.data_ptr(), pages.stride(0), n, _X_TYPES[dtype], k.data_ptr(), v.data_ptr(), _stream()))
@@ -790,7 +790,7 @@ def _paged_queries(q, c, table, lengths, starts, before):
     tokens, heads, head_dim = q.shape
     n, width = table.shape
     token_stride, head_stride, one = q.stride()
-    assert head_dim == c.head_dim and one == 1 and lengths.shape == (n,) and starts.shape == (n + 1,)
+    assert q.is_cuda and head_dim == c.head_dim and one == 1 and lengths.shape == (n,) and starts.shape == (n + 1,)
     return tokens, heads, n, width, token_stride, head_stride
 
 
@@ -809,11 +809,11 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, before=None, window
         out_token, out_head = heads * c.head_dim, c.head_dim
     else:
         out_token, out_head, one = out.stride()
-        assert out.shape == q.shape and out.dtype is q.dtype and one == 1
+        assert out.is_cuda and out.shape == q.shape and out.dtype is q.dtype and one == 1
     if lists is not None:
         _int32(lists)
         assert lists.is_contiguous() and lists.shape[:2] == (tokens, c.kv_heads)
-    assert sinks is None or (sinks.dtype == torch.float32 and sinks.shape == (heads,) and sinks.is_contiguous())
+    assert sinks is None or (sinks.is_cuda and sinks.dtype == torch.float32 and sinks.shape == (heads,) and sinks.is_contiguous())
     if tokens == 0:
         return out
     op = _lib.PagedAttend(c, q.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(lists), _ptr(sinks),
@@ -836,7 +836,7 @@ def paged_select(cache, q, table, lengths, starts, keep, *, before=None, first=1
     if out is None:
         out = torch.empty((tokens, c.kv_heads, keep), dtype=torch.int32, device=q.device)
     else:
-        assert out.shape == (tokens, c.kv_heads, keep) and out.dtype is torch.int32 and out.is_contiguous()
+        assert out.is_cuda and out.shape == (tokens, c.kv_heads, keep) and out.dtype is torch.int32 and out.is_contiguous()
     if tokens == 0:
         return out
     op = _lib.PagedSelect(c, q.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), out.data_ptr(), q_token, q_head,

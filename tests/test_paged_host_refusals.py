@@ -1,7 +1,10 @@
 """What the paged cache's entry points refuse, and the scratch they ask for, beyond tests/test_paged_host.py."""
 import ctypes as C
 
-from llmp_amd import _lib
+import pytest
+import torch
+
+from llmp_amd import _lib, ops
 from test_paged_host import attend, cache, plan, refused, select, store
 
 
@@ -49,3 +52,18 @@ def test_strides_of_one_token_or_one_head_are_not_looked_at():
     assert lib.llmp_hip_paged_attend_scratch(C.byref(attend(cache(kv_heads=1), heads=1, q_head_stride=1, out_head_stride=-1)), 256) > 0
     refused(lib.llmp_hip_paged_attend(C.byref(attend(q_head_stride=65, **one)), 0x100000, 1 << 40, 256, None), "16-byte")
     refused(lib.llmp_hip_paged_store(C.byref(store(cache(kv_heads=1), tokens=2, k_token_stride=65, k_head_stride=1)), None), "16-byte")
+
+
+def test_the_wrappers_take_no_host_memory():
+    """A tensor in host memory would be an address that no kernel may read: refused before anything is asked of the GPU."""
+    host = ops.paged_cache(4, 2, 16, 64, device="cpu")
+    ints = [torch.zeros(n, dtype=torch.int32) for n in (2, 2, 8, 3, 3)]
+    q, table = torch.zeros(2, 4, 64), torch.zeros((2, 2), dtype=torch.int32)
+    work = torch.zeros((2, 4), dtype=torch.int32)
+    for call in (lambda: ops.paged_plan(ints[0], ints[1], table, ints[2], ints[3], 16, 2),
+                 lambda: ops.paged_store(host, q[:, :2], q[:, :2], work),
+                 lambda: ops.paged_read(host, ints[0]),
+                 lambda: ops.paged_attend(host, q, table, ints[0], ints[3], 0.125),
+                 lambda: ops.paged_select(host, q, table, ints[0], ints[3], 2)):
+        with pytest.raises(AssertionError, match="GPU"):
+            call()
