@@ -693,7 +693,8 @@ int llmp_hip_paged_read(const llmp_paged_cache* cache, const int32_t* pages, int
  * for F32). Probabilities times the V scale are rounded to F16 (for F32 to a sum of two) against V codes as F16 (exact): one is off by 2^-11
  * (F32: 2^-22) of itself, or by 2^-35 (F32: 2^-46) of the row's largest where that is more.
  * scratch: llmp_hip_paged_attend_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal, the reason in last_error).
- * Launch arguments depend on the descriptor alone, never on the lengths: a captured launch replays at other lengths. */
+ * Launch arguments depend on the descriptor alone, never on the lengths: a captured launch replays at other lengths. The sums are cut by
+ * the step's whole work: a row's last bits depend on what else the call holds. out does not overlap q. */
 typedef struct llmp_paged_attend {
   llmp_paged_cache cache;
   const void* q;

@@ -15,9 +15,9 @@
 //   innermost, is 16 bytes of one dimension a lane.
 // A lane's 16 tokens are of one page (pages are multiples of 16): one scale each for K and V.
 //
-// Measured (both launches, 8 KV heads): 131072 tokens of one request at head size 128, 268 MB, 61 us, 4.4 TB/s (a large copy reaches
+// Measured (both launches, 8 KV heads): 131072 tokens of one request at head size 128, 268 MB, 61.6 us, 4.4 TB/s (a large copy reaches
 // 4.9, a read alone 7.0); 32 requests of up to 16384 tokens, 453 MB, 98 us, 4.6 TB/s; 8192 tokens at 256 in F32, 34 MB, a tile a
-// wave, 19.6 us: that is the chain of a launch, the lengths, the table, one tile and the waves' meeting, and the join's.
+// wave, 19.7 us: that is the chain of a launch, the lengths, the table, one tile and the waves' meeting, and the join's.
 #include <cmath>
 #include <type_traits>
 
@@ -631,7 +631,9 @@ void LaunchFewOf(const PagedAttendArgs& args, int groups, hipStream_t stream) {
 // Requests of more rows than this are the many rows' form's, where the call has any and is work enough: rows times their most tokens
 // times head size. In us, this form against that one, bf16, 8 KV heads of 128, groups of 4: of 1000 tokens, 128 and 512 and 1000 new
 // 24/41, 36/49, 58/50; of 2000, 32, 256, 512, 1000 24/42, 32/53, 52/57, 93/73; of 8000, 32, 128, 256, 512 31/60, 60/77, 98/90, 168/117;
-// groups of 2 at 256, of 2000 128, 256, 512 31/54, 40/55, 70/61; groups of 7 at 64, 64, 512, 1000 21/34, 38/38, 42/43.
+// groups of 2 at 256, of 2000 128, 256, 512 31/54, 40/55, 70/61; groups of 7 at 64, 64, 512, 1000 21/34, 38/38, 42/43. (The tables there were
+// as wide as the request is long: the lengths are the device's to know, so a wider table moves calls of fewer tokens to the other
+// form, at the cost that the figures of its left sides show.)
 constexpr int kFewRows = 64;
 constexpr int64_t kFewWork = 4000000ll * 128;
 constexpr int kMostGroup = 1024, kMostFewRows = 1 << 20;  // (PagedDivide's range together)

@@ -18,8 +18,10 @@
 // (groups of 4 at 128) 154/172, behind 6000 319/346, a prompt of 4000 (groups of 2 at 256) 196/216; of 2000 there, whose last 128
 // rows are nearly twice the share, 102/90, 6 ragged prompts 147/109.
 //
-// Measured at the chunk of 2048 behind 2048, 103 GFLOP: 150 us, 0.69 PFLOP/s (a large F16 product by the library reaches 1.15): 388
-// vector operations a wave's 32 x 64 logits, about 1800 cycles beside the products' 1024, at two waves a SIMD.
+// Measured at the chunk of 2048 behind 2048, 103 GFLOP: 154 us with the list's and the join's launches, 0.67 PFLOP/s (a large F16 product
+// by the library reaches 1.15): 388 vector operations a wave's 32 x 64 logits, about 1800 cycles beside the products' 1024, at two
+// waves a SIMD. The products stand apart from the softmax by fences that the compiler's scheduling does not cross; without
+// them it is 155.7 us where it is 155.3.
 #include <type_traits>
 
 #include "paged_attend.h"
@@ -221,7 +223,6 @@ __global__ __launch_bounds__(ManyGeo<D>::kThreads, 2) void ManyKernel(const Many
   constexpr int kWaveRows = G::kWaveRows, kThreads = G::kThreads, kInner = G::kInner;
   constexpr int kSteps = D / kInner, kBlocks = D / kWaveRows, kPieces = D / 16, kLoads = 4 * D / kThreads;
   typedef std::conditional_t<kWaveRows == 32, F32x16, F32x4> Values;  // a lane's of a block of dimensions
-  typedef std::conditional_t<kWaveRows == 32, I32x16, I32x4> Dots;
   constexpr int kValues = kWaveRows * kWaveRows / kWave;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const PagedAttendArgs& a = m.a;

@@ -12,7 +12,7 @@
 // (a histogram a pass), and writes the pages at or above it in order; ties go to the lower page. Where there are workgroups enough
 // for the card, both are one launch and the scores stay in LDS.
 //
-// Measured: 8 requests of up to 65536 tokens, pages of 64, 8 KV heads of 128: the scores 9.4 us for 7 MB of codes (a chain: lengths, table,
+// Measured: 8 requests of up to 65536 tokens, pages of 64, 8 KV heads of 128: the scores 9.6 us for 7 MB of codes (a chain: lengths, table,
 // codes, products), the choice 6.3 us.
 #include "paged_attend.h"
 

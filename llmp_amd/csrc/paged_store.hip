@@ -11,8 +11,8 @@
 //
 // Measured: a decode step of 63 tokens, 8 KV heads of 128, 5.8 us, the chain of item, rows, barrier and codes; prompts of 3139 tokens,
 // 8 heads of 256 in F16, 18.8 us for 39 MB, 2.1 TB/s (the chain again, with every workgroup on the device at once: rows kept in
-// registers, four a thread, took 20.0 us and the decode step 8.6, with code for four rows' divisions where one row is). Reading 14 MB of
-// codes back as 27 MB of F16 values 8.2 us, 4.9 TB/s.
+// registers, four a thread, took 20.0 us and the decode step 8.6, with code for four rows' divisions where one row is). Reading 13 MB of
+// codes back as 27 MB of F16 values 8.6 us, 4.7 TB/s; 8 MB as 17 MB of BF16 8.2 us, 3.0 TB/s, its launch and chain being most of it.
 #include "paged.h"
 
 namespace llmp_hip {
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kStoreThreads) void StoreKernel(const llmp_paged_st
     return;
   }
   // V: the new codes to LDS, a dimension's 16-token pieces whole; then piece by piece into the page.
-  const int pitch = c.page + 4;  // (four bytes on: the eight dimensions a lane writes of a token are in eight banks)
+  const int pitch = c.page + 4;  // (four bytes on: a token's lanes write dimensions eight apart, 8 * pitch bytes, which are eight banks at every page size)
   for (int i = tid / kLanes; i < it.count; i += kRows) {
     float v[8];
     LoadEight<TYPE>(x, first + i * token_stride + d0, v);
