@@ -2,7 +2,7 @@
 shared latent vector a token (keys and values of all heads come from it, a small rotated key beside it) does in a layer.
 
 The paged cache holds, for each token, `width` latent values and `rope` values of the rotated key: both in 16 bits, or the
-latent in 8 (E4M3 codes, an E8M0 scale for every 32 of them). A request's row of the table names its pages in order; a slot is
+latent in 8 (E4M3 codes, one E8M0 scale a token). A request's row of the table names its pages in order; a slot is
 page * (tokens a page) + offset. A case's "path" says which operator a pass makes:
 
   rope     part of every head's channels rotated by their token's position: halves or neighbours, plain or YaRN frequencies
@@ -145,8 +145,7 @@ def _rope_options(case):
 
 
 def _codes(x):
-    """E4M3 codes of float32 values (nearest, ties to even, at most 448) and the E8M0 scales of every 32."""
-    x = x.reshape(x.shape[:-1] + (-1, 32))
+    """E4M3 codes of float32 rows (nearest, ties to even, at most 448) and the rows' E8M0 scales."""
     bits = (x.abs().amax(-1) * (1.0 / 448.0)).view(torch.int32)
     e = ((bits >> 23) + ((bits & 0x7FFFFF) != 0).to(torch.int32)).clamp(max=253)
     y = x * ((254 - e) << 23).view(torch.float32)[..., None]
@@ -154,7 +153,7 @@ def _codes(x):
     large = ((bits + 0x7FFFF + ((bits >> 20) & 1)) >> 20) - 960
     small = torch.round(y.abs() * 512.0).to(torch.int32)
     code = torch.where(bits < 0x3C800000, small, large).clamp(max=0x7E) + torch.where(y < 0, 128, 0)
-    return code.to(torch.uint8).flatten(-2), e.to(torch.uint8)
+    return code.to(torch.uint8), e.to(torch.uint8)
 
 
 def _values(codes, scales, dtype):
@@ -163,8 +162,8 @@ def _values(codes, scales, dtype):
     mag, sign = c & 0x7F, 1 - 2 * (c >> 7)
     exponent = (mag >> 3).clamp(min=1)
     fraction = torch.where(mag < 8, mag, 8 + (mag & 7))
-    x = torch.ldexp((fraction * sign).to(dtype), exponent - 10).reshape(codes.shape[:-1] + (-1, 32))
-    return torch.ldexp(x, (scales.to(torch.int32) - 127)[..., None]).flatten(-2)
+    x = torch.ldexp((fraction * sign).to(dtype), exponent - 10)
+    return torch.ldexp(x, (scales.to(torch.int32) - 127)[..., None])
 
 
 def _cache(case, pages, g, kept):
@@ -173,7 +172,7 @@ def _cache(case, pages, g, kept):
     step = max(1, (1 << 26) // (page * width))
     bits8 = case["bits"] == 8
     latent = torch.empty((pages, page, width), dtype=torch.uint8 if bits8 else kept, device="cuda")
-    scale = torch.empty((pages, page, width // 32), dtype=torch.uint8, device="cuda") if bits8 else None
+    scale = torch.empty((pages, page), dtype=torch.uint8, device="cuda") if bits8 else None
     for at in range(0, pages, step):
         n = min(step, pages - at)
         x = torch.randn((n, page, width), device="cuda", generator=g) + 0.7 * torch.randn((n, 1, width), device="cuda", generator=g)
@@ -315,7 +314,7 @@ def _store(s):
         x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * s["weight"]
     key = _rotate(s["rows"][:, width:], s["positions"], s["rope"], s["layout"], {})
     slots, read = s["slots"].long(), s["read_slots"].long()
-    flat = {name: c.view(-1, c.shape[-1]) for name, c in cache.items()}
+    flat = {name: c.flatten(0, 1) for name, c in cache.items()}
     flat["rope"][slots] = key.to(kept)
     if s["bits"] == 8:
         flat["latent"][slots], flat["scale"][slots] = _codes(x)
@@ -398,7 +397,7 @@ def work(case):
                 "flops": 2 * pairs * heads * (nope + rope + value)}
     width, rope = case["width"], case["rope"]
     kept = SIZES[case.get("kept", case["dtype"])]
-    row = (width + width // 32 if case["bits"] == 8 else kept * width) + kept * rope  # a token's in the cache
+    row = (width + 1 if case["bits"] == 8 else kept * width) + kept * rope  # a token's in the cache
     if case["path"] == "store":
         read = tokens if case["read"] == "new" else sum(after)
         # Rows in and into the cache with their slots and positions; rows out of the cache as values.
@@ -436,14 +435,13 @@ def _exact_rotation(x, positions, layout, options):
 
 def _exact_codes(x):
     """The values that 8 bits hold of x: the smallest power of two s with |x| <= 448 s, then the nearest E4M3 value."""
-    x = x.reshape(x.shape[:-1] + (-1, 32))
     most = x.abs().amax(-1, keepdim=True)
     s = torch.exp2(torch.ceil(torch.log2(most / 448.0)).clamp(min=-127.0))
     s = torch.where(most > 448.0 * s, 2.0 * s, s)
     s = torch.where((most <= 224.0 * s) & (s > 2.0 ** -127), 0.5 * s, s)
     y = x / s
     step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3.0)
-    return (torch.round(y / step) * step * s).flatten(-2)
+    return torch.round(y / step) * step * s
 
 
 def exact(case, seed):
@@ -506,7 +504,7 @@ def _exact_store(s):
         x = _exact_codes(x)
     key = _exact_rotation(s["rows"][:, width:], s["positions"], s["layout"], {})
     latent = cache["latent"].view(-1, width)
-    latent = _values(latent, cache["scale"].view(-1, width // 32), torch.float64) if s["bits"] == 8 else latent.double()
+    latent = _values(latent, cache["scale"].view(-1), torch.float64) if s["bits"] == 8 else latent.double()
     rope = cache["rope"].view(-1, s["rope"]).double()
     latent[s["slots"].long()] = x
     rope[s["slots"].long()] = key
