@@ -734,6 +734,135 @@ typedef struct llmp_paged_select {
 size_t llmp_hip_paged_select_scratch(const llmp_paged_select* op);
 int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch, size_t scratch_bytes, void* stream);
 
+/* ------------------------------------------------------------ attention over latent vectors
+ * No counterpart in the reference: the layer of models whose keys and values of all heads come from one latent vector a token, with a
+ * small rotated key beside it that all heads share. In the expanded form every head's keys and values are made from the latent rows
+ * (a caller's product) and attended (llmp.latent.prompt); in the absorbed form each head's query goes to the latent width
+ * (llmp.latent.project), is attended with the latent rows themselves as keys and values (llmp.latent.attend), and the result comes
+ * back to the head's width (llmp.latent.project). llmp.rope rotates the queries' part, llmp.latent.store the key's on its way into the cache.
+ *
+ * llmp.rope: y = x, but in every head channels first to first + n_dims - 1 are rotated: pair p by the angle positions[token] * f_p, where a pair
+ * is channels (p, p + n_dims / 2) of them or, interleaved, (2p, 2p + 1): (a cos - b sin, a sin + b cos) * magnitude, or with
+ * `inverse` by the negative angle (which is the rotation's gradient). f_p is turns[p] / 2^64 of a whole turn a position
+ * (device U64 [n_dims / 2], as llmp_hip_rope_table makes it): the angle is exact to 2^-33 of a turn at any position, negative ones
+ * among them. x and out are LLMP_X_* `type` [tokens][heads][head_dim], element strides, a head's channels side by side; out is x (with
+ * its strides: the other channels are then not touched) or does not overlap it. Cosines and sines are F32 (2^-24 off), products and sums F32,
+ * rounded once. n_dims up to 1024. One launch. */
+typedef struct llmp_rope {
+  const void* x;
+  void* out;
+  const int32_t* positions;
+  const uint64_t* turns;
+  int64_t tokens;
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  int32_t type, heads, head_dim, first, n_dims, interleaved, inverse;
+  float magnitude;
+} llmp_rope;
+int llmp_hip_rope(const llmp_rope* op, void* stream);
+/* The table, on the host, in FP64 (no device is used): f_p = base^(-2p / n_dims) / freq_factors[p] (null: 1), times freq_scale, or where ext_factor is
+ * not zero freq_scale's mix with the unscaled one: weight ext_factor up to pair corr_low, falling to none at pair corr_high. */
+int llmp_hip_rope_table(int n_dims, double base, double freq_scale, double ext_factor, double corr_low, double corr_high,
+                        const float* freq_factors, uint64_t* turns);
+
+/* The paged latent cache: for a token, by its slot (page * `page` + offset in the page, as llmp.paged.plan gives them),
+ *   latent  [pages][page][width]       16-bit values of LLMP_X_BF16 or LLMP_X_F16 `type`, or E4M3 codes where scale is not null
+ *   scale   U8 [pages][page] or null   E8M0: a token's values are its codes times 2^(scale - 127)
+ *   rope    [pages][page][rope_width]  16-bit values of `type`
+ * width 256 or 512, rope_width 32 or 64, `page` a multiple of 16 from 16 to 256, at most 2^30 slots; the arrays lie at 16-byte boundaries. */
+typedef struct llmp_latent_cache {
+  void* latent;
+  void* scale;
+  void* rope;
+  int32_t type, pages, page, width, rope_width;
+} llmp_latent_cache;
+
+/* llmp.latent.store: token i's rows into slots[i] (one outside the cache: the row is skipped; the slots of a call that are not
+ * skipped are distinct, or their rows' pieces end there in any mixture). latent (LLMP_X_* `type`, latent_stride elements apart, rows at 16-byte
+ * boundaries) is normalised where `weight` (F32 [width], 16-byte aligned) is given: c / sqrt(mean of c^2 + eps) * weight. It is rounded once, to the cache's type
+ * or to E4M3 with the smallest scale that holds the row (448 at most; infinities become 448 times the largest scale, a NaN a NaN). rope (the same type,
+ * rope_stride elements apart) is rotated as llmp.rope has it with n_dims = rope_width, by positions[i] and `turns` times `magnitude`; turns null: stored as
+ * it is. One launch. */
+typedef struct llmp_latent_store {
+  llmp_latent_cache cache;
+  const void* latent;
+  const void* rope;
+  const int32_t* slots;
+  const int32_t* positions;
+  const uint64_t* turns;
+  const float* weight;
+  int64_t latent_stride, rope_stride;
+  int32_t type, tokens, interleaved;
+  float eps, magnitude;
+} llmp_latent_store;
+int llmp_hip_latent_store(const llmp_latent_store* op, void* stream);
+
+/* llmp.latent.read: rows back as values: latent_out [count][width] and rope_out [count][rope_width] of LLMP_X_* `type`, 16-byte aligned, by their slots
+ * (one outside the cache gives zeros). One launch. */
+int llmp_hip_latent_read(const llmp_latent_cache* cache, const int32_t* slots, int64_t count, int type, void* latent_out, void* rope_out, void* stream);
+
+/* llmp.latent.project: y[t][h][n] = sum over k of x[t][h][k] * w[h][n][k]: every head's rows times that head's matrix. x, w and y are of one type
+ * (LLMP_X_BF16 or LLMP_X_F16), element strides, the last index side by side, rows at 16-byte boundaries; k and n multiples of 32, sums F32,
+ * rounded once. y overlaps neither. One launch. */
+typedef struct llmp_latent_project {
+  const void* x;
+  const void* w;
+  void* y;
+  int64_t x_token_stride, x_head_stride, w_head_stride, w_row_stride, y_token_stride, y_head_stride;
+  int32_t type, tokens, heads, k, n;
+} llmp_latent_project;
+int llmp_hip_latent_project(const llmp_latent_project* op, void* stream);
+
+/* llmp.latent.attend: causal attention of a step's queries over their requests' latent rows: request r's rows are starts[r] to starts[r + 1] - 1,
+ * at positions before[r] on (before null: at the last of its lengths[r] positions); a token at position p sees positions 0 to min(p, length - 1).
+ * Logits are scale * (q_latent . latent + q_rope . rope), the result sum of softmax * latent, [tokens][heads][width]. The queries and the result are of
+ * the cache's type, element strides, rows at 16-byte boundaries. A table entry that is no page of the cache, a token that a row does not see, and what they hold
+ * (infinities and NaN too) change nothing of the row; a row that sees nothing is zero; rows past starts[requests] are not written.
+ * The products' inputs are the 16-bit values as they are (codes are exact in both types, times their scale in F32); sums, maximum and
+ * normalisation are F32; a weight is rounded to the cache's type once (BF16 2^-8 of itself; F16 2^-11, or 2^-33 of the row's largest
+ * where that is more). most_tokens: at least every request's new tokens (a bound from the host; the form goes by it). scratch:
+ * llmp_hip_latent_attend_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal, the reason in last_error). Launch arguments depend on the
+ * descriptor alone, never on the lengths: a captured launch replays at other lengths. The sums are cut by the step's whole work: a row's
+ * last bits depend on what else the call holds. out overlaps no operand. Two launches. */
+typedef struct llmp_latent_attend {
+  llmp_latent_cache cache;
+  const void* q_latent;
+  const void* q_rope;
+  void* out;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const int32_t* table;
+  const int32_t* before; /* I32 [requests], the plan's; null: every new token found a page */
+  int64_t q_latent_token_stride, q_latent_head_stride, q_rope_token_stride, q_rope_head_stride, out_token_stride, out_head_stride, table_stride;
+  int32_t heads, requests, tokens, most_tokens, table_width;
+  float scale;
+} llmp_latent_attend;
+size_t llmp_hip_latent_attend_scratch(const llmp_latent_attend* op, int cus);
+int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream);
+
+/* llmp.latent.prompt: causal attention in the expanded form over ragged requests: request r's queries are rows starts[r] to starts[r + 1] - 1 of q
+ * [tokens][heads][nope + rope_width] (the rotated part last), its keys rows key_starts[r] to key_starts[r + 1] - 1 of k [keys][heads][nope], of k_rope
+ * [keys][rope_width], which all heads share, and of v [keys][heads][value]; its queries are at the last positions of its keys (key_starts
+ * null: starts). Logits are scale * (q . (k, k_rope)); out [tokens][heads][value]. All of one type (LLMP_X_BF16 or LLMP_X_F16), element strides, the last index side by
+ * side, rows at 16-byte boundaries; nope and value are both 64 or both 128, rope_width 32 or 64. What a row does not see changes nothing
+ * of it; a row that sees nothing is zero; rows past starts[requests] are not written. Roundings and most_tokens as llmp.latent.attend's. Where a
+ * call has few rows for the device, its keys are cut into runs, by the descriptor's sizes alone: a row's last bits depend on those. scratch:
+ * llmp_hip_latent_prompt_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal). A captured launch replays with other starts. out overlaps no
+ * operand. One launch, two where keys are cut. */
+typedef struct llmp_latent_prompt {
+  const void* q;
+  const void* k;
+  const void* k_rope;
+  const void* v;
+  void* out;
+  const int32_t* starts;
+  const int32_t* key_starts;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, k_rope_token_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+  int32_t type, heads, requests, tokens, keys, most_tokens, nope, rope_width, value;
+  float scale;
+} llmp_latent_prompt;
+size_t llmp_hip_latent_prompt_scratch(const llmp_latent_prompt* op, int cus);
+int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratch, size_t scratch_bytes, int cus, void* stream);
+
 /* ------------------------------------------------------------ a yardstick
  * No counterpart in the reference: a launch that only reads `bytes` (whole 16-byte chunks at a 16-byte boundary),
  * eight loads in flight a lane, folded into `sink` (llmp_hip_stream_read_sink(cus) bytes, the caller's). What it

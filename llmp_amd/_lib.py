@@ -155,6 +155,53 @@ class PagedSelect(C.Structure):
                 ("recent", C.c_int32), ("before", C.c_void_p)]
 
 
+class Rope(C.Structure):
+    """llmp_rope: part of every head's channels rotated by the tokens' positions."""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("positions", C.c_void_p), ("turns", C.c_void_p), ("tokens", C.c_int64),
+                ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("type", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("first", C.c_int32), ("n_dims", C.c_int32),
+                ("interleaved", C.c_int32), ("inverse", C.c_int32), ("magnitude", C.c_float)]
+
+
+class LatentCache(C.Structure):
+    """llmp_latent_cache: a paged cache of latent vectors and rotated keys."""
+    _fields_ = [("latent", C.c_void_p), ("scale", C.c_void_p), ("rope", C.c_void_p), ("type", C.c_int32), ("pages", C.c_int32),
+                ("page", C.c_int32), ("width", C.c_int32), ("rope_width", C.c_int32)]
+
+
+class LatentStore(C.Structure):
+    """llmp_latent_store: new tokens' rows into their slots."""
+    _fields_ = [("cache", LatentCache), ("latent", C.c_void_p), ("rope", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p),
+                ("turns", C.c_void_p), ("weight", C.c_void_p), ("latent_stride", C.c_int64), ("rope_stride", C.c_int64), ("type", C.c_int32),
+                ("tokens", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float), ("magnitude", C.c_float)]
+
+
+class LatentProject(C.Structure):
+    """llmp_latent_project: every head's rows times that head's matrix."""
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("y", C.c_void_p), ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64),
+                ("w_head_stride", C.c_int64), ("w_row_stride", C.c_int64), ("y_token_stride", C.c_int64), ("y_head_stride", C.c_int64),
+                ("type", C.c_int32), ("tokens", C.c_int32), ("heads", C.c_int32), ("k", C.c_int32), ("n", C.c_int32)]
+
+
+class LatentAttend(C.Structure):
+    """llmp_latent_attend: the absorbed form over the paged latent cache."""
+    _fields_ = [("cache", LatentCache), ("q_latent", C.c_void_p), ("q_rope", C.c_void_p), ("out", C.c_void_p), ("lengths", C.c_void_p),
+                ("starts", C.c_void_p), ("table", C.c_void_p), ("before", C.c_void_p), ("q_latent_token_stride", C.c_int64),
+                ("q_latent_head_stride", C.c_int64), ("q_rope_token_stride", C.c_int64), ("q_rope_head_stride", C.c_int64),
+                ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("table_stride", C.c_int64), ("heads", C.c_int32),
+                ("requests", C.c_int32), ("tokens", C.c_int32), ("most_tokens", C.c_int32), ("table_width", C.c_int32), ("scale", C.c_float)]
+
+
+class LatentPrompt(C.Structure):
+    """llmp_latent_prompt: the expanded form over ragged requests."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("k_rope", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("starts", C.c_void_p),
+                ("key_starts", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64), ("k_token_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("k_rope_token_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("type", C.c_int32), ("heads", C.c_int32),
+                ("requests", C.c_int32), ("tokens", C.c_int32), ("keys", C.c_int32), ("most_tokens", C.c_int32), ("nope", C.c_int32),
+                ("rope_width", C.c_int32), ("value", C.c_int32), ("scale", C.c_float)]
+
+
 class VecQSource(C.Structure):
     _fields_ = [("x", C.c_void_p), ("x_type", C.c_int), ("x_token", C.c_int64),
                 ("x_slot", C.c_int64)]
@@ -192,6 +239,15 @@ SYMBOLS = {
     "llmp_hip_moe_token": (_int, [C.POINTER(MoeToken), _int, _int, _vp]),
     "llmp_hip_attn_vec_quant_scratch": (C.c_size_t, [C.POINTER(AttnVecQuant), _int]),
     "llmp_hip_attn_vec_quant": (_int, [C.POINTER(AttnVecQuant), _vp, C.c_size_t, _int, _vp]),
+    "llmp_hip_rope": (_int, [C.POINTER(Rope), _vp]),
+    "llmp_hip_rope_table": (_int, [_int, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _vp, _vp]),
+    "llmp_hip_latent_store": (_int, [C.POINTER(LatentStore), _vp]),
+    "llmp_hip_latent_read": (_int, [C.POINTER(LatentCache), _vp, _i64, _int, _vp, _vp, _vp]),
+    "llmp_hip_latent_project": (_int, [C.POINTER(LatentProject), _vp]),
+    "llmp_hip_latent_attend_scratch": (C.c_size_t, [C.POINTER(LatentAttend), _int]),
+    "llmp_hip_latent_attend": (_int, [C.POINTER(LatentAttend), _vp, C.c_size_t, _int, _vp]),
+    "llmp_hip_latent_prompt_scratch": (C.c_size_t, [C.POINTER(LatentPrompt), _int]),
+    "llmp_hip_latent_prompt": (_int, [C.POINTER(LatentPrompt), _vp, C.c_size_t, _int, _vp]),
     "llmp_hip_paged_work_items": (_i64, [_int, _int, _int]),
     "llmp_hip_paged_plan_scratch": (C.c_size_t, [_int]),
     "llmp_hip_paged_plan": (_int, [C.POINTER(PagedPlan), _vp]),

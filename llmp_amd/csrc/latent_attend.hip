@@ -1,0 +1,736 @@
+// llmp.latent.attend: the absorbed form over the paged latent cache. All heads share a token's latent vector, which is key and value, so
+// the rows of a request are its (token, head) pairs and one read of a tile serves all of them:
+//   S^T = C Q^T (latent and rotated part), P = exp2(S - E), O^T += C^T P^T, out = O / sum of P.
+//
+// What bounds it: with few heads the cache's bytes (1152 a token at 512 + 64 values against 2 * 1088 operations a row); from about 128 rows a
+// token on the matrix instructions take as long. A tile is 32 tokens, brought into LDS by loads that pass no register; the rows' queries and
+// results stay in registers. Two forms:
+//   few rows   (no request has more than 16) every wave of a workgroup's four has all rows, a ring of tiles of its own and 16 x 16 products; it
+//              waits for nobody, and the waves' results are added up at the end;
+//   many rows  a workgroup takes 128 rows of one request, 32 a wave, 32 x 32 products, all waves the same ring of tiles. A wave's results are 256 dimensions
+//              (128 registers, two waves a SIMD): at width 512 two waves share 32 rows, each with half the dimensions of both products, and
+//              add their halves of the logits through LDS. (One wave with 512 dimensions needs 256 registers of results and 144 of queries;
+//              the compiler then spilled hundreds.)
+// Both products take the tile from LDS as it lies. A product's rows are tokens in an order that leaves a lane with consecutive tokens of one row, in the
+// order in which the second product takes them; the values' columns come by transposing reads.
+//
+// All tiles of all rows lie on one line, a request's after the other's, that the workgroups cut evenly, so that one long request and many short ones fill
+// the device alike; what is cut is joined by a second launch. The line is counted in tokens, kVisit more for a (request, rows) pair's beginning.
+#include <algorithm>
+#include <cmath>
+
+#include "latent.h"
+#include "paged_attend.h"
+
+namespace llmp_hip {
+namespace {
+
+constexpr int kTokens = 32;  // a tile's
+constexpr int kFewRows = 16, kManyRows = 128;
+constexpr int kLdsBytes = 160 * 1024;
+constexpr int kVisit = 64;                         // what a pair's beginning and end cost, in tokens
+constexpr int kLeastFew = 256, kLeastMany = 128;  // of the line, to a workgroup: finer parts cost more to write and to join
+
+// The running maximum follows once it is kFollow (log2) behind; weights stay kUp above it, for F16's range.
+constexpr float kUp = 8.0f, kFollow = 6.0f;
+
+struct LatentArgs {
+  llmp_latent_attend op;
+  float* values;   // [2 * workgroups][rows][width]
+  float* numbers;  // [2 * workgroups][rows][2]: maximum, sum
+  int32_t* parts;  // [2 * workgroups][4]: request, pair, rows, first row of the call's
+  int most_length, least;
+  int tokens_a_pair, pairs_a_token;  // rows of several whole tokens, or of part of one
+};
+
+template <int R, int P, bool EIGHT, bool FEW>
+struct LatentGeo {
+  static constexpr int kSplit = FEW ? 1 : R / 256;  // waves that share rows, by dimensions
+  static constexpr int kWaves = FEW ? 4 : 4 * kSplit, kThreads = kWaves * kWave;
+  static constexpr int kRows = FEW ? kFewRows : kManyRows, kWaveRows = FEW ? 16 : 32;
+  static constexpr int kPitch = EIGHT ? R : 2 * R, kRopePitch = 2 * P;
+  static constexpr int kLatentBytes = kTokens * kPitch, kRopeBytes = kTokens * kRopePitch, kScaleBytes = EIGHT ? 256 : 0;
+  static constexpr int kTile = kLatentBytes + kRopeBytes + kScaleBytes;
+  static constexpr int kQueries = kSplit > 1 ? kManyRows * 2 * P : 0;  // the queries' rotated part, where registers are short
+  static constexpr int kExchange = kSplit > 1 ? kWaves * 4096 + kQueries : 0;
+  static constexpr int kAGroups = FEW || kSplit > 1 ? 1 : 2;  // workgroups a compute unit
+  static constexpr int kRing = FEW ? std::min(2, kLdsBytes / 4 / kTile) : std::min(5, (kLdsBytes / kAGroups - kExchange) / kTile);
+  static constexpr int kSharing = FEW ? 1 : kWaves;  // waves that bring a tile in
+  static constexpr int kAll = (kLatentBytes + kRopeBytes) / 1024 + (EIGHT ? 1 : 0);
+  static constexpr int kLoads = (kAll + kSharing - 1) / kSharing;  // a wave's for a tile
+  static constexpr int kArea = kFewRows * R * 4 + 2 * kFewRows * 4;  // the few rows' form: a wave's results for the others
+  static constexpr int kLds = FEW ? std::max(4 * kRing * kTile, 4 * kArea) : kRing * kTile + kExchange;
+  static constexpr int kWaveR = R / kSplit, kWaveP = P / kSplit;  // a wave's dimensions
+
+  // What the pieces (of 16 bytes) of a token's row are turned by: the 16 lanes that a 16-byte read takes at once (KPiece in paged_attend.h), and the 32
+  // that a transposing read does, then find theirs in all banks.
+  static __device__ __forceinline__ int Turn(int token) {
+    if constexpr (EIGHT) return (token & 7) << 1 | (token >> 3 & 1);
+    if constexpr (FEW) return (token & 3) << 2 | (0x1320 >> (4 * (token >> 3 & 3)) & 3);  // (0, 2, 3, 1)
+    return (token & 3) << 2 | (token >> 2 & 3);
+  }
+  static __device__ __forceinline__ int RopeTurn(int token) {
+    if constexpr (FEW) return P == 64 ? ((token >> 1 & 1) << 2 | (0x1320 >> (4 * (token >> 3 & 3)) & 3)) : (0x1320 >> (4 * (token >> 3 & 3)) & 3);
+    return P == 64 ? ((token >> 1 & 1) | (token >> 2 & 3) << 1) : (token >> 2 & 3);
+  }
+};
+
+// ---- a request's pairs on the line.
+struct Line {
+  int start, n, length, base;  // PagedRequest's
+  int groups;                  // of tokens_a_pair tokens
+};
+__device__ __forceinline__ Line LineOf(const LatentArgs& a, int r) {
+  const PagedRequest q = RequestOf(a.op.starts, a.op.lengths, a.op.before, r, a.op.tokens, a.most_length);
+  return {q.start, q.n, q.length, q.base, (q.n + a.tokens_a_pair - 1) / a.tokens_a_pair};
+}
+// The tokens that group k's last token sees.
+__device__ __forceinline__ int SeenOf(const LatentArgs& a, const Line& l, int k) {
+  return max(min(l.base + min((k + 1) * a.tokens_a_pair, l.n), l.length), 0);
+}
+// The line before group k: the sum of min(base + (i + 1) t, most), none below 0, over i < k, and the visits; all pairs of a group.
+__device__ __forceinline__ int64_t LengthBefore(const LatentArgs& a, const Line& l, int k) {
+  const int64_t t = a.tokens_a_pair, most = max(min(l.length, l.base + l.n), 0);
+  const int64_t low = l.base < 0 ? min(static_cast<int64_t>(k), -static_cast<int64_t>(l.base) / t) : 0;
+  const int64_t high = max(low, min(static_cast<int64_t>(k), most > l.base ? (most - l.base) / t : 0));
+  const int64_t risen = (high - low) * l.base + t * ((high * (high + 1) - low * (low + 1)) / 2);
+  return (risen + (k - high) * most + static_cast<int64_t>(k) * kVisit) * a.pairs_a_token;
+}
+
+template <int TYPE, int R, int P, bool EIGHT, bool FEW>
+__global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 : 2)) void LatentAttendKernel(const LatentArgs a) {
+  using G = LatentGeo<R, P, EIGHT, FEW>;
+  using S = Sixteen<TYPE>;
+  typedef typename S::Eight Eight;
+  typedef std::conditional_t<FEW, F32x4, F32x16> Values;  // a lane's of a block of the result
+  constexpr int kValues = FEW ? 4 : 16, kBlock = G::kWaveRows, kInner = FEW ? 32 : 16;
+  constexpr int kSteps = G::kWaveR / kInner, kRopeSteps = G::kWaveP / kInner, kBlocks = G::kWaveR / kBlock;
+  constexpr int kLogits = FEW ? 8 : 16, kWeights = kLogits / 8;  // a lane's
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const llmp_latent_attend& op = a.op;
+  const llmp_latent_cache& c = op.cache;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int half = lane / kBlock, column = lane % kBlock;  // (`half` a quarter where rows are 16)
+  const int split = G::kSplit > 1 ? wave % G::kSplit : 0;
+  const int groups = gridDim.x, w = blockIdx.x;
+  const uint32_t ring_off = FEW ? wave * G::kRing * G::kTile : 0;
+  const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + ring_off;
+
+  // ---- this workgroup's part of the line: every wave adds the requests up, a lane a request.
+  const auto wave_sums = [&](int64_t v) {  // inclusive
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      const int64_t up = __shfl_up(v, m);
+      v += lane >= m ? up : 0;
+    }
+    return v;
+  };
+  const auto last_of = [](int64_t v) {
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(v), kWave - 1);
+    return static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), kWave - 1)) << 32 | low;
+  };
+  const auto request_length = [&](int r) {
+    if (r >= op.requests) return static_cast<int64_t>(0);
+    const Line l = LineOf(a, r);
+    return LengthBefore(a, l, l.groups);
+  };
+  int64_t total = 0;
+  for (int r0 = 0; r0 < op.requests; r0 += kWave) total += last_of(wave_sums(request_length(r0 + lane)));
+  const int64_t per = max((total + groups - 1) / groups, static_cast<int64_t>(a.least));
+  int64_t u = w * per;
+  const int64_t u_end = min(u + per, total);
+  if (tid < 2) a.parts[(2 * w + tid) * 4] = -1;
+  if (u >= u_end) return;
+  int request = 0;
+  int64_t before = 0;  // the line before the request
+  for (int r0 = 0; r0 < op.requests; r0 += kWave) {
+    const int64_t mine = request_length(r0 + lane), upto = before + wave_sums(mine);
+    const int passed = __popcll(__ballot(upto <= u));
+    if (passed < kWave) {
+      const int64_t from = upto - mine;
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(from), passed);
+      before = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(from >> 32), passed)) << 32 | low;
+      request = r0 + passed;
+      break;
+    }
+    before = last_of(upto);
+  }
+
+  const float sign_scale = fabsf(op.scale) * kLog2E;
+  const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
+
+  for (; u < u_end; ++request) {
+    const Line l = LineOf(a, request);
+    const int64_t all = LengthBefore(a, l, l.groups);
+    if (u >= before + all) {
+      before += all;
+      continue;
+    }
+    // The group that holds u: the last that begins at or before it.
+    int k = 0, k_high = l.groups;
+    while (k_high - k > 1) {
+      const int mid = (k + k_high) / 2;
+      if (before + LengthBefore(a, l, mid) <= u) {
+        k = mid;
+      } else {
+        k_high = mid;
+      }
+    }
+    for (; k < l.groups && u < u_end; ++k) {
+      const int seen = SeenOf(a, l, k), whole = seen + kVisit;
+      const int64_t group_from = before + LengthBefore(a, l, k);
+      for (int part = static_cast<int>((u - group_from) / whole); part < a.pairs_a_token && u < u_end; ++part) {
+        const int64_t from = group_from + static_cast<int64_t>(part) * whole;
+        const int x0 = static_cast<int>(u - from), x1 = static_cast<int>(min(u_end - from, static_cast<int64_t>(whole)));
+        u = from + x1;
+        // Tiles whose first token lies in [x0, x1) - kVisit.
+        const int tiles = (seen + kTokens - 1) / kTokens;
+        const int tile_from = (max(x0 - kVisit, 0) + kTokens - 1) / kTokens;
+        const int tile_to = x1 == whole ? tiles : (max(x1 - kVisit, 0) + kTokens - 1) / kTokens;
+        const bool begins = tile_from == 0 && (tile_to > 0 || x0 == 0), ends = tile_to == tiles;
+        if (tiles == 0 ? x0 != 0 : tile_from >= tile_to) continue;
+
+        // ---- the lane's row.
+        const int first_token = k * a.tokens_a_pair;
+        const int row0 = FEW ? 0 : wave / G::kSplit * G::kWaveRows;
+        int rows, token, head;  // of the pair, of the lane's row
+        {
+          const int row = row0 + column;
+          if (a.pairs_a_token == 1) {
+            rows = min(a.tokens_a_pair, l.n - first_token) * op.heads;
+            token = first_token + row / op.heads;
+            head = row % op.heads;
+          } else {
+            rows = min(G::kRows, op.heads - part * G::kRows);
+            token = first_token;
+            head = part * G::kRows + row;
+          }
+        }
+        const bool real = row0 + column < rows;
+        token = real ? token : first_token;
+        head = real ? head : 0;
+        const int see_to = real ? max(min(l.base + token + 1, l.length), 0) : 0;
+        const bool busy = row0 < rows;
+        const int all_to = max(min(l.base + first_token + 1 + (a.pairs_a_token == 1 ? row0 / op.heads : 0), l.length), 0);  // seen by all of the wave's rows
+
+        constexpr bool kRopeInLds = G::kQueries > 0;
+        Eight q[kSteps + (kRopeInLds ? 0 : kRopeSteps)];
+        Eight* const q_rope = reinterpret_cast<Eight*>(lds + G::kRing * G::kTile + G::kExchange - G::kQueries) + wave * kRopeSteps * kWave;
+        {
+          const uint16_t* const ql = static_cast<const uint16_t*>(op.q_latent) + (l.start + token) * op.q_latent_token_stride + head * op.q_latent_head_stride + split * G::kWaveR + 8 * half;
+          const uint16_t* const qr = static_cast<const uint16_t*>(op.q_rope) + (l.start + token) * op.q_rope_token_stride + head * op.q_rope_head_stride + split * G::kWaveP + 8 * half;
+#pragma unroll
+          for (int x = 0; x < kSteps + kRopeSteps; ++x) {
+            U32x4 v = *reinterpret_cast<const U32x4*>(x < kSteps ? ql + kInner * x : qr + kInner * (x - kSteps));
+            v ^= U32x4{flip, flip, flip, flip};
+            if (kRopeInLds && x >= kSteps) {
+              q_rope[(x - kSteps) * kWave + lane] = __builtin_bit_cast(Eight, v);
+            } else {
+              q[x] = __builtin_bit_cast(Eight, v);
+            }
+          }
+        }
+        Values out[kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int i = 0; i < kValues; ++i) out[b][i] = 0.0f;
+        }
+        float top = -INFINITY, sum = 0.0f;
+
+        // ---- the tiles. A lane holds the cache's row of the first token of one 16-token group of the line (-1: no page); they are looked up 64
+        // at a time.
+        const int32_t* const table = op.table + request * op.table_stride;
+        int held_from = -1, held = 0;
+        const auto look_up = [&](int tile) {
+          held_from = tile;
+          const uint32_t position = static_cast<uint32_t>(2 * tile + lane) * 16u, entry = position / static_cast<uint32_t>(c.page);
+          held = -1;
+          if (position < static_cast<uint32_t>(seen) && entry < static_cast<uint32_t>(op.table_width)) {
+            const int page = table[entry];
+            if (page >= 0 && page < c.pages) held = page * c.page + static_cast<int>(position - entry * c.page);
+          }
+        };
+        const int step = FEW ? G::kWaves : 1;
+        const int my_from = tile_from + (FEW ? wave : 0);
+        uint32_t absent = 0;  // two bits a slot of the ring: the tile's groups without a page
+        const auto fetch = [&](int tile, int slot) {
+          if (held_from < 0 || tile >= held_from + 32) look_up(tile);
+          const int at0 = __builtin_amdgcn_readlane(held, 2 * (tile - held_from)), at1 = __builtin_amdgcn_readlane(held, 2 * (tile - held_from) + 1);
+          absent = (absent & ~(3u << (2 * slot))) | ((at0 < 0 ? 1u : 0u) | (at1 < 0 ? 2u : 0u)) << (2 * slot);
+          const int left = seen - tile * kTokens;  // tokens of the tile, at least one; past them the last one again
+          const int row_a = max(at0, 0), row_b = left > 16 ? max(at1, 0) : row_a;
+          const int last_a = min(left - 1, 15), last_b = left > 16 ? min(left - 17, 15) : last_a;
+          const uint8_t* const latent_a = static_cast<const uint8_t*>(c.latent) + static_cast<int64_t>(row_a) * G::kPitch;
+          const uint8_t* const latent_b = static_cast<const uint8_t*>(c.latent) + static_cast<int64_t>(row_b) * G::kPitch;
+          const uint8_t* const rope_a = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_a) * G::kRopePitch;
+          const uint8_t* const rope_b = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_b) * G::kRopePitch;
+          const uint32_t to = ring_at + slot * G::kTile;
+          // (Lanes and waves as something new at every tile: the compiler otherwise keeps every load's offsets, and then spills them.)
+          int lane_now = lane, wave_now = wave;
+          asm volatile("" : "+v"(lane_now), "+s"(wave_now));
+          const auto load = [&](auto whole) {
+#pragma unroll
+            for (int i = 0; i < G::kLoads; ++i) {
+              const int n = FEW ? i : (i * G::kWaves + wave_now) % G::kAll;  // (the last ones again where they do not go round)
+              if (n < G::kLatentBytes / 1024) {
+                constexpr int kLanes = G::kPitch / 16, kRowsALoad = kWave / kLanes;
+                const int row0 = n * kRowsALoad, row = row0 + lane_now / kLanes;
+                const bool second = row0 >= 16;
+                const uint32_t piece = 16 * ((lane_now % kLanes) ^ G::Turn(row));
+                if constexpr (decltype(whole)::value) {
+                  LineToLds((second ? latent_b : latent_a) + (row0 & 15) * G::kPitch, lane_now / kLanes * G::kPitch + piece, to + 1024 * n);
+                } else {
+                  LineToLds(second ? latent_b : latent_a, min(row & 15, second ? last_b : last_a) * G::kPitch + piece, to + 1024 * n);
+                }
+              } else if (n < (G::kLatentBytes + G::kRopeBytes) / 1024) {
+                constexpr int kLanes = G::kRopePitch / 16, kRowsALoad = kWave / kLanes;
+                const int row0 = (n - G::kLatentBytes / 1024) * kRowsALoad, row = row0 + lane_now / kLanes;
+                const bool second = row0 >= 16;
+                const uint32_t piece = 16 * ((lane_now % kLanes) ^ G::RopeTurn(row));
+                LineToLds(second ? rope_b : rope_a, (decltype(whole)::value ? row & 15 : min(row & 15, second ? last_b : last_a)) * G::kRopePitch + piece, to + 1024 * n);
+              } else {  // the scales: four tokens a lane, eight lanes of them
+                WordToLds(c.scale, (lane_now & 4 ? row_b : row_a) + 4 * (lane_now & 3), to + G::kLatentBytes + G::kRopeBytes);
+              }
+            }
+          };
+          if (left >= kTokens) {
+            load(std::true_type{});
+          } else {
+            load(std::false_type{});
+          }
+        };
+
+        // What a lane reads of a tile. Rows are whole 256 bytes, so that a place is the lane's own (its row, its piece turned) with a constant's bits turned
+        // in and a constant added. Keys: row m of a product is token 16 (m / 4 % 2) + 4 (m / 8) + m % 4, where products are of 16 rows (the `m_block`-th) 8 (m / 4) +
+        // 4 m_block + m % 4. Values: a column's lanes name their rows, of four tokens (eight where they are bytes).
+        // (Worked out at every tile, from a lane number as something new: kept, they were the registers too many.)
+        struct Places {
+          uint32_t key, rope, value;
+        };
+        const auto places = [&]() {
+          int l = lane;
+          if constexpr (!FEW) asm volatile("" : "+v"(l));
+          const int half = l / kBlock, column = l % kBlock;
+          const int k_token = FEW ? 8 * (column >> 2) + (column & 3) : 16 * (column >> 2 & 1) + 4 * (column >> 3) + (column & 3);
+          const int i16 = l & 15, block16 = FEW ? 0 : l >> 4 & 1;
+          const int v_token = (FEW ? 8 : 16) * half + (EIGHT ? i16 >> 1 : i16 >> 2);
+          Places p;
+          p.key = k_token * G::kPitch + (EIGHT ? 16 * (G::Turn(k_token) ^ (FEW ? half >> 1 : 0)) + 8 * (half & 1) : 16 * (G::Turn(k_token) ^ half)) +
+                  split * (G::kPitch / G::kSplit);
+          p.rope = G::kLatentBytes + k_token * G::kRopePitch + 16 * (G::RopeTurn(k_token) ^ (half + split * (G::kWaveP / 8)));
+          p.value = v_token * G::kPitch + (EIGHT ? 16 * (block16 ^ G::Turn(v_token)) : 16 * ((2 * block16 + (i16 >> 1 & 1)) ^ G::Turn(v_token))) + 8 * (i16 & 1) +
+                    split * (G::kPitch / G::kSplit);
+          return p;
+        };
+        // Constants of a place: Turn of tokens + 4 m_block (keys of 16-row products), + 8 s and + 4 of it (values).
+        const auto key = [&](uint32_t at, uint32_t rope_at, int x, int m_block) {
+          constexpr int kPieces = EIGHT ? kInner / 16 : kInner / 8;
+          if (x >= kSteps) return *reinterpret_cast<const Eight*>(lds + (rope_at ^ 16 * (kInner / 8 * (x - kSteps))) + 4 * m_block * G::kRopePitch);
+          const uint32_t place = (at ^ 16 * ((kPieces * x & 15) ^ (EIGHT && FEW ? 8 * m_block : 0))) + 256 * (kPieces * x >> 4) + 4 * m_block * G::kPitch;
+          if constexpr (EIGHT) {
+            const uint2 v = *reinterpret_cast<const uint2*>(lds + place);
+            return EightE4m3<TYPE>(v.x, v.y);
+          } else {
+            return *reinterpret_cast<const Eight*>(lds + place);
+          }
+        };
+        // Tokens 16 half + 8 s to + 7 (8 half to + 7) of dimension kBlock b + column.
+        const auto value = [&](uint32_t at, int b, int s) {
+          constexpr int kPieces = EIGHT ? kBlock / 16 : kBlock / 8;
+          const int x = kPieces * b;
+          if constexpr (EIGHT) {
+            const I32x2 v = Column8(lds + (at ^ 16 * ((x & 15) ^ s)) + 256 * (x >> 4) + 8 * s * G::kPitch);
+            return EightE4m3<TYPE>(v.x, v.y);
+          } else {
+            constexpr int kTurnOf4 = FEW ? 0 : 1;
+            const S16x4 v = Column4(lds + (at ^ 16 * ((x & 15) ^ 2 * s)) + 256 * (x >> 4) + 8 * s * G::kPitch);
+            return JoinFours<Eight>(v, Column4(lds + (at ^ 16 * ((x & 15) ^ 2 * s ^ kTurnOf4)) + 256 * (x >> 4) + (8 * s + 4) * G::kPitch));
+          }
+        };
+        float* const exchange = reinterpret_cast<float*>(lds + G::kRing * G::kTile);
+
+        // A tile's logits of a wave's rows over its dimensions: element i is token 16 half + i (8 half + i).
+        float dots[kLogits], scale8[kLogits];
+        const auto keys = [&](uint32_t tile) {
+          const Places p = places();
+          const uint32_t key_at = tile + p.key, rope_at = tile + p.rope;
+          Values sums[kLogits / kValues];
+#pragma unroll
+          for (int m = 0; m < kLogits / kValues; ++m) {
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) sums[m][i] = 0.0f;
+          }
+          const auto steps = [&](int from, int to) {
+#pragma unroll
+            for (int x = from; x < to; ++x) {
+              const Eight query = kRopeInLds && x >= kSteps ? q_rope[(x - kSteps) * kWave + lane] : q[kRopeInLds && x >= kSteps ? 0 : x];
+#pragma unroll
+              for (int m = 0; m < kLogits / kValues; ++m) {
+                if constexpr (FEW) sums[m] = S::Product16(key(key_at, rope_at, x, m), query, sums[m]);
+                if constexpr (!FEW) sums[m] = S::Product32(key(key_at, rope_at, x, m), query, sums[m]);
+              }
+            }
+          };
+          if constexpr (EIGHT) {
+            // Codes' products first: their scale is the token's, the rotated part's is one.
+            steps(0, kSteps);
+            uint32_t e[kLogits / 4];
+            const uint32_t scales_at = tile + G::kLatentBytes + G::kRopeBytes + kLogits * half;
+#pragma unroll
+            for (int i = 0; i < kLogits / 4; ++i) e[i] = *reinterpret_cast<const uint32_t*>(lds + scales_at + 4 * i);
+#pragma unroll
+            for (int i = 0; i < kLogits; ++i) {
+              const uint32_t bits = e[i / 4] >> (8 * (i & 3)) & 0xFFu;
+              scale8[i] = __builtin_bit_cast(float, bits == 0 ? 0x00400000u : bits << 23);
+              sums[i / kValues][i % kValues] *= scale8[i];
+            }
+            steps(kSteps, kSteps + kRopeSteps);
+          } else {
+            steps(0, kSteps + kRopeSteps);
+          }
+#pragma unroll
+          for (int i = 0; i < kLogits; ++i) dots[i] = sums[i / kValues][i % kValues];
+        };
+        const auto give = [&]() {
+#pragma unroll
+          for (int i = 0; i < kLogits / 4; ++i)
+            reinterpret_cast<F32x4*>(exchange)[(wave * (kLogits / 4) + i) * kWave + lane] = F32x4{dots[4 * i], dots[4 * i + 1], dots[4 * i + 2], dots[4 * i + 3]};
+        };
+        const auto take = [&]() {
+#pragma unroll
+          for (int i = 0; i < kLogits / 4; ++i) {
+            const F32x4 v = reinterpret_cast<const F32x4*>(exchange)[((wave ^ 1) * (kLogits / 4) + i) * kWave + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dots[4 * i + e] += v[e];
+          }
+        };
+
+        const auto values = [&](int tile_number, uint32_t tile, uint32_t gone) {
+          const uint32_t value_at = tile + places().value;
+          // ---- what the rows see
+          const int p0 = tile_number * kTokens, lane_token = kLogits * half;
+          bool garbage = false;
+#pragma unroll
+          for (int i = 0; i < kLogits; ++i) dots[i] *= sign_scale;
+          if (p0 + kTokens > all_to || gone != 0) {
+            asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
+            const int to = (gone >> (lane_token >> 4) & 1) != 0 ? 0 : see_to - p0 - lane_token;
+#pragma unroll
+            for (int i = 0; i < kLogits; ++i) {
+              // (A value that is no number, or one that a product with zero would make none, has no finite product with any query.)
+              garbage = garbage || (i >= to && !(fabsf(dots[i]) < INFINITY));
+              dots[i] = i < to ? dots[i] : -INFINITY;
+              if constexpr (EIGHT) scale8[i] = i < to ? scale8[i] : 0.0f;
+            }
+          }
+          // ---- softmax. Eight-bit weights take the token's scale along; the maximum is of both.
+          float peak = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kLogits; ++i) {
+            peak = fmaxf(peak, EIGHT ? dots[i] + __builtin_amdgcn_logf(fmaxf(scale8[i], 0x1p-80f)) : dots[i]);
+          }
+          peak = Across<kBlock>(peak);
+          if (__any(peak > top + (kUp + kFollow))) {
+            const float higher = fmaxf(top, peak - kUp);
+            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+            top = higher;
+            sum *= keep;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
+          }
+          const float less = top == -INFINITY ? 0.0f : top;
+          Eight weights[kWeights];
+#pragma unroll
+          for (int i = 0; i < kLogits; ++i) {
+            const float p = __builtin_amdgcn_exp2f(dots[i] - less);
+            sum += p;
+            weights[i / 8][i % 8] = static_cast<typename S::One>(EIGHT ? p * scale8[i] : p);
+          }
+          const auto product = [](Eight x, Eight y, Values z) {
+            if constexpr (FEW) return S::Product16(x, y, z);
+            if constexpr (!FEW) return S::Product32(x, y, z);
+          };
+          if (__any(garbage)) {
+            // A token that some row must not see holds infinities or NaN, which a weight of zero does not keep out: they become zeros in LDS. (A row that
+            // sees them has no finite logit there, and no finite sum. Nobody reads the tile as keys any more.)
+#pragma unroll 1
+            for (uint32_t i = 16 * lane; i < G::kLatentBytes; i += 1024) {
+              U32x4* const at = reinterpret_cast<U32x4*>(lds + tile + i);
+              *at = EIGHT ? FiniteCodes(*at) : Finite<TYPE>(*at);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+            for (int s = 0; s < kWeights; ++s) out[b] = product(value(value_at, b, s), weights[s], out[b]);
+          }
+        };
+
+        if constexpr (FEW) {
+          // A wave's own ring: nobody waits for anybody.
+          const int count = tile_to > my_from ? (tile_to - my_from + step - 1) / step : 0;
+          for (int i = 0; i < G::kRing && i < count; ++i) fetch(my_from + i * step, i);
+          for (int i = 0; i < count; ++i) {
+            if (G::kRing == 2 && i + 1 < count) {
+              WaitLoads<G::kLoads>();
+            } else {
+              WaitLoads<0>();
+            }
+            const int tile = my_from + i * step;
+            keys(ring_off + i % G::kRing * G::kTile);
+            values(tile, ring_off + i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (i + G::kRing < count) fetch(my_from + (i + G::kRing) * step, i % G::kRing);
+          }
+        } else {
+          const int count = tile_to - tile_from;
+          constexpr int kAhead = G::kRing - 1;
+          for (int i = 0; i < kAhead && i < count; ++i) fetch(tile_from + i, i);
+          for (int i = 0; i < count; ++i) {
+            // Tile i has landed: of the tiles asked for only later ones are under way.
+            const int later = min(kAhead - 1, count - 1 - i);
+            if (later >= 3) {
+              WaitLoads<3 * G::kLoads>();
+            } else if (later == 2) {
+              WaitLoads<2 * G::kLoads>();
+            } else if (later == 1) {
+              WaitLoads<G::kLoads>();
+            } else {
+              WaitLoads<0>();
+            }
+            MeetLds();
+            if (i + kAhead < count) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
+            if (busy) keys(i % G::kRing * G::kTile);
+            if constexpr (G::kSplit > 1) {
+              if (busy) give();
+            }
+            MeetLds();
+            if constexpr (G::kSplit > 1) {
+              if (busy) take();
+            }
+            if (busy) values(tile_from + i, i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u);
+          }
+          MeetLds();
+        }
+        sum = AcrossSum<kBlock>(sum);
+
+        // ---- the few rows' form: the waves' results added up, a quarter of the dimensions each.
+        constexpr int kMine = FEW ? kBlocks / 4 : kBlocks;  // blocks that the wave writes
+        const int first_block = FEW ? wave * kMine : split * kBlocks;
+        Values result[kMine];
+        if constexpr (FEW) {
+          MeetLds();
+          uint8_t* const area = lds + wave * G::kArea;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) reinterpret_cast<F32x4*>(area)[b * kWave + lane] = out[b];
+          if (half == 0) reinterpret_cast<float2*>(area + kFewRows * R * 4)[column] = make_float2(top, sum);
+          MeetLds();
+          float2 numbers[4];
+          top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) numbers[i] = reinterpret_cast<const float2*>(lds + i * G::kArea + kFewRows * R * 4)[column], top = fmaxf(top, numbers[i].x);
+          sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            numbers[i].x = __builtin_amdgcn_exp2f(numbers[i].x - (top == -INFINITY ? 0.0f : top));
+            sum = fmaf(numbers[i].x, numbers[i].y, sum);
+          }
+#pragma unroll
+          for (int b = 0; b < kMine; ++b) {
+            result[b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) result[b] += reinterpret_cast<const F32x4*>(lds + i * G::kArea)[(first_block + b) * kWave + lane] * numbers[i].x;
+          }
+          MeetLds();
+        } else {
+#pragma unroll
+          for (int b = 0; b < kMine; ++b) result[b] = out[b];
+        }
+
+        // ---- out, or a part for the join. Element 4i + e of a block is dimension 8i + 4 half + e of it.
+        const int first_dimension = first_block * kBlock + 4 * half;
+        if (begins && ends) {
+          if (busy && real) {
+            const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            const int64_t to = (l.start + token) * op.out_token_stride + head * op.out_head_stride + first_dimension;
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+#pragma unroll
+              for (int i = 0; i < kValues / 4; ++i) {
+                const float v[4] = {result[b][4 * i] * by, result[b][4 * i + 1] * by, result[b][4 * i + 2] * by, result[b][4 * i + 3] * by};
+                StoreValues<TYPE, 4>(op.out, to + kBlock * b + 8 * i, v);
+              }
+            }
+          }
+        } else {
+          const int which = 2 * w + (begins ? 1 : 0);
+          if (tid == 0) {
+            int32_t* const p = a.parts + 4 * which;
+            p[0] = request, p[1] = k * a.pairs_a_token + part, p[2] = rows, p[3] = l.start + first_token;
+          }
+          if (busy) {
+            const int64_t row = static_cast<int64_t>(which) * G::kRows + row0 + column;
+            if (half == 0) reinterpret_cast<float2*>(a.numbers)[row] = make_float2(top, sum);
+            float* const to = a.values + row * R + first_dimension;
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+#pragma unroll
+              for (int i = 0; i < kValues / 4; ++i)
+                *reinterpret_cast<F32x4*>(to + kBlock * b + 8 * i) = F32x4{result[b][4 * i], result[b][4 * i + 1], result[b][4 * i + 2], result[b][4 * i + 3]};
+            }
+          }
+        }
+      }
+    }
+    before += all;
+  }
+}
+
+// The parts of a pair, joined: a wave a row, eight (four) values a lane. grid (workgroups of the first launch, rows / 4).
+template <int TYPE, int R>
+__global__ __launch_bounds__(256) void LatentJoinKernel(const LatentArgs a, int part_rows, int groups) {
+  constexpr int kValues = R / kWave;
+  const llmp_latent_attend& op = a.op;
+  const int lane = threadIdx.x & (kWave - 1), row = blockIdx.y * 4 + threadIdx.x / kWave;
+  const int first = 2 * blockIdx.x + 1;
+  const int32_t* const p = a.parts + 4 * first;
+  const int request = p[0], pair = p[1], rows = p[2], token0 = p[3];
+  if (request < 0 || row >= rows) return;
+  // The parts after the first are the next workgroups' first ones, as long as they are of this pair.
+  int count = 1;
+  for (int base = blockIdx.x + 1;; base += kWave) {
+    const int g = base + lane;
+    const bool same = g < groups && a.parts[8 * g] == request && a.parts[8 * g + 1] == pair;
+    const uint64_t not_same = ~__ballot(same);
+    const int here = not_same == 0 ? kWave : __ffsll(static_cast<unsigned long long>(not_same)) - 1;
+    count += here;
+    if (here < kWave) break;
+  }
+  const auto part_row = [&](int i) { return static_cast<int64_t>(i == 0 ? first : 2 * (static_cast<int>(blockIdx.x) + i)) * part_rows + row; };
+  float most = -INFINITY;
+  for (int i = lane; i < count; i += kWave) most = fmaxf(most, a.numbers[2 * part_row(i)]);
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+  const float less = most == -INFINITY ? 0.0f : most;
+  float sum = 0.0f, v[kValues];
+#pragma unroll
+  for (int e = 0; e < kValues; ++e) v[e] = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const int64_t at = part_row(i);
+    const float2 n = reinterpret_cast<const float2*>(a.numbers)[at];
+    const float by = __builtin_amdgcn_exp2f(n.x - less);
+    sum = fmaf(n.y, by, sum);
+    const F32x4* const from = reinterpret_cast<const F32x4*>(a.values + at * R + kValues * lane);
+#pragma unroll
+    for (int e = 0; e < kValues / 4; ++e) {
+      const F32x4 x = from[e];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) v[4 * e + f] = fmaf(x[f], by, v[4 * e + f]);
+    }
+  }
+  const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int e = 0; e < kValues; ++e) v[e] *= by;
+  const int token = token0 + (a.pairs_a_token == 1 ? row / op.heads : 0);
+  const int head = a.pairs_a_token == 1 ? row % op.heads : pair % a.pairs_a_token * part_rows + row;
+  StoreValues<TYPE, kValues>(op.out, token * op.out_token_stride + head * op.out_head_stride + kValues * lane, v);
+}
+
+// f with the type, width, rope width, 8 bits or not and the form as constants.
+template <class F>
+void WithForm(const llmp_latent_attend& op, bool few, F&& f) {
+  const auto form = [&](auto type, auto r, auto p) {
+    const bool eight = op.cache.scale != nullptr;
+    if (eight && few) f(type, r, p, std::true_type{}, std::true_type{});
+    if (eight && !few) f(type, r, p, std::true_type{}, std::false_type{});
+    if (!eight && few) f(type, r, p, std::false_type{}, std::true_type{});
+    if (!eight && !few) f(type, r, p, std::false_type{}, std::false_type{});
+  };
+  const auto widths = [&](auto type) {
+    const auto rope = [&](auto r) {
+      if (op.cache.rope_width == 32) form(type, r, std::integral_constant<int, 32>{});
+      if (op.cache.rope_width == 64) form(type, r, std::integral_constant<int, 64>{});
+    };
+    if (op.cache.width == 256) rope(std::integral_constant<int, 256>{});
+    if (op.cache.width == 512) rope(std::integral_constant<int, 512>{});
+  };
+  if (op.cache.type == LLMP_X_BF16) widths(std::integral_constant<int, LLMP_X_BF16>{});
+  if (op.cache.type == LLMP_X_F16) widths(std::integral_constant<int, LLMP_X_F16>{});
+}
+
+bool FewRows(const llmp_latent_attend& op) { return static_cast<int64_t>(std::min(op.most_tokens, op.tokens)) * op.heads <= kFewRows; }
+int RowsOf(const llmp_latent_attend& op) { return FewRows(op) ? kFewRows : kManyRows; }
+
+int CheckLatentAttend(const llmp_latent_attend* op, int cus) {
+  if (op == nullptr) return Refuse(1, "latent_attend: null operands");
+  if (const int bad = CheckLatentCache("latent_attend", op->cache); bad != 0) return bad;
+  if (op->heads < 1 || op->requests < 1 || op->requests > 1 << 24 || op->tokens < 1 || op->most_tokens < 1 || op->table_width < 1 ||
+      static_cast<int64_t>(op->heads) * op->tokens > INT_MAX / 2 || op->heads > 65535)
+    return Refuse(1, "latent_attend: 1 to 2^24 requests, at least one token and one page a table row, at most 65535 heads and 2^30 of them in all tokens (%d, %d, %d, %d, %d)",
+                  op->requests, op->tokens, op->most_tokens, op->table_width, op->heads);
+  const int type = op->cache.type;
+  if (const int bad = CheckPagedRows("latent_attend", "q_latent", op->q_latent, op->tokens, op->heads, op->q_latent_token_stride, op->q_latent_head_stride, type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("latent_attend", "q_rope", op->q_rope, op->tokens, op->heads, op->q_rope_token_stride, op->q_rope_head_stride, type); bad != 0) return bad;
+  if (const int bad = CheckPagedRows("latent_attend", "out", op->out, op->tokens, op->heads, op->out_token_stride, op->out_head_stride, type); bad != 0) return bad;
+  if (op->lengths == nullptr || op->starts == nullptr || op->table == nullptr) return Refuse(1, "latent_attend: null operand");
+  if ((reinterpret_cast<uintptr_t>(op->lengths) | reinterpret_cast<uintptr_t>(op->starts) | reinterpret_cast<uintptr_t>(op->table) |
+       reinterpret_cast<uintptr_t>(op->before)) % 4 != 0)
+    return Refuse(1, "latent_attend: I32 arrays at 4-byte boundaries");
+  if (op->requests > 1 && op->table_stride < op->table_width)
+    return Refuse(1, "latent_attend: a table row of %d entries every %lld", op->table_width, (long long)op->table_stride);
+  if (static_cast<int64_t>(op->table_width) * op->cache.page > kMostPagedLength) return Refuse(1, "latent_attend: a table row of at most 2^30 tokens");
+  if (!std::isfinite(op->scale)) return Refuse(1, "latent_attend: a scale that is not finite");
+  if (cus < 1 || cus > 4096) return Refuse(1, "latent_attend: %d compute units", cus);
+  return 0;
+}
+
+int Groups(const llmp_latent_attend& op, int cus) { return !FewRows(op) && op.cache.width == 256 ? 2 * cus : cus; }
+size_t PartsBytes(int groups) { return static_cast<size_t>(2 * groups) * 16; }
+
+}  // namespace
+}  // namespace llmp_hip
+
+using namespace llmp_hip;
+
+extern "C" size_t llmp_hip_latent_attend_scratch(const llmp_latent_attend* op, int cus) {
+  if (CheckLatentAttend(op, cus) != 0) return 0;
+  const int groups = Groups(*op, cus);
+  const size_t rows = static_cast<size_t>(2 * groups) * RowsOf(*op);
+  return PartsBytes(groups) + rows * 8 + rows * op->cache.width * 4;
+}
+
+extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream) {
+  if (const int bad = CheckLatentAttend(op, cus); bad != 0) return bad;
+  const size_t need = llmp_hip_latent_attend_scratch(op, cus);
+  if (scratch == nullptr || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
+    return Refuse(1, "latent_attend: %zu bytes of scratch at a 16-byte boundary, not %zu", need, scratch_bytes);
+  const bool few = FewRows(*op);
+  const int rows = RowsOf(*op);
+  // (Workgroups: as many as the compute units hold at once.)
+  const int groups = Groups(*op, cus);
+  LatentArgs a;
+  a.op = *op;
+  a.parts = static_cast<int32_t*>(scratch);
+  a.numbers = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + PartsBytes(groups));
+  a.values = a.numbers + static_cast<size_t>(2 * groups) * rows * 2;
+  a.most_length = op->table_width * op->cache.page;
+  a.least = few ? kLeastFew : kLeastMany;
+  a.tokens_a_pair = std::max(1, rows / op->heads);
+  a.pairs_a_token = (op->heads + rows - 1) / rows;
+  BeginLaunches();
+  const auto s = static_cast<hipStream_t>(stream);
+  WithForm(*op, few, [&](auto type, auto r, auto p, auto eight, auto few_rows) {
+    constexpr int kType = decltype(type)::value, kR = decltype(r)::value, kP = decltype(p)::value;
+    constexpr bool kEight = decltype(eight)::value, kFew = decltype(few_rows)::value;
+    using G = LatentGeo<kR, kP, kEight, kFew>;
+    static_assert(G::kRing >= (kFew ? 1 : 3) && G::kLds <= kLdsBytes, "a ring of tiles");
+    constexpr int kLds = G::kLds;
+    static bool sized = false;
+    if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kFew>), kLds, &sized)) return;
+    hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(groups), dim3(G::kThreads), kLds, s, a);
+    hipLaunchKernelGGL((LatentJoinKernel<kType, kR>), dim3(groups, (rows + 3) / 4), dim3(256), 0, s, a, rows, groups);
+  });
+  return LaunchStatus("latent_attend");
+}

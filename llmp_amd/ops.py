@@ -4,6 +4,7 @@ lib/libllmp_hip.so and only queues work, as the reference's Run* operators do
 (src/kernels/ggml/vecq.cu:1095-1175)."""
 import ctypes as C
 import functools
+import math
 
 import torch
 
@@ -845,4 +846,193 @@ def paged_select(cache, q, table, lengths, starts, keep, *, before=None, first=1
     if scratch is None:
         scratch = torch.empty(max(lib.llmp_hip_paged_select_scratch(at), 16), dtype=torch.uint8, device=q.device)
     _lib.check(lib.llmp_hip_paged_select(at, scratch.data_ptr(), scratch.numel(), _stream()))
+    return out
+
+
+def rope_table(n_dims, base=10000.0, *, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, corr_dims=(0.0, 0.0), freq_factors=None, device="cuda"):
+    """The angles of rope and latent_store, made once for a model: a dict of turns (int64 [n_dims / 2]: the bits of a 64-bit fraction of a turn a
+    position; base^(-2p / n_dims) / freq_factors[p], scaled or mixed as rope_set_rows_quant has it) and magnitude, what cosine and sine are
+    scaled by (attn_factor, times 1 + 0.1 ln(1 / freq_scale) where ext_factor is not zero). freq_factors: n_dims / 2 numbers."""
+    lib = _lib.load()
+    turns = torch.empty(n_dims // 2, dtype=torch.int64)
+    factors = None if freq_factors is None else torch.as_tensor(freq_factors, dtype=torch.float32).cpu().contiguous()
+    assert factors is None or factors.shape == turns.shape
+    _lib.check(lib.llmp_hip_rope_table(n_dims, base, freq_scale, ext_factor, corr_dims[0], corr_dims[1], _ptr(factors), turns.data_ptr()))
+    magnitude = attn_factor * (1.0 + 0.1 * math.log(1.0 / freq_scale)) if ext_factor != 0.0 else attn_factor
+    return {"turns": turns.to(device), "magnitude": magnitude}
+
+
+def _turns(table):
+    turns = table["turns"]
+    assert turns.is_cuda and turns.dtype is torch.int64 and turns.dim() == 1 and turns.is_contiguous()
+    return turns
+
+
+_INTERLEAVED = {"half": 0, "interleaved": 1}
+
+
+def _here(*tensors):
+    """On the current device: its stream is the one that the launch goes to."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        assert t.is_cuda and t.get_device() == device, "tensors on the current device"
+
+
+def rope(x, positions, table, *, layout="half", first=0, inverse=False, out=None):
+    """llmp.rope: x (float32, bfloat16 or float16 [tokens, heads, head_dim]) with the channels first to first + n_dims - 1 of every head (n_dims:
+    the rope_table's) rotated at int32 positions [tokens]: channel c with c + n_dims / 2 ("half") or 2p with 2p + 1 ("interleaved"). `inverse`:
+    by the negative angles, which is also the gradient's way back. `out` may be x itself."""
+    lib = _lib.load()
+    turns = _turns(table)
+    tokens, heads, head_dim = x.shape
+    if out is None:
+        out = torch.empty((tokens, heads, head_dim), dtype=x.dtype, device=x.device)
+    assert out.shape == x.shape and out.dtype is x.dtype and positions.dtype is torch.int32 and positions.shape == (tokens,)
+    assert positions.stride(0) == 1 or tokens < 2
+    (xt, xh, xd), (ot, oh, od) = x.stride(), out.stride()
+    assert (xd == od == 1) or head_dim == 1
+    _here(x, out, positions, turns)
+    op = _lib.Rope(x.data_ptr(), out.data_ptr(), positions.data_ptr(), turns.data_ptr(), tokens, xt, xh, ot, oh, _X_TYPES[x.dtype], heads, head_dim,
+                   first, 2 * turns.shape[0], _INTERLEAVED[layout], int(inverse), table["magnitude"])
+    _lib.check(lib.llmp_hip_rope(C.byref(op), _stream()))
+    return out
+
+
+def latent_cache(pages, page, width, rope, dtype=torch.bfloat16, bits=16, device="cuda"):
+    """An empty paged cache of latent vectors (include/llmp_hip.h, llmp_latent_cache) as a dict of tensors: latent [pages, page, width] of
+    `dtype` (bfloat16 or float16), or with bits=8 uint8 E4M3 codes and scale uint8 [pages, page]; rope [pages, page, rope] of `dtype`."""
+    assert bits in (8, 16)
+    cache = {"latent": torch.zeros((pages, page, width), dtype=torch.uint8 if bits == 8 else dtype, device=device),
+             "rope": torch.zeros((pages, page, rope), dtype=dtype, device=device)}
+    if bits == 8:
+        cache["scale"] = torch.zeros((pages, page), dtype=torch.uint8, device=device)
+    return cache
+
+
+def _latent_cache(cache):
+    latent, rope, scale = cache["latent"], cache["rope"], cache.get("scale")
+    pages, page, width = latent.shape
+    whole = (latent.is_contiguous() and rope.is_contiguous() and rope.dim() == 3 and rope.shape[:2] == (pages, page)
+             and latent.dtype is (rope.dtype if scale is None else torch.uint8)
+             and (scale is None or (scale.dtype is torch.uint8 and scale.is_contiguous() and scale.shape == (pages, page))))
+    assert whole, "the cache's arrays are whole, of one set of sizes"
+    _here(latent, rope, *(() if scale is None else (scale,)))
+    return _lib.LatentCache(latent.data_ptr(), _ptr(scale), rope.data_ptr(), _X_TYPES[rope.dtype], pages, page, width, rope.shape[2])
+
+
+def latent_store(cache, latent, rope, slots, positions=None, table=None, *, layout="interleaved", weight=None, eps=1e-6):
+    """llmp.latent.store: rows latent [tokens, width] and rope [tokens, rope] (float32, bfloat16 or float16) into the cache's `slots` (int32 [tokens],
+    paged_plan's; outside the cache: skipped). With `weight` (float32 [width]) the latent rows are normalised by their root mean square first; with
+    `table` (rope_table's) the keys are rotated at int32 `positions`. The cache is updated in place."""
+    lib = _lib.load()
+    c = _latent_cache(cache)
+    tokens = latent.shape[0]
+    assert latent.shape == (tokens, c.width) and rope.shape == (tokens, c.rope_width) and latent.dtype is rope.dtype
+    assert latent.stride(1) == rope.stride(1) == 1 and slots.dtype is torch.int32 and slots.shape == (tokens,) and slots.is_contiguous()
+    _here(latent, rope, slots)
+    at_positions = at_turns = None
+    if table is not None:
+        turns = _turns(table)
+        assert turns.shape[0] * 2 == c.rope_width and positions.dtype is torch.int32 and positions.shape == (tokens,) and positions.is_contiguous()
+        _here(turns, positions)
+        at_positions, at_turns = positions.data_ptr(), turns.data_ptr()
+    if weight is not None:
+        assert weight.dtype is torch.float32 and weight.shape == (c.width,) and weight.is_contiguous()
+        _here(weight)
+    op = _lib.LatentStore(c, latent.data_ptr(), rope.data_ptr(), slots.data_ptr(), at_positions, at_turns, _ptr(weight), latent.stride(0), rope.stride(0),
+                          _X_TYPES[latent.dtype], tokens, _INTERLEAVED[layout], eps, table["magnitude"] if table is not None else 1.0)
+    _lib.check(lib.llmp_hip_latent_store(C.byref(op), _stream()))
+
+
+def latent_read(cache, slots, dtype=None):
+    """llmp.latent.read: the cache's rows at `slots` (int32 [n]; outside the cache: zeros) as values of `dtype` (the cache's): latent [n, width] and
+    rope [n, rope]."""
+    lib = _lib.load()
+    c = _latent_cache(cache)
+    assert slots.dtype is torch.int32 and slots.dim() == 1 and slots.is_contiguous()
+    _here(slots)
+    n, dtype = slots.shape[0], cache["rope"].dtype if dtype is None else dtype
+    latent = torch.empty((n, c.width), dtype=dtype, device=slots.device)
+    rope = torch.empty((n, c.rope_width), dtype=dtype, device=slots.device)
+    _lib.check(lib.llmp_hip_latent_read(C.byref(c), slots.data_ptr(), n, _X_TYPES[dtype], latent.data_ptr(), rope.data_ptr(), _stream()))
+    return latent, rope
+
+
+def latent_project(x, w, out=None):
+    """llmp.latent.project: out[t, h] = w[h] @ x[t, h]: x [tokens, heads, k] times w [heads, n, k] (both bfloat16 or float16), [tokens, heads, n]. A
+    head's query to the latent width, or its result back: views of one expansion matrix, or a transposed copy made once."""
+    lib = _lib.load()
+    tokens, heads, k = x.shape
+    n = w.shape[1]
+    if out is None:
+        out = torch.empty((tokens, heads, n), dtype=x.dtype, device=x.device)
+    assert w.shape == (heads, n, k) and out.shape == (tokens, heads, n) and x.dtype is w.dtype and x.dtype is out.dtype
+    (xt, xh, xd), (wh, wr, wd), (yt, yh, yd) = x.stride(), w.stride(), out.stride()
+    assert xd == wd == yd == 1
+    _here(x, w, out)
+    op = _lib.LatentProject(x.data_ptr(), w.data_ptr(), out.data_ptr(), xt, xh, wh, wr, yt, yh, _X_TYPES[x.dtype], tokens, heads, k, n)
+    _lib.check(lib.llmp_hip_latent_project(C.byref(op), _stream()))
+    return out
+
+
+def latent_attend(cache, q_latent, q_rope, table, lengths, starts, scale, *, before=None, most=None, out=None, scratch=None):
+    """llmp.latent.attend: causal attention in the absorbed form: q_latent [tokens, heads, width] and q_rope [tokens, heads, rope] of the cache's type
+    over the requests' latent rows, which are keys and values of all heads. table, lengths, starts, before, most as paged_attend takes them.
+    Returns [tokens, heads, width]; rows past starts[requests] are not written."""
+    lib = _lib.load()
+    c = _latent_cache(cache)
+    _int32(table, lengths, starts)
+    tokens, heads, width = q_latent.shape
+    n, table_width = table.shape
+    dtype = cache["rope"].dtype
+    if out is None:
+        out = torch.empty((tokens, heads, width), dtype=dtype, device=q_latent.device)
+    assert width == c.width and q_rope.shape == (tokens, heads, c.rope_width) and out.shape == q_latent.shape
+    assert q_latent.dtype is dtype and q_rope.dtype is dtype and out.dtype is dtype and lengths.shape == (n,) and starts.shape == (n + 1,)
+    (lt, lh, ld), (rt, rh, rd), (ot, oh, od) = q_latent.stride(), q_rope.stride(), out.stride()
+    assert ld == rd == od == 1
+    if before is not None:
+        _int32(before)
+        assert before.shape == (n,)
+    _here(q_latent, q_rope, out, table, lengths, starts)
+    if tokens == 0:
+        return out
+    op = _lib.LatentAttend(c, q_latent.data_ptr(), q_rope.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(before),
+                           lt, lh, rt, rh, ot, oh, _table_stride(table), heads, n, tokens, tokens if most is None else most, table_width, scale)
+    cus, at = _compute_units(), C.byref(op)
+    if scratch is None:
+        scratch = torch.empty(max(lib.llmp_hip_latent_attend_scratch(at, cus), 16), dtype=torch.uint8, device=q_latent.device)
+    _lib.check(lib.llmp_hip_latent_attend(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
+    return out
+
+
+def latent_prompt(q, k, k_rope, v, starts, scale, *, key_starts=None, most=None, out=None, scratch=None):
+    """llmp.latent.prompt: causal attention in the expanded form: q [tokens, heads, nope + rope] (the rotated part last), k [keys, heads, nope], k_rope
+    [keys, rope] (all heads'), v [keys, heads, value], bfloat16 or float16; request r's queries are rows starts[r] to starts[r + 1] - 1 (int32
+    [requests + 1]), at the last of its keys, rows key_starts[r] to key_starts[r + 1] - 1 (starts'). `most`: the largest number of a request's
+    queries, if it is known. Returns [tokens, heads, value]; rows past starts[requests] are not written."""
+    lib = _lib.load()
+    _int32(starts)
+    tokens, heads, qk = q.shape
+    keys, rope = k_rope.shape
+    nope, value = k.shape[2], v.shape[2]
+    if out is None:
+        out = torch.empty((tokens, heads, value), dtype=q.dtype, device=q.device)
+    assert qk == nope + rope and k.shape == (keys, heads, nope) and v.shape == (keys, heads, value) and out.shape == (tokens, heads, value)
+    assert q.dtype is k.dtype and q.dtype is k_rope.dtype and q.dtype is v.dtype and q.dtype is out.dtype
+    (qt, qh, qd), (kt, kh, kd), (rt, rd), (vt, vh, vd), (ot, oh, od) = q.stride(), k.stride(), k_rope.stride(), v.stride(), out.stride()
+    assert qd == kd == rd == vd == od == 1 and starts.dim() == 1
+    if key_starts is not None:
+        _int32(key_starts)
+        assert key_starts.shape == starts.shape
+    _here(q, k, k_rope, v, out, starts)
+    if tokens == 0:
+        return out
+    op = _lib.LatentPrompt(q.data_ptr(), k.data_ptr(), k_rope.data_ptr(), v.data_ptr(), out.data_ptr(), starts.data_ptr(), _ptr(key_starts), qt, qh, kt, kh,
+                           rt, vt, vh, ot, oh, _X_TYPES[q.dtype], heads, starts.shape[0] - 1, tokens, keys, tokens if most is None else most, nope, rope,
+                           value, scale)
+    cus, at = _compute_units(), C.byref(op)
+    if scratch is None:
+        scratch = torch.empty(max(lib.llmp_hip_latent_prompt_scratch(at, cus), 16), dtype=torch.uint8, device=q.device)
+    _lib.check(lib.llmp_hip_latent_prompt(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
     return out
