@@ -22,6 +22,10 @@ struct Sixteen<LLMP_X_BF16> {
   typedef __bf16 One;
   static __device__ __forceinline__ F32x16 Product32(Eight a, Eight b, F32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ F32x4 Product16(Eight a, Eight b, F32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ float AddTwo(Two v, float sum) {
+    const __bf16 one = static_cast<__bf16>(1.0f);
+    return __builtin_amdgcn_fdot2_f32_bf16(v, Two{one, one}, sum, false);
+  }
   template <bool HIGH>
   static __device__ __forceinline__ Two OfE4m3(uint32_t codes) { return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, HIGH); }
 };
@@ -32,6 +36,10 @@ struct Sixteen<LLMP_X_F16> {
   typedef _Float16 One;
   static __device__ __forceinline__ F32x16 Product32(Eight a, Eight b, F32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ F32x4 Product16(Eight a, Eight b, F32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ float AddTwo(Two v, float sum) {
+    const _Float16 one = static_cast<_Float16>(1.0f);
+    return __builtin_amdgcn_fdot2(v, Two{one, one}, sum, false);
+  }
   template <bool HIGH>
   static __device__ __forceinline__ Two OfE4m3(uint32_t codes) { return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, HIGH); }
 };
@@ -77,6 +85,29 @@ __device__ __forceinline__ void LaneLineToLds(const void* from, uint32_t to) {
 template <int LEFT>
 __device__ __forceinline__ void WaitLoads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
+// A row of COUNT products whose operands come from LDS, in groups: a group's reads stand before the products of the group before it. (Left to itself the
+// compiler saves registers, reads for one product at a time and waits for it: about 130 cycles a product of 32.) read(i) gives product i's operand,
+// multiply(i, operand) makes it.
+template <int COUNT, int GROUP, class Eight, class Read, class Multiply>
+__device__ __forceinline__ void ProductsInGroups(const Read& read, const Multiply& multiply) {
+  Eight held[2][GROUP];
+#pragma unroll
+  for (int i = 0; i < GROUP && i < COUNT; ++i) held[0][i] = read(i);
+#pragma unroll
+  for (int g = 0; g * GROUP < COUNT; ++g) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) {
+      if ((g + 1) * GROUP + i < COUNT) held[(g + 1) & 1][i] = read((g + 1) * GROUP + i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) {
+      if (g * GROUP + i < COUNT) multiply(g * GROUP + i, held[g & 1][i]);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
 }
 // All the wave's reads of LDS have been answered, and every wave of the workgroup is here.
 __device__ __forceinline__ void MeetLds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }

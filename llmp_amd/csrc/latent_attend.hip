@@ -5,12 +5,10 @@
 // What bounds it: with few heads the cache's bytes (1152 a token at 512 + 64 values against 2 * 1088 operations a row); from about 128 rows a
 // token on the matrix instructions take as long. A tile is 32 tokens, brought into LDS by loads that pass no register; the rows' queries and
 // results stay in registers. Two forms:
-//   few rows   (no request has more than 16) every wave of a workgroup's four has all rows, a ring of tiles of its own and 16 x 16 products; it
-//              waits for nobody, and the waves' results are added up at the end;
-//   many rows  a workgroup takes 128 rows of one request, 32 a wave, 32 x 32 products, all waves the same ring of tiles. A wave's results are 256 dimensions
-//              (128 registers, two waves a SIMD): at width 512 two waves share 32 rows, each with half the dimensions of both products, and
-//              add their halves of the logits through LDS. (One wave with 512 dimensions needs 256 registers of results and 144 of queries;
-//              the compiler then spilled hundreds.)
+//   few rows   (no request has more than 16) every wave of a workgroup's four has all rows and a ring of tiles of its own; it waits for nobody, and the
+//              waves' results are added up at the end;
+//   many rows  a workgroup takes 128 rows of one request, 16 a wave (128 registers of results and 64 of queries at width 512: two waves a SIMD), all
+//              waves the same ring of tiles.
 // Both products take the tile from LDS as it lies. A product's rows are tokens in an order that leaves a lane with consecutive tokens of one row, in the
 // order in which the second product takes them; the values' columns come by transposing reads.
 //
@@ -45,33 +43,28 @@ struct LatentArgs {
 
 template <int R, int P, bool EIGHT, bool FEW>
 struct LatentGeo {
-  static constexpr int kSplit = FEW ? 1 : R / 256;  // waves that share rows, by dimensions
-  static constexpr int kWaves = FEW ? 4 : 4 * kSplit, kThreads = kWaves * kWave;
-  static constexpr int kRows = FEW ? kFewRows : kManyRows, kWaveRows = FEW ? 16 : 32;
+  static constexpr int kWaves = FEW ? 4 : 8, kThreads = kWaves * kWave;
+  static constexpr int kRows = FEW ? kFewRows : kManyRows;
   static constexpr int kPitch = EIGHT ? R : 2 * R, kRopePitch = 2 * P;
   static constexpr int kLatentBytes = kTokens * kPitch, kRopeBytes = kTokens * kRopePitch, kScaleBytes = EIGHT ? 256 : 0;
   static constexpr int kTile = kLatentBytes + kRopeBytes + kScaleBytes;
-  static constexpr int kQueries = kSplit > 1 ? kManyRows * 2 * P : 0;  // the queries' rotated part, where registers are short
-  static constexpr int kExchange = kSplit > 1 ? kWaves * 4096 + kQueries : 0;
-  static constexpr int kAGroups = FEW || kSplit > 1 ? 1 : 2;  // workgroups a compute unit
-  static constexpr int kRing = FEW ? std::min(2, kLdsBytes / 4 / kTile) : std::min(5, (kLdsBytes / kAGroups - kExchange) / kTile);
+  static constexpr int kQueries = FEW ? 0 : kManyRows * 2 * P;  // the queries' rotated part, where registers are short
+  static constexpr int kRing = FEW ? std::min(2, kLdsBytes / 4 / kTile) : std::min(5, (kLdsBytes - kQueries) / kTile);
   static constexpr int kSharing = FEW ? 1 : kWaves;  // waves that bring a tile in
-  static constexpr int kAll = (kLatentBytes + kRopeBytes) / 1024 + (EIGHT ? 1 : 0);
-  static constexpr int kLoads = (kAll + kSharing - 1) / kSharing;  // a wave's for a tile
+  static constexpr int kLatentLoads = kLatentBytes / 1024 / kSharing, kRopeLoads = (kRopeBytes / 1024 + kSharing - 1) / kSharing;
+  static constexpr int kLoads = kLatentLoads + kRopeLoads + (EIGHT ? 1 : 0);  // a wave's for a tile
   static constexpr int kArea = kFewRows * R * 4 + 2 * kFewRows * 4;  // the few rows' form: a wave's results for the others
-  static constexpr int kLds = FEW ? std::max(4 * kRing * kTile, 4 * kArea) : kRing * kTile + kExchange;
-  static constexpr int kWaveR = R / kSplit, kWaveP = P / kSplit;  // a wave's dimensions
+  static constexpr int kLds = FEW ? std::max(4 * kRing * kTile, 4 * kArea) : kRing * kTile + kQueries;
 
   // What the pieces (of 16 bytes) of a token's row are turned by: the 16 lanes that a 16-byte read takes at once (KPiece in paged_attend.h), and the 32
   // that a transposing read does, then find theirs in all banks.
   static __device__ __forceinline__ int Turn(int token) {
     if constexpr (EIGHT) return (token & 7) << 1 | (token >> 3 & 1);
-    if constexpr (FEW) return (token & 3) << 2 | (0x1320 >> (4 * (token >> 3 & 3)) & 3);  // (0, 2, 3, 1)
-    return (token & 3) << 2 | (token >> 2 & 3);
+    return (token & 3) << 2 | (0x1320 >> (4 * (token >> 3 & 3)) & 3);  // (0, 2, 3, 1)
   }
   static __device__ __forceinline__ int RopeTurn(int token) {
-    if constexpr (FEW) return P == 64 ? ((token >> 1 & 1) << 2 | (0x1320 >> (4 * (token >> 3 & 3)) & 3)) : (0x1320 >> (4 * (token >> 3 & 3)) & 3);
-    return P == 64 ? ((token >> 1 & 1) | (token >> 2 & 3) << 1) : (token >> 2 & 3);
+    const int eight = 0x1320 >> (4 * (token >> 3 & 3)) & 3;
+    return P == 64 ? ((token >> 1 & 1) << 2 | eight) : eight;
   }
 };
 
@@ -102,16 +95,14 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
   using G = LatentGeo<R, P, EIGHT, FEW>;
   using S = Sixteen<TYPE>;
   typedef typename S::Eight Eight;
-  typedef std::conditional_t<FEW, F32x4, F32x16> Values;  // a lane's of a block of the result
-  constexpr int kValues = FEW ? 4 : 16, kBlock = G::kWaveRows, kInner = FEW ? 32 : 16;
-  constexpr int kSteps = G::kWaveR / kInner, kRopeSteps = G::kWaveP / kInner, kBlocks = G::kWaveR / kBlock;
-  constexpr int kLogits = FEW ? 8 : 16, kWeights = kLogits / 8;  // a lane's
+  constexpr int kSteps = R / 32, kRopeSteps = P / 32, kBlocks = R / 16;
+  constexpr int kLogits = 8;  // a lane's of a tile
+  constexpr int kKeyGroup = FEW ? 8 : 3, kValueGroup = FEW ? 8 : 3;  // products that are read for at a time
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const llmp_latent_attend& op = a.op;
   const llmp_latent_cache& c = op.cache;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int half = lane / kBlock, column = lane % kBlock;  // (`half` a quarter where rows are 16)
-  const int split = G::kSplit > 1 ? wave % G::kSplit : 0;
+  const int quarter = lane / 16, column = lane % 16;
   const int groups = gridDim.x, w = blockIdx.x;
   const uint32_t ring_off = FEW ? wave * G::kRing * G::kTile : 0;
   const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + ring_off;
@@ -156,11 +147,16 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
     before = last_of(upto);
   }
 
-  const float sign_scale = fabsf(op.scale) * kLog2E;
+  const auto scalar = [](auto v) {
+    static_assert(sizeof(v) == 4, "32 bits");
+    return __builtin_bit_cast(decltype(v), __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  };
+  const float sign_scale = scalar(fabsf(op.scale) * kLog2E);
   const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
 
   for (; u < u_end; ++request) {
-    const Line l = LineOf(a, request);
+    Line l = LineOf(a, request);
+    l = {scalar(l.start), scalar(l.n), scalar(l.length), scalar(l.base), scalar(l.groups)};
     const int64_t all = LengthBefore(a, l, l.groups);
     if (u >= before + all) {
       before += all;
@@ -192,7 +188,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
 
         // ---- the lane's row.
         const int first_token = k * a.tokens_a_pair;
-        const int row0 = FEW ? 0 : wave / G::kSplit * G::kWaveRows;
+        const int row0 = FEW ? 0 : 16 * wave;
         int rows, token, head;  // of the pair, of the lane's row
         {
           const int row = row0 + column;
@@ -211,40 +207,45 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         head = real ? head : 0;
         const int see_to = real ? max(min(l.base + token + 1, l.length), 0) : 0;
         const bool busy = row0 < rows;
+        const int all_rows_to = max(min(l.base + first_token + 1, l.length), 0);  // seen by all rows of the pair
         const int all_to = max(min(l.base + first_token + 1 + (a.pairs_a_token == 1 ? row0 / op.heads : 0), l.length), 0);  // seen by all of the wave's rows
 
         constexpr bool kRopeInLds = G::kQueries > 0;
         Eight q[kSteps + (kRopeInLds ? 0 : kRopeSteps)];
-        Eight* const q_rope = reinterpret_cast<Eight*>(lds + G::kRing * G::kTile + G::kExchange - G::kQueries) + wave * kRopeSteps * kWave;
+        const uint32_t q_rope = G::kRing * G::kTile + wave * kRopeSteps * 1024;
         {
-          const uint16_t* const ql = static_cast<const uint16_t*>(op.q_latent) + (l.start + token) * op.q_latent_token_stride + head * op.q_latent_head_stride + split * G::kWaveR + 8 * half;
-          const uint16_t* const qr = static_cast<const uint16_t*>(op.q_rope) + (l.start + token) * op.q_rope_token_stride + head * op.q_rope_head_stride + split * G::kWaveP + 8 * half;
+          const uint16_t* const ql = static_cast<const uint16_t*>(op.q_latent) + (l.start + token) * op.q_latent_token_stride + head * op.q_latent_head_stride + 8 * quarter;
+          const uint16_t* const qr = static_cast<const uint16_t*>(op.q_rope) + (l.start + token) * op.q_rope_token_stride + head * op.q_rope_head_stride + 8 * quarter;
 #pragma unroll
           for (int x = 0; x < kSteps + kRopeSteps; ++x) {
-            U32x4 v = *reinterpret_cast<const U32x4*>(x < kSteps ? ql + kInner * x : qr + kInner * (x - kSteps));
+            U32x4 v = *reinterpret_cast<const U32x4*>(x < kSteps ? ql + 32 * x : qr + 32 * (x - kSteps));
             v ^= U32x4{flip, flip, flip, flip};
             if (kRopeInLds && x >= kSteps) {
-              q_rope[(x - kSteps) * kWave + lane] = __builtin_bit_cast(Eight, v);
+              *reinterpret_cast<U32x4*>(lds + q_rope + (x - kSteps) * 1024 + 16 * lane) = v;
             } else {
               q[x] = __builtin_bit_cast(Eight, v);
             }
           }
         }
-        Values out[kBlocks];
+        F32x4 out[kBlocks];
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-          for (int i = 0; i < kValues; ++i) out[b][i] = 0.0f;
-        }
+        for (int b = 0; b < kBlocks; ++b) out[b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float top = -INFINITY, sum = 0.0f;
 
         // ---- the tiles. A lane holds the cache's row of the first token of one 16-token group of the line (-1: no page); they are looked up 64
         // at a time.
+        // (All that depends on the lane alone is worked out at every tile, from a lane number as something new: kept, it is the registers too many, and
+        // what the compiler then brings back from memory waits for the tiles under way.)
+        const auto lane_anew = [&]() {
+          int l = lane;
+          if constexpr (!FEW) asm volatile("" : "+v"(l));
+          return l;
+        };
         const int32_t* const table = op.table + request * op.table_stride;
         int held_from = -1, held = 0;
         const auto look_up = [&](int tile) {
           held_from = tile;
-          const uint32_t position = static_cast<uint32_t>(2 * tile + lane) * 16u, entry = position / static_cast<uint32_t>(c.page);
+          const uint32_t position = static_cast<uint32_t>(2 * tile + lane_anew()) * 16u, entry = position / static_cast<uint32_t>(c.page);
           held = -1;
           if (position < static_cast<uint32_t>(seen) && entry < static_cast<uint32_t>(op.table_width)) {
             const int page = table[entry];
@@ -267,32 +268,33 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           const uint8_t* const rope_b = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_b) * G::kRopePitch;
           const uint32_t to = ring_at + slot * G::kTile;
           // (Lanes and waves as something new at every tile: the compiler otherwise keeps every load's offsets, and then spills them.)
-          int lane_now = lane, wave_now = wave;
+          int lane_now = lane, wave_now = FEW ? 0 : wave;
           asm volatile("" : "+v"(lane_now), "+s"(wave_now));
           const auto load = [&](auto whole) {
+            constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
-            for (int i = 0; i < G::kLoads; ++i) {
-              const int n = FEW ? i : (i * G::kWaves + wave_now) % G::kAll;  // (the last ones again where they do not go round)
-              if (n < G::kLatentBytes / 1024) {
-                constexpr int kLanes = G::kPitch / 16, kRowsALoad = kWave / kLanes;
-                const int row0 = n * kRowsALoad, row = row0 + lane_now / kLanes;
-                const bool second = row0 >= 16;
-                const uint32_t piece = 16 * ((lane_now % kLanes) ^ G::Turn(row));
-                if constexpr (decltype(whole)::value) {
-                  LineToLds((second ? latent_b : latent_a) + (row0 & 15) * G::kPitch, lane_now / kLanes * G::kPitch + piece, to + 1024 * n);
-                } else {
-                  LineToLds(second ? latent_b : latent_a, min(row & 15, second ? last_b : last_a) * G::kPitch + piece, to + 1024 * n);
-                }
-              } else if (n < (G::kLatentBytes + G::kRopeBytes) / 1024) {
-                constexpr int kLanes = G::kRopePitch / 16, kRowsALoad = kWave / kLanes;
-                const int row0 = (n - G::kLatentBytes / 1024) * kRowsALoad, row = row0 + lane_now / kLanes;
-                const bool second = row0 >= 16;
-                const uint32_t piece = 16 * ((lane_now % kLanes) ^ G::RopeTurn(row));
-                LineToLds(second ? rope_b : rope_a, (decltype(whole)::value ? row & 15 : min(row & 15, second ? last_b : last_a)) * G::kRopePitch + piece, to + 1024 * n);
-              } else {  // the scales: four tokens a lane, eight lanes of them
-                WordToLds(c.scale, (lane_now & 4 ? row_b : row_a) + 4 * (lane_now & 3), to + G::kLatentBytes + G::kRopeBytes);
+            for (int i = 0; i < G::kLatentLoads; ++i) {
+              constexpr int kLanes = G::kPitch / 16, kRowsALoad = kWave / kLanes;
+              const int n = i * G::kSharing + wave_now, row0 = n * kRowsALoad, row = row0 + lane_now / kLanes;
+              const bool second = G::kSharing * kRowsALoad > 16 ? row0 >= 16 : i * G::kSharing * kRowsALoad >= 16;
+              const uint32_t piece = 16 * ((lane_now % kLanes) ^ G::Turn(row));
+              if constexpr (kWhole) {
+                LineToLds((second ? latent_b : latent_a) + (row0 & 15) * G::kPitch, lane_now / kLanes * G::kPitch + piece, to + 1024 * n);
+              } else {
+                LineToLds(second ? latent_b : latent_a, min(row & 15, second ? last_b : last_a) * G::kPitch + piece, to + 1024 * n);
               }
             }
+#pragma unroll
+            for (int i = 0; i < G::kRopeLoads; ++i) {
+              constexpr int kLanes = G::kRopePitch / 16, kRowsALoad = kWave / kLanes;
+              const int n = FEW ? i : wave_now % (G::kRopeBytes / 1024);  // (where there are fewer than waves some come twice)
+              const int row0 = n * kRowsALoad, row = row0 + lane_now / kLanes;
+              const bool second = row0 >= 16;
+              const uint32_t piece = 16 * ((lane_now % kLanes) ^ G::RopeTurn(row));
+              LineToLds(second ? rope_b : rope_a, (kWhole ? row & 15 : min(row & 15, second ? last_b : last_a)) * G::kRopePitch + piece, to + G::kLatentBytes + 1024 * n);
+            }
+            // The scales: four tokens a lane, eight lanes of them.
+            if constexpr (EIGHT) WordToLds(c.scale, (lane_now & 4 ? row_b : row_a) + 4 * (lane_now & 3), to + G::kLatentBytes + G::kRopeBytes);
           };
           if (left >= kTokens) {
             load(std::true_type{});
@@ -302,32 +304,24 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         };
 
         // What a lane reads of a tile. Rows are whole 256 bytes, so that a place is the lane's own (its row, its piece turned) with a constant's bits turned
-        // in and a constant added. Keys: row m of a product is token 16 (m / 4 % 2) + 4 (m / 8) + m % 4, where products are of 16 rows (the `m_block`-th) 8 (m / 4) +
-        // 4 m_block + m % 4. Values: a column's lanes name their rows, of four tokens (eight where they are bytes).
-        // (Worked out at every tile, from a lane number as something new: kept, they were the registers too many.)
+        // in and a constant added. Keys: row m of the first or second product of 16 tokens (`block`) is token 8 (m / 4) + 4 block + m % 4. Values: a column's lanes name
+        // their rows, of four tokens (eight where they are bytes).
         struct Places {
           uint32_t key, rope, value;
         };
         const auto places = [&]() {
-          int l = lane;
-          if constexpr (!FEW) asm volatile("" : "+v"(l));
-          const int half = l / kBlock, column = l % kBlock;
-          const int k_token = FEW ? 8 * (column >> 2) + (column & 3) : 16 * (column >> 2 & 1) + 4 * (column >> 3) + (column & 3);
-          const int i16 = l & 15, block16 = FEW ? 0 : l >> 4 & 1;
-          const int v_token = (FEW ? 8 : 16) * half + (EIGHT ? i16 >> 1 : i16 >> 2);
+          const int l = lane_anew(), quarter = l / 16, i16 = l % 16;
+          const int k_token = 8 * (i16 >> 2) + (i16 & 3), v_token = 8 * quarter + (EIGHT ? i16 >> 1 : i16 >> 2);
           Places p;
-          p.key = k_token * G::kPitch + (EIGHT ? 16 * (G::Turn(k_token) ^ (FEW ? half >> 1 : 0)) + 8 * (half & 1) : 16 * (G::Turn(k_token) ^ half)) +
-                  split * (G::kPitch / G::kSplit);
-          p.rope = G::kLatentBytes + k_token * G::kRopePitch + 16 * (G::RopeTurn(k_token) ^ (half + split * (G::kWaveP / 8)));
-          p.value = v_token * G::kPitch + (EIGHT ? 16 * (block16 ^ G::Turn(v_token)) : 16 * ((2 * block16 + (i16 >> 1 & 1)) ^ G::Turn(v_token))) + 8 * (i16 & 1) +
-                    split * (G::kPitch / G::kSplit);
+          p.key = k_token * G::kPitch + (EIGHT ? 16 * (G::Turn(k_token) ^ (quarter >> 1)) + 8 * (quarter & 1) : 16 * (G::Turn(k_token) ^ quarter));
+          p.rope = G::kLatentBytes + k_token * G::kRopePitch + 16 * (G::RopeTurn(k_token) ^ quarter);
+          p.value = v_token * G::kPitch + 16 * (EIGHT ? G::Turn(v_token) : (i16 >> 1 & 1) ^ G::Turn(v_token)) + 8 * (i16 & 1);
           return p;
         };
-        // Constants of a place: Turn of tokens + 4 m_block (keys of 16-row products), + 8 s and + 4 of it (values).
-        const auto key = [&](uint32_t at, uint32_t rope_at, int x, int m_block) {
-          constexpr int kPieces = EIGHT ? kInner / 16 : kInner / 8;
-          if (x >= kSteps) return *reinterpret_cast<const Eight*>(lds + (rope_at ^ 16 * (kInner / 8 * (x - kSteps))) + 4 * m_block * G::kRopePitch);
-          const uint32_t place = (at ^ 16 * ((kPieces * x & 15) ^ (EIGHT && FEW ? 8 * m_block : 0))) + 256 * (kPieces * x >> 4) + 4 * m_block * G::kPitch;
+        const auto key = [&](uint32_t at, uint32_t rope_at, int x, int block) {
+          constexpr int kPieces = EIGHT ? 2 : 4;  // a step's
+          if (x >= kSteps) return *reinterpret_cast<const Eight*>(lds + (rope_at ^ 64 * (x - kSteps)) + 4 * block * G::kRopePitch);
+          const uint32_t place = (at ^ 16 * ((kPieces * x & 15) ^ (EIGHT ? 8 * block : 0))) + 256 * (kPieces * x >> 4) + 4 * block * G::kPitch;
           if constexpr (EIGHT) {
             const uint2 v = *reinterpret_cast<const uint2*>(lds + place);
             return EightE4m3<TYPE>(v.x, v.y);
@@ -335,102 +329,98 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             return *reinterpret_cast<const Eight*>(lds + place);
           }
         };
-        // Tokens 16 half + 8 s to + 7 (8 half to + 7) of dimension kBlock b + column.
-        const auto value = [&](uint32_t at, int b, int s) {
-          constexpr int kPieces = EIGHT ? kBlock / 16 : kBlock / 8;
-          const int x = kPieces * b;
+        // Tokens 8 quarter to + 7 of dimension 16 b + column.
+        const auto value = [&](uint32_t at, int b) {
+          constexpr int kPieces = EIGHT ? 1 : 2;
+          const uint32_t place = (at ^ 16 * (kPieces * b & 15)) + 256 * (kPieces * b >> 4);
           if constexpr (EIGHT) {
-            const I32x2 v = Column8(lds + (at ^ 16 * ((x & 15) ^ s)) + 256 * (x >> 4) + 8 * s * G::kPitch);
+            const I32x2 v = Column8(lds + place);
             return EightE4m3<TYPE>(v.x, v.y);
           } else {
-            constexpr int kTurnOf4 = FEW ? 0 : 1;
-            const S16x4 v = Column4(lds + (at ^ 16 * ((x & 15) ^ 2 * s)) + 256 * (x >> 4) + 8 * s * G::kPitch);
-            return JoinFours<Eight>(v, Column4(lds + (at ^ 16 * ((x & 15) ^ 2 * s ^ kTurnOf4)) + 256 * (x >> 4) + (8 * s + 4) * G::kPitch));
+            const S16x4 v = Column4(lds + place);
+            return JoinFours<Eight>(v, Column4(lds + place + 4 * G::kPitch));
           }
         };
-        float* const exchange = reinterpret_cast<float*>(lds + G::kRing * G::kTile);
 
-        // A tile's logits of a wave's rows over its dimensions: element i is token 16 half + i (8 half + i).
-        float dots[kLogits], scale8[kLogits];
+        // A tile's logits of a wave's rows: element i is token 8 quarter + i.
+        float dots[kLogits];
+        const auto scales = [&](uint32_t tile, float (&scale)[kLogits]) {
+          const uint2 e = *reinterpret_cast<const uint2*>(lds + tile + G::kLatentBytes + G::kRopeBytes + 8 * (lane_anew() / 16));
+#pragma unroll
+          for (int i = 0; i < kLogits; ++i) {
+            const uint32_t bits = (i < 4 ? e.x : e.y) >> (8 * (i & 3)) & 0xFFu;
+            scale[i] = __builtin_bit_cast(float, bits == 0 ? 0x00400000u : bits << 23);
+          }
+        };
         const auto keys = [&](uint32_t tile) {
           const Places p = places();
-          const uint32_t key_at = tile + p.key, rope_at = tile + p.rope;
-          Values sums[kLogits / kValues];
-#pragma unroll
-          for (int m = 0; m < kLogits / kValues; ++m) {
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) sums[m][i] = 0.0f;
-          }
-          const auto steps = [&](int from, int to) {
-#pragma unroll
-            for (int x = from; x < to; ++x) {
-              const Eight query = kRopeInLds && x >= kSteps ? q_rope[(x - kSteps) * kWave + lane] : q[kRopeInLds && x >= kSteps ? 0 : x];
-#pragma unroll
-              for (int m = 0; m < kLogits / kValues; ++m) {
-                if constexpr (FEW) sums[m] = S::Product16(key(key_at, rope_at, x, m), query, sums[m]);
-                if constexpr (!FEW) sums[m] = S::Product32(key(key_at, rope_at, x, m), query, sums[m]);
-              }
-            }
+          const uint32_t key_at = tile + p.key, rope_at = tile + p.rope, query_at = kRopeInLds ? q_rope + 16 * lane_anew() : 0;
+          F32x4 sums[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          const auto steps = [&](auto from, auto to) {
+            constexpr int kFrom = decltype(from)::value;
+            // (Steps 256 bytes apart side by side: their places are one with two constants.)
+            const auto step_of = [](int i) {
+              constexpr int kSame = EIGHT ? kSteps / 8 : kSteps / 4;
+              const int x = kFrom + i / 2;
+              return x >= kSteps ? x : x / kSame + kSteps / kSame * (x % kSame);
+            };
+            ProductsInGroups<2 * (decltype(to)::value - kFrom), kKeyGroup, Eight>([&](int i) { return key(key_at, rope_at, step_of(i), i % 2); },
+                                                                                  [&](int i, Eight k) {
+                                                                                    const int x = step_of(i);
+                                                                                    const Eight query = kRopeInLds && x >= kSteps ? *reinterpret_cast<const Eight*>(lds + query_at + (x - kSteps) * 1024)
+                                                                                                                                  : q[kRopeInLds && x >= kSteps ? 0 : x];
+                                                                                    sums[i % 2] = S::Product16(k, query, sums[i % 2]);
+                                                                                  });
           };
+          constexpr std::integral_constant<int, 0> kBegin{};
+          constexpr std::integral_constant<int, kSteps> kMiddle{};
+          constexpr std::integral_constant<int, kSteps + kRopeSteps> kEnd{};
           if constexpr (EIGHT) {
             // Codes' products first: their scale is the token's, the rotated part's is one.
-            steps(0, kSteps);
-            uint32_t e[kLogits / 4];
-            const uint32_t scales_at = tile + G::kLatentBytes + G::kRopeBytes + kLogits * half;
+            steps(kBegin, kMiddle);
+            float scale8[kLogits];
+            scales(tile, scale8);
 #pragma unroll
-            for (int i = 0; i < kLogits / 4; ++i) e[i] = *reinterpret_cast<const uint32_t*>(lds + scales_at + 4 * i);
-#pragma unroll
-            for (int i = 0; i < kLogits; ++i) {
-              const uint32_t bits = e[i / 4] >> (8 * (i & 3)) & 0xFFu;
-              scale8[i] = __builtin_bit_cast(float, bits == 0 ? 0x00400000u : bits << 23);
-              sums[i / kValues][i % kValues] *= scale8[i];
-            }
-            steps(kSteps, kSteps + kRopeSteps);
+            for (int i = 0; i < kLogits; ++i) sums[i / 4][i % 4] *= scale8[i];
+            steps(kMiddle, kEnd);
           } else {
-            steps(0, kSteps + kRopeSteps);
+            steps(kBegin, kEnd);
           }
 #pragma unroll
-          for (int i = 0; i < kLogits; ++i) dots[i] = sums[i / kValues][i % kValues];
+          for (int i = 0; i < kLogits; ++i) dots[i] = sums[i / 4][i % 4];
         };
-        const auto give = [&]() {
-#pragma unroll
-          for (int i = 0; i < kLogits / 4; ++i)
-            reinterpret_cast<F32x4*>(exchange)[(wave * (kLogits / 4) + i) * kWave + lane] = F32x4{dots[4 * i], dots[4 * i + 1], dots[4 * i + 2], dots[4 * i + 3]};
-        };
-        const auto take = [&]() {
-#pragma unroll
-          for (int i = 0; i < kLogits / 4; ++i) {
-            const F32x4 v = reinterpret_cast<const F32x4*>(exchange)[((wave ^ 1) * (kLogits / 4) + i) * kWave + lane];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dots[4 * i + e] += v[e];
-          }
-        };
-
-        const auto values = [&](int tile_number, uint32_t tile, uint32_t gone) {
+        const auto values = [&](int tile_number, uint32_t tile, uint32_t gone, bool alone) {
           const uint32_t value_at = tile + places().value;
+          const int p0 = tile_number * kTokens;
+          float scale8[kLogits];
+          if constexpr (EIGHT) scales(tile, scale8);
           // ---- what the rows see
-          const int p0 = tile_number * kTokens, lane_token = kLogits * half;
           bool garbage = false;
-#pragma unroll
-          for (int i = 0; i < kLogits; ++i) dots[i] *= sign_scale;
+          float worth = sign_scale;
           if (p0 + kTokens > all_to || gone != 0) {
             asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
+            const int lane_token = 8 * (lane_anew() / 16);
             const int to = (gone >> (lane_token >> 4) & 1) != 0 ? 0 : see_to - p0 - lane_token;
 #pragma unroll
             for (int i = 0; i < kLogits; ++i) {
               // (A value that is no number, or one that a product with zero would make none, has no finite product with any query.)
-              garbage = garbage || (i >= to && !(fabsf(dots[i]) < INFINITY));
-              dots[i] = i < to ? dots[i] : -INFINITY;
+              garbage |= (i >= to) & !(fabsf(dots[i]) < INFINITY);
+              dots[i] = i < to ? dots[i] * sign_scale : -INFINITY;
               if constexpr (EIGHT) scale8[i] = i < to ? scale8[i] : 0.0f;
             }
+            worth = 1.0f;
           }
           // ---- softmax. Eight-bit weights take the token's scale along; the maximum is of both.
           float peak = -INFINITY;
+          if constexpr (EIGHT) {
 #pragma unroll
-          for (int i = 0; i < kLogits; ++i) {
-            peak = fmaxf(peak, EIGHT ? dots[i] + __builtin_amdgcn_logf(fmaxf(scale8[i], 0x1p-80f)) : dots[i]);
+            for (int i = 0; i < kLogits; ++i) peak = fmaxf(peak, fmaf(dots[i], worth, __builtin_amdgcn_logf(fmaxf(scale8[i], 0x1p-80f))));
+          } else {
+#pragma unroll
+            for (int i = 0; i < kLogits; i += 2) peak = fmaxf(fmaxf(peak, dots[i]), dots[i + 1]);
+            peak *= worth;
           }
-          peak = Across<kBlock>(peak);
+          peak = AcrossGroupsMax(peak);
           if (__any(peak > top + (kUp + kFollow))) {
             const float higher = fmaxf(top, peak - kUp);
             const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
@@ -440,31 +430,35 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
           }
           const float less = top == -INFINITY ? 0.0f : top;
-          Eight weights[kWeights];
+          Eight weights;
 #pragma unroll
-          for (int i = 0; i < kLogits; ++i) {
-            const float p = __builtin_amdgcn_exp2f(dots[i] - less);
-            sum += p;
-            weights[i / 8][i % 8] = static_cast<typename S::One>(EIGHT ? p * scale8[i] : p);
+          for (int i = 0; i < kLogits; i += 2) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(dots[i], worth, -less)), p1 = __builtin_amdgcn_exp2f(fmaf(dots[i + 1], worth, -less));
+            if constexpr (EIGHT) {
+              sum += p + p1;
+              weights[i] = static_cast<typename S::One>(p * scale8[i]), weights[i + 1] = static_cast<typename S::One>(p1 * scale8[i + 1]);
+            } else {
+              weights[i] = static_cast<typename S::One>(p), weights[i + 1] = static_cast<typename S::One>(p1);
+              // (The sum is of the weights as they are rounded, two in an instruction.)
+              sum = S::AddTwo(typename S::Two{weights[i], weights[i + 1]}, sum);
+            }
           }
-          const auto product = [](Eight x, Eight y, Values z) {
-            if constexpr (FEW) return S::Product16(x, y, z);
-            if constexpr (!FEW) return S::Product32(x, y, z);
-          };
-          if (__any(garbage)) {
+          if (alone && __any(garbage)) {
             // A token that some row must not see holds infinities or NaN, which a weight of zero does not keep out: they become zeros in LDS. (A row that
-            // sees them has no finite logit there, and no finite sum. Nobody reads the tile as keys any more.)
+            // sees them has no finite logit there, and no finite sum. `alone`: nobody reads the tile as keys any more. Elsewhere all rows see the same.)
 #pragma unroll 1
             for (uint32_t i = 16 * lane; i < G::kLatentBytes; i += 1024) {
               U32x4* const at = reinterpret_cast<U32x4*>(lds + tile + i);
               *at = EIGHT ? FiniteCodes(*at) : Finite<TYPE>(*at);
             }
           }
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-            for (int s = 0; s < kWeights; ++s) out[b] = product(value(value_at, b, s), weights[s], out[b]);
-          }
+          // (Blocks 256 bytes apart side by side, for the same reason as the keys' steps.)
+          const auto block_of = [](int i) {
+            constexpr int kSame = EIGHT ? kBlocks / 16 : kBlocks / 8;
+            return i / kSame + kBlocks / kSame * (i % kSame);
+          };
+          ProductsInGroups<kBlocks, kValueGroup, Eight>([&](int i) { return value(value_at, block_of(i)); },
+                                                        [&](int i, Eight v) { out[block_of(i)] = S::Product16(v, weights, out[block_of(i)]); });
         };
 
         if constexpr (FEW) {
@@ -479,7 +473,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             }
             const int tile = my_from + i * step;
             keys(ring_off + i % G::kRing * G::kTile);
-            values(tile, ring_off + i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u);
+            values(tile, ring_off + i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u, true);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (i + G::kRing < count) fetch(my_from + (i + G::kRing) * step, i % G::kRing);
           }
@@ -487,6 +481,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           const int count = tile_to - tile_from;
           constexpr int kAhead = G::kRing - 1;
           for (int i = 0; i < kAhead && i < count; ++i) fetch(tile_from + i, i);
+          const bool one_token = a.tokens_a_pair == 1 || rows <= op.heads;
           for (int i = 0; i < count; ++i) {
             // Tile i has landed: of the tiles asked for only later ones are under way.
             const int later = min(kAhead - 1, count - 1 - i);
@@ -501,30 +496,27 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             }
             MeetLds();
             if (i + kAhead < count) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
-            if (busy) keys(i % G::kRing * G::kTile);
-            if constexpr (G::kSplit > 1) {
-              if (busy) give();
-            }
-            MeetLds();
-            if constexpr (G::kSplit > 1) {
-              if (busy) take();
-            }
-            if (busy) values(tile_from + i, i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u);
+            const uint32_t at = i % G::kRing * G::kTile, gone = absent >> (2 * (i % G::kRing)) & 3u;
+            // (Values that some row must not see may have to be changed in LDS: once nobody multiplies them as keys any more.)
+            const bool careful = gone != 0 || (!one_token && (tile_from + i + 1) * kTokens > all_rows_to);
+            if (busy) keys(at);
+            if (careful) MeetLds();
+            if (busy) values(tile_from + i, at, gone, careful);
           }
           MeetLds();
         }
-        sum = AcrossSum<kBlock>(sum);
+        sum = AcrossGroupsSum(sum);
 
         // ---- the few rows' form: the waves' results added up, a quarter of the dimensions each.
         constexpr int kMine = FEW ? kBlocks / 4 : kBlocks;  // blocks that the wave writes
-        const int first_block = FEW ? wave * kMine : split * kBlocks;
-        Values result[kMine];
+        const int first_block = FEW ? wave * kMine : 0;
+        F32x4 result[kMine];
         if constexpr (FEW) {
           MeetLds();
           uint8_t* const area = lds + wave * G::kArea;
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) reinterpret_cast<F32x4*>(area)[b * kWave + lane] = out[b];
-          if (half == 0) reinterpret_cast<float2*>(area + kFewRows * R * 4)[column] = make_float2(top, sum);
+          if (quarter == 0) reinterpret_cast<float2*>(area + kFewRows * R * 4)[column] = make_float2(top, sum);
           MeetLds();
           float2 numbers[4];
           top = -INFINITY;
@@ -548,19 +540,15 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           for (int b = 0; b < kMine; ++b) result[b] = out[b];
         }
 
-        // ---- out, or a part for the join. Element 4i + e of a block is dimension 8i + 4 half + e of it.
-        const int first_dimension = first_block * kBlock + 4 * half;
+        // ---- out, or a part for the join. Element e of a block is dimension 4 quarter + e of it.
         if (begins && ends) {
           if (busy && real) {
             const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-            const int64_t to = (l.start + token) * op.out_token_stride + head * op.out_head_stride + first_dimension;
+            const int64_t to = (l.start + token) * op.out_token_stride + head * op.out_head_stride + 16 * first_block + 4 * quarter;
 #pragma unroll
             for (int b = 0; b < kMine; ++b) {
-#pragma unroll
-              for (int i = 0; i < kValues / 4; ++i) {
-                const float v[4] = {result[b][4 * i] * by, result[b][4 * i + 1] * by, result[b][4 * i + 2] * by, result[b][4 * i + 3] * by};
-                StoreValues<TYPE, 4>(op.out, to + kBlock * b + 8 * i, v);
-              }
+              const float v[4] = {result[b][0] * by, result[b][1] * by, result[b][2] * by, result[b][3] * by};
+              StoreValues<TYPE, 4>(op.out, to + 16 * b, v);
             }
           }
         } else {
@@ -570,15 +558,11 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             p[0] = request, p[1] = k * a.pairs_a_token + part, p[2] = rows, p[3] = l.start + first_token;
           }
           if (busy) {
-            const int64_t row = static_cast<int64_t>(which) * G::kRows + row0 + column;
-            if (half == 0) reinterpret_cast<float2*>(a.numbers)[row] = make_float2(top, sum);
-            float* const to = a.values + row * R + first_dimension;
+            const int64_t rows16 = static_cast<int64_t>(which) * (G::kRows / 16) + row0 / 16;
+            if (quarter == 0) reinterpret_cast<float2*>(a.numbers)[rows16 * 16 + column] = make_float2(top, sum);
+            F32x4* const to = reinterpret_cast<F32x4*>(a.values) + (rows16 * kBlocks + first_block) * kWave + lane;
 #pragma unroll
-            for (int b = 0; b < kMine; ++b) {
-#pragma unroll
-              for (int i = 0; i < kValues / 4; ++i)
-                *reinterpret_cast<F32x4*>(to + kBlock * b + 8 * i) = F32x4{result[b][4 * i], result[b][4 * i + 1], result[b][4 * i + 2], result[b][4 * i + 3]};
-            }
+            for (int b = 0; b < kMine; ++b) to[b * kWave] = result[b];
           }
         }
       }
@@ -587,16 +571,16 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
   }
 }
 
-// The parts of a pair, joined: a wave a row, eight (four) values a lane. grid (workgroups of the first launch, rows / 4).
+// The parts of a pair, joined, as they lie: a thread four values of a row, four blocks of dimensions a wave. grid (workgroups of the first launch, 16 rows, blocks / 16).
+constexpr int kJoinBlocks = 4;  // of a wave
 template <int TYPE, int R>
 __global__ __launch_bounds__(256) void LatentJoinKernel(const LatentArgs a, int part_rows, int groups) {
-  constexpr int kValues = R / kWave;
   const llmp_latent_attend& op = a.op;
-  const int lane = threadIdx.x & (kWave - 1), row = blockIdx.y * 4 + threadIdx.x / kWave;
-  const int first = 2 * blockIdx.x + 1;
+  const int lane = threadIdx.x & (kWave - 1), column = lane % 16, quarter = lane / 16;
+  const int first = 2 * blockIdx.x + 1, block0 = kJoinBlocks * (4 * blockIdx.z + threadIdx.x / kWave);
   const int32_t* const p = a.parts + 4 * first;
   const int request = p[0], pair = p[1], rows = p[2], token0 = p[3];
-  if (request < 0 || row >= rows) return;
+  if (request < 0 || 16 * static_cast<int>(blockIdx.y) >= rows) return;
   // The parts after the first are the next workgroups' first ones, as long as they are of this pair.
   int count = 1;
   for (int base = blockIdx.x + 1;; base += kWave) {
@@ -607,35 +591,37 @@ __global__ __launch_bounds__(256) void LatentJoinKernel(const LatentArgs a, int 
     count += here;
     if (here < kWave) break;
   }
-  const auto part_row = [&](int i) { return static_cast<int64_t>(i == 0 ? first : 2 * (static_cast<int>(blockIdx.x) + i)) * part_rows + row; };
+  const auto rows16 = [&](int i) { return static_cast<int64_t>(i == 0 ? first : 2 * (static_cast<int>(blockIdx.x) + i)) * (part_rows / 16) + blockIdx.y; };
   float most = -INFINITY;
-  for (int i = lane; i < count; i += kWave) most = fmaxf(most, a.numbers[2 * part_row(i)]);
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+  for (int i = quarter; i < count; i += 4) most = fmaxf(most, a.numbers[2 * (rows16(i) * 16 + column)]);
+  most = fmaxf(most, __shfl_xor(most, 16));
+  most = fmaxf(most, __shfl_xor(most, 32));
   const float less = most == -INFINITY ? 0.0f : most;
-  float sum = 0.0f, v[kValues];
+  float sum = 0.0f;
+  F32x4 v[kJoinBlocks];
 #pragma unroll
-  for (int e = 0; e < kValues; ++e) v[e] = 0.0f;
-#pragma unroll 4
+  for (int b = 0; b < kJoinBlocks; ++b) v[b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
   for (int i = 0; i < count; ++i) {
-    const int64_t at = part_row(i);
-    const float2 n = reinterpret_cast<const float2*>(a.numbers)[at];
+    const int64_t at = rows16(i);
+    const float2 n = reinterpret_cast<const float2*>(a.numbers)[at * 16 + column];
     const float by = __builtin_amdgcn_exp2f(n.x - less);
     sum = fmaf(n.y, by, sum);
-    const F32x4* const from = reinterpret_cast<const F32x4*>(a.values + at * R + kValues * lane);
+    const F32x4* const from = reinterpret_cast<const F32x4*>(a.values) + (at * (R / 16) + block0) * kWave + lane;
 #pragma unroll
-    for (int e = 0; e < kValues / 4; ++e) {
-      const F32x4 x = from[e];
-#pragma unroll
-      for (int f = 0; f < 4; ++f) v[4 * e + f] = fmaf(x[f], by, v[4 * e + f]);
-    }
+    for (int b = 0; b < kJoinBlocks; ++b) v[b] += from[b * kWave] * by;
   }
+  const int row = 16 * blockIdx.y + column;
+  if (row >= rows) return;
   const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-  for (int e = 0; e < kValues; ++e) v[e] *= by;
   const int token = token0 + (a.pairs_a_token == 1 ? row / op.heads : 0);
   const int head = a.pairs_a_token == 1 ? row % op.heads : pair % a.pairs_a_token * part_rows + row;
-  StoreValues<TYPE, kValues>(op.out, token * op.out_token_stride + head * op.out_head_stride + kValues * lane, v);
+  const int64_t to = token * op.out_token_stride + head * op.out_head_stride + 16 * block0 + 4 * quarter;
+#pragma unroll
+  for (int b = 0; b < kJoinBlocks; ++b) {
+    const float x[4] = {v[b][0] * by, v[b][1] * by, v[b][2] * by, v[b][3] * by};
+    StoreValues<TYPE, 4>(op.out, to + 16 * b, x);
+  }
 }
 
 // f with the type, width, rope width, 8 bits or not and the form as constants.
@@ -686,7 +672,6 @@ int CheckLatentAttend(const llmp_latent_attend* op, int cus) {
   return 0;
 }
 
-int Groups(const llmp_latent_attend& op, int cus) { return !FewRows(op) && op.cache.width == 256 ? 2 * cus : cus; }
 size_t PartsBytes(int groups) { return static_cast<size_t>(2 * groups) * 16; }
 
 }  // namespace
@@ -696,7 +681,7 @@ using namespace llmp_hip;
 
 extern "C" size_t llmp_hip_latent_attend_scratch(const llmp_latent_attend* op, int cus) {
   if (CheckLatentAttend(op, cus) != 0) return 0;
-  const int groups = Groups(*op, cus);
+  const int groups = cus;
   const size_t rows = static_cast<size_t>(2 * groups) * RowsOf(*op);
   return PartsBytes(groups) + rows * 8 + rows * op->cache.width * 4;
 }
@@ -708,8 +693,7 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
     return Refuse(1, "latent_attend: %zu bytes of scratch at a 16-byte boundary, not %zu", need, scratch_bytes);
   const bool few = FewRows(*op);
   const int rows = RowsOf(*op);
-  // (Workgroups: as many as the compute units hold at once.)
-  const int groups = Groups(*op, cus);
+  const int groups = cus;
   LatentArgs a;
   a.op = *op;
   a.parts = static_cast<int32_t*>(scratch);
@@ -730,7 +714,7 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
     static bool sized = false;
     if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kFew>), kLds, &sized)) return;
     hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(groups), dim3(G::kThreads), kLds, s, a);
-    hipLaunchKernelGGL((LatentJoinKernel<kType, kR>), dim3(groups, (rows + 3) / 4), dim3(256), 0, s, a, rows, groups);
+    hipLaunchKernelGGL((LatentJoinKernel<kType, kR>), dim3(groups, rows / 16, kR / (64 * kJoinBlocks)), dim3(256), 0, s, a, rows, groups);
   });
   return LaunchStatus("latent_attend");
 }
