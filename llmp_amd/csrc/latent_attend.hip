@@ -266,10 +266,11 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           const uint8_t* const latent_b = static_cast<const uint8_t*>(c.latent) + static_cast<int64_t>(row_b) * G::kPitch;
           const uint8_t* const rope_a = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_a) * G::kRopePitch;
           const uint8_t* const rope_b = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_b) * G::kRopePitch;
-          const uint32_t to = ring_at + slot * G::kTile;
+          const uint32_t to = scalar(ring_at + slot * G::kTile);
           // (Lanes and waves as something new at every tile: the compiler otherwise keeps every load's offsets, and then spills them.)
           int lane_now = lane, wave_now = FEW ? 0 : wave;
-          asm volatile("" : "+v"(lane_now), "+s"(wave_now));
+          asm volatile("" : "+v"(lane_now));
+          asm volatile("" : "+s"(wave_now));
           const auto load = [&](auto whole) {
             constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
@@ -478,9 +479,10 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             if (i + G::kRing < count) fetch(my_from + (i + G::kRing) * step, i % G::kRing);
           }
         } else {
-          const int count = tile_to - tile_from;
+          const int count = scalar(tile_to - tile_from);
           constexpr int kAhead = G::kRing - 1;
           for (int i = 0; i < kAhead && i < count; ++i) fetch(tile_from + i, i);
+          const bool early = wave < G::kWaves / 2;
           const bool one_token = a.tokens_a_pair == 1 || rows <= op.heads;
           for (int i = 0; i < count; ++i) {
             // Tile i has landed: of the tiles asked for only later ones are under way.
@@ -495,11 +497,14 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
               WaitLoads<0>();
             }
             MeetLds();
-            if (i + kAhead < count) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
+            // (Half of the waves ask for their part now, half between the products: all at once they wait for each other's loads to be taken.)
+            const bool more = i + kAhead < count;
+            if (more && early) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
             const uint32_t at = i % G::kRing * G::kTile, gone = absent >> (2 * (i % G::kRing)) & 3u;
             // (Values that some row must not see may have to be changed in LDS: once nobody multiplies them as keys any more.)
             const bool careful = gone != 0 || (!one_token && (tile_from + i + 1) * kTokens > all_rows_to);
             if (busy) keys(at);
+            if (more && !early) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
             if (careful) MeetLds();
             if (busy) values(tile_from + i, at, gone, careful);
           }
@@ -571,56 +576,82 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
   }
 }
 
-// The parts of a pair, joined, as they lie: a thread four values of a row, four blocks of dimensions a wave. grid (workgroups of the first launch, 16 rows, blocks / 16).
-constexpr int kJoinBlocks = 4;  // of a wave
+// The parts of a pair, joined, as they lie: an item is 16 rows by 16 dimensions, a lane four values of a row. The pair's items are dealt to the workgroups
+// (of this launch, kJoinGroups for each of the first one's) that hold its parts, so that what one reads is about the same whatever the number of parts. A wave takes an
+// item, or where there are many parts a workgroup one together, a wave every fourth part. (One wave an item: 256 parts of a pair 180 us.)
+constexpr int kJoinGroups = 8, kJoinAlone = 16;
 template <int TYPE, int R>
 __global__ __launch_bounds__(256) void LatentJoinKernel(const LatentArgs a, int part_rows, int groups) {
+  constexpr int kBlocks = R / 16;
+  __shared__ F32x4 met[3][kWave];
+  __shared__ float met_sums[3][kWave];
   const llmp_latent_attend& op = a.op;
-  const int lane = threadIdx.x & (kWave - 1), column = lane % 16, quarter = lane / 16;
-  const int first = 2 * blockIdx.x + 1, block0 = kJoinBlocks * (4 * blockIdx.z + threadIdx.x / kWave);
-  const int32_t* const p = a.parts + 4 * first;
-  const int request = p[0], pair = p[1], rows = p[2], token0 = p[3];
-  if (request < 0 || 16 * static_cast<int>(blockIdx.y) >= rows) return;
-  // The parts after the first are the next workgroups' first ones, as long as they are of this pair.
-  int count = 1;
-  for (int base = blockIdx.x + 1;; base += kWave) {
-    const int g = base + lane;
-    const bool same = g < groups && a.parts[8 * g] == request && a.parts[8 * g + 1] == pair;
-    const uint64_t not_same = ~__ballot(same);
-    const int here = not_same == 0 ? kWave : __ffsll(static_cast<unsigned long long>(not_same)) - 1;
-    count += here;
-    if (here < kWave) break;
-  }
-  const auto rows16 = [&](int i) { return static_cast<int64_t>(i == 0 ? first : 2 * (static_cast<int>(blockIdx.x) + i)) * (part_rows / 16) + blockIdx.y; };
-  float most = -INFINITY;
-  for (int i = quarter; i < count; i += 4) most = fmaxf(most, a.numbers[2 * (rows16(i) * 16 + column)]);
-  most = fmaxf(most, __shfl_xor(most, 16));
-  most = fmaxf(most, __shfl_xor(most, 32));
-  const float less = most == -INFINITY ? 0.0f : most;
-  float sum = 0.0f;
-  F32x4 v[kJoinBlocks];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, column = lane % 16, quarter = lane / 16;
+  const int x = blockIdx.x;
+  // This workgroup's parts: its pair's later one (0), its pair's first one (1).
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int32_t* const mine = a.parts + 8 * x + 4 * which;
+    const int request = mine[0], pair = mine[1], rows = mine[2], token0 = mine[3];
+    if (request < 0) continue;
+    int leader = x;
+    if (which == 0) {  // the last workgroup before this one that begins a pair has begun this one
+      for (int base = x - 1;; base -= kWave) {
+        const int g = base - lane;
+        const uint64_t begins = __ballot(g >= 0 && a.parts[8 * max(g, 0) + 4] >= 0);
+        leader = base - (__ffsll(static_cast<unsigned long long>(begins)) - 1);
+        if (begins != 0 || base < kWave) break;
+      }
+    }
+    // The parts after the first are the next workgroups' first ones, as long as they are of this pair.
+    int count = 1;
+    for (int base = leader + 1;; base += kWave) {
+      const int g = base + lane;
+      const bool same = g < groups && a.parts[8 * min(g, groups - 1)] == request && a.parts[8 * min(g, groups - 1) + 1] == pair;
+      const uint64_t not_same = ~__ballot(same);
+      const int here = not_same == 0 ? kWave : __ffsll(static_cast<unsigned long long>(not_same)) - 1;
+      count += here;
+      if (here < kWave) break;
+    }
+    const auto rows16 = [&](int i, int r16) { return static_cast<int64_t>(i == 0 ? 2 * leader + 1 : 2 * (leader + i)) * (part_rows / 16) + r16; };
+    const bool together = count > kJoinAlone;
+    const int items = (rows + 15) / 16 * kBlocks;
+    const int waves = together ? 1 : 4, first = together ? 0 : wave;
+    for (int item = ((x - leader) * kJoinGroups + static_cast<int>(blockIdx.y)) * waves + first; item < items; item += count * kJoinGroups * waves) {
+      const int r16 = item / kBlocks, block = item % kBlocks;
+      float most = -INFINITY;
+      for (int i = quarter; i < count; i += 4) most = fmaxf(most, a.numbers[2 * (rows16(i, r16) * 16 + column)]);
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      const float less = most == -INFINITY ? 0.0f : most;
+      float sum = 0.0f;
+      F32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+      for (int i = together ? wave : 0; i < count; i += together ? 4 : 1) {
+        const int64_t at = rows16(i, r16);
+        const float2 n = reinterpret_cast<const float2*>(a.numbers)[at * 16 + column];
+        const float by = __builtin_amdgcn_exp2f(n.x - less);
+        sum = fmaf(n.y, by, sum);
+        v += reinterpret_cast<const F32x4*>(a.values)[(at * kBlocks + block) * kWave + lane] * by;
+      }
+      if (together) {
+        if (wave > 0) met[wave - 1][lane] = v, met_sums[wave - 1][lane] = sum;
+        __syncthreads();
+        if (wave == 0) {
 #pragma unroll
-  for (int b = 0; b < kJoinBlocks; ++b) v[b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-  for (int i = 0; i < count; ++i) {
-    const int64_t at = rows16(i);
-    const float2 n = reinterpret_cast<const float2*>(a.numbers)[at * 16 + column];
-    const float by = __builtin_amdgcn_exp2f(n.x - less);
-    sum = fmaf(n.y, by, sum);
-    const F32x4* const from = reinterpret_cast<const F32x4*>(a.values) + (at * (R / 16) + block0) * kWave + lane;
-#pragma unroll
-    for (int b = 0; b < kJoinBlocks; ++b) v[b] += from[b * kWave] * by;
-  }
-  const int row = 16 * blockIdx.y + column;
-  if (row >= rows) return;
-  const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-  const int token = token0 + (a.pairs_a_token == 1 ? row / op.heads : 0);
-  const int head = a.pairs_a_token == 1 ? row % op.heads : pair % a.pairs_a_token * part_rows + row;
-  const int64_t to = token * op.out_token_stride + head * op.out_head_stride + 16 * block0 + 4 * quarter;
-#pragma unroll
-  for (int b = 0; b < kJoinBlocks; ++b) {
-    const float x[4] = {v[b][0] * by, v[b][1] * by, v[b][2] * by, v[b][3] * by};
-    StoreValues<TYPE, 4>(op.out, to + 16 * b, x);
+          for (int i = 0; i < 3; ++i) v += met[i][lane], sum += met_sums[i][lane];
+        }
+        __syncthreads();
+      }
+      const int row = 16 * r16 + column;
+      if (row < rows && (!together || wave == 0)) {
+        const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        const float out[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
+        const int token = token0 + (a.pairs_a_token == 1 ? row / op.heads : 0);
+        const int head = a.pairs_a_token == 1 ? row % op.heads : pair % a.pairs_a_token * part_rows + row;
+        StoreValues<TYPE, 4>(op.out, token * op.out_token_stride + head * op.out_head_stride + 16 * block + 4 * quarter, out);
+      }
+    }
   }
 }
 
@@ -714,7 +745,7 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
     static bool sized = false;
     if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kFew>), kLds, &sized)) return;
     hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(groups), dim3(G::kThreads), kLds, s, a);
-    hipLaunchKernelGGL((LatentJoinKernel<kType, kR>), dim3(groups, rows / 16, kR / (64 * kJoinBlocks)), dim3(256), 0, s, a, rows, groups);
+    hipLaunchKernelGGL((LatentJoinKernel<kType, kR>), dim3(groups, kJoinGroups), dim3(256), 0, s, a, rows, groups);
   });
   return LaunchStatus("latent_attend");
 }
