@@ -11,14 +11,11 @@
 //              waves the same ring of tiles.
 // Both products take the tile from LDS as it lies. A product's rows are tokens in an order that leaves a lane with consecutive tokens of one row, in the
 // order in which the second product takes them; the values' columns come by transposing reads.
-//
-// All tiles of all rows lie on one line, a request's after the other's, that the workgroups cut evenly, so that one long request and many short ones fill
-// the device alike; what is cut is joined by a second launch. The line is counted in tokens, kVisit more for a (request, rows) pair's beginning.
+// The work is cut evenly over the workgroups (latent_line.h).
 #include <algorithm>
 #include <cmath>
 
-#include "latent.h"
-#include "paged_attend.h"
+#include "latent_line.h"
 
 namespace llmp_hip {
 namespace {
@@ -26,17 +23,11 @@ namespace {
 constexpr int kTokens = 32;  // a tile's
 constexpr int kFewRows = 16, kManyRows = 128;
 constexpr int kLdsBytes = 160 * 1024;
-constexpr int kVisit = 64;                         // what a pair's beginning and end cost, in tokens
 constexpr int kLeastFew = 256, kLeastMany = 128;  // of the line, to a workgroup: finer parts cost more to write and to join
-
-// The running maximum follows once it is kFollow (log2) behind; weights stay kUp above it, for F16's range.
-constexpr float kUp = 8.0f, kFollow = 6.0f;
 
 struct LatentArgs {
   llmp_latent_attend op;
-  float* values;   // [2 * workgroups][rows][width]
-  float* numbers;  // [2 * workgroups][rows][2]: maximum, sum
-  int32_t* parts;  // [2 * workgroups][4]: request, pair, rows, first row of the call's
+  LatentParts parts;
   int most_length, least;
   int tokens_a_pair, pairs_a_token;  // rows of several whole tokens, or of part of one
 };
@@ -68,26 +59,9 @@ struct LatentGeo {
   }
 };
 
-// ---- a request's pairs on the line.
-struct Line {
-  int start, n, length, base;  // PagedRequest's
-  int groups;                  // of tokens_a_pair tokens
-};
-__device__ __forceinline__ Line LineOf(const LatentArgs& a, int r) {
+__device__ __forceinline__ LatentRequest AttendRequest(const LatentArgs& a, int r) {
   const PagedRequest q = RequestOf(a.op.starts, a.op.lengths, a.op.before, r, a.op.tokens, a.most_length);
   return {q.start, q.n, q.length, q.base, (q.n + a.tokens_a_pair - 1) / a.tokens_a_pair};
-}
-// The tokens that group k's last token sees.
-__device__ __forceinline__ int SeenOf(const LatentArgs& a, const Line& l, int k) {
-  return max(min(l.base + min((k + 1) * a.tokens_a_pair, l.n), l.length), 0);
-}
-// The line before group k: the sum of min(base + (i + 1) t, most), none below 0, over i < k, and the visits; all pairs of a group.
-__device__ __forceinline__ int64_t LengthBefore(const LatentArgs& a, const Line& l, int k) {
-  const int64_t t = a.tokens_a_pair, most = max(min(l.length, l.base + l.n), 0);
-  const int64_t low = l.base < 0 ? min(static_cast<int64_t>(k), -static_cast<int64_t>(l.base) / t) : 0;
-  const int64_t high = max(low, min(static_cast<int64_t>(k), most > l.base ? (most - l.base) / t : 0));
-  const int64_t risen = (high - low) * l.base + t * ((high * (high + 1) - low * (low + 1)) / 2);
-  return (risen + (k - high) * most + static_cast<int64_t>(k) * kVisit) * a.pairs_a_token;
 }
 
 template <int TYPE, int R, int P, bool EIGHT, bool FEW>
@@ -97,7 +71,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
   typedef typename S::Eight Eight;
   constexpr int kSteps = R / 32, kRopeSteps = P / 32, kBlocks = R / 16;
   constexpr int kLogits = 8;  // a lane's of a tile
-  constexpr int kKeyGroup = FEW ? 8 : 3, kValueGroup = FEW ? 8 : 3;  // products that are read for at a time
+  constexpr int kKeyGroup = FEW ? 8 : 2, kValueGroup = FEW ? 8 : 2;  // products that are read for at a time
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const llmp_latent_attend& op = a.op;
   const llmp_latent_cache& c = op.cache;
@@ -107,84 +81,37 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
   const uint32_t ring_off = FEW ? wave * G::kRing * G::kTile : 0;
   const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + ring_off;
 
-  // ---- this workgroup's part of the line: every wave adds the requests up, a lane a request.
-  const auto wave_sums = [&](int64_t v) {  // inclusive
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) {
-      const int64_t up = __shfl_up(v, m);
-      v += lane >= m ? up : 0;
-    }
-    return v;
-  };
-  const auto last_of = [](int64_t v) {
-    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(v), kWave - 1);
-    return static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), kWave - 1)) << 32 | low;
-  };
-  const auto request_length = [&](int r) {
-    if (r >= op.requests) return static_cast<int64_t>(0);
-    const Line l = LineOf(a, r);
-    return LengthBefore(a, l, l.groups);
-  };
-  int64_t total = 0;
-  for (int r0 = 0; r0 < op.requests; r0 += kWave) total += last_of(wave_sums(request_length(r0 + lane)));
-  const int64_t per = max((total + groups - 1) / groups, static_cast<int64_t>(a.least));
-  int64_t u = w * per;
-  const int64_t u_end = min(u + per, total);
-  if (tid < 2) a.parts[(2 * w + tid) * 4] = -1;
+  // ---- this workgroup's run of the line
+  const int64_t t = a.tokens_a_pair;
+  if (tid < 2) a.parts.which[(2 * w + tid) * 4] = -1;
+  const LatentRun run = RunOf(op.requests, w, groups, a.least, [&](int r) {
+    const LatentRequest l = AttendRequest(a, r);
+    return LineBefore(l, t, l.groups) * a.pairs_a_token;
+  });
+  int64_t u = run.from, before = run.before;
+  const int64_t u_end = run.to;
   if (u >= u_end) return;
-  int request = 0;
-  int64_t before = 0;  // the line before the request
-  for (int r0 = 0; r0 < op.requests; r0 += kWave) {
-    const int64_t mine = request_length(r0 + lane), upto = before + wave_sums(mine);
-    const int passed = __popcll(__ballot(upto <= u));
-    if (passed < kWave) {
-      const int64_t from = upto - mine;
-      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(from), passed);
-      before = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(from >> 32), passed)) << 32 | low;
-      request = r0 + passed;
-      break;
-    }
-    before = last_of(upto);
-  }
 
-  const auto scalar = [](auto v) {
-    static_assert(sizeof(v) == 4, "32 bits");
-    return __builtin_bit_cast(decltype(v), __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
-  };
-  const float sign_scale = scalar(fabsf(op.scale) * kLog2E);
+  const float sign_scale = Scalar(fabsf(op.scale) * kLog2E);
   const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
 
-  for (; u < u_end; ++request) {
-    Line l = LineOf(a, request);
-    l = {scalar(l.start), scalar(l.n), scalar(l.length), scalar(l.base), scalar(l.groups)};
-    const int64_t all = LengthBefore(a, l, l.groups);
+  for (int request = run.request; u < u_end; ++request) {
+    const LatentRequest l = Scalar(AttendRequest(a, request));
+    const int64_t all = LineBefore(l, t, l.groups) * a.pairs_a_token;
     if (u >= before + all) {
       before += all;
       continue;
     }
-    // The group that holds u: the last that begins at or before it.
-    int k = 0, k_high = l.groups;
-    while (k_high - k > 1) {
-      const int mid = (k + k_high) / 2;
-      if (before + LengthBefore(a, l, mid) <= u) {
-        k = mid;
-      } else {
-        k_high = mid;
-      }
-    }
-    for (; k < l.groups && u < u_end; ++k) {
-      const int seen = SeenOf(a, l, k), whole = seen + kVisit;
-      const int64_t group_from = before + LengthBefore(a, l, k);
+    for (int k = GroupAt(l, t, (u - before) / a.pairs_a_token); k < l.groups && u < u_end; ++k) {
+      const int seen = SeenOf(l, a.tokens_a_pair, k), whole = seen + kVisit;
+      const int64_t group_from = before + LineBefore(l, t, k) * a.pairs_a_token;
       for (int part = static_cast<int>((u - group_from) / whole); part < a.pairs_a_token && u < u_end; ++part) {
         const int64_t from = group_from + static_cast<int64_t>(part) * whole;
         const int x0 = static_cast<int>(u - from), x1 = static_cast<int>(min(u_end - from, static_cast<int64_t>(whole)));
         u = from + x1;
-        // Tiles whose first token lies in [x0, x1) - kVisit.
-        const int tiles = (seen + kTokens - 1) / kTokens;
-        const int tile_from = (max(x0 - kVisit, 0) + kTokens - 1) / kTokens;
-        const int tile_to = x1 == whole ? tiles : (max(x1 - kVisit, 0) + kTokens - 1) / kTokens;
-        const bool begins = tile_from == 0 && (tile_to > 0 || x0 == 0), ends = tile_to == tiles;
-        if (tiles == 0 ? x0 != 0 : tile_from >= tile_to) continue;
+        const LatentPiece piece = PieceOf(seen, kTokens, x0, x1);
+        if (!piece.any) continue;
+        const int tile_from = piece.from, tile_to = piece.to;
 
         // ---- the lane's row.
         const int first_token = k * a.tokens_a_pair;
@@ -266,7 +193,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           const uint8_t* const latent_b = static_cast<const uint8_t*>(c.latent) + static_cast<int64_t>(row_b) * G::kPitch;
           const uint8_t* const rope_a = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_a) * G::kRopePitch;
           const uint8_t* const rope_b = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_b) * G::kRopePitch;
-          const uint32_t to = scalar(ring_at + slot * G::kTile);
+          const uint32_t to = Scalar(ring_at + slot * G::kTile);
           // (Lanes and waves as something new at every tile: the compiler otherwise keeps every load's offsets, and then spills them.)
           int lane_now = lane, wave_now = FEW ? 0 : wave;
           asm volatile("" : "+v"(lane_now));
@@ -479,7 +406,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             if (i + G::kRing < count) fetch(my_from + (i + G::kRing) * step, i % G::kRing);
           }
         } else {
-          const int count = scalar(tile_to - tile_from);
+          const int count = Scalar(tile_to - tile_from);
           constexpr int kAhead = G::kRing - 1;
           for (int i = 0; i < kAhead && i < count; ++i) fetch(tile_from + i, i);
           const bool early = wave < G::kWaves / 2;
@@ -546,7 +473,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         }
 
         // ---- out, or a part for the join. Element e of a block is dimension 4 quarter + e of it.
-        if (begins && ends) {
+        if (piece.begins && piece.ends) {
           if (busy && real) {
             const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
             const int64_t to = (l.start + token) * op.out_token_stride + head * op.out_head_stride + 16 * first_block + 4 * quarter;
@@ -557,15 +484,15 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             }
           }
         } else {
-          const int which = 2 * w + (begins ? 1 : 0);
+          const int which = 2 * w + (piece.begins ? 1 : 0);
           if (tid == 0) {
-            int32_t* const p = a.parts + 4 * which;
+            int32_t* const p = a.parts.which + 4 * which;
             p[0] = request, p[1] = k * a.pairs_a_token + part, p[2] = rows, p[3] = l.start + first_token;
           }
           if (busy) {
             const int64_t rows16 = static_cast<int64_t>(which) * (G::kRows / 16) + row0 / 16;
-            if (quarter == 0) reinterpret_cast<float2*>(a.numbers)[rows16 * 16 + column] = make_float2(top, sum);
-            F32x4* const to = reinterpret_cast<F32x4*>(a.values) + (rows16 * kBlocks + first_block) * kWave + lane;
+            if (quarter == 0) a.parts.numbers[rows16 * 16 + column] = make_float2(top, sum);
+            F32x4* const to = reinterpret_cast<F32x4*>(a.parts.values) + (rows16 * kBlocks + first_block) * kWave + lane;
 #pragma unroll
             for (int b = 0; b < kMine; ++b) to[b * kWave] = result[b];
           }
@@ -573,85 +500,6 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
       }
     }
     before += all;
-  }
-}
-
-// The parts of a pair, joined, as they lie: an item is 16 rows by 16 dimensions, a lane four values of a row. The pair's items are dealt to the workgroups
-// (of this launch, kJoinGroups for each of the first one's) that hold its parts, so that what one reads is about the same whatever the number of parts. A wave takes an
-// item, or where there are many parts a workgroup one together, a wave every fourth part. (One wave an item: 256 parts of a pair 180 us.)
-constexpr int kJoinGroups = 8, kJoinAlone = 16;
-template <int TYPE, int R>
-__global__ __launch_bounds__(256) void LatentJoinKernel(const LatentArgs a, int part_rows, int groups) {
-  constexpr int kBlocks = R / 16;
-  __shared__ F32x4 met[3][kWave];
-  __shared__ float met_sums[3][kWave];
-  const llmp_latent_attend& op = a.op;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, column = lane % 16, quarter = lane / 16;
-  const int x = blockIdx.x;
-  // This workgroup's parts: its pair's later one (0), its pair's first one (1).
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const int32_t* const mine = a.parts + 8 * x + 4 * which;
-    const int request = mine[0], pair = mine[1], rows = mine[2], token0 = mine[3];
-    if (request < 0) continue;
-    int leader = x;
-    if (which == 0) {  // the last workgroup before this one that begins a pair has begun this one
-      for (int base = x - 1;; base -= kWave) {
-        const int g = base - lane;
-        const uint64_t begins = __ballot(g >= 0 && a.parts[8 * max(g, 0) + 4] >= 0);
-        leader = base - (__ffsll(static_cast<unsigned long long>(begins)) - 1);
-        if (begins != 0 || base < kWave) break;
-      }
-    }
-    // The parts after the first are the next workgroups' first ones, as long as they are of this pair.
-    int count = 1;
-    for (int base = leader + 1;; base += kWave) {
-      const int g = base + lane;
-      const bool same = g < groups && a.parts[8 * min(g, groups - 1)] == request && a.parts[8 * min(g, groups - 1) + 1] == pair;
-      const uint64_t not_same = ~__ballot(same);
-      const int here = not_same == 0 ? kWave : __ffsll(static_cast<unsigned long long>(not_same)) - 1;
-      count += here;
-      if (here < kWave) break;
-    }
-    const auto rows16 = [&](int i, int r16) { return static_cast<int64_t>(i == 0 ? 2 * leader + 1 : 2 * (leader + i)) * (part_rows / 16) + r16; };
-    const bool together = count > kJoinAlone;
-    const int items = (rows + 15) / 16 * kBlocks;
-    const int waves = together ? 1 : 4, first = together ? 0 : wave;
-    for (int item = ((x - leader) * kJoinGroups + static_cast<int>(blockIdx.y)) * waves + first; item < items; item += count * kJoinGroups * waves) {
-      const int r16 = item / kBlocks, block = item % kBlocks;
-      float most = -INFINITY;
-      for (int i = quarter; i < count; i += 4) most = fmaxf(most, a.numbers[2 * (rows16(i, r16) * 16 + column)]);
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, __shfl_xor(most, 32));
-      const float less = most == -INFINITY ? 0.0f : most;
-      float sum = 0.0f;
-      F32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-      for (int i = together ? wave : 0; i < count; i += together ? 4 : 1) {
-        const int64_t at = rows16(i, r16);
-        const float2 n = reinterpret_cast<const float2*>(a.numbers)[at * 16 + column];
-        const float by = __builtin_amdgcn_exp2f(n.x - less);
-        sum = fmaf(n.y, by, sum);
-        v += reinterpret_cast<const F32x4*>(a.values)[(at * kBlocks + block) * kWave + lane] * by;
-      }
-      if (together) {
-        if (wave > 0) met[wave - 1][lane] = v, met_sums[wave - 1][lane] = sum;
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-          for (int i = 0; i < 3; ++i) v += met[i][lane], sum += met_sums[i][lane];
-        }
-        __syncthreads();
-      }
-      const int row = 16 * r16 + column;
-      if (row < rows && (!together || wave == 0)) {
-        const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-        const float out[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
-        const int token = token0 + (a.pairs_a_token == 1 ? row / op.heads : 0);
-        const int head = a.pairs_a_token == 1 ? row % op.heads : pair % a.pairs_a_token * part_rows + row;
-        StoreValues<TYPE, 4>(op.out, token * op.out_token_stride + head * op.out_head_stride + 16 * block + 4 * quarter, out);
-      }
-    }
   }
 }
 
@@ -703,8 +551,6 @@ int CheckLatentAttend(const llmp_latent_attend* op, int cus) {
   return 0;
 }
 
-size_t PartsBytes(int groups) { return static_cast<size_t>(2 * groups) * 16; }
-
 }  // namespace
 }  // namespace llmp_hip
 
@@ -712,9 +558,7 @@ using namespace llmp_hip;
 
 extern "C" size_t llmp_hip_latent_attend_scratch(const llmp_latent_attend* op, int cus) {
   if (CheckLatentAttend(op, cus) != 0) return 0;
-  const int groups = cus;
-  const size_t rows = static_cast<size_t>(2 * groups) * RowsOf(*op);
-  return PartsBytes(groups) + rows * 8 + rows * op->cache.width * 4;
+  return LatentPartsBytes(cus, RowsOf(*op), op->cache.width);
 }
 
 extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream) {
@@ -724,16 +568,14 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
     return Refuse(1, "latent_attend: %zu bytes of scratch at a 16-byte boundary, not %zu", need, scratch_bytes);
   const bool few = FewRows(*op);
   const int rows = RowsOf(*op);
-  const int groups = cus;
   LatentArgs a;
   a.op = *op;
-  a.parts = static_cast<int32_t*>(scratch);
-  a.numbers = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + PartsBytes(groups));
-  a.values = a.numbers + static_cast<size_t>(2 * groups) * rows * 2;
+  a.parts = LatentPartsAt(scratch, cus, rows);
   a.most_length = op->table_width * op->cache.page;
   a.least = few ? kLeastFew : kLeastMany;
   a.tokens_a_pair = std::max(1, rows / op->heads);
   a.pairs_a_token = (op->heads + rows - 1) / rows;
+  const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, cus, a.pairs_a_token};
   BeginLaunches();
   const auto s = static_cast<hipStream_t>(stream);
   WithForm(*op, few, [&](auto type, auto r, auto p, auto eight, auto few_rows) {
@@ -744,8 +586,8 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
     constexpr int kLds = G::kLds;
     static bool sized = false;
     if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kFew>), kLds, &sized)) return;
-    hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(groups), dim3(G::kThreads), kLds, s, a);
-    hipLaunchKernelGGL((LatentJoinKernel<kType, kR>), dim3(groups, kJoinGroups), dim3(256), 0, s, a, rows, groups);
+    hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(cus), dim3(G::kThreads), kLds, s, a);
+    hipLaunchKernelGGL((LatentJoinKernel<kType, kR, 16, G::kRows>), dim3(cus, kJoinGroups), dim3(256), 0, s, join);
   });
   return LaunchStatus("latent_attend");
 }

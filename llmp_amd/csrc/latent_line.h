@@ -1,0 +1,214 @@
+// How the attentions over latent vectors cut a call's work evenly: pairs (a request's rows, some at a time, and the keys that they see) lie on one
+// line, a request's after the other's, and every workgroup takes an equal run of it, so that one long request and many short ones fill the device alike.
+// A run's first pair may have begun and its last one end in other workgroups: their parts are joined by a second launch. The line is counted in keys, kVisit more for
+// a pair's beginning; a tile of keys is the workgroup's in whose run its first key lies.
+#ifndef LLMP_AMD_CSRC_LATENT_LINE_H_
+#define LLMP_AMD_CSRC_LATENT_LINE_H_
+
+#include "latent.h"
+#include "paged_attend.h"
+
+namespace llmp_hip {
+
+constexpr int kVisit = 64;  // what a pair's beginning and end cost, in keys
+
+// The running maximum follows once it is kFollow (log2) behind; weights stay kUp above it, for F16's range.
+constexpr float kUp = 8.0f, kFollow = 6.0f;
+
+// Where parts go: a workgroup's later part of a pair that another began (0) and its first part of one that another ends (1).
+struct LatentParts {
+  float* values;    // [2 * workgroups][rows of a pair][width], in the order of the lanes' registers
+  float2* numbers;  // [2 * workgroups][rows of a pair]: maximum, sum
+  int32_t* which;   // [2 * workgroups][4]: request (-1: no part), pair, rows, first row of the call's
+};
+inline size_t LatentPartsBytes(int groups, int rows, int width) { return static_cast<size_t>(2 * groups) * (16 + rows * (8 + 4 * static_cast<size_t>(width))); }
+inline LatentParts LatentPartsAt(void* scratch, int groups, int rows) {
+  LatentParts p;
+  p.which = static_cast<int32_t*>(scratch);
+  p.numbers = reinterpret_cast<float2*>(p.which + static_cast<size_t>(2 * groups) * 4);
+  p.values = reinterpret_cast<float*>(p.numbers + static_cast<size_t>(2 * groups) * rows);
+  return p;
+}
+
+// ---- device: a request's rows in groups of `t` tokens, the first at position `base`; a token sees the keys up to its position, of `length`.
+struct LatentRequest {
+  int start, n, length, base;  // PagedRequest's
+  int groups;
+};
+// What group k's last token sees.
+__device__ __forceinline__ int SeenOf(const LatentRequest& l, int t, int k) { return max(min(l.base + min((k + 1) * t, l.n), l.length), 0); }
+// The line before group k, of one pair a group: the sum of min(base + (i + 1) t, most), none below 0, over i < k, and the visits.
+__device__ __forceinline__ int64_t LineBefore(const LatentRequest& l, int64_t t, int k) {
+  const int64_t most = max(min(l.length, l.base + l.n), 0);
+  const int64_t low = l.base < 0 ? min(static_cast<int64_t>(k), -static_cast<int64_t>(l.base) / t) : 0;
+  const int64_t high = max(low, min(static_cast<int64_t>(k), most > l.base ? (most - l.base) / t : 0));
+  const int64_t risen = (high - low) * l.base + t * ((high * (high + 1) - low * (low + 1)) / 2);
+  return risen + (k - high) * most + static_cast<int64_t>(k) * kVisit;
+}
+// The last group that begins at or before `u`.
+__device__ __forceinline__ int GroupAt(const LatentRequest& l, int64_t t, int64_t u) {
+  int k = 0, above = l.groups;
+  while (above - k > 1) {
+    const int mid = (k + above) / 2;
+    if (LineBefore(l, t, mid) <= u) {
+      k = mid;
+    } else {
+      above = mid;
+    }
+  }
+  return k;
+}
+
+// Every wave by itself, a lane a request: length_of(r) is a request's of the line. The run [from, to) of this workgroup (`index` of `groups`), the request that
+// holds its beginning, and the line before that.
+struct LatentRun {
+  int64_t from, to, before;
+  int request;
+};
+template <class LengthOf>
+__device__ __forceinline__ LatentRun RunOf(int requests, int index, int groups, int64_t least, const LengthOf& length_of) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const auto sums = [&](int64_t v) {  // inclusive
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      const int64_t up = __shfl_up(v, m);
+      v += lane >= m ? up : 0;
+    }
+    return v;
+  };
+  const auto from_lane = [](int64_t v, int l) {
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(v), l);
+    return static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l)) << 32 | low;
+  };
+  // (The first 64 requests' lengths are kept: most calls have no more.)
+  const int64_t first = lane < requests ? length_of(lane) : 0, first_upto = sums(first);
+  int64_t total = from_lane(first_upto, kWave - 1);
+  for (int r0 = kWave; r0 < requests; r0 += kWave) total += from_lane(sums(r0 + lane < requests ? length_of(r0 + lane) : 0), kWave - 1);
+  const int64_t per = max((total + groups - 1) / groups, least);
+  LatentRun run = {index * per, min((index + 1) * per, total), 0, 0};
+  if (run.from >= run.to) return run;
+  for (int r0 = 0; r0 < requests; r0 += kWave) {
+    const int64_t mine = r0 == 0 ? first : r0 + lane < requests ? length_of(r0 + lane) : 0;
+    const int64_t upto = run.before + (r0 == 0 ? first_upto : sums(mine));
+    const int passed = __popcll(__ballot(upto <= run.from));
+    if (passed < kWave) {
+      run.before = from_lane(upto - mine, passed);
+      run.request = r0 + passed;
+      break;
+    }
+    run.before = from_lane(upto, kWave - 1);
+  }
+  return run;
+}
+
+// What of a pair that sees `seen` keys lies in [x0, x1) of its kVisit + seen: tiles [from, to) of `tile` keys, whether they are its first and its last. A pair
+// that sees nothing is its beginning's.
+struct LatentPiece {
+  int from, to;
+  bool begins, ends, any;
+};
+__device__ __forceinline__ LatentPiece PieceOf(int seen, int tile, int x0, int x1) {
+  const int tiles = (seen + tile - 1) / tile;
+  LatentPiece p;
+  p.from = (max(x0 - kVisit, 0) + tile - 1) / tile;
+  p.to = x1 == seen + kVisit ? tiles : (max(x1 - kVisit, 0) + tile - 1) / tile;
+  p.begins = p.from == 0 && (p.to > 0 || x0 == 0);
+  p.ends = p.to == tiles;
+  p.any = tiles == 0 ? x0 == 0 : p.from < p.to;
+  return p;
+}
+
+template <class T>
+__device__ __forceinline__ T Scalar(T v) {
+  static_assert(sizeof(T) == 4, "32 bits");
+  return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+__device__ __forceinline__ LatentRequest Scalar(const LatentRequest& l) { return {Scalar(l.start), Scalar(l.n), Scalar(l.length), Scalar(l.base), Scalar(l.groups)}; }
+
+// ---- the parts of a pair, joined. They are as the lanes held them: an item is UNIT rows by 256 / UNIT dimensions, lane l four of them, 4 (l / UNIT) on, of row
+// l % UNIT. The pair's items are dealt to the workgroups (of this launch, kJoinGroups for each of the first one's) that hold its parts, so that what one reads is
+// about the same whatever the number of parts. A wave takes an item, or where there are many parts a workgroup one together, a wave every fourth part.
+// (One wave an item: 256 parts of 128 rows of 512 values 180 us, 16 so.)
+constexpr int kJoinGroups = 8, kJoinAlone = 16;
+struct JoinArgs {
+  LatentParts parts;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  int heads, groups;
+  int pairs_a_token;  // 0: a pair is `heads`' of them: rows are tokens; 1: rows are (token, head); more: rows are heads
+};
+template <int TYPE, int WIDTH, int UNIT, int ROWS>
+__global__ __launch_bounds__(256) void LatentJoinKernel(const JoinArgs a) {
+  constexpr int kItemValues = 256 / UNIT, kBlocks = WIDTH / kItemValues;
+  __shared__ F32x4 met[3][kWave];
+  __shared__ float met_sums[3][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, column = lane % UNIT, part_of = lane / UNIT;
+  const int x = blockIdx.x;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int32_t* const mine = a.parts.which + 8 * x + 4 * which;
+    const int request = mine[0], pair = mine[1], rows = mine[2], token0 = mine[3];
+    if (request < 0) continue;
+    int leader = x;
+    if (which == 0) {  // the last workgroup before this one that begins a pair has begun this one
+      for (int base = x - 1;; base -= kWave) {
+        const int g = base - lane;
+        const uint64_t begins = __ballot(g >= 0 && a.parts.which[8 * max(g, 0) + 4] >= 0);
+        leader = base - (__ffsll(static_cast<unsigned long long>(begins)) - 1);
+        if (begins != 0 || base < kWave) break;
+      }
+    }
+    // The parts after the first are the next workgroups' later ones, as long as they are of this pair.
+    int count = 1;
+    for (int base = leader + 1;; base += kWave) {
+      const int g = base + lane, at = 8 * min(g, a.groups - 1);
+      const uint64_t others = ~__ballot(g < a.groups && a.parts.which[at] == request && a.parts.which[at + 1] == pair);
+      const int here = others == 0 ? kWave : __ffsll(static_cast<unsigned long long>(others)) - 1;
+      count += here;
+      if (here < kWave) break;
+    }
+    const auto unit = [&](int i, int u) { return static_cast<int64_t>(i == 0 ? 2 * leader + 1 : 2 * (leader + i)) * (ROWS / UNIT) + u; };
+    const bool together = count > kJoinAlone;
+    const int items = (rows + UNIT - 1) / UNIT * kBlocks;
+    const int waves = together ? 1 : 4;
+    for (int item = ((x - leader) * kJoinGroups + static_cast<int>(blockIdx.y)) * waves + (together ? 0 : wave); item < items; item += count * kJoinGroups * waves) {
+      const int u = item / kBlocks, block = item % kBlocks;
+      float most = -INFINITY;
+      for (int i = part_of; i < count; i += kWave / UNIT) most = fmaxf(most, a.parts.numbers[unit(i, u) * UNIT + column].x);
+#pragma unroll
+      for (int m = UNIT; m < kWave; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+      const float less = most == -INFINITY ? 0.0f : most;
+      float sum = 0.0f;
+      F32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+      for (int i = together ? wave : 0; i < count; i += together ? 4 : 1) {
+        const int64_t at = unit(i, u);
+        const float2 n = a.parts.numbers[at * UNIT + column];
+        const float by = __builtin_amdgcn_exp2f(n.x - less);
+        sum = fmaf(n.y, by, sum);
+        v += reinterpret_cast<const F32x4*>(a.parts.values)[(at * kBlocks + block) * kWave + lane] * by;
+      }
+      if (together) {
+        if (wave > 0) met[wave - 1][lane] = v, met_sums[wave - 1][lane] = sum;
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+          for (int i = 0; i < 3; ++i) v += met[i][lane], sum += met_sums[i][lane];
+        }
+        __syncthreads();
+      }
+      const int row = UNIT * u + column;
+      if (row < rows && (!together || wave == 0)) {
+        const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        const float out[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
+        const int token = token0 + (a.pairs_a_token == 0 ? row : a.pairs_a_token == 1 ? row / a.heads : 0);
+        const int head = a.pairs_a_token == 0 ? pair % a.heads : a.pairs_a_token == 1 ? row % a.heads : pair % a.pairs_a_token * ROWS + row;
+        StoreValues<TYPE, 4>(a.out, token * a.out_token_stride + head * a.out_head_stride + kItemValues * block + 4 * part_of, out);
+      }
+    }
+  }
+}
+
+}  // namespace llmp_hip
+
+#endif  // LLMP_AMD_CSRC_LATENT_LINE_H_

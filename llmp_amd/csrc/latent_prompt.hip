@@ -6,43 +6,45 @@
 // pass no register, the next tile under this one's work:
 //   S^T = K Q^T, P = exp2(S - E), O^T += V^T P^T, all by 32 x 32 products.
 // Row 8a + 4h + b of the first product is key 16h + 4a + b of its 32, so that a lane (half h) ends with 16 keys in order of one row, which is what the
-// second product takes; V's columns come by transposing reads. Where rows are few for the device, the keys are cut in equal runs, and a
-// second launch joins them.
+// second product takes; V's columns come by transposing reads.
+//
+// Where no request's rows can see more keys than a workgroup's share of the whole, a workgroup takes (head, 128 rows) pairs whole, one a launch's block, a head's on one
+// chiplet, the longest first. Elsewhere the pairs' keys are cut evenly (latent_line.h).
 #include <algorithm>
 #include <cmath>
 
-#include "latent.h"
-#include "paged_attend.h"
+#include "latent_line.h"
 
 namespace llmp_hip {
 namespace {
 
 constexpr int kKeys = 64;  // a tile's
 constexpr int kPromptRows = 128, kPromptThreads = 256;
-constexpr float kUp = 8.0f, kFollow = 6.0f;  // log2: as in latent_attend.hip
-constexpr int kMostRuns = 64;
+constexpr int kAUnit = 2;                            // workgroups a compute unit
+constexpr int kLeast = 256;                          // of the line, to a workgroup: finer parts cost more to write and to join
 
 struct PromptArgs {
   llmp_latent_prompt op;
-  float* values;   // [runs][row tiles of all][kPromptRows][value]
-  float* numbers;  // [runs][row tiles of all][kPromptRows][2]: maximum, sum
-  int tiles;       // row tiles a request, at most
-  int runs;        // that a row tile's keys are cut into
+  LatentParts parts;
+  int tiles;  // row tiles a request, at most
 };
 
 // A request's rows of q and its keys, none where the arrays name rows outside the call's.
 struct PromptRequest {
-  int start, n, key_start, keys;
+  LatentRequest l;
+  int key_start;
 };
 __device__ __forceinline__ PromptRequest PromptOf(const llmp_latent_prompt& op, int r) {
   PromptRequest q;
-  q.start = op.starts[r];
+  q.l.start = op.starts[r];
   const int end = op.starts[r + 1];
-  q.n = q.start >= 0 && end > q.start && end <= op.tokens ? end - q.start : 0;
+  q.l.n = q.l.start >= 0 && end > q.l.start && end <= op.tokens ? end - q.l.start : 0;
   const int32_t* const keys = op.key_starts != nullptr ? op.key_starts : op.starts;
   q.key_start = keys[r];
   const int key_end = keys[r + 1];
-  q.keys = q.key_start >= 0 && key_end > q.key_start && key_end <= op.keys ? key_end - q.key_start : 0;
+  q.l.length = q.key_start >= 0 && key_end > q.key_start && key_end <= op.keys ? key_end - q.key_start : 0;
+  q.l.base = q.l.length - q.l.n;
+  q.l.groups = (q.l.n + kPromptRows - 1) / kPromptRows;
   return q;
 }
 
@@ -65,49 +67,84 @@ struct PromptGeo {
   static constexpr int kKeyBytes = kKeys * kKeyPitch, kRopeBytes = kKeys * kRopePitch, kValueBytes = kKeys * kValuePitch;
   static constexpr int kTile = kKeyBytes + kRopeBytes + kValueBytes;
   static constexpr int kRing = 2;
+  static constexpr int kKeyLoads = kKeyBytes / 4096, kRopeLoads = kRopeBytes / 4096, kValueLoads = kValueBytes / 4096;  // a wave's
   static constexpr int kLds = kRing * kTile;
 };
 
-// grid: row tiles, requests and heads and runs in an order that keeps a head's row tiles on one chiplet, the longest first.
-template <int TYPE, int N, int P>
-__global__ __launch_bounds__(kPromptThreads, 2) void LatentPromptKernel(const PromptArgs a) {
+// LINE: the grid is the device's, each workgroup a run of the line; else a block a (request, head, row tile).
+template <int TYPE, int N, int P, bool LINE>
+__global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(const PromptArgs a) {
   using G = PromptGeo<N, P>;
   using S = Sixteen<TYPE>;
   typedef typename S::Eight Eight;
   constexpr int kSteps = N / 16, kRopeSteps = P / 16, kBlocks = N / 32;
+  constexpr int kKeyGroup = 4, kValueGroup = 4;  // products that are read for at a time
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const llmp_latent_prompt& op = a.op;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int half = lane / 32, column = lane % 32;
   const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
+  const float worth = Scalar(fabsf(op.scale) * kLog2E);
 
-  // Eight workgroups in a row go to eight chiplets: a chiplet takes every eighth (run, head, request).
-  const uint32_t index = blockIdx.x, turn = index / 8;
-  const uint32_t set = turn / a.tiles * 8 + index % 8;
-  const int tile_index = a.tiles - 1 - static_cast<int>(turn % a.tiles);
-  const uint32_t request_head = set / a.runs;
-  const int run = static_cast<int>(set % a.runs);
-  if (request_head >= static_cast<uint32_t>(op.requests) * op.heads) return;
-  const int request = request_head / op.heads, head = request_head % op.heads;
-  const PromptRequest r = PromptOf(op, request);
-  const int first = tile_index * kPromptRows;
-  if (first >= r.n) return;
-
+  // Eight workgroups in a row go to eight chiplets: a chiplet takes every eighth (request, head), or an eighth of the line.
+  const int groups = gridDim.x;
+  const int index = LINE ? static_cast<int>(blockIdx.x % 8) * (groups / 8) + static_cast<int>(blockIdx.x / 8) : 0;
+  int request, head = 0, k = 0;
+  int64_t u = 0, u_end = 1, before = 0;
+  if constexpr (LINE) {
+    if (tid < 2) a.parts.which[(2 * index + tid) * 4] = -1;
+    const LatentRun run = RunOf(op.requests, index, groups, kLeast, [&](int r) {
+      const LatentRequest l = PromptOf(op, r).l;
+      return LineBefore(l, kPromptRows, l.groups) * op.heads;
+    });
+    u = run.from, u_end = run.to, before = run.before, request = run.request;
+  } else {
+    const uint32_t turn = blockIdx.x / 8, set = turn / a.tiles * 8 + blockIdx.x % 8;
+    if (set >= static_cast<uint32_t>(op.requests) * op.heads) return;
+    request = set / op.heads, head = set % op.heads, k = a.tiles - 1 - static_cast<int>(turn % a.tiles);
+  }
+  for (; u < u_end;) {
+  // ---- the next pair, or part of one.
+  PromptRequest r = PromptOf(op, request);
+  r = {Scalar(r.l), Scalar(r.key_start)};
+  LatentPiece piece = {};
+  int any_to;
+  if constexpr (LINE) {
+    const int64_t a_head = LineBefore(r.l, kPromptRows, r.l.groups);
+    if (u >= before + a_head * op.heads) {
+      before += a_head * op.heads;
+      ++request;
+      continue;
+    }
+    head = static_cast<int>((u - before) / a_head);
+    const int64_t head_from = before + head * a_head;
+    k = GroupAt(r.l, kPromptRows, u - head_from);
+    any_to = SeenOf(r.l, kPromptRows, k);
+    const int64_t from = head_from + LineBefore(r.l, kPromptRows, k);
+    const int x0 = static_cast<int>(u - from), x1 = static_cast<int>(min(u_end - from, static_cast<int64_t>(any_to + kVisit)));
+    u = from + x1;
+    piece = PieceOf(any_to, kKeys, x0, x1);
+    if (!piece.any) continue;
+  } else {
+    u = u_end;
+    if (k >= r.l.groups) return;
+    any_to = SeenOf(r.l, kPromptRows, k);
+    piece = {0, (any_to + kKeys - 1) / kKeys, true, true, true};
+  }
+  head = Scalar(head), k = Scalar(k);
+  const int tile_from = Scalar(piece.from), tile_to = Scalar(piece.to);
+  const int first = k * kPromptRows, base = r.l.base;
   const int row = first + wave * 32 + column;
-  const bool real = row < r.n, busy = first + wave * 32 < r.n;
+  const bool real = row < r.l.n, busy = first + wave * 32 < r.l.n;
   const int token = real ? row : first;
-  const int base = r.keys - r.n;  // the first query's position
   const int see_to = real ? max(base + row + 1, 0) : 0;
-  const int all_to = max(base + first + wave * 32 + 1, 0);        // seen by all of the wave's rows
-  const int all_rows_to = max(base + first + 1, 0);               // of the workgroup's
-  const int any_to = max(base + min(first + kPromptRows, r.n), 0);  // seen by any
-  const int tiles = (any_to + kKeys - 1) / kKeys;
-  const int tile_from = static_cast<int>(static_cast<int64_t>(tiles) * run / a.runs), tile_to = static_cast<int>(static_cast<int64_t>(tiles) * (run + 1) / a.runs);
+  const int all_to = max(base + first + wave * 32 + 1, 0);  // seen by all of the wave's rows
+  const int all_rows_to = max(base + first + 1, 0);         // of the workgroup's
 
   Eight q[kSteps + kRopeSteps];
   {
-    const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
-    const uint16_t* const from = static_cast<const uint16_t*>(op.q) + static_cast<int64_t>(r.start + token) * op.q_token_stride + head * op.q_head_stride + 8 * half;
+    const uint16_t* const from = static_cast<const uint16_t*>(op.q) + static_cast<int64_t>(r.l.start + token) * op.q_token_stride + head * op.q_head_stride + 8 * half;
 #pragma unroll
     for (int x = 0; x < kSteps + kRopeSteps; ++x) {
       U32x4 v = *reinterpret_cast<const U32x4*>(from + 16 * x);
@@ -115,7 +152,6 @@ __global__ __launch_bounds__(kPromptThreads, 2) void LatentPromptKernel(const Pr
       q[x] = __builtin_bit_cast(Eight, v);
     }
   }
-  const float worth = fabsf(op.scale) * kLog2E;
   F32x16 out[kBlocks];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
@@ -124,24 +160,44 @@ __global__ __launch_bounds__(kPromptThreads, 2) void LatentPromptKernel(const Pr
   }
   float top = -INFINITY, sum = 0.0f;
 
-  const auto fetch = [&](int tile, int slot) {
-    const uint32_t to = lds_at + slot * G::kTile;
-    int lane_now = lane;
-    asm volatile("" : "+v"(lane_now));  // (as something new: the compiler otherwise keeps every load's place)
-    const auto part = [&](auto pitch, auto is_value, uint32_t area, const void* rows, int64_t stride) {
-      constexpr int kPitch = decltype(pitch)::value, kLanes = kPitch / 16, kRowsALoad = kWave / kLanes, kCount = kKeys / kRowsALoad / 4;
+  // A lane's places in a tile's rows, for every load of the wave's (row strides stay below 2^24 values: the host looks). A load's rows follow the one's
+  // before it.
+  uint32_t k_places[G::kKeyLoads], r_places[G::kRopeLoads], v_places[G::kValueLoads];
+  const auto place = [&](auto pitch, auto turn, uint32_t* places, int count, int64_t stride) {
+    constexpr int kLanes = decltype(pitch)::value / 16, kRowsALoad = kWave / kLanes;
 #pragma unroll
-      for (int i = 0; i < kCount; ++i) {
-        const int n = wave * kCount + i, in = n * kRowsALoad + lane_now / kLanes;
-        const int turned = decltype(is_value)::value ? ValueTurn<kPitch>(in) : KeyTurn<kPitch>(in);
-        const int key = min(tile * kKeys + in, r.keys - 1);  // (past the last one: the last one again)
-        const uint16_t* const from = static_cast<const uint16_t*>(rows) + static_cast<int64_t>(r.key_start + key) * stride + 8 * ((lane_now % kLanes) ^ turned);
-        LaneLineToLds(from, to + area + 1024 * n);
+    for (int i = 0; i < count; ++i) {
+      const int in = (wave * count + i) * kRowsALoad + lane / kLanes;
+      places[i] = static_cast<uint32_t>(in) * static_cast<uint32_t>(2 * stride) + 16 * ((lane % kLanes) ^ turn(in));
+    }
+  };
+  place(std::integral_constant<int, G::kKeyPitch>{}, KeyTurn<G::kKeyPitch>, k_places, G::kKeyLoads, op.k_token_stride);
+  place(std::integral_constant<int, G::kRopePitch>{}, KeyTurn<G::kRopePitch>, r_places, G::kRopeLoads, op.k_rope_token_stride);
+  place(std::integral_constant<int, G::kValuePitch>{}, ValueTurn<G::kValuePitch>, v_places, G::kValueLoads, op.v_token_stride);
+  const uint16_t* const k_base = static_cast<const uint16_t*>(op.k) + head * op.k_head_stride;
+  const uint16_t* const r_base = static_cast<const uint16_t*>(op.k_rope);
+  const uint16_t* const v_base = static_cast<const uint16_t*>(op.v) + head * op.v_head_stride;
+  const auto fetch = [&](int tile, int slot) {
+    const int64_t key = r.key_start + static_cast<int64_t>(tile) * kKeys;
+    const int left = r.l.length - tile * kKeys;  // at least one; past them the last one again
+    const auto part = [&](auto pitch, const uint32_t* places, int count, uint32_t area, const uint16_t* rows, int64_t stride) {
+      constexpr int kLanes = decltype(pitch)::value / 16, kRowsALoad = kWave / kLanes;
+      const uint16_t* const from = rows + key * stride;
+      const uint32_t to = Scalar(lds_at + slot * G::kTile + area + 1024 * wave * count);
+      if (left >= kKeys) {
+#pragma unroll
+        for (int i = 0; i < count; ++i) LineToLds(from, places[i], to + 1024 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < count; ++i) {
+          const int in = (wave * count + i) * kRowsALoad + lane / kLanes;
+          LineToLds(from, places[i] - static_cast<uint32_t>(max(in - left + 1, 0)) * static_cast<uint32_t>(2 * stride), to + 1024 * i);
+        }
       }
     };
-    part(std::integral_constant<int, G::kKeyPitch>{}, std::false_type{}, 0, static_cast<const uint16_t*>(op.k) + head * op.k_head_stride, op.k_token_stride);
-    part(std::integral_constant<int, G::kRopePitch>{}, std::false_type{}, G::kKeyBytes, op.k_rope, op.k_rope_token_stride);
-    part(std::integral_constant<int, G::kValuePitch>{}, std::true_type{}, G::kKeyBytes + G::kRopeBytes, static_cast<const uint16_t*>(op.v) + head * op.v_head_stride, op.v_token_stride);
+    part(std::integral_constant<int, G::kKeyPitch>{}, k_places, G::kKeyLoads, 0, k_base, op.k_token_stride);
+    part(std::integral_constant<int, G::kRopePitch>{}, r_places, G::kRopeLoads, G::kKeyBytes, r_base, op.k_rope_token_stride);
+    part(std::integral_constant<int, G::kValuePitch>{}, v_places, G::kValueLoads, G::kKeyBytes + G::kRopeBytes, v_base, op.v_token_stride);
   };
 
   const int k_row = 16 * (column >> 2 & 1) + 4 * (column >> 3) + (column & 3);
@@ -165,20 +221,22 @@ __global__ __launch_bounds__(kPromptThreads, 2) void LatentPromptKernel(const Pr
     if (tile + 1 < tile_to) fetch(tile + 1, slot ^ 1);
     const uint32_t at = slot * G::kTile;
     const int p0 = tile * kKeys;
-    const bool works = busy && p0 < base + min(first + wave * 32 + 32, r.n);
+    const bool works = busy && p0 < base + min(first + wave * 32 + 32, r.l.n);
     F32x16 dots[2];
     if (works) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) dots[k][i] = 0.0f;
-#pragma unroll
-        for (int x = 0; x < kSteps + kRopeSteps; ++x) {
-          const Eight key = x < kSteps ? *reinterpret_cast<const Eight*>(lds + ((at + key_lane) ^ 32 * x) + 32 * k * G::kKeyPitch)
-                                       : *reinterpret_cast<const Eight*>(lds + ((at + rope_lane) ^ 32 * (x - kSteps)) + 32 * k * G::kRopePitch);
-          dots[k] = S::Product32(key, q[x], dots[k]);
-        }
       }
+      // (The two blocks of 32 keys in turn: their places differ by a constant.)
+      ProductsInGroups<2 * (kSteps + kRopeSteps), kKeyGroup, Eight>(
+          [&](int i) {
+            const int x = i / 2, k = i % 2;
+            return x < kSteps ? *reinterpret_cast<const Eight*>(lds + ((at + key_lane) ^ 32 * x) + 32 * k * G::kKeyPitch)
+                              : *reinterpret_cast<const Eight*>(lds + ((at + rope_lane) ^ 32 * (x - kSteps)) + 32 * k * G::kRopePitch);
+          },
+          [&](int i, Eight key) { dots[i % 2] = S::Product32(key, q[i / 2], dots[i % 2]); });
     }
     float worth_now = worth;
     if (p0 + kKeys > all_rows_to) {
@@ -242,7 +300,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void LatentPromptKernel(const Pr
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) peak = fmaxf(peak, dots[k][i]);
+      for (int i = 0; i < 16; i += 2) peak = fmaxf(fmaxf(peak, dots[k][i]), dots[k][i + 1]);
     }
     peak = AcrossHalvesMax(peak) * worth_now;
     if (__any(peak > top + (kUp + kFollow))) {
@@ -258,76 +316,55 @@ __global__ __launch_bounds__(kPromptThreads, 2) void LatentPromptKernel(const Pr
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(dots[k][i], worth_now, -less));
-        sum += p;
-        weights[2 * k + i / 8][i % 8] = static_cast<typename S::One>(p);
+      for (int i = 0; i < 16; i += 2) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(dots[k][i], worth_now, -less)), p1 = __builtin_amdgcn_exp2f(fmaf(dots[k][i + 1], worth_now, -less));
+        weights[2 * k + i / 8][i % 8] = static_cast<typename S::One>(p), weights[2 * k + i / 8][i % 8 + 1] = static_cast<typename S::One>(p1);
+        // (The sum is of the weights as they are rounded, two in an instruction.)
+        sum = S::AddTwo(typename S::Two{weights[2 * k + i / 8][i % 8], weights[2 * k + i / 8][i % 8 + 1]}, sum);
       }
     }
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) out[b] = S::Product32(value(at + value_lane, b, k / 2, k % 2), weights[k], out[b]);
-    }
+    // (For one part of the keys the blocks in turn, both halves of the keys: places differ by a constant where the turned bits are the same.)
+    const uint32_t value_at = at + value_lane;
+    ProductsInGroups<4 * kBlocks, kValueGroup, Eight>([&](int i) { return value(value_at, i / 4, i % 2, i / 2 % 2); },
+                                                      [&](int i, Eight v) { out[i / 4] = S::Product32(v, weights[2 * (i % 2) + i / 2 % 2], out[i / 4]); });
   }
   sum = AcrossHalvesSum(sum);
-  if (!real) return;
-  // ---- out, or a run for the join. Element 4i + e of block b is dimension 32b + 8i + 4 half + e.
-  if (a.runs == 1) {
-    const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    const int64_t to = static_cast<int64_t>(r.start + row) * op.out_token_stride + head * op.out_head_stride + 4 * half;
+  if constexpr (LINE) MeetLds();  // (the next pair's tiles come where this one's were)
+  // ---- out, or a part for the join. Element 4i + e of block b is dimension 32b + 8i + 4 half + e.
+  if (!LINE || (piece.begins && piece.ends)) {
+    if (real) {
+      const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+      const int64_t to = static_cast<int64_t>(r.l.start + row) * op.out_token_stride + head * op.out_head_stride + 4 * half;
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
+      for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v[4] = {out[b][4 * i] * by, out[b][4 * i + 1] * by, out[b][4 * i + 2] * by, out[b][4 * i + 3] * by};
-        StoreValues<TYPE, 4>(op.out, to + 32 * b + 8 * i, v);
+        for (int i = 0; i < 4; ++i) {
+          const float v[4] = {out[b][4 * i] * by, out[b][4 * i + 1] * by, out[b][4 * i + 2] * by, out[b][4 * i + 3] * by};
+          StoreValues<TYPE, 4>(op.out, to + 32 * b + 8 * i, v);
+        }
       }
     }
   } else {
-    const int64_t at = (static_cast<int64_t>(request_head * a.tiles + tile_index) * a.runs + run) * kPromptRows + wave * 32 + column;
-    if (half == 0) reinterpret_cast<float2*>(a.numbers)[at] = make_float2(top, sum);
-    float* const to = a.values + at * N + 4 * half;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<F32x4*>(to + 32 * b + 8 * i) = F32x4{out[b][4 * i], out[b][4 * i + 1], out[b][4 * i + 2], out[b][4 * i + 3]};
+    const int which = 2 * index + (piece.begins ? 1 : 0);
+    if (tid == 0) {
+      int32_t* const p = a.parts.which + 4 * which;
+      p[0] = request, p[1] = k * op.heads + head, p[2] = min(r.l.n - first, kPromptRows), p[3] = r.l.start + first;
     }
+    if (busy) {
+      const int64_t unit = static_cast<int64_t>(which) * (kPromptRows / 32) + wave;
+      if (half == 0) a.parts.numbers[unit * 32 + column] = make_float2(top, sum);
+      F32x4* const to = reinterpret_cast<F32x4*>(a.parts.values) + unit * (N / 8) * kWave + lane;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(4 * b + i) * kWave] = F32x4{out[b][4 * i], out[b][4 * i + 1], out[b][4 * i + 2], out[b][4 * i + 3]};
+      }
+    }
+  }
   }
 }
 
-// The runs of a row joined: 16 (32) lanes a row, eight (four) values a lane... a thread eight values. grid (row tiles of all).
-template <int TYPE, int N>
-__global__ __launch_bounds__(kPromptThreads) void LatentPromptJoinKernel(const PromptArgs a) {
-  constexpr int kLanes = N / 8, kRowsAGo = kPromptThreads / kLanes;
-  const llmp_latent_prompt& op = a.op;
-  const uint32_t request_head = blockIdx.x / a.tiles;
-  const int tile_index = blockIdx.x % a.tiles, request = request_head / op.heads, head = request_head % op.heads;
-  const PromptRequest r = PromptOf(op, request);
-  const int first = tile_index * kPromptRows, rows = min(r.n - first, kPromptRows);
-  for (int row = threadIdx.x / kLanes; row < rows; row += kRowsAGo) {
-    const int d0 = 8 * (threadIdx.x % kLanes);
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * a.runs * kPromptRows + row;
-    float most = -INFINITY;
-    for (int i = 0; i < a.runs; ++i) most = fmaxf(most, a.numbers[2 * (at + i * kPromptRows)]);
-    const float less = most == -INFINITY ? 0.0f : most;
-    float sum = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = 0; i < a.runs; ++i) {
-      const float2 n = reinterpret_cast<const float2*>(a.numbers)[at + i * kPromptRows];
-      const float by = __builtin_amdgcn_exp2f(n.x - less);
-      sum = fmaf(n.y, by, sum);
-      const F32x4* const from = reinterpret_cast<const F32x4*>(a.values + (at + i * kPromptRows) * N + d0);
-      const F32x4 x = from[0], y = from[1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], by, v[e]), v[4 + e] = fmaf(y[e], by, v[4 + e]);
-    }
-    const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= by;
-    StoreValues<TYPE, 8>(op.out, static_cast<int64_t>(r.start + first + row) * op.out_token_stride + head * op.out_head_stride + d0, v);
-  }
-}
+int TilesOf(const llmp_latent_prompt& op) { return (std::min(op.most_tokens, op.tokens) + kPromptRows - 1) / kPromptRows; }
 
 int CheckLatentPrompt(const llmp_latent_prompt* op, int cus) {
   if (op == nullptr) return Refuse(1, "latent_prompt: null operands");
@@ -348,18 +385,25 @@ int CheckLatentPrompt(const llmp_latent_prompt* op, int cus) {
     return Refuse(1, "latent_prompt: I32 arrays at 4-byte boundaries");
   if (!std::isfinite(op->scale)) return Refuse(1, "latent_prompt: a scale that is not finite");
   if (cus < 1 || cus > 4096) return Refuse(1, "latent_prompt: %d compute units", cus);
-  const int64_t tiles = (std::min(op->most_tokens, op->tokens) + kPromptRows - 1) / kPromptRows;
-  if ((static_cast<int64_t>(op->requests) * op->heads + 8) * tiles * kMostRuns > INT_MAX) return Refuse(1, "latent_prompt: %d requests of %d heads with up to %d rows are too many", op->requests, op->heads, op->most_tokens);
+  const int64_t most_stride = 1 << 24;
+  if (op->k_token_stride >= most_stride || op->v_token_stride >= most_stride || op->k_rope_token_stride >= most_stride)
+    return Refuse(1, "latent_prompt: keys and values at most 2^24 values apart");
+  if ((static_cast<int64_t>(op->requests) * op->heads + 8) * TilesOf(*op) > INT_MAX)
+    return Refuse(1, "latent_prompt: %d requests of %d heads with up to %d rows are too many", op->requests, op->heads, op->most_tokens);
   return 0;
 }
 
-// How the keys are cut: the least runs that give every compute unit two workgroups, none shorter than four tiles of the longest request that there can be.
-int RunsOf(const llmp_latent_prompt& op, int cus, int tiles) {
-  const int64_t sets = static_cast<int64_t>(op.requests) * op.heads * tiles;
-  const int64_t most = std::max<int64_t>(1, op.keys / (4 * kKeys));
-  return static_cast<int>(std::min<int64_t>({most, kMostRuns, std::max<int64_t>(1, 2 * cus / sets)}));
+// Of the line: an eighth of them on every chiplet.
+int LineGroups(int cus) { return (kAUnit * cus + 7) / 8 * 8; }
+
+// Whether pairs are taken whole: where the longest that there can be (all the call's keys) is no more than a workgroup's share, as far as the sizes tell it: rows in
+// tiles, at least one a request, keys spread evenly over the requests. (A prompt of 4096, 32 heads: whole %WHOLE%, cut %CUT%; six ragged ones of 12 heads, up to 700 rows behind
+// 3500 keys: whole %RWHOLE%, cut %RCUT%.)
+bool WholePairs(const llmp_latent_prompt& op, int cus) {
+  const int64_t row_tiles = op.tokens / kPromptRows + op.requests, tiles = op.keys / kKeys + 1;
+  const int64_t work = row_tiles * op.heads * (tiles / op.requests + 1);
+  return tiles <= work / (kAUnit * cus);
 }
-int TilesOf(const llmp_latent_prompt& op) { return (std::min(op.most_tokens, op.tokens) + kPromptRows - 1) / kPromptRows; }
 
 }  // namespace
 }  // namespace llmp_hip
@@ -368,9 +412,7 @@ using namespace llmp_hip;
 
 extern "C" size_t llmp_hip_latent_prompt_scratch(const llmp_latent_prompt* op, int cus) {
   if (CheckLatentPrompt(op, cus) != 0) return 0;
-  const int tiles = TilesOf(*op), runs = RunsOf(*op, cus, tiles);
-  if (runs == 1) return 16;
-  return static_cast<size_t>(op->requests) * op->heads * tiles * runs * kPromptRows * (8 + 4 * static_cast<size_t>(op->value));
+  return WholePairs(*op, cus) ? 16 : LatentPartsBytes(LineGroups(cus), kPromptRows, op->value);
 }
 
 extern "C" int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratch, size_t scratch_bytes, int cus, void* stream) {
@@ -378,23 +420,28 @@ extern "C" int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratc
   const size_t need = llmp_hip_latent_prompt_scratch(op, cus);
   if (scratch == nullptr || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
     return Refuse(1, "latent_prompt: %zu bytes of scratch at a 16-byte boundary, not %zu", need, scratch_bytes);
+  const bool whole = WholePairs(*op, cus);
+  const int line_groups = LineGroups(cus);
   PromptArgs a;
   a.op = *op;
   a.tiles = TilesOf(*op);
-  a.runs = RunsOf(*op, cus, a.tiles);
+  a.parts = LatentPartsAt(scratch, line_groups, kPromptRows);
   const size_t sets = static_cast<size_t>(op->requests) * op->heads;
-  a.numbers = static_cast<float*>(scratch);
-  a.values = a.numbers + sets * a.tiles * a.runs * kPromptRows * 2;
-  const dim3 grid(static_cast<unsigned>((sets * a.runs + 7) / 8 * 8 * a.tiles));
+  const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, line_groups, 0};
   const auto s = static_cast<hipStream_t>(stream);
   BeginLaunches();
   const auto launch = [&](auto type, auto n, auto p) {
     constexpr int kType = decltype(type)::value, kN = decltype(n)::value, kP = decltype(p)::value;
-    static bool sized = false;
     constexpr int kLds = PromptGeo<kN, kP>::kLds;
-    if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP>), kLds, &sized)) return;
-    hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP>), grid, dim3(kPromptThreads), kLds, s, a);
-    if (a.runs > 1) hipLaunchKernelGGL((LatentPromptJoinKernel<kType, kN>), dim3(static_cast<unsigned>(sets * a.tiles)), dim3(kPromptThreads), 0, s, a);
+    static bool sized[2] = {false, false};
+    if (whole) {
+      if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, false>), kLds, &sized[0])) return;
+      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, false>), dim3(static_cast<unsigned>((sets + 7) / 8 * 8 * a.tiles)), dim3(kPromptThreads), kLds, s, a);
+    } else {
+      if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, true>), kLds, &sized[1])) return;
+      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, true>), dim3(line_groups), dim3(kPromptThreads), kLds, s, a);
+      hipLaunchKernelGGL((LatentJoinKernel<kType, kN, 32, kPromptRows>), dim3(line_groups, kJoinGroups), dim3(256), 0, s, join);
+    }
   };
   const auto sizes = [&](auto type) {
     const auto rope = [&](auto n) {
