@@ -587,7 +587,7 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
     static bool sized = false;
     if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kFew>), kLds, &sized)) return;
     hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(cus), dim3(G::kThreads), kLds, s, a);
-    hipLaunchKernelGGL((LatentJoinKernel<kType, kR, 16, G::kRows>), dim3(cus, kJoinGroups), dim3(256), 0, s, join);
+    hipLaunchKernelGGL((LatentJoinKernel<kType, kR, 16, G::kRows>), dim3(cus, 2), dim3(kJoinWaves * kWave), 0, s, join);
   });
   return LaunchStatus("latent_attend");
 }

@@ -126,10 +126,11 @@ __device__ __forceinline__ T Scalar(T v) {
 __device__ __forceinline__ LatentRequest Scalar(const LatentRequest& l) { return {Scalar(l.start), Scalar(l.n), Scalar(l.length), Scalar(l.base), Scalar(l.groups)}; }
 
 // ---- the parts of a pair, joined. They are as the lanes held them: an item is UNIT rows by 256 / UNIT dimensions, lane l four of them, 4 (l / UNIT) on, of row
-// l % UNIT. The pair's items are dealt to the workgroups (of this launch, kJoinGroups for each of the first one's) that hold its parts, so that what one reads is
-// about the same whatever the number of parts. A wave takes an item, or where there are many parts a workgroup one together, a wave every fourth part.
-// (One wave an item: 256 parts of 128 rows of 512 values 180 us, 16 so.)
-constexpr int kJoinGroups = 8, kJoinAlone = 16;
+// l % UNIT. The pair's items are dealt to the workgroups (one for each of the first launch's) that hold its parts, so that what one reads is
+// about the same whatever the number of parts. A wave takes an item, or where there are many parts a workgroup one together, the waves' parts in turn. Bound by the
+// parts' bytes where they are many (256 of 128 rows of 512 values, 67 MB: 17 to 27 us), else by four loads one after the other (16 rows: 5.6 us): a wave reads a
+// part's numbers with its values and scales by a running maximum (the numbers first, for the maximum: 33 and 10 us). (One wave an item: 180 us.)
+constexpr int kJoinWaves = 16, kJoinAhead = 4;
 struct JoinArgs {
   LatentParts parts;
   void* out;
@@ -137,74 +138,92 @@ struct JoinArgs {
   int heads, groups;
   int pairs_a_token;  // 0: a pair is `heads`' of them: rows are tokens; 1: rows are (token, head); more: rows are heads
 };
+// grid (the first launch's workgroups, 2: by its later part of a pair, by its first one of another)
 template <int TYPE, int WIDTH, int UNIT, int ROWS>
-__global__ __launch_bounds__(256) void LatentJoinKernel(const JoinArgs a) {
+__global__ __launch_bounds__(kJoinWaves * kWave) void LatentJoinKernel(const JoinArgs a) {
   constexpr int kItemValues = 256 / UNIT, kBlocks = WIDTH / kItemValues;
-  __shared__ F32x4 met[3][kWave];
-  __shared__ float met_sums[3][kWave];
+  __shared__ F32x4 met[kJoinWaves - 1][kWave];
+  __shared__ float2 met_numbers[kJoinWaves - 1][kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, column = lane % UNIT, part_of = lane / UNIT;
   const int x = blockIdx.x;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const int32_t* const mine = a.parts.which + 8 * x + 4 * which;
-    const int request = mine[0], pair = mine[1], rows = mine[2], token0 = mine[3];
-    if (request < 0) continue;
-    int leader = x;
-    if (which == 0) {  // the last workgroup before this one that begins a pair has begun this one
-      for (int base = x - 1;; base -= kWave) {
-        const int g = base - lane;
-        const uint64_t begins = __ballot(g >= 0 && a.parts.which[8 * max(g, 0) + 4] >= 0);
-        leader = base - (__ffsll(static_cast<unsigned long long>(begins)) - 1);
-        if (begins != 0 || base < kWave) break;
-      }
+  const int which = blockIdx.y;
+  const I32x4 mine = *reinterpret_cast<const I32x4*>(a.parts.which + 8 * x + 4 * which);
+  const int request = mine[0], pair = mine[1], rows = mine[2], token0 = mine[3];
+  if (request < 0) return;
+  int leader = x;
+  if (which == 0) {  // the last workgroup before this one that begins a pair has begun this one
+    for (int base = x - 1;; base -= kWave) {
+      const int g = base - lane;
+      const uint64_t begins = __ballot(g >= 0 && a.parts.which[8 * max(g, 0) + 4] >= 0);
+      leader = base - (__ffsll(static_cast<unsigned long long>(begins)) - 1);
+      if (begins != 0 || base < kWave) break;
     }
-    // The parts after the first are the next workgroups' later ones, as long as they are of this pair.
-    int count = 1;
-    for (int base = leader + 1;; base += kWave) {
-      const int g = base + lane, at = 8 * min(g, a.groups - 1);
-      const uint64_t others = ~__ballot(g < a.groups && a.parts.which[at] == request && a.parts.which[at + 1] == pair);
-      const int here = others == 0 ? kWave : __ffsll(static_cast<unsigned long long>(others)) - 1;
-      count += here;
-      if (here < kWave) break;
-    }
-    const auto unit = [&](int i, int u) { return static_cast<int64_t>(i == 0 ? 2 * leader + 1 : 2 * (leader + i)) * (ROWS / UNIT) + u; };
-    const bool together = count > kJoinAlone;
-    const int items = (rows + UNIT - 1) / UNIT * kBlocks;
-    const int waves = together ? 1 : 4;
-    for (int item = ((x - leader) * kJoinGroups + static_cast<int>(blockIdx.y)) * waves + (together ? 0 : wave); item < items; item += count * kJoinGroups * waves) {
-      const int u = item / kBlocks, block = item % kBlocks;
-      float most = -INFINITY;
-      for (int i = part_of; i < count; i += kWave / UNIT) most = fmaxf(most, a.parts.numbers[unit(i, u) * UNIT + column].x);
+  }
+  // The parts after the first are the next workgroups' later ones, as long as they are of this pair.
+  int count = 1;
+  for (int base = leader + 1;; base += kWave) {
+    const int g = base + lane, at = 8 * min(g, a.groups - 1);
+    const uint64_t others = ~__ballot(g < a.groups && a.parts.which[at] == request && a.parts.which[at + 1] == pair);
+    const int here = others == 0 ? kWave : __ffsll(static_cast<unsigned long long>(others)) - 1;
+    count += here;
+    if (here < kWave) break;
+  }
+  const auto unit = [&](int i, int u) { return static_cast<int64_t>(i == 0 ? 2 * leader + 1 : 2 * (leader + i)) * (ROWS / UNIT) + u; };
+  const int items = (rows + UNIT - 1) / UNIT * kBlocks;
+  // In loads that wait for each other; a meeting of the waves counts as one.
+  const auto over = [](int n, int d) { return (n + d - 1) / d; };
+  const bool together = over(items, count) * (over(count, kJoinAhead * kJoinWaves) + 1) < over(items, count * kJoinWaves) * over(count, kJoinAhead);
+  const int waves = together ? 1 : kJoinWaves;
+  for (int item = (x - leader) * waves + (together ? 0 : wave); item < items; item += count * waves) {
+    const int u = item / kBlocks, block = item % kBlocks;
+    float most = -INFINITY, sum = 0.0f;
+    F32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    // (Four parts' loads at a time, the last one's again past the end, and nothing that they wait for: one after the other each waits for memory.)
+    const int from = together ? wave : 0, step = together ? kJoinWaves : 1;
+    for (int i0 = from; i0 < count; i0 += kJoinAhead * step) {
+      float2 n[kJoinAhead];
+      F32x4 x[kJoinAhead];
 #pragma unroll
-      for (int m = UNIT; m < kWave; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
-      const float less = most == -INFINITY ? 0.0f : most;
-      float sum = 0.0f;
-      F32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-      for (int i = together ? wave : 0; i < count; i += together ? 4 : 1) {
-        const int64_t at = unit(i, u);
-        const float2 n = a.parts.numbers[at * UNIT + column];
-        const float by = __builtin_amdgcn_exp2f(n.x - less);
-        sum = fmaf(n.y, by, sum);
-        v += reinterpret_cast<const F32x4*>(a.parts.values)[(at * kBlocks + block) * kWave + lane] * by;
+      for (int j = 0; j < kJoinAhead; ++j) {
+        const int64_t at = unit(min(i0 + j * step, count - 1), u);
+        n[j] = a.parts.numbers[at * UNIT + column];
+        x[j] = reinterpret_cast<const F32x4*>(a.parts.values)[(at * kBlocks + block) * kWave + lane];
       }
-      if (together) {
-        if (wave > 0) met[wave - 1][lane] = v, met_sums[wave - 1][lane] = sum;
-        __syncthreads();
-        if (wave == 0) {
+      const float before = most;
 #pragma unroll
-          for (int i = 0; i < 3; ++i) v += met[i][lane], sum += met_sums[i][lane];
+      for (int j = 0; j < kJoinAhead; ++j) most = fmaxf(most, n[j].x);
+      const float less = most == -INFINITY ? 0.0f : most, keeps = __builtin_amdgcn_exp2f(before - less);
+      sum *= keeps, v *= keeps;
+#pragma unroll
+      for (int j = 0; j < kJoinAhead; ++j) {
+        if (i0 + j * step < count) {
+          const float by = __builtin_amdgcn_exp2f(n[j].x - less);
+          sum = fmaf(n[j].y, by, sum), v += x[j] * by;
         }
-        __syncthreads();
       }
-      const int row = UNIT * u + column;
-      if (row < rows && (!together || wave == 0)) {
-        const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-        const float out[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
-        const int token = token0 + (a.pairs_a_token == 0 ? row : a.pairs_a_token == 1 ? row / a.heads : 0);
-        const int head = a.pairs_a_token == 0 ? pair % a.heads : a.pairs_a_token == 1 ? row % a.heads : pair % a.pairs_a_token * ROWS + row;
-        StoreValues<TYPE, 4>(a.out, token * a.out_token_stride + head * a.out_head_stride + kItemValues * block + 4 * part_of, out);
+    }
+    if (together) {
+      if (wave > 0) met[wave - 1][lane] = v, met_numbers[wave - 1][lane] = make_float2(most, sum);
+      __syncthreads();
+      if (wave == 0) {
+        const float own = most;
+        for (int i = 0; i < kJoinWaves - 1; ++i) most = fmaxf(most, met_numbers[i][lane].x);
+        const float less = most == -INFINITY ? 0.0f : most, keeps = __builtin_amdgcn_exp2f(own - less);
+        sum *= keeps, v *= keeps;
+        for (int i = 0; i < kJoinWaves - 1; ++i) {
+          const float by = __builtin_amdgcn_exp2f(met_numbers[i][lane].x - less);
+          sum = fmaf(met_numbers[i][lane].y, by, sum), v += met[i][lane] * by;
+        }
       }
+      __syncthreads();
+    }
+    const int row = UNIT * u + column;
+    if (row < rows && (!together || wave == 0)) {
+      const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+      const float out[4] = {v[0] * by, v[1] * by, v[2] * by, v[3] * by};
+      const int token = token0 + (a.pairs_a_token == 0 ? row : a.pairs_a_token == 1 ? row / a.heads : 0);
+      const int head = a.pairs_a_token == 0 ? pair % a.heads : a.pairs_a_token == 1 ? row % a.heads : pair % a.pairs_a_token * ROWS + row;
+      StoreValues<TYPE, 4>(a.out, token * a.out_token_stride + head * a.out_head_stride + kItemValues * block + 4 * part_of, out);
     }
   }
 }

@@ -100,9 +100,9 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
     });
     u = run.from, u_end = run.to, before = run.before, request = run.request;
   } else {
-    const uint32_t turn = blockIdx.x / 8, set = turn / a.tiles * 8 + blockIdx.x % 8;
-    if (set >= static_cast<uint32_t>(op.requests) * op.heads) return;
-    request = set / op.heads, head = set % op.heads, k = a.tiles - 1 - static_cast<int>(turn % a.tiles);
+    const uint32_t sets = static_cast<uint32_t>(op.requests) * op.heads, padded = (sets + 7) / 8 * 8, set = blockIdx.x % padded;
+    if (set >= sets) return;
+    request = set / op.heads, head = set % op.heads, k = a.tiles - 1 - static_cast<int>(blockIdx.x / padded);
   }
   for (; u < u_end;) {
   // ---- the next pair, or part of one.
@@ -323,10 +323,10 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
         sum = S::AddTwo(typename S::Two{weights[2 * k + i / 8][i % 8], weights[2 * k + i / 8][i % 8 + 1]}, sum);
       }
     }
-    // (For one part of the keys the blocks in turn, both halves of the keys: places differ by a constant where the turned bits are the same.)
+    // (Two blocks of dimensions in turn: a product does not wait for the one before it.)
     const uint32_t value_at = at + value_lane;
-    ProductsInGroups<4 * kBlocks, kValueGroup, Eight>([&](int i) { return value(value_at, i / 4, i % 2, i / 2 % 2); },
-                                                      [&](int i, Eight v) { out[i / 4] = S::Product32(v, weights[2 * (i % 2) + i / 2 % 2], out[i / 4]); });
+    ProductsInGroups<4 * kBlocks, kValueGroup, Eight>([&](int i) { return value(value_at, 2 * (i / 8) + i % 2, i / 2 % 2, i / 4 % 2); },
+                                                      [&](int i, Eight v) { const int b = 2 * (i / 8) + i % 2; out[b] = S::Product32(v, weights[2 * (i / 2 % 2) + i / 4 % 2], out[b]); });
   }
   sum = AcrossHalvesSum(sum);
   if constexpr (LINE) MeetLds();  // (the next pair's tiles come where this one's were)
@@ -396,13 +396,18 @@ int CheckLatentPrompt(const llmp_latent_prompt* op, int cus) {
 // Of the line: an eighth of them on every chiplet.
 int LineGroups(int cus) { return (kAUnit * cus + 7) / 8 * 8; }
 
-// Whether pairs are taken whole: where the longest that there can be (all the call's keys) is no more than a workgroup's share, as far as the sizes tell it: rows in
-// tiles, at least one a request, keys spread evenly over the requests. (A prompt of 4096, 32 heads: whole %WHOLE%, cut %CUT%; six ragged ones of 12 heads, up to 700 rows behind
-// 3500 keys: whole %RWHOLE%, cut %RCUT%.)
+// Whether pairs are taken whole. Then a call lasts as long as its longest pair (1.2 us a key tile, a workgroup alone on its unit) or as a workgroup's share (3 us a
+// tile, two of them on it), and cut into runs as long as the share and 20 us, for the parts. As far as the sizes tell those: half of the last row tile of a
+// request is empty, a request has an equal part of the keys and no more than twice that, a row sees all of them, or half where all of them are new. (A
+// prompt of 4096, nope 128, rope 64: 32 heads whole 199 us, cut 277, 8 heads (of 64 values) 79 and 61; one of 1000, 8 heads: 34 and 50; six ragged ones of 12
+// heads, up to 700 rows behind 3500 keys: 96 and 53; 16 of up to 1000, 32 heads: 63 and 91.)
 bool WholePairs(const llmp_latent_prompt& op, int cus) {
-  const int64_t row_tiles = op.tokens / kPromptRows + op.requests, tiles = op.keys / kKeys + 1;
-  const int64_t work = row_tiles * op.heads * (tiles / op.requests + 1);
-  return tiles <= work / (kAUnit * cus);
+  const bool fresh = op.key_starts == nullptr || op.keys == op.tokens;
+  const double requests = op.requests, tiles = op.keys / static_cast<double>(kKeys) + 1.0, share = tiles / requests + 1.0;
+  const double longest = fresh ? std::min(tiles, op.most_tokens / static_cast<double>(kKeys) + 1.0) : std::min(tiles, 2.0 * share);
+  const double row_tiles = op.tokens / static_cast<double>(kPromptRows) + 0.5 * requests;
+  const double each = row_tiles * op.heads * share * (fresh ? 0.5 : 1.0) / (kAUnit * cus);
+  return longest <= 2.5 * each + 15.0;
 }
 
 }  // namespace
@@ -440,7 +445,7 @@ extern "C" int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratc
     } else {
       if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, true>), kLds, &sized[1])) return;
       hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, true>), dim3(line_groups), dim3(kPromptThreads), kLds, s, a);
-      hipLaunchKernelGGL((LatentJoinKernel<kType, kN, 32, kPromptRows>), dim3(line_groups, kJoinGroups), dim3(256), 0, s, join);
+      hipLaunchKernelGGL((LatentJoinKernel<kType, kN, 32, kPromptRows>), dim3(line_groups, 2), dim3(kJoinWaves * kWave), 0, s, join);
     }
   };
   const auto sizes = [&](auto type) {
