@@ -23,12 +23,12 @@ namespace {
 constexpr int kTokens = 32;  // a tile's
 constexpr int kFewRows = 16, kManyRows = 128;
 constexpr int kLdsBytes = 160 * 1024;
-constexpr int kLeastFew = 256, kLeastMany = 128;  // of the line, to a workgroup: finer parts cost more to write and to join
+constexpr int kLeast = 128;  // of the line, to a workgroup: finer parts cost more to write and to join (16 rows, 16 requests of up to 2000: 30.2 us so, 32.4 at 256)
 
 struct LatentArgs {
   llmp_latent_attend op;
   LatentParts parts;
-  int most_length, least;
+  int most_length;
   int tokens_a_pair, pairs_a_token;  // rows of several whole tokens, or of part of one
 };
 
@@ -37,13 +37,13 @@ struct LatentGeo {
   static constexpr int kWaves = FEW ? 4 : 8, kThreads = kWaves * kWave;
   static constexpr int kRows = FEW ? kFewRows : kManyRows;
   static constexpr int kPitch = EIGHT ? R : 2 * R, kRopePitch = 2 * P;
-  static constexpr int kLatentBytes = kTokens * kPitch, kRopeBytes = kTokens * kRopePitch, kScaleBytes = EIGHT ? 256 : 0;
+  static constexpr int kLatentBytes = kTokens * kPitch, kRopeBytes = kTokens * kRopePitch, kScaleBytes = EIGHT && !FEW ? 256 : 0;
   static constexpr int kTile = kLatentBytes + kRopeBytes + kScaleBytes;
   static constexpr int kQueries = FEW ? 0 : kManyRows * 2 * P;  // the queries' rotated part, where registers are short
   static constexpr int kRing = FEW ? std::min(2, kLdsBytes / 4 / kTile) : std::min(5, (kLdsBytes - kQueries) / kTile);
   static constexpr int kSharing = FEW ? 1 : kWaves;  // waves that bring a tile in
   static constexpr int kLatentLoads = kLatentBytes / 1024 / kSharing, kRopeLoads = (kRopeBytes / 1024 + kSharing - 1) / kSharing;
-  static constexpr int kLoads = kLatentLoads + kRopeLoads + (EIGHT ? 1 : 0);  // a wave's for a tile
+  static constexpr int kLoads = kLatentLoads + kRopeLoads + (kScaleBytes > 0 ? 1 : 0);  // a wave's for a tile
   static constexpr int kArea = kFewRows * R * 4 + 2 * kFewRows * 4;  // the few rows' form: a wave's results for the others
   static constexpr int kLds = FEW ? std::max(4 * kRing * kTile, 4 * kArea) : kRing * kTile + kQueries;
 
@@ -84,7 +84,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
   // ---- this workgroup's run of the line
   const int64_t t = a.tokens_a_pair;
   if (tid < 2) a.parts.which[(2 * w + tid) * 4] = -1;
-  const LatentRun run = RunOf(op.requests, w, groups, a.least, [&](int r) {
+  const LatentRun run = RunOf(op.requests, w, groups, kLeast, [&](int r) {
     const LatentRequest l = AttendRequest(a, r);
     return LineBefore(l, t, l.groups) * a.pairs_a_token;
   });
@@ -102,10 +102,10 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
       before += all;
       continue;
     }
-    for (int k = GroupAt(l, t, (u - before) / a.pairs_a_token); k < l.groups && u < u_end; ++k) {
+    for (int k = GroupAt(l, t, Over(u - before, a.pairs_a_token)); k < l.groups && u < u_end; ++k) {
       const int seen = SeenOf(l, a.tokens_a_pair, k), whole = seen + kVisit;
       const int64_t group_from = before + LineBefore(l, t, k) * a.pairs_a_token;
-      for (int part = static_cast<int>((u - group_from) / whole); part < a.pairs_a_token && u < u_end; ++part) {
+      for (int part = static_cast<int>(Over(u - group_from, whole)); part < a.pairs_a_token && u < u_end; ++part) {
         const int64_t from = group_from + static_cast<int64_t>(part) * whole;
         const int x0 = static_cast<int>(u - from), x1 = static_cast<int>(min(u_end - from, static_cast<int64_t>(whole)));
         u = from + x1;
@@ -181,8 +181,14 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         };
         const int step = FEW ? G::kWaves : 1;
         const int my_from = tile_from + (FEW ? wave : 0);
+        // The few rows' form holds a tile's scales in scalar registers: with them there two tiles a wave fill LDS (one tile: 65536 tokens, rope 32: 139 us, two 123).
+        struct TileScales {
+          U32x4 a, b;
+        };
+        TileScales scales_now = {}, scales_next = {};
+        const auto tile_scales = [&](int row) { return *(const __attribute__((address_space(4))) U32x4*)(static_cast<const uint8_t*>(c.scale) + row); };
         uint32_t absent = 0;  // two bits a slot of the ring: the tile's groups without a page
-        const auto fetch = [&](int tile, int slot) {
+        const auto fetch = [&](int tile, int slot) -> TileScales {
           if (held_from < 0 || tile >= held_from + 32) look_up(tile);
           const int at0 = __builtin_amdgcn_readlane(held, 2 * (tile - held_from)), at1 = __builtin_amdgcn_readlane(held, 2 * (tile - held_from) + 1);
           absent = (absent & ~(3u << (2 * slot))) | ((at0 < 0 ? 1u : 0u) | (at1 < 0 ? 2u : 0u)) << (2 * slot);
@@ -222,13 +228,15 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
               LineToLds(second ? rope_b : rope_a, (kWhole ? row & 15 : min(row & 15, second ? last_b : last_a)) * G::kRopePitch + piece, to + G::kLatentBytes + 1024 * n);
             }
             // The scales: four tokens a lane, eight lanes of them.
-            if constexpr (EIGHT) WordToLds(c.scale, (lane_now & 4 ? row_b : row_a) + 4 * (lane_now & 3), to + G::kLatentBytes + G::kRopeBytes);
+            if constexpr (G::kScaleBytes > 0) WordToLds(c.scale, (lane_now & 4 ? row_b : row_a) + 4 * (lane_now & 3), to + G::kLatentBytes + G::kRopeBytes);
           };
           if (left >= kTokens) {
             load(std::true_type{});
           } else {
             load(std::false_type{});
           }
+          if constexpr (EIGHT && FEW) return {tile_scales(row_a), tile_scales(row_b)};
+          return {};
         };
 
         // What a lane reads of a tile. Rows are whole 256 bytes, so that a place is the lane's own (its row, its piece turned) with a constant's bits turned
@@ -273,7 +281,13 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         // A tile's logits of a wave's rows: element i is token 8 quarter + i.
         float dots[kLogits];
         const auto scales = [&](uint32_t tile, float (&scale)[kLogits]) {
-          const uint2 e = *reinterpret_cast<const uint2*>(lds + tile + G::kLatentBytes + G::kRopeBytes + 8 * (lane_anew() / 16));
+          uint2 e;
+          if constexpr (FEW) {
+            const U32x4 four = quarter < 2 ? scales_now.a : scales_now.b;
+            e = quarter % 2 == 0 ? make_uint2(four.x, four.y) : make_uint2(four.z, four.w);
+          } else {
+            e = *reinterpret_cast<const uint2*>(lds + tile + G::kLatentBytes + G::kRopeBytes + 8 * (lane_anew() / 16));
+          }
 #pragma unroll
           for (int i = 0; i < kLogits; ++i) {
             const uint32_t bits = (i < 4 ? e.x : e.y) >> (8 * (i & 3)) & 0xFFu;
@@ -392,7 +406,8 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         if constexpr (FEW) {
           // A wave's own ring: nobody waits for anybody.
           const int count = tile_to > my_from ? (tile_to - my_from + step - 1) / step : 0;
-          for (int i = 0; i < G::kRing && i < count; ++i) fetch(my_from + i * step, i);
+          if (count > 0) scales_now = fetch(my_from, 0);
+          if (G::kRing == 2 && count > 1) scales_next = fetch(my_from + step, 1);
           for (int i = 0; i < count; ++i) {
             if (G::kRing == 2 && i + 1 < count) {
               WaitLoads<G::kLoads>();
@@ -403,7 +418,8 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             keys(ring_off + i % G::kRing * G::kTile);
             values(tile, ring_off + i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u, true);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (i + G::kRing < count) fetch(my_from + (i + G::kRing) * step, i % G::kRing);
+            scales_now = scales_next;
+            if (i + G::kRing < count) (G::kRing == 1 ? scales_now : scales_next) = fetch(my_from + (i + G::kRing) * step, i % G::kRing);
           }
         } else {
           const int count = Scalar(tile_to - tile_from);
@@ -572,7 +588,6 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
   a.op = *op;
   a.parts = LatentPartsAt(scratch, cus, rows);
   a.most_length = op->table_width * op->cache.page;
-  a.least = few ? kLeastFew : kLeastMany;
   a.tokens_a_pair = std::max(1, rows / op->heads);
   a.pairs_a_token = (op->heads + rows - 1) / rows;
   const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, cus, a.pairs_a_token};

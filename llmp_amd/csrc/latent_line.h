@@ -35,13 +35,15 @@ struct LatentRequest {
   int start, n, length, base;  // PagedRequest's
   int groups;
 };
+// a / b, for a >= 0 and b > 0. (A division of 64 bits is 0.3 us where a wave waits for it, and hardly any line is that long.)
+__device__ __forceinline__ int64_t Over(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b; }
 // What group k's last token sees.
 __device__ __forceinline__ int SeenOf(const LatentRequest& l, int t, int k) { return max(min(l.base + min((k + 1) * t, l.n), l.length), 0); }
 // The line before group k, of one pair a group: the sum of min(base + (i + 1) t, most), none below 0, over i < k, and the visits.
 __device__ __forceinline__ int64_t LineBefore(const LatentRequest& l, int64_t t, int k) {
   const int64_t most = max(min(l.length, l.base + l.n), 0);
-  const int64_t low = l.base < 0 ? min(static_cast<int64_t>(k), -static_cast<int64_t>(l.base) / t) : 0;
-  const int64_t high = max(low, min(static_cast<int64_t>(k), most > l.base ? (most - l.base) / t : 0));
+  const int64_t low = l.base < 0 ? min(static_cast<int64_t>(k), Over(-static_cast<int64_t>(l.base), t)) : 0;
+  const int64_t high = max(low, min(static_cast<int64_t>(k), most > l.base ? Over(most - static_cast<int64_t>(l.base), t) : 0));
   const int64_t risen = (high - low) * l.base + t * ((high * (high + 1) - low * (low + 1)) / 2);
   return risen + (k - high) * most + static_cast<int64_t>(k) * kVisit;
 }
@@ -84,7 +86,7 @@ __device__ __forceinline__ LatentRun RunOf(int requests, int index, int groups, 
   const int64_t first = lane < requests ? length_of(lane) : 0, first_upto = sums(first);
   int64_t total = from_lane(first_upto, kWave - 1);
   for (int r0 = kWave; r0 < requests; r0 += kWave) total += from_lane(sums(r0 + lane < requests ? length_of(r0 + lane) : 0), kWave - 1);
-  const int64_t per = max((total + groups - 1) / groups, least);
+  const int64_t per = max(Over(total + groups - 1, groups), least);
   LatentRun run = {index * per, min((index + 1) * per, total), 0, 0};
   if (run.from >= run.to) return run;
   for (int r0 = 0; r0 < requests; r0 += kWave) {
