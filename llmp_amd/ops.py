@@ -920,7 +920,7 @@ def _latent_cache(cache):
     return _lib.LatentCache(latent.data_ptr(), _ptr(scale), rope.data_ptr(), _X_TYPES[rope.dtype], pages, page, width, rope.shape[2])
 
 
-def latent_store(cache, latent, rope, slots, positions=None, table=None, *, layout="interleaved", weight=None, eps=1e-6):
+def latent_store(cache, latent, rope, slots, positions=None, table=None, *, layout="half", weight=None, eps=1e-6):
     """llmp.latent.store: rows latent [tokens, width] and rope [tokens, rope] (float32, bfloat16 or float16) into the cache's `slots` (int32 [tokens],
     paged_plan's; outside the cache: skipped). With `weight` (float32 [width]) the latent rows are normalised by their root mean square first; with
     `table` (rope_table's) the keys are rotated at int32 `positions`. The cache is updated in place."""
