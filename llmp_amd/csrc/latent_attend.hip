@@ -502,8 +502,8 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         } else {
           const int which = 2 * w + (piece.begins ? 1 : 0);
           if (tid == 0) {
-            int32_t* const p = a.parts.which + 4 * which;
-            p[0] = request, p[1] = k * a.pairs_a_token + part, p[2] = rows, p[3] = l.start + first_token;
+            const LatentOwners owners = OwnersOf(from, seen, kTokens, run.per);
+            *reinterpret_cast<I32x4*>(a.parts.which + 4 * which) = I32x4{owners.first, k * a.pairs_a_token + part, rows | owners.count << 8, l.start + first_token};
           }
           if (busy) {
             const int64_t rows16 = static_cast<int64_t>(which) * (G::kRows / 16) + row0 / 16;

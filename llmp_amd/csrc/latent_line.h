@@ -19,7 +19,7 @@ constexpr float kUp = 8.0f, kFollow = 6.0f;
 struct LatentParts {
   float* values;    // [2 * workgroups][rows of a pair][width], in the order of the lanes' registers
   float2* numbers;  // [2 * workgroups][rows of a pair]: maximum, sum
-  int32_t* which;   // [2 * workgroups][4]: request (-1: no part), pair, rows, first row of the call's
+  int32_t* which;   // [2 * workgroups][4]: the workgroup of its pair's first part (-1: no part here), pair, rows and 256 times the pair's parts, first row of the call's
 };
 inline size_t LatentPartsBytes(int groups, int rows, int width) { return static_cast<size_t>(2 * groups) * (16 + rows * (8 + 4 * static_cast<size_t>(width))); }
 inline LatentParts LatentPartsAt(void* scratch, int groups, int rows) {
@@ -64,7 +64,7 @@ __device__ __forceinline__ int GroupAt(const LatentRequest& l, int64_t t, int64_
 // Every wave by itself, a lane a request: length_of(r) is a request's of the line. The run [from, to) of this workgroup (`index` of `groups`), the request that
 // holds its beginning, and the line before that.
 struct LatentRun {
-  int64_t from, to, before;
+  int64_t from, to, before, per;
   int request;
 };
 template <class LengthOf>
@@ -87,7 +87,7 @@ __device__ __forceinline__ LatentRun RunOf(int requests, int index, int groups, 
   int64_t total = from_lane(first_upto, kWave - 1);
   for (int r0 = kWave; r0 < requests; r0 += kWave) total += from_lane(sums(r0 + lane < requests ? length_of(r0 + lane) : 0), kWave - 1);
   const int64_t per = max(Over(total + groups - 1, groups), least);
-  LatentRun run = {index * per, min((index + 1) * per, total), 0, 0};
+  LatentRun run = {index * per, min((index + 1) * per, total), 0, per, 0};
   if (run.from >= run.to) return run;
   for (int r0 = 0; r0 < requests; r0 += kWave) {
     const int64_t mine = r0 == 0 ? first : r0 + lane < requests ? length_of(r0 + lane) : 0;
@@ -127,6 +127,15 @@ __device__ __forceinline__ T Scalar(T v) {
 }
 __device__ __forceinline__ LatentRequest Scalar(const LatentRequest& l) { return {Scalar(l.start), Scalar(l.n), Scalar(l.length), Scalar(l.base), Scalar(l.groups)}; }
 
+// Which workgroups hold parts of a pair at `from` of the line: those from its first tile's to its last one's, each of which has a tile (a run is at least as long).
+struct LatentOwners {
+  int first, count;
+};
+__device__ __forceinline__ LatentOwners OwnersOf(int64_t from, int seen, int tile, int64_t per) {
+  const int64_t first = Over(from + kVisit, per), last = Over(from + kVisit + static_cast<int64_t>(seen - 1) / tile * tile, per);
+  return {static_cast<int>(first), static_cast<int>(last - first) + 1};
+}
+
 // ---- the parts of a pair, joined. They are as the lanes held them: an item is UNIT rows by 256 / UNIT dimensions, lane l four of them, 4 (l / UNIT) on, of row
 // l % UNIT. The pair's items are dealt to the workgroups (one for each of the first launch's) that hold its parts, so that what one reads is
 // about the same whatever the number of parts. A wave takes an item, or where there are many parts a workgroup one together, the waves' parts in turn. Bound by the
@@ -150,26 +159,8 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void LatentJoinKernel(const Joi
   const int x = blockIdx.x;
   const int which = blockIdx.y;
   const I32x4 mine = *reinterpret_cast<const I32x4*>(a.parts.which + 8 * x + 4 * which);
-  const int request = mine[0], pair = mine[1], rows = mine[2], token0 = mine[3];
-  if (request < 0) return;
-  int leader = x;
-  if (which == 0) {  // the last workgroup before this one that begins a pair has begun this one
-    for (int base = x - 1;; base -= kWave) {
-      const int g = base - lane;
-      const uint64_t begins = __ballot(g >= 0 && a.parts.which[8 * max(g, 0) + 4] >= 0);
-      leader = base - (__ffsll(static_cast<unsigned long long>(begins)) - 1);
-      if (begins != 0 || base < kWave) break;
-    }
-  }
-  // The parts after the first are the next workgroups' later ones, as long as they are of this pair.
-  int count = 1;
-  for (int base = leader + 1;; base += kWave) {
-    const int g = base + lane, at = 8 * min(g, a.groups - 1);
-    const uint64_t others = ~__ballot(g < a.groups && a.parts.which[at] == request && a.parts.which[at + 1] == pair);
-    const int here = others == 0 ? kWave : __ffsll(static_cast<unsigned long long>(others)) - 1;
-    count += here;
-    if (here < kWave) break;
-  }
+  const int leader = mine[0], pair = mine[1], rows = mine[2] & 0xFF, count = mine[2] >> 8, token0 = mine[3];
+  if (leader < 0) return;
   const auto unit = [&](int i, int u) { return static_cast<int64_t>(i == 0 ? 2 * leader + 1 : 2 * (leader + i)) * (ROWS / UNIT) + u; };
   const int items = (rows + UNIT - 1) / UNIT * kBlocks;
   // In loads that wait for each other; a meeting of the waves counts as one.

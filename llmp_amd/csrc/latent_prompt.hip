@@ -91,14 +91,14 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
   const int groups = gridDim.x;
   const int index = LINE ? static_cast<int>(blockIdx.x % 8) * (groups / 8) + static_cast<int>(blockIdx.x / 8) : 0;
   int request, head = 0, k = 0;
-  int64_t u = 0, u_end = 1, before = 0;
+  int64_t u = 0, u_end = 1, before = 0, per = 1, pair_from = 0;
   if constexpr (LINE) {
     if (tid < 2) a.parts.which[(2 * index + tid) * 4] = -1;
     const LatentRun run = RunOf(op.requests, index, groups, kLeast, [&](int r) {
       const LatentRequest l = PromptOf(op, r).l;
       return LineBefore(l, kPromptRows, l.groups) * op.heads;
     });
-    u = run.from, u_end = run.to, before = run.before, request = run.request;
+    u = run.from, u_end = run.to, before = run.before, request = run.request, per = run.per;
   } else {
     const uint32_t sets = static_cast<uint32_t>(op.requests) * op.heads, padded = (sets + 7) / 8 * 8, set = blockIdx.x % padded;
     if (set >= sets) return;
@@ -117,13 +117,13 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
       ++request;
       continue;
     }
-    head = static_cast<int>((u - before) / a_head);
+    head = static_cast<int>(Over(u - before, a_head));
     const int64_t head_from = before + head * a_head;
     k = GroupAt(r.l, kPromptRows, u - head_from);
     any_to = SeenOf(r.l, kPromptRows, k);
-    const int64_t from = head_from + LineBefore(r.l, kPromptRows, k);
-    const int x0 = static_cast<int>(u - from), x1 = static_cast<int>(min(u_end - from, static_cast<int64_t>(any_to + kVisit)));
-    u = from + x1;
+    pair_from = head_from + LineBefore(r.l, kPromptRows, k);
+    const int x0 = static_cast<int>(u - pair_from), x1 = static_cast<int>(min(u_end - pair_from, static_cast<int64_t>(any_to + kVisit)));
+    u = pair_from + x1;
     piece = PieceOf(any_to, kKeys, x0, x1);
     if (!piece.any) continue;
   } else {
@@ -347,8 +347,8 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
   } else {
     const int which = 2 * index + (piece.begins ? 1 : 0);
     if (tid == 0) {
-      int32_t* const p = a.parts.which + 4 * which;
-      p[0] = request, p[1] = k * op.heads + head, p[2] = min(r.l.n - first, kPromptRows), p[3] = r.l.start + first;
+      const LatentOwners owners = OwnersOf(pair_from, any_to, kKeys, per);
+      *reinterpret_cast<I32x4*>(a.parts.which + 4 * which) = I32x4{owners.first, k * op.heads + head, min(r.l.n - first, kPromptRows) | owners.count << 8, r.l.start + first};
     }
     if (busy) {
       const int64_t unit = static_cast<int64_t>(which) * (kPromptRows / 32) + wave;

@@ -864,7 +864,7 @@ def rope_table(n_dims, base=10000.0, *, freq_scale=1.0, ext_factor=0.0, attn_fac
 
 def _turns(table):
     turns = table["turns"]
-    assert turns.is_cuda and turns.dtype is torch.int64 and turns.dim() == 1 and turns.is_contiguous()
+    assert turns.dtype is torch.int64 and turns.dim() == 1 and turns.is_contiguous()
     return turns
 
 
@@ -875,7 +875,7 @@ def _here(*tensors):
     """On the current device: its stream is the one that the launch goes to."""
     device = torch._C._cuda_getDevice()
     for t in tensors:
-        assert t.is_cuda and t.get_device() == device, "tensors on the current device"
+        assert t.get_device() == device, "tensors on the current device"
 
 
 def rope(x, positions, table, *, layout="half", first=0, inverse=False, out=None):
@@ -910,14 +910,17 @@ def latent_cache(pages, page, width, rope, dtype=torch.bfloat16, bits=16, device
 
 
 def _latent_cache(cache):
-    latent, rope, scale = cache["latent"], cache["rope"], cache.get("scale")
-    pages, page, width = latent.shape
-    whole = (latent.is_contiguous() and rope.is_contiguous() and rope.dim() == 3 and rope.shape[:2] == (pages, page)
-             and latent.dtype is (rope.dtype if scale is None else torch.uint8)
-             and (scale is None or (scale.dtype is torch.uint8 and scale.is_contiguous() and scale.shape == (pages, page))))
+    latent, rope, scale, dtype = cache["latent"], cache["rope"], cache.get("scale"), cache["rope"].dtype
+    (pages, page, width), (rope_pages, rope_page, rope_width) = latent.shape, rope.shape
+    whole = latent.is_contiguous() and rope.is_contiguous() and rope_pages == pages and rope_page == page
+    if scale is None:
+        whole = whole and latent.dtype is dtype
+        _here(latent, rope)
+    else:
+        whole = whole and latent.dtype is torch.uint8 and scale.dtype is torch.uint8 and scale.is_contiguous() and scale.shape == (pages, page)
+        _here(latent, rope, scale)
     assert whole, "the cache's arrays are whole, of one set of sizes"
-    _here(latent, rope, *(() if scale is None else (scale,)))
-    return _lib.LatentCache(latent.data_ptr(), _ptr(scale), rope.data_ptr(), _X_TYPES[rope.dtype], pages, page, width, rope.shape[2])
+    return _lib.LatentCache(latent.data_ptr(), _ptr(scale), rope.data_ptr(), _X_TYPES[dtype], pages, page, width, rope_width)
 
 
 def latent_store(cache, latent, rope, slots, positions=None, table=None, *, layout="half", weight=None, eps=1e-6):
@@ -994,7 +997,7 @@ def latent_attend(cache, q_latent, q_rope, table, lengths, starts, scale, *, bef
     if before is not None:
         _int32(before)
         assert before.shape == (n,)
-    _here(q_latent, q_rope, out, table, lengths, starts)
+    _here(q_latent, q_rope, out, table, lengths, starts, *(() if before is None else (before,)))
     if tokens == 0:
         return out
     op = _lib.LatentAttend(c, q_latent.data_ptr(), q_rope.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(before),
@@ -1025,7 +1028,7 @@ def latent_prompt(q, k, k_rope, v, starts, scale, *, key_starts=None, most=None,
     if key_starts is not None:
         _int32(key_starts)
         assert key_starts.shape == starts.shape
-    _here(q, k, k_rope, v, out, starts)
+    _here(q, k, k_rope, v, out, starts, *(() if key_starts is None else (key_starts,)))
     if tokens == 0:
         return out
     op = _lib.LatentPrompt(q.data_ptr(), k.data_ptr(), k_rope.data_ptr(), v.data_ptr(), out.data_ptr(), starts.data_ptr(), _ptr(key_starts), qt, qh, kt, kh,
