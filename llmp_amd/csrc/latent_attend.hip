@@ -25,6 +25,9 @@ constexpr int kFewRows = 16, kManyRows = 128;
 constexpr int kLdsBytes = 160 * 1024;
 constexpr int kLeast = 128;  // of the line, to a workgroup: finer parts cost more to write and to join (16 rows, 16 requests of up to 2000: 30.2 us so, 32.4 at 256)
 
+// The forms: up to 16 rows a request, each wave a tile by itself; 128 rows a workgroup, 16 a wave; so, 32 a wave, two workgroups a compute unit.
+enum Form { kFewForm, kManyForm, kWideForm };
+
 struct LatentArgs {
   llmp_latent_attend op;
   LatentParts parts;
@@ -32,20 +35,23 @@ struct LatentArgs {
   int tokens_a_pair, pairs_a_token;  // rows of several whole tokens, or of part of one
 };
 
-template <int R, int P, bool EIGHT, bool FEW>
+template <int R, int P, bool EIGHT, Form FORM>
 struct LatentGeo {
-  static constexpr int kWaves = FEW ? 4 : 8, kThreads = kWaves * kWave;
-  static constexpr int kRows = FEW ? kFewRows : kManyRows;
+  static constexpr bool kFew = FORM == kFewForm;
+  static constexpr int kSets = FORM == kWideForm ? 2 : 1;  // groups of 16 rows that a wave has
+  static constexpr int kAUnit = kSets;                     // workgroups a compute unit
+  static constexpr int kWaves = kFew ? 4 : 8 / kSets, kThreads = kWaves * kWave;
+  static constexpr int kRows = kFew ? kFewRows : kManyRows;
   static constexpr int kPitch = EIGHT ? R : 2 * R, kRopePitch = 2 * P;
-  static constexpr int kLatentBytes = kTokens * kPitch, kRopeBytes = kTokens * kRopePitch, kScaleBytes = EIGHT && !FEW ? 256 : 0;
+  static constexpr int kLatentBytes = kTokens * kPitch, kRopeBytes = kTokens * kRopePitch, kScaleBytes = EIGHT && !kFew ? 256 : 0;
   static constexpr int kTile = kLatentBytes + kRopeBytes + kScaleBytes;
-  static constexpr int kQueries = FEW ? 0 : kManyRows * 2 * P;  // the queries' rotated part, where registers are short
-  static constexpr int kRing = FEW ? std::min(2, kLdsBytes / 4 / kTile) : std::min(5, (kLdsBytes - kQueries) / kTile);
-  static constexpr int kSharing = FEW ? 1 : kWaves;  // waves that bring a tile in
+  static constexpr int kQueries = kFew ? 0 : kManyRows * 2 * P;  // the queries' rotated part, where registers are short
+  static constexpr int kRing = kFew ? std::min(2, kLdsBytes / 4 / kTile) : std::min(5, (kLdsBytes / kAUnit - kQueries) / kTile);
+  static constexpr int kSharing = kFew ? 1 : kWaves;  // waves that bring a tile in
   static constexpr int kLatentLoads = kLatentBytes / 1024 / kSharing, kRopeLoads = (kRopeBytes / 1024 + kSharing - 1) / kSharing;
   static constexpr int kLoads = kLatentLoads + kRopeLoads + (kScaleBytes > 0 ? 1 : 0);  // a wave's for a tile
   static constexpr int kArea = kFewRows * R * 4 + 2 * kFewRows * 4;  // the few rows' form: a wave's results for the others
-  static constexpr int kLds = FEW ? std::max(4 * kRing * kTile, 4 * kArea) : kRing * kTile + kQueries;
+  static constexpr int kLds = kFew ? std::max(4 * kRing * kTile, 4 * kArea) : kRing * kTile + kQueries;
 
   // What the pieces (of 16 bytes) of a token's row are turned by: the 16 lanes that a 16-byte read takes at once (KPiece in paged_attend.h), and the 32
   // that a transposing read does, then find theirs in all banks.
@@ -64,26 +70,34 @@ __device__ __forceinline__ LatentRequest AttendRequest(const LatentArgs& a, int 
   return {q.start, q.n, q.length, q.base, (q.n + a.tokens_a_pair - 1) / a.tokens_a_pair};
 }
 
-template <int TYPE, int R, int P, bool EIGHT, bool FEW>
-__global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 : 2)) void LatentAttendKernel(const LatentArgs a) {
-  using G = LatentGeo<R, P, EIGHT, FEW>;
+template <int TYPE, int R, int P, bool EIGHT, Form FORM>
+__global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == kFewForm ? 1 : 2)) void LatentAttendKernel(const LatentArgs a) {
+  using G = LatentGeo<R, P, EIGHT, FORM>;
+  constexpr bool FEW = G::kFew;
   using S = Sixteen<TYPE>;
   typedef typename S::Eight Eight;
-  constexpr int kSteps = R / 32, kRopeSteps = P / 32, kBlocks = R / 16;
+  constexpr int kSteps = R / 32, kRopeSteps = P / 32, kBlocks = R / 16, kSets = G::kSets;
   constexpr int kLogits = 8;  // a lane's of a tile
   constexpr int kKeyGroup = FEW ? 8 : 2, kValueGroup = FEW ? 8 : 2;  // products that are read for at a time
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const llmp_latent_attend& op = a.op;
   const llmp_latent_cache& c = op.cache;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int quarter = lane / 16, column = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // (All that depends on the lane alone is worked out where it is needed, from a lane number as something new: kept, it is the registers too many, and what the
+  // compiler then brings back from memory waits for the tiles under way.)
+  const auto lane_anew = [&]() {
+    if constexpr (FEW) return static_cast<int>(threadIdx.x & (kWave - 1));
+    uint32_t all = ~0u;
+    asm volatile("" : "+s"(all));
+    return static_cast<int>(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)));
+  };
   const int groups = gridDim.x, w = blockIdx.x;
   const uint32_t ring_off = FEW ? wave * G::kRing * G::kTile : 0;
   const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + ring_off;
 
   // ---- this workgroup's run of the line
   const int64_t t = a.tokens_a_pair;
-  if (tid < 2) a.parts.which[(2 * w + tid) * 4] = -1;
+  if (threadIdx.x < 2) a.parts.which[(2 * w + threadIdx.x) * 4] = -1;
   const LatentRun run = RunOf(op.requests, w, groups, kLeast, [&](int r) {
     const LatentRequest l = AttendRequest(a, r);
     return LineBefore(l, t, l.groups) * a.pairs_a_token;
@@ -115,59 +129,55 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
 
         // ---- the lane's row.
         const int first_token = k * a.tokens_a_pair;
-        const int row0 = FEW ? 0 : 16 * wave;
-        int rows, token, head;  // of the pair, of the lane's row
-        {
-          const int row = row0 + column;
-          if (a.pairs_a_token == 1) {
-            rows = min(a.tokens_a_pair, l.n - first_token) * op.heads;
-            token = first_token + row / op.heads;
-            head = row % op.heads;
-          } else {
-            rows = min(G::kRows, op.heads - part * G::kRows);
-            token = first_token;
-            head = part * G::kRows + row;
-          }
-        }
-        const bool real = row0 + column < rows;
-        token = real ? token : first_token;
-        head = real ? head : 0;
-        const int see_to = real ? max(min(l.base + token + 1, l.length), 0) : 0;
+        const int row0 = FEW ? 0 : 16 * kSets * wave;
+        const int rows = a.pairs_a_token == 1 ? min(a.tokens_a_pair, l.n - first_token) * op.heads : min(G::kRows, op.heads - part * G::kRows);
+        struct Row {
+          int token, head, see_to;
+          bool real;
+        };
+        const auto row_of = [&](int s) {
+          const int row = row0 + 16 * s + lane_anew() % 16;
+          Row r = {first_token, 0, 0, row < rows};
+          if (r.real && a.pairs_a_token == 1) r.token = first_token + row / op.heads, r.head = row % op.heads;
+          if (r.real && a.pairs_a_token != 1) r.head = part * G::kRows + row;
+          if (r.real) r.see_to = max(min(l.base + r.token + 1, l.length), 0);
+          return r;
+        };
         const bool busy = row0 < rows;
         const int all_rows_to = max(min(l.base + first_token + 1, l.length), 0);  // seen by all rows of the pair
         const int all_to = max(min(l.base + first_token + 1 + (a.pairs_a_token == 1 ? row0 / op.heads : 0), l.length), 0);  // seen by all of the wave's rows
 
         constexpr bool kRopeInLds = G::kQueries > 0;
-        Eight q[kSteps + (kRopeInLds ? 0 : kRopeSteps)];
-        const uint32_t q_rope = G::kRing * G::kTile + wave * kRopeSteps * 1024;
-        {
-          const uint16_t* const ql = static_cast<const uint16_t*>(op.q_latent) + (l.start + token) * op.q_latent_token_stride + head * op.q_latent_head_stride + 8 * quarter;
-          const uint16_t* const qr = static_cast<const uint16_t*>(op.q_rope) + (l.start + token) * op.q_rope_token_stride + head * op.q_rope_head_stride + 8 * quarter;
+        Eight q[kSets][kSteps + (kRopeInLds ? 0 : kRopeSteps)];
+        const uint32_t q_rope = G::kRing * G::kTile + wave * kSets * kRopeSteps * 1024;
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const Row row = row_of(s);
+          const int lane = lane_anew(), quarter = lane / 16;
+          const uint16_t* const ql = static_cast<const uint16_t*>(op.q_latent) + (l.start + row.token) * op.q_latent_token_stride + row.head * op.q_latent_head_stride + 8 * quarter;
+          const uint16_t* const qr = static_cast<const uint16_t*>(op.q_rope) + (l.start + row.token) * op.q_rope_token_stride + row.head * op.q_rope_head_stride + 8 * quarter;
 #pragma unroll
           for (int x = 0; x < kSteps + kRopeSteps; ++x) {
             U32x4 v = *reinterpret_cast<const U32x4*>(x < kSteps ? ql + 32 * x : qr + 32 * (x - kSteps));
             v ^= U32x4{flip, flip, flip, flip};
             if (kRopeInLds && x >= kSteps) {
-              *reinterpret_cast<U32x4*>(lds + q_rope + (x - kSteps) * 1024 + 16 * lane) = v;
+              *reinterpret_cast<U32x4*>(lds + q_rope + (s * kRopeSteps + x - kSteps) * 1024 + 16 * lane) = v;
             } else {
-              q[x] = __builtin_bit_cast(Eight, v);
+              q[s][x] = __builtin_bit_cast(Eight, v);
             }
           }
         }
-        F32x4 out[kBlocks];
+        F32x4 out[kSets][kBlocks];
+        float top[kSets], sum[kSets];
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) out[b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        float top = -INFINITY, sum = 0.0f;
+        for (int s = 0; s < kSets; ++s) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) out[s][b] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          top[s] = -INFINITY, sum[s] = 0.0f;
+        }
 
         // ---- the tiles. A lane holds the cache's row of the first token of one 16-token group of the line (-1: no page); they are looked up 64
         // at a time.
-        // (All that depends on the lane alone is worked out at every tile, from a lane number as something new: kept, it is the registers too many, and
-        // what the compiler then brings back from memory waits for the tiles under way.)
-        const auto lane_anew = [&]() {
-          int l = lane;
-          if constexpr (!FEW) asm volatile("" : "+v"(l));
-          return l;
-        };
         const int32_t* const table = op.table + request * op.table_stride;
         int held_from = -1, held = 0;
         const auto look_up = [&](int tile) {
@@ -201,7 +211,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           const uint8_t* const rope_b = static_cast<const uint8_t*>(c.rope) + static_cast<int64_t>(row_b) * G::kRopePitch;
           const uint32_t to = Scalar(ring_at + slot * G::kTile);
           // (Lanes and waves as something new at every tile: the compiler otherwise keeps every load's offsets, and then spills them.)
-          int lane_now = lane, wave_now = FEW ? 0 : wave;
+          int lane_now = lane_anew(), wave_now = FEW ? 0 : wave;
           asm volatile("" : "+v"(lane_now));
           asm volatile("" : "+s"(wave_now));
           const auto load = [&](auto whole) {
@@ -279,12 +289,14 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         };
 
         // A tile's logits of a wave's rows: element i is token 8 quarter + i.
-        float dots[kLogits];
+        float dots[kSets][kLogits];
         const auto scales = [&](uint32_t tile, float (&scale)[kLogits]) {
           uint2 e;
           if constexpr (FEW) {
-            const U32x4 four = quarter < 2 ? scales_now.a : scales_now.b;
-            e = quarter % 2 == 0 ? make_uint2(four.x, four.y) : make_uint2(four.z, four.w);
+            const int quarter = lane_anew() / 16;
+            const U32x4 a4 = scales_now.a, b4 = scales_now.b;  // (a choice of places would keep them in memory)
+            const uint32_t x = quarter < 2 ? a4.x : b4.x, y = quarter < 2 ? a4.y : b4.y, z = quarter < 2 ? a4.z : b4.z, w4 = quarter < 2 ? a4.w : b4.w;
+            e = make_uint2(quarter % 2 == 0 ? x : z, quarter % 2 == 0 ? y : w4);
           } else {
             e = *reinterpret_cast<const uint2*>(lds + tile + G::kLatentBytes + G::kRopeBytes + 8 * (lane_anew() / 16));
           }
@@ -297,7 +309,9 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
         const auto keys = [&](uint32_t tile) {
           const Places p = places();
           const uint32_t key_at = tile + p.key, rope_at = tile + p.rope, query_at = kRopeInLds ? q_rope + 16 * lane_anew() : 0;
-          F32x4 sums[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          F32x4 sums[kSets][2];
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) sums[s][0] = sums[s][1] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
           const auto steps = [&](auto from, auto to) {
             constexpr int kFrom = decltype(from)::value;
             // (Steps 256 bytes apart side by side: their places are one with two constants.)
@@ -306,13 +320,16 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
               const int x = kFrom + i / 2;
               return x >= kSteps ? x : x / kSame + kSteps / kSame * (x % kSame);
             };
-            ProductsInGroups<2 * (decltype(to)::value - kFrom), kKeyGroup, Eight>([&](int i) { return key(key_at, rope_at, step_of(i), i % 2); },
-                                                                                  [&](int i, Eight k) {
-                                                                                    const int x = step_of(i);
-                                                                                    const Eight query = kRopeInLds && x >= kSteps ? *reinterpret_cast<const Eight*>(lds + query_at + (x - kSteps) * 1024)
-                                                                                                                                  : q[kRopeInLds && x >= kSteps ? 0 : x];
-                                                                                    sums[i % 2] = S::Product16(k, query, sums[i % 2]);
-                                                                                  });
+            ProductsInGroups<2 * (decltype(to)::value - kFrom), kKeyGroup, Eight>(
+                [&](int i) { return key(key_at, rope_at, step_of(i), i % 2); },
+                [&](int i, Eight k) {
+                  const int x = step_of(i);
+#pragma unroll
+                  for (int s = 0; s < kSets; ++s) {
+                    const Eight query = kRopeInLds && x >= kSteps ? *reinterpret_cast<const Eight*>(lds + query_at + (s * kRopeSteps + x - kSteps) * 1024) : q[s][kRopeInLds && x >= kSteps ? 0 : x];
+                    sums[s][i % 2] = S::Product16(k, query, sums[s][i % 2]);
+                  }
+                });
           };
           constexpr std::integral_constant<int, 0> kBegin{};
           constexpr std::integral_constant<int, kSteps> kMiddle{};
@@ -323,73 +340,83 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             float scale8[kLogits];
             scales(tile, scale8);
 #pragma unroll
-            for (int i = 0; i < kLogits; ++i) sums[i / 4][i % 4] *= scale8[i];
+            for (int i = 0; i < kSets * kLogits; ++i) sums[i / kLogits][i / 4 % 2][i % 4] *= scale8[i % kLogits];
             steps(kMiddle, kEnd);
           } else {
             steps(kBegin, kEnd);
           }
 #pragma unroll
-          for (int i = 0; i < kLogits; ++i) dots[i] = sums[i / 4][i % 4];
+          for (int i = 0; i < kSets * kLogits; ++i) dots[i / kLogits][i % kLogits] = sums[i / kLogits][i / 4 % 2][i % 4];
         };
         const auto values = [&](int tile_number, uint32_t tile, uint32_t gone, bool alone) {
           const uint32_t value_at = tile + places().value;
           const int p0 = tile_number * kTokens;
           float scale8[kLogits];
           if constexpr (EIGHT) scales(tile, scale8);
-          // ---- what the rows see
           bool garbage = false;
-          float worth = sign_scale;
-          if (p0 + kTokens > all_to || gone != 0) {
-            asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
-            const int lane_token = 8 * (lane_anew() / 16);
-            const int to = (gone >> (lane_token >> 4) & 1) != 0 ? 0 : see_to - p0 - lane_token;
+          Eight weights[kSets];
+          const bool masked = p0 + kTokens > all_to || gone != 0;
+          const float worth = masked ? 1.0f : sign_scale;
 #pragma unroll
-            for (int i = 0; i < kLogits; ++i) {
-              // (A value that is no number, or one that a product with zero would make none, has no finite product with any query.)
-              garbage |= (i >= to) & !(fabsf(dots[i]) < INFINITY);
-              dots[i] = i < to ? dots[i] * sign_scale : -INFINITY;
-              if constexpr (EIGHT) scale8[i] = i < to ? scale8[i] : 0.0f;
+          for (int s = 0; s < kSets; ++s) {
+            // ---- what the rows see
+            float (&dot)[kLogits] = dots[s];
+            float copy8[kLogits];
+            float (&seen8)[kLogits] = kSets == 1 ? scale8 : copy8;
+            if constexpr (EIGHT && kSets > 1) {
+#pragma unroll
+              for (int i = 0; i < kLogits; ++i) seen8[i] = scale8[i];
             }
-            worth = 1.0f;
-          }
-          // ---- softmax. Eight-bit weights take the token's scale along; the maximum is of both.
-          float peak = -INFINITY;
-          if constexpr (EIGHT) {
+            if (masked) {
+              asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
+              const int lane_token = 8 * (lane_anew() / 16);
+              const int to = (gone >> (lane_token >> 4) & 1) != 0 ? 0 : row_of(s).see_to - p0 - lane_token;
 #pragma unroll
-            for (int i = 0; i < kLogits; ++i) peak = fmaxf(peak, fmaf(dots[i], worth, __builtin_amdgcn_logf(fmaxf(scale8[i], 0x1p-80f))));
-          } else {
-#pragma unroll
-            for (int i = 0; i < kLogits; i += 2) peak = fmaxf(fmaxf(peak, dots[i]), dots[i + 1]);
-            peak *= worth;
-          }
-          peak = AcrossGroupsMax(peak);
-          if (__any(peak > top + (kUp + kFollow))) {
-            const float higher = fmaxf(top, peak - kUp);
-            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
-            top = higher;
-            sum *= keep;
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
-          }
-          const float less = top == -INFINITY ? 0.0f : top;
-          Eight weights;
-#pragma unroll
-          for (int i = 0; i < kLogits; i += 2) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(dots[i], worth, -less)), p1 = __builtin_amdgcn_exp2f(fmaf(dots[i + 1], worth, -less));
+              for (int i = 0; i < kLogits; ++i) {
+                // (A value that is no number, or one that a product with zero would make none, has no finite product with any query.)
+                garbage |= (i >= to) & !(fabsf(dot[i]) < INFINITY);
+                dot[i] = i < to ? dot[i] * sign_scale : -INFINITY;
+                if constexpr (EIGHT) seen8[i] = i < to ? seen8[i] : 0.0f;
+              }
+            }
+            // ---- softmax. Eight-bit weights take the token's scale along; the maximum is of both.
+            float peak = -INFINITY;
             if constexpr (EIGHT) {
-              sum += p + p1;
-              weights[i] = static_cast<typename S::One>(p * scale8[i]), weights[i + 1] = static_cast<typename S::One>(p1 * scale8[i + 1]);
+#pragma unroll
+              for (int i = 0; i < kLogits; ++i) peak = fmaxf(peak, fmaf(dot[i], worth, __builtin_amdgcn_logf(fmaxf(seen8[i], 0x1p-80f))));
             } else {
-              weights[i] = static_cast<typename S::One>(p), weights[i + 1] = static_cast<typename S::One>(p1);
-              // (The sum is of the weights as they are rounded, two in an instruction.)
-              sum = S::AddTwo(typename S::Two{weights[i], weights[i + 1]}, sum);
+#pragma unroll
+              for (int i = 0; i < kLogits; i += 2) peak = fmaxf(fmaxf(peak, dot[i]), dot[i + 1]);
+              peak *= worth;
+            }
+            peak = AcrossGroupsMax(peak);
+            if (__any(peak > top[s] + (kUp + kFollow))) {
+              const float higher = fmaxf(top[s], peak - kUp);
+              const float keep = top[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[s] - higher);
+              top[s] = higher;
+              sum[s] *= keep;
+#pragma unroll
+              for (int b = 0; b < kBlocks; ++b) out[s][b] *= keep;
+            }
+            const float less = top[s] == -INFINITY ? 0.0f : top[s];
+#pragma unroll
+            for (int i = 0; i < kLogits; i += 2) {
+              const float p = __builtin_amdgcn_exp2f(fmaf(dot[i], worth, -less)), p1 = __builtin_amdgcn_exp2f(fmaf(dot[i + 1], worth, -less));
+              if constexpr (EIGHT) {
+                sum[s] += p + p1;
+                weights[s][i] = static_cast<typename S::One>(p * seen8[i]), weights[s][i + 1] = static_cast<typename S::One>(p1 * seen8[i + 1]);
+              } else {
+                weights[s][i] = static_cast<typename S::One>(p), weights[s][i + 1] = static_cast<typename S::One>(p1);
+                // (The sum is of the weights as they are rounded, two in an instruction.)
+                sum[s] = S::AddTwo(typename S::Two{weights[s][i], weights[s][i + 1]}, sum[s]);
+              }
             }
           }
           if (alone && __any(garbage)) {
             // A token that some row must not see holds infinities or NaN, which a weight of zero does not keep out: they become zeros in LDS. (A row that
             // sees them has no finite logit there, and no finite sum. `alone`: nobody reads the tile as keys any more. Elsewhere all rows see the same.)
 #pragma unroll 1
-            for (uint32_t i = 16 * lane; i < G::kLatentBytes; i += 1024) {
+            for (uint32_t i = 16 * lane_anew(); i < G::kLatentBytes; i += 1024) {
               U32x4* const at = reinterpret_cast<U32x4*>(lds + tile + i);
               *at = EIGHT ? FiniteCodes(*at) : Finite<TYPE>(*at);
             }
@@ -400,7 +427,10 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             return i / kSame + kBlocks / kSame * (i % kSame);
           };
           ProductsInGroups<kBlocks, kValueGroup, Eight>([&](int i) { return value(value_at, block_of(i)); },
-                                                        [&](int i, Eight v) { out[block_of(i)] = S::Product16(v, weights, out[block_of(i)]); });
+                                                        [&](int i, Eight v) {
+#pragma unroll
+                                                          for (int s = 0; s < kSets; ++s) out[s][block_of(i)] = S::Product16(v, weights[s], out[s][block_of(i)]);
+                                                        });
         };
 
         if constexpr (FEW) {
@@ -453,28 +483,30 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
           }
           MeetLds();
         }
-        sum = AcrossGroupsSum(sum);
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) sum[s] = AcrossGroupsSum(sum[s]);
 
         // ---- the few rows' form: the waves' results added up, a quarter of the dimensions each.
+        const int lane = lane_anew(), quarter = lane / 16, column = lane % 16;
         constexpr int kMine = FEW ? kBlocks / 4 : kBlocks;  // blocks that the wave writes
         const int first_block = FEW ? wave * kMine : 0;
-        F32x4 result[kMine];
         if constexpr (FEW) {
+          F32x4 result[kMine];
           MeetLds();
           uint8_t* const area = lds + wave * G::kArea;
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) reinterpret_cast<F32x4*>(area)[b * kWave + lane] = out[b];
-          if (quarter == 0) reinterpret_cast<float2*>(area + kFewRows * R * 4)[column] = make_float2(top, sum);
+          for (int b = 0; b < kBlocks; ++b) reinterpret_cast<F32x4*>(area)[b * kWave + lane] = out[0][b];
+          if (quarter == 0) reinterpret_cast<float2*>(area + kFewRows * R * 4)[column] = make_float2(top[0], sum[0]);
           MeetLds();
           float2 numbers[4];
-          top = -INFINITY;
+          top[0] = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) numbers[i] = reinterpret_cast<const float2*>(lds + i * G::kArea + kFewRows * R * 4)[column], top = fmaxf(top, numbers[i].x);
-          sum = 0.0f;
+          for (int i = 0; i < 4; ++i) numbers[i] = reinterpret_cast<const float2*>(lds + i * G::kArea + kFewRows * R * 4)[column], top[0] = fmaxf(top[0], numbers[i].x);
+          sum[0] = 0.0f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            numbers[i].x = __builtin_amdgcn_exp2f(numbers[i].x - (top == -INFINITY ? 0.0f : top));
-            sum = fmaf(numbers[i].x, numbers[i].y, sum);
+            numbers[i].x = __builtin_amdgcn_exp2f(numbers[i].x - (top[0] == -INFINITY ? 0.0f : top[0]));
+            sum[0] = fmaf(numbers[i].x, numbers[i].y, sum[0]);
           }
 #pragma unroll
           for (int b = 0; b < kMine; ++b) {
@@ -483,34 +515,38 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
             for (int i = 0; i < 4; ++i) result[b] += reinterpret_cast<const F32x4*>(lds + i * G::kArea)[(first_block + b) * kWave + lane] * numbers[i].x;
           }
           MeetLds();
-        } else {
 #pragma unroll
-          for (int b = 0; b < kMine; ++b) result[b] = out[b];
+          for (int b = 0; b < kMine; ++b) out[0][b] = result[b];
         }
 
         // ---- out, or a part for the join. Element e of a block is dimension 4 quarter + e of it.
         if (piece.begins && piece.ends) {
-          if (busy && real) {
-            const float by = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-            const int64_t to = (l.start + token) * op.out_token_stride + head * op.out_head_stride + 16 * first_block + 4 * quarter;
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) {
+            const Row row = row_of(s);
+            if (!row.real) continue;
+            const float by = sum[s] > 0.0f || sum[s] != sum[s] ? 1.0f / sum[s] : 0.0f;
+            const int64_t to = (l.start + row.token) * op.out_token_stride + row.head * op.out_head_stride + 16 * first_block + 4 * quarter;
 #pragma unroll
             for (int b = 0; b < kMine; ++b) {
-              const float v[4] = {result[b][0] * by, result[b][1] * by, result[b][2] * by, result[b][3] * by};
+              const float v[4] = {out[s][b][0] * by, out[s][b][1] * by, out[s][b][2] * by, out[s][b][3] * by};
               StoreValues<TYPE, 4>(op.out, to + 16 * b, v);
             }
           }
         } else {
           const int which = 2 * w + (piece.begins ? 1 : 0);
-          if (tid == 0) {
+          if (wave == 0 && lane == 0) {
             const LatentOwners owners = OwnersOf(from, seen, kTokens, run.per);
             *reinterpret_cast<I32x4*>(a.parts.which + 4 * which) = I32x4{owners.first, k * a.pairs_a_token + part, rows | owners.count << 8, l.start + first_token};
           }
-          if (busy) {
-            const int64_t rows16 = static_cast<int64_t>(which) * (G::kRows / 16) + row0 / 16;
-            if (quarter == 0) a.parts.numbers[rows16 * 16 + column] = make_float2(top, sum);
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) {
+            if (row0 + 16 * s >= rows) continue;
+            const int64_t rows16 = static_cast<int64_t>(which) * (G::kRows / 16) + row0 / 16 + s;
+            if (quarter == 0) a.parts.numbers[rows16 * 16 + column] = make_float2(top[s], sum[s]);
             F32x4* const to = reinterpret_cast<F32x4*>(a.parts.values) + (rows16 * kBlocks + first_block) * kWave + lane;
 #pragma unroll
-            for (int b = 0; b < kMine; ++b) to[b * kWave] = result[b];
+            for (int b = 0; b < kMine; ++b) to[b * kWave] = out[s][b];
           }
         }
       }
@@ -521,13 +557,17 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FEW>::kThreads), (FEW ? 1 :
 
 // f with the type, width, rope width, 8 bits or not and the form as constants.
 template <class F>
-void WithForm(const llmp_latent_attend& op, bool few, F&& f) {
+void WithForm(const llmp_latent_attend& op, Form which, F&& f) {
   const auto form = [&](auto type, auto r, auto p) {
-    const bool eight = op.cache.scale != nullptr;
-    if (eight && few) f(type, r, p, std::true_type{}, std::true_type{});
-    if (eight && !few) f(type, r, p, std::true_type{}, std::false_type{});
-    if (!eight && few) f(type, r, p, std::false_type{}, std::true_type{});
-    if (!eight && !few) f(type, r, p, std::false_type{}, std::false_type{});
+    const auto forms = [&](auto eight) {
+      if (which == kFewForm) f(type, r, p, eight, std::integral_constant<Form, kFewForm>{});
+      if (which == kManyForm) f(type, r, p, eight, std::integral_constant<Form, kManyForm>{});
+      if constexpr (decltype(r)::value == 256) {
+        if (which == kWideForm) f(type, r, p, eight, std::integral_constant<Form, kWideForm>{});
+      }
+    };
+    if (op.cache.scale != nullptr) forms(std::true_type{});
+    if (op.cache.scale == nullptr) forms(std::false_type{});
   };
   const auto widths = [&](auto type) {
     const auto rope = [&](auto r) {
@@ -541,8 +581,15 @@ void WithForm(const llmp_latent_attend& op, bool few, F&& f) {
   if (op.cache.type == LLMP_X_F16) widths(std::integral_constant<int, LLMP_X_F16>{});
 }
 
-bool FewRows(const llmp_latent_attend& op) { return static_cast<int64_t>(std::min(op.most_tokens, op.tokens)) * op.heads <= kFewRows; }
-int RowsOf(const llmp_latent_attend& op) { return FewRows(op) ? kFewRows : kManyRows; }
+// 32 rows a wave read LDS half as often and share what is worked out a tile, but there are twice the parts to join: where requests have more rows than one pair.
+// (Width 256, 20 heads, three chunks of up to 300 tokens behind 5000: 94 us, 104 with
+// 16 rows a wave; of codes 127 and 150; 32 requests of two tokens and 128 heads behind up to 9000: 69 and 72; a single pair a request would lose 5 us to the join.)
+Form FormOf(const llmp_latent_attend& op) {
+  const int64_t rows = static_cast<int64_t>(std::min(op.most_tokens, op.tokens)) * op.heads;
+  return rows <= kFewRows ? kFewForm : op.cache.width == 256 && rows > kManyRows ? kWideForm : kManyForm;
+}
+int RowsOf(const llmp_latent_attend& op) { return FormOf(op) == kFewForm ? kFewRows : kManyRows; }
+int GroupsOf(const llmp_latent_attend& op, int cus) { return FormOf(op) == kWideForm ? 2 * cus : cus; }
 
 int CheckLatentAttend(const llmp_latent_attend* op, int cus) {
   if (op == nullptr) return Refuse(1, "latent_attend: null operands");
@@ -574,7 +621,7 @@ using namespace llmp_hip;
 
 extern "C" size_t llmp_hip_latent_attend_scratch(const llmp_latent_attend* op, int cus) {
   if (CheckLatentAttend(op, cus) != 0) return 0;
-  return LatentPartsBytes(cus, RowsOf(*op), op->cache.width);
+  return LatentPartsBytes(GroupsOf(*op, cus), RowsOf(*op), op->cache.width);
 }
 
 extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t scratch_bytes, int cus, void* stream) {
@@ -582,27 +629,27 @@ extern "C" int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratc
   const size_t need = llmp_hip_latent_attend_scratch(op, cus);
   if (scratch == nullptr || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16 != 0)
     return Refuse(1, "latent_attend: %zu bytes of scratch at a 16-byte boundary, not %zu", need, scratch_bytes);
-  const bool few = FewRows(*op);
-  const int rows = RowsOf(*op);
+  const int rows = RowsOf(*op), groups = GroupsOf(*op, cus);
   LatentArgs a;
   a.op = *op;
-  a.parts = LatentPartsAt(scratch, cus, rows);
+  a.parts = LatentPartsAt(scratch, groups, rows);
   a.most_length = op->table_width * op->cache.page;
   a.tokens_a_pair = std::max(1, rows / op->heads);
   a.pairs_a_token = (op->heads + rows - 1) / rows;
-  const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, cus, a.pairs_a_token};
+  const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, groups, a.pairs_a_token};
   BeginLaunches();
   const auto s = static_cast<hipStream_t>(stream);
-  WithForm(*op, few, [&](auto type, auto r, auto p, auto eight, auto few_rows) {
+  WithForm(*op, FormOf(*op), [&](auto type, auto r, auto p, auto eight, auto form) {
     constexpr int kType = decltype(type)::value, kR = decltype(r)::value, kP = decltype(p)::value;
-    constexpr bool kEight = decltype(eight)::value, kFew = decltype(few_rows)::value;
-    using G = LatentGeo<kR, kP, kEight, kFew>;
-    static_assert(G::kRing >= (kFew ? 1 : 3) && G::kLds <= kLdsBytes, "a ring of tiles");
+    constexpr bool kEight = decltype(eight)::value;
+    constexpr Form kForm = decltype(form)::value;
+    using G = LatentGeo<kR, kP, kEight, kForm>;
+    static_assert(G::kRing >= (G::kFew ? 1 : 3) && G::kLds <= kLdsBytes / G::kAUnit, "a ring of tiles");
     constexpr int kLds = G::kLds;
     static bool sized = false;
-    if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kFew>), kLds, &sized)) return;
-    hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kFew>), dim3(cus), dim3(G::kThreads), kLds, s, a);
-    hipLaunchKernelGGL((LatentJoinKernel<kType, kR, 16, G::kRows>), dim3(cus, 2), dim3(kJoinWaves * kWave), 0, s, join);
+    if (!AllowLds(reinterpret_cast<const void*>(&LatentAttendKernel<kType, kR, kP, kEight, kForm>), kLds, &sized)) return;
+    hipLaunchKernelGGL((LatentAttendKernel<kType, kR, kP, kEight, kForm>), dim3(groups), dim3(G::kThreads), kLds, s, a);
+    hipLaunchKernelGGL((LatentJoinKernel<kType, kR, 16, G::kRows>), dim3(groups, 2), dim3(kJoinWaves * kWave), 0, s, join);
   });
   return LaunchStatus("latent_attend");
 }

@@ -150,14 +150,15 @@ def test_attend_refusals():
         refused(lib.llmp_hip_latent_attend(C.byref(attend()), 0x100000, 1 << 40, cus, None), "compute units")
 
 
-@pytest.mark.parametrize("kw,rows", [(dict(heads=16, most_tokens=1), 16), (dict(heads=17, most_tokens=1), 128), (dict(heads=4, most_tokens=4, tokens=3), 16), (dict(heads=4, most_tokens=5, tokens=9), 128)])
+@pytest.mark.parametrize("kw,rows", [(dict(heads=16, most_tokens=1), 16), (dict(heads=17, most_tokens=1), 128), (dict(heads=4, most_tokens=4, tokens=3), 16), (dict(heads=4, most_tokens=5, tokens=9), 128), (dict(heads=129, most_tokens=1), 128)])
 def test_attend_scratch(kw, rows):
     """Two parts a workgroup: whose they are, and a row's maximum, sum and values in F32."""
     lib = _lib.load()
     for width in (256, 512):
         op = attend(cache(width=width), **kw)
         needs = lib.llmp_hip_latent_attend_scratch(C.byref(op), 256)
-        assert needs == 2 * 256 * (16 + rows * (8 + 4 * width))
+        groups = 512 if width == 256 and op.most_tokens * op.heads > 128 else 256
+        assert needs == 2 * groups * (16 + rows * (8 + 4 * width))
         for scratch, size in ((None, needs), (0x100000, needs - 1), (0x100008, needs)):
             refused(lib.llmp_hip_latent_attend(C.byref(op), scratch, size, 256, None), "scratch")
 
