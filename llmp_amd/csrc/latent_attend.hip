@@ -98,7 +98,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
   // ---- this workgroup's run of the line
   const int64_t t = a.tokens_a_pair;
   if (threadIdx.x < 2) a.parts.which[(2 * w + threadIdx.x) * 4] = -1;
-  const LatentRun run = RunOf(op.requests, w, groups, kLeast, [&](int r) {
+  const LatentRun run = RunOf<false>(op.requests, w, groups, kLeast, [&](int r) {
     const LatentRequest l = AttendRequest(a, r);
     return LineBefore(l, t, l.groups) * a.pairs_a_token;
   });

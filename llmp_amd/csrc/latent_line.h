@@ -61,14 +61,14 @@ __device__ __forceinline__ int GroupAt(const LatentRequest& l, int64_t t, int64_
   return k;
 }
 
-// Every wave by itself, a lane a request: length_of(r) is a request's of the line. The run [from, to) of this workgroup (`index` of `groups`), the request that
-// holds its beginning, and the line before that.
+// Every wave by itself, a lane a request: length_of(r) is a request's of the line. The run [from, to) of this workgroup (`block` of `groups`), the request that
+// holds its beginning, and the line before that. Eight workgroups in a row go to eight chiplets: runs side by side are on eight of them, or on one (CHIPLETS).
 struct LatentRun {
   int64_t from, to, before, per;
-  int request;
+  int request, index;
 };
-template <class LengthOf>
-__device__ __forceinline__ LatentRun RunOf(int requests, int index, int groups, int64_t least, const LengthOf& length_of) {
+template <bool CHIPLETS, class LengthOf>
+__device__ __forceinline__ LatentRun RunOf(int requests, int block, int groups, int64_t least, const LengthOf& length_of) {
   const int lane = threadIdx.x & (kWave - 1);
   const auto sums = [&](int64_t v) {  // inclusive
 #pragma unroll
@@ -87,7 +87,13 @@ __device__ __forceinline__ LatentRun RunOf(int requests, int index, int groups, 
   int64_t total = from_lane(first_upto, kWave - 1);
   for (int r0 = kWave; r0 < requests; r0 += kWave) total += from_lane(sums(r0 + lane < requests ? length_of(r0 + lane) : 0), kWave - 1);
   const int64_t per = max(Over(total + groups - 1, groups), least);
-  LatentRun run = {index * per, min((index + 1) * per, total), 0, per, 0};
+  int index = block;
+  if constexpr (CHIPLETS) {
+    // An eighth of the runs that there are to each chiplet, and so of the others (`groups` is a multiple of 8).
+    const int chiplet = block % 8, i = block / 8, share = static_cast<int>((Over(total + per - 1, per) + 7) / 8);
+    index = i < share ? chiplet * share + i : 8 * share + chiplet * (groups / 8 - share) + i - share;
+  }
+  LatentRun run = {index * per, min((index + 1) * per, total), 0, per, 0, index};
   if (run.from >= run.to) return run;
   for (int r0 = 0; r0 < requests; r0 += kWave) {
     const int64_t mine = r0 == 0 ? first : r0 + lane < requests ? length_of(r0 + lane) : 0;

@@ -87,18 +87,19 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
   const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
   const float worth = Scalar(fabsf(op.scale) * kLog2E);
 
-  // Eight workgroups in a row go to eight chiplets: a chiplet takes every eighth (request, head), or an eighth of the line.
+  // Eight workgroups in a row go to eight chiplets: a chiplet takes every eighth (request, head), or an eighth of the line, so that its L2 holds the keys that
+  // neighbouring pairs share (one prompt of 4096, 8 heads of 64: 47 us, runs in the order of the workgroups 54).
   const int groups = gridDim.x;
-  const int index = LINE ? static_cast<int>(blockIdx.x % 8) * (groups / 8) + static_cast<int>(blockIdx.x / 8) : 0;
+  int index = 0;
   int request, head = 0, k = 0;
   int64_t u = 0, u_end = 1, before = 0, per = 1, pair_from = 0;
   if constexpr (LINE) {
-    if (tid < 2) a.parts.which[(2 * index + tid) * 4] = -1;
-    const LatentRun run = RunOf(op.requests, index, groups, kLeast, [&](int r) {
+    const LatentRun run = RunOf<true>(op.requests, blockIdx.x, groups, kLeast, [&](int r) {
       const LatentRequest l = PromptOf(op, r).l;
       return LineBefore(l, kPromptRows, l.groups) * op.heads;
     });
-    u = run.from, u_end = run.to, before = run.before, request = run.request, per = run.per;
+    u = run.from, u_end = run.to, before = run.before, request = run.request, per = run.per, index = run.index;
+    if (tid < 2) a.parts.which[(2 * index + tid) * 4] = -1;
   } else {
     const uint32_t sets = static_cast<uint32_t>(op.requests) * op.heads, padded = (sets + 7) / 8 * 8, set = blockIdx.x % padded;
     if (set >= sets) return;
