@@ -744,9 +744,9 @@ int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch, size_t scr
  * llmp.rope: y = x, but in every head channels first to first + n_dims - 1 are rotated: pair p by the angle positions[token] * f_p, where a pair
  * is channels (p, p + n_dims / 2) of them or, interleaved, (2p, 2p + 1): (a cos - b sin, a sin + b cos) * magnitude, or with
  * `inverse` by the negative angle (which is the rotation's gradient). f_p is turns[p] / 2^64 of a whole turn a position
- * (device U64 [n_dims / 2], as llmp_hip_rope_table makes it): the angle is exact to 2^-33 of a turn at any position, negative ones
+ * (device U64 [n_dims / 2], as llmp_hip_rope_table makes it): the angle is exact to 2^-32 of a turn at any position, negative ones
  * among them. x and out are LLMP_X_* `type` [tokens][heads][head_dim], element strides, a head's channels side by side; out is x (with
- * its strides: the other channels are then not touched) or does not overlap it. Cosines and sines are F32 (2^-24 off), products and sums F32,
+ * its strides: the other channels are then not touched) or does not overlap it. Cosines and sines are F32 (2^-23 off), products and sums F32,
  * rounded once. n_dims up to 1024. One launch. */
 typedef struct llmp_rope {
   const void* x;
@@ -844,7 +844,8 @@ int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t s
  * [keys][rope_width], which all heads share, and of v [keys][heads][value]; its queries are at the last positions of its keys (key_starts
  * null: starts). Logits are scale * (q . (k, k_rope)); out [tokens][heads][value]. All of one type (LLMP_X_BF16 or LLMP_X_F16), element strides, the last index side by
  * side, rows at 16-byte boundaries; nope and value are both 64 or both 128, rope_width 32 or 64. What a row does not see changes nothing
- * of it; a row that sees nothing is zero; rows past starts[requests] are not written. Roundings and most_tokens as llmp.latent.attend's. Where a
+ * of it; a row that sees nothing is zero; rows past starts[requests] are not written. Roundings as llmp.latent.attend's; most_tokens is at least every request's
+ * queries (rows past it are not written). The tokens of k, k_rope and v are less than 2^24 values apart. Where a
  * call has few rows for the device, its keys are cut into runs, by the descriptor's sizes alone: a row's last bits depend on those. scratch:
  * llmp_hip_latent_prompt_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal). A captured launch replays with other starts. out overlaps no
  * operand. One launch, two where keys are cut. */

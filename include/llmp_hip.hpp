@@ -580,6 +580,18 @@ inline std::vector<Implementation> Implementations() {
   follows_rows();
   add("llmp.paged.select", "paged.select", {"paged_q8"}, {1, any, 64, 1}, Rung::kNative, kInt8Mma, {"llmp_hip_paged_select"},
       "page bounds on the matrix cores, the choice by their bits; one launch or two");
+  // Attention over latent vectors (no counterpart in the reference). Both attentions' sums are cut by the call's sizes or its whole work.
+  add("llmp.rope", "rope", {"f32", "bf16", "f16"}, {1, any, 2, 1}, Rung::kNative, 0, {"llmp_hip_rope"}, "a workgroup some tokens, their angles in LDS");
+  add("llmp.latent.store", "latent.store", {"latent", "latent_e4m3"}, {1, any, 256, 1}, Rung::kNative, 0, {"llmp_hip_latent_store"}, "a wave a token");
+  add("llmp.latent.read", "latent.read", {"latent", "latent_e4m3"}, {1, any, 256, 1}, Rung::kNative, 0, {"llmp_hip_latent_read"}, "a wave a token");
+  add("llmp.latent.project", "latent.project", {"bf16", "f16"}, {1, any, 32, 32}, Rung::kNative, kBf16Mma, {"llmp_hip_latent_project"},
+      "128 outputs of a head by 32 or 128 tokens a workgroup");
+  add("llmp.latent.attend", "latent.attend", {"latent", "latent_e4m3"}, {1, any, 256, 1}, Rung::kNative, kBf16Mma, {"llmp_hip_latent_attend"},
+      "an even cut of the call's keys: up to 16 rows a wave, or 128 a workgroup; and a join");
+  follows_rows();
+  add("llmp.latent.prompt", "latent.prompt", {"bf16", "f16"}, {1, any, 64, 1}, Rung::kNative, kBf16Mma, {"llmp_hip_latent_prompt"},
+      "128 rows of a head a workgroup, whole, or an even cut of the keys and a join");
+  follows_rows();
   // One token through a routed-expert layer: the router, the experts' products, their GLU and the ordered sum fused
   // (no single counterpart in the reference: ir/decompose.cc:1080-1109 holds the five operations).
   add("llmp.moe.token", "fused.moe_ffn_token", {"q4_k"}, {1, 1, 256, 256}, Rung::kNative, 0, {"llmp_hip_moe_token"},

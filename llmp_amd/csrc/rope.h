@@ -7,9 +7,9 @@
 namespace llmp_hip {
 
 // cos and sin of position * turns, where `turns` is a 64-bit fraction of a whole turn: the product modulo 2^64 is the angle's own
-// fraction, exactly, at any position. Its upper 32 bits (2^-33 of a turn off at most) are split into quarter turns and a rest
+// fraction, exactly, at any position. Its upper 32 bits (2^-32 of a turn off at most) are split into quarter turns and a rest
 // within an eighth of a turn, whose sine and cosine are their Taylor sums through x^9 and x^10: the terms left out are
-// below 2^-28. Off by about 2^-24 in all.
+// below 2^-28. Off by 2^-23 at most in all.
 __device__ __forceinline__ void Turn(uint64_t turns, int32_t position, float* cosine, float* sine) {
   const uint64_t phase = turns * static_cast<uint64_t>(static_cast<int64_t>(position));
   const uint32_t t = static_cast<uint32_t>(phase >> 32);
