@@ -747,7 +747,7 @@ int llmp_hip_paged_select(const llmp_paged_select* op, void* scratch, size_t scr
  * (device U64 [n_dims / 2], as llmp_hip_rope_table makes it): the angle is exact to 2^-32 of a turn at any position, negative ones
  * among them. x and out are LLMP_X_* `type` [tokens][heads][head_dim], element strides, a head's channels side by side; out is x (with
  * its strides: the other channels are then not touched) or does not overlap it. Cosines and sines are F32 (2^-23 off), products and sums F32,
- * rounded once. n_dims up to 1024. One launch. */
+ * rounded once. n_dims up to 1024, tokens less than 2^24. One launch. */
 typedef struct llmp_rope {
   const void* x;
   void* out;
@@ -778,10 +778,10 @@ typedef struct llmp_latent_cache {
 
 /* llmp.latent.store: token i's rows into slots[i] (one outside the cache: the row is skipped; the slots of a call that are not
  * skipped are distinct, or their rows' pieces end there in any mixture). latent (LLMP_X_* `type`, latent_stride elements apart, rows at 16-byte
- * boundaries) is normalised where `weight` (F32 [width], 16-byte aligned) is given: c / sqrt(mean of c^2 + eps) * weight. It is rounded once, to the cache's type
+ * boundaries) is normalised where `weight` (F32 [width], 16-byte aligned) is given: c / sqrt(mean of c^2 + eps) * weight, in F32. It is rounded once, to the cache's type
  * or to E4M3 with the smallest scale that holds the row (448 at most; infinities become 448 times the largest scale, a NaN a NaN). rope (the same type,
  * rope_stride elements apart) is rotated as llmp.rope has it with n_dims = rope_width, by positions[i] and `turns` times `magnitude`; turns null: stored as
- * it is. One launch. */
+ * it is. At most 2^25 tokens. One launch. */
 typedef struct llmp_latent_store {
   llmp_latent_cache cache;
   const void* latent;
@@ -797,7 +797,7 @@ typedef struct llmp_latent_store {
 int llmp_hip_latent_store(const llmp_latent_store* op, void* stream);
 
 /* llmp.latent.read: rows back as values: latent_out [count][width] and rope_out [count][rope_width] of LLMP_X_* `type`, 16-byte aligned, by their slots
- * (one outside the cache gives zeros). One launch. */
+ * (one outside the cache gives zeros), at most 2^25 of them. One launch. */
 int llmp_hip_latent_read(const llmp_latent_cache* cache, const int32_t* slots, int64_t count, int type, void* latent_out, void* rope_out, void* stream);
 
 /* llmp.latent.project: y[t][h][n] = sum over k of x[t][h][k] * w[h][n][k]: every head's rows times that head's matrix. x, w and y are of one type

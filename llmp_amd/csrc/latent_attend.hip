@@ -415,13 +415,14 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
           }
           if (alone && __any(garbage)) {
             // A token that some row must not see holds infinities or NaN, which a weight of zero does not keep out: they become zeros in LDS. (A row that
-            // sees them has no finite logit there, and no finite sum. `alone`: nobody reads the tile as keys any more. Elsewhere all rows see the same.)
+            // sees them has no finite logit there. `alone`: nobody reads the tile as keys any more. Elsewhere all rows see the same.)
 #pragma unroll 1
             for (uint32_t i = 16 * lane_anew(); i < G::kLatentBytes; i += 1024) {
               U32x4* const at = reinterpret_cast<U32x4*>(lds + tile + i);
               *at = EIGHT ? FiniteCodes(*at) : Finite<TYPE>(*at);
             }
           }
+          if (!FEW && alone) MeetLds();
           // (Blocks 256 bytes apart side by side, for the same reason as the keys' steps.)
           const auto block_of = [](int i) {
             constexpr int kSame = EIGHT ? kBlocks / 16 : kBlocks / 8;
@@ -481,6 +482,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
             if (more && !early) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
             if (careful) MeetLds();
             if (busy) values(tile_from + i, at, gone, careful);
+            if (!busy && careful) MeetLds();  // (with the others, before they read the values)
           }
           MeetLds();
         }

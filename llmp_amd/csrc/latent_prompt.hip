@@ -409,6 +409,8 @@ bool WholePairs(const llmp_latent_prompt& op, int cus) {
   const double requests = op.requests, tiles = op.keys / static_cast<double>(kKeys) + 1.0, share = tiles / requests + 1.0;
   const double longest = fresh ? std::min(tiles, op.most_tokens / static_cast<double>(kKeys) + 1.0) : std::min(tiles, 2.0 * share);
   const double row_tiles = op.tokens / static_cast<double>(kPromptRows) + 0.5 * requests;
+  // (Blocks are dealt by the largest number of queries that the caller says: where that says little, most would have no pair.)
+  if (static_cast<double>(TilesOf(op)) * requests > 4.0 * (op.tokens / static_cast<double>(kPromptRows) + requests)) return false;
   const double each = row_tiles * op.heads * share * (fresh ? 0.5 : 1.0) / (kAUnit * cus);
   return longest <= 2.5 * each + 15.0;
 }

@@ -23,6 +23,7 @@ int CheckLatentCache(const char* who, const llmp_latent_cache& c) {
 namespace {
 
 constexpr int kRowThreads = 256, kRowWaves = kRowThreads / kWave;
+constexpr int kMostRows = 1 << 25;  // a call's: a grid has less than 2^32 threads
 
 __device__ __forceinline__ float WaveSum(float v) {
 #pragma unroll
@@ -162,7 +163,7 @@ using namespace llmp_hip;
 extern "C" int llmp_hip_latent_store(const llmp_latent_store* op, void* stream) {
   if (op == nullptr) return Refuse(1, "latent_store: null operands");
   if (const int bad = CheckLatentCache("latent_store", op->cache); bad != 0) return bad;
-  if (op->tokens < 0) return Refuse(1, "latent_store: %d tokens", op->tokens);
+  if (op->tokens < 0 || op->tokens > kMostRows) return Refuse(1, "latent_store: %d tokens (at most 2^25)", op->tokens);
   if (op->tokens == 0) return 0;
   if (const int bad = CheckPagedRows("latent_store", "latent", op->latent, op->tokens, 1, op->latent_stride, 0, op->type); bad != 0) return bad;
   const int64_t element = PagedElementBytes(op->type);
@@ -185,7 +186,7 @@ extern "C" int llmp_hip_latent_store(const llmp_latent_store* op, void* stream) 
 extern "C" int llmp_hip_latent_read(const llmp_latent_cache* cache, const int32_t* slots, int64_t count, int type, void* latent_out, void* rope_out, void* stream) {
   if (cache == nullptr) return Refuse(1, "latent_read: null operands");
   if (const int bad = CheckLatentCache("latent_read", *cache); bad != 0) return bad;
-  if (count < 0 || count > INT_MAX) return Refuse(1, "latent_read: %lld rows", (long long)count);
+  if (count < 0 || count > kMostRows) return Refuse(1, "latent_read: %lld rows (at most 2^25)", (long long)count);
   if (count == 0) return 0;
   if (slots == nullptr || reinterpret_cast<uintptr_t>(slots) % 4 != 0) return Refuse(1, "latent_read: slots at a 4-byte boundary");
   if (const int bad = CheckPagedRows("latent_read", "latent_out", latent_out, 1, 1, 0, 0, type); bad != 0) return bad;

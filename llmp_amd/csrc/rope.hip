@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kMostPairs = 512;  // of a head: n_dims up to 1024
+constexpr int kMostTokens = (1 << 24) - 1;  // a call's: a grid has less than 2^32 threads
 
 struct RopeArgs {
   llmp_rope op;
@@ -142,7 +143,7 @@ extern "C" int llmp_hip_rope_table(int n_dims, double base, double freq_scale, d
 extern "C" int llmp_hip_rope(const llmp_rope* op, void* stream) {
   if (op == nullptr) return Refuse(1, "rope: null operands");
   if (op->type != LLMP_X_F32 && op->type != LLMP_X_BF16 && op->type != LLMP_X_F16) return Refuse(1, "rope: element type %d", op->type);
-  if (op->tokens < 0 || op->tokens > INT_MAX || op->heads <= 0 || op->heads > 65535) return Refuse(1, "rope: %lld tokens, %d heads", (long long)op->tokens, op->heads);
+  if (op->tokens < 0 || op->tokens > kMostTokens || op->heads <= 0 || op->heads > 65535) return Refuse(1, "rope: %lld tokens, %d heads", (long long)op->tokens, op->heads);
   if (op->head_dim <= 0 || op->head_dim > 65536 || op->n_dims <= 0 || op->n_dims % 2 != 0 || op->n_dims > 2 * kMostPairs || op->first < 0 ||
       op->first + op->n_dims > op->head_dim) {
     return Refuse(1, "rope: channels %d to %d of %d (an even number up to %d)", op->first, op->first + op->n_dims, op->head_dim, 2 * kMostPairs);

@@ -54,6 +54,21 @@ def test_later_tokens_of_infinities_and_nan(device, heads, width, rope, dtype, b
         assert not torch.isfinite(got[starts[r + 1] - 1][:, ::3].float()).any(), r
 
 
+@pytest.mark.parametrize("width", [512, 256])
+def test_rows_that_see_infinities_give_the_same_bits_again(device, width):
+    """Rows that see a token of infinities whose logit is the lowest, beside rows that must not see it."""
+    g = torch.Generator().manual_seed(width)
+    cache, table, starts, q_latent, q_rope = latent_case(g, [90], [33], 16, 48, width, 64, "bf16", 16)
+    page, at = int(table[0, 75 // 16]), 75 % 16
+    cache["latent"][page, at] = 0.0
+    cache["latent"][page, at, 5] = math.inf
+    q_latent[..., 5] = -q_latent[..., 5].abs() - 0.5
+    first = attend(device, cache, table, [90], starts, q_latent, q_rope, 0.02)
+    for _ in range(5):
+        again = attend(device, cache, table, [90], starts, q_latent, q_rope, 0.02)
+        assert torch.equal(first[:33].view(torch.int16), again[:33].view(torch.int16))
+
+
 @pytest.mark.parametrize("heads,most", [(8, 1), (16, 1), (128, 1), (20, 9)])
 @pytest.mark.parametrize("bits", [16, 8])
 def test_pages_that_are_missing(device, heads, most, bits):
@@ -209,6 +224,15 @@ def test_prompt_of_many_requests_and_a_first_row_further_on(device):
     q = normal(g, starts[-1] + 1, 2, 96, dtype=torch.float16)
     k, v, k_rope = normal(g, key_starts[-1] + 2, 2, 64, dtype=torch.float16), normal(g, key_starts[-1] + 2, 2, 64, dtype=torch.float16), normal(g, key_starts[-1] + 2, 32, dtype=torch.float16)
     check_prompt(device, q, k, k_rope, v, starts, key_starts, 0.1, most=8)
+
+
+def test_prompt_of_many_requests_without_a_bound(device):
+    """No word of how many queries a request has: 600 prompts of a few tokens."""
+    g = torch.Generator().manual_seed(22)
+    new = torch.randint(0, 7, (600,), generator=g).tolist()
+    starts = [sum(new[:i]) for i in range(601)]
+    q, k, v, k_rope = (normal(g, starts[-1], *s, dtype=torch.bfloat16) for s in ((2, 192), (2, 128), (2, 128), (64,)))
+    check_prompt(device, q, k, k_rope, v, starts, None, 0.1, most=None)
 
 
 # ---------------------------------------------------------------- streams and graphs

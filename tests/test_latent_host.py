@@ -32,7 +32,7 @@ def rope(**kw):
     return _lib.Rope(**base)
 
 
-@pytest.mark.parametrize("kw,why", [(dict(type=5), "type"), (dict(tokens=-1), "tokens"), (dict(heads=0), "heads"), (dict(heads=70000), "heads"), (dict(head_dim=0), "channels"),
+@pytest.mark.parametrize("kw,why", [(dict(type=5), "type"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 24), "tokens"), (dict(heads=0), "heads"), (dict(heads=70000), "heads"), (dict(head_dim=0), "channels"),
                                     (dict(n_dims=0), "channels"), (dict(n_dims=63), "channels"), (dict(n_dims=66), "channels"), (dict(first=2), "channels"), (dict(first=-2), "channels"),
                                     (dict(n_dims=1026, head_dim=2048), "channels"), (dict(magnitude=math.nan), "magnitude"), (dict(x=None), "null"), (dict(out=None), "null"),
                                     (dict(positions=None), "null"), (dict(turns=None), "null"), (dict(x=0x1001), "boundaries"), (dict(positions=0x3002), "boundaries"),
@@ -86,7 +86,7 @@ def test_store_and_read_refusals():
     for kw, why in CACHE_REFUSALS:
         refused(lib.llmp_hip_latent_store(C.byref(store(cache(**kw))), None), why)
         refused(read(cache(**kw)), why)
-    for kw, why in [(dict(latent=None), "null"), (dict(rope=None), "null"), (dict(slots=None), "null"), (dict(type=4), "type"), (dict(tokens=-1), "tokens"), (dict(latent=0x1008), "16-byte"),
+    for kw, why in [(dict(latent=None), "null"), (dict(rope=None), "null"), (dict(slots=None), "null"), (dict(type=4), "type"), (dict(tokens=-1), "tokens"), (dict(tokens=(1 << 25) + 1), "tokens"), (dict(latent=0x1008), "16-byte"),
                     (dict(latent_stride=578), "16-byte"), (dict(latent_stride=-576), "16-byte"), (dict(rope=0x2001), "boundaries"), (dict(rope_stride=-64), "boundaries"),
                     (dict(slots=0x3002), "boundaries"), (dict(turns=0x5004), "boundaries"), (dict(positions=0x4001), "boundaries"), (dict(positions=None), "needs positions"),
                     (dict(weight=0x6008), "weight"), (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps")]:
@@ -94,7 +94,7 @@ def test_store_and_read_refusals():
     assert lib.llmp_hip_latent_store(C.byref(store(tokens=0, latent=None)), None) == 0
     refused(lib.llmp_hip_latent_store(None, None), "null")
     assert read(count=0, slots=None) == 0
-    for kw, why in [(dict(slots=None), "slots"), (dict(slots=0x1002), "slots"), (dict(count=-1), "rows"), (dict(count=1 << 31), "rows"), (dict(kind=7), "type"), (dict(a=None), "null"),
+    for kw, why in [(dict(slots=None), "slots"), (dict(slots=0x1002), "slots"), (dict(count=-1), "rows"), (dict(count=(1 << 25) + 1), "rows"), (dict(kind=7), "type"), (dict(a=None), "null"),
                     (dict(a=0x2008), "16-byte"), (dict(b=0x3004), "16-byte")]:
         refused(read(**kw), why)
     refused(lib.llmp_hip_latent_read(None, 0x1000, 1, 1, 0x2000, 0x3000, None), "null")
@@ -194,7 +194,9 @@ def test_prompt_scratch():
     lib = _lib.load()
     parts = 2 * 512 * (16 + 128 * (8 + 4 * 128))
     for kw, needs in [(dict(), 16), (dict(tokens=8192, keys=8192, most_tokens=8192, heads=64, requests=1), 16), (dict(tokens=1, keys=100000, most_tokens=1, requests=1, key_starts=0x7000), parts),
-                      (dict(tokens=300, keys=9000, most_tokens=100, requests=3, key_starts=0x7000), parts)]:
+                      (dict(tokens=300, keys=9000, most_tokens=100, requests=3, key_starts=0x7000), parts),
+                      # 1000 prompts of a hundred tokens: whole with a bound on one's, cut where nothing is known of it (25 million blocks else).
+                      (dict(tokens=100000, keys=100000, most_tokens=128, heads=32, requests=1000), 16), (dict(tokens=100000, keys=100000, most_tokens=100000, heads=32, requests=1000), parts)]:
         op = prompt(**kw)
         assert lib.llmp_hip_latent_prompt_scratch(C.byref(op), 256) == needs, kw
         for scratch, size in ((None, needs), (0x100000, needs - 1), (0x100008, needs)):
