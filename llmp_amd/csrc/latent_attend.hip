@@ -99,8 +99,11 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
   // ---- this workgroup's run of the line
   const int64_t t = a.tokens_a_pair;
   if (threadIdx.x < 2) a.parts.which[(2 * w + threadIdx.x) * 4] = -1;
+  // (The few rows' form keeps the first 64 requests, a lane each: looked up again, what its chain of loads begins with is one load longer.)
+  LatentRequest first = {};
+  if (FEW && lane_anew() < op.requests) first = AttendRequest(a, lane_anew());
   const LatentRun run = RunOf<false>(op.requests, w, groups, kLeast, [&](int r) {
-    const LatentRequest l = AttendRequest(a, r);
+    const LatentRequest l = FEW && r < kWave ? first : AttendRequest(a, r);
     return LineBefore(l, t, l.groups) * a.pairs_a_token;
   });
   int64_t u = run.from, before = run.before;
@@ -111,7 +114,14 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
   const uint32_t flip = op.scale < 0.0f ? 0x80008000u : 0u;  // (a negative scale goes into the queries: the largest product is the largest logit)
 
   for (int request = run.request; u < u_end; ++request) {
-    const LatentRequest l = Scalar(AttendRequest(a, request));
+    LatentRequest l;
+    if (FEW && request < kWave) {
+      l.start = __builtin_amdgcn_readlane(first.start, request), l.n = __builtin_amdgcn_readlane(first.n, request);
+      l.length = __builtin_amdgcn_readlane(first.length, request), l.base = __builtin_amdgcn_readlane(first.base, request);
+      l.groups = __builtin_amdgcn_readlane(first.groups, request);
+    } else {
+      l = Scalar(AttendRequest(a, request));
+    }
     const int64_t all = LineBefore(l, t, l.groups) * a.pairs_a_token;
     if (u >= before + all) {
       before += all;
