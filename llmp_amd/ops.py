@@ -886,7 +886,7 @@ def rope(x, positions, table, *, layout="half", first=0, inverse=False, out=None
     turns = _turns(table)
     tokens, heads, head_dim = x.shape
     if out is None:
-        out = torch.empty((tokens, heads, head_dim), dtype=x.dtype, device=x.device)
+        out = x.new_empty((tokens, heads, head_dim))
     assert out.shape == x.shape and out.dtype is x.dtype and positions.dtype is torch.int32 and positions.shape == (tokens,)
     assert positions.stride(0) == 1 or tokens < 2
     (xt, xh, xd), (ot, oh, od) = x.stride(), out.stride()
@@ -955,8 +955,8 @@ def latent_read(cache, slots, dtype=None):
     assert slots.dtype is torch.int32 and slots.dim() == 1 and slots.is_contiguous()
     _here(slots)
     n, dtype = slots.shape[0], cache["rope"].dtype if dtype is None else dtype
-    latent = torch.empty((n, c.width), dtype=dtype, device=slots.device)
-    rope = torch.empty((n, c.rope_width), dtype=dtype, device=slots.device)
+    latent = slots.new_empty((n, c.width), dtype=dtype)
+    rope = slots.new_empty((n, c.rope_width), dtype=dtype)
     _lib.check(lib.llmp_hip_latent_read(C.byref(c), slots.data_ptr(), n, _X_TYPES[dtype], latent.data_ptr(), rope.data_ptr(), _stream()))
     return latent, rope
 
@@ -968,7 +968,7 @@ def latent_project(x, w, out=None):
     tokens, heads, k = x.shape
     n = w.shape[1]
     if out is None:
-        out = torch.empty((tokens, heads, n), dtype=x.dtype, device=x.device)
+        out = x.new_empty((tokens, heads, n))
     assert w.shape == (heads, n, k) and out.shape == (tokens, heads, n) and x.dtype is w.dtype and x.dtype is out.dtype
     (xt, xh, xd), (wh, wr, wd), (yt, yh, yd) = x.stride(), w.stride(), out.stride()
     assert xd == wd == yd == 1
@@ -989,7 +989,7 @@ def latent_attend(cache, q_latent, q_rope, table, lengths, starts, scale, *, bef
     n, table_width = table.shape
     dtype = cache["rope"].dtype
     if out is None:
-        out = torch.empty((tokens, heads, width), dtype=dtype, device=q_latent.device)
+        out = q_latent.new_empty((tokens, heads, width))
     assert width == c.width and q_rope.shape == (tokens, heads, c.rope_width) and out.shape == q_latent.shape
     assert q_latent.dtype is dtype and q_rope.dtype is dtype and out.dtype is dtype and lengths.shape == (n,) and starts.shape == (n + 1,)
     (lt, lh, ld), (rt, rh, rd), (ot, oh, od) = q_latent.stride(), q_rope.stride(), out.stride()
@@ -1004,7 +1004,7 @@ def latent_attend(cache, q_latent, q_rope, table, lengths, starts, scale, *, bef
                            lt, lh, rt, rh, ot, oh, _table_stride(table), heads, n, tokens, tokens if most is None else most, table_width, scale)
     cus, at = _compute_units(), C.byref(op)
     if scratch is None:
-        scratch = torch.empty(max(lib.llmp_hip_latent_attend_scratch(at, cus), 16), dtype=torch.uint8, device=q_latent.device)
+        scratch = q_latent.new_empty(max(lib.llmp_hip_latent_attend_scratch(at, cus), 16), dtype=torch.uint8)
     _lib.check(lib.llmp_hip_latent_attend(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
     return out
 
@@ -1020,7 +1020,7 @@ def latent_prompt(q, k, k_rope, v, starts, scale, *, key_starts=None, most=None,
     keys, rope = k_rope.shape
     nope, value = k.shape[2], v.shape[2]
     if out is None:
-        out = torch.empty((tokens, heads, value), dtype=q.dtype, device=q.device)
+        out = q.new_empty((tokens, heads, value))
     assert qk == nope + rope and k.shape == (keys, heads, nope) and v.shape == (keys, heads, value) and out.shape == (tokens, heads, value)
     assert q.dtype is k.dtype and q.dtype is k_rope.dtype and q.dtype is v.dtype and q.dtype is out.dtype
     (qt, qh, qd), (kt, kh, kd), (rt, rd), (vt, vh, vd), (ot, oh, od) = q.stride(), k.stride(), k_rope.stride(), v.stride(), out.stride()
@@ -1036,6 +1036,6 @@ def latent_prompt(q, k, k_rope, v, starts, scale, *, key_starts=None, most=None,
                            value, scale)
     cus, at = _compute_units(), C.byref(op)
     if scratch is None:
-        scratch = torch.empty(max(lib.llmp_hip_latent_prompt_scratch(at, cus), 16), dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(max(lib.llmp_hip_latent_prompt_scratch(at, cus), 16), dtype=torch.uint8)
     _lib.check(lib.llmp_hip_latent_prompt(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
     return out
