@@ -2,9 +2,9 @@
 // the rows of a request are its (token, head) pairs and one read of a tile serves all of them:
 //   S^T = C Q^T (latent and rotated part), P = exp2(S - E), O^T += C^T P^T, out = O / sum of P.
 //
-// What bounds it: with few heads the cache's bytes (1152 a token at 512 + 64 values against 2 * 1088 operations a row; 32 requests of up to 65536, 16 heads: 206 us,
-// 5.4 TB/s; of codes 135 us, 4.6 TB/s); from about 128 rows a token on the matrix instructions take as long (128 heads: 430 us,
-// 0.63 PFLOP/s: a wave reads 68 KB of LDS a tile for 1088 cycles of products, and about as many of other instructions stand beside them). A tile is 32 tokens, brought into LDS by loads that pass no register; the rows' queries and
+// What bounds it: with few heads the cache's bytes (1152 a token at 512 + 64 values against 2 * 1088 operations a row; 32 requests of up to 65536, 16 heads: 202 us,
+// 5.5 TB/s; of codes 129 us, 4.8 TB/s); from about 128 rows a token on the matrix instructions take as long (128 heads: 420 us,
+// 0.64 PFLOP/s: a wave reads 68 KB of LDS a tile for 1088 cycles of products, and about as many of other instructions stand beside them). A tile is 32 tokens, brought into LDS by loads that pass no register; the rows' queries and
 // results stay in registers. Two forms:
 //   few rows   (no request has more than 16) every wave of a workgroup's four has all rows and a ring of tiles of its own; it waits for nobody, and the
 //              waves' results are added up at the end;
