@@ -402,7 +402,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
             }
             peak = AcrossGroupsMax(peak);
             if (__any(peak > top[s] + (kUp + kFollow))) {
-              const float higher = fmaxf(top[s], peak - kUp);
+              const float higher = peak > top[s] + (kUp + kFollow) ? peak - kUp : top[s];  // (a row's own: what other rows see changes no bit of it)
               const float keep = top[s] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[s] - higher);
               top[s] = higher;
               sum[s] *= keep;

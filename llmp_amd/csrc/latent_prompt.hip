@@ -63,9 +63,9 @@ __device__ __forceinline__ int ValueTurn(int row) {
   return (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 
-template <int N, int P>
+template <int N, int P, int V>
 struct PromptGeo {
-  static constexpr int kKeyPitch = 2 * N, kRopePitch = 2 * P, kValuePitch = 2 * N;
+  static constexpr int kKeyPitch = 2 * N, kRopePitch = 2 * P, kValuePitch = 2 * V;
   static constexpr int kKeyBytes = kKeys * kKeyPitch, kRopeBytes = kKeys * kRopePitch, kValueBytes = kKeys * kValuePitch;
   static constexpr int kTile = kKeyBytes + kRopeBytes + kValueBytes;
   static constexpr int kRing = 2;
@@ -74,12 +74,12 @@ struct PromptGeo {
 };
 
 // LINE: the grid is the device's, each workgroup a run of the line; else a block a (request, head, row tile).
-template <int TYPE, int N, int P, bool LINE>
+template <int TYPE, int N, int P, int V, bool LINE>
 __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(const PromptArgs a) {
-  using G = PromptGeo<N, P>;
+  using G = PromptGeo<N, P, V>;
   using S = Sixteen<TYPE>;
   typedef typename S::Eight Eight;
-  constexpr int kSteps = N / 16, kRopeSteps = P / 16, kBlocks = N / 32;
+  constexpr int kSteps = N / 16, kRopeSteps = P / 16, kBlocks = V / 32;
   constexpr int kKeyGroup = 4, kValueGroup = 4;  // products that are read for at a time
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const llmp_latent_prompt& op = a.op;
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
     }
     peak = AcrossHalvesMax(peak) * worth_now;
     if (__any(peak > top + (kUp + kFollow))) {
-      const float higher = fmaxf(top, peak - kUp);
+      const float higher = peak > top + (kUp + kFollow) ? peak - kUp : top;  // (a row's own: what other rows see changes no bit of it)
       const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
       top = higher;
       sum *= keep;
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
     if (busy) {
       const int64_t unit = static_cast<int64_t>(which) * (kPromptRows / 32) + wave;
       if (half == 0) a.parts.numbers[unit * 32 + column] = make_float2(top, sum);
-      F32x4* const to = reinterpret_cast<F32x4*>(a.parts.values) + unit * (N / 8) * kWave + lane;
+      F32x4* const to = reinterpret_cast<F32x4*>(a.parts.values) + unit * (V / 8) * kWave + lane;
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
@@ -372,8 +372,8 @@ int TilesOf(const llmp_latent_prompt& op) { return (std::min(op.most_tokens, op.
 int CheckLatentPrompt(const llmp_latent_prompt* op, int cus) {
   if (op == nullptr) return Refuse(1, "latent_prompt: null operands");
   if (op->type != LLMP_X_BF16 && op->type != LLMP_X_F16) return Refuse(1, "latent_prompt: BF16 or F16 values, not type %d", op->type);
-  if ((op->nope != 64 && op->nope != 128) || op->value != op->nope || (op->rope_width != 32 && op->rope_width != 64))
-    return Refuse(1, "latent_prompt: heads of 64 or 128 values for keys and values alike, rotated keys of 32 or 64 (%d, %d, %d)", op->nope, op->value, op->rope_width);
+  if ((op->nope != 64 && op->nope != 128) || (op->value != 64 && op->value != 128) || (op->rope_width != 32 && op->rope_width != 64))
+    return Refuse(1, "latent_prompt: heads of 64 or 128 values for keys and for values, rotated keys of 32 or 64 (%d, %d, %d)", op->nope, op->value, op->rope_width);
   if (op->heads < 1 || op->heads > 65535 || op->requests < 1 || op->requests > 1 << 24 || op->tokens < 1 || op->keys < 0 || op->most_tokens < 1 ||
       op->keys > 1 << 30 || op->tokens > 1 << 30)
     return Refuse(1, "latent_prompt: 1 to 2^24 requests, 1 to 65535 heads, 1 to 2^30 tokens, at most 2^30 keys (%d, %d, %d, %d, %d)", op->requests, op->heads, op->tokens, op->keys, op->most_tokens);
@@ -440,23 +440,27 @@ extern "C" int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratc
   const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, line_groups, 0};
   const auto s = static_cast<hipStream_t>(stream);
   BeginLaunches();
-  const auto launch = [&](auto type, auto n, auto p) {
-    constexpr int kType = decltype(type)::value, kN = decltype(n)::value, kP = decltype(p)::value;
-    constexpr int kLds = PromptGeo<kN, kP>::kLds;
+  const auto launch = [&](auto type, auto n, auto p, auto v) {
+    constexpr int kType = decltype(type)::value, kN = decltype(n)::value, kP = decltype(p)::value, kV = decltype(v)::value;
+    constexpr int kLds = PromptGeo<kN, kP, kV>::kLds;
     static bool sized[2] = {false, false};
     if (whole) {
-      if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, false>), kLds, &sized[0])) return;
-      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, false>), dim3(static_cast<unsigned>((sets + 7) / 8 * 8 * a.tiles)), dim3(kPromptThreads), kLds, s, a);
+      if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, kV, false>), kLds, &sized[0])) return;
+      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, kV, false>), dim3(static_cast<unsigned>((sets + 7) / 8 * 8 * a.tiles)), dim3(kPromptThreads), kLds, s, a);
     } else {
-      if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, true>), kLds, &sized[1])) return;
-      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, true>), dim3(line_groups), dim3(kPromptThreads), kLds, s, a);
-      hipLaunchKernelGGL((LatentJoinKernel<kType, kN, 32, kPromptRows>), dim3(line_groups, 2), dim3(kJoinWaves * kWave), 0, s, join);
+      if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, kV, true>), kLds, &sized[1])) return;
+      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, kV, true>), dim3(line_groups), dim3(kPromptThreads), kLds, s, a);
+      hipLaunchKernelGGL((LatentJoinKernel<kType, kV, 32, kPromptRows>), dim3(line_groups, 2), dim3(kJoinWaves * kWave), 0, s, join);
     }
   };
   const auto sizes = [&](auto type) {
+    const auto value = [&](auto n, auto p) {
+      if (op->value == 64) launch(type, n, p, std::integral_constant<int, 64>{});
+      if (op->value == 128) launch(type, n, p, std::integral_constant<int, 128>{});
+    };
     const auto rope = [&](auto n) {
-      if (op->rope_width == 32) launch(type, n, std::integral_constant<int, 32>{});
-      if (op->rope_width == 64) launch(type, n, std::integral_constant<int, 64>{});
+      if (op->rope_width == 32) value(n, std::integral_constant<int, 32>{});
+      if (op->rope_width == 64) value(n, std::integral_constant<int, 64>{});
     };
     if (op->nope == 64) rope(std::integral_constant<int, 64>{});
     if (op->nope == 128) rope(std::integral_constant<int, 128>{});

@@ -343,14 +343,15 @@ def check_prompt(device, q, k, k_rope, v, starts, key_starts, scale, most=None):
 
 @pytest.mark.parametrize("new,keys,heads,most", [([1], None, 1, None), ([1], [1], 3, 1), ([64], None, 2, 64), ([129], [300], 2, None), ([5, 0, 40, 1], [70, 9, 40, 65], 3, 40),
                                                  ([3], [2000], 2, 3), ([127, 2], [127, 800], 5, 127), ([7, 3], [4, 0], 2, 7)])
-@pytest.mark.parametrize("nope,rope,dtype", [(128, 64, "bf16"), (64, 32, "f16"), (64, 64, "bf16"), (128, 32, "f16")])
-def test_prompt(device, new, keys, heads, most, nope, rope, dtype):
+@pytest.mark.parametrize("nope,rope,value,dtype", [(128, 64, 128, "bf16"), (64, 32, 64, "f16"), (64, 64, 64, "bf16"), (128, 32, 128, "f16"), (64, 64, 128, "bf16"), (128, 32, 64, "f16"), (128, 64, 64, "bf16"),
+                                                   (64, 32, 128, "f16")])
+def test_prompt(device, new, keys, heads, most, nope, rope, value, dtype):
     g = torch.Generator().manual_seed(sum(new) + heads + nope)
     add = lambda v: [sum(v[:i]) for i in range(len(v) + 1)]  # noqa: E731
     starts, key_starts = add(new), None if keys is None else add(keys)
     count = starts[-1] if keys is None else key_starts[-1]
     dtype = TYPES[dtype]
     q = normal(g, starts[-1] + 2, heads, nope + rope, dtype=dtype, size=1.5)
-    kv = normal(g, count, heads, 2 * nope + 8, dtype=dtype)
+    kv = normal(g, count, heads, nope + value + 8, dtype=dtype)
     k_rope = normal(g, count, rope + 16, dtype=dtype)[:, 8:8 + rope]
-    check_prompt(device, q, kv[..., :nope], k_rope, kv[..., nope:2 * nope], starts, key_starts, 1.0 / math.sqrt(nope + rope), most)
+    check_prompt(device, q, kv[..., :nope], k_rope, kv[..., nope:nope + value], starts, key_starts, 1.0 / math.sqrt(nope + rope), most)

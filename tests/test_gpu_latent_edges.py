@@ -174,13 +174,13 @@ def test_a_cache_of_more_than_four_gib(device, bits):
 # ---------------------------------------------------------------- the expanded form
 
 
-@pytest.mark.parametrize("dtype,nope,rope", [("bf16", 128, 64), ("f16", 64, 32)])
-def test_prompt_later_values_of_infinities_and_nan(device, dtype, nope, rope):
+@pytest.mark.parametrize("dtype,nope,rope,value", [("bf16", 128, 64, 128), ("f16", 64, 32, 64), ("bf16", 64, 64, 128), ("f16", 128, 32, 64)])
+def test_prompt_later_values_of_infinities_and_nan(device, dtype, nope, rope, value):
     """Keys and values that only later rows see, and those of other requests."""
     g = torch.Generator().manual_seed(nope)
     starts, key_starts, heads = [0, 70, 140, 141], [0, 70, 290, 300], 3
     q, k = normal(g, 141, heads, nope + rope, dtype=TYPES[dtype]), normal(g, 300, heads, nope, dtype=TYPES[dtype])
-    v, k_rope = normal(g, 300, heads, nope, dtype=TYPES[dtype]), normal(g, 300, rope, dtype=TYPES[dtype])
+    v, k_rope = normal(g, 300, heads, value, dtype=TYPES[dtype]), normal(g, 300, rope, dtype=TYPES[dtype])
 
     def run():
         return ops.latent_prompt(q.to(device), k.to(device), k_rope.to(device), v.to(device), ints(starts, device), 0.05, key_starts=ints(key_starts, device)).cpu()
@@ -195,14 +195,15 @@ def test_prompt_later_values_of_infinities_and_nan(device, dtype, nope, rope):
     assert not torch.isfinite(got[69][:, ::2].float()).any() and not torch.isfinite(got[139][:, ::2].float()).any() and torch.isnan(got[140].float()).all()
 
 
-@pytest.mark.parametrize("heads,new,keys,nope,rope", [(64, [1100], None, 128, 64), (64, [1100], None, 64, 32), (128, [300, 700, 5], [900, 700, 1200], 64, 64)])
-def test_prompt_of_whole_pairs(device, heads, new, keys, nope, rope):
+@pytest.mark.parametrize("heads,new,keys,nope,rope,value", [(64, [1100], None, 128, 64, 128), (64, [1100], None, 64, 32, 64), (128, [300, 700, 5], [900, 700, 1200], 64, 64, 64),
+                                                            (64, [1100], None, 64, 64, 128), (64, [1100], None, 128, 32, 64)])
+def test_prompt_of_whole_pairs(device, heads, new, keys, nope, rope, value):
     """Where rows are many a workgroup takes all keys of its rows; three heads of them are checked."""
     g = torch.Generator().manual_seed(heads + sum(new))
     add = lambda v: [sum(v[:i]) for i in range(len(v) + 1)]  # noqa: E731
     starts, key_starts = add(new), add(keys or new)
     dtype = torch.bfloat16
-    q, k, v = (normal(g, n, heads, d, dtype=dtype) for n, d in ((starts[-1], nope + rope), (key_starts[-1], nope), (key_starts[-1], nope)))
+    q, k, v = (normal(g, n, heads, d, dtype=dtype) for n, d in ((starts[-1], nope + rope), (key_starts[-1], nope), (key_starts[-1], value)))
     k_rope = normal(g, key_starts[-1], rope, dtype=dtype)
     got = ops.latent_prompt(q.to(device), k.to(device), k_rope.to(device), v.to(device), ints(starts, device), 0.08, key_starts=None if keys is None else ints(key_starts, device), most=max(new)).cpu()
     for r in range(len(new)):

@@ -171,7 +171,7 @@ def prompt(**kw):
     return _lib.LatentPrompt(**base)
 
 
-PROMPT_REFUSALS = [(dict(type=0), "type"), (dict(nope=96, value=96), "heads of"), (dict(nope=128, value=64), "heads of"), (dict(rope_width=16), "rotated keys"), (dict(heads=0), "heads"),
+PROMPT_REFUSALS = [(dict(type=0), "type"), (dict(nope=96, value=96), "heads of"), (dict(nope=128, value=96), "heads of"), (dict(nope=32, value=64), "heads of"), (dict(rope_width=16), "rotated keys"), (dict(heads=0), "heads"),
                    (dict(heads=65536), "heads"), (dict(requests=0), "requests"), (dict(tokens=0), "tokens"), (dict(keys=-1), "keys"), (dict(keys=(1 << 30) + 1), "keys"), (dict(most_tokens=0), "tokens"),
                    (dict(q=None), "null q"), (dict(k=None), "null k"), (dict(v=None), "null v"), (dict(k_rope=None), "null k_rope"), (dict(out=None), "null out"), (dict(starts=None), "I32"),
                    (dict(key_starts=0x7002), "4-byte"), (dict(q=0x1008), "16-byte"), (dict(k_token_stride=1026), "16-byte"), (dict(v_head_stride=-256), "16-byte"), (dict(scale=math.inf), "scale"),
