@@ -10,7 +10,7 @@
 //
 // Where pairs of (head, 128 rows) are many for the device, a workgroup takes one whole, a head's pairs on one chiplet, the longest first (a prompt of 4096, 32 heads:
 // 205 us, 242 in the rows' order). Elsewhere the pairs' keys are cut evenly (latent_line.h).
-// (That prompt, nope 128, rope 64: 189 us, 0.91 PFLOP/s; the matrix instructions are busy 52 % of the cycles, other vector instructions 36 %, and a wave's products
+// (That prompt, nope 128, rope 64, values of 128: 187 us, 0.92 PFLOP/s; the matrix instructions are busy 52 % of the cycles, other vector instructions 36 %, and a wave's products
 // and softmax wait for each other. Six ragged ones of 12 heads, up to 700 rows of 64 + 32 behind 3500 keys: 34 us and 9 for the join.)
 #include <algorithm>
 #include <cmath>
