@@ -227,6 +227,13 @@ def test_prompt_of_many_requests_and_a_first_row_further_on(device):
     check_prompt(device, q, k, k_rope, v, starts, key_starts, 0.1, most=8)
 
 
+def test_prompt_without_any_keys(device):
+    q, none, starts = torch.randn(5, 3, 192, device=device).bfloat16(), torch.empty(0, 3, 128, dtype=torch.bfloat16, device=device), ints([0, 2, 5], device)
+    out = torch.full((5, 3, 128), 9.0, dtype=torch.bfloat16, device=device)
+    ops.latent_prompt(q, none, torch.empty(0, 64, dtype=torch.bfloat16, device=device), none, starts, 0.1, key_starts=ints([0, 0, 0], device), out=out)
+    assert (out == 0).all()
+
+
 def test_prompt_of_many_requests_without_a_bound(device):
     """No word of how many queries a request has: 600 prompts of a few tokens."""
     g = torch.Generator().manual_seed(22)
