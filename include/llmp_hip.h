@@ -844,7 +844,8 @@ int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t s
  * [keys][rope_width], which all heads share, and of v [keys][heads][value]; its queries are at the last positions of its keys (key_starts
  * null: starts). Logits are scale * (q . (k, k_rope)); out [tokens][heads][value]. All of one type (LLMP_X_BF16 or LLMP_X_F16), element strides, the last index side by
  * side, rows at 16-byte boundaries; nope and value are 64 or 128, rope_width 32 or 64. What a row does not see changes nothing
- * of it; a row that sees nothing is zero; rows past starts[requests] are not written. Roundings as llmp.latent.attend's; most_tokens is at least every request's
+ * of it; a row that sees nothing is zero; an infinite value that it sees is infinite in its sum, or no number where the rounded weight is zero; rows past
+ * starts[requests] are not written. Roundings as llmp.latent.attend's; most_tokens is at least every request's
  * queries (rows past it are not written). The tokens of k, k_rope and v are less than 2^24 values apart. Where a
  * call has few rows for the device, its keys are cut into runs, by the descriptor's sizes alone: a row's last bits depend on those. scratch:
  * llmp_hip_latent_prompt_scratch(op, cus) bytes at a 16-byte boundary (0: a refusal). A captured launch replays with other starts. out overlaps no

@@ -243,52 +243,23 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
           },
           [&](int i, Eight key) { dots[i % 2] = S::Product32(key, q[i / 2], dots[i % 2]); });
     }
+    uint8_t* const values = lds + at + G::kKeyBytes + G::kRopeBytes;
     float worth_now = worth;
+    int odd = 0;
     if (p0 + kKeys > all_rows_to) {
       // ---- a tile that some row does not see all of. Infinities and NaN among values that a row does not see are not kept out by a weight of zero:
-      // where there are any, they become zeros here, and what they are to the rows that see them is added by itself.
+      // where there are any, they become zeros before the second product, and what they are to the rows that see them is added by itself.
       MeetLds();  // (nobody reads the keys any more: the flags lie there)
-      uint8_t* const values = lds + at + G::kKeyBytes + G::kRopeBytes;
-      bool odd = false;
+      bool mine = false;
       for (int i = 16 * tid; i < G::kValueBytes; i += 16 * kPromptThreads) {
         const U32x4 v = *reinterpret_cast<const U32x4*>(values + i), f = Finite<TYPE>(v);
-        odd = odd || v[0] != f[0] || v[1] != f[1] || v[2] != f[2] || v[3] != f[3];
+        mine = mine || v[0] != f[0] || v[1] != f[1] || v[2] != f[2] || v[3] != f[3];
       }
       if (lane == 0) reinterpret_cast<int*>(lds + at)[wave] = 0;
-      if (__any(odd) && lane == 0) reinterpret_cast<int*>(lds + at)[wave] = 1;
+      if (__any(mine) && lane == 0) reinterpret_cast<int*>(lds + at)[wave] = 1;
       MeetLds();
       const int* const flags = reinterpret_cast<const int*>(lds + at);
-      if ((flags[0] | flags[1] | flags[2] | flags[3]) != 0) {
-        // (A value that is no number makes every row that sees its key none in that dimension, whatever its weight; an infinity does with
-        // it what the product of the weight is: either way the row's sum in that dimension ends as weight * value added to it.)
-        if (works) {
-#pragma unroll 1
-          for (int t = 0; t < kKeys; ++t) {
-            const bool sees = p0 + t < see_to;
-            if (!__any(sees)) continue;
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-              // Four dimensions of a lane's element group at a time: 8 i + 4 half + e.
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int piece = (4 * b + i) ^ ValueTurn<G::kValuePitch>(t);
-                const uint16_t* const v = reinterpret_cast<const uint16_t*>(values + t * G::kValuePitch + 16 * piece + 8 * half);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float x = TYPE == LLMP_X_BF16 ? Bf16BitsToFloat(v[e]) : HalfBitsToFloat(v[e]);
-                  if (sees && !(fabsf(x) < INFINITY)) out[b][4 * i + e] += x;
-                }
-              }
-            }
-          }
-        }
-        MeetLds();
-        for (int i = 16 * tid; i < G::kValueBytes; i += 16 * kPromptThreads) {
-          U32x4* const v = reinterpret_cast<U32x4*>(values + i);
-          *v = Finite<TYPE>(*v);
-        }
-        MeetLds();
-      }
+      odd = Scalar(flags[0] | flags[1] | flags[2] | flags[3]);
       if (p0 + kKeys > all_to) {
         asm volatile("" ::: "memory");  // (a branch: selects would be in every tile's way)
 #pragma unroll
@@ -300,7 +271,19 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
         worth_now = 1.0f;
       }
     }
-    if (!works) continue;
+    // (All four waves, or none.)
+    const auto clean = [&]() {
+      MeetLds();
+      for (int i = 16 * tid; i < G::kValueBytes; i += 16 * kPromptThreads) {
+        U32x4* const v = reinterpret_cast<U32x4*>(values + i);
+        *v = Finite<TYPE>(*v);
+      }
+      MeetLds();
+    };
+    if (!works) {
+      if (odd != 0) clean();
+      continue;
+    }
     float peak = -INFINITY;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -317,6 +300,41 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
       for (int b = 0; b < kBlocks; ++b) out[b] *= keep;
     }
     const float less = top == -INFINITY ? 0.0f : top;
+    if (odd != 0) {
+      // What the second product would add, weight * value, is the value where the weight is not zero and no number where it is. (Here the row's
+      // scale has followed. The weights are worked out by themselves: beside the branch everything stays in one piece, the weights with the second product's first reads.)
+      uint32_t own = 0;  // the lane's keys with a weight: 16 of the first 32, 16 of the others
+      float less_again = less;
+      asm volatile("" : "+v"(less_again));
+#pragma unroll
+      for (int i = 31; i >= 0; --i) {
+        const auto weight = static_cast<typename S::One>(__builtin_amdgcn_exp2f(fmaf(dots[i / 16][i % 16], worth_now, -less_again)));
+        own = own * 2 + (weight != static_cast<typename S::One>(0.0f) ? 1u : 0u);
+      }
+      const uint32_t other = ShflXor(own, 32), low = half == 0 ? own : other, high = half == 0 ? other : own;
+      const uint32_t heavy[2] = {(low & 0xFFFFu) | high << 16, low >> 16 | (high & 0xFFFF0000u)};  // of the row's 64
+#pragma unroll 1
+      for (int t = 0; t < kKeys; ++t) {
+        const bool sees = p0 + t < see_to;
+        const float weight = ((t < 32 ? heavy[0] : heavy[1]) >> (t & 31) & 1u) != 0 ? 1.0f : 0.0f;
+        if (!__any(sees)) continue;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+          // Four dimensions of a lane's element group at a time: 8 i + 4 half + e.
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int place = (4 * b + i) ^ ValueTurn<G::kValuePitch>(t);
+            const uint16_t* const v = reinterpret_cast<const uint16_t*>(values + t * G::kValuePitch + 16 * place + 8 * half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = TYPE == LLMP_X_BF16 ? Bf16BitsToFloat(v[e]) : HalfBitsToFloat(v[e]);
+              if (sees && !(fabsf(x) < INFINITY)) out[b][4 * i + e] = fmaf(x, weight, out[b][4 * i + e]);
+            }
+          }
+        }
+      }
+      clean();
+    }
     Eight weights[4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
