@@ -817,6 +817,7 @@ int llmp_hip_latent_project(const llmp_latent_project* op, void* stream);
  * Logits are scale * (q_latent . latent + q_rope . rope), the result sum of softmax * latent, [tokens][heads][width]. The queries and the result are of
  * the cache's type, element strides, rows at 16-byte boundaries. A table entry that is no page of the cache, a token that a row does not see, and what they hold
  * (infinities and NaN too) change nothing of the row; a row that sees nothing is zero; rows past starts[requests] are not written.
+ * A token of infinities that a row sees makes the row no number; with a logit of minus infinity, those of its dimensions that are infinite.
  * The products' inputs are the 16-bit values as they are (codes are exact in both types, times their scale in F32); sums, maximum and
  * normalisation are F32; a weight is rounded to the cache's type once (BF16 2^-8 of itself; F16 2^-11, or 2^-33 of the row's largest
  * where that is more). most_tokens: at least every request's new tokens (a bound from the host; the form goes by it). scratch:

@@ -359,12 +359,56 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
 #pragma unroll
           for (int i = 0; i < kSets * kLogits; ++i) dots[i / kLogits][i % kLogits] = sums[i / kLogits][i / 4 % 2][i % 4];
         };
-        const auto values = [&](int tile_number, uint32_t tile, uint32_t gone, bool alone) {
+        // A token of infinities has a weight of zero for a row that sees it with a logit of minus infinity (with another logit the row is no number altogether), which is no
+        // number where it is infinite. The second product makes it so, but not of a tile whose infinities become zeros for other rows' sake (below): so it is done here, before
+        // any wave does that, and then they do become zeros, whatever the others see.
+        const auto keep_infinities = [&](int tile_number, uint32_t tile, uint32_t gone) -> bool {
+          const int p0 = tile_number * kTokens, lane_token = 8 * (lane_anew() / 16);
+          bool none = false;  // a logit that is no finite number
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) {
+            const int to = (gone >> (lane_token >> 4) & 1) != 0 ? 0 : row_of(s).see_to - p0 - lane_token;
+#pragma unroll
+            for (int i = 0; i < kLogits; ++i) none |= (i < to) & !(fabsf(dots[s][i]) < INFINITY);
+          }
+          if (!__any(none)) return false;
+          // How many tokens that a row sees are odd in a dimension: a product of zeros and ones, laid out as the results are. (Without constants that the compiler would keep
+          // in registers all along.)
+          constexpr uint32_t kExponents = TYPE == LLMP_X_BF16 ? 0x7F807F80u : 0x7C007C00u, kLast = kExponents & (0u - kExponents);
+          const auto ones = [](uint32_t two) { return (two << 14) - (TYPE == LLMP_X_BF16 ? two << 7 : two << 10); };  // of 1 or 0 in both halves
+          uint32_t value_at = tile + places().value;
+          asm volatile("" : "+v"(value_at));
+          int to[kSets];
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) to[s] = (gone >> (lane_token >> 4) & 1) != 0 ? 0 : row_of(s).see_to - p0 - lane_token;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            U32x4 odd = __builtin_bit_cast(U32x4, value(value_at, b));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd[i] = ones(((odd[i] & kExponents) + (kLast | kLast << 16)) >> 15 & 0x00010001u);
+#pragma unroll
+            for (int s = 0; s < kSets; ++s) {
+              asm volatile("" : "+v"(to[s]));  // (anew for every product, for the same reason)
+              U32x4 sees;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sees[i] = ones((2 * i < to[s] ? 1u : 0u) | (2 * i + 1 < to[s] ? 1u : 0u) << 16);
+              const F32x4 many = S::Product16(__builtin_bit_cast(Eight, odd), __builtin_bit_cast(Eight, sees), F32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float keeps = fmaxf(1.0f - many[e], 0.0f);
+                out[s][b][e] *= __builtin_amdgcn_rcpf(keeps) * keeps;  // 1, or no number
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          return true;
+        };
+        const auto values = [&](int tile_number, uint32_t tile, uint32_t gone, bool alone, bool kept) {
           const uint32_t value_at = tile + places().value;
           const int p0 = tile_number * kTokens;
           float scale8[kLogits];
           if constexpr (EIGHT) scales(tile, scale8);
-          bool garbage = false;
+          bool garbage = kept;
           Eight weights[kSets];
           const bool masked = p0 + kTokens > all_to || gone != 0;
           const float worth = masked ? 1.0f : sign_scale;
@@ -425,7 +469,7 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
           }
           if (alone && __any(garbage)) {
             // A token that some row must not see holds infinities or NaN, which a weight of zero does not keep out: they become zeros in LDS. (A row that
-            // sees them has no finite logit there. `alone`: nobody reads the tile as keys any more. Elsewhere all rows see the same.)
+            // sees them is no number, or has been seen to. `alone`: nobody reads the tile as keys any more. Elsewhere all rows see the same.)
 #pragma unroll 1
             for (uint32_t i = 16 * lane_anew(); i < G::kLatentBytes; i += 1024) {
               U32x4* const at = reinterpret_cast<U32x4*>(lds + tile + i);
@@ -457,8 +501,9 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
               WaitLoads<0>();
             }
             const int tile = my_from + i * step;
-            keys(ring_off + i % G::kRing * G::kTile);
-            values(tile, ring_off + i % G::kRing * G::kTile, absent >> (2 * (i % G::kRing)) & 3u, true);
+            const uint32_t at = ring_off + i % G::kRing * G::kTile, gone = absent >> (2 * (i % G::kRing)) & 3u;
+            keys(at);
+            values(tile, at, gone, true, !EIGHT && ((tile + 1) * kTokens > all_to || gone != 0) && keep_infinities(tile, at, gone));
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             scales_now = scales_next;
             if (i + G::kRing < count) (G::kRing == 1 ? scales_now : scales_next) = fetch(my_from + (i + G::kRing) * step, i % G::kRing);
@@ -490,8 +535,12 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
             const bool careful = gone != 0 || (!one_token && (tile_from + i + 1) * kTokens > all_rows_to);
             if (busy) keys(at);
             if (more && !early) fetch(tile_from + i + kAhead, (i + kAhead) % G::kRing);
-            if (careful) MeetLds();
-            if (busy) values(tile_from + i, at, gone, careful);
+            bool kept = false;
+            if (careful) {
+              kept = !EIGHT && busy && keep_infinities(tile_from + i, at, gone);
+              MeetLds();
+            }
+            if (busy) values(tile_from + i, at, gone, careful, kept);
             if (!busy && careful) MeetLds();  // (with the others, before they read the values)
           }
           MeetLds();

@@ -5,8 +5,9 @@ import math
 import pytest
 import torch
 
+import latent_plain as plain
 from llmp_amd import ops
-from test_gpu_latent import TYPES, normal
+from test_gpu_latent import TYPES, latent_case, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,49 @@ def test_prompt_infinities_of_no_weight(device, more):
         odd[key - more:, 10 * i] = True
     for h in range(heads):
         assert torch.isnan(got[:, h].float()[odd]).all() and torch.equal(bits(got[:, h])[~odd], bits(clean[:, h])[~odd])
+
+
+# ---------------------------------------------------------------- the absorbed form
+
+
+@pytest.mark.parametrize("width,dtype", [(512, "bf16"), (256, "f16"), (512, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("heads,new,at", [(8, 2, 75), (5, 3, 75), (16, 1, 75), (16, 1, 89), (3, 5, 86), (48, 33, 75), (40, 3, 70), (128, 1, 89), (128, 2, 75), (20, 60, 64), (160, 3, 87)])
+def test_infinities_of_no_weight(device, width, dtype, heads, new, at):
+    """A token of infinities whose logit is minus infinity for all: no number in those dimensions of the rows that see it, and nothing anywhere else; and so whatever the later
+    tokens hold that a row does not see, which are cleaned out of the same tile."""
+    g = torch.Generator().manual_seed(width + heads + at)
+    cache, table, starts, q_latent, q_rope = latent_case(g, [90], [new], 16, heads, width, 64, dtype, 16)
+    q_latent[..., 5], q_latent[..., 131] = -q_latent[..., 5].abs() - 0.5, -q_latent[..., 131].abs() - 0.5
+    latent = cache["latent"]
+
+    def run():
+        on = {k: v.to(device) for k, v in cache.items()}
+        return ops.latent_attend(on, q_latent.to(device), q_rope.to(device), table.to(device), ints([90], device), ints(starts, device), 0.02, most=new).cpu()[:new]
+
+    def where(p):
+        return int(table[0, p // 16]), p % 16
+
+    latent[where(at)] = 0.0
+    latent[where(at)][5], latent[where(at)][131] = math.inf, math.inf
+    first = run()
+    sees = (torch.arange(90 - new, 90) >= at)[:, None, None].expand(-1, heads, width)
+    odd = sees & torch.isin(torch.arange(width), torch.tensor([5, 131]))[None, None]
+    assert torch.equal(torch.isnan(first.float()), odd) and torch.isfinite(first.float()[~odd]).all()
+    # The same but for the last token, which the rows of the last new token see alone.
+    if at != 89 and new > 1:
+        for bad in (math.nan, math.inf):
+            latent[where(89)][::3] = bad
+            again = run()
+            assert torch.equal(bits(again[:-1]), bits(first[:-1]))
+    # The other dimensions are as without the token: its weight is zero.
+    latent[where(at)] = 0.0
+    latent[where(89)][::3] = latent[where(89)].nan_to_num(0.0, 0.0, 0.0)[::3]
+    entries = table[0, :6].long()
+    c = latent.double()[entries].reshape(-1, width)[:90]
+    k = torch.cat([c, cache["rope"].double()[entries].reshape(-1, 64)[:90]], 1)
+    q = torch.cat([q_latent[:new], q_rope[:new]], -1).double().reshape(new * heads, -1)
+    want, size, logits = plain.attention(q, k, c, 0.02, (90 - new + torch.arange(new)).repeat_interleave(heads), torch.arange(90) != at)
+    rows = slice(0, new * heads if at == 89 or new == 1 else (new - 1) * heads)  # (the last token's own values were others)
+    got = torch.where(odd, 0.0, first.float()).reshape(new * heads, width)
+    want, size = torch.where(odd.reshape(new * heads, width), 0.0, want), torch.where(odd.reshape(new * heads, width), 0.0, size)
+    plain.close(got[rows], want[rows], size[rows], logits[rows], TYPES[dtype], width + 64, 90)
