@@ -419,6 +419,9 @@ int CheckLatentPrompt(const llmp_latent_prompt* op, int cus) {
 // Of the line: an eighth of them on every chiplet.
 int LineGroups(int cus) { return (kAUnit * cus + 7) / 8 * 8; }
 
+// Blocks where pairs are taken whole: (request, head) by eights, so that a chiplet has all row tiles of its own.
+int64_t WholeBlocks(const llmp_latent_prompt& op) { return (static_cast<int64_t>(op.requests) * op.heads + 7) / 8 * 8 * TilesOf(op); }
+
 // Whether pairs are taken whole. Then a call lasts as long as its longest pair (1.2 us a key tile, a workgroup alone on its unit) or as a workgroup's share (3 us a
 // tile, two of them on it), and cut into runs as long as the share and 20 us, for the parts. As far as the sizes tell those: half of the last row tile of a
 // request is empty, a request has an equal part of the keys and no more than twice that, a row sees all of them, or half where all of them are new. (A
@@ -430,6 +433,7 @@ bool WholePairs(const llmp_latent_prompt& op, int cus) {
   const double longest = fresh ? std::min(tiles, op.most_tokens / static_cast<double>(kKeys) + 1.0) : std::min(tiles, 2.0 * share);
   const double row_tiles = op.tokens / static_cast<double>(kPromptRows) + 0.5 * requests;
   // (Blocks are dealt by the largest number of queries that the caller says: where that says little, most would have no pair.)
+  if (WholeBlocks(op) >= (int64_t{1} << 32) / kPromptThreads) return false;  // (a launch has less than 2^32 threads)
   if (static_cast<double>(TilesOf(op)) * requests > 4.0 * (op.tokens / static_cast<double>(kPromptRows) + requests)) return false;
   const double each = row_tiles * op.heads * share * (fresh ? 0.5 : 1.0) / (kAUnit * cus);
   return longest <= 2.5 * each + 15.0;
@@ -456,7 +460,6 @@ extern "C" int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratc
   a.op = *op;
   a.tiles = TilesOf(*op);
   a.parts = LatentPartsAt(scratch, line_groups, kPromptRows);
-  const size_t sets = static_cast<size_t>(op->requests) * op->heads;
   const JoinArgs join = {a.parts, op->out, op->out_token_stride, op->out_head_stride, op->heads, line_groups, 0};
   const auto s = static_cast<hipStream_t>(stream);
   BeginLaunches();
@@ -466,7 +469,7 @@ extern "C" int llmp_hip_latent_prompt(const llmp_latent_prompt* op, void* scratc
     static bool sized[2] = {false, false};
     if (whole) {
       if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, kV, false>), kLds, &sized[0])) return;
-      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, kV, false>), dim3(static_cast<unsigned>((sets + 7) / 8 * 8 * a.tiles)), dim3(kPromptThreads), kLds, s, a);
+      hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, kV, false>), dim3(static_cast<unsigned>(WholeBlocks(*op))), dim3(kPromptThreads), kLds, s, a);
     } else {
       if (!AllowLds(reinterpret_cast<const void*>(&LatentPromptKernel<kType, kN, kP, kV, true>), kLds, &sized[1])) return;
       hipLaunchKernelGGL((LatentPromptKernel<kType, kN, kP, kV, true>), dim3(line_groups), dim3(kPromptThreads), kLds, s, a);
