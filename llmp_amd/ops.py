@@ -35,6 +35,16 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def _workspace(scratch, needs, like):
+    """A call's workspace: `scratch`, the caller's, or a new one of the bytes that the call needs. (The library sees an address and a size:
+    memory that the device may not write is refused here.)"""
+    if scratch is None:
+        scratch = like.new_empty(max(needs, 16), dtype=torch.uint8)
+    else:
+        assert scratch.is_cuda and scratch.device == like.device and scratch.is_contiguous(), "a workspace in one piece on the operands' GPU"
+    return scratch
+
+
 _X_TYPES = {torch.float32: X_F32, torch.bfloat16: X_BF16, torch.float16: X_F16}
 
 
@@ -326,10 +336,8 @@ def attn_vec_quant(t, q, k_cache, v_cache, mask, head_dim, heads, kv_heads, cell
     op.type, op.head_dim, op.heads, op.kv_heads, op.rows, op.cells = t, head_dim, heads, kv_heads, rows, cells
     op.scale, op.softcap = scale, softcap
     cus = lib.llmp_hip_compute_units()
-    need = lib.llmp_hip_attn_vec_quant_scratch(C.byref(op), cus)
-    if scratch is None:
-        scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-    _lib.check(lib.llmp_hip_attn_vec_quant(C.byref(op), _ptr(scratch), scratch.numel(), cus, _stream()))
+    scratch = _workspace(scratch, lib.llmp_hip_attn_vec_quant_scratch(C.byref(op), cus) if scratch is None else 0, q)
+    _lib.check(lib.llmp_hip_attn_vec_quant(C.byref(op), scratch.data_ptr(), scratch.nbytes, cus, _stream()))
     return out
 
 
@@ -821,9 +829,8 @@ def paged_attend(cache, q, table, lengths, starts, scale, *, before=None, window
                           q_token, q_head, out_token, out_head, _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens,
                           tokens if most is None else most, width, lists.shape[2] if lists is not None else 0, window, scale, softcap, _ptr(before))
     cus, at = _compute_units(), C.byref(op)
-    if scratch is None:
-        scratch = torch.empty(max(lib.llmp_hip_paged_attend_scratch(at, cus), 16), dtype=torch.uint8, device=q.device)
-    _lib.check(lib.llmp_hip_paged_attend(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
+    scratch = _workspace(scratch, lib.llmp_hip_paged_attend_scratch(at, cus) if scratch is None else 0, q)
+    _lib.check(lib.llmp_hip_paged_attend(at, scratch.data_ptr(), scratch.nbytes, cus, _stream()))
     return out
 
 
@@ -843,9 +850,8 @@ def paged_select(cache, q, table, lengths, starts, keep, *, before=None, first=1
     op = _lib.PagedSelect(c, q.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), out.data_ptr(), q_token, q_head,
                           _table_stride(table), _X_TYPES[q.dtype], heads, n, tokens, tokens if most is None else most, width, keep, first, recent, _ptr(before))
     at = C.byref(op)
-    if scratch is None:
-        scratch = torch.empty(max(lib.llmp_hip_paged_select_scratch(at), 16), dtype=torch.uint8, device=q.device)
-    _lib.check(lib.llmp_hip_paged_select(at, scratch.data_ptr(), scratch.numel(), _stream()))
+    scratch = _workspace(scratch, lib.llmp_hip_paged_select_scratch(at) if scratch is None else 0, q)
+    _lib.check(lib.llmp_hip_paged_select(at, scratch.data_ptr(), scratch.nbytes, _stream()))
     return out
 
 
@@ -1003,9 +1009,8 @@ def latent_attend(cache, q_latent, q_rope, table, lengths, starts, scale, *, bef
     op = _lib.LatentAttend(c, q_latent.data_ptr(), q_rope.data_ptr(), out.data_ptr(), lengths.data_ptr(), starts.data_ptr(), table.data_ptr(), _ptr(before),
                            lt, lh, rt, rh, ot, oh, _table_stride(table), heads, n, tokens, tokens if most is None else most, table_width, scale)
     cus, at = _compute_units(), C.byref(op)
-    if scratch is None:
-        scratch = q_latent.new_empty(max(lib.llmp_hip_latent_attend_scratch(at, cus), 16), dtype=torch.uint8)
-    _lib.check(lib.llmp_hip_latent_attend(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
+    scratch = _workspace(scratch, lib.llmp_hip_latent_attend_scratch(at, cus) if scratch is None else 0, q_latent)
+    _lib.check(lib.llmp_hip_latent_attend(at, scratch.data_ptr(), scratch.nbytes, cus, _stream()))
     return out
 
 
@@ -1035,7 +1040,6 @@ def latent_prompt(q, k, k_rope, v, starts, scale, *, key_starts=None, most=None,
                            rt, vt, vh, ot, oh, _X_TYPES[q.dtype], heads, starts.shape[0] - 1, tokens, keys, tokens if most is None else most, nope, rope,
                            value, scale)
     cus, at = _compute_units(), C.byref(op)
-    if scratch is None:
-        scratch = q.new_empty(max(lib.llmp_hip_latent_prompt_scratch(at, cus), 16), dtype=torch.uint8)
-    _lib.check(lib.llmp_hip_latent_prompt(at, scratch.data_ptr(), scratch.numel(), cus, _stream()))
+    scratch = _workspace(scratch, lib.llmp_hip_latent_prompt_scratch(at, cus) if scratch is None else 0, q)
+    _lib.check(lib.llmp_hip_latent_prompt(at, scratch.data_ptr(), scratch.nbytes, cus, _stream()))
     return out
