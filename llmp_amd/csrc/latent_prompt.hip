@@ -165,8 +165,8 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
   }
   float top = -INFINITY, sum = 0.0f;
 
-  // A lane's places in a tile's rows, for every load of the wave's (row strides stay below 2^24 values: the host looks). A load's rows follow the one's
-  // before it.
+  // A lane's places in a tile's rows, for every load of the wave's (row strides stay below 2^24 values: the host looks; one
+  // key's takes itself off again). A load's rows follow the one's before it.
   uint32_t k_places[G::kKeyLoads], r_places[G::kRopeLoads], v_places[G::kValueLoads];
   const auto place = [&](auto pitch, auto turn, uint32_t* places, int count, int64_t stride) {
     constexpr int kLanes = decltype(pitch)::value / 16, kRowsALoad = kWave / kLanes;
@@ -409,7 +409,7 @@ int CheckLatentPrompt(const llmp_latent_prompt* op, int cus) {
   if (!std::isfinite(op->scale)) return Refuse(1, "latent_prompt: a scale that is not finite");
   if (cus < 1 || cus > 4096) return Refuse(1, "latent_prompt: %d compute units", cus);
   const int64_t most_stride = 1 << 24;
-  if (op->k_token_stride >= most_stride || op->v_token_stride >= most_stride || op->k_rope_token_stride >= most_stride)
+  if (op->keys > 1 && (op->k_token_stride >= most_stride || op->v_token_stride >= most_stride || op->k_rope_token_stride >= most_stride))
     return Refuse(1, "latent_prompt: keys and values at most 2^24 values apart");
   if ((static_cast<int64_t>(op->requests) * op->heads + 8) * TilesOf(*op) > INT_MAX)
     return Refuse(1, "latent_prompt: %d requests of %d heads with up to %d rows are too many", op->requests, op->heads, op->most_tokens);
