@@ -88,9 +88,9 @@ __device__ __forceinline__ void AttnFor(F&& f) {
 template <int BYTES, int OFFSET>
 __device__ __forceinline__ void ToLds(const uint8_t* base, uint32_t offset, uint32_t to) {
   if constexpr (BYTES == 16) {
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "n"(OFFSET) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base), "n"(OFFSET) : "memory", "scc", "m0");
   } else {
-    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base), "n"(OFFSET) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base), "n"(OFFSET) : "memory", "scc", "m0");
   }
 }
 // The same pointer known to the compiler as the same in every lane.

@@ -73,14 +73,14 @@ __device__ __forceinline__ U32x4 FiniteCodes(U32x4 w) {
 // A scalar address and a 32-bit lane offset; the lanes' 16 (4) bytes go to LDS one after the other from byte `to` on. Written as an instruction:
 // the compiler, which knows the builtin's write to LDS, waits for it before every later read of LDS. A wait of the caller's own stands before what landed is read.
 __device__ __forceinline__ void LineToLds(const void* base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void WordToLds(const void* base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
 // ... from an address of each lane's own.
 __device__ __forceinline__ void LaneLineToLds(const void* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory", "m0");
 }
 template <int LEFT>
 __device__ __forceinline__ void WaitLoads() {
