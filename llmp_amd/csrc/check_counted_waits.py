@@ -13,6 +13,11 @@ compiler takes them for written, copies them, and gives those that nothing reads
 of four stages in LDS: a stage's words may be asked for when its loads have landed, and its place filled again when they
 have come.
 
+latent_attend.hip and latent_project.hip, tiles of latent rows and of matrices: brought to LDS by instructions some tiles
+ahead, and waited for by the number of loads of those that may stay on their way. All of them are written by hand, and other
+operations among them make such a wait longer only; what it needs is that a wave asks for whole tiles: on every path
+the same number of loads a tile, the number that the waits are multiples of.
+
 Needs hipcc, no GPU. Run by the library's build (__graft_entry__.build) and by tests/test_counted_waits.py;
 `python check_counted_waits.py` runs it alone."""
 import concurrent.futures
@@ -27,6 +32,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 MOST_STATES = 400000
+FLAGS = {"latent_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}  # of a source by itself, as the Makefile has them
 MEMORY = re.compile(r"(global|buffer|flat|scratch)_(load|store|atomic)")
 BRANCH = re.compile(r"s_(cbranch_\w+|branch)\s+(\S+)")
 
@@ -38,7 +44,7 @@ def assembly_of(source):
         out = os.path.join(tmp, "kernels.s")
         subprocess.run(
             [HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-I" + os.path.join(ROOT, "include"), "-I" + HERE,
-             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-S", "-o", out,
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *FLAGS.get(source, ()), "--cuda-device-only", "-S", "-o", out,
              os.path.join(HERE, source)],
             check=True, capture_output=True, timeout=1200)
         with open(out) as f:
@@ -222,10 +228,31 @@ def ring_loads(name):
     return (bits * 256 + 1023) // 1024
 
 
+def check_tiles(name, body):
+    """Raises AssertionError where a wave may ask for part of a tile's loads between two of its waits or barriers, or waits for part
+    of one. Returns the loads of a tile, None where every wait is for all loads."""
+    waits = {int(n) for n in re.findall(r"#ASMSTART\s+s_waitcnt vmcnt\((\d+)\)", body)} - {0}
+    if not waits:
+        return None
+    tile = min(waits)
+    assert all(n % tile == 0 for n in waits), f"{name}: waits that leave {sorted(waits)} loads on their way are not whole tiles'"
+
+    def step(code, own, asked):
+        if code.startswith("global_load_lds"):
+            assert own, f"{name}: the compiler's own load to LDS among those that the waits count"
+            return (asked + 1) % tile
+        if own and (code.startswith("s_barrier") or "vmcnt" in code):
+            assert asked == 0, f"{name}: part of a tile ({asked} of {tile} loads) asked for where others are waited for"
+        return asked
+
+    follow(body, 0, step)
+    return tile
+
+
 def check():
     """The number of kernels followed; raises AssertionError (or the compiler's error) where a count does not hold."""
     with concurrent.futures.ThreadPoolExecutor() as pool:
-        decode, exl3 = pool.map(assembly_of, ("decode.hip", "exl3.hip"))
+        decode, exl3, attend, project = pool.map(assembly_of, ("decode.hip", "exl3.hip", "latent_attend.hip", "latent_project.hip"))
     kernels = 0
     for name, body in kernels_of(decode, "DecodeMatrixPanelKernel"):
         check_panel(name, body)
@@ -237,7 +264,10 @@ def check():
         check_ring(name, body, ring_loads(name))
         products += 1
     assert products >= 48, f"only {products} packed products were found"
-    return kernels + products
+    tiles = [check_tiles(name, body) for name, body in (*kernels_of(attend, "LatentAttendKernel"), *kernels_of(project, "13ProjectKernel"))]
+    counted = sum(tile is not None for tile in tiles)
+    assert len(tiles) >= 44 and counted >= 38, f"only {counted} of {len(tiles)} kernels over latent rows count their loads"
+    return kernels + products + counted
 
 
 if __name__ == "__main__":
