@@ -817,7 +817,8 @@ int llmp_hip_latent_project(const llmp_latent_project* op, void* stream);
  * Logits are scale * (q_latent . latent + q_rope . rope), the result sum of softmax * latent, [tokens][heads][width]. The queries and the result are of
  * the cache's type, element strides, rows at 16-byte boundaries. A table entry that is no page of the cache, a token that a row does not see, and what they hold
  * (infinities and NaN too) change nothing of the row; a row that sees nothing is zero; rows past starts[requests] are not written.
- * A token of infinities that a row sees makes the row no number; with a logit of minus infinity, those of its dimensions that are infinite.
+ * A token of infinities that a row sees makes the row no number; with a logit of minus infinity, those of its dimensions that are infinite. A row
+ * with no other logits is as one that sees nothing.
  * The products' inputs are the 16-bit values as they are (codes are exact in both types, times their scale in F32); sums, maximum and
  * normalisation are F32; a weight is rounded to the cache's type once (BF16 2^-8 of itself; F16 2^-11, or 2^-33 of the row's largest
  * where that is more). most_tokens: at least every request's new tokens (a bound from the host; the form goes by it). scratch:
@@ -845,7 +846,7 @@ int llmp_hip_latent_attend(const llmp_latent_attend* op, void* scratch, size_t s
  * [keys][rope_width], which all heads share, and of v [keys][heads][value]; its queries are at the last positions of its keys (key_starts
  * null: starts). Logits are scale * (q . (k, k_rope)); out [tokens][heads][value]. All of one type (LLMP_X_BF16 or LLMP_X_F16), element strides, the last index side by
  * side, rows at 16-byte boundaries; nope and value are 64 or 128, rope_width 32 or 64. What a row does not see changes nothing
- * of it; a row that sees nothing is zero; an infinite value that it sees is infinite in its sum, or no number where the rounded weight is zero; rows past
+ * of it; a row that sees nothing, or has no logits but minus infinity, is zero; an infinite value that it sees is infinite in its sum, or no number where the rounded weight is zero; rows past
  * starts[requests] are not written. Roundings as llmp.latent.attend's; most_tokens is at least every request's
  * queries (rows past it are not written). The tokens of k, k_rope and v are less than 2^24 values apart. Where a
  * call has few rows for the device, its keys are cut into runs, by the descriptor's sizes alone: a row's last bits depend on those. scratch:

@@ -2,9 +2,9 @@
 // the rows of a request are its (token, head) pairs and one read of a tile serves all of them:
 //   S^T = C Q^T (latent and rotated part), P = exp2(S - E), O^T += C^T P^T, out = O / sum of P.
 //
-// What bounds it: with few heads the cache's bytes (1152 a token at 512 + 64 values against 2 * 1088 operations a row; 32 requests of up to 65536, 16 heads: 202 us,
-// 5.5 TB/s; of codes 129 us, 4.8 TB/s); from about 128 rows a token on the matrix instructions take as long (128 heads: 420 us,
-// 0.64 PFLOP/s: a wave reads 68 KB of LDS a tile for 1088 cycles of products, and about as many of other instructions stand beside them). A tile is 32 tokens, brought into LDS by loads that pass no register; the rows' queries and
+// What bounds it: with few heads the cache's bytes (1152 a token at 512 + 64 values against 2 * 1088 operations a row; 32 requests of up to 65536, 16 heads: 213 us the
+// call, 5.2 TB/s; of codes 136 us, 4.5 TB/s); from about 128 rows a token on the matrix instructions take as long (128 heads: 357 us,
+// 0.75 PFLOP/s, of codes 488 us: a wave reads 68 KB of LDS a tile for 1088 cycles of products, and about as many of other instructions stand beside them). A tile is 32 tokens, brought into LDS by loads that pass no register; the rows' queries and
 // results stay in registers. Two forms:
 //   few rows   (no request has more than 16) every wave of a workgroup's four has all rows and a ring of tiles of its own; it waits for nobody, and the
 //              waves' results are added up at the end;
@@ -24,7 +24,8 @@ namespace {
 constexpr int kTokens = 32;  // a tile's
 constexpr int kFewRows = 16, kManyRows = 128;
 constexpr int kLdsBytes = 160 * 1024;
-constexpr int kLeast = 128;  // of the line, to a workgroup: finer parts cost more to write and to join (16 rows, 16 requests of up to 2000: 30.2 us so, 32.4 at 256)
+constexpr int kLeast = 128;  // of the line, to a workgroup: finer parts cost more to write and to join (chunks of 20 heads at width 256: 90.3 us so, 91.8 at 64, 91.5 at 256; one
+                             // request of 2000, 16 rows: 19.5, 18.1 and 22.0)
 
 // The forms: up to 16 rows a request, each wave a tile by itself; 128 rows a workgroup, 16 a wave; so, 32 a wave, two workgroups a compute unit.
 enum Form { kFewForm, kManyForm, kWideForm };
@@ -85,7 +86,8 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
   const llmp_latent_cache& c = op.cache;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   // (All that depends on the lane alone is worked out where it is needed, from a lane number as something new: kept, it is the registers too many, and what the
-  // compiler then brings back from memory waits for the tiles under way.)
+  // compiler then brings back from memory waits for the tiles under way. 32 rows a wave over codes have ten or eleven registers too many all the same, of which one comes
+  // back between every tile's first products, and waits so.)
   const auto lane_anew = [&]() {
     if constexpr (FEW) return static_cast<int>(threadIdx.x & (kWave - 1));
     uint32_t all = ~0u;
@@ -202,7 +204,8 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
         };
         const int step = FEW ? G::kWaves : 1;
         const int my_from = tile_from + (FEW ? wave : 0);
-        // The few rows' form holds a tile's scales in scalar registers: with them there two tiles a wave fill LDS (one tile: 65536 tokens, rope 32: 139 us, two 123).
+        // The few rows' form holds a tile's scales in scalar registers: with them there two tiles a wave fill LDS (32 requests of up to 65536 tokens, rope 32:
+        // one tile 135 us, two 128).
         struct TileScales {
           U32x4 a, b;
         };
@@ -458,9 +461,12 @@ __global__ __launch_bounds__((LatentGeo<R, P, EIGHT, FORM>::kThreads), (FORM == 
             for (int i = 0; i < kLogits; i += 2) {
               const float p = __builtin_amdgcn_exp2f(fmaf(dot[i], worth, -less)), p1 = __builtin_amdgcn_exp2f(fmaf(dot[i + 1], worth, -less));
               if constexpr (EIGHT) {
+                // (Rounded with the token's scale in them, for the reason below; the sum is of what they are before that, and so a weight's rounding is in it once.)
                 sum[s] += p + p1;
                 weights[s][i] = static_cast<typename S::One>(p * seen8[i]), weights[s][i + 1] = static_cast<typename S::One>(p1 * seen8[i + 1]);
               } else {
+                // (Rounded to the cache's type, for the matrix instructions that take 16-bit values: 2^-8 of a weight, F16 2^-11, beside the result's own rounding, which
+                // is as large. Weights of 32 bits as two of 16 would be twice the second product.)
                 weights[s][i] = static_cast<typename S::One>(p), weights[s][i + 1] = static_cast<typename S::One>(p1);
                 // (The sum is of the weights as they are rounded, two in an instruction.)
                 sum[s] = S::AddTwo(typename S::Two{weights[s][i], weights[s][i + 1]}, sum[s]);
@@ -644,8 +650,9 @@ void WithForm(const llmp_latent_attend& op, Form which, F&& f) {
 }
 
 // 32 rows a wave read LDS half as often and share what is worked out a tile, but there are twice the parts to join: where requests have more rows than one pair.
-// (Width 256, 20 heads, three chunks of up to 300 tokens behind 5000: 94 us, 104 with
-// 16 rows a wave; of codes 127 and 150; 32 requests of two tokens and 128 heads behind up to 9000: 69 and 72; a single pair a request would lose 5 us to the join.)
+// (Width 256, 20 heads, three chunks of up to 300 tokens behind 5000: 90 us, 104 with
+// 16 rows a wave; of codes 116 and 138; 32 requests of two tokens and 128 heads behind up to 9000: 67 and 73, of codes 81 and 90; of one token, a single pair a
+// request, 63 and 56.)
 Form FormOf(const llmp_latent_attend& op) {
   const int64_t rows = static_cast<int64_t>(std::min(op.most_tokens, op.tokens)) * op.heads;
   return rows <= kFewRows ? kFewForm : op.cache.width == 256 && rows > kManyRows ? kWideForm : kManyForm;

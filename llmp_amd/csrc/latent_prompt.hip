@@ -9,9 +9,9 @@
 // second product takes; V's columns come by transposing reads.
 //
 // Where pairs of (head, 128 rows) are many for the device, a workgroup takes one whole, a head's pairs on one chiplet, the longest first (a prompt of 4096, 32 heads:
-// 205 us, 242 in the rows' order). Elsewhere the pairs' keys are cut evenly (latent_line.h).
-// (That prompt, nope 128, rope 64, values of 128: 187 us, 0.92 PFLOP/s; the matrix instructions are busy 52 % of the cycles, other vector instructions 36 %, and a wave's products
-// and softmax wait for each other. Six ragged ones of 12 heads, up to 700 rows of 64 + 32 behind 3500 keys: 34 us and 9 for the join.)
+// 194 us, 215 in the rows' order; of 64 + 32 and 64 values 105 and 128). Elsewhere the pairs' keys are cut evenly (latent_line.h).
+// (That prompt, nope 128, rope 64, values of 128: 0.89 PFLOP/s; the matrix instructions are busy 52 % of the cycles, other vector instructions 36 %, and a wave's products
+// and softmax wait for each other. Six ragged ones of 12 heads, up to 700 rows of 64 + 32 behind 3500 keys: 35 us and 9 for the join.)
 #include <algorithm>
 #include <cmath>
 
@@ -23,8 +23,8 @@ namespace {
 constexpr int kKeys = 64;  // a tile's
 constexpr int kPromptRows = 128, kPromptThreads = 256;
 constexpr int kAUnit = 2;                            // workgroups a compute unit
-// Of the line, to a workgroup: finer parts cost more to write and to join (one row behind 4000 keys, 8 heads: 19.0 us, 18.0 at 128, 25.9 at 512; 100 rows behind 3000,
-// 4 heads: 22.2, 24.5 and 25.7).
+// Of the line, to a workgroup: finer parts cost more to write and to join (six ragged prompts of 12 heads: 41.6 us, 44.0 at 128, 44.0 at 512; 100 rows behind 3000,
+// 4 heads: 26.3, 23.0 and 30.2; one row behind 4000 keys, 8 heads: 19.6, 17.9 and 26.4).
 constexpr int kLeast = 256;
 
 struct PromptArgs {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
   const float worth = Scalar(fabsf(op.scale) * kLog2E);
 
   // Eight workgroups in a row go to eight chiplets: a chiplet takes every eighth (request, head), or an eighth of the line, so that its L2 holds the keys that
-  // neighbouring pairs share (one prompt of 4096, 8 heads of 64: 47 us, runs in the order of the workgroups 54).
+  // neighbouring pairs share (one prompt of 4096, 8 heads: 79 us, of 64 + 32 and 64 values 57; runs in the order of the workgroups 92 and 64).
   const int groups = gridDim.x;
   int index = 0;
   int request, head = 0, k = 0;
@@ -341,6 +341,7 @@ __global__ __launch_bounds__(kPromptThreads, kAUnit) void LatentPromptKernel(con
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const float p = __builtin_amdgcn_exp2f(fmaf(dots[k][i], worth_now, -less)), p1 = __builtin_amdgcn_exp2f(fmaf(dots[k][i + 1], worth_now, -less));
+        // (Rounded to the type, for the matrix instructions that take 16-bit values: 2^-8 of a weight, F16 2^-11, beside the result's own rounding, which is as large.)
         weights[2 * k + i / 8][i % 8] = static_cast<typename S::One>(p), weights[2 * k + i / 8][i % 8 + 1] = static_cast<typename S::One>(p1);
         // (The sum is of the weights as they are rounded, two in an instruction.)
         sum = S::AddTwo(typename S::Two{weights[2 * k + i / 8][i % 8], weights[2 * k + i / 8][i % 8 + 1]}, sum);
@@ -422,18 +423,19 @@ int LineGroups(int cus) { return (kAUnit * cus + 7) / 8 * 8; }
 // Blocks where pairs are taken whole: (request, head) by eights, so that a chiplet has all row tiles of its own.
 int64_t WholeBlocks(const llmp_latent_prompt& op) { return (static_cast<int64_t>(op.requests) * op.heads + 7) / 8 * 8 * TilesOf(op); }
 
-// Whether pairs are taken whole. Then a call lasts as long as its longest pair (1.2 us a key tile, a workgroup alone on its unit) or as a workgroup's share (3 us a
-// tile, two of them on it), and cut into runs as long as the share and 20 us, for the parts. As far as the sizes tell those: half of the last row tile of a
-// request is empty, a request has an equal part of the keys and no more than twice that, a row sees all of them, or half where all of them are new. (A
-// prompt of 4096, nope 128, rope 64: 32 heads whole 199 us, cut 277, 8 heads (of 64 values) 79 and 61; one of 1000, 8 heads: 34 and 50; six ragged ones of 12
-// heads, up to 700 rows behind 3500 keys: 96 and 53; 16 of up to 1000, 32 heads: 63 and 91.)
+// Whether pairs are taken whole. Then a call lasts as long as its longest pair (1.5 us a key tile of 128 + 64 and 128 values, a workgroup alone on its unit; 1.1 of 64 + 32 and
+// 64) or as a workgroup's share (2.9 and 1.6 us a tile, two of them on it), and cut into runs as long as the share and 25 to 50 us, for the parts. As far as the sizes
+// tell those: half of the last row tile of a request is empty, a request has an equal part of the keys and no more than twice that, a row sees all of them, or half where
+// all of them are new. The 2.5 and 15 tiles below were found by such calls as these. (Whole and cut, heads of 128 + 64 and 128, then of 64 + 32 and 64: a prompt of 4096, 32 heads 192 and 247 us, 104 and 154, 8 heads 100 and 78, 72 and 52; one of 1000, 8
+// heads 30 and 32, 22 and 24; 16 of up to 1000, 32 heads 58 and 82, 37 and 55; six ragged ones of 12 heads, up to 700 rows behind 3500 keys 118 and 59, 82 and 41: the rule
+// takes the shorter each time. Of those with 32 heads, wide, it takes them whole: 119 and 108.)
 bool WholePairs(const llmp_latent_prompt& op, int cus) {
   const bool fresh = op.key_starts == nullptr || op.keys == op.tokens;
   const double requests = op.requests, tiles = op.keys / static_cast<double>(kKeys) + 1.0, share = tiles / requests + 1.0;
   const double longest = fresh ? std::min(tiles, op.most_tokens / static_cast<double>(kKeys) + 1.0) : std::min(tiles, 2.0 * share);
   const double row_tiles = op.tokens / static_cast<double>(kPromptRows) + 0.5 * requests;
-  // (Blocks are dealt by the largest number of queries that the caller says: where that says little, most would have no pair.)
   if (WholeBlocks(op) >= (int64_t{1} << 32) / kPromptThreads) return false;  // (a launch has less than 2^32 threads)
+  // (Blocks are dealt by the largest number of queries that the caller says: where that says little, most would have no pair.)
   if (static_cast<double>(TilesOf(op)) * requests > 4.0 * (op.tokens / static_cast<double>(kPromptRows) + requests)) return false;
   const double each = row_tiles * op.heads * share * (fresh ? 0.5 : 1.0) / (kAUnit * cus);
   return longest <= 2.5 * each + 15.0;

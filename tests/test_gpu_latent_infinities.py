@@ -124,3 +124,20 @@ def test_infinities_of_no_weight(device, width, dtype, heads, new, at):
     got = torch.where(odd, 0.0, first.float()).reshape(new * heads, width)
     want, size = torch.where(odd.reshape(new * heads, width), 0.0, want), torch.where(odd.reshape(new * heads, width), 0.0, size)
     plain.close(got[rows], want[rows], size[rows], logits[rows], TYPES[dtype], width + 64, 90)
+
+
+@pytest.mark.parametrize("heads,new", [(16, 1), (40, 3)])
+def test_rows_of_no_logit_but_minus_infinity(device, heads, new):
+    """They are as rows that see nothing: zeros (but where an infinity of the absorbed form's own rows is seen)."""
+    g = torch.Generator().manual_seed(heads)
+    cache, table, starts, q_latent, q_rope = latent_case(g, [50], [new], 16, heads, 512, 64, "bf16", 16)
+    q_rope[..., 3] = -2.0
+    for p in range(50):
+        cache["rope"][int(table[0, p // 16]), p % 16, 3] = math.inf
+    on = {k: v.to(device) for k, v in cache.items()}
+    got = ops.latent_attend(on, q_latent.to(device), q_rope.to(device), table.to(device), ints([50], device), ints(starts, device), 0.02, most=new)
+    assert (got[:new] == 0).all()
+    q, k, v, k_rope = (normal(g, *s, dtype=torch.bfloat16) for s in ((new, 2, 192), (50, 2, 128), (50, 2, 128), (50, 64)))
+    q[..., 130], k_rope[:, 2] = -2.0, math.inf
+    got = ops.latent_prompt(q.to(device), k.to(device), k_rope.to(device), v.to(device), ints([0, new], device), 0.05, key_starts=ints([0, 50], device), most=new)
+    assert (got == 0).all()
