@@ -10,8 +10,9 @@
 //
 // Where pairs of (head, 128 rows) are many for the device, a workgroup takes one whole, a head's pairs on one chiplet, the longest first (a prompt of 4096, 32 heads:
 // 194 us, 215 in the rows' order; of 64 + 32 and 64 values 105 and 128). Elsewhere the pairs' keys are cut evenly (latent_line.h).
-// (That prompt, nope 128, rope 64, values of 128: 0.89 PFLOP/s; the matrix instructions are busy 52 % of the cycles, other vector instructions 36 %, and a wave's products
-// and softmax wait for each other. Six ragged ones of 12 heads, up to 700 rows of 64 + 32 behind 3500 keys: 35 us and 9 for the join.)
+// (Times in this file are passes of one call after the other, host and join with them. That prompt, nope 128, rope 64, values of 128: 0.89 PFLOP/s; the matrix
+// instructions are busy 52 % of the cycles, other vector instructions 36 %, and a wave's products and softmax wait for each other. Six ragged ones of 12 heads, up to
+// 700 rows of 64 + 32 behind 3500 keys: the kernel 35 us and 9 the join, 41.6 the call.)
 #include <algorithm>
 #include <cmath>
 
@@ -426,7 +427,7 @@ int64_t WholeBlocks(const llmp_latent_prompt& op) { return (static_cast<int64_t>
 // Whether pairs are taken whole. Then a call lasts as long as its longest pair (1.5 us a key tile of 128 + 64 and 128 values, a workgroup alone on its unit; 1.1 of 64 + 32 and
 // 64) or as a workgroup's share (2.9 and 1.6 us a tile, two of them on it), and cut into runs as long as the share and 25 to 50 us, for the parts. As far as the sizes
 // tell those: half of the last row tile of a request is empty, a request has an equal part of the keys and no more than twice that, a row sees all of them, or half where
-// all of them are new. The 2.5 and 15 tiles below were found by such calls as these. (Whole and cut, heads of 128 + 64 and 128, then of 64 + 32 and 64: a prompt of 4096, 32 heads 192 and 247 us, 104 and 154, 8 heads 100 and 78, 72 and 52; one of 1000, 8
+// all of them are new. The 2.5 and 15 tiles below were found by such calls as these. (Whole and cut, heads of 128 + 64 and 128, then of 64 + 32 and 64: a prompt of 4096, 32 heads 194 and 247 us, 105 and 154, 8 heads 100 and 78, 72 and 52; one of 1000, 8
 // heads 30 and 32, 22 and 24; 16 of up to 1000, 32 heads 58 and 82, 37 and 55; six ragged ones of 12 heads, up to 700 rows behind 3500 keys 118 and 59, 82 and 41: the rule
 // takes the shorter each time. Of those with 32 heads, wide, it takes them whole: 119 and 108.)
 bool WholePairs(const llmp_latent_prompt& op, int cus) {
